@@ -1,0 +1,897 @@
+// Post-training of the vocabulary models: log-probabilities of given tokens with their gradient, the paired preference loss, the
+// clipped policy loss with a KL term, the global gradient norm over a list of tensors, clipping, and the Adam step that clips.
+//
+// Softmax in base 2.  With k = scale * log2(e) the kernels sum 2^(k x - r) for an INTEGER reference r >= max(k x): partial sums with
+// different references meet exactly (powers of two).  A row is kept as the pair (r, s): softmax_j = 2^(k x_j - r) / s, log
+// softmax_j = (k x_j - r - log2 s) ln 2, the latter once per row in 64 bits.  k comes in two parts (K2): rounded to 32 bits it would
+// be another temperature, 1.3e-8 off, which moves every log-probability of a sequence to the same side (measured on four
+// sequences of 1024 tokens: the sum of log-ratios 2.7e-5 off, in two parts 2e-6, which is the rounding of the log-probabilities).
+#include "common.cuh"
+#include <limits.h>
+#include <math.h>
+#include <stdio.h>
+
+namespace {
+
+constexpr int ROW_THREADS = 256;
+
+template <typename T> struct Elem;
+template <> struct Elem<__nv_bfloat16> {
+  static constexpr int VEC = 8;
+  static __device__ __forceinline__ float get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ void unpack(const uint4& q, float* f) {
+    f[0] = bb::bf16_lo(q.x); f[1] = bb::bf16_hi(q.x); f[2] = bb::bf16_lo(q.y); f[3] = bb::bf16_hi(q.y);
+    f[4] = bb::bf16_lo(q.z); f[5] = bb::bf16_hi(q.z); f[6] = bb::bf16_lo(q.w); f[7] = bb::bf16_hi(q.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float* f) {
+    return make_uint4(bb::pack_bf16x2(f[0], f[1]), bb::pack_bf16x2(f[2], f[3]), bb::pack_bf16x2(f[4], f[5]), bb::pack_bf16x2(f[6], f[7]));
+  }
+  static __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+};
+template <> struct Elem<float> {
+  static constexpr int VEC = 4;
+  static __device__ __forceinline__ float get(const float* p) { return *p; }
+  static __device__ __forceinline__ void unpack(const uint4& q, float* f) {
+    f[0] = __uint_as_float(q.x); f[1] = __uint_as_float(q.y); f[2] = __uint_as_float(q.z); f[3] = __uint_as_float(q.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float* f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+  static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// k = hi + lo, hi with 16 significant bits (x hi is exact for a bf16 x), lo > 0 (so that -inf stays -inf)
+struct K2 { float hi, lo; };
+__device__ __forceinline__ float expo(float x, K2 k, float r) { return fmaf(x, k.lo, fmaf(x, k.hi, -r)); }
+
+// A row of n elements as [0, lead) up to the first 16-byte boundary, nvec vectors, and the rest from `tail`.
+template <typename T> struct Span {
+  int lead, nvec, tail;
+  __device__ __forceinline__ Span(const T* p, int n) {
+    const int off = (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T);
+    lead = off < n ? off : n;
+    nvec = (n - lead) / Elem<T>::VEC;
+    tail = lead + nvec * Elem<T>::VEC;
+  }
+};
+
+// ---- partial softmax sums: (r, s), r an integer or -inf (nothing yet, or only -inf logits)
+__device__ __forceinline__ void soft_merge(float& r, float& s, float r2, float s2) {
+  const float rn = fmaxf(r, r2);
+  // (equal references add as they are: -inf - -inf would be NaN)
+  s = (r == rn ? s : s * ex2(r - rn)) + (r2 == rn ? s2 : s2 * ex2(r2 - rn));
+  r = rn;
+}
+template <int N> __device__ __forceinline__ void soft_add(float& r, float& s, const float* f, K2 k) {
+  float top = f[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) top = fmaxf(top, f[i]);
+  const float rn = ceilf(expo(top, k, 0.f));
+  if (rn > r) { s = r == -INFINITY ? s : s * ex2(r - rn); r = rn; }
+  const float ref = r == -INFINITY ? 0.f : r;          // only -inf so far: 2^-inf = 0 is added, NaN stays NaN
+#pragma unroll
+  for (int i = 0; i < N; ++i) s += ex2(expo(f[i], k, ref));
+}
+
+// (r, s) of the block's threads merged; every thread gets the result
+template <int THREADS> __device__ __forceinline__ void soft_block(float& r, float& s, float2* smem /*[THREADS/32]*/) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) soft_merge(r, s, __shfl_xor_sync(0xffffffffu, r, o), __shfl_xor_sync(0xffffffffu, s, o));
+  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = make_float2(r, s);
+  __syncthreads();
+  r = -INFINITY; s = 0.f;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) soft_merge(r, s, smem[w].x, smem[w].y);
+}
+
+template <typename T, int THREADS> __device__ __forceinline__ void soft_row(const T* x, int n, K2 k, float& r, float& s) {
+  constexpr int VEC = Elem<T>::VEC;
+  const Span<T> sp(x, n);
+  r = -INFINITY; s = 0.f;
+  const uint4* v = reinterpret_cast<const uint4*>(x + sp.lead);
+  for (int c = threadIdx.x; c < sp.nvec; c += THREADS) {
+    float f[VEC];
+    Elem<T>::unpack(v[c], f);
+    soft_add<VEC>(r, s, f, k);
+  }
+  for (int j = threadIdx.x; j < sp.lead + n - sp.tail; j += THREADS) {
+    const float f = Elem<T>::get(x + (j < sp.lead ? j : sp.tail + j - sp.lead));
+    soft_add<1>(r, s, &f, k);
+  }
+}
+
+// A row whose largest logit is so far from zero that k x is not finite (a row of the type's lowest value): differences at that
+// magnitude leave all of the softmax to the logits that equal the largest.  Kept as (largest, -how many of them there are);
+// (NaN, NaN) with a NaN or +inf in the row, (-inf, 0) when every logit is -inf.  Called by the whole block where r is infinite.
+template <typename T, int THREADS> __device__ __noinline__ void soft_row_extreme(const T* x, int n, float& r, float& s, float2* smem) {
+  float top = -INFINITY;
+  int count = 0, bad = 0;
+  for (int j = threadIdx.x; j < n; j += THREADS) {
+    const float f = Elem<T>::get(x + j);
+    bad |= f != f || f == INFINITY;
+    if (f > top) { top = f; count = 1; } else if (f == top) ++count;
+  }
+  bad = __syncthreads_or(bad);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float t2 = __shfl_xor_sync(0xffffffffu, top, o);
+    const int c2 = __shfl_xor_sync(0xffffffffu, count, o);
+    count = (top >= t2 ? count : 0) + (t2 >= top ? c2 : 0);
+    top = fmaxf(top, t2);
+  }
+  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = make_float2(top, (float)count);
+  __syncthreads();
+  r = -INFINITY;
+  for (int w = 0; w < THREADS / 32; ++w) r = fmaxf(r, smem[w].x);
+  s = 0.f;
+  for (int w = 0; w < THREADS / 32; ++w) if (smem[w].x == r) s -= smem[w].y;
+  if (r == -INFINITY) s = 0.f;
+  if (bad) r = s = NAN;
+}
+
+template <typename T, int THREADS> __device__ __forceinline__ void soft_whole_row(const T* x, int n, K2 k, float& r, float& s, float2* smem) {
+  soft_row<T, THREADS>(x, n, k, r, s);
+  soft_block<THREADS>(r, s, smem);
+  if (isinf(r)) soft_row_extreme<T, THREADS>(x, n, r, s, smem);
+}
+
+// log softmax of logit x in 64 bits; a row without any finite logit (s = 0) has no distribution: -inf
+__device__ __forceinline__ double row_logp(float x, K2 k, float r, float s) {
+  if (s == 0.f) return -INFINITY;
+  if (s < 0.f) return x == r ? -log((double)-s) : -INFINITY;
+  return ((double)x * ((double)k.hi + (double)k.lo) - ((double)r + log2((double)s))) * 0.69314718055994531;
+}
+
+// d[j] = g * ([j == t] - softmax_j) for j < V, 0 in [V, cols); zeros throughout when g == 0 (nothing is read then)
+template <typename T, int THREADS>
+__device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int t, float g, K2 k, float r, float s) {
+  constexpr int VEC = Elem<T>::VEC;
+  if (s == 0.f) g = 0.f;
+  const float ng = g == 0.f ? 0.f : -g / s;
+  const bool aligned = (((uintptr_t)x ^ (uintptr_t)d) & 15) == 0;
+  const Span<T> sp(d, aligned ? cols : 0);
+  auto one = [&](int j) {
+    float v = 0.f;
+    if (g != 0.f && j < V) {
+      const float f = Elem<T>::get(x + j);
+      v = s < 0.f ? (f == r ? -ng : 0.f) : ng * ex2(expo(f, k, r));
+      if (j == t) v += g;
+    }
+    Elem<T>::put(d + j, v);
+  };
+  if (!aligned || s < 0.f) {
+    for (int j = threadIdx.x; j < cols; j += THREADS) one(j);
+    return;
+  }
+  const uint4* xv = reinterpret_cast<const uint4*>(x + sp.lead);
+  uint4* dv = reinterpret_cast<uint4*>(d + sp.lead);
+  for (int c = threadIdx.x; c < sp.nvec; c += THREADS) {
+    const int j0 = sp.lead + c * VEC;
+    if (g == 0.f || j0 >= V) { dv[c] = make_uint4(0, 0, 0, 0); continue; }
+    float f[VEC];
+    Elem<T>::unpack(xv[c], f);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      f[i] = j0 + i < V ? ng * ex2(expo(f[i], k, r)) : 0.f;
+      if (j0 + i == t) f[i] += g;
+    }
+    dv[c] = Elem<T>::pack(f);
+  }
+  for (int j = threadIdx.x; j < sp.lead + cols - sp.tail; j += THREADS) one(j < sp.lead ? j : sp.tail + j - sp.lead);
+}
+
+// ------------------------------------------------------------------ token log-probabilities
+template <typename T>
+__global__ void __launch_bounds__(ROW_THREADS)
+token_logprob_fwd_kernel(const T* logits, long long ld, const long long* targets, K2 k, float* logp, float2* stats,
+                         int V, long long ignore_index, int* status) {
+  __shared__ float2 smem[ROW_THREADS / 32];
+  bb::pdl_sync();
+  const int row = blockIdx.x;
+  const long long t = targets[row];
+  if (t == ignore_index || t < 0 || t >= V) {
+    if (threadIdx.x == 0) {
+      if (t != ignore_index) atomicCAS(status, 0, BB_ERR_INVALID_ARG);
+      logp[row] = 0.f;
+      stats[row] = make_float2(0.f, 0.f);
+    }
+    return;
+  }
+  const T* x = logits + (size_t)row * ld;
+  float r, s;
+  soft_whole_row<T, ROW_THREADS>(x, V, k, r, s, smem);
+  if (threadIdx.x == 0) {
+    logp[row] = (float)row_logp(Elem<T>::get(x + t), k, r, s);
+    stats[row] = make_float2(r, s);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(ROW_THREADS)
+token_logprob_bwd_kernel(const T* logits, long long ld, const long long* targets, const float2* stats, const float* row_grad,
+                         const float* gscale_dev, float gscale, K2 k, T* dlogits, long long ldd, int V, int cols,
+                         long long ignore_index) {
+  bb::pdl_sync();
+  const int row = blockIdx.x;
+  const long long t = targets[row];
+  const float2 st = stats[row];
+  const bool counted = t != ignore_index && t >= 0 && t < V;
+  const float g = counted ? row_grad[row] * (gscale_dev ? gscale_dev[0] : 1.f) * gscale : 0.f;
+  grad_row<T, ROW_THREADS>(logits + (size_t)row * ld, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, st.x, st.y);
+}
+
+// ------------------------------------------------------------------ sums of a block
+template <int THREADS> __device__ __forceinline__ double block_sum(double v, double* smem /*[THREADS/32]*/) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) v += smem[w];
+  return v;
+}
+
+// Tokens [a, b) of sequence q: rows of `seq_len` tokens, or between two offsets.  Offsets that do not ascend within [0, tokens]
+// are recorded and cut to it.
+__device__ __forceinline__ void sequence(const long long* offsets, long long seq_len, long long tokens, int q, long long& a, long long& b,
+                                         int* status) {
+  a = offsets ? offsets[q] : q * seq_len;
+  b = offsets ? offsets[q + 1] : a + seq_len;
+  if (a < 0 || b < a || b > tokens) {
+    if (threadIdx.x == 0) atomicCAS(status, 0, BB_ERR_INVALID_ARG);
+    a = a < 0 ? 0 : a > tokens ? tokens : a;
+    b = b < a ? a : b > tokens ? tokens : b;
+  }
+}
+
+// Zeros for the tokens in front of the first sequence (first CTA) and behind the last (last CTA) of `sequences`
+__device__ __forceinline__ void outside_zero(const long long* offsets, long long tokens, int sequences, float* out) {
+  if (!offsets) return;
+  if (blockIdx.x == 0)
+    for (long long i = threadIdx.x; i < offsets[0] && i < tokens; i += 256) out[i] = 0.f;
+  if (blockIdx.x == gridDim.x - 1) {
+    const long long end = offsets[sequences];
+    for (long long i = (end > 0 ? end : 0) + threadIdx.x; i < tokens; i += 256) out[i] = 0.f;
+  }
+}
+
+// ------------------------------------------------------------------ preference loss
+// One CTA per pair.  s_q = sum (or mean) over counted tokens of logp - ref; h = beta (s_2i - s_2i+1); pair_loss[i] = f(h);
+// row_grad = +-beta f'(h) / pairs (/ count) on counted tokens, 0 elsewhere.
+__global__ void __launch_bounds__(256)
+preference_pair_kernel(const float* logp, const float* ref, const long long* targets, const long long* offsets, long long seq_len,
+                       long long tokens, int pairs, int form, double beta, double smoothing, int average, long long ignore_index,
+                       double* pair_loss, float* rewards, float* row_grad, int* status) {
+  __shared__ double smem[8];
+  bb::pdl_sync();
+  const int pair = blockIdx.x;
+  double score[2], length[2];
+  long long a[2], b[2];
+  for (int w = 0; w < 2; ++w) {
+    sequence(offsets, seq_len, tokens, 2 * pair + w, a[w], b[w], status);
+    double sum = 0.0;
+    int count = 0;
+    for (long long i = a[w] + threadIdx.x; i < b[w]; i += 256) {
+      if (targets[i] == ignore_index) continue;
+      sum += (double)logp[i] - (ref ? (double)ref[i] : 0.0);
+      ++count;
+    }
+    score[w] = block_sum<256>(sum, smem);
+    const double n = block_sum<256>((double)count, smem);
+    length[w] = average ? (n > 1.0 ? n : 1.0) : 1.0;
+    score[w] /= length[w];
+  }
+  const double h = beta * (score[0] - score[1]);
+  double loss, slope;
+  if (form == BB_PREFERENCE_SIGMOID) {
+    // softplus(z) = max(z, 0) + log(1 + e^-|z|);  -log sig(h) = softplus(-h)
+    const double tail = log1p(exp(-fabs(h)));
+    loss = (1.0 - smoothing) * (fmax(-h, 0.0) + tail) + smoothing * (fmax(h, 0.0) + tail);
+    const double sig = 1.0 / (1.0 + exp(-h));
+    slope = sig - 1.0 + smoothing;
+  } else if (form == BB_PREFERENCE_HINGE) {
+    loss = fmax(0.0, 1.0 - h);
+    slope = h < 1.0 ? -1.0 : 0.0;
+    if (h != h) loss = slope = h;
+  } else {
+    const double gap = (h - 0.5) / beta;
+    loss = gap * gap;
+    slope = 2.0 * gap / beta;
+  }
+  if (threadIdx.x == 0) {
+    pair_loss[pair] = loss;
+    rewards[2 * pair] = (float)(beta * score[0]);
+    rewards[2 * pair + 1] = (float)(beta * score[1]);
+  }
+  for (int w = 0; w < 2; ++w) {
+    const float g = (float)((w ? -slope : slope) * beta / ((double)pairs * length[w]));
+    for (long long i = a[w] + threadIdx.x; i < b[w]; i += 256) row_grad[i] = targets[i] == ignore_index ? 0.f : g;
+  }
+  outside_zero(offsets, tokens, 2 * pairs, row_grad);
+}
+
+// loss = mean of pair_loss, in a fixed order
+__global__ void __launch_bounds__(256)
+preference_mean_kernel(const double* pair_loss, int pairs, float* loss) {
+  __shared__ double smem[8];
+  bb::pdl_sync();
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < pairs; i += 256) sum += pair_loss[i];
+  sum = block_sum<256>(sum, smem);
+  if (threadIdx.x == 0) loss[0] = (float)(sum / pairs);
+}
+
+// ------------------------------------------------------------------ policy loss
+struct PolicyParams {
+  const float* old_logp;        // NULL: the tokens were sampled by this very policy (ratio 1)
+  const float* advantages;      // index = row / adv_div
+  const float* ref;             // NULL: no KL term
+  const float* weight;          // per token (sequence reduction); NULL: 1 / number of counted tokens
+  const int* counts; int num_counts;
+  long long adv_div;
+  float low, high, kl_coef;     // ratio bounds 1 - clip_low, 1 + clip_high
+};
+struct PolicyToken { float loss, kl, clipped, slope; };
+
+__device__ __forceinline__ PolicyToken policy_token(const PolicyParams& p, long long row, double lp) {
+  PolicyToken o;
+  const float adv = p.advantages[row / p.adv_div];
+  const float ratio = p.old_logp ? expf((float)(lp - (double)p.old_logp[row])) : 1.f;
+  // (an advantage of 0 has no part in the surrogate, whatever the ratio overflowed to)
+  const float plain = adv == 0.f ? 0.f : ratio * adv, bounded = fminf(fmaxf(ratio, p.low), p.high) * adv;
+  const bool cut = bounded < plain;
+  o.clipped = cut ? 1.f : 0.f;
+  o.loss = cut ? -bounded : -plain;
+  o.slope = cut ? 0.f : -plain;
+  o.kl = 0.f;
+  if (p.ref) {
+    const float gap = (float)((double)p.ref[row] - lp), e = expm1f(gap);       // e^gap - gap - 1 without the cancellation
+    o.kl = e - gap;
+    o.loss += p.kl_coef * o.kl;
+    o.slope -= p.kl_coef * e;
+  }
+  return o;
+}
+
+// Counted tokens of each of `gridDim.x` pieces of the targets (sequences, or equal pieces when weight is NULL) and, per sequence,
+// the weight 1 / (sequences * counted) of its tokens
+__global__ void __launch_bounds__(256)
+policy_count_kernel(const long long* targets, const long long* offsets, long long piece, long long tokens, long long ignore_index,
+                    int* counts, float* weight, int* status) {
+  __shared__ double smem[8];
+  bb::pdl_sync();
+  long long a, b;
+  if (weight) {
+    sequence(offsets, piece, tokens, blockIdx.x, a, b, status);
+  } else {
+    a = blockIdx.x * piece;
+    b = a + piece < tokens ? a + piece : tokens;
+  }
+  int count = 0;
+  for (long long i = a + threadIdx.x; i < b; i += 256) count += targets[i] != ignore_index;
+  const double n = block_sum<256>((double)count, smem);
+  if (threadIdx.x == 0) counts[blockIdx.x] = (int)n;
+  if (!weight) return;
+  const float w = (float)(1.0 / ((double)gridDim.x * (n > 1.0 ? n : 1.0)));
+  for (long long i = a + threadIdx.x; i < b; i += 256) weight[i] = w;
+  outside_zero(offsets, tokens, gridDim.x, weight);
+}
+
+__device__ __forceinline__ float policy_weight(const PolicyParams& p, long long row) {
+  if (p.weight) return p.weight[row];
+  double n = 0.0;
+  for (int i = 0; i < p.num_counts; ++i) n += (double)p.counts[i];
+  return (float)(1.0 / (n > 1.0 ? n : 1.0));
+}
+
+// Token by token: row_grad, and the sums of a CTA's tokens: weighted loss, KL, clipped
+__global__ void __launch_bounds__(256)
+policy_token_kernel(const float* logp, const long long* targets, const PolicyParams p, long long tokens, long long ignore_index,
+                    float* row_grad, double* partial) {
+  __shared__ double smem[8];
+  bb::pdl_sync();
+  double loss = 0.0, kl = 0.0, clipped = 0.0;
+  const float whole = p.weight ? 0.f : policy_weight(p, 0);
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < tokens; i += (long long)gridDim.x * 256) {
+    const float w = p.weight ? p.weight[i] : whole;
+    if (targets[i] == ignore_index || w == 0.f) { row_grad[i] = 0.f; continue; }
+    const PolicyToken o = policy_token(p, i, (double)logp[i]);
+    row_grad[i] = o.slope * w;
+    loss += (double)o.loss * w; kl += o.kl; clipped += o.clipped;
+  }
+  loss = block_sum<256>(loss, smem); kl = block_sum<256>(kl, smem); clipped = block_sum<256>(clipped, smem);
+  if (threadIdx.x == 0) { partial[3 * blockIdx.x] = loss; partial[3 * blockIdx.x + 1] = kl; partial[3 * blockIdx.x + 2] = clipped; }
+}
+
+// One CTA per row of logits: log-probability, the token's loss and, because a row's gradient needs nothing of the other rows (the
+// weights follow from the targets), that gradient too
+template <typename T>
+__global__ void __launch_bounds__(ROW_THREADS)
+policy_row_kernel(const T* logits, long long ld, const long long* targets, const PolicyParams p, K2 k, float gscale,
+                  T* dlogits, long long ldd, int V, int cols, long long ignore_index, float* logp, double* partial, int* status) {
+  __shared__ float2 smem[ROW_THREADS / 32];
+  __shared__ float s_slope;
+  bb::pdl_sync();
+  const int row = blockIdx.x;
+  const long long t = targets[row];
+  const T* x = logits + (size_t)row * ld;
+  const bool counted = t != ignore_index && t >= 0 && t < V && !(p.weight && p.weight[row] == 0.f);
+  float r = 0.f, s = 0.f, g = 0.f;
+  if (counted) {
+    soft_whole_row<T, ROW_THREADS>(x, V, k, r, s, smem);
+  }
+  if (threadIdx.x == 0) {
+    double lp = 0.0;
+    PolicyToken o = {0.f, 0.f, 0.f, 0.f};
+    float w = 0.f;
+    if (counted) {
+      lp = row_logp(Elem<T>::get(x + t), k, r, s);
+      o = policy_token(p, row, lp);
+      w = policy_weight(p, row);
+    } else if (t != ignore_index && (t < 0 || t >= V)) {
+      atomicCAS(status, 0, BB_ERR_INVALID_ARG);
+    }
+    s_slope = o.slope * w * gscale;
+    logp[row] = (float)lp;
+    partial[3LL * row] = (double)o.loss * w; partial[3LL * row + 1] = o.kl; partial[3LL * row + 2] = o.clipped;
+  }
+  __syncthreads();            // also: every thread is past its reads of the row before it may be overwritten
+  g = s_slope;
+  grad_row<T, ROW_THREADS>(x, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, r, s);
+}
+
+// A gradient that was made for an upstream gradient of `made_for`, times *grad / made_for: nothing to do where they are the same
+template <typename T>
+__global__ void __launch_bounds__(ROW_THREADS)
+rescale_kernel(T* d, long long ld, int cols, const float* grad, float made_for) {
+  constexpr int VEC = Elem<T>::VEC;
+  bb::pdl_sync();
+  if (grad[0] == made_for) return;
+  const float c = grad[0] / made_for;
+  T* x = d + (size_t)blockIdx.x * ld;
+  const Span<T> sp(x, cols);
+  uint4* v = reinterpret_cast<uint4*>(x + sp.lead);
+  for (int i = threadIdx.x; i < sp.nvec; i += ROW_THREADS) {
+    float f[VEC];
+    Elem<T>::unpack(v[i], f);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] *= c;
+    v[i] = Elem<T>::pack(f);
+  }
+  for (int j = threadIdx.x; j < sp.lead + cols - sp.tail; j += ROW_THREADS) {
+    T* at = x + (j < sp.lead ? j : sp.tail + j - sp.lead);
+    Elem<T>::put(at, Elem<T>::get(at) * c);
+  }
+}
+
+// loss[0] = sum of the weighted losses; stats = mean KL and share of clipped among counted tokens
+__global__ void __launch_bounds__(1024)
+policy_finish_kernel(const double* partial, long long n, const int* counts, int num_counts, float* loss, float* stats) {
+  __shared__ double smem[32];
+  bb::pdl_sync();
+  double v[3] = {0.0, 0.0, 0.0};
+  for (long long i = threadIdx.x; i < n; i += 1024)
+    for (int c = 0; c < 3; ++c) v[c] += partial[3 * i + c];
+  double total = 0.0;
+  for (int i = threadIdx.x; i < num_counts; i += 1024) total += (double)counts[i];
+  for (int c = 0; c < 3; ++c) v[c] = block_sum<1024>(v[c], smem);
+  total = block_sum<1024>(total, smem);
+  if (threadIdx.x == 0) {
+    if (total < 1.0) total = 1.0;
+    loss[0] = (float)v[0]; stats[0] = (float)(v[1] / total); stats[1] = (float)(v[2] / total);
+  }
+}
+
+// ------------------------------------------------------------------ gradient norm, clipping
+constexpr int LIST_TENSORS = 128;             // tensors of one launch: their table travels as a kernel argument
+constexpr int NORM_THREADS = 512;
+struct TensorTable {
+  void* data[LIST_TENSORS];
+  long long numel[LIST_TENSORS];
+  int first[LIST_TENSORS + 1];                // first piece of each tensor, a piece being `piece` elements
+  unsigned char dtype[LIST_TENSORS];
+  int count, piece;
+};
+
+// tensor and element range of a piece
+__device__ __forceinline__ int table_find(const TensorTable& t, int piece, long long& a, long long& n) {
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.first[mid] <= piece) lo = mid; else hi = mid - 1;
+  }
+  a = (long long)(piece - t.first[lo]) * t.piece;
+  n = t.numel[lo] - a < t.piece ? t.numel[lo] - a : t.piece;
+  return lo;
+}
+
+template <typename T> __device__ __forceinline__ double sumsq_piece(const T* x, int n) {
+  constexpr int VEC = Elem<T>::VEC;
+  const Span<T> sp(x, n);
+  const uint4* v = reinterpret_cast<const uint4*>(x + sp.lead);
+  double sum = 0.0;
+  for (int c = threadIdx.x; c < sp.nvec; c += NORM_THREADS) {
+    float f[VEC], q = 0.f;
+    Elem<T>::unpack(v[c], f);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) q = fmaf(f[i], f[i], q);
+    sum += (double)q;
+  }
+  for (int j = threadIdx.x; j < sp.lead + n - sp.tail; j += NORM_THREADS) {
+    const float f = Elem<T>::get(x + (j < sp.lead ? j : sp.tail + j - sp.lead));
+    sum += (double)(f * f);
+  }
+  return sum;
+}
+
+// partial[blockIdx.x] = sum of squares of the CTA's pieces (every gridDim.x-th), in a fixed order
+__global__ void __launch_bounds__(NORM_THREADS)
+grad_sumsq_kernel(const __grid_constant__ TensorTable t, double* partial) {
+  __shared__ double smem[NORM_THREADS / 32];
+  bb::pdl_sync();
+  double sum = 0.0;
+  for (int piece = blockIdx.x; piece < t.first[t.count]; piece += gridDim.x) {
+    long long a, n;
+    const int i = table_find(t, piece, a, n);
+    sum += t.dtype[i] == BB_DTYPE_F32 ? sumsq_piece(reinterpret_cast<const float*>(t.data[i]) + a, (int)n)
+                                      : sumsq_piece(reinterpret_cast<const __nv_bfloat16*>(t.data[i]) + a, (int)n);
+  }
+  sum = block_sum<NORM_THREADS>(sum, smem);
+  if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+}
+
+// norm = pre_scale * sqrt(sum of partials); min(1, max_norm / (norm + 1e-6)), NaN for a NaN norm
+template <int THREADS> __device__ __forceinline__ float clip_coef(const double* partial, int n, double pre_scale, double max_norm, double* smem,
+                                                                 float* norm_out) {
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < n; i += THREADS) sum += partial[i];
+  const double norm = pre_scale * sqrt(block_sum<THREADS>(sum, smem));
+  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = (float)norm;
+  const double coef = max_norm / (norm + 1e-6);
+  return coef >= 1.0 ? 1.f : (float)coef;
+}
+
+template <typename T> __device__ __forceinline__ void scale_piece(T* x, int n, float c) {
+  constexpr int VEC = Elem<T>::VEC;
+  const Span<T> sp(x, n);
+  uint4* v = reinterpret_cast<uint4*>(x + sp.lead);
+  for (int i = threadIdx.x; i < sp.nvec; i += NORM_THREADS) {
+    float f[VEC];
+    Elem<T>::unpack(v[i], f);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] *= c;
+    v[i] = Elem<T>::pack(f);
+  }
+  for (int j = threadIdx.x; j < sp.lead + n - sp.tail; j += NORM_THREADS) {
+    T* p = x + (j < sp.lead ? j : sp.tail + j - sp.lead);
+    Elem<T>::put(p, Elem<T>::get(p) * c);
+  }
+}
+
+__global__ void __launch_bounds__(NORM_THREADS)
+grad_clip_kernel(const __grid_constant__ TensorTable t, const double* partial, int num_partials, double max_norm, float* norm_out) {
+  __shared__ double smem[NORM_THREADS / 32];
+  bb::pdl_sync();
+  const float c = clip_coef<NORM_THREADS>(partial, num_partials, 1.0, max_norm, smem, norm_out);
+  if (c == 1.f) return;                         // within the norm: the gradients stay as they are
+  for (int piece = blockIdx.x; piece < t.first[t.count]; piece += gridDim.x) {
+    long long a, n;
+    const int i = table_find(t, piece, a, n);
+    if (t.dtype[i] == BB_DTYPE_F32) scale_piece(reinterpret_cast<float*>(t.data[i]) + a, (int)n, c);
+    else scale_piece(reinterpret_cast<__nv_bfloat16*>(t.data[i]) + a, (int)n, c);
+  }
+}
+
+// Adam on the clipped gradient; what the host can fold is folded there in 64 bits (1 - beta, bias corrections)
+struct AdamParams { float lr, b1, omb1, b2, omb2, eps, inv_bc1, inv_bc2, decay; int decoupled, zero_grad; };
+
+__global__ void __launch_bounds__(256)
+adam_clip_kernel(float* p, float* g, float* m, float* v, __nv_bfloat16* lp, long long n, const AdamParams a, const double* partial,
+                 int num_partials, double pre_scale, double max_norm, float* norm_out) {
+  __shared__ double smem[8];
+  bb::pdl_sync();
+  const float c = clip_coef<256>(partial, num_partials, pre_scale, max_norm, smem, norm_out) * (float)pre_scale;
+  const long long n4 = n >> 2, stride = (long long)gridDim.x * 256;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n4; i += stride) {
+    const float4 P = reinterpret_cast<float4*>(p)[i], G = reinterpret_cast<float4*>(g)[i];
+    const float4 M = reinterpret_cast<float4*>(m)[i], W = reinterpret_cast<float4*>(v)[i];
+    float pp[4] = {P.x, P.y, P.z, P.w}, gg[4] = {G.x, G.y, G.z, G.w}, mm[4] = {M.x, M.y, M.z, M.w}, vv[4] = {W.x, W.y, W.z, W.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float x = gg[e] * c;
+      if (!a.decoupled) x = fmaf(a.decay, pp[e], x);
+      mm[e] = fmaf(a.b1, mm[e], a.omb1 * x);
+      vv[e] = fmaf(a.b2, vv[e], a.omb2 * x * x);
+      float step = (mm[e] * a.inv_bc1) / (sqrtf(vv[e] * a.inv_bc2) + a.eps);
+      if (a.decoupled) step = fmaf(a.decay, pp[e], step);
+      pp[e] = fmaf(-a.lr, step, pp[e]);
+    }
+    reinterpret_cast<float4*>(p)[i] = make_float4(pp[0], pp[1], pp[2], pp[3]);
+    reinterpret_cast<float4*>(m)[i] = make_float4(mm[0], mm[1], mm[2], mm[3]);
+    reinterpret_cast<float4*>(v)[i] = make_float4(vv[0], vv[1], vv[2], vv[3]);
+    if (a.zero_grad) reinterpret_cast<float4*>(g)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (lp) reinterpret_cast<uint2*>(lp)[i] = make_uint2(bb::pack_bf16x2(pp[0], pp[1]), bb::pack_bf16x2(pp[2], pp[3]));
+  }
+}
+
+// ------------------------------------------------------------------ host side
+K2 split_k(double scale) {
+  const double k = scale * 1.4426950408889634;
+  int e;
+  const double m = frexp(k, &e);                       // [0.5, 1)
+  double hi = ldexp(floor(m * 65536.0), e - 16);
+  if (hi == k) hi = ldexp(floor(m * 65536.0) - 1.0, e - 16);
+  return {(float)hi, (float)(k - hi)};
+}
+
+bool bad_logits(const char* who, const void* logits, int dtype, long long ld, const void* targets, long long rows, int vocab, double scale) {
+  if (!logits || !targets || rows <= 0 || rows > INT_MAX || vocab <= 0 || ld < vocab || !(scale > 1e-30) || !(scale < 1e30) ||
+      (dtype != BB_DTYPE_BF16 && dtype != BB_DTYPE_F32) || ((uintptr_t)logits & (dtype == BB_DTYPE_F32 ? 3 : 1))) {
+    char msg[256];
+    snprintf(msg, sizeof(msg), "%s: null or misaligned pointer, a size that is not positive, ld < vocab, an unknown type or a scale outside (1e-30, 1e30)", who);
+    bb_set_last_error_msg(msg);
+    return true;
+  }
+  return false;
+}
+
+// Whether the gradient may be written where it is asked for: apart from the logits, or exactly over them
+bool bad_output(const void* logits, long long ld, const void* dlogits, long long ldd, int dtype, long long rows, int vocab, int cols) {
+  const size_t item = dtype == BB_DTYPE_F32 ? 4 : 2;
+  if (!dlogits || cols < vocab || ldd < cols || ((uintptr_t)dlogits & (item - 1))) return true;
+  if (dlogits == logits) return ldd != ld;
+  const uintptr_t a = (uintptr_t)logits, b = (uintptr_t)dlogits;
+  const size_t an = ((size_t)(rows - 1) * (size_t)ld + (size_t)vocab) * item, bn = ((size_t)(rows - 1) * (size_t)ldd + (size_t)cols) * item;
+  return a < b + bn && b < a + an;
+}
+
+int refuse(const char* msg) { bb_set_last_error_msg(msg); return BB_ERR_INVALID_ARG; }
+
+// counts of counted tokens, and the weights of the sequence reduction; both at the front of the workspace
+struct PolicyPlan { int num_counts; long long piece; size_t weight_at, partial_at, logp_at, bytes; };
+PolicyPlan policy_plan(long long tokens, int n_seq, int by_sequence, long long partials, bool logp) {
+  PolicyPlan pl;
+  pl.piece = 16384;
+  pl.num_counts = by_sequence ? n_seq : (int)((tokens + pl.piece - 1) / pl.piece);
+  size_t at = ((size_t)pl.num_counts * 4 + 15) & ~(size_t)15;
+  pl.weight_at = at; at += by_sequence ? (size_t)tokens * 4 : 0;
+  at = (at + 15) & ~(size_t)15;
+  pl.logp_at = at; at += logp ? (size_t)tokens * 4 : 0;
+  at = (at + 15) & ~(size_t)15;
+  pl.partial_at = at; at += (size_t)partials * 24;
+  pl.bytes = at;
+  return pl;
+}
+int policy_token_ctas(long long tokens) {
+  const long long want = (tokens + 1023) / 1024, cap = 4LL * bb_num_sms();
+  return (int)(want < cap ? want : cap);
+}
+
+// Pieces of the list's tensors dealt over the machine: enough for every SM, none below 4096 elements
+int table_fill(TensorTable& t, const bb_grad_tensor* list, int count) {
+  long long total = 0;
+  for (int i = 0; i < count; ++i) total += list[i].numel;
+  long long piece = (total / (4LL * bb_num_sms()) + 4095) / 4096 * 4096;
+  piece = piece < 4096 ? 4096 : piece > 65536 ? 65536 : piece;
+  while (total / piece + count > INT_MAX / 2) piece *= 2;
+  t.piece = (int)piece;
+  t.count = count;
+  int pieces = 0;
+  for (int i = 0; i < count; ++i) {
+    t.data[i] = list[i].data; t.numel[i] = list[i].numel; t.dtype[i] = (unsigned char)list[i].dtype;
+    t.first[i] = pieces;
+    pieces += (int)((list[i].numel + piece - 1) / piece);
+  }
+  t.first[count] = pieces;
+  return pieces;
+}
+int norm_ctas() { return 4 * bb_num_sms(); }
+
+bool bad_list(const bb_grad_tensor* list, int count) {
+  if (!list || count <= 0) return true;
+  for (int i = 0; i < count; ++i) {
+    const int d = list[i].dtype;
+    if (!list[i].data || list[i].numel <= 0 || list[i].numel > (1LL << 40) || (d != BB_DTYPE_BF16 && d != BB_DTYPE_F32) ||
+        ((uintptr_t)list[i].data & (d == BB_DTYPE_F32 ? 3 : 1)))
+      return true;
+  }
+  return false;
+}
+
+}  // namespace
+
+extern "C" int bb_token_logprob_fwd(const void* logits, int dtype, long long ld, const long long* targets, double scale, float* logp,
+                                    float* stats, long long rows, int vocab, long long ignore_index, void* stream) {
+  if (bad_logits("bb_token_logprob_fwd", logits, dtype, ld, targets, rows, vocab, scale)) return BB_ERR_INVALID_ARG;
+  if (!logp || !stats || ((uintptr_t)stats & 7)) return refuse("bb_token_logprob_fwd: logp and stats (8-byte aligned) are needed");
+  const K2 k = split_k(scale);
+  int* status = bb_device_status_word();
+  if (dtype == BB_DTYPE_BF16)
+    BB_CUDA_CHECK(bb_launch(token_logprob_fwd_kernel<__nv_bfloat16>, (int)rows, ROW_THREADS, 0, (cudaStream_t)stream, (const __nv_bfloat16*)logits, ld, targets,
+                            k, logp, (float2*)stats, vocab, ignore_index, status));
+  else
+    BB_CUDA_CHECK(bb_launch(token_logprob_fwd_kernel<float>, (int)rows, ROW_THREADS, 0, (cudaStream_t)stream, (const float*)logits, ld, targets, k,
+                            logp, (float2*)stats, vocab, ignore_index, status));
+  return BB_OK;
+}
+
+extern "C" int bb_token_logprob_bwd(const void* logits, int dtype, long long ld, const long long* targets, double scale, const float* stats,
+                                    const float* row_grad, const float* grad_scale_dev, float grad_scale, void* dlogits, long long ldd,
+                                    long long rows, int vocab, int cols, long long ignore_index, void* stream) {
+  if (bad_logits("bb_token_logprob_bwd", logits, dtype, ld, targets, rows, vocab, scale)) return BB_ERR_INVALID_ARG;
+  if (!stats || ((uintptr_t)stats & 7) || !row_grad || bad_output(logits, ld, dlogits, ldd, dtype, rows, vocab, cols))
+    return refuse("bb_token_logprob_bwd: null pointer, columns that do not cover the vocabulary, or a gradient that overlaps the logits without being in place");
+  const K2 k = split_k(scale);
+  const float g = (float)(scale * grad_scale);
+  if (dtype == BB_DTYPE_BF16)
+    BB_CUDA_CHECK(bb_launch(token_logprob_bwd_kernel<__nv_bfloat16>, (int)rows, ROW_THREADS, 0, (cudaStream_t)stream, (const __nv_bfloat16*)logits, ld, targets,
+                            (const float2*)stats, row_grad, grad_scale_dev, g, k, (__nv_bfloat16*)dlogits, ldd, vocab, cols, ignore_index));
+  else
+    BB_CUDA_CHECK(bb_launch(token_logprob_bwd_kernel<float>, (int)rows, ROW_THREADS, 0, (cudaStream_t)stream, (const float*)logits, ld, targets,
+                            (const float2*)stats, row_grad, grad_scale_dev, g, k, (float*)dlogits, ldd, vocab, cols, ignore_index));
+  return BB_OK;
+}
+
+extern "C" int bb_preference_loss(const bb_preference_desc* d, const float* logp, const float* ref, const long long* targets,
+                                  const long long* offsets, float* loss, float* rewards, float* row_grad, void* workspace,
+                                  long long workspace_bytes, void* stream) {
+  if (!d || !logp || !targets || !loss || !rewards || !row_grad || !workspace || ((uintptr_t)workspace & 7))
+    return refuse("bb_preference_loss: null pointer, or a workspace that is not 8-byte aligned");
+  if (d->tokens <= 0 || d->sequences <= 0 || d->sequences % 2 || (!offsets && d->tokens % d->sequences))
+    return refuse("bb_preference_loss: sequences come in pairs, and without offsets all have tokens / sequences tokens");
+  if (d->form < BB_PREFERENCE_SIGMOID || d->form > BB_PREFERENCE_SQUARED || !(d->beta > 0.0) || !(d->label_smoothing >= 0.0 && d->label_smoothing <= 1.0))
+    return refuse("bb_preference_loss: unknown form, beta that is not positive, or label smoothing outside [0, 1]");
+  const int pairs = d->sequences / 2;
+  if (workspace_bytes < bb_preference_workspace_bytes(d)) return refuse("bb_preference_loss: workspace smaller than bb_preference_workspace_bytes()");
+  cudaStream_t s = (cudaStream_t)stream;
+  double* pair_loss = (double*)workspace;
+  BackToBack overlap;
+  BB_CUDA_CHECK(bb_launch(preference_pair_kernel, pairs, 256, 0, s, logp, ref, targets, offsets, d->tokens / d->sequences, d->tokens, pairs, d->form,
+                          d->beta, d->label_smoothing, d->average, d->ignore_index, pair_loss, rewards, row_grad, bb_device_status_word()));
+  BB_CUDA_CHECK(bb_launch(preference_mean_kernel, 1, 256, 0, s, (const double*)pair_loss, pairs, loss));
+  return BB_OK;
+}
+extern "C" long long bb_preference_workspace_bytes(const bb_preference_desc* d) { return d && d->sequences > 0 ? (long long)d->sequences * 4 + 8 : -1; }
+
+namespace {
+int policy_check(const bb_policy_desc* d, const long long* targets, const long long* offsets, const float* advantages, const float* loss,
+                 const float* stats, const void* workspace) {
+  if (!d || !targets || !advantages || !loss || !stats || !workspace || ((uintptr_t)workspace & 15))
+    return refuse("bb_policy_loss: null pointer, or a workspace that is not 16-byte aligned");
+  if (d->tokens <= 0 || d->tokens > INT_MAX || d->sequences <= 0 || (!offsets && d->tokens % d->sequences))
+    return refuse("bb_policy_loss: sizes have to be positive, and without offsets all sequences have tokens / sequences tokens");
+  if (d->advantage_per_sequence && offsets) return refuse("bb_policy_loss: advantages per sequence go with sequences of one length");
+  if (!(d->clip_low >= 0.0) || !(d->clip_high >= 0.0) || !(d->kl_coef >= 0.0) || (d->reduction != BB_POLICY_TOKEN && d->reduction != BB_POLICY_SEQUENCE))
+    return refuse("bb_policy_loss: clipping bounds and the KL weight cannot be negative, the reduction is by token or by sequence");
+  return BB_OK;
+}
+// Counts of counted tokens and weights into the workspace, and what the token functions take
+int policy_front(const bb_policy_desc* d, const PolicyPlan& pl, const long long* targets, const long long* offsets, const float* old_logp,
+                 const float* advantages, const float* ref, void* workspace, PolicyParams& p, cudaStream_t s) {
+  char* ws = (char*)workspace;
+  const bool by_sequence = d->reduction == BB_POLICY_SEQUENCE;
+  int* counts = (int*)ws;
+  float* weight = by_sequence ? (float*)(ws + pl.weight_at) : nullptr;
+  const long long seq_len = d->tokens / d->sequences;
+  p.old_logp = old_logp; p.advantages = advantages; p.ref = ref; p.weight = weight; p.counts = counts; p.num_counts = pl.num_counts;
+  p.adv_div = d->advantage_per_sequence ? seq_len : 1;
+  p.low = (float)(1.0 - d->clip_low); p.high = (float)(1.0 + d->clip_high); p.kl_coef = ref ? (float)d->kl_coef : 0.f;
+  BB_CUDA_CHECK(bb_launch(policy_count_kernel, pl.num_counts, 256, 0, s, targets, offsets, by_sequence ? seq_len : pl.piece, d->tokens, d->ignore_index,
+                          counts, weight, bb_device_status_word()));
+  return BB_OK;
+}
+}  // namespace
+
+extern "C" long long bb_policy_workspace_bytes(const bb_policy_desc* d) {
+  if (!d || d->tokens <= 0 || d->sequences <= 0) return -1;
+  const long long partials = d->tokens > policy_token_ctas(d->tokens) ? d->tokens : policy_token_ctas(d->tokens);
+  return (long long)policy_plan(d->tokens, d->sequences, d->reduction == BB_POLICY_SEQUENCE, partials, true).bytes;
+}
+
+extern "C" int bb_policy_loss(const bb_policy_desc* d, const float* logp, const float* old_logp, const float* advantages, const float* ref,
+                              const long long* targets, const long long* offsets, float* loss, float* stats, float* row_grad,
+                              void* workspace, long long workspace_bytes, void* stream) {
+  if (int rc = policy_check(d, targets, offsets, advantages, loss, stats, workspace)) return rc;
+  if (!logp || !row_grad) return refuse("bb_policy_loss: logp and row_grad are needed");
+  if (workspace_bytes < bb_policy_workspace_bytes(d)) return refuse("bb_policy_loss: workspace smaller than bb_policy_workspace_bytes()");
+  cudaStream_t s = (cudaStream_t)stream;
+  const int ctas = policy_token_ctas(d->tokens);
+  const PolicyPlan pl = policy_plan(d->tokens, d->sequences, d->reduction == BB_POLICY_SEQUENCE, ctas, false);
+  double* partial = (double*)((char*)workspace + pl.partial_at);
+  PolicyParams p;
+  BackToBack overlap;
+  if (int rc = policy_front(d, pl, targets, offsets, old_logp, advantages, ref, workspace, p, s)) return rc;
+  BB_CUDA_CHECK(bb_launch(policy_token_kernel, ctas, 256, 0, s, logp, targets, p, d->tokens, d->ignore_index, row_grad, partial));
+  BB_CUDA_CHECK(bb_launch(policy_finish_kernel, 1, 1024, 0, s, (const double*)partial, (long long)ctas, p.counts, p.num_counts, loss, stats));
+  return BB_OK;
+}
+
+extern "C" int bb_policy_loss_logits(const bb_policy_desc* d, const void* logits, int dtype, long long ld, double scale, int vocab, int cols,
+                                     const float* old_logp, const float* advantages, const float* ref, const long long* targets,
+                                     const long long* offsets, float* loss, float* stats, float* logp, void* dlogits, long long ldd,
+                                     float grad_scale, void* workspace, long long workspace_bytes, void* stream) {
+  if (int rc = policy_check(d, targets, offsets, advantages, loss, stats, workspace)) return rc;
+  if (bad_logits("bb_policy_loss_logits", logits, dtype, ld, targets, d->tokens, vocab, scale)) return BB_ERR_INVALID_ARG;
+  if (!logp || bad_output(logits, ld, dlogits, ldd, dtype, d->tokens, vocab, cols))
+    return refuse("bb_policy_loss_logits: null pointer, columns that do not cover the vocabulary, or a gradient that overlaps the logits without being in place");
+  if (workspace_bytes < bb_policy_workspace_bytes(d)) return refuse("bb_policy_loss_logits: workspace smaller than bb_policy_workspace_bytes()");
+  cudaStream_t s = (cudaStream_t)stream;
+  const PolicyPlan pl = policy_plan(d->tokens, d->sequences, d->reduction == BB_POLICY_SEQUENCE, d->tokens, false);
+  double* partial = (double*)((char*)workspace + pl.partial_at);
+  const K2 k = split_k(scale);
+  const float g = (float)(scale * grad_scale);
+  int* status = bb_device_status_word();
+  PolicyParams p;
+  BackToBack overlap;
+  if (int rc = policy_front(d, pl, targets, offsets, old_logp, advantages, ref, workspace, p, s)) return rc;
+  if (dtype == BB_DTYPE_BF16)
+    BB_CUDA_CHECK(bb_launch(policy_row_kernel<__nv_bfloat16>, (int)d->tokens, ROW_THREADS, 0, s, (const __nv_bfloat16*)logits, ld, targets, p, k, g,
+                            (__nv_bfloat16*)dlogits, ldd, vocab, cols, d->ignore_index, logp, partial, status));
+  else
+    BB_CUDA_CHECK(bb_launch(policy_row_kernel<float>, (int)d->tokens, ROW_THREADS, 0, s, (const float*)logits, ld, targets, p, k, g, (float*)dlogits, ldd,
+                            vocab, cols, d->ignore_index, logp, partial, status));
+  BB_CUDA_CHECK(bb_launch(policy_finish_kernel, 1, 1024, 0, s, (const double*)partial, d->tokens, p.counts, p.num_counts, loss, stats));
+  return BB_OK;
+}
+
+extern "C" int bb_rescale_grad(void* grad, int dtype, long long ld, long long rows, int cols, const float* upstream, float made_for, void* stream) {
+  if (!grad || !upstream || rows <= 0 || rows > INT_MAX || cols <= 0 || ld < cols || made_for == 0.f || (dtype != BB_DTYPE_BF16 && dtype != BB_DTYPE_F32) ||
+      ((uintptr_t)grad & (dtype == BB_DTYPE_F32 ? 3 : 1)))
+    return refuse("bb_rescale_grad: null or misaligned pointer, a size that is not positive, an unknown type, or made_for = 0");
+  if (dtype == BB_DTYPE_BF16)
+    BB_CUDA_CHECK(bb_launch(rescale_kernel<__nv_bfloat16>, (int)rows, ROW_THREADS, 0, (cudaStream_t)stream, (__nv_bfloat16*)grad, ld, cols, upstream, made_for));
+  else
+    BB_CUDA_CHECK(bb_launch(rescale_kernel<float>, (int)rows, ROW_THREADS, 0, (cudaStream_t)stream, (float*)grad, ld, cols, upstream, made_for));
+  return BB_OK;
+}
+
+extern "C" int bb_grad_norm_partials(int count) { return count > 0 ? (count + LIST_TENSORS - 1) / LIST_TENSORS * norm_ctas() : 0; }
+
+extern "C" int bb_grad_sumsq(const bb_grad_tensor* tensors, int count, double* partials, void* stream) {
+  if (bad_list(tensors, count) || !partials) return refuse("bb_grad_sumsq: null pointer, an empty tensor, or a type other than bf16 and fp32");
+  for (int at = 0; at < count; at += LIST_TENSORS) {
+    TensorTable t;
+    table_fill(t, tensors + at, count - at < LIST_TENSORS ? count - at : LIST_TENSORS);
+    BB_CUDA_CHECK(bb_launch(grad_sumsq_kernel, norm_ctas(), NORM_THREADS, 0, (cudaStream_t)stream, t, partials + (long long)(at / LIST_TENSORS) * norm_ctas()));
+  }
+  return BB_OK;
+}
+
+extern "C" int bb_grad_clip(const bb_grad_tensor* tensors, int count, const double* partials, int num_partials, double max_norm, float* norm,
+                            void* stream) {
+  if (bad_list(tensors, count) || !partials || num_partials <= 0 || !norm || !(max_norm > 0.0))
+    return refuse("bb_grad_clip: null pointer, an empty tensor, a type other than bf16 and fp32, or a norm that is not positive");
+  for (int at = 0; at < count; at += LIST_TENSORS) {
+    TensorTable t;
+    const int pieces = table_fill(t, tensors + at, count - at < LIST_TENSORS ? count - at : LIST_TENSORS);
+    const int grid = pieces < norm_ctas() ? pieces : norm_ctas();
+    BB_CUDA_CHECK(bb_launch(grad_clip_kernel, grid, NORM_THREADS, 0, (cudaStream_t)stream, t, partials, num_partials, max_norm, norm));
+  }
+  return BB_OK;
+}
+
+extern "C" int bb_adam_step_clipped(float* master, float* grad, float* exp_avg, float* exp_avg_sq, void* param_bf16, long long n, double lr,
+                                    double beta1, double beta2, double eps, int step, int adam_w_mode, int bias_correction,
+                                    double weight_decay, double grad_scale, int zero_grad, const double* partials, int num_partials,
+                                    double max_norm, float* norm, void* stream) {
+  if (!master || !grad || !exp_avg || !exp_avg_sq || n <= 0 || (n & 3) || step < 1 || !partials || num_partials <= 0 || !norm || !(max_norm > 0.0) ||
+      (((uintptr_t)master | (uintptr_t)grad | (uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & 15) || ((uintptr_t)param_bf16 & 7))
+    return refuse("bb_adam_step_clipped: null or unaligned pointer, n not a multiple of 4, step < 1, or a norm that is not positive");
+  AdamParams a;
+  a.lr = (float)lr; a.b1 = (float)beta1; a.omb1 = (float)(1.0 - beta1); a.b2 = (float)beta2; a.omb2 = (float)(1.0 - beta2); a.eps = (float)eps;
+  a.inv_bc1 = bias_correction ? (float)(1.0 / (1.0 - pow(beta1, step))) : 1.f;
+  a.inv_bc2 = bias_correction ? (float)(1.0 / (1.0 - pow(beta2, step))) : 1.f;
+  a.decay = (float)weight_decay; a.decoupled = adam_w_mode ? 1 : 0; a.zero_grad = zero_grad;
+  const long long want = ((n >> 2) + 255) / 256, cap = 8LL * bb_num_sms();
+  BB_CUDA_CHECK(bb_launch(adam_clip_kernel, (int)(want < cap ? want : cap), 256, 0, (cudaStream_t)stream, master, grad, exp_avg, exp_avg_sq,
+                          (__nv_bfloat16*)param_bf16, n, a, partials, num_partials, grad_scale, max_norm, norm));
+  return BB_OK;
+}

@@ -6,6 +6,7 @@ or a call fails, an exception is raised.
 import ctypes
 import functools
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -61,6 +62,27 @@ class ConvDesc(ctypes.Structure):
     ]
 
 
+class PreferenceDesc(ctypes.Structure):
+    """bb_preference_desc: geometry and form of the paired preference loss (see include/bamboo_b200.h)."""
+    _fields_ = [
+        ("tokens", ctypes.c_longlong), ("sequences", ctypes.c_int), ("form", ctypes.c_int),
+        ("beta", ctypes.c_double), ("label_smoothing", ctypes.c_double),
+        ("average", ctypes.c_int), ("ignore_index", ctypes.c_longlong),
+    ]
+
+
+class PolicyDesc(ctypes.Structure):
+    """bb_policy_desc: geometry and constants of the clipped policy loss (see include/bamboo_b200.h)."""
+    _fields_ = [
+        ("tokens", ctypes.c_longlong), ("sequences", ctypes.c_int), ("reduction", ctypes.c_int),
+        ("clip_low", ctypes.c_double), ("clip_high", ctypes.c_double), ("kl_coef", ctypes.c_double),
+        ("advantage_per_sequence", ctypes.c_int), ("ignore_index", ctypes.c_longlong),
+    ]
+
+
+PREFERENCE_FORMS = {"sigmoid": 0, "hinge": 1, "squared": 2}
+POLICY_REDUCTIONS = {"token": 0, "sequence": 1}
+
 HALF_ATTENTION, HALF_MLP = 0, 1
 # kernels behind one call of bb_block_half_fwd / bb_block_half_bwd, per half (launch accounting)
 HALF_FWD_LAUNCHES = {HALF_ATTENTION: 4, HALF_MLP: 3}
@@ -101,6 +123,18 @@ def load():
         lib.bb_conv_bn_bwd_no_residual.argtypes = [vp] * 9 + [ll, vp]
         lib.bb_conv_bn_fwd_affine.argtypes = [vp] * 8 + [ll, vp]
         lib.bb_conv_bn_bwd_affine.argtypes = [vp] * 9 + [ll, vp]
+        d, f = ctypes.c_double, ctypes.c_float
+        lib.bb_token_logprob_fwd.argtypes = [vp, i, ll, vp, d, vp, vp, ll, i, ll, vp]
+        lib.bb_token_logprob_bwd.argtypes = [vp, i, ll, vp, d, vp, vp, vp, f, vp, ll, ll, i, i, ll, vp]
+        lib.bb_preference_workspace_bytes.restype = ll
+        lib.bb_preference_loss.argtypes = [vp] * 9 + [ll, vp]
+        lib.bb_policy_workspace_bytes.restype = ll
+        lib.bb_policy_loss.argtypes = [vp] * 11 + [ll, vp]
+        lib.bb_policy_loss_logits.argtypes = [vp, vp, i, ll, d, i, i] + [vp] * 9 + [ll, f, vp, ll, vp]
+        lib.bb_rescale_grad.argtypes = [vp, i, ll, ll, i, vp, f, vp]
+        lib.bb_grad_sumsq.argtypes = [vp, i, vp, vp]
+        lib.bb_grad_clip.argtypes = [vp, i, vp, i, d, vp, vp]
+        lib.bb_adam_step_clipped.argtypes = [vp] * 5 + [ll, d, d, d, d, i, i, i, d, d, i, vp, i, d, vp, vp]
         _lib = lib
     return _lib
 
@@ -534,3 +568,116 @@ def conv_bn_bwd(desc, x, y, z, mean, rstd, dz, dx, dres, scratch, residual=True,
     if rc < 0:
         check(rc, "bb_conv_bn_bwd")
     return dx
+
+
+# ---------------------------------------------------------------------------- post-training
+def _dtype(t, what):
+    import torch
+    if t.dtype == torch.bfloat16:
+        return 0
+    if t.dtype == torch.float32:
+        return 1
+    raise BambooNativeError(f"{what}: bf16 or fp32 expected, got {t.dtype}")
+
+
+def token_logprob_fwd(logits, targets, logp, stats, vocab, scale=1.0, ignore_index=-100):
+    """logits: [rows, cols] bf16 / fp32, unit inner stride; targets [rows] int64; logp [rows], stats [rows, 2] fp32."""
+    global LAUNCHES
+    LAUNCHES += 1
+    check(load().bb_token_logprob_fwd(logits.data_ptr(), _dtype(logits, "logits"), logits.stride(0), targets.data_ptr(), scale, logp.data_ptr(),
+                                      stats.data_ptr(), logits.shape[0], vocab, ignore_index, _raw_stream()), "bb_token_logprob_fwd")
+    return logp
+
+
+def token_logprob_bwd(logits, targets, stats, row_grad, dlogits, vocab, scale=1.0, ignore_index=-100, grad_scale=1.0, grad_scale_dev=None):
+    global LAUNCHES
+    LAUNCHES += 1
+    rows, cols = logits.shape
+    check(load().bb_token_logprob_bwd(logits.data_ptr(), _dtype(logits, "logits"), logits.stride(0), targets.data_ptr(), scale, stats.data_ptr(),
+                                      row_grad.data_ptr(), _addr(grad_scale_dev), grad_scale, dlogits.data_ptr(), dlogits.stride(0), rows, vocab,
+                                      cols, ignore_index, _raw_stream()), "bb_token_logprob_bwd")
+    return dlogits
+
+
+def preference_loss(desc, logp, ref, targets, offsets, loss, rewards, row_grad):
+    global LAUNCHES
+    LAUNCHES += 2
+    lib = load()
+    ws = workspace(max(0, lib.bb_preference_workspace_bytes(ctypes.byref(desc))), "post_training")
+    check(lib.bb_preference_loss(ctypes.byref(desc), logp.data_ptr(), _addr(ref), targets.data_ptr(), _addr(offsets), loss.data_ptr(),
+                                 rewards.data_ptr(), row_grad.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream()), "bb_preference_loss")
+    return loss
+
+
+def policy_loss(desc, logp, old_logp, advantages, ref, targets, offsets, loss, stats, row_grad):
+    global LAUNCHES
+    LAUNCHES += 3
+    lib = load()
+    ws = workspace(max(0, lib.bb_policy_workspace_bytes(ctypes.byref(desc))), "post_training")
+    check(lib.bb_policy_loss(ctypes.byref(desc), logp.data_ptr(), _addr(old_logp), advantages.data_ptr(), _addr(ref), targets.data_ptr(),
+                             _addr(offsets), loss.data_ptr(), stats.data_ptr(), row_grad.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream()),
+          "bb_policy_loss")
+    return loss
+
+
+def policy_loss_logits(desc, logits, targets, vocab, old_logp, advantages, ref, offsets, loss, stats, logp, dlogits, scale=1.0, grad_scale=1.0):
+    global LAUNCHES
+    LAUNCHES += 3
+    lib = load()
+    ws = workspace(max(0, lib.bb_policy_workspace_bytes(ctypes.byref(desc))), "post_training")
+    check(lib.bb_policy_loss_logits(ctypes.byref(desc), logits.data_ptr(), _dtype(logits, "logits"), logits.stride(0), scale, vocab, logits.shape[1],
+                                    _addr(old_logp), advantages.data_ptr(), _addr(ref), targets.data_ptr(), _addr(offsets), loss.data_ptr(),
+                                    stats.data_ptr(), logp.data_ptr(), dlogits.data_ptr(), dlogits.stride(0), grad_scale, ws.data_ptr(), ws.numel(),
+                                    _raw_stream()), "bb_policy_loss_logits")
+    return loss
+
+
+def rescale(grad, upstream, made_for):
+    """``grad`` [rows, cols], made for an upstream gradient of ``made_for``, times ``upstream`` (device) / made_for."""
+    global LAUNCHES
+    LAUNCHES += 1
+    rows, cols = grad.shape
+    check(load().bb_rescale_grad(grad.data_ptr(), _dtype(grad, "gradient"), grad.stride(0), rows, cols, upstream.data_ptr(), made_for, _raw_stream()),
+          "bb_rescale_grad")
+    return grad
+
+
+@functools.lru_cache(maxsize=None)
+def _tensor_table(n):
+    return struct.Struct("QqiI" * n)        # bb_grad_tensor[n]
+
+
+def grad_tensors(tensors):
+    """bb_grad_tensor[len(tensors)]: every tensor fills its memory without gaps."""
+    flat = []
+    for t in tensors:
+        flat += (t.data_ptr(), t.numel(), _dtype(t, "gradient"), 0)
+    return _tensor_table(len(tensors)).pack(*flat)
+
+
+def grad_norm_partials(count):
+    return load().bb_grad_norm_partials(count)
+
+
+def grad_sumsq(table, count, partials):
+    """Partial sums of squares of a list (``grad_tensors``) into ``partials`` (fp64, ``grad_norm_partials(count)`` values)."""
+    global LAUNCHES
+    LAUNCHES += (count + 127) // 128
+    check(load().bb_grad_sumsq(table, count, _addr(partials), _raw_stream()), "bb_grad_sumsq")
+
+
+def grad_clip(table, count, partials, num_partials, max_norm, norm):
+    global LAUNCHES
+    LAUNCHES += (count + 127) // 128
+    check(load().bb_grad_clip(table, count, _addr(partials), num_partials, max_norm, norm.data_ptr(), _raw_stream()), "bb_grad_clip")
+    return norm
+
+
+def adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, *, lr, beta1=0.9, beta2=0.999, eps=1e-8, step, adam_w_mode=True,
+                      bias_correction=True, weight_decay=0.0, grad_scale=1.0, zero_grad=True, partials, num_partials, max_norm, norm):
+    global LAUNCHES
+    LAUNCHES += 1
+    check(load().bb_adam_step_clipped(master.data_ptr(), grad.data_ptr(), exp_avg.data_ptr(), exp_avg_sq.data_ptr(), _addr(param_lp), master.numel(),
+                                      lr, beta1, beta2, eps, step, int(adam_w_mode), int(bias_correction), weight_decay, grad_scale, int(zero_grad),
+                                      _addr(partials), num_partials, max_norm, norm.data_ptr(), _raw_stream()), "bb_adam_step_clipped")
+    return norm

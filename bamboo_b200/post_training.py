@@ -1,0 +1,417 @@
+"""Post-training of the vocabulary models: what follows token cross entropy when a model learns from preferences or rewards.
+
+    token_logprobs      log-probabilities of given tokens, from logits
+    preference_loss     paired preference loss over token log-probabilities (reference against policy)
+    policy_loss         clipped policy loss with a KL term over token log-probabilities
+    PreferenceLoss,     the two from logits, as ``loss_fn`` of a ``PipelineModule`` (labels are a tuple of tensors) or in one
+    PolicyLoss          call without autograd (``loss_and_grad``)
+    clip_grad_norm_,    global norm over a list of gradients, clipping in place, and the Adam step that clips;
+    global_grad_norm,   ``gradient_clipping`` in the engine's configuration uses the same kernels
+    adam_step_clipped
+
+Formulas stand beside the kernels' declarations (``include/bamboo_b200.h``) and in ``csrc/post_training.cu``.  Tokens whose target is
+``ignore_index`` (prompts, padding) count nowhere and get no gradient; what stands at their places in logits, log-probabilities and
+advantages may be anything, NaN and infinities included.  Everything runs on the current stream, nothing synchronises, and there is no
+fallback: CPU tensors are refused.
+"""
+import torch
+from torch import nn
+
+from . import lib as L
+
+
+# ----------------------------------------------------------------------------------- arguments
+def _rows(logits, vocab):
+    """logits [..., cols] as [rows, cols] with unit inner stride (a copy only where strides ask for one)."""
+    if not logits.is_cuda:
+        raise L.BambooNativeError("logits: expected a CUDA tensor; the sm_100a kernels have no CPU fallback")
+    cols = logits.shape[-1]
+    vocab = cols if vocab is None else vocab
+    if not 0 < vocab <= cols:
+        raise ValueError(f"vocab {vocab} does not fit logits with {cols} columns")
+    lg = logits.detach().reshape(-1, cols)
+    if lg.stride(1) != 1 or (lg.shape[0] > 1 and lg.stride(0) < cols):
+        lg = lg.contiguous()
+    return lg, vocab
+
+
+def _flat(t, name, numel, dtype, device):
+    """A per-token (or per-sequence) tensor as contiguous 1-D memory of the given type."""
+    if t.device != device:
+        raise L.BambooNativeError(f"{name}: on {t.device}, the logits are on {device}")
+    if t.numel() != numel:
+        raise ValueError(f"{name}: {t.numel()} values for {numel}")
+    t = t.detach().reshape(-1)
+    if t.dtype != dtype:
+        if dtype == torch.int64 and t.is_floating_point():
+            raise TypeError(f"{name}: token ids are integers, got {t.dtype}")
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _geometry(targets, offsets):
+    """(sequences, offsets as int64): the rows of 2-D targets, or what the offsets delimit in 1-D ones."""
+    if offsets is not None:
+        if offsets.dim() != 1 or offsets.numel() < 2:
+            raise ValueError("offsets: one more than there are sequences, 1-D")
+        return offsets.numel() - 1, _flat(offsets, "offsets", offsets.numel(), torch.int64, targets.device)
+    if targets.dim() != 2:
+        raise ValueError("targets [sequences, tokens], or 1-D with offsets")
+    return targets.shape[0], None
+
+
+def _inverse(temperature):
+    if not temperature > 0:
+        raise ValueError(f"temperature has to be positive, got {temperature}")
+    return 1.0 / temperature
+
+
+def _wants_grad(t):
+    return t.requires_grad and torch.is_grad_enabled()
+
+
+# ----------------------------------------------------------------------------------- token log-probabilities
+def _logprobs(lg, tg, vocab, scale, ignore_index):
+    logp = torch.empty(lg.shape[0], dtype=torch.float32, device=lg.device)
+    stats = torch.empty(lg.shape[0], 2, dtype=torch.float32, device=lg.device)
+    if lg.shape[0]:
+        L.token_logprob_fwd(lg, tg, logp, stats, vocab, scale, ignore_index)
+    return logp, stats
+
+
+class _TokenLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, vocab, scale, ignore_index, inplace):
+        lg, vocab = _rows(logits, vocab)
+        tg = _flat(targets, "targets", lg.shape[0], torch.int64, lg.device)
+        logp, stats = _logprobs(lg, tg, vocab, scale, ignore_index)
+        ctx.args, ctx.shape, ctx.inplace = (vocab, scale, ignore_index), logits.shape, inplace
+        ctx.save_for_backward(lg, tg, stats)
+        return logp.view(targets.shape)
+
+    @staticmethod
+    def backward(ctx, grad):
+        lg, tg, stats = ctx.saved_tensors
+        vocab, scale, ignore_index = ctx.args
+        out = lg if ctx.inplace else torch.empty(lg.shape, dtype=lg.dtype, device=lg.device)
+        if lg.shape[0]:
+            row_grad = _flat(grad, "gradient", lg.shape[0], torch.float32, lg.device)
+            L.token_logprob_bwd(lg, tg, stats, row_grad, out, vocab, scale, ignore_index)
+        return out.view(ctx.shape), None, None, None, None, None
+
+
+def token_logprobs(logits, targets, vocab=None, *, temperature=1.0, ignore_index=-100, inplace=False):
+    """Log-probabilities (fp32, shaped like ``targets``) of ``targets`` under softmax(logits[..., :vocab] / temperature).
+
+    ``logits`` [..., cols] bf16 or fp32; columns from ``vocab`` on are padding and get a zero gradient.  Ignored targets give 0.
+    ``inplace``: the gradient overwrites the logits in the backward pass (once)."""
+    scale = _inverse(temperature)
+    if _wants_grad(logits):
+        return _TokenLogprobsFn.apply(logits, targets, vocab, scale, ignore_index, inplace)
+    lg, vocab = _rows(logits, vocab)
+    return _logprobs(lg, _flat(targets, "targets", lg.shape[0], torch.int64, lg.device), vocab, scale, ignore_index)[0].view(targets.shape)
+
+
+# ----------------------------------------------------------------------------------- losses over log-probabilities
+def _preference_desc(tokens, sequences, beta, form, label_smoothing, average, ignore_index):
+    if form not in L.PREFERENCE_FORMS:
+        raise ValueError(f"form {form!r}: one of {sorted(L.PREFERENCE_FORMS)}")
+    if sequences % 2:
+        raise ValueError(f"{sequences} sequences: preferences come in pairs (preferred, rejected)")
+    return L.PreferenceDesc(tokens=tokens, sequences=sequences, form=L.PREFERENCE_FORMS[form], beta=beta, label_smoothing=label_smoothing,
+                            average=int(average), ignore_index=ignore_index)
+
+
+def _policy_desc(tokens, sequences, advantages, clip_low, clip_high, kl_coef, reduction, ignore_index):
+    if reduction not in L.POLICY_REDUCTIONS:
+        raise ValueError(f"reduction {reduction!r}: one of {sorted(L.POLICY_REDUCTIONS)}")
+    per_sequence = advantages.numel() == sequences and tokens != sequences
+    return L.PolicyDesc(tokens=tokens, sequences=sequences, reduction=L.POLICY_REDUCTIONS[reduction], clip_low=clip_low, clip_high=clip_high,
+                        kl_coef=kl_coef, advantage_per_sequence=int(per_sequence), ignore_index=ignore_index)
+
+
+class _ScaledFn(torch.autograd.Function):
+    """A loss whose gradient was computed with it: backward multiplies by what arrives."""
+
+    @staticmethod
+    def forward(ctx, logps, loss, row_grad):
+        ctx.save_for_backward(row_grad)
+        return loss.clone()
+
+    @staticmethod
+    def backward(ctx, grad):
+        (row_grad,) = ctx.saved_tensors
+        return row_grad * grad, None, None
+
+
+def preference_loss(logps, ref_logps, targets, *, beta=0.1, form="sigmoid", label_smoothing=0.0, average=False, offsets=None,
+                    ignore_index=-100):
+    """(loss, rewards [sequences]) over token log-probabilities, with autograd for ``logps``.
+
+    Sequences 2i (preferred) and 2i + 1 (rejected) are a pair: the rows of 2-D ``targets``, or ``offsets`` [sequences + 1] into 1-D ones.
+    ``ref_logps``: the reference model's, or None.  ``form``: "sigmoid" (with ``label_smoothing``), "hinge" or "squared"; ``average``:
+    mean instead of sum over a sequence's tokens."""
+    sequences, offsets = _geometry(targets, offsets)
+    lp = _flat(logps, "logps", targets.numel(), torch.float32, targets.device)
+    loss, rewards, row_grad = _preference(lp, ref_logps, targets, offsets, _preference_desc(
+        lp.numel(), sequences, beta, form, label_smoothing, average, ignore_index))
+    if _wants_grad(logps):
+        loss = _ScaledFn.apply(logps, loss, row_grad.view(logps.shape))
+    return loss, rewards
+
+
+def _preference(lp, ref, targets, offsets, desc):
+    if not lp.is_cuda:
+        raise L.BambooNativeError("logps: expected a CUDA tensor; the sm_100a kernels have no CPU fallback")
+    n, dev = desc.tokens, lp.device
+    tg = _flat(targets, "targets", n, torch.int64, dev)
+    ref = None if ref is None else _flat(ref, "ref_logps", n, torch.float32, dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    rewards = torch.empty(desc.sequences, dtype=torch.float32, device=dev)
+    row_grad = torch.empty_like(lp)
+    L.preference_loss(desc, lp, ref, tg, offsets, loss, rewards, row_grad)
+    return loss, rewards, row_grad
+
+
+def policy_loss(logps, old_logps, advantages, targets, *, ref_logps=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, reduction="token",
+                offsets=None, ignore_index=-100):
+    """(loss, stats) over token log-probabilities, with autograd for ``logps``; stats [2]: mean KL, share of clipped tokens.
+
+    ``old_logps``: those of the policy that sampled the tokens (None: this very policy).  ``advantages``: per token, or per sequence of
+    2-D ``targets``.  ``reduction``: "token" averages over all counted tokens, "sequence" averages the sequences' means."""
+    sequences, offsets = _geometry(targets, offsets)
+    lp = _flat(logps, "logps", targets.numel(), torch.float32, targets.device)
+    if not lp.is_cuda:
+        raise L.BambooNativeError("logps: expected a CUDA tensor; the sm_100a kernels have no CPU fallback")
+    desc = _policy_desc(lp.numel(), sequences, advantages, clip_low, clip_high, kl_coef, reduction, ignore_index)
+    loss, stats = torch.empty((), dtype=torch.float32, device=lp.device), torch.empty(2, dtype=torch.float32, device=lp.device)
+    row_grad = torch.empty_like(lp)
+    L.policy_loss(desc, lp, *_policy_inputs(desc, old_logps, advantages, ref_logps, targets, lp.device), offsets, loss, stats, row_grad)
+    if _wants_grad(logps):
+        loss = _ScaledFn.apply(logps, loss, row_grad.view(logps.shape))
+    return loss, stats
+
+
+def _policy_inputs(desc, old, advantages, ref, targets, dev):
+    n = desc.tokens
+    return (None if old is None else _flat(old, "old_logps", n, torch.float32, dev),
+            _flat(advantages, "advantages", desc.sequences if desc.advantage_per_sequence else n, torch.float32, dev),
+            None if ref is None else _flat(ref, "ref_logps", n, torch.float32, dev),
+            _flat(targets, "targets", n, torch.int64, dev))
+
+
+# ----------------------------------------------------------------------------------- losses from logits
+class _LogitsLossFn(torch.autograd.Function):
+    """loss_fn(logits, labels) with the gradient made by ``loss.forward_for_backward`` / ``loss.gradient``."""
+
+    @staticmethod
+    def forward(ctx, logits, loss_fn, labels, offsets):
+        ctx.loss_fn, ctx.shape = loss_fn, logits.shape
+        loss, saved, ctx.args = loss_fn._forward(logits, labels, offsets)
+        ctx.save_for_backward(*saved)
+        return loss
+
+    @staticmethod
+    def backward(ctx, grad):
+        out = ctx.loss_fn._backward(ctx.saved_tensors, ctx.args, grad.reshape(1).to(torch.float32).contiguous())
+        return out.view(ctx.shape), None, None, None
+
+
+class PreferenceLoss:
+    """Paired preference loss from logits: ``loss_fn(logits, (targets, ref_logps))`` for the last stage; reference-free with targets alone.
+
+    ``vocab``: real logit columns (the rest is padding).  The gradient overwrites the logits in the backward pass unless ``inplace`` is
+    off.  ``rewards`` keeps the last call's beta-scaled log-ratios per sequence (device)."""
+
+    def __init__(self, vocab, *, beta=0.1, form="sigmoid", label_smoothing=0.0, average=False, temperature=1.0, ignore_index=-100,
+                 inplace=True):
+        self.vocab, self.scale, self.ignore_index, self.inplace = vocab, _inverse(temperature), ignore_index, inplace
+        self.form = (beta, form, label_smoothing, average)
+        self.rewards = None
+
+    def _losses(self, logits, labels, offsets):
+        targets, ref = labels if isinstance(labels, (tuple, list)) else (labels, None)
+        lg, vocab = _rows(logits, self.vocab)
+        sequences, offsets = _geometry(targets, offsets)
+        tg = _flat(targets, "targets", lg.shape[0], torch.int64, lg.device)
+        desc = _preference_desc(lg.shape[0], sequences, *self.form, self.ignore_index)
+        logp, stats = _logprobs(lg, tg, vocab, self.scale, self.ignore_index)
+        loss, self.rewards, row_grad = _preference(logp, ref, tg, offsets, desc)
+        return lg, tg, stats, row_grad, loss
+
+    def _forward(self, logits, labels, offsets):
+        *saved, loss = self._losses(logits, labels, offsets)
+        return loss, saved, ()
+
+    def _backward(self, saved, args, grad):
+        lg, tg, stats, row_grad = saved
+        out = lg if self.inplace else torch.empty(lg.shape, dtype=lg.dtype, device=lg.device)
+        return L.token_logprob_bwd(lg, tg, stats, row_grad, out, self.vocab, self.scale, self.ignore_index, grad_scale_dev=grad)
+
+    def __call__(self, logits, labels, offsets=None):
+        if _wants_grad(logits):
+            return _LogitsLossFn.apply(logits, self, labels, offsets)
+        return self._losses(logits, labels, offsets)[-1]
+
+    def loss_and_grad(self, logits, labels, *, offsets=None, out=None, grad_scale=1.0):
+        """(loss, rewards, gradient of the logits times ``grad_scale``) without autograd; ``out`` receives the gradient (the logits
+        themselves are allowed)."""
+        lg, tg, stats, row_grad, loss = self._losses(logits, labels, offsets)
+        d, grad = _gradient_buffer(lg, logits, out)
+        L.token_logprob_bwd(lg, tg, stats, row_grad, d, self.vocab, self.scale, self.ignore_index, grad_scale=grad_scale)
+        return loss, self.rewards, grad
+
+
+def _gradient_buffer(lg, logits, out):
+    """(rows view for the kernels, tensor for the caller) of the gradient."""
+    if out is None:
+        d = torch.empty(lg.shape, dtype=lg.dtype, device=lg.device)
+        return d, d.view(logits.shape)
+    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        raise ValueError("out: a tensor like the logits is expected")
+    d = out.detach().view(-1, out.shape[-1])
+    if d.stride(1) != 1:
+        raise ValueError("out: rows with unit stride are expected")
+    return d, out
+
+
+class PolicyLoss:
+    """Clipped policy loss from logits: ``loss_fn(logits, (targets, old_logps, advantages[, ref_logps]))`` for the last stage.
+
+    The gradient of a row of logits needs that row alone, so loss and gradient come from one pass in the forward call, for an upstream
+    gradient of ``grad_scale`` (the pipeline engine sets it to 1 / micro-batches); a different upstream gradient costs a pass
+    over the gradient in the backward call.  It overwrites the logits IN THE FORWARD call unless ``inplace`` is off.  ``stats`` keeps the
+    last call's mean KL and share of clipped tokens (device)."""
+
+    def __init__(self, vocab, *, clip_low=0.2, clip_high=0.2, kl_coef=0.0, reduction="token", temperature=1.0, ignore_index=-100,
+                 inplace=True):
+        self.vocab, self.scale, self.ignore_index, self.inplace = vocab, _inverse(temperature), ignore_index, inplace
+        self.form = (clip_low, clip_high, kl_coef, reduction)
+        self.grad_scale = 1.0
+        self.stats = None
+
+    def _prepare(self, logits, labels, offsets):
+        targets, old, advantages = labels[:3]
+        ref = labels[3] if len(labels) > 3 else None
+        lg, vocab = _rows(logits, self.vocab)
+        sequences, offsets = _geometry(targets, offsets)
+        desc = _policy_desc(lg.shape[0], sequences, advantages, *self.form, self.ignore_index)
+        return lg, vocab, desc, _policy_inputs(desc, old, advantages, ref, targets, lg.device), offsets
+
+    def _both(self, lg, vocab, desc, inputs, offsets, d, grad_scale):
+        old, advantages, ref, tg = inputs
+        loss = torch.empty((), dtype=torch.float32, device=lg.device)
+        logp = torch.empty(lg.shape[0], dtype=torch.float32, device=lg.device)
+        self.stats = torch.empty(2, dtype=torch.float32, device=lg.device)
+        L.policy_loss_logits(desc, lg, tg, vocab, old, advantages, ref, offsets, loss, self.stats, logp, d, self.scale, grad_scale)
+        return loss
+
+    def _forward(self, logits, labels, offsets):
+        lg, *rest = self._prepare(logits, labels, offsets)
+        d = lg if self.inplace else torch.empty(lg.shape, dtype=lg.dtype, device=lg.device)
+        return self._both(lg, *rest, d, self.grad_scale), (d,), (self.grad_scale,)
+
+    def _backward(self, saved, args, grad):
+        (d,) = saved
+        return L.rescale(d, grad, args[0])
+
+    def __call__(self, logits, labels, offsets=None):
+        if _wants_grad(logits):
+            return _LogitsLossFn.apply(logits, self, labels, offsets)
+        lg, vocab, desc, (old, advantages, ref, tg), offsets = self._prepare(logits, labels, offsets)
+        logp, _ = _logprobs(lg, tg, vocab, self.scale, self.ignore_index)
+        loss, self.stats = torch.empty((), dtype=torch.float32, device=lg.device), torch.empty(2, dtype=torch.float32, device=lg.device)
+        return L.policy_loss(desc, logp, old, advantages, ref, tg, offsets, loss, self.stats, torch.empty_like(logp))
+
+    def loss_and_grad(self, logits, labels, *, offsets=None, out=None, grad_scale=1.0):
+        """(loss, stats, gradient of the logits times ``grad_scale``) without autograd; ``out`` receives the gradient (the logits
+        themselves are allowed)."""
+        lg, *rest = self._prepare(logits, labels, offsets)
+        d, grad = _gradient_buffer(lg, logits, out)
+        return self._both(lg, *rest, d, grad_scale), self.stats, grad
+
+
+# ----------------------------------------------------------------------------------- gradient norm
+def _dense(t):
+    """Whether a tensor fills its memory without gaps, in whatever order of dimensions."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _gradients(tensors):
+    """The gradients of parameters (``main_grad`` of an arena's, else ``grad``), other tensors as they are; empty ones left out."""
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else tensors
+    grads = []
+    for t in tensors:
+        if isinstance(t, nn.Parameter):
+            t = t.main_grad if getattr(t, "main_grad", None) is not None else t.grad
+        if t is None or t.numel() == 0:
+            continue
+        if not t.is_cuda or (grads and t.device != grads[0].device):
+            raise L.BambooNativeError("gradients: CUDA tensors of one device are expected; the sm_100a kernels have no CPU fallback")
+        grads.append(t.detach() if t.requires_grad else t)
+    return grads
+
+
+def _partials(grads):
+    n = L.grad_norm_partials(len(grads))
+    return L.workspace(8 * n, "grad_norm"), n
+
+
+def global_grad_norm(tensors):
+    """2-norm over all gradients together (fp32 scalar on their device); nothing is changed."""
+    grads = _gradients(tensors)
+    if not grads:
+        return torch.zeros(())
+    grads = [g if _dense(g) else g.contiguous() for g in grads]
+    partials, n = _partials(grads)
+    L.grad_sumsq(L.grad_tensors(grads), len(grads), partials)
+    return partials[:8 * n].view(torch.float64).sum().sqrt().float()
+
+
+def clip_grad_norm_(tensors, max_norm):
+    """Scale the gradients in place so that their global 2-norm is at most ``max_norm``; returns the norm before (fp32 scalar, device).
+
+    ``tensors``: parameters, or the gradients themselves (bf16 and fp32 may be mixed).  coefficient = min(1, max_norm / (norm + 1e-6));
+    within the norm nothing is written."""
+    if not max_norm > 0:
+        raise ValueError(f"max_norm has to be positive, got {max_norm}")
+    grads = _gradients(tensors)
+    if not grads:
+        return torch.zeros(())
+    staged = [g if _dense(g) else g.contiguous() for g in grads]
+    partials, n = _partials(staged)
+    table = L.grad_tensors(staged)
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    L.grad_sumsq(table, len(staged), partials)
+    L.grad_clip(table, len(staged), partials, n, max_norm, norm)
+    for g, s in zip(grads, staged):
+        if s is not g:
+            g.copy_(s)
+    return norm
+
+
+def adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, *, max_norm, grad_scale=1.0, sumsq=None, **adam):
+    """One Adam step over a flat arena on the gradient clipped to ``max_norm``; returns the norm before clipping (fp32 scalar, device).
+
+    ``grad_scale`` multiplies the gradient first (1/dp averaging), the norm included.  ``sumsq``: sum of squares of the unscaled
+    gradients that the norm is over (fp64 [1], device) where it covers more than this arena.  ``adam``: as ``lib.adam_step``."""
+    if not max_norm > 0:
+        raise ValueError(f"max_norm has to be positive, got {max_norm}")
+    for t in (master, grad, exp_avg, exp_avg_sq):
+        if not t.is_cuda or t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != master.numel():
+            raise L.BambooNativeError("adam_step_clipped: contiguous fp32 CUDA tensors of one size are expected")
+    norm = torch.empty((), dtype=torch.float32, device=master.device)
+    if sumsq is None:
+        partials, n = _partials([grad])
+        L.grad_sumsq(L.grad_tensors([grad]), 1, partials)
+    else:
+        partials, n = sumsq, 1
+    return L.adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, grad_scale=grad_scale, partials=partials, num_partials=n,
+                               max_norm=max_norm, norm=norm, **adam)

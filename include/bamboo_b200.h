@@ -300,6 +300,89 @@ int bb_adam_step(float* master, float* grad, float* exp_avg, float* exp_avg_sq, 
  * (PipelineModule.build_layers(stage, buffer), DS/runtime/pipe/module.py:262-332). */
 int bb_cast_f32_to_bf16(const float* src, void* dst, long long n, void* stream);
 
+/* ---- post-training ---------------------------------------------------------------- */
+/* What follows pre-training: log-probabilities of given tokens, the paired preference loss and the clipped policy loss over
+ * them, the global gradient norm and clipping.  The reference stops at loss_fn(outputs, labels) (DS/runtime/pipe/engine.py:
+ * 1650-1663) and, for clipping, at get_grad_norm / clip_grad_norm_ in eager tensor operations (DS/runtime/utils.py:141-192,319). */
+enum { BB_DTYPE_BF16 = 0, BB_DTYPE_F32 = 1 };
+
+/* logp[r] = log softmax(scale * logits[r, :vocab])[targets[r]], 0 for rows whose target is ignore_index (such rows are not
+ * read).  Rows start anywhere (ld >= vocab elements, no alignment beyond the type's).  stats [rows, 2], 8-byte aligned, keeps
+ * what the backward call needs of each row's softmax.  A row without a finite logit gives -inf and a zero gradient; a
+ * target outside [0, vocab) sets the status word to BB_ERR_INVALID_ARG and counts as ignored. */
+int bb_token_logprob_fwd(const void* logits, int dtype, long long ld, const long long* targets, double scale, float* logp,
+                         float* stats, long long rows, int vocab, long long ignore_index, void* stream);
+/* dlogits[r, j] = row_grad[r] * grad_scale * (*grad_scale_dev, if given) * scale * ([j == target] - softmax_j), 0 in the padded
+ * columns vocab..cols and in ignored rows.  A row whose factor is 0 is written as zeros without being read.  May run in place. */
+int bb_token_logprob_bwd(const void* logits, int dtype, long long ld, const long long* targets, double scale, const float* stats,
+                         const float* row_grad, const float* grad_scale_dev, float grad_scale, void* dlogits, long long ldd,
+                         long long rows, int vocab, int cols, long long ignore_index, void* stream);
+
+/* Paired preference loss over token log-probabilities.  Sequences 2i (preferred) and 2i + 1 (rejected) form pair i; sequence q is
+ * tokens [q n, (q + 1) n) with n = tokens / sequences, or [offsets[q], offsets[q + 1]).  s_q = sum (average: mean) over counted
+ * tokens of logp - ref (ref may be NULL: 0), h = beta (s_2i - s_2i+1), and the loss is the mean over pairs of
+ *   SIGMOID  -(1 - e) log sig(h) - e log sig(-h), e = label_smoothing      HINGE  max(0, 1 - h)
+ *   SQUARED  (h / beta - 1 / (2 beta))^2
+ * rewards[q] = beta s_q; row_grad[t] = d loss / d logp[t] for the tokens of the sequences.  A sequence without counted tokens
+ * scores 0, tokens outside all sequences count nowhere.  Offsets that do not ascend within [0, tokens] set the status word and
+ * are cut to it. */
+enum { BB_PREFERENCE_SIGMOID = 0, BB_PREFERENCE_HINGE = 1, BB_PREFERENCE_SQUARED = 2 };
+typedef struct bb_preference_desc {
+  long long tokens;
+  int sequences, form;
+  double beta, label_smoothing;
+  int average;
+  long long ignore_index;
+} bb_preference_desc;
+long long bb_preference_workspace_bytes(const bb_preference_desc* d);
+int bb_preference_loss(const bb_preference_desc* d, const float* logp, const float* ref, const long long* targets,
+                       const long long* offsets, float* loss, float* rewards, float* row_grad, void* workspace,
+                       long long workspace_bytes, void* stream);
+
+/* Clipped policy loss.  Per counted token: ratio = exp(logp - old) (old NULL: 1), surrogate = min(ratio A, clamp(ratio, 1 -
+ * clip_low, 1 + clip_high) A), KL = exp(ref - logp) - (ref - logp) - 1 (ref NULL: none), loss = -surrogate + kl_coef KL.
+ * TOKEN averages over all counted tokens; SEQUENCE averages the means of the sequences, those without counted tokens
+ * as 0.  advantages: one per token, or (advantage_per_sequence, sequences of one length) one per sequence.
+ * stats[0] = mean KL, stats[1] = share of counted tokens whose surrogate is the clipped one. */
+enum { BB_POLICY_TOKEN = 0, BB_POLICY_SEQUENCE = 1 };
+typedef struct bb_policy_desc {
+  long long tokens;
+  int sequences, reduction;
+  double clip_low, clip_high, kl_coef;
+  int advantage_per_sequence;
+  long long ignore_index;
+} bb_policy_desc;
+long long bb_policy_workspace_bytes(const bb_policy_desc* d);
+int bb_policy_loss(const bb_policy_desc* d, const float* logp, const float* old_logp, const float* advantages, const float* ref,
+                   const long long* targets, const long long* offsets, float* loss, float* stats, float* row_grad,
+                   void* workspace, long long workspace_bytes, void* stream);
+/* The same from logits, with their gradient (times grad_scale) in the same pass: a row's gradient needs nothing of the other
+ * rows.  logp [tokens] receives the log-probabilities; arguments otherwise as above and in bb_token_logprob_*. */
+int bb_policy_loss_logits(const bb_policy_desc* d, const void* logits, int dtype, long long ld, double scale, int vocab, int cols,
+                          const float* old_logp, const float* advantages, const float* ref, const long long* targets,
+                          const long long* offsets, float* loss, float* stats, float* logp, void* dlogits, long long ldd,
+                          float grad_scale, void* workspace, long long workspace_bytes, void* stream);
+
+/* grad *= *upstream / made_for: a gradient made by bb_policy_loss_logits for another upstream gradient than the one that
+ * arrived.  Reads the scalar and returns where the two are the same. */
+int bb_rescale_grad(void* grad, int dtype, long long ld, long long rows, int cols, const float* upstream, float made_for,
+                    void* stream);
+
+/* Global norm of a list of gradients and clipping.  bb_grad_sumsq writes bb_grad_norm_partials(count) partial sums of squares
+ * (64-bit); their sum, over whatever else the caller adds (other pipeline stages), is the squared norm.  The consumers take
+ * `num_partials` such values, norm = grad_scale * sqrt(sum), coefficient = min(1, max_norm / (norm + 1e-6)), and write the
+ * norm before clipping to `norm` (device).  bb_grad_clip scales the tensors in place (not at all within the norm);
+ * bb_adam_step_clipped is an Adam step on coefficient * grad_scale * grad.  A norm that is NaN makes everything NaN. */
+typedef struct bb_grad_tensor { void* data; long long numel; int dtype; } bb_grad_tensor;
+int bb_grad_norm_partials(int count);
+int bb_grad_sumsq(const bb_grad_tensor* tensors, int count, double* partials, void* stream);
+int bb_grad_clip(const bb_grad_tensor* tensors, int count, const double* partials, int num_partials, double max_norm, float* norm,
+                 void* stream);
+int bb_adam_step_clipped(float* master, float* grad, float* exp_avg, float* exp_avg_sq, void* param_bf16, long long n, double lr,
+                         double beta1, double beta2, double eps, int step, int adam_w_mode, int bias_correction,
+                         double weight_decay, double grad_scale, int zero_grad, const double* partials, int num_partials,
+                         double max_norm, float* norm, void* stream);
+
 /* ---- inter-stage transfer --------------------------------------------------------- */
 /* Set-up (these four are the only entry points that allocate or map device memory; call
  * them when a channel to a neighbour is created, not per message): a receive mailbox in
