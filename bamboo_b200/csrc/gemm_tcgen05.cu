@@ -26,6 +26,7 @@
 // (template parameter CONV, bb_conv_gemm).
 #include "common.cuh"
 #include "bamboo_b200.h"
+#include "softmax2.cuh"
 #include "tma_host.cuh"
 #include <atomic>
 #include <mutex>
@@ -86,6 +87,27 @@ struct ConvParams {
 struct NoConv {};
 template <bool CONV> struct ConvArg { typedef NoConv type; };
 template <> struct ConvArg<true> { typedef ConvParams type; };
+
+// A vocabulary projection whose logits are not stored (template parameter HEAD): the epilogue turns them into partial softmax sums
+// (HEAD_SUMS), or into the gradient of the targets' log-probabilities (HEAD_GRAD, the bf16 output).
+constexpr int HEAD_NONE = 0, HEAD_SUMS = 1, HEAD_GRAD = 2;
+struct HeadParams {
+  const long long* targets;   // per row
+  long long ignore_index;
+  int vocab, col0;            // targets count up to vocab; column 0 of this product is vocabulary entry col0
+  K2 k;
+  float2* partial;            // SUMS: (r, s) of each half of a tile's columns, [2 * column tiles][M]
+  float* target_logit;        // SUMS: logit of the target, [M]
+  const float2* stats;        // GRAD: (r, s) per row
+  const float* row_grad; const float* gscale_dev; float gscale;
+};
+// The tensor core's fp32 additions truncate, so a sum's error grows with the number of its k-blocks (a logit of 4096 products
+// 4.6e-5 off, of 1024 products 2.4e-6).  Projections from more than 2048 columns sum the halves of the reduction into the two
+// accumulators and add those in the epilogue; the main loop of the next tile then covers less of the epilogue.
+constexpr int HEAD_WHOLE_KB = 2048 / BK;
+struct NoHead {};
+template <int HEAD> struct HeadArg { typedef HeadParams type; };
+template <> struct HeadArg<HEAD_NONE> { typedef NoHead type; };
 
 __device__ __forceinline__ void unpack8(const uint4& q, float* f) {
   f[0] = bb::bf16_lo(q.x); f[1] = bb::bf16_hi(q.x); f[2] = bb::bf16_lo(q.y); f[3] = bb::bf16_hi(q.y);
@@ -540,10 +562,57 @@ __device__ __forceinline__ void narrow_panel(const GemmParams& p, uint8_t* slab,
   __syncwarp();
 }
 
-template <int BN, bool PAIR, int EW, bool CONV>
+// A lane's row of a vocabulary projection: what it needs besides the accumulator, and the epilogue's arithmetic on 64 columns
+template <int HEAD> struct HeadRow {
+  float r, s;                 // SUMS: sums so far; GRAD: the row's sums
+  float g;                    // GRAD: factor of the row
+  int t;                      // its target as a column of this product; outside of it, or -1 for a row that does not count
+  __device__ __forceinline__ void load(const HeadParams& h, int row, int M) {
+    long long target = row < M ? h.targets[row] : h.ignore_index;
+    if (target == h.ignore_index || target < 0 || target >= h.vocab) target = -1;
+    t = target < 0 ? -1 : (int)(target - h.col0);
+    r = -INFINITY; s = 0.f; g = 0.f;
+    if constexpr (HEAD == HEAD_GRAD) {
+      if (target < 0) return;
+      const float2 st = h.stats[row];
+      r = st.x; s = st.y;
+      g = s == 0.f ? 0.f : h.row_grad[row] * (h.gscale_dev ? h.gscale_dev[0] : 1.f) * h.gscale;
+    }
+  }
+  __device__ __forceinline__ void sums(const HeadParams& h, int nb, int N, int row, int M, float* v) {
+    if (t >= nb && t < nb + 64) {
+      float x = 0.f;
+#pragma unroll
+      for (int i = 0; i < 64; ++i) if (nb + i == t) x = v[i];
+      h.target_logit[row] = x;
+    }
+    if (nb + 64 > N) {
+#pragma unroll
+      for (int i = 0; i < 64; ++i) if (nb + i >= N) v[i] = -INFINITY;
+    }
+    bb::soft_add<64>(r, s, v, h.k);
+  }
+  __device__ __forceinline__ void gradient(const HeadParams& h, int nb, float* v) {
+    const float ng = -g / s;
+    // (a row without a factor is zeros whatever its logits are)
+#pragma unroll
+    for (int i = 0; i < 64; i += 2) {
+      const float2 e = bb::expo2(make_float2(v[i], v[i + 1]), h.k, r);
+      v[i] = g == 0.f ? 0.f : ng * bb::ex2(e.x);
+      v[i + 1] = g == 0.f ? 0.f : ng * bb::ex2(e.y);
+    }
+    if (t >= nb && t < nb + 64) {
+#pragma unroll
+      for (int i = 0; i < 64; ++i) if (nb + i == t) v[i] += g;
+    }
+  }
+};
+template <> struct HeadRow<HEAD_NONE> {};
+
+template <int BN, bool PAIR, int EW, bool CONV, int HEAD>
 __global__ void __launch_bounds__(num_threads(EW), 1)
 gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                         const GemmParams p, const typename ConvArg<CONV>::type cv) {
+                         const GemmParams p, const typename ConvArg<CONV>::type cv, const typename HeadArg<HEAD>::type hd) {
   using C = Cfg<BN, PAIR>;
   extern __shared__ uint8_t smem_raw[];
   // 128-byte swizzle atoms need 1024-byte aligned stage buffers
@@ -705,7 +774,18 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
       const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
       int mi, ni, ks;
       unit_coords(p, tile, mi, ni, ks);
-      const int num_kb = min(total_kb, (ks + 1) * p.kb_per_split) - ks * p.kb_per_split;
+      int num_kb = min(total_kb, (ks + 1) * p.kb_per_split) - ks * p.kb_per_split;
+      if constexpr (HEAD != HEAD_NONE) {
+        if (total_kb > HEAD_WHOLE_KB) {         // first half here (accumulator 0), the second below
+          const int first = num_kb >> 1;
+          if (!issue_mmas<BN, PAIR>(p, sA, sB, full_bar, empty_bar, &tmem_full[0], abort_flag, 3, tmem_base, first, s, phase)) { alive = false; break; }
+          if (!bb::mbar_wait_warp(&tmem_empty[1], acc_phase ^ 1, abort_flag, p.status)) { alive = false; break; }
+          bb::tc_fence_after_sync();
+          if (!issue_mmas<BN, PAIR>(p, sA, sB, full_bar, empty_bar, &tmem_full[1], abort_flag, 3, tmem_base + BN, num_kb - first, s, phase)) { alive = false; break; }
+          acc_phase ^= 1;
+          continue;
+        }
+      }
       if (!issue_mmas<BN, PAIR>(p, sA, sB, full_bar, empty_bar, &tmem_full[acc], abort_flag, 3, d_tmem, num_kb, s, phase)) { alive = false; break; }
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
@@ -718,7 +798,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
     // another warp or on the TMA queue, which the producer keeps full of operand loads.
     const int eg = (warp - EPI_WARP) >> 2;         // which of the quarter's EW warps
     const int quarter = warp & 3;
-    const int epi = p.epi;
+    const int epi = HEAD == HEAD_NONE ? p.epi : (int)BB_EPI_STORE;
     const bool f32 = (epi == BB_EPI_ACCUM_F32 || epi == BB_EPI_STORE_F32);
     const bool dual = (epi == BB_EPI_BIAS_GELU);
     const bool has_aux = (epi == BB_EPI_MUL_DGELU || epi == BB_EPI_BIAS_RESIDUAL);
@@ -776,9 +856,20 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
       unit_coords(p, tile, mi, ni, ks);
       const int m0 = mi * C::TILE_M + (int)rank * BM, n0 = ni * BN;
       const int r0 = m0 + quarter * 32;            // first output row of this warp
+      HeadRow<HEAD> head;
+      if constexpr (HEAD != HEAD_NONE) head.load(hd, r0 + lane, p.M);      // in flight while the accumulator is waited for
       const bool got = bb::mbar_wait(&tmem_full[acc], acc_phase, abort_flag, p.status);
       if (!__all_sync(0xffffffffu, got)) { alive = false; break; }
       bb::tc_fence_after_sync();
+      bool halves = false;                         // the reduction's second half is in accumulator 1
+      if constexpr (HEAD != HEAD_NONE) {
+        halves = total_kb > HEAD_WHOLE_KB;
+        if (halves) {
+          const bool both = bb::mbar_wait(&tmem_full[1], acc_phase, abort_flag, p.status);
+          if (!__all_sync(0xffffffffu, both)) { alive = false; break; }
+          bb::tc_fence_after_sync();
+        }
+      }
       const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN);
       const int width = f32 ? 32 : 64;             // columns per panel
       const int npanels = BN / width;
@@ -806,6 +897,17 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[32 + i] = __uint_as_float(r[i]);
           }
+          if constexpr (HEAD != HEAD_NONE) {
+            if (halves) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                bb::tmem_ld_32x32b_x32(t_row + BN + pn * width + 32 * h, r);
+                bb::tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[32 * h + i] += __uint_as_float(r[i]);
+              }
+            }
+          }
         }
         if (pn + 2 >= npanels) {
           // this warp has read its share of the accumulator: hand it back before the last stores
@@ -814,9 +916,15 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
           if (lane == 0) {
             if (PAIR) bb::mbar_arrive_cluster_relaxed(bb::mapa_shared(bb::smem_u32(&tmem_empty[acc]), 0));
             else bb::mbar_arrive(&tmem_empty[acc]);
+            if (halves) {
+              if (PAIR) bb::mbar_arrive_cluster_relaxed(bb::mapa_shared(bb::smem_u32(&tmem_empty[1]), 0));
+              else bb::mbar_arrive(&tmem_empty[1]);
+            }
           }
         }
         if (!some) continue;                     // panel entirely outside the matrix
+        if constexpr (HEAD == HEAD_SUMS) { head.sums(hd, nb, p.N, r0 + lane, p.M, v); continue; }
+        if constexpr (HEAD == HEAD_GRAD) head.gradient(hd, nb, v);
         if (f32) {
           panel_store_row_f32(slab, lane, v);
           __syncwarp();
@@ -847,6 +955,12 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
         __syncwarp();
         slab_flush_bf16(slab, reinterpret_cast<__nv_bfloat16*>(p.D), p.ldd, r0, nb, p.M, p.N, lane);
         __syncwarp();
+      }
+      if constexpr (HEAD == HEAD_SUMS) {
+        if (r0 + lane < p.M) hd.partial[(long long)(2 * ni + eg) * p.M + r0 + lane] = make_float2(head.r, head.s);
+      }
+      if constexpr (HEAD != HEAD_NONE) {
+        if (halves) { acc_phase ^= 1; continue; }
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
@@ -1132,8 +1246,9 @@ int operands(const bb_gemm_desc* g, const bb_conv_gemm_args* cv, CUtensorMap& tm
   return BB_OK;
 }
 
-template <int BN, bool PAIR, int EW, bool CONV>
-int launch(const bb_gemm_desc* g, cudaStream_t stream, const bb_conv_gemm_args* cv = nullptr) {
+template <int BN, bool PAIR, int EW, bool CONV, int HEAD = HEAD_NONE>
+int launch(const bb_gemm_desc* g, cudaStream_t stream, const bb_conv_gemm_args* cv = nullptr,
+           const typename HeadArg<HEAD>::type& hd = typename HeadArg<HEAD>::type()) {
   using C = Cfg<BN, PAIR>;
   CUtensorMap tmA, tmB;
   GemmParams p;
@@ -1154,7 +1269,7 @@ int launch(const bb_gemm_desc* g, cudaStream_t stream, const bb_conv_gemm_args* 
   if (ksplit < 1) ksplit = 1;
   p.kb_per_split = (total_kb + ksplit - 1) / ksplit;
   p.ksplit = (total_kb + p.kb_per_split - 1) / p.kb_per_split;   // no empty splits
-  BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(gemm_bf16_tcgen05_kernel<BN, PAIR, EW, CONV>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES)));
+  BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(gemm_bf16_tcgen05_kernel<BN, PAIR, EW, CONV, HEAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES)));
   const int tiles = mn_tiles * p.ksplit;
   int workers = workers_max;
   if (g->max_ctas > 0 && g->max_ctas / (PAIR ? 2 : 1) < workers) workers = g->max_ctas / (PAIR ? 2 : 1);
@@ -1184,14 +1299,14 @@ int launch(const bb_gemm_desc* g, cudaStream_t stream, const bb_conv_gemm_args* 
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = bb_back_to_back > 0 ? 2 : 1;
-    cudaError_t le = cudaLaunchKernelEx(&cfg, gemm_bf16_tcgen05_kernel<BN, true, EW, CONV>, tmA, tmB, p, cp);
+    cudaError_t le = cudaLaunchKernelEx(&cfg, gemm_bf16_tcgen05_kernel<BN, true, EW, CONV, HEAD>, tmA, tmB, p, cp, hd);
     if (le != cudaSuccess) {
       if (tt) tt->base[slot] -= (unsigned)tiles;     // nothing ran: the counter keeps its value
       bb_set_last_error("gemm_bf16_tcgen05_kernel (pair) launch", le);
       return BB_ERR_CUDA;
     }
   } else {
-    bb_launch(gemm_bf16_tcgen05_kernel<BN, false, EW, CONV>, workers, num_threads(EW), C::SMEM_BYTES, stream, tmA, tmB, p, cp);
+    bb_launch(gemm_bf16_tcgen05_kernel<BN, false, EW, CONV, HEAD>, workers, num_threads(EW), C::SMEM_BYTES, stream, tmA, tmB, p, cp, hd);
   }
   {
     cudaError_t le = cudaGetLastError();
@@ -1478,6 +1593,110 @@ extern "C" int bb_gemm_bf16(const bb_gemm_desc* g, void* stream) {
   if (pair) return wide_epi ? launch<256, true, 4, false>(g, s) : launch<256, true, 2, false>(g, s);
   if (bn == 256) return wide_epi ? launch<256, false, 4, false>(g, s) : launch<256, false, 2, false>(g, s);
   return wide_epi ? launch<128, false, 4, false>(g, s) : launch<128, false, 2, false>(g, s);
+}
+
+// ------------------------------------------------------------------ vocabulary projection without stored logits
+namespace {
+// (r, s) of a row from its partial sums, and the log-probability of its target.  32 rows per CTA, one lane each; the warps share
+// the partial sums.
+__global__ void __launch_bounds__(1024)
+head_combine_kernel(const float2* partial, int num, int rows, const float* target_logit, const long long* targets, long long ignore_index,
+                    int vocab, K2 k, float* logp, float2* stats, int* status) {
+  __shared__ float2 sums[32][32];
+  bb::pdl_sync();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
+  float r = -INFINITY, s = 0.f;
+  if (row < rows) {
+#pragma unroll 4
+    for (int i = warp; i < num; i += 32) {
+      const float2 q = __ldcg(partial + (long long)i * rows + row);
+      bb::soft_merge(r, s, q.x, q.y);
+    }
+  }
+  sums[warp][lane] = make_float2(r, s);
+  __syncthreads();
+  if (warp != 0 || row >= rows) return;
+  for (int w = 1; w < 32; ++w) bb::soft_merge(r, s, sums[w][lane].x, sums[w][lane].y);
+  const long long t = targets[row];
+  const bool counted = t != ignore_index && t >= 0 && t < vocab;
+  if (!counted && t != ignore_index) atomicCAS(status, 0, BB_ERR_INVALID_ARG);
+  logp[row] = counted ? (float)bb::row_logp(target_logit[row], k, r, s) : 0.f;
+  stats[row] = counted ? make_float2(r, s) : make_float2(0.f, 0.f);
+}
+
+// Tile of the projection, from the same expected times as any stored product (its epilogue stores nothing, but the main loop
+// is what the tile is chosen by)
+StorePlan head_plan(int rows, int vocab, int hidden) { return plan_store(rows, vocab, hidden, 0, true); }
+
+template <int HEAD> int head_launch(const bb_gemm_desc& g, const HeadParams& hd, cudaStream_t s) {
+  const StorePlan pl = head_plan(g.M, g.N, g.K);
+  if (pl.pair) return launch<256, true, 2, false, HEAD>(&g, s, nullptr, hd);
+  return pl.bn == 256 ? launch<256, false, 2, false, HEAD>(&g, s, nullptr, hd) : launch<128, false, 2, false, HEAD>(&g, s, nullptr, hd);
+}
+
+int head_check(const char* who, const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets) {
+  const bool ok = d && hidden_states && weight && targets && d->rows > 0 && d->vocab > 0 && d->hidden > 0 && d->ld_hidden % 8 == 0 && d->ld_weight % 8 == 0 &&
+                  d->ld_hidden >= d->hidden && d->ld_weight >= d->hidden && !((uintptr_t)hidden_states & 15) && !((uintptr_t)weight & 15) &&
+                  d->scale > 1e-30 && d->scale < 1e30;
+  if (ok) return BB_OK;
+  char msg[256];
+  snprintf(msg, sizeof(msg), "%s: null pointer, a size that is not positive, rows that are not 16-byte aligned, or a scale outside (1e-30, 1e30)", who);
+  bb_set_last_error_msg(msg);
+  return BB_ERR_INVALID_ARG;
+}
+
+HeadParams head_params(const bb_head_desc* d, const long long* targets) {
+  HeadParams h = {};
+  h.targets = targets; h.ignore_index = d->ignore_index; h.vocab = d->vocab; h.k = split_k(d->scale);
+  return h;
+}
+}  // namespace
+
+extern "C" long long bb_head_logprob_workspace_bytes(const bb_head_desc* d) {
+  if (!d || d->rows <= 0 || d->vocab <= 0 || d->hidden <= 0) return -1;
+  const StorePlan pl = head_plan(d->rows, d->vocab, d->hidden);
+  return (long long)d->rows * (2LL * ((d->vocab + pl.bn - 1) / pl.bn) * 8 + 4);
+}
+
+extern "C" int bb_head_logprob_fwd(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets, float* logp,
+                                   float* stats, void* workspace, long long workspace_bytes, void* stream) {
+  if (int rc = head_check("bb_head_logprob_fwd", d, hidden_states, weight, targets)) return rc;
+  if (!logp || !stats || !workspace || (((uintptr_t)stats | (uintptr_t)workspace) & 7) || workspace_bytes < bb_head_logprob_workspace_bytes(d)) {
+    bb_set_last_error_msg("bb_head_logprob_fwd: outputs and a workspace of bb_head_logprob_workspace_bytes() are needed, 8-byte aligned");
+    return BB_ERR_INVALID_ARG;
+  }
+  if (int rc = bbhost::bind_context()) return rc;
+  cudaStream_t s = (cudaStream_t)stream;
+  const int bn = head_plan(d->rows, d->vocab, d->hidden).bn, num = 2 * ((d->vocab + bn - 1) / bn);
+  bb_gemm_desc g = {};
+  g.M = d->rows; g.N = d->vocab; g.K = d->hidden; g.A = hidden_states; g.lda = d->ld_hidden; g.B = weight; g.ldb = d->ld_weight;
+  g.epilogue = BB_EPI_STORE;
+  HeadParams h = head_params(d, targets);
+  h.partial = (float2*)workspace;
+  h.target_logit = (float*)(h.partial + (long long)num * d->rows);
+  BackToBack overlap;
+  if (int rc = head_launch<HEAD_SUMS>(g, h, s)) return rc;
+  BB_CUDA_CHECK(bb_launch(head_combine_kernel, (d->rows + 31) / 32, 1024, 0, s, (const float2*)h.partial, num, d->rows, (const float*)h.target_logit, targets,
+                          d->ignore_index, d->vocab, h.k, logp, (float2*)stats, bb_device_status_word()));
+  return BB_OK;
+}
+
+extern "C" int bb_head_logprob_grad(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets, const float* stats,
+                                    const float* row_grad, const float* grad_scale_dev, float grad_scale, int col0, int cols, void* dlogits,
+                                    long long ldd, void* stream) {
+  if (int rc = head_check("bb_head_logprob_grad", d, hidden_states, weight, targets)) return rc;
+  if (!stats || ((uintptr_t)stats & 7) || !row_grad || !dlogits || ((uintptr_t)dlogits & 15) || ldd % 8 || col0 < 0 || cols <= 0 || cols > d->vocab - col0 || ldd < cols) {
+    bb_set_last_error_msg("bb_head_logprob_grad: null or unaligned pointer, or columns that are no part of the vocabulary");
+    return BB_ERR_INVALID_ARG;
+  }
+  if (int rc = bbhost::bind_context()) return rc;
+  bb_gemm_desc g = {};
+  g.M = d->rows; g.N = cols; g.K = d->hidden; g.A = hidden_states; g.lda = d->ld_hidden;
+  g.B = (const __nv_bfloat16*)weight + (long long)col0 * d->ld_weight; g.ldb = d->ld_weight;
+  g.D = dlogits; g.ldd = ldd; g.epilogue = BB_EPI_STORE;
+  HeadParams h = head_params(d, targets);
+  h.col0 = col0; h.stats = (const float2*)stats; h.row_grad = row_grad; h.gscale_dev = grad_scale_dev; h.gscale = (float)(d->scale * grad_scale);
+  return head_launch<HEAD_GRAD>(g, h, (cudaStream_t)stream);
 }
 
 double bb_gemm_store_us(long long M, long long N, long long K, int max_ctas) {

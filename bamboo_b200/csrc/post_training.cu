@@ -1,12 +1,7 @@
 // Post-training of the vocabulary models: log-probabilities of given tokens with their gradient, the paired preference loss, the
 // clipped policy loss with a KL term, the global gradient norm over a list of tensors, clipping, and the Adam step that clips.
-//
-// Softmax in base 2.  With k = scale * log2(e) the kernels sum 2^(k x - r) for an INTEGER reference r >= max(k x): partial sums with
-// different references meet exactly (powers of two).  A row is kept as the pair (r, s): softmax_j = 2^(k x_j - r) / s, log
-// softmax_j = (k x_j - r - log2 s) ln 2, the latter once per row in 64 bits.  k comes in two parts (K2): rounded to 32 bits it would
-// be another temperature, 1.3e-8 off, which moves every log-probability of a sequence to the same side (measured on four
-// sequences of 1024 tokens: the sum of log-ratios 2.7e-5 off, in two parts 2e-6, which is the rounding of the log-probabilities).
-#include "common.cuh"
+// Softmax sums as in softmax2.cuh.
+#include "softmax2.cuh"
 #include <limits.h>
 #include <math.h>
 #include <stdio.h>
@@ -40,15 +35,12 @@ template <> struct Elem<float> {
   static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// k = hi + lo, hi with 16 significant bits (x hi is exact for a bf16 x), lo > 0 (so that -inf stays -inf)
-struct K2 { float hi, lo; };
-__device__ __forceinline__ float expo(float x, K2 k, float r) { return fmaf(x, k.lo, fmaf(x, k.hi, -r)); }
+using bb::expo;
+using bb::expo2;
+using bb::ex2;
+using bb::row_logp;
+using bb::soft_add;
+using bb::soft_merge;
 
 // A row of n elements as [0, lead) up to the first 16-byte boundary, nvec vectors, and the rest from `tail`.
 template <typename T> struct Span {
@@ -60,24 +52,6 @@ template <typename T> struct Span {
     tail = lead + nvec * Elem<T>::VEC;
   }
 };
-
-// ---- partial softmax sums: (r, s), r an integer or -inf (nothing yet, or only -inf logits)
-__device__ __forceinline__ void soft_merge(float& r, float& s, float r2, float s2) {
-  const float rn = fmaxf(r, r2);
-  // (equal references add as they are: -inf - -inf would be NaN)
-  s = (r == rn ? s : s * ex2(r - rn)) + (r2 == rn ? s2 : s2 * ex2(r2 - rn));
-  r = rn;
-}
-template <int N> __device__ __forceinline__ void soft_add(float& r, float& s, const float* f, K2 k) {
-  float top = f[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) top = fmaxf(top, f[i]);
-  const float rn = ceilf(expo(top, k, 0.f));
-  if (rn > r) { s = r == -INFINITY ? s : s * ex2(r - rn); r = rn; }
-  const float ref = r == -INFINITY ? 0.f : r;          // only -inf so far: 2^-inf = 0 is added, NaN stays NaN
-#pragma unroll
-  for (int i = 0; i < N; ++i) s += ex2(expo(f[i], k, ref));
-}
 
 // (r, s) of the block's threads merged; every thread gets the result
 template <int THREADS> __device__ __forceinline__ void soft_block(float& r, float& s, float2* smem /*[THREADS/32]*/) {
@@ -139,13 +113,6 @@ template <typename T, int THREADS> __device__ __forceinline__ void soft_whole_ro
   soft_row<T, THREADS>(x, n, k, r, s);
   soft_block<THREADS>(r, s, smem);
   if (isinf(r)) soft_row_extreme<T, THREADS>(x, n, r, s, smem);
-}
-
-// log softmax of logit x in 64 bits; a row without any finite logit (s = 0) has no distribution: -inf
-__device__ __forceinline__ double row_logp(float x, K2 k, float r, float s) {
-  if (s == 0.f) return -INFINITY;
-  if (s < 0.f) return x == r ? -log((double)-s) : -INFINITY;
-  return ((double)x * ((double)k.hi + (double)k.lo) - ((double)r + log2((double)s))) * 0.69314718055994531;
 }
 
 // d[j] = g * ([j == t] - softmax_j) for j < V, 0 in [V, cols); zeros throughout when g == 0 (nothing is read then)
@@ -623,15 +590,6 @@ adam_clip_kernel(float* p, float* g, float* m, float* v, __nv_bfloat16* lp, long
 }
 
 // ------------------------------------------------------------------ host side
-K2 split_k(double scale) {
-  const double k = scale * 1.4426950408889634;
-  int e;
-  const double m = frexp(k, &e);                       // [0.5, 1)
-  double hi = ldexp(floor(m * 65536.0), e - 16);
-  if (hi == k) hi = ldexp(floor(m * 65536.0) - 1.0, e - 16);
-  return {(float)hi, (float)(k - hi)};
-}
-
 bool bad_logits(const char* who, const void* logits, int dtype, long long ld, const void* targets, long long rows, int vocab, double scale) {
   if (!logits || !targets || rows <= 0 || rows > INT_MAX || vocab <= 0 || ld < vocab || !(scale > 1e-30) || !(scale < 1e30) ||
       (dtype != BB_DTYPE_BF16 && dtype != BB_DTYPE_F32) || ((uintptr_t)logits & (dtype == BB_DTYPE_F32 ? 3 : 1))) {

@@ -80,6 +80,15 @@ class PolicyDesc(ctypes.Structure):
     ]
 
 
+class HeadDesc(ctypes.Structure):
+    """bb_head_desc: a vocabulary projection whose logits are not stored (see include/bamboo_b200.h)."""
+    _fields_ = [
+        ("rows", ctypes.c_int), ("vocab", ctypes.c_int), ("hidden", ctypes.c_int),
+        ("ld_hidden", ctypes.c_longlong), ("ld_weight", ctypes.c_longlong),
+        ("scale", ctypes.c_double), ("ignore_index", ctypes.c_longlong),
+    ]
+
+
 PREFERENCE_FORMS = {"sigmoid": 0, "hinge": 1, "squared": 2}
 POLICY_REDUCTIONS = {"token": 0, "sequence": 1}
 
@@ -131,6 +140,9 @@ def load():
         lib.bb_policy_workspace_bytes.restype = ll
         lib.bb_policy_loss.argtypes = [vp] * 11 + [ll, vp]
         lib.bb_policy_loss_logits.argtypes = [vp, vp, i, ll, d, i, i] + [vp] * 9 + [ll, f, vp, ll, vp]
+        lib.bb_head_logprob_workspace_bytes.restype = ll
+        lib.bb_head_logprob_fwd.argtypes = [vp] * 7 + [ll, vp]
+        lib.bb_head_logprob_grad.argtypes = [vp] * 7 + [f, i, i, vp, ll, vp]
         lib.bb_rescale_grad.argtypes = [vp, i, ll, ll, i, vp, f, vp]
         lib.bb_grad_sumsq.argtypes = [vp, i, vp, vp]
         lib.bb_grad_clip.argtypes = [vp, i, vp, i, d, vp, vp]
@@ -596,6 +608,27 @@ def token_logprob_bwd(logits, targets, stats, row_grad, dlogits, vocab, scale=1.
     check(load().bb_token_logprob_bwd(logits.data_ptr(), _dtype(logits, "logits"), logits.stride(0), targets.data_ptr(), scale, stats.data_ptr(),
                                       row_grad.data_ptr(), _addr(grad_scale_dev), grad_scale, dlogits.data_ptr(), dlogits.stride(0), rows, vocab,
                                       cols, ignore_index, _raw_stream()), "bb_token_logprob_bwd")
+    return dlogits
+
+
+def head_logprob_fwd(desc, hidden, weight, targets, logp, stats):
+    """hidden [rows, n], weight [>= vocab, n] bf16; targets [rows] int64; logp [rows], stats [rows, 2] fp32."""
+    global LAUNCHES
+    LAUNCHES += 2
+    lib = load()
+    ws = workspace(max(0, lib.bb_head_logprob_workspace_bytes(ctypes.byref(desc))), "post_training")
+    check(lib.bb_head_logprob_fwd(ctypes.byref(desc), hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), logp.data_ptr(), stats.data_ptr(),
+                                  ws.data_ptr(), ws.numel(), _raw_stream()), "bb_head_logprob_fwd")
+    return logp
+
+
+def head_logprob_grad(desc, hidden, weight, targets, stats, row_grad, col0, cols, dlogits, grad_scale=1.0, grad_scale_dev=None):
+    """Gradient of the logits of vocabulary entries [col0, col0 + cols) into dlogits [rows, >= cols] bf16."""
+    global LAUNCHES
+    LAUNCHES += 1
+    check(load().bb_head_logprob_grad(ctypes.byref(desc), hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), stats.data_ptr(),
+                                      row_grad.data_ptr(), _addr(grad_scale_dev), grad_scale, col0, cols, dlogits.data_ptr(), dlogits.stride(0),
+                                      _raw_stream()), "bb_head_logprob_grad")
     return dlogits
 
 

@@ -1,6 +1,7 @@
 """Post-training of the vocabulary models: what follows token cross entropy when a model learns from preferences or rewards.
 
     token_logprobs      log-probabilities of given tokens, from logits
+    head_logprobs       the same from hidden states and the vocabulary projection, whose logits are never stored
     preference_loss     paired preference loss over token log-probabilities (reference against policy)
     policy_loss         clipped policy loss with a KL term over token log-probabilities
     PreferenceLoss,     the two from logits, as ``loss_fn`` of a ``PipelineModule`` (labels are a tuple of tensors) or in one
@@ -110,6 +111,97 @@ def token_logprobs(logits, targets, vocab=None, *, temperature=1.0, ignore_index
         return _TokenLogprobsFn.apply(logits, targets, vocab, scale, ignore_index, inplace)
     lg, vocab = _rows(logits, vocab)
     return _logprobs(lg, _flat(targets, "targets", lg.shape[0], torch.int64, lg.device), vocab, scale, ignore_index)[0].view(targets.shape)
+
+
+# ----------------------------------------------------------------------------------- through the vocabulary projection
+# Bytes of logit gradient that exist at a time in the backward pass of head_logprobs
+HEAD_GRAD_BYTES = 256 << 20
+
+
+def _head_operands(hidden, weight, targets, vocab, scale, ignore_index):
+    for name, t in (("hidden", hidden), ("weight", weight)):
+        if not t.is_cuda:
+            raise L.BambooNativeError(f"{name}: expected a CUDA tensor; the sm_100a kernels have no CPU fallback")
+        if t.dtype != torch.bfloat16:
+            raise L.BambooNativeError(f"{name}: bf16 expected, got {t.dtype}")
+    n = hidden.shape[-1]
+    if weight.dim() != 2 or weight.shape[1] != n or weight.device != hidden.device:
+        raise ValueError(f"weight {tuple(weight.shape)} on {weight.device} for hidden states of {n} on {hidden.device}")
+    vocab = weight.shape[0] if vocab is None else vocab
+    if not 0 < vocab <= weight.shape[0]:
+        raise ValueError(f"vocab {vocab} does not fit a weight of {weight.shape[0]} rows")
+    if n % 8:
+        raise ValueError(f"hidden size {n}: a multiple of 8 is needed (16-byte rows)")
+
+    def rows_of(t):
+        ok = t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= n and t.data_ptr() % 16 == 0
+        return t if ok else t.clone(memory_format=torch.contiguous_format)
+    h2, w = rows_of(hidden.detach().reshape(-1, n)), rows_of(weight.detach())
+    tg = _flat(targets, "targets", h2.shape[0], torch.int64, h2.device)
+    desc = L.HeadDesc(rows=h2.shape[0], vocab=vocab, hidden=n, ld_hidden=h2.stride(0), ld_weight=w.stride(0), scale=scale, ignore_index=ignore_index)
+    return desc, h2, w, tg
+
+
+def _head_forward(desc, h2, w, tg):
+    logp = torch.empty(desc.rows, dtype=torch.float32, device=h2.device)
+    stats = torch.empty(desc.rows, 2, dtype=torch.float32, device=h2.device)
+    if desc.rows:
+        L.head_logprob_fwd(desc, h2, w, tg, logp, stats)
+    return logp, stats
+
+
+class _HeadLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, vocab, scale, ignore_index):
+        desc, h2, w, tg = _head_operands(hidden, weight, targets, vocab, scale, ignore_index)
+        logp, stats = _head_forward(desc, h2, w, tg)
+        ctx.desc, ctx.weight, ctx.shape = desc, weight, hidden.shape
+        ctx.save_for_backward(h2, w, tg, stats)
+        return logp.view(targets.shape)
+
+    @staticmethod
+    def backward(ctx, grad):
+        h2, w, tg, stats = ctx.saved_tensors
+        desc, weight, dev = ctx.desc, ctx.weight, h2.device
+        rows, n, vocab = desc.rows, desc.hidden, desc.vocab
+        need_h, need_w = ctx.needs_input_grad[:2]
+        main = getattr(weight, "main_grad", None)
+        dh = torch.empty(rows, n, dtype=torch.bfloat16, device=dev) if need_h else None
+        dw = torch.empty(weight.shape, dtype=torch.bfloat16, device=dev) if need_w and main is None else None
+        if dw is not None:
+            dw[vocab if rows else 0:].zero_()
+        if not rows:
+            return (None if dh is None else dh.view(ctx.shape)), dw, None, None, None, None
+        row_grad = _flat(grad, "gradient", rows, torch.float32, dev)
+        # vocabulary entries in pieces, so that the gradient of the logits never exists whole; a multiple of 256, the widest tile
+        piece = min(vocab, max(2048, HEAD_GRAD_BYTES // (2 * rows) // 256 * 256))
+        whole = piece >= vocab
+        acc = torch.zeros(rows, n, dtype=torch.float32, device=dev) if need_h and not whole else None
+        buffer = torch.empty(rows, (piece + 7) // 8 * 8, dtype=torch.bfloat16, device=dev)
+        for col0 in range(0, vocab, piece):
+            cols = min(piece, vocab - col0)
+            d = L.head_logprob_grad(desc, h2, w, tg, stats, row_grad, col0, cols, buffer)
+            if need_h:
+                L.gemm(d, w[col0:], dh if whole else acc, b_mn=True, epilogue=L.EPI_STORE if whole else L.EPI_ACCUM_F32, M=rows, N=n, K=cols)
+            if dw is not None:
+                L.gemm(d, h2, dw[col0:], a_mn=True, b_mn=True, M=cols, N=n, K=rows)
+            elif need_w:
+                L.gemm(d, h2, main[col0:], a_mn=True, b_mn=True, epilogue=L.EPI_ACCUM_F32, M=cols, N=n, K=rows)
+        if acc is not None:
+            L.cast_f32_to_bf16(acc, dh)
+        return (None if dh is None else dh.view(ctx.shape)), dw, None, None, None, None
+
+
+def head_logprobs(hidden, weight, targets, vocab=None, *, temperature=1.0, ignore_index=-100):
+    """``token_logprobs(hidden @ weight.T, targets, vocab)`` without storing the logits: bf16 ``hidden`` [..., n] and ``weight`` [>= vocab, n],
+    n a multiple of 8, fp32 logits inside.
+
+    The backward pass computes the logits again, in pieces of the vocabulary.  The weight's gradient is added to ``weight.main_grad`` where
+    the weight belongs to an arena, like the layers' gradients, and returned to autograd (bf16) otherwise."""
+    scale = _inverse(temperature)
+    if _wants_grad(hidden) or _wants_grad(weight):
+        return _HeadLogprobsFn.apply(hidden, weight, targets, vocab, scale, ignore_index)
+    return _head_forward(*_head_operands(hidden, weight, targets, vocab, scale, ignore_index))[0].view(targets.shape)
 
 
 # ----------------------------------------------------------------------------------- losses over log-probabilities

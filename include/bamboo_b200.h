@@ -318,6 +318,24 @@ int bb_token_logprob_bwd(const void* logits, int dtype, long long ld, const long
                          const float* row_grad, const float* grad_scale_dev, float grad_scale, void* dlogits, long long ldd,
                          long long rows, int vocab, int cols, long long ignore_index, void* stream);
 
+/* The same from hidden states, through the vocabulary projection, without storing the logits: logits = hidden_states [rows,
+ * hidden] * weight [vocab, hidden]^T (bf16, rows 16-byte aligned; fp32 accumulation, the logits are not rounded).  _fwd: one
+ * GEMM whose epilogue keeps softmax sums, and a small kernel that joins them.  _grad: the gradient of the logits for vocabulary entries
+ * [col0, col0 + cols) (bf16 [rows, cols], row stride ldd), from a second GEMM over the same operands; the input and weight
+ * gradients are bb_gemm_bf16 products of it.  A logit so large that scale * log2(e) * logit overflows counts as infinite here. */
+typedef struct bb_head_desc {
+  int rows, vocab, hidden;
+  long long ld_hidden, ld_weight;
+  double scale;
+  long long ignore_index;
+} bb_head_desc;
+long long bb_head_logprob_workspace_bytes(const bb_head_desc* d);
+int bb_head_logprob_fwd(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets, float* logp,
+                        float* stats, void* workspace, long long workspace_bytes, void* stream);
+int bb_head_logprob_grad(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets,
+                         const float* stats, const float* row_grad, const float* grad_scale_dev, float grad_scale, int col0,
+                         int cols, void* dlogits, long long ldd, void* stream);
+
 /* Paired preference loss over token log-probabilities.  Sequences 2i (preferred) and 2i + 1 (rejected) form pair i; sequence q is
  * tokens [q n, (q + 1) n) with n = tokens / sequences, or [offsets[q], offsets[q + 1]).  s_q = sum (average: mean) over counted
  * tokens of logp - ref (ref may be NULL: 0), h = beta (s_2i - s_2i+1), and the loss is the mean over pairs of

@@ -187,6 +187,115 @@ def test_targets_outside_the_vocabulary_are_reported(pt):
     assert got[1] == 0 and got[2] == 0 and got[0] != 0
 
 
+# ----------------------------------------------------------------------------------- through the vocabulary projection
+def ref_head(h, w, t, vocab, temperature, g=None):
+    """64-bit log-probabilities and, for an incoming gradient, the gradients of hidden states and weight."""
+    h, w = h.double(), w.double()
+    lp, probs, counted = ref_logps(h @ w[:vocab].t(), t, vocab, temperature)
+    if g is None:
+        return lp
+    d = ref_dlogits(probs, counted, t, g, w.shape[0], temperature)
+    return lp, d @ w, d.t() @ h
+
+
+# Logits are fp32 sums of up to 4096 bf16 products of size 1 / hidden: 1e-5 at most; log-probabilities 1e-6 of their magnitude on top.
+# The logit gradient is rounded to bf16 (2^-8 of each), the results too; sums of such errors stay below 2^-7 of the sums of magnitudes.
+HEAD_SHAPES = [(1, 64, 300, 300), (1, 1024, 50257, 50304), (3, 8, 1, 1), (128, 256, 1000, 1024), (129, 264, 257, 257), (300, 520, 2049, 2056),
+               (1000, 128, 30522, 30592), (2500, 64, 5000, 5000), (7, 4096, 777, 777), (40, 72, 128, 128), (700, 1024, 12345, 12345)]
+
+
+@pytest.mark.parametrize("rows,hidden,vocab,cols", HEAD_SHAPES)
+def test_head_logprobs_and_gradients(pt, rows, hidden, vocab, cols):
+    h = torch.randn(rows, hidden, device="cuda", generator=gen(101)).bfloat16()
+    w = (torch.randn(cols, hidden, device="cuda", generator=gen(102)) * 2 / math.sqrt(hidden)).bfloat16()
+    t = targets_of(rows, vocab, 103)
+    g = torch.randn(rows, device="cuda", generator=gen(104))
+    lp, dh, dw = ref_head(h, w, t, vocab, 0.8, g)
+    near(pt.head_logprobs(h, w, t, vocab, temperature=0.8), lp, 1e-6, 2e-5)
+    hl, wl = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    pt.head_logprobs(hl, wl, t, vocab, temperature=0.8).backward(g)
+    d = (ref_dlogits(*ref_logps(h.double() @ w[:vocab].double().t(), t, vocab, 0.8)[1:], t, g, cols, 0.8)).abs()
+    for got, want, size in ((hl.grad, dh, d @ w.double().abs()), (wl.grad, dw, d.t() @ h.double().abs())):
+        assert ((got.double() - want).abs() <= 2 ** -8 * want.abs() + 2 ** -7 * size + 1e-6).all()
+    assert torch.all(wl.grad[vocab:] == 0) and torch.all(hl.grad[t == IGNORE] == 0)
+
+
+def test_head_backward_in_pieces_and_into_an_arena(pt, monkeypatch):
+    """Pieces of the vocabulary give the gradients of the whole, and a weight with ``main_grad`` is added to there."""
+    rows, hidden, vocab, cols = 300, 128, 5003, 5120
+    h = torch.randn(rows, hidden, device="cuda", generator=gen(105)).bfloat16()
+    w = (torch.randn(cols, hidden, device="cuda", generator=gen(106)) * 0.2).bfloat16()
+    t, g = targets_of(rows, vocab, 107), torch.randn(rows, device="cuda", generator=gen(108))
+    whole = torch.autograd.grad(pt.head_logprobs(hl := h.clone().requires_grad_(True), wl := w.clone().requires_grad_(True), t, vocab), (hl, wl), g)
+    monkeypatch.setattr(pt, "HEAD_GRAD_BYTES", 1)                   # the least: 2048 entries at a time
+    pieces = torch.autograd.grad(pt.head_logprobs(hl, wl, t, vocab), (hl, wl), g)
+    assert torch.equal(whole[1], pieces[1])
+    near(pieces[0], whole[0].double(), 2 ** -7, 2 ** -8 * whole[0].abs().max().item())
+    p = torch.nn.Parameter(w.clone())
+    p.main_grad = torch.ones(cols, hidden, device="cuda")
+    pt.head_logprobs(h, p, t, vocab).backward(g)
+    assert p.grad is None
+    near((p.main_grad - 1).bfloat16(), whole[1].double(), 2 ** -7, 1e-6)
+
+
+def test_head_operands_of_other_layouts(pt):
+    h = torch.randn(4, 9, 96, device="cuda", generator=gen(109)).bfloat16()
+    w = (torch.randn(400, 104, device="cuda", generator=gen(110)) * 0.2).bfloat16()
+    t = targets_of(36, 333, 111).view(4, 9)
+    for wv in (w[:, :96], w[:, 1:97], w[3:, 8:], w.t()[:96].t()):
+        for hv in (h, h.transpose(0, 1).contiguous().transpose(0, 1), h[:, 1:]):
+            tv = t[:, :hv.shape[1]]
+            want = ref_head(hv.reshape(-1, 96), wv, tv.reshape(-1), 333, 1.0)
+            near(pt.head_logprobs(hv, wv, tv, 333).reshape(-1), want, 1e-6, 2e-5)
+    assert pt.head_logprobs(h[:0], w[:, :96], t[:0]).shape == (0, 9)
+
+
+def test_head_gradient_against_differences(pt):
+    rows, hidden, vocab = 6, 32, 211
+    h = torch.randn(rows, hidden, device="cuda", generator=gen(112)).bfloat16()
+    w = (torch.randn(vocab, hidden, device="cuda", generator=gen(113)) * 0.3).bfloat16()
+    t, g = targets_of(rows, vocab, 114, 0.0), torch.randn(rows, device="cuda", generator=gen(115)).double()
+    hl, wl = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    pt.head_logprobs(hl, wl, t).backward(g.float())
+    f = lambda a, b: (g * torch.log_softmax(a @ b.t(), 1).gather(1, t[:, None])[:, 0]).sum()  # noqa: E731
+    for seed in range(3):
+        v = torch.randn(rows, hidden, device="cuda", generator=gen(116 + seed)).double()
+        u = torch.randn(vocab, hidden, device="cuda", generator=gen(126 + seed)).double()
+        e = 1e-5
+        slope_h = (f(h.double() + e * v, w.double()) - f(h.double() - e * v, w.double())) / (2 * e)
+        slope_w = (f(h.double(), w.double() + e * u) - f(h.double(), w.double() - e * u)) / (2 * e)
+        # bf16 roundings, independent of the direction
+        assert abs((hl.grad.double() * v).sum() - slope_h) <= 2 ** -7 * hl.grad.double().norm() * v.norm()
+        assert abs((wl.grad.double() * u).sum() - slope_w) <= 2 ** -7 * wl.grad.double().norm() * u.norm()
+
+
+def test_head_rows_that_do_not_count_and_refusals(pt):
+    from bamboo_b200 import lib
+    h = torch.randn(5, 64, device="cuda", generator=gen(119)).bfloat16()
+    w = (torch.randn(100, 64, device="cuda", generator=gen(120)) * 0.2).bfloat16()
+    t = torch.tensor([3, IGNORE, 99, IGNORE, 0], device="cuda")
+    want = ref_head(h, w, t, 100, 1.0)
+    h[1], h[3] = math.nan, math.inf
+    hl = h.clone().requires_grad_(True)
+    out = pt.head_logprobs(hl, w, t)
+    near(out.detach(), want, 1e-6, 2e-5)
+    out.sum().backward()
+    assert torch.isfinite(hl.grad).all() and torch.all(hl.grad[[1, 3]] == 0)
+    out = pt.head_logprobs(h, w, torch.tensor([3, 100, -7, IGNORE, 0], device="cuda"))
+    torch.cuda.synchronize()
+    assert lib.read_status() < 0 and torch.all(out[1:4] == 0)
+    with pytest.raises(ValueError):
+        pt.head_logprobs(h, w, t, 101)
+    with pytest.raises(ValueError):
+        pt.head_logprobs(h[:, :60], w[:, :60], t)
+    with pytest.raises(ValueError):
+        pt.head_logprobs(h, w[:, :56], t)
+    with pytest.raises(lib.BambooNativeError):
+        pt.head_logprobs(h.float(), w, t)
+    with pytest.raises(lib.BambooNativeError):
+        pt.head_logprobs(h, w.cpu(), t)
+
+
 # ----------------------------------------------------------------------------------- preference loss
 def spans_of(lengths):
     ends = torch.tensor(lengths).cumsum(0).tolist()
