@@ -98,19 +98,38 @@ class ParamArena:
         """What a shadow copy of this stage needs: weights and both Adam moments."""
         return [self.master, self.exp_avg, self.exp_avg_sq]
 
-    def adam_step(self, *, lr, beta1, beta2, eps, weight_decay, adam_w_mode, bias_correction, grad_scale=1.0):
+    def grad_sumsq(self):
+        """Sum of squares of the gradient accumulator (fp64 [1], on its device)."""
+        if self.master.is_cuda:
+            from . import post_training
+            return post_training.grad_sumsq([self.grad])
+        return self.grad.double().square().sum().reshape(1)
+
+    def adam_step(self, *, lr, beta1, beta2, eps, weight_decay, adam_w_mode, bias_correction, grad_scale=1.0, max_norm=0.0, sumsq=None):
         """One Adam step; clears the gradient.  CUDA arenas use the fused kernel; CPU arenas
         (plumbing runs) evaluate the same formula (csrc/adam/multi_tensor_adam.cu:72-108 of
-        the reference) with tensor ops."""
+        the reference) with tensor ops.  ``max_norm`` > 0: on the gradient clipped to that norm, which is over ``sumsq`` (sum of squares
+        of unscaled gradients) where it covers more than this arena; returns the norm before clipping."""
         self.step_count += 1
         step = self.step_count
         if self.master.is_cuda:
             from . import lib as L
+            if max_norm > 0:
+                from . import post_training
+                return post_training.adam_step_clipped(
+                    self.master, self.grad, self.exp_avg, self.exp_avg_sq, None if self.lp is self.master else self.lp, max_norm=max_norm,
+                    grad_scale=grad_scale, sumsq=sumsq, lr=lr, beta1=beta1, beta2=beta2, eps=eps, step=step, adam_w_mode=adam_w_mode,
+                    bias_correction=bias_correction, weight_decay=weight_decay)
             L.adam_step(self.master, self.grad, self.exp_avg, self.exp_avg_sq,
                         None if self.lp is self.master else self.lp, lr=lr, beta1=beta1, beta2=beta2, eps=eps,
                         step=step, adam_w_mode=adam_w_mode, bias_correction=bias_correction,
                         weight_decay=weight_decay, grad_scale=grad_scale, zero_grad=True)
             return
+        norm = None
+        if max_norm > 0:
+            norm = grad_scale * (self.grad_sumsq() if sumsq is None else sumsq).sqrt()
+            grad_scale = grad_scale * min(1.0, max_norm / (float(norm) + 1e-6))
+            norm = norm.float().reshape(())
         g = self.grad * grad_scale if grad_scale != 1.0 else self.grad
         bc1 = 1.0 - beta1 ** step if bias_correction else 1.0
         bc2 = 1.0 - beta2 ** step if bias_correction else 1.0
@@ -124,3 +143,4 @@ class ParamArena:
         self.master.add_(update, alpha=-lr)
         self.grad.zero_()
         self.refresh_lp()
+        return norm

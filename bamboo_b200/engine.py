@@ -271,6 +271,10 @@ class PipelineEngine:
         self.total_loss = None
         self.agg_train_loss = None
         self.loss_model = self.module.loss_fn
+        if hasattr(self.loss_model, "grad_scale"):
+            # a loss that makes its gradient with its value: every micro-batch contributes loss / GAS
+            self.loss_model.grad_scale = 1.0 / self.micro_batches
+        self._global_grad_norm, self._clip_epoch = None, 0
         self._compute_loss = True
         self._losses: Dict[Tuple[int, int], torch.Tensor] = {}
         self.timers = collections.defaultdict(float)
@@ -908,6 +912,7 @@ class PipelineEngine:
         (``deepspeed/runtime/engine.py:1925-1990``); the stage partition may differ from the
         one that wrote the checkpoint."""
         from . import checkpoint
+        self._clip_epoch += 1           # (step numbers come again)
         return checkpoint.load_checkpoint(self, load_dir, tag, load_optimizer_states, load_lr_scheduler_states)
 
     def eval_batch(self, *a, **k):
@@ -949,7 +954,7 @@ class PipelineEngine:
             if torch.is_tensor(y):
                 y = y.to(self.device, non_blocking=True)
             elif isinstance(y, (tuple, list)):
-                y = tuple(t.to(self.device, non_blocking=True).detach() for t in y)
+                y = tuple(None if t is None else t.to(self.device, non_blocking=True).detach() for t in y)
             self.pipe_buffers["label"][buffer_id] = y
 
     def _is_shadow(self, stage_id):
@@ -976,8 +981,9 @@ class PipelineEngine:
                 if torch.is_tensor(t) and t.is_cuda:
                     t.record_stream(self.rc_stream)
             label = self.pipe_buffers["label"][buffer_id] if stage_id == self.num_stages - 1 else None
-            if torch.is_tensor(label) and label.is_cuda:
-                label.record_stream(self.rc_stream)
+            for t in (label if isinstance(label, tuple) else (label,)):
+                if torch.is_tensor(t) and t.is_cuda:
+                    t.record_stream(self.rc_stream)
             if self._config.rc_deferred and hasattr(self.transport, "idle_hook"):
                 # issued layer by layer whenever the host finds the main stream idle (waiting for a
                 # neighbour's message), the rest at the end of the batch: see _rc_pump
@@ -1200,16 +1206,54 @@ class PipelineEngine:
         scales = getattr(self, "_reduce_scale", {})
         if getattr(self, "capture_grads", False):
             self.last_grads = {sid: self.arenas[sid].grad.clone() * scales.get(sid, 1.0) for sid in self.stage_ids}
+        limit = self._config.gradient_clipping
+        total = self._pipeline_sumsq(scales) if limit > 0 and self.num_stages > 1 else None
         for sid in self.stage_ids:
-            a = self._adam
-            self.arenas[sid].adam_step(lr=a["lr"], beta1=a["beta1"], beta2=a["beta2"], eps=a["eps"],
-                                       weight_decay=a["weight_decay"], adam_w_mode=a["adam_w_mode"],
-                                       bias_correction=a["bias_correction"], grad_scale=scales.get(sid, 1.0))
+            a, scale = self._adam, scales.get(sid, 1.0)
+            clip = dict(max_norm=limit, sumsq=None if total is None else total / scale ** 2) if limit > 0 else {}
+            norm = self.arenas[sid].adam_step(lr=a["lr"], beta1=a["beta1"], beta2=a["beta2"], eps=a["eps"],
+                                              weight_decay=a["weight_decay"], adam_w_mode=a["adam_w_mode"],
+                                              bias_correction=a["bias_correction"], grad_scale=scale, **clip)
+            if limit > 0:
+                self._global_grad_norm = norm
         if self.lr_scheduler is not None:
             self.lr_scheduler.step(**(lr_kwargs or {}))
         self.global_steps += 1
         self.global_samples += self.train_batch_size()
         self._sync_shadow_state()
+
+    def _pipeline_sumsq(self, scales):
+        """Sum of squares of the (averaged) gradients of all stages of this pipeline, fp64 [1] on the device, for
+        ``gradient_clipping``.  The stages exchange one number each through the job's store, named by stage and not by rank:
+        who owns a stage may change between steps, and a collective over the pipeline would wait for a member that left.  Costs a
+        pipeline of several ranks a read of the device and a round through the store per step; a rank that owns every stage
+        adds up on the device."""
+        parts = {sid: self.arenas[sid].grad_sumsq() * scales.get(sid, 1.0) ** 2 for sid in self.stage_ids}
+        if len(parts) == self.num_stages:
+            return sum(parts[sid] for sid in range(self.num_stages))
+        step = f"{self._clip_epoch}-{self.global_steps}"
+        # two keys per stage in turn: nobody is two steps ahead of a neighbour whose messages it needs
+        key = f"grad-sumsq-{self.grid.get_data_parallel_id()}-{{}}-{self.global_steps & 1}"
+        values = {sid: float(v) for sid, v in parts.items()}
+        for sid, v in values.items():
+            self.global_store.set(key.format(sid), f"{step}:{v!r}")
+        deadline = time.time() + self._config.p2p_timeout_s
+        for sid in range(self.num_stages):
+            while sid not in values:
+                if self.global_store.check([key.format(sid)]):
+                    at, _, v = _decode(self.global_store.get(key.format(sid))).partition(":")
+                    if at == step:
+                        values[sid] = float(v)
+                        break
+                if time.time() > deadline:
+                    raise PipelineError(f"gradient norm of stage {sid} did not arrive within {self._config.p2p_timeout_s} s")
+                time.sleep(0.0002)
+        # added in stage order, the same on every rank
+        return torch.tensor([sum(values[sid] for sid in range(self.num_stages))], dtype=torch.float64).to(self.device)
+
+    def get_global_grad_norm(self):
+        """Norm of the last step's gradients before clipping (``gradient_clipping``), or None; reads the device."""
+        return None if self._global_grad_norm is None else float(self._global_grad_norm)
 
     def _sync_shadow_state(self):
         """End of step: every live stage ships (weights, exp_avg, exp_avg_sq) to the rank that

@@ -456,15 +456,20 @@ def _partials(grads):
     return L.workspace(8 * n, "grad_norm"), n
 
 
+def grad_sumsq(tensors):
+    """Sum of squares over all gradients together (fp64 [1] on their device)."""
+    grads = [g if _dense(g) else g.contiguous() for g in _gradients(tensors)]
+    partials, n = _partials(grads)
+    L.grad_sumsq(L.grad_tensors(grads), len(grads), partials)
+    return partials[:8 * n].view(torch.float64).sum().reshape(1)
+
+
 def global_grad_norm(tensors):
     """2-norm over all gradients together (fp32 scalar on their device); nothing is changed."""
     grads = _gradients(tensors)
     if not grads:
         return torch.zeros(())
-    grads = [g if _dense(g) else g.contiguous() for g in grads]
-    partials, n = _partials(grads)
-    L.grad_sumsq(L.grad_tensors(grads), len(grads), partials)
-    return partials[:8 * n].view(torch.float64).sum().sqrt().float()
+    return grad_sumsq(grads).sqrt().float().reshape(())
 
 
 def clip_grad_norm_(tensors, max_norm):
