@@ -8,7 +8,10 @@
 
 namespace {
 
-constexpr int ROW_THREADS = 256;
+constexpr int ROW_THREADS = 256, ROW_LOADS = 4;      // threads per row, 16-byte loads that each has in flight
+
+// dynamic shared memory next to a kernel's few static bytes: of one CTA per SM, and of each of two
+constexpr size_t MAX_CACHE = 226 * 1024, PAIR_CACHE = 112 * 1024;
 
 template <typename T> struct Elem;
 template <> struct Elem<__nv_bfloat16> {
@@ -22,6 +25,7 @@ template <> struct Elem<__nv_bfloat16> {
     return make_uint4(bb::pack_bf16x2(f[0], f[1]), bb::pack_bf16x2(f[2], f[3]), bb::pack_bf16x2(f[4], f[5]), bb::pack_bf16x2(f[6], f[7]));
   }
   static __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+  static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u); }   // -inf
 };
 template <> struct Elem<float> {
   static constexpr int VEC = 4;
@@ -33,6 +37,7 @@ template <> struct Elem<float> {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
   }
   static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+  static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u); }
 };
 
 using bb::expo;
@@ -64,16 +69,51 @@ template <int THREADS> __device__ __forceinline__ void soft_block(float& r, floa
   for (int w = 0; w < THREADS / 32; ++w) soft_merge(r, s, smem[w].x, smem[w].y);
 }
 
-template <typename T, int THREADS> __device__ __forceinline__ void soft_row(const T* x, int n, K2 k, float& r, float& s) {
+// This thread's share of a row, chunk by chunk with the reference kept below the largest logit (the exact form)
+template <typename T, int THREADS> __device__ __noinline__ float2 soft_share_exact(const uint4* v, int nvec, K2 k) {
   constexpr int VEC = Elem<T>::VEC;
-  const Span<T> sp(x, n);
-  r = -INFINITY; s = 0.f;
-  const uint4* v = reinterpret_cast<const uint4*>(x + sp.lead);
-  for (int c = threadIdx.x; c < sp.nvec; c += THREADS) {
+  float r = -INFINITY, s = 0.f;
+  for (int c = threadIdx.x; c < nvec; c += THREADS) {
     float f[VEC];
     Elem<T>::unpack(v[c], f);
     soft_add<VEC>(r, s, f, k);
   }
+  return make_float2(r, s);
+}
+
+// (r, s) of this thread's share of a row.  The reference comes from the thread's first chunk and stays: a later logit may be larger,
+// 2^(k x - r) is a float all the same as long as it is below 2^127, so the loop needs no maximum (5 instead of 7 issue slots a
+// logit, at 4.5 of them a clock and SM at the full memory rate); a sum that did overflow is taken again in the exact form.  U loads
+// are in flight per thread.  `cache`: the chunks are left there too (shared memory, one place each).
+template <typename T, int THREADS, int U, bool CACHE>
+__device__ __forceinline__ void soft_row(const T* x, int n, K2 k, float& r, float& s, uint4* cache) {
+  constexpr int VEC = Elem<T>::VEC;
+  const Span<T> sp(x, n);
+  r = -INFINITY; s = 0.f;
+  const uint4* v = reinterpret_cast<const uint4*>(x + sp.lead);
+  float2 sum = make_float2(0.f, 0.f);
+  for (int c = threadIdx.x; c < sp.nvec; c += U * THREADS) {
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) q[u] = c + u * THREADS < sp.nvec ? v[c + u * THREADS] : Elem<T>::nothing();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (CACHE && c + u * THREADS < sp.nvec) cache[c + u * THREADS] = q[u];
+      float f[VEC];
+      Elem<T>::unpack(q[u], f);
+      if (r == -INFINITY) {
+        soft_add<VEC>(r, s, f, k);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) {
+          const float2 t = expo2(make_float2(f[i], f[i + 1]), k, r);
+          sum = bb::add2(sum, make_float2(ex2(t.x), ex2(t.y)));
+        }
+      }
+    }
+  }
+  s += sum.x + sum.y;
+  if (!(s < INFINITY)) { const float2 e = soft_share_exact<T, THREADS>(v, sp.nvec, k); r = e.x; s = e.y; }
   for (int j = threadIdx.x; j < sp.lead + n - sp.tail; j += THREADS) {
     const float f = Elem<T>::get(x + (j < sp.lead ? j : sp.tail + j - sp.lead));
     soft_add<1>(r, s, &f, k);
@@ -109,15 +149,17 @@ template <typename T, int THREADS> __device__ __noinline__ void soft_row_extreme
   if (bad) r = s = NAN;
 }
 
-template <typename T, int THREADS> __device__ __forceinline__ void soft_whole_row(const T* x, int n, K2 k, float& r, float& s, float2* smem) {
-  soft_row<T, THREADS>(x, n, k, r, s);
+template <typename T, int THREADS, int U, bool CACHE>
+__device__ __forceinline__ void soft_whole_row(const T* x, int n, K2 k, float& r, float& s, float2* smem, uint4* cache) {
+  soft_row<T, THREADS, U, CACHE>(x, n, k, r, s, cache);
   soft_block<THREADS>(r, s, smem);
   if (isinf(r)) soft_row_extreme<T, THREADS>(x, n, r, s, smem);
 }
 
-// d[j] = g * ([j == t] - softmax_j) for j < V, 0 in [V, cols); zeros throughout when g == 0 (nothing is read then)
-template <typename T, int THREADS>
-__device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int t, float g, K2 k, float r, float s) {
+// d[j] = g * ([j == t] - softmax_j) for j < V, 0 in [V, cols); zeros throughout when g == 0 (nothing is read then).  `cache`: the
+// chunks of the row as soft_row left them.
+template <typename T, int THREADS, int U, bool CACHE>
+__device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int t, float g, K2 k, float r, float s, const uint4* cache) {
   constexpr int VEC = Elem<T>::VEC;
   if (s == 0.f) g = 0.f;
   const float ng = g == 0.f ? 0.f : -g / s;
@@ -136,21 +178,60 @@ __device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int 
     for (int j = threadIdx.x; j < cols; j += THREADS) one(j);
     return;
   }
-  const uint4* xv = reinterpret_cast<const uint4*>(x + sp.lead);
+  const uint4* xv = CACHE ? cache : reinterpret_cast<const uint4*>(x + sp.lead);
   uint4* dv = reinterpret_cast<uint4*>(d + sp.lead);
-  for (int c = threadIdx.x; c < sp.nvec; c += THREADS) {
-    const int j0 = sp.lead + c * VEC;
-    if (g == 0.f || j0 >= V) { dv[c] = make_uint4(0, 0, 0, 0); continue; }
-    float f[VEC];
-    Elem<T>::unpack(xv[c], f);
+  // chunks of vocabulary entries only, then the one that the padding begins in and the padding
+  const int whole = g == 0.f || V < sp.lead ? 0 : (V - sp.lead) / VEC;
+  for (int c = threadIdx.x; c < whole; c += U * THREADS) {
+    uint4 q[U];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      f[i] = j0 + i < V ? ng * ex2(expo(f[i], k, r)) : 0.f;
-      if (j0 + i == t) f[i] += g;
+    for (int u = 0; u < U; ++u) q[u] = c + u * THREADS < whole ? xv[c + u * THREADS] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[VEC];
+      Elem<T>::unpack(q[u], f);
+#pragma unroll
+      for (int i = 0; i < VEC; i += 2) {
+        const float2 e = expo2(make_float2(f[i], f[i + 1]), k, r);
+        const float2 m = bb::mul2(make_float2(ex2(e.x), ex2(e.y)), make_float2(ng, ng));
+        f[i] = m.x; f[i + 1] = m.y;
+      }
+      const int at = t - (sp.lead + (c + u * THREADS) * VEC);
+      if (at >= 0 && at < VEC) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) if (i == at) f[i] += g;
+      }
+      if (c + u * THREADS < whole) dv[c + u * THREADS] = Elem<T>::pack(f);
     }
-    dv[c] = Elem<T>::pack(f);
+  }
+  for (int c = whole + threadIdx.x; c < sp.nvec; c += THREADS) {
+    const int j0 = sp.lead + c * VEC;
+    if (g == 0.f || j0 >= V) dv[c] = make_uint4(0, 0, 0, 0);
+    else for (int i = 0; i < VEC; ++i) one(j0 + i);
   }
   for (int j = threadIdx.x; j < sp.lead + cols - sp.tail; j += THREADS) one(j < sp.lead ? j : sp.tail + j - sp.lead);
+}
+
+// ------------------------------------------------------------------ sums of a block
+template <int THREADS> __device__ __forceinline__ double block_sum(double v, double* smem /*[THREADS/32]*/) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) v += smem[w];
+  return v;
+}
+
+// loss = mean of pair_loss, in a fixed order; by the 256 threads of a block
+__device__ __forceinline__ void mean_of(const double* pair_loss, int pairs, float* loss) {
+  __shared__ double smem[8];
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < pairs; i += 256) sum += pair_loss[i];
+  sum = block_sum<256>(sum, smem);
+  if (threadIdx.x == 0) loss[0] = (float)(sum / pairs);
 }
 
 // ------------------------------------------------------------------ token log-probabilities
@@ -172,7 +253,7 @@ token_logprob_fwd_kernel(const T* logits, long long ld, const long long* targets
   }
   const T* x = logits + (size_t)row * ld;
   float r, s;
-  soft_whole_row<T, ROW_THREADS>(x, V, k, r, s, smem);
+  soft_whole_row<T, ROW_THREADS, ROW_LOADS, false>(x, V, k, r, s, smem, nullptr);
   if (threadIdx.x == 0) {
     logp[row] = (float)row_logp(Elem<T>::get(x + t), k, r, s);
     stats[row] = make_float2(r, s);
@@ -183,27 +264,15 @@ template <typename T>
 __global__ void __launch_bounds__(ROW_THREADS)
 token_logprob_bwd_kernel(const T* logits, long long ld, const long long* targets, const float2* stats, const float* row_grad,
                          const float* gscale_dev, float gscale, K2 k, T* dlogits, long long ldd, int V, int cols,
-                         long long ignore_index) {
+                         long long ignore_index, const double* pair_loss, int pairs, float* loss) {
   bb::pdl_sync();
-  const int row = blockIdx.x;
+  if (pair_loss && blockIdx.x == 0) mean_of(pair_loss, pairs, loss);     // (the preference loss: one launch less)
+  const int row = gridDim.x - 1 - blockIdx.x;     // the rows that the forward pass read last may still be in L2
   const long long t = targets[row];
   const float2 st = stats[row];
   const bool counted = t != ignore_index && t >= 0 && t < V;
   const float g = counted ? row_grad[row] * (gscale_dev ? gscale_dev[0] : 1.f) * gscale : 0.f;
-  grad_row<T, ROW_THREADS>(logits + (size_t)row * ld, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, st.x, st.y);
-}
-
-// ------------------------------------------------------------------ sums of a block
-template <int THREADS> __device__ __forceinline__ double block_sum(double v, double* smem /*[THREADS/32]*/) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) v += smem[w];
-  return v;
+  grad_row<T, ROW_THREADS, ROW_LOADS, false>(logits + (size_t)row * ld, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, st.x, st.y, nullptr);
 }
 
 // Tokens [a, b) of sequence q: rows of `seq_len` tokens, or between two offsets.  Offsets that do not ascend within [0, tokens]
@@ -285,15 +354,10 @@ preference_pair_kernel(const float* logp, const float* ref, const long long* tar
   outside_zero(offsets, tokens, 2 * pairs, row_grad);
 }
 
-// loss = mean of pair_loss, in a fixed order
 __global__ void __launch_bounds__(256)
 preference_mean_kernel(const double* pair_loss, int pairs, float* loss) {
-  __shared__ double smem[8];
   bb::pdl_sync();
-  double sum = 0.0;
-  for (int i = threadIdx.x; i < pairs; i += 256) sum += pair_loss[i];
-  sum = block_sum<256>(sum, smem);
-  if (threadIdx.x == 0) loss[0] = (float)(sum / pairs);
+  mean_of(pair_loss, pairs, loss);
 }
 
 // ------------------------------------------------------------------ policy loss
@@ -379,12 +443,14 @@ policy_token_kernel(const float* logp, const long long* targets, const PolicyPar
 }
 
 // One CTA per row of logits: log-probability, the token's loss and, because a row's gradient needs nothing of the other rows (the
-// weights follow from the targets), that gradient too
-template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS)
+// weights follow from the targets), that gradient too.  CACHE: the row waits in shared memory for its gradient, so that it is read
+// once; rows that do not fit are read again, from L2.
+template <typename T, int THREADS, bool CACHE>
+__global__ void __launch_bounds__(THREADS)
 policy_row_kernel(const T* logits, long long ld, const long long* targets, const PolicyParams p, K2 k, float gscale,
                   T* dlogits, long long ldd, int V, int cols, long long ignore_index, float* logp, double* partial, int* status) {
-  __shared__ float2 smem[ROW_THREADS / 32];
+  extern __shared__ uint4 cache[];
+  __shared__ float2 smem[THREADS / 32];
   __shared__ float s_slope;
   bb::pdl_sync();
   const int row = blockIdx.x;
@@ -393,7 +459,7 @@ policy_row_kernel(const T* logits, long long ld, const long long* targets, const
   const bool counted = t != ignore_index && t >= 0 && t < V && !(p.weight && p.weight[row] == 0.f);
   float r = 0.f, s = 0.f, g = 0.f;
   if (counted) {
-    soft_whole_row<T, ROW_THREADS>(x, V, k, r, s, smem);
+    soft_whole_row<T, THREADS, ROW_LOADS, CACHE>(x, V, k, r, s, smem, cache);
   }
   if (threadIdx.x == 0) {
     double lp = 0.0;
@@ -412,7 +478,7 @@ policy_row_kernel(const T* logits, long long ld, const long long* targets, const
   }
   __syncthreads();            // also: every thread is past its reads of the row before it may be overwritten
   g = s_slope;
-  grad_row<T, ROW_THREADS>(x, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, r, s);
+  grad_row<T, THREADS, ROW_LOADS, CACHE>(x, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, r, s, cache);
 }
 
 // A gradient that was made for an upstream gradient of `made_for`, times *grad / made_for: nothing to do where they are the same
@@ -617,7 +683,8 @@ int refuse(const char* msg) { bb_set_last_error_msg(msg); return BB_ERR_INVALID_
 struct PolicyPlan { int num_counts; long long piece; size_t weight_at, partial_at, logp_at, bytes; };
 PolicyPlan policy_plan(long long tokens, int n_seq, int by_sequence, long long partials, bool logp) {
   PolicyPlan pl;
-  pl.piece = 16384;
+  // (64 pieces at most: every CTA of the next kernel adds them up)
+  pl.piece = (tokens + 63) / 64 > 2048 ? (tokens + 63) / 64 : 2048;
   pl.num_counts = by_sequence ? n_seq : (int)((tokens + pl.piece - 1) / pl.piece);
   size_t at = ((size_t)pl.num_counts * 4 + 15) & ~(size_t)15;
   pl.weight_at = at; at += by_sequence ? (size_t)tokens * 4 : 0;
@@ -664,21 +731,39 @@ bool bad_list(const bb_grad_tensor* list, int count) {
   return false;
 }
 
+int logprob_fwd(const void* logits, int dtype, long long ld, const long long* targets, double scale, float* logp, float* stats, long long rows, int vocab,
+                long long ignore_index, cudaStream_t s) {
+  const K2 k = split_k(scale);
+  int* status = bb_device_status_word();
+  if (dtype == BB_DTYPE_BF16)
+    BB_CUDA_CHECK(bb_launch(token_logprob_fwd_kernel<__nv_bfloat16>, (int)rows, ROW_THREADS, 0, s, (const __nv_bfloat16*)logits, ld, targets, k, logp,
+                            (float2*)stats, vocab, ignore_index, status));
+  else
+    BB_CUDA_CHECK(bb_launch(token_logprob_fwd_kernel<float>, (int)rows, ROW_THREADS, 0, s, (const float*)logits, ld, targets, k, logp, (float2*)stats, vocab,
+                            ignore_index, status));
+  return BB_OK;
+}
+int logprob_bwd(const void* logits, int dtype, long long ld, const long long* targets, double scale, const float* stats, const float* row_grad,
+                const float* grad_scale_dev, float grad_scale, void* dlogits, long long ldd, long long rows, int vocab, int cols, long long ignore_index,
+                const double* pair_loss, int pairs, float* loss, cudaStream_t s) {
+  const K2 k = split_k(scale);
+  const float g = (float)(scale * grad_scale);
+  if (dtype == BB_DTYPE_BF16)
+    BB_CUDA_CHECK(bb_launch(token_logprob_bwd_kernel<__nv_bfloat16>, (int)rows, ROW_THREADS, 0, s, (const __nv_bfloat16*)logits, ld, targets,
+                            (const float2*)stats, row_grad, grad_scale_dev, g, k, (__nv_bfloat16*)dlogits, ldd, vocab, cols, ignore_index, pair_loss, pairs, loss));
+  else
+    BB_CUDA_CHECK(bb_launch(token_logprob_bwd_kernel<float>, (int)rows, ROW_THREADS, 0, s, (const float*)logits, ld, targets, (const float2*)stats, row_grad,
+                            grad_scale_dev, g, k, (float*)dlogits, ldd, vocab, cols, ignore_index, pair_loss, pairs, loss));
+  return BB_OK;
+}
+
 }  // namespace
 
 extern "C" int bb_token_logprob_fwd(const void* logits, int dtype, long long ld, const long long* targets, double scale, float* logp,
                                     float* stats, long long rows, int vocab, long long ignore_index, void* stream) {
   if (bad_logits("bb_token_logprob_fwd", logits, dtype, ld, targets, rows, vocab, scale)) return BB_ERR_INVALID_ARG;
   if (!logp || !stats || ((uintptr_t)stats & 7)) return refuse("bb_token_logprob_fwd: logp and stats (8-byte aligned) are needed");
-  const K2 k = split_k(scale);
-  int* status = bb_device_status_word();
-  if (dtype == BB_DTYPE_BF16)
-    BB_CUDA_CHECK(bb_launch(token_logprob_fwd_kernel<__nv_bfloat16>, (int)rows, ROW_THREADS, 0, (cudaStream_t)stream, (const __nv_bfloat16*)logits, ld, targets,
-                            k, logp, (float2*)stats, vocab, ignore_index, status));
-  else
-    BB_CUDA_CHECK(bb_launch(token_logprob_fwd_kernel<float>, (int)rows, ROW_THREADS, 0, (cudaStream_t)stream, (const float*)logits, ld, targets, k,
-                            logp, (float2*)stats, vocab, ignore_index, status));
-  return BB_OK;
+  return logprob_fwd(logits, dtype, ld, targets, scale, logp, stats, rows, vocab, ignore_index, (cudaStream_t)stream);
 }
 
 extern "C" int bb_token_logprob_bwd(const void* logits, int dtype, long long ld, const long long* targets, double scale, const float* stats,
@@ -687,37 +772,66 @@ extern "C" int bb_token_logprob_bwd(const void* logits, int dtype, long long ld,
   if (bad_logits("bb_token_logprob_bwd", logits, dtype, ld, targets, rows, vocab, scale)) return BB_ERR_INVALID_ARG;
   if (!stats || ((uintptr_t)stats & 7) || !row_grad || bad_output(logits, ld, dlogits, ldd, dtype, rows, vocab, cols))
     return refuse("bb_token_logprob_bwd: null pointer, columns that do not cover the vocabulary, or a gradient that overlaps the logits without being in place");
-  const K2 k = split_k(scale);
-  const float g = (float)(scale * grad_scale);
-  if (dtype == BB_DTYPE_BF16)
-    BB_CUDA_CHECK(bb_launch(token_logprob_bwd_kernel<__nv_bfloat16>, (int)rows, ROW_THREADS, 0, (cudaStream_t)stream, (const __nv_bfloat16*)logits, ld, targets,
-                            (const float2*)stats, row_grad, grad_scale_dev, g, k, (__nv_bfloat16*)dlogits, ldd, vocab, cols, ignore_index));
-  else
-    BB_CUDA_CHECK(bb_launch(token_logprob_bwd_kernel<float>, (int)rows, ROW_THREADS, 0, (cudaStream_t)stream, (const float*)logits, ld, targets,
-                            (const float2*)stats, row_grad, grad_scale_dev, g, k, (float*)dlogits, ldd, vocab, cols, ignore_index));
+  return logprob_bwd(logits, dtype, ld, targets, scale, stats, row_grad, grad_scale_dev, grad_scale, dlogits, ldd, rows, vocab, cols, ignore_index, nullptr, 0,
+                     nullptr, (cudaStream_t)stream);
+}
+
+namespace {
+int preference_check(const bb_preference_desc* d, const long long* targets, const long long* offsets, const float* loss, const float* rewards,
+                     const void* workspace) {
+  if (!d || !targets || !loss || !rewards || !workspace || ((uintptr_t)workspace & 15))
+    return refuse("bb_preference_loss: null pointer, or a workspace that is not 16-byte aligned");
+  if (d->tokens <= 0 || d->tokens > INT_MAX || d->sequences <= 0 || d->sequences % 2 || (!offsets && d->tokens % d->sequences))
+    return refuse("bb_preference_loss: sequences come in pairs, and without offsets all have tokens / sequences tokens");
+  if (d->form < BB_PREFERENCE_SIGMOID || d->form > BB_PREFERENCE_SQUARED || !(d->beta > 0.0) || !(d->label_smoothing >= 0.0 && d->label_smoothing <= 1.0))
+    return refuse("bb_preference_loss: unknown form, beta that is not positive, or label smoothing outside [0, 1]");
   return BB_OK;
 }
+int preference_pairs(const bb_preference_desc* d, const float* logp, const float* ref, const long long* targets, const long long* offsets, float* rewards,
+                     float* row_grad, double* pair_loss, cudaStream_t s) {
+  const int pairs = d->sequences / 2;
+  BB_CUDA_CHECK(bb_launch(preference_pair_kernel, pairs, 256, 0, s, logp, ref, targets, offsets, d->tokens / d->sequences, d->tokens, pairs, d->form,
+                          d->beta, d->label_smoothing, d->average, d->ignore_index, pair_loss, rewards, row_grad, bb_device_status_word()));
+  return BB_OK;
+}
+}  // namespace
 
 extern "C" int bb_preference_loss(const bb_preference_desc* d, const float* logp, const float* ref, const long long* targets,
                                   const long long* offsets, float* loss, float* rewards, float* row_grad, void* workspace,
                                   long long workspace_bytes, void* stream) {
-  if (!d || !logp || !targets || !loss || !rewards || !row_grad || !workspace || ((uintptr_t)workspace & 7))
-    return refuse("bb_preference_loss: null pointer, or a workspace that is not 8-byte aligned");
-  if (d->tokens <= 0 || d->sequences <= 0 || d->sequences % 2 || (!offsets && d->tokens % d->sequences))
-    return refuse("bb_preference_loss: sequences come in pairs, and without offsets all have tokens / sequences tokens");
-  if (d->form < BB_PREFERENCE_SIGMOID || d->form > BB_PREFERENCE_SQUARED || !(d->beta > 0.0) || !(d->label_smoothing >= 0.0 && d->label_smoothing <= 1.0))
-    return refuse("bb_preference_loss: unknown form, beta that is not positive, or label smoothing outside [0, 1]");
-  const int pairs = d->sequences / 2;
+  if (int rc = preference_check(d, targets, offsets, loss, rewards, workspace)) return rc;
+  if (!logp || !row_grad) return refuse("bb_preference_loss: logp and row_grad are needed");
   if (workspace_bytes < bb_preference_workspace_bytes(d)) return refuse("bb_preference_loss: workspace smaller than bb_preference_workspace_bytes()");
   cudaStream_t s = (cudaStream_t)stream;
   double* pair_loss = (double*)workspace;
   BackToBack overlap;
-  BB_CUDA_CHECK(bb_launch(preference_pair_kernel, pairs, 256, 0, s, logp, ref, targets, offsets, d->tokens / d->sequences, d->tokens, pairs, d->form,
-                          d->beta, d->label_smoothing, d->average, d->ignore_index, pair_loss, rewards, row_grad, bb_device_status_word()));
-  BB_CUDA_CHECK(bb_launch(preference_mean_kernel, 1, 256, 0, s, (const double*)pair_loss, pairs, loss));
+  if (int rc = preference_pairs(d, logp, ref, targets, offsets, rewards, row_grad, pair_loss, s)) return rc;
+  BB_CUDA_CHECK(bb_launch(preference_mean_kernel, 1, 256, 0, s, (const double*)pair_loss, d->sequences / 2, loss));
   return BB_OK;
 }
-extern "C" long long bb_preference_workspace_bytes(const bb_preference_desc* d) { return d && d->sequences > 0 ? (long long)d->sequences * 4 + 8 : -1; }
+
+extern "C" int bb_preference_loss_logits(const bb_preference_desc* d, const void* logits, int dtype, long long ld, double scale, int vocab, int cols,
+                                         const float* ref, const long long* targets, const long long* offsets, float* loss, float* rewards,
+                                         void* dlogits, long long ldd, float grad_scale, void* workspace, long long workspace_bytes, void* stream) {
+  if (int rc = preference_check(d, targets, offsets, loss, rewards, workspace)) return rc;
+  if (bad_logits("bb_preference_loss_logits", logits, dtype, ld, targets, d->tokens, vocab, scale)) return BB_ERR_INVALID_ARG;
+  if (bad_output(logits, ld, dlogits, ldd, dtype, d->tokens, vocab, cols))
+    return refuse("bb_preference_loss_logits: columns that do not cover the vocabulary, or a gradient that overlaps the logits without being in place");
+  if (workspace_bytes < bb_preference_workspace_bytes(d)) return refuse("bb_preference_loss_logits: workspace smaller than bb_preference_workspace_bytes()");
+  cudaStream_t s = (cudaStream_t)stream;
+  // pair losses | softmax sums | log-probabilities | row gradients
+  double* pair_loss = (double*)workspace;
+  float* stats = (float*)(pair_loss + d->sequences / 2);
+  float *logp = stats + 2 * d->tokens, *row_grad = logp + d->tokens;
+  BackToBack overlap;
+  if (int rc = logprob_fwd(logits, dtype, ld, targets, scale, logp, stats, d->tokens, vocab, d->ignore_index, s)) return rc;
+  if (int rc = preference_pairs(d, logp, ref, targets, offsets, rewards, row_grad, pair_loss, s)) return rc;
+  return logprob_bwd(logits, dtype, ld, targets, scale, stats, row_grad, nullptr, grad_scale, dlogits, ldd, d->tokens, vocab, cols, d->ignore_index, pair_loss,
+                     d->sequences / 2, loss, s);
+}
+extern "C" long long bb_preference_workspace_bytes(const bb_preference_desc* d) {
+  return d && d->sequences > 0 && d->tokens > 0 ? (long long)d->sequences * 4 + 8 + 16 * d->tokens : -1;
+}
 
 namespace {
 int policy_check(const bb_policy_desc* d, const long long* targets, const long long* offsets, const float* advantages, const float* loss,
@@ -745,6 +859,27 @@ int policy_front(const bb_policy_desc* d, const PolicyPlan& pl, const long long*
   BB_CUDA_CHECK(bb_launch(policy_count_kernel, pl.num_counts, 256, 0, s, targets, offsets, by_sequence ? seq_len : pl.piece, d->tokens, d->ignore_index,
                           counts, weight, bb_device_status_word()));
   return BB_OK;
+}
+}  // namespace
+
+namespace {
+struct PolicyRowCall {
+  long long ld; const long long* targets; PolicyParams p; K2 k; float gscale; long long ldd; int V, cols; long long ignore_index;
+  float* logp; double* partial; int* status; int rows; cudaStream_t stream;
+};
+template <typename T, int THREADS, bool CACHE> int policy_rows_as(const T* logits, T* dlogits, const PolicyRowCall& c, size_t bytes) {
+  if (CACHE)
+    BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(policy_row_kernel<T, THREADS, CACHE>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_CACHE)));
+  BB_CUDA_CHECK(bb_launch(policy_row_kernel<T, THREADS, CACHE>, c.rows, THREADS, CACHE ? bytes : 0, c.stream, logits, c.ld, c.targets, c.p, c.k, c.gscale,
+                          dlogits, c.ldd, c.V, c.cols, c.ignore_index, c.logp, c.partial, c.status));
+  return BB_OK;
+}
+// Threads by how many rows an SM holds at a time
+template <typename T> int policy_rows(const T* logits, T* dlogits, const PolicyRowCall& c) {
+  const size_t bytes = (size_t)c.V * sizeof(T) / 16 * 16;
+  if (bytes > MAX_CACHE) return policy_rows_as<T, 512, false>(logits, dlogits, c, 0);
+  if (bytes > PAIR_CACHE) return policy_rows_as<T, 1024, true>(logits, dlogits, c, bytes);
+  return bytes > 32768 ? policy_rows_as<T, 512, true>(logits, dlogits, c, bytes) : policy_rows_as<T, 256, true>(logits, dlogits, c, bytes);
 }
 }  // namespace
 
@@ -790,12 +925,9 @@ extern "C" int bb_policy_loss_logits(const bb_policy_desc* d, const void* logits
   PolicyParams p;
   BackToBack overlap;
   if (int rc = policy_front(d, pl, targets, offsets, old_logp, advantages, ref, workspace, p, s)) return rc;
-  if (dtype == BB_DTYPE_BF16)
-    BB_CUDA_CHECK(bb_launch(policy_row_kernel<__nv_bfloat16>, (int)d->tokens, ROW_THREADS, 0, s, (const __nv_bfloat16*)logits, ld, targets, p, k, g,
-                            (__nv_bfloat16*)dlogits, ldd, vocab, cols, d->ignore_index, logp, partial, status));
-  else
-    BB_CUDA_CHECK(bb_launch(policy_row_kernel<float>, (int)d->tokens, ROW_THREADS, 0, s, (const float*)logits, ld, targets, p, k, g, (float*)dlogits, ldd,
-                            vocab, cols, d->ignore_index, logp, partial, status));
+  const PolicyRowCall c = {ld, targets, p, k, g, ldd, vocab, cols, d->ignore_index, logp, partial, status, (int)d->tokens, s};
+  if (int rc = dtype == BB_DTYPE_BF16 ? policy_rows((const __nv_bfloat16*)logits, (__nv_bfloat16*)dlogits, c) : policy_rows((const float*)logits, (float*)dlogits, c))
+    return rc;
   BB_CUDA_CHECK(bb_launch(policy_finish_kernel, 1, 1024, 0, s, (const double*)partial, d->tokens, p.counts, p.num_counts, loss, stats));
   return BB_OK;
 }
@@ -823,24 +955,29 @@ extern "C" int bb_grad_sumsq(const bb_grad_tensor* tensors, int count, double* p
   return BB_OK;
 }
 
-extern "C" int bb_grad_clip(const bb_grad_tensor* tensors, int count, const double* partials, int num_partials, double max_norm, float* norm,
+extern "C" int bb_grad_clip(const bb_grad_tensor* tensors, int count, double* partials, int num_partials, double max_norm, float* norm,
                             void* stream) {
-  if (bad_list(tensors, count) || !partials || num_partials <= 0 || !norm || !(max_norm > 0.0))
+  if (bad_list(tensors, count) || !partials || num_partials < 0 || !norm || !(max_norm > 0.0))
     return refuse("bb_grad_clip: null pointer, an empty tensor, a type other than bf16 and fp32, or a norm that is not positive");
+  BackToBack overlap;
+  if (num_partials == 0) {
+    if (int rc = bb_grad_sumsq(tensors, count, partials, stream)) return rc;
+    num_partials = bb_grad_norm_partials(count);
+  }
   for (int at = 0; at < count; at += LIST_TENSORS) {
     TensorTable t;
     const int pieces = table_fill(t, tensors + at, count - at < LIST_TENSORS ? count - at : LIST_TENSORS);
     const int grid = pieces < norm_ctas() ? pieces : norm_ctas();
-    BB_CUDA_CHECK(bb_launch(grad_clip_kernel, grid, NORM_THREADS, 0, (cudaStream_t)stream, t, partials, num_partials, max_norm, norm));
+    BB_CUDA_CHECK(bb_launch(grad_clip_kernel, grid, NORM_THREADS, 0, (cudaStream_t)stream, t, (const double*)partials, num_partials, max_norm, norm));
   }
   return BB_OK;
 }
 
 extern "C" int bb_adam_step_clipped(float* master, float* grad, float* exp_avg, float* exp_avg_sq, void* param_bf16, long long n, double lr,
                                     double beta1, double beta2, double eps, int step, int adam_w_mode, int bias_correction,
-                                    double weight_decay, double grad_scale, int zero_grad, const double* partials, int num_partials,
+                                    double weight_decay, double grad_scale, int zero_grad, double* partials, int num_partials,
                                     double max_norm, float* norm, void* stream) {
-  if (!master || !grad || !exp_avg || !exp_avg_sq || n <= 0 || (n & 3) || step < 1 || !partials || num_partials <= 0 || !norm || !(max_norm > 0.0) ||
+  if (!master || !grad || !exp_avg || !exp_avg_sq || n <= 0 || (n & 3) || step < 1 || !partials || num_partials < 0 || !norm || !(max_norm > 0.0) ||
       (((uintptr_t)master | (uintptr_t)grad | (uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & 15) || ((uintptr_t)param_bf16 & 7))
     return refuse("bb_adam_step_clipped: null or unaligned pointer, n not a multiple of 4, step < 1, or a norm that is not positive");
   AdamParams a;
@@ -848,8 +985,14 @@ extern "C" int bb_adam_step_clipped(float* master, float* grad, float* exp_avg, 
   a.inv_bc1 = bias_correction ? (float)(1.0 / (1.0 - pow(beta1, step))) : 1.f;
   a.inv_bc2 = bias_correction ? (float)(1.0 / (1.0 - pow(beta2, step))) : 1.f;
   a.decay = (float)weight_decay; a.decoupled = adam_w_mode ? 1 : 0; a.zero_grad = zero_grad;
+  BackToBack overlap;
+  if (num_partials == 0) {
+    const bb_grad_tensor t = {grad, n, BB_DTYPE_F32};
+    if (int rc = bb_grad_sumsq(&t, 1, partials, stream)) return rc;
+    num_partials = bb_grad_norm_partials(1);
+  }
   const long long want = ((n >> 2) + 255) / 256, cap = 8LL * bb_num_sms();
   BB_CUDA_CHECK(bb_launch(adam_clip_kernel, (int)(want < cap ? want : cap), 256, 0, (cudaStream_t)stream, master, grad, exp_avg, exp_avg_sq,
-                          (__nv_bfloat16*)param_bf16, n, a, partials, num_partials, grad_scale, max_norm, norm));
+                          (__nv_bfloat16*)param_bf16, n, a, (const double*)partials, num_partials, grad_scale, max_norm, norm));
   return BB_OK;
 }

@@ -137,6 +137,7 @@ def load():
         lib.bb_token_logprob_bwd.argtypes = [vp, i, ll, vp, d, vp, vp, vp, f, vp, ll, ll, i, i, ll, vp]
         lib.bb_preference_workspace_bytes.restype = ll
         lib.bb_preference_loss.argtypes = [vp] * 9 + [ll, vp]
+        lib.bb_preference_loss_logits.argtypes = [vp, vp, i, ll, d, i, i] + [vp] * 6 + [ll, f, vp, ll, vp]
         lib.bb_policy_workspace_bytes.restype = ll
         lib.bb_policy_loss.argtypes = [vp] * 11 + [ll, vp]
         lib.bb_policy_loss_logits.argtypes = [vp, vp, i, ll, d, i, i] + [vp] * 9 + [ll, f, vp, ll, vp]
@@ -642,6 +643,17 @@ def preference_loss(desc, logp, ref, targets, offsets, loss, rewards, row_grad):
     return loss
 
 
+def preference_loss_logits(desc, logits, targets, vocab, ref, offsets, loss, rewards, dlogits, scale=1.0, grad_scale=1.0):
+    global LAUNCHES
+    LAUNCHES += 3
+    lib = load()
+    ws = workspace(max(0, lib.bb_preference_workspace_bytes(ctypes.byref(desc))), "post_training")
+    check(lib.bb_preference_loss_logits(ctypes.byref(desc), logits.data_ptr(), _dtype(logits, "logits"), logits.stride(0), scale, vocab, logits.shape[1],
+                                        _addr(ref), targets.data_ptr(), _addr(offsets), loss.data_ptr(), rewards.data_ptr(), dlogits.data_ptr(),
+                                        dlogits.stride(0), grad_scale, ws.data_ptr(), ws.numel(), _raw_stream()), "bb_preference_loss_logits")
+    return loss
+
+
 def policy_loss(desc, logp, old_logp, advantages, ref, targets, offsets, loss, stats, row_grad):
     global LAUNCHES
     LAUNCHES += 3
@@ -699,17 +711,19 @@ def grad_sumsq(table, count, partials):
     check(load().bb_grad_sumsq(table, count, _addr(partials), _raw_stream()), "bb_grad_sumsq")
 
 
-def grad_clip(table, count, partials, num_partials, max_norm, norm):
+def grad_clip(table, count, partials, max_norm, norm, num_partials=0):
+    """``num_partials`` 0: the norm is over this list, and made by this call (``partials``: room for it)."""
     global LAUNCHES
-    LAUNCHES += (count + 127) // 128
+    LAUNCHES += (count + 127) // 128 * (1 if num_partials else 2)
     check(load().bb_grad_clip(table, count, _addr(partials), num_partials, max_norm, norm.data_ptr(), _raw_stream()), "bb_grad_clip")
     return norm
 
 
 def adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, *, lr, beta1=0.9, beta2=0.999, eps=1e-8, step, adam_w_mode=True,
-                      bias_correction=True, weight_decay=0.0, grad_scale=1.0, zero_grad=True, partials, num_partials, max_norm, norm):
+                      bias_correction=True, weight_decay=0.0, grad_scale=1.0, zero_grad=True, partials, num_partials=0, max_norm, norm):
+    """``num_partials`` 0: the norm is over ``grad``, and made by this call (``partials``: room for ``grad_norm_partials(1)`` values)."""
     global LAUNCHES
-    LAUNCHES += 1
+    LAUNCHES += 1 if num_partials else 2
     check(load().bb_adam_step_clipped(master.data_ptr(), grad.data_ptr(), exp_avg.data_ptr(), exp_avg_sq.data_ptr(), _addr(param_lp), master.numel(),
                                       lr, beta1, beta2, eps, step, int(adam_w_mode), int(bias_correction), weight_decay, grad_scale, int(zero_grad),
                                       _addr(partials), num_partials, max_norm, norm.data_ptr(), _raw_stream()), "bb_adam_step_clipped")

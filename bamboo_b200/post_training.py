@@ -37,7 +37,9 @@ def _rows(logits, vocab):
 
 
 def _flat(t, name, numel, dtype, device):
-    """A per-token (or per-sequence) tensor as contiguous 1-D memory of the given type."""
+    """A per-token (or per-sequence) tensor as contiguous memory of the given type, whatever its shape."""
+    if t.dtype is dtype and t.numel() == numel and t.device == device and t.is_contiguous():
+        return t
     if t.device != device:
         raise L.BambooNativeError(f"{name}: on {t.device}, the logits are on {device}")
     if t.numel() != numel:
@@ -321,12 +323,15 @@ class PreferenceLoss:
         self.form = (beta, form, label_smoothing, average)
         self.rewards = None
 
-    def _losses(self, logits, labels, offsets):
+    def _prepare(self, logits, labels, offsets):
         targets, ref = labels if isinstance(labels, (tuple, list)) else (labels, None)
         lg, vocab = _rows(logits, self.vocab)
         sequences, offsets = _geometry(targets, offsets)
         tg = _flat(targets, "targets", lg.shape[0], torch.int64, lg.device)
-        desc = _preference_desc(lg.shape[0], sequences, *self.form, self.ignore_index)
+        return lg, vocab, tg, ref, offsets, _preference_desc(lg.shape[0], sequences, *self.form, self.ignore_index)
+
+    def _losses(self, logits, labels, offsets):
+        lg, vocab, tg, ref, offsets, desc = self._prepare(logits, labels, offsets)
         logp, stats = _logprobs(lg, tg, vocab, self.scale, self.ignore_index)
         loss, self.rewards, row_grad = _preference(logp, ref, tg, offsets, desc)
         return lg, tg, stats, row_grad, loss
@@ -348,9 +353,12 @@ class PreferenceLoss:
     def loss_and_grad(self, logits, labels, *, offsets=None, out=None, grad_scale=1.0):
         """(loss, rewards, gradient of the logits times ``grad_scale``) without autograd; ``out`` receives the gradient (the logits
         themselves are allowed)."""
-        lg, tg, stats, row_grad, loss = self._losses(logits, labels, offsets)
+        lg, vocab, tg, ref, offsets, desc = self._prepare(logits, labels, offsets)
+        ref = None if ref is None else _flat(ref, "ref_logps", lg.shape[0], torch.float32, lg.device)
+        loss = torch.empty((), dtype=torch.float32, device=lg.device)
+        self.rewards = torch.empty(desc.sequences, dtype=torch.float32, device=lg.device)
         d, grad = _gradient_buffer(lg, logits, out)
-        L.token_logprob_bwd(lg, tg, stats, row_grad, d, self.vocab, self.scale, self.ignore_index, grad_scale=grad_scale)
+        L.preference_loss_logits(desc, lg, tg, vocab, ref, offsets, loss, self.rewards, d, self.scale, grad_scale)
         return loss, self.rewards, grad
 
 
@@ -483,11 +491,10 @@ def clip_grad_norm_(tensors, max_norm):
     if not grads:
         return torch.zeros(())
     staged = [g if _dense(g) else g.contiguous() for g in grads]
-    partials, n = _partials(staged)
+    partials, _ = _partials(staged)
     table = L.grad_tensors(staged)
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    L.grad_sumsq(table, len(staged), partials)
-    L.grad_clip(table, len(staged), partials, n, max_norm, norm)
+    L.grad_clip(table, len(staged), partials, max_norm, norm)
     for g, s in zip(grads, staged):
         if s is not g:
             g.copy_(s)
@@ -505,10 +512,6 @@ def adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, *, max_norm, 
         if not t.is_cuda or t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != master.numel():
             raise L.BambooNativeError("adam_step_clipped: contiguous fp32 CUDA tensors of one size are expected")
     norm = torch.empty((), dtype=torch.float32, device=master.device)
-    if sumsq is None:
-        partials, n = _partials([grad])
-        L.grad_sumsq(L.grad_tensors([grad]), 1, partials)
-    else:
-        partials, n = sumsq, 1
+    partials, n = (_partials([grad])[0], 0) if sumsq is None else (sumsq, 1)
     return L.adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, grad_scale=grad_scale, partials=partials, num_partials=n,
                                max_norm=max_norm, norm=norm, **adam)

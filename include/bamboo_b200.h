@@ -356,6 +356,12 @@ long long bb_preference_workspace_bytes(const bb_preference_desc* d);
 int bb_preference_loss(const bb_preference_desc* d, const float* logp, const float* ref, const long long* targets,
                        const long long* offsets, float* loss, float* rewards, float* row_grad, void* workspace,
                        long long workspace_bytes, void* stream);
+/* The same from logits, and their gradient times grad_scale: the three passes in one call; arguments otherwise as in
+ * bb_token_logprob_*. */
+int bb_preference_loss_logits(const bb_preference_desc* d, const void* logits, int dtype, long long ld, double scale, int vocab,
+                              int cols, const float* ref, const long long* targets, const long long* offsets, float* loss,
+                              float* rewards, void* dlogits, long long ldd, float grad_scale, void* workspace,
+                              long long workspace_bytes, void* stream);
 
 /* Clipped policy loss.  Per counted token: ratio = exp(logp - old) (old NULL: 1), surrogate = min(ratio A, clamp(ratio, 1 -
  * clip_low, 1 + clip_high) A), KL = exp(ref - logp) - (ref - logp) - 1 (ref NULL: none), loss = -surrogate + kl_coef KL.
@@ -388,17 +394,18 @@ int bb_rescale_grad(void* grad, int dtype, long long ld, long long rows, int col
 
 /* Global norm of a list of gradients and clipping.  bb_grad_sumsq writes bb_grad_norm_partials(count) partial sums of squares
  * (64-bit); their sum, over whatever else the caller adds (other pipeline stages), is the squared norm.  The consumers take
- * `num_partials` such values, norm = grad_scale * sqrt(sum), coefficient = min(1, max_norm / (norm + 1e-6)), and write the
+ * `num_partials` such values (0: they make them first, from their own gradients, in the room for
+ * bb_grad_norm_partials(count) values at `partials`; 1 tensor for the Adam step), norm = grad_scale * sqrt(sum), coefficient = min(1, max_norm / (norm + 1e-6)), and write the
  * norm before clipping to `norm` (device).  bb_grad_clip scales the tensors in place (not at all within the norm);
  * bb_adam_step_clipped is an Adam step on coefficient * grad_scale * grad.  A norm that is NaN makes everything NaN. */
 typedef struct bb_grad_tensor { void* data; long long numel; int dtype; } bb_grad_tensor;
 int bb_grad_norm_partials(int count);
 int bb_grad_sumsq(const bb_grad_tensor* tensors, int count, double* partials, void* stream);
-int bb_grad_clip(const bb_grad_tensor* tensors, int count, const double* partials, int num_partials, double max_norm, float* norm,
+int bb_grad_clip(const bb_grad_tensor* tensors, int count, double* partials, int num_partials, double max_norm, float* norm,
                  void* stream);
 int bb_adam_step_clipped(float* master, float* grad, float* exp_avg, float* exp_avg_sq, void* param_bf16, long long n, double lr,
                          double beta1, double beta2, double eps, int step, int adam_w_mode, int bias_correction,
-                         double weight_decay, double grad_scale, int zero_grad, const double* partials, int num_partials,
+                         double weight_decay, double grad_scale, int zero_grad, double* partials, int num_partials,
                          double max_norm, float* norm, void* stream);
 
 /* ---- inter-stage transfer --------------------------------------------------------- */
