@@ -8,10 +8,11 @@
 
 namespace {
 
-constexpr int ROW_THREADS = 256, ROW_LOADS = 4;      // threads per row, 16-byte loads that each has in flight
+constexpr int ROW_LOADS = 4;              // 16-byte loads that a thread has in flight
+constexpr size_t LONG_ROW = 32768;        // bytes from which a row gets more threads
 
 // dynamic shared memory next to a kernel's few static bytes: of one CTA per SM, and of each of two
-constexpr size_t MAX_CACHE = 226 * 1024, PAIR_CACHE = 112 * 1024;
+constexpr size_t MAX_RING = 226 * 1024, PAIR_RING = 112 * 1024;
 
 template <typename T> struct Elem;
 template <> struct Elem<__nv_bfloat16> {
@@ -58,15 +59,31 @@ template <typename T> struct Span {
   }
 };
 
-// (r, s) of the block's threads merged; every thread gets the result
-template <int THREADS> __device__ __forceinline__ void soft_block(float& r, float& s, float2* smem /*[THREADS/32]*/) {
+// (r, s) of a warp's lanes merged: the largest reference first, one scaling, then plain sums
+__device__ __forceinline__ void soft_warp(float& r, float& s) {
+  float top = r;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) soft_merge(r, s, __shfl_xor_sync(0xffffffffu, r, o), __shfl_xor_sync(0xffffffffu, s, o));
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (r != top) s *= ex2(r - top);             // (-inf - -inf would be NaN)
+  r = top;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+}
+// Barrier of the block's first THREADS threads: the whole block, or all but a warp that feeds the others
+template <int THREADS, bool FED = false> __device__ __forceinline__ void row_barrier() {
+  if constexpr (FED) asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+  else __syncthreads();
+}
+// (r, s) of the block's threads merged; the first warp gets the result
+template <int THREADS, bool FED = false> __device__ __forceinline__ void soft_block(float& r, float& s, float2* smem /*[THREADS/32]*/) {
+  soft_warp(r, s);
   if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = make_float2(r, s);
-  __syncthreads();
-  r = -INFINITY; s = 0.f;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) soft_merge(r, s, smem[w].x, smem[w].y);
+  row_barrier<THREADS, FED>();
+  if (threadIdx.x < 32) {
+    const float2 q = threadIdx.x < THREADS / 32 ? smem[threadIdx.x] : make_float2(-INFINITY, 0.f);
+    r = q.x; s = q.y;
+    soft_warp(r, s);
+  }
 }
 
 // This thread's share of a row, chunk by chunk with the reference kept below the largest logit (the exact form)
@@ -81,57 +98,70 @@ template <typename T, int THREADS> __device__ __noinline__ float2 soft_share_exa
   return make_float2(r, s);
 }
 
-// (r, s) of this thread's share of a row.  The reference comes from the thread's first chunk and stays: a later logit may be larger,
-// 2^(k x - r) is a float all the same as long as it is below 2^127, so the loop needs no maximum (5 instead of 7 issue slots a
-// logit, at 4.5 of them a clock and SM at the full memory rate); a sum that did overflow is taken again in the exact form.  U loads
-// are in flight per thread.  `cache`: the chunks are left there too (shared memory, one place each).
-template <typename T, int THREADS, int U, bool CACHE>
-__device__ __forceinline__ void soft_row(const T* x, int n, K2 k, float& r, float& s, uint4* cache) {
-  constexpr int VEC = Elem<T>::VEC;
-  const Span<T> sp(x, n);
-  r = -INFINITY; s = 0.f;
-  const uint4* v = reinterpret_cast<const uint4*>(x + sp.lead);
-  float2 sum = make_float2(0.f, 0.f);
-  for (int c = threadIdx.x; c < sp.nvec; c += U * THREADS) {
-    uint4 q[U];
+// VEC logits added to sums whose reference stays (see soft_row)
+template <int VEC> __device__ __forceinline__ void soft_chunk(float2& sum, const float* f, K2 k, float r) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) q[u] = c + u * THREADS < sp.nvec ? v[c + u * THREADS] : Elem<T>::nothing();
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (CACHE && c + u * THREADS < sp.nvec) cache[c + u * THREADS] = q[u];
-      float f[VEC];
-      Elem<T>::unpack(q[u], f);
-      if (r == -INFINITY) {
-        soft_add<VEC>(r, s, f, k);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; i += 2) {
-          const float2 t = expo2(make_float2(f[i], f[i + 1]), k, r);
-          sum = bb::add2(sum, make_float2(ex2(t.x), ex2(t.y)));
-        }
-      }
-    }
+  for (int i = 0; i < VEC; i += 2) {
+    const float2 t = expo2(make_float2(f[i], f[i + 1]), k, r);
+    sum = bb::add2(sum, make_float2(ex2(t.x), ex2(t.y)));
   }
-  s += sum.x + sum.y;
-  if (!(s < INFINITY)) { const float2 e = soft_share_exact<T, THREADS>(v, sp.nvec, k); r = e.x; s = e.y; }
+}
+// the elements of a row in front of its first 16-byte boundary and behind its last
+template <typename T, int THREADS> __device__ __forceinline__ void soft_edges(const T* x, const Span<T>& sp, int n, K2 k, float& r, float& s) {
   for (int j = threadIdx.x; j < sp.lead + n - sp.tail; j += THREADS) {
     const float f = Elem<T>::get(x + (j < sp.lead ? j : sp.tail + j - sp.lead));
     soft_add<1>(r, s, &f, k);
   }
 }
 
+// (r, s) of this thread's share of a row.  The reference comes from the thread's first chunk and stays: a later logit may be larger,
+// 2^(k x - r) is a float all the same as long as it is below 2^127, so the loop needs no maximum; a share whose first chunk
+// is all -inf or whose sum did overflow is taken (again) in the exact form.  U loads are in flight per thread.
+template <typename T, int THREADS, int U>
+__device__ __forceinline__ void soft_row(const T* x, int n, K2 k, float& r, float& s) {
+  constexpr int VEC = Elem<T>::VEC;
+  const Span<T> sp(x, n);
+  r = -INFINITY; s = 0.f;
+  const uint4* v = reinterpret_cast<const uint4*>(x + sp.lead);
+  int c = threadIdx.x;
+  float2 sum = make_float2(0.f, 0.f);
+  float f[VEC];
+  if (c < sp.nvec) {
+    Elem<T>::unpack(v[c], f);
+    soft_add<VEC>(r, s, f, k);
+    c += THREADS;
+  }
+  for (; c + (U - 1) * THREADS < sp.nvec; c += U * THREADS) {
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) q[u] = v[c + u * THREADS];
+#pragma unroll
+    for (int u = 0; u < U; ++u) { Elem<T>::unpack(q[u], f); soft_chunk<VEC>(sum, f, k, r); }
+  }
+  if (c < sp.nvec) {             // up to U - 1 more
+    uint4 q[U - 1];
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u) q[u] = c + u * THREADS < sp.nvec ? v[c + u * THREADS] : Elem<T>::nothing();
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u) { Elem<T>::unpack(q[u], f); soft_chunk<VEC>(sum, f, k, r); }
+  }
+  s += sum.x + sum.y;
+  // (with r = -inf the loop has added NaN or +inf)
+  if (!(s < INFINITY)) { const float2 e = soft_share_exact<T, THREADS>(v, sp.nvec, k); r = e.x; s = e.y; }
+  soft_edges<T, THREADS>(x, sp, n, k, r, s);
+}
+
 // A row whose largest logit is so far from zero that k x is not finite (a row of the type's lowest value): differences at that
 // magnitude leave all of the softmax to the logits that equal the largest.  Kept as (largest, -how many of them there are);
-// (NaN, NaN) with a NaN or +inf in the row, (-inf, 0) when every logit is -inf.  Called by the whole block where r is infinite.
-template <typename T, int THREADS> __device__ __noinline__ void soft_row_extreme(const T* x, int n, float& r, float& s, float2* smem) {
+// (NaN, NaN) with a NaN or +inf in the row, (-inf, 0) when every logit is -inf.  Called by the first warp where r is infinite.
+template <typename T> __device__ __noinline__ float2 soft_row_extreme(const T* x, int n) {
   float top = -INFINITY;
   int count = 0, bad = 0;
-  for (int j = threadIdx.x; j < n; j += THREADS) {
+  for (int j = threadIdx.x; j < n; j += 32) {
     const float f = Elem<T>::get(x + j);
     bad |= f != f || f == INFINITY;
     if (f > top) { top = f; count = 1; } else if (f == top) ++count;
   }
-  bad = __syncthreads_or(bad);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float t2 = __shfl_xor_sync(0xffffffffu, top, o);
@@ -139,77 +169,94 @@ template <typename T, int THREADS> __device__ __noinline__ void soft_row_extreme
     count = (top >= t2 ? count : 0) + (t2 >= top ? c2 : 0);
     top = fmaxf(top, t2);
   }
-  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = make_float2(top, (float)count);
-  __syncthreads();
-  r = -INFINITY;
-  for (int w = 0; w < THREADS / 32; ++w) r = fmaxf(r, smem[w].x);
-  s = 0.f;
-  for (int w = 0; w < THREADS / 32; ++w) if (smem[w].x == r) s -= smem[w].y;
-  if (r == -INFINITY) s = 0.f;
-  if (bad) r = s = NAN;
+  if (__any_sync(0xffffffffu, bad)) return make_float2(NAN, NAN);
+  return make_float2(top, top == -INFINITY ? 0.f : -(float)count);
 }
 
-template <typename T, int THREADS, int U, bool CACHE>
-__device__ __forceinline__ void soft_whole_row(const T* x, int n, K2 k, float& r, float& s, float2* smem, uint4* cache) {
-  soft_row<T, THREADS, U, CACHE>(x, n, k, r, s, cache);
+// The row's (r, s), in the first warp
+template <typename T, int THREADS, int U>
+__device__ __forceinline__ void soft_whole_row(const T* x, int n, K2 k, float& r, float& s, float2* smem) {
+  soft_row<T, THREADS, U>(x, n, k, r, s);
   soft_block<THREADS>(r, s, smem);
-  if (isinf(r)) soft_row_extreme<T, THREADS>(x, n, r, s, smem);
+  if (threadIdx.x < 32 && isinf(r)) { const float2 e = soft_row_extreme(x, n); r = e.x; s = e.y; }
 }
 
-// d[j] = g * ([j == t] - softmax_j) for j < V, 0 in [V, cols); zeros throughout when g == 0 (nothing is read then).  `cache`: the
-// chunks of the row as soft_row left them.
-template <typename T, int THREADS, int U, bool CACHE>
-__device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int t, float g, K2 k, float r, float s, const uint4* cache) {
+// -g softmax of a chunk of logits (ng = -g / s)
+template <typename T> __device__ __forceinline__ void grad_chunk(uint4* d, const uint4& q, K2 k, float r, float ng) {
   constexpr int VEC = Elem<T>::VEC;
-  if (s == 0.f) g = 0.f;
-  const float ng = g == 0.f ? 0.f : -g / s;
-  const bool aligned = (((uintptr_t)x ^ (uintptr_t)d) & 15) == 0;
-  const Span<T> sp(d, aligned ? cols : 0);
+  float f[VEC];
+  Elem<T>::unpack(q, f);
+#pragma unroll
+  for (int i = 0; i < VEC; i += 2) {
+    const float2 e = expo2(make_float2(f[i], f[i + 1]), k, r);
+    const float2 m = bb::mul2(make_float2(ex2(e.x), ex2(e.y)), make_float2(ng, ng));
+    f[i] = m.x; f[i + 1] = m.y;
+  }
+  *d = Elem<T>::pack(f);
+}
+// What follows the chunks [0, whole): the target's entry (xt its logit, read before d, which may be x, was written; by the thread
+// that wrote its chunk), the chunk that the padding begins in, the padding, and the elements around the 16-byte boundaries
+template <typename T, int THREADS>
+__device__ __forceinline__ void grad_rest(const T* x, float xt, T* d, int lead, int whole, int V, int cols, int t, float g, float ng, K2 k, float r) {
+  constexpr int VEC = Elem<T>::VEC;
+  if (t >= lead) {
+    const int tc = (t - lead) / VEC;
+    if (tc < whole && tc % THREADS == (int)threadIdx.x) Elem<T>::put(d + t, ng * ex2(expo(xt, k, r)) + g);
+  }
   auto one = [&](int j) {
     float v = 0.f;
-    if (g != 0.f && j < V) {
-      const float f = Elem<T>::get(x + j);
-      v = s < 0.f ? (f == r ? -ng : 0.f) : ng * ex2(expo(f, k, r));
-      if (j == t) v += g;
-    }
+    if (j < V) { v = ng * ex2(expo(Elem<T>::get(x + j), k, r)); if (j == t) v += g; }
     Elem<T>::put(d + j, v);
   };
-  if (!aligned || s < 0.f) {
-    for (int j = threadIdx.x; j < cols; j += THREADS) one(j);
-    return;
-  }
-  const uint4* xv = CACHE ? cache : reinterpret_cast<const uint4*>(x + sp.lead);
-  uint4* dv = reinterpret_cast<uint4*>(d + sp.lead);
-  // chunks of vocabulary entries only, then the one that the padding begins in and the padding
-  const int whole = g == 0.f || V < sp.lead ? 0 : (V - sp.lead) / VEC;
-  for (int c = threadIdx.x; c < whole; c += U * THREADS) {
-    uint4 q[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) q[u] = c + u * THREADS < whole ? xv[c + u * THREADS] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float f[VEC];
-      Elem<T>::unpack(q[u], f);
-#pragma unroll
-      for (int i = 0; i < VEC; i += 2) {
-        const float2 e = expo2(make_float2(f[i], f[i + 1]), k, r);
-        const float2 m = bb::mul2(make_float2(ex2(e.x), ex2(e.y)), make_float2(ng, ng));
-        f[i] = m.x; f[i + 1] = m.y;
-      }
-      const int at = t - (sp.lead + (c + u * THREADS) * VEC);
-      if (at >= 0 && at < VEC) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) if (i == at) f[i] += g;
-      }
-      if (c + u * THREADS < whole) dv[c + u * THREADS] = Elem<T>::pack(f);
-    }
-  }
-  for (int c = whole + threadIdx.x; c < sp.nvec; c += THREADS) {
-    const int j0 = sp.lead + c * VEC;
-    if (g == 0.f || j0 >= V) dv[c] = make_uint4(0, 0, 0, 0);
+  const int nvec = (cols - lead) / VEC, tail = lead + nvec * VEC;
+  for (int c = whole + threadIdx.x; c < nvec; c += THREADS) {
+    const int j0 = lead + c * VEC;
+    if (j0 >= V) *reinterpret_cast<uint4*>(d + j0) = make_uint4(0, 0, 0, 0);
     else for (int i = 0; i < VEC; ++i) one(j0 + i);
   }
-  for (int j = threadIdx.x; j < sp.lead + cols - sp.tail; j += THREADS) one(j < sp.lead ? j : sp.tail + j - sp.lead);
+  for (int j = threadIdx.x; j < lead + cols - tail; j += THREADS) one(j < lead ? j : tail + j - lead);
+}
+
+// d[j] = g * ([j == t] - softmax_j) for j < V, 0 in [V, cols); zeros throughout when g == 0 (nothing is read then)
+template <typename T, int THREADS, int U>
+__device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int t, float g, K2 k, float r, float s) {
+  constexpr int VEC = Elem<T>::VEC;
+  if (s == 0.f) g = 0.f;
+  if (g == 0.f) {
+    const Span<T> sp(d, cols);
+    uint4* dv = reinterpret_cast<uint4*>(d + sp.lead);
+    for (int c = threadIdx.x; c < sp.nvec; c += THREADS) dv[c] = make_uint4(0, 0, 0, 0);
+    for (int j = threadIdx.x; j < sp.lead + cols - sp.tail; j += THREADS) Elem<T>::put(d + (j < sp.lead ? j : sp.tail + j - sp.lead), 0.f);
+    return;
+  }
+  const float ng = -g / s;
+  if (s < 0.f || (((uintptr_t)x ^ (uintptr_t)d) & 15) != 0) {      // element by element
+    for (int j = threadIdx.x; j < cols; j += THREADS) {
+      float v = 0.f;
+      if (j < V) {
+        const float f = Elem<T>::get(x + j);
+        v = s < 0.f ? (f == r ? -ng : 0.f) : ng * ex2(expo(f, k, r));
+        if (j == t) v += g;
+      }
+      Elem<T>::put(d + j, v);
+    }
+    return;
+  }
+  const Span<T> sp(x, V);
+  const uint4* xv = reinterpret_cast<const uint4*>(x + sp.lead);
+  uint4* dv = reinterpret_cast<uint4*>(d + sp.lead);
+  const int whole = sp.nvec;                            // chunks of vocabulary entries only
+  const float xt = t >= sp.lead && (t - sp.lead) / VEC % THREADS == (int)threadIdx.x ? Elem<T>::get(x + t) : 0.f;
+  int c = threadIdx.x;
+  for (; c + (U - 1) * THREADS < whole; c += U * THREADS) {
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) q[u] = xv[c + u * THREADS];
+#pragma unroll
+    for (int u = 0; u < U; ++u) grad_chunk<T>(dv + c + u * THREADS, q[u], k, r, ng);
+  }
+  for (; c < whole; c += THREADS) grad_chunk<T>(dv + c, xv[c], k, r, ng);
+  grad_rest<T, THREADS>(x, xt, d, sp.lead, whole, V, cols, t, g, ng, k, r);
 }
 
 // ------------------------------------------------------------------ sums of a block
@@ -225,21 +272,21 @@ template <int THREADS> __device__ __forceinline__ double block_sum(double v, dou
   return v;
 }
 
-// loss = mean of pair_loss, in a fixed order; by the 256 threads of a block
-__device__ __forceinline__ void mean_of(const double* pair_loss, int pairs, float* loss) {
-  __shared__ double smem[8];
+// loss = mean of pair_loss, in a fixed order; by a block
+template <int THREADS> __device__ __forceinline__ void mean_of(const double* pair_loss, int pairs, float* loss) {
+  __shared__ double smem[THREADS / 32];
   double sum = 0.0;
-  for (int i = threadIdx.x; i < pairs; i += 256) sum += pair_loss[i];
-  sum = block_sum<256>(sum, smem);
+  for (int i = threadIdx.x; i < pairs; i += THREADS) sum += pair_loss[i];
+  sum = block_sum<THREADS>(sum, smem);
   if (threadIdx.x == 0) loss[0] = (float)(sum / pairs);
 }
 
 // ------------------------------------------------------------------ token log-probabilities
-template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS)
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS)
 token_logprob_fwd_kernel(const T* logits, long long ld, const long long* targets, K2 k, float* logp, float2* stats,
                          int V, long long ignore_index, int* status) {
-  __shared__ float2 smem[ROW_THREADS / 32];
+  __shared__ float2 smem[THREADS / 32];
   bb::pdl_sync();
   const int row = blockIdx.x;
   const long long t = targets[row];
@@ -253,26 +300,26 @@ token_logprob_fwd_kernel(const T* logits, long long ld, const long long* targets
   }
   const T* x = logits + (size_t)row * ld;
   float r, s;
-  soft_whole_row<T, ROW_THREADS, ROW_LOADS, false>(x, V, k, r, s, smem, nullptr);
+  soft_whole_row<T, THREADS, ROW_LOADS>(x, V, k, r, s, smem);
   if (threadIdx.x == 0) {
     logp[row] = (float)row_logp(Elem<T>::get(x + t), k, r, s);
     stats[row] = make_float2(r, s);
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS)
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS)
 token_logprob_bwd_kernel(const T* logits, long long ld, const long long* targets, const float2* stats, const float* row_grad,
                          const float* gscale_dev, float gscale, K2 k, T* dlogits, long long ldd, int V, int cols,
                          long long ignore_index, const double* pair_loss, int pairs, float* loss) {
   bb::pdl_sync();
-  if (pair_loss && blockIdx.x == 0) mean_of(pair_loss, pairs, loss);     // (the preference loss: one launch less)
+  if (pair_loss && blockIdx.x == 0) mean_of<THREADS>(pair_loss, pairs, loss);     // (the preference loss: one launch less)
   const int row = gridDim.x - 1 - blockIdx.x;     // the rows that the forward pass read last may still be in L2
   const long long t = targets[row];
   const float2 st = stats[row];
   const bool counted = t != ignore_index && t >= 0 && t < V;
   const float g = counted ? row_grad[row] * (gscale_dev ? gscale_dev[0] : 1.f) * gscale : 0.f;
-  grad_row<T, ROW_THREADS, ROW_LOADS, false>(logits + (size_t)row * ld, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, st.x, st.y, nullptr);
+  grad_row<T, THREADS, ROW_LOADS>(logits + (size_t)row * ld, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, st.x, st.y);
 }
 
 // Tokens [a, b) of sequence q: rows of `seq_len` tokens, or between two offsets.  Offsets that do not ascend within [0, tokens]
@@ -357,7 +404,7 @@ preference_pair_kernel(const float* logp, const float* ref, const long long* tar
 __global__ void __launch_bounds__(256)
 preference_mean_kernel(const double* pair_loss, int pairs, float* loss) {
   bb::pdl_sync();
-  mean_of(pair_loss, pairs, loss);
+  mean_of<256>(pair_loss, pairs, loss);
 }
 
 // ------------------------------------------------------------------ policy loss
@@ -370,21 +417,24 @@ struct PolicyParams {
   long long adv_div;
   float low, high, kl_coef;     // ratio bounds 1 - clip_low, 1 + clip_high
 };
+struct PolicyInput { float old, adv, ref; };
 struct PolicyToken { float loss, kl, clipped, slope; };
 
-__device__ __forceinline__ PolicyToken policy_token(const PolicyParams& p, long long row, double lp) {
+__device__ __forceinline__ PolicyInput policy_input(const PolicyParams& p, long long row) {
+  return {p.old_logp ? p.old_logp[row] : 0.f, p.advantages[p.adv_div == 1 ? row : row / p.adv_div], p.ref ? p.ref[row] : 0.f};
+}
+__device__ __forceinline__ PolicyToken policy_token(const PolicyParams& p, const PolicyInput& in, double lp) {
   PolicyToken o;
-  const float adv = p.advantages[row / p.adv_div];
-  const float ratio = p.old_logp ? expf((float)(lp - (double)p.old_logp[row])) : 1.f;
+  const float ratio = p.old_logp ? expf((float)(lp - (double)in.old)) : 1.f;
   // (an advantage of 0 has no part in the surrogate, whatever the ratio overflowed to)
-  const float plain = adv == 0.f ? 0.f : ratio * adv, bounded = fminf(fmaxf(ratio, p.low), p.high) * adv;
+  const float plain = in.adv == 0.f ? 0.f : ratio * in.adv, bounded = fminf(fmaxf(ratio, p.low), p.high) * in.adv;
   const bool cut = bounded < plain;
   o.clipped = cut ? 1.f : 0.f;
   o.loss = cut ? -bounded : -plain;
   o.slope = cut ? 0.f : -plain;
   o.kl = 0.f;
   if (p.ref) {
-    const float gap = (float)((double)p.ref[row] - lp), e = expm1f(gap);       // e^gap - gap - 1 without the cancellation
+    const float gap = (float)((double)in.ref - lp), e = expm1f(gap);       // e^gap - gap - 1 without the cancellation
     o.kl = e - gap;
     o.loss += p.kl_coef * o.kl;
     o.slope -= p.kl_coef * e;
@@ -434,7 +484,7 @@ policy_token_kernel(const float* logp, const long long* targets, const PolicyPar
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < tokens; i += (long long)gridDim.x * 256) {
     const float w = p.weight ? p.weight[i] : whole;
     if (targets[i] == ignore_index || w == 0.f) { row_grad[i] = 0.f; continue; }
-    const PolicyToken o = policy_token(p, i, (double)logp[i]);
+    const PolicyToken o = policy_token(p, policy_input(p, i), (double)logp[i]);
     row_grad[i] = o.slope * w;
     loss += (double)o.loss * w; kl += o.kl; clipped += o.clipped;
   }
@@ -442,48 +492,181 @@ policy_token_kernel(const float* logp, const long long* targets, const PolicyPar
   if (threadIdx.x == 0) { partial[3 * blockIdx.x] = loss; partial[3 * blockIdx.x + 1] = kl; partial[3 * blockIdx.x + 2] = clipped; }
 }
 
+// What thread 0 does between the two halves of a row
+__device__ __forceinline__ void policy_row_finish(const PolicyParams& p, const PolicyInput& in, int row, float xt, K2 k, float r, float s, float weight, float gscale,
+                                                  float* s_row, float* logp, double* partial) {
+  const double lp = row_logp(xt, k, r, s);
+  const PolicyToken o = policy_token(p, in, lp);
+  s_row[0] = r; s_row[1] = s; s_row[2] = o.slope * weight * gscale; s_row[3] = xt;
+  logp[row] = (float)lp;
+  partial[3LL * row] = (double)o.loss * weight; partial[3LL * row + 1] = o.kl; partial[3LL * row + 2] = o.clipped;
+}
+__device__ __forceinline__ void policy_row_skip(int row, bool bad, float* logp, double* partial, int* status) {
+  if (bad) atomicCAS(status, 0, BB_ERR_INVALID_ARG);
+  logp[row] = 0.f;
+  partial[3LL * row] = 0.0; partial[3LL * row + 1] = 0.0; partial[3LL * row + 2] = 0.0;
+}
+
 // One CTA per row of logits: log-probability, the token's loss and, because a row's gradient needs nothing of the other rows (the
-// weights follow from the targets), that gradient too.  CACHE: the row waits in shared memory for its gradient, so that it is read
-// once; rows that do not fit are read again, from L2.
-template <typename T, int THREADS, bool CACHE>
+// weights follow from the targets), that gradient too.  For rows that are short, or too long for policy_ring_kernel: the second half reads
+// the row again, from L1 or L2.
+template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS)
 policy_row_kernel(const T* logits, long long ld, const long long* targets, const PolicyParams p, K2 k, float gscale,
-                  T* dlogits, long long ldd, int V, int cols, long long ignore_index, float* logp, double* partial, int* status) {
-  extern __shared__ uint4 cache[];
+                  T* dlogits, long long ldd, int rows, int V, int cols, long long ignore_index, float* logp, double* partial, int* status) {
   __shared__ float2 smem[THREADS / 32];
-  __shared__ float s_slope;
+  __shared__ float s_row[4];
   bb::pdl_sync();
   const int row = blockIdx.x;
   const long long t = targets[row];
   const T* x = logits + (size_t)row * ld;
-  const bool counted = t != ignore_index && t >= 0 && t < V && !(p.weight && p.weight[row] == 0.f);
+  const bool valid = t != ignore_index && t >= 0 && t < V, counted = valid && !(p.weight && p.weight[row] == 0.f);
   float r = 0.f, s = 0.f, g = 0.f;
   if (counted) {
-    soft_whole_row<T, THREADS, ROW_LOADS, CACHE>(x, V, k, r, s, smem, cache);
+    // (in flight while the row is read: one after the other their latencies would stand between the two halves)
+    PolicyInput in = {};
+    float xt = 0.f, weight = 0.f;
+    if (threadIdx.x == 0) { in = policy_input(p, row); xt = Elem<T>::get(x + t); weight = policy_weight(p, row); }
+    soft_whole_row<T, THREADS, ROW_LOADS>(x, V, k, r, s, smem);
+    if (threadIdx.x == 0) policy_row_finish(p, in, row, xt, k, r, s, weight, gscale, s_row, logp, partial);
+    __syncthreads();            // also: every thread is past its reads of the row before it may be overwritten
+    r = s_row[0]; s = s_row[1]; g = s_row[2];
+  } else if (threadIdx.x == 0) {
+    policy_row_skip(row, !valid && t != ignore_index, logp, partial, status);
   }
-  if (threadIdx.x == 0) {
-    double lp = 0.0;
-    PolicyToken o = {0.f, 0.f, 0.f, 0.f};
-    float w = 0.f;
-    if (counted) {
-      lp = row_logp(Elem<T>::get(x + t), k, r, s);
-      o = policy_token(p, row, lp);
-      w = policy_weight(p, row);
-    } else if (t != ignore_index && (t < 0 || t >= V)) {
-      atomicCAS(status, 0, BB_ERR_INVALID_ARG);
-    }
-    s_slope = o.slope * w * gscale;
-    logp[row] = (float)lp;
-    partial[3LL * row] = (double)o.loss * w; partial[3LL * row + 1] = o.kl; partial[3LL * row + 2] = o.clipped;
-  }
-  __syncthreads();            // also: every thread is past its reads of the row before it may be overwritten
-  g = s_slope;
-  grad_row<T, THREADS, ROW_LOADS, CACHE>(x, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, r, s, cache);
+  grad_row<T, THREADS, ROW_LOADS>(x, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, r, s);
 }
 
+// The same for long rows, each read from memory once.  A row lands in shared memory (a ring of stages of 16 bytes per thread that holds
+// one row; bulk copies by a warp of their own), stays there for its gradient, and as that consumes stage after stage the next row
+// follows into them.  Two CTAs per SM fill each other's turns: a row takes a CTA (V = 50257, bf16) about 1.7 us of ex2
+// for the sum and again for the gradient, one between them for the sum's barrier and the token's arithmetic, and an SM's
+// share of the memory rate is a row in 4.5 us.
+constexpr int RING_THREADS = 512, RING_STAGE = RING_THREADS * 16;
+template <typename T>
+__global__ void __launch_bounds__(RING_THREADS + 32, 2)
+policy_ring_kernel(const T* logits, long long ld, const long long* targets, const PolicyParams p, K2 k, float gscale,
+                   T* dlogits, long long ldd, int rows, int V, int cols, long long ignore_index, float* logp, double* partial, int* status, int stages) {
+  constexpr int VEC = Elem<T>::VEC, THREADS = RING_THREADS;
+  extern __shared__ __align__(128) uint4 ring[];
+  __shared__ float2 smem[THREADS / 32];
+  __shared__ float s_row[4];
+  __shared__ int s_abort;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + stages * THREADS);
+  uint64_t* empty = full + stages;
+  volatile int* abort_flag = &s_abort;
+  const int warp = bb::warp_index();
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int j = 0; j < stages; ++j) { bb::mbar_init(&full[j], 1); bb::mbar_init(&empty[j], THREADS / 32); }
+    bb::fence_barrier_init();
+  }
+  __syncthreads();
+  bb::pdl_sync();
+  if (warp == THREADS / 32) {
+    // ---- the warp that loads: stage j of a counted row follows the gradient of the row before it into the same place
+    bool alive = true;
+    uint32_t phase = 0;
+    for (int row = blockIdx.x; row < rows && alive; row += gridDim.x) {
+      const long long t = targets[row];
+      if (t == ignore_index || t < 0 || t >= V || (p.weight && p.weight[row] == 0.f)) continue;
+      const T* x = logits + (size_t)row * ld;
+      const Span<T> sp(x, V);
+      for (int j = 0; j < stages; ++j) {
+        alive = bb::mbar_wait_warp(&empty[j], phase ^ 1, abort_flag, status);
+        if (!alive) break;
+        const int left = sp.nvec - j * THREADS;
+        const int bytes = left <= 0 ? 0 : (left < THREADS ? left : THREADS) * 16;
+        if (bb::elect_one()) {
+          bb::mbar_arrive_expect_tx(&full[j], bytes);
+          if (bytes) bb::bulk_load(ring + j * THREADS, x + sp.lead + (size_t)j * THREADS * VEC, bytes, &full[j]);
+        }
+        __syncwarp();
+      }
+      phase ^= 1;
+    }
+    return;
+  }
+  const float whole_weight = p.weight || threadIdx.x ? 0.f : policy_weight(p, 0);
+  long long t = targets[blockIdx.x];
+  float w = p.weight ? p.weight[blockIdx.x] : 1.f;
+  PolicyInput in = {};
+  if (threadIdx.x == 0) in = policy_input(p, blockIdx.x);
+  bool alive = true;                 // (after a wait that ran out the rows go on without waiting: barriers stay matched)
+  uint32_t phase = 0;
+  for (int row = blockIdx.x; row < rows;) {
+    const int next = row + gridDim.x;
+    long long t_next = ignore_index;
+    float w_next = 1.f;
+    PolicyInput in_next = {};
+    if (next < rows) {               // what the next row's token brings along, a row ahead
+      t_next = targets[next];
+      if (p.weight) w_next = p.weight[next];
+      if (threadIdx.x == 0) in_next = policy_input(p, next);
+    }
+    const T* x = logits + (size_t)row * ld;
+    T* d = dlogits + (size_t)row * ldd;
+    const bool valid = t != ignore_index && t >= 0 && t < V;
+    if (!valid || w == 0.f) {
+      if (threadIdx.x == 0) policy_row_skip(row, !valid && t != ignore_index, logp, partial, status);
+      grad_row<T, THREADS, ROW_LOADS>(x, d, V, cols, 0, 0.f, k, 0.f, 0.f);
+      row = next; t = t_next; w = w_next; in = in_next;
+      continue;
+    }
+    // ---- sum
+    const Span<T> sp(x, V);
+    float xt = threadIdx.x == 0 ? Elem<T>::get(x + t) : 0.f;
+    float r = -INFINITY, s = 0.f;
+    float2 sum = make_float2(0.f, 0.f);
+    for (int j = 0; j < stages; ++j) {
+      if (alive) alive = bb::mbar_wait_warp(&full[j], phase, abort_flag, status);
+      const int c = j * THREADS + threadIdx.x;
+      if (c < sp.nvec) {
+        float f[VEC];
+        Elem<T>::unpack(ring[c], f);
+        if (j == 0) soft_add<VEC>(r, s, f, k);
+        else soft_chunk<VEC>(sum, f, k, r);
+      }
+    }
+    s += sum.x + sum.y;
+    if (!(s < INFINITY)) { const float2 e = soft_share_exact<T, THREADS>(ring, sp.nvec, k); r = e.x; s = e.y; }
+    soft_edges<T, THREADS>(x, sp, V, k, r, s);
+    soft_block<THREADS, true>(r, s, smem);
+    if (threadIdx.x < 32 && isinf(r)) { const float2 e = soft_row_extreme(x, V); r = e.x; s = e.y; }
+    if (threadIdx.x == 0) policy_row_finish(p, in, row, xt, k, r, s, p.weight ? w : whole_weight, gscale, s_row, logp, partial);
+    row_barrier<THREADS, true>();    // also: every thread is past its reads of the row before it may be overwritten
+    r = s_row[0]; s = s_row[1]; xt = s_row[3];
+    float g = s_row[2];
+    if (s == 0.f) g = 0.f;
+    // ---- gradient; a stage is handed back by the warps that have taken their chunks out of it
+    const bool plain = g == 0.f || s < 0.f || (((uintptr_t)x ^ (uintptr_t)d) & 15) != 0;
+    const float ng = plain ? 0.f : -g / s;
+    const int whole = plain ? 0 : (V - sp.lead) / VEC;         // chunks of vocabulary entries only
+    uint4* dv = reinterpret_cast<uint4*>(d + sp.lead);
+    for (int j = 0; j < stages; ++j) {
+      const int c = j * THREADS + threadIdx.x;
+      uint4 q = make_uint4(0, 0, 0, 0);
+      if (c < whole) q = ring[c];
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) bb::mbar_arrive(&empty[j]);
+      if (c < whole) grad_chunk<T>(dv + c, q, k, r, ng);
+    }
+    if (plain) grad_row<T, THREADS, ROW_LOADS>(x, d, V, cols, (int)t, g, k, r, s);
+    else grad_rest<T, THREADS>(x, xt, d, sp.lead, whole, V, cols, (int)t, g, ng, k, r);
+    phase ^= 1;
+    row = next; t = t_next; w = w_next; in = in_next;
+  }
+  if (!alive) {
+    // copies that may still be in flight land before the CTA's shared memory is released (bounded)
+    const uint64_t t0 = bb::globaltimer_ns();
+    while (bb::globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+  }
+}
+
+constexpr int RESCALE_THREADS = 256;
 // A gradient that was made for an upstream gradient of `made_for`, times *grad / made_for: nothing to do where they are the same
 template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS)
+__global__ void __launch_bounds__(RESCALE_THREADS)
 rescale_kernel(T* d, long long ld, int cols, const float* grad, float made_for) {
   constexpr int VEC = Elem<T>::VEC;
   bb::pdl_sync();
@@ -492,14 +675,14 @@ rescale_kernel(T* d, long long ld, int cols, const float* grad, float made_for) 
   T* x = d + (size_t)blockIdx.x * ld;
   const Span<T> sp(x, cols);
   uint4* v = reinterpret_cast<uint4*>(x + sp.lead);
-  for (int i = threadIdx.x; i < sp.nvec; i += ROW_THREADS) {
+  for (int i = threadIdx.x; i < sp.nvec; i += RESCALE_THREADS) {
     float f[VEC];
     Elem<T>::unpack(v[i], f);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) f[e] *= c;
     v[i] = Elem<T>::pack(f);
   }
-  for (int j = threadIdx.x; j < sp.lead + cols - sp.tail; j += ROW_THREADS) {
+  for (int j = threadIdx.x; j < sp.lead + cols - sp.tail; j += RESCALE_THREADS) {
     T* at = x + (j < sp.lead ? j : sp.tail + j - sp.lead);
     Elem<T>::put(at, Elem<T>::get(at) * c);
   }
@@ -731,30 +914,40 @@ bool bad_list(const bb_grad_tensor* list, int count) {
   return false;
 }
 
+template <typename T> struct FwdCall { const T* logits; long long ld; const long long* targets; K2 k; float* logp; float2* stats; int rows, V; long long ignore; int* status; cudaStream_t s; };
+template <typename T, int THREADS> int fwd_rows(const FwdCall<T>& c) {
+  BB_CUDA_CHECK(bb_launch(token_logprob_fwd_kernel<T, THREADS>, c.rows, THREADS, 0, c.s, c.logits, c.ld, c.targets, c.k, c.logp, c.stats, c.V, c.ignore, c.status));
+  return BB_OK;
+}
+template <typename T> int fwd_call(const FwdCall<T>& c) { return fwd_rows<T, 256>(c); }
 int logprob_fwd(const void* logits, int dtype, long long ld, const long long* targets, double scale, float* logp, float* stats, long long rows, int vocab,
                 long long ignore_index, cudaStream_t s) {
   const K2 k = split_k(scale);
   int* status = bb_device_status_word();
-  if (dtype == BB_DTYPE_BF16)
-    BB_CUDA_CHECK(bb_launch(token_logprob_fwd_kernel<__nv_bfloat16>, (int)rows, ROW_THREADS, 0, s, (const __nv_bfloat16*)logits, ld, targets, k, logp,
-                            (float2*)stats, vocab, ignore_index, status));
-  else
-    BB_CUDA_CHECK(bb_launch(token_logprob_fwd_kernel<float>, (int)rows, ROW_THREADS, 0, s, (const float*)logits, ld, targets, k, logp, (float2*)stats, vocab,
-                            ignore_index, status));
+  if (dtype == BB_DTYPE_BF16) return fwd_call<__nv_bfloat16>({(const __nv_bfloat16*)logits, ld, targets, k, logp, (float2*)stats, (int)rows, vocab, ignore_index, status, s});
+  return fwd_call<float>({(const float*)logits, ld, targets, k, logp, (float2*)stats, (int)rows, vocab, ignore_index, status, s});
+}
+
+template <typename T> struct BwdCall {
+  const T* logits; long long ld; const long long* targets; const float2* stats; const float* row_grad; const float* gscale_dev; float gscale; K2 k; T* dlogits;
+  long long ldd; int rows, V, cols; long long ignore; const double* pair_loss; int pairs; float* loss; cudaStream_t s;
+};
+template <typename T, int THREADS> int bwd_rows(const BwdCall<T>& c) {
+  BB_CUDA_CHECK(bb_launch(token_logprob_bwd_kernel<T, THREADS>, c.rows, THREADS, 0, c.s, c.logits, c.ld, c.targets, c.stats, c.row_grad, c.gscale_dev, c.gscale, c.k,
+                          c.dlogits, c.ldd, c.V, c.cols, c.ignore, c.pair_loss, c.pairs, c.loss));
   return BB_OK;
 }
+template <typename T> int bwd_call(const BwdCall<T>& c) { return bwd_rows<T, 256>(c); }
 int logprob_bwd(const void* logits, int dtype, long long ld, const long long* targets, double scale, const float* stats, const float* row_grad,
                 const float* grad_scale_dev, float grad_scale, void* dlogits, long long ldd, long long rows, int vocab, int cols, long long ignore_index,
                 const double* pair_loss, int pairs, float* loss, cudaStream_t s) {
   const K2 k = split_k(scale);
   const float g = (float)(scale * grad_scale);
   if (dtype == BB_DTYPE_BF16)
-    BB_CUDA_CHECK(bb_launch(token_logprob_bwd_kernel<__nv_bfloat16>, (int)rows, ROW_THREADS, 0, s, (const __nv_bfloat16*)logits, ld, targets,
-                            (const float2*)stats, row_grad, grad_scale_dev, g, k, (__nv_bfloat16*)dlogits, ldd, vocab, cols, ignore_index, pair_loss, pairs, loss));
-  else
-    BB_CUDA_CHECK(bb_launch(token_logprob_bwd_kernel<float>, (int)rows, ROW_THREADS, 0, s, (const float*)logits, ld, targets, (const float2*)stats, row_grad,
-                            grad_scale_dev, g, k, (float*)dlogits, ldd, vocab, cols, ignore_index, pair_loss, pairs, loss));
-  return BB_OK;
+    return bwd_call<__nv_bfloat16>({(const __nv_bfloat16*)logits, ld, targets, (const float2*)stats, row_grad, grad_scale_dev, g, k, (__nv_bfloat16*)dlogits, ldd, (int)rows,
+                                    vocab, cols, ignore_index, pair_loss, pairs, loss, s});
+  return bwd_call<float>({(const float*)logits, ld, targets, (const float2*)stats, row_grad, grad_scale_dev, g, k, (float*)dlogits, ldd, (int)rows, vocab, cols, ignore_index,
+                          pair_loss, pairs, loss, s});
 }
 
 }  // namespace
@@ -867,19 +1060,23 @@ struct PolicyRowCall {
   long long ld; const long long* targets; PolicyParams p; K2 k; float gscale; long long ldd; int V, cols; long long ignore_index;
   float* logp; double* partial; int* status; int rows; cudaStream_t stream;
 };
-template <typename T, int THREADS, bool CACHE> int policy_rows_as(const T* logits, T* dlogits, const PolicyRowCall& c, size_t bytes) {
-  if (CACHE)
-    BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(policy_row_kernel<T, THREADS, CACHE>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_CACHE)));
-  BB_CUDA_CHECK(bb_launch(policy_row_kernel<T, THREADS, CACHE>, c.rows, THREADS, CACHE ? bytes : 0, c.stream, logits, c.ld, c.targets, c.p, c.k, c.gscale,
-                          dlogits, c.ldd, c.V, c.cols, c.ignore_index, c.logp, c.partial, c.status));
+template <typename T, int THREADS> int policy_rows_as(const T* logits, T* dlogits, const PolicyRowCall& c) {
+  BB_CUDA_CHECK(bb_launch(policy_row_kernel<T, THREADS>, c.rows, THREADS, 0, c.stream, logits, c.ld, c.targets, c.p, c.k, c.gscale, dlogits, c.ldd, c.rows, c.V, c.cols,
+                          c.ignore_index, c.logp, c.partial, c.status));
   return BB_OK;
 }
-// Threads by how many rows an SM holds at a time
 template <typename T> int policy_rows(const T* logits, T* dlogits, const PolicyRowCall& c) {
-  const size_t bytes = (size_t)c.V * sizeof(T) / 16 * 16;
-  if (bytes > MAX_CACHE) return policy_rows_as<T, 512, false>(logits, dlogits, c, 0);
-  if (bytes > PAIR_CACHE) return policy_rows_as<T, 1024, true>(logits, dlogits, c, bytes);
-  return bytes > 32768 ? policy_rows_as<T, 512, true>(logits, dlogits, c, bytes) : policy_rows_as<T, 256, true>(logits, dlogits, c, bytes);
+  const size_t bytes = (size_t)c.V * sizeof(T);
+  if (bytes <= LONG_ROW) return policy_rows_as<T, 256>(logits, dlogits, c);
+  const int stages = (int)((bytes / 16 + RING_THREADS - 1) / RING_THREADS);
+  const size_t smem = (size_t)stages * (RING_STAGE + 16);
+  if (smem > MAX_RING) return policy_rows_as<T, 512>(logits, dlogits, c);
+  BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(policy_ring_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_RING)));
+  // as many CTAs as the machine holds
+  const int per_sm = smem <= PAIR_RING ? 2 : 1, most = per_sm * bb_num_sms();
+  BB_CUDA_CHECK(bb_launch(policy_ring_kernel<T>, c.rows < most ? c.rows : most, RING_THREADS + 32, smem, c.stream, logits, c.ld, c.targets, c.p, c.k, c.gscale, dlogits,
+                          c.ldd, c.rows, c.V, c.cols, c.ignore_index, c.logp, c.partial, c.status, stages));
+  return BB_OK;
 }
 }  // namespace
 
@@ -937,9 +1134,9 @@ extern "C" int bb_rescale_grad(void* grad, int dtype, long long ld, long long ro
       ((uintptr_t)grad & (dtype == BB_DTYPE_F32 ? 3 : 1)))
     return refuse("bb_rescale_grad: null or misaligned pointer, a size that is not positive, an unknown type, or made_for = 0");
   if (dtype == BB_DTYPE_BF16)
-    BB_CUDA_CHECK(bb_launch(rescale_kernel<__nv_bfloat16>, (int)rows, ROW_THREADS, 0, (cudaStream_t)stream, (__nv_bfloat16*)grad, ld, cols, upstream, made_for));
+    BB_CUDA_CHECK(bb_launch(rescale_kernel<__nv_bfloat16>, (int)rows, RESCALE_THREADS, 0, (cudaStream_t)stream, (__nv_bfloat16*)grad, ld, cols, upstream, made_for));
   else
-    BB_CUDA_CHECK(bb_launch(rescale_kernel<float>, (int)rows, ROW_THREADS, 0, (cudaStream_t)stream, (float*)grad, ld, cols, upstream, made_for));
+    BB_CUDA_CHECK(bb_launch(rescale_kernel<float>, (int)rows, RESCALE_THREADS, 0, (cudaStream_t)stream, (float*)grad, ld, cols, upstream, made_for));
   return BB_OK;
 }
 
