@@ -2,13 +2,16 @@
 // clipped policy loss with a KL term, the global gradient norm over a list of tensors, clipping, and the Adam step that clips.
 // Softmax sums as in softmax2.cuh.
 #include "softmax2.cuh"
+#include <atomic>
 #include <limits.h>
 #include <math.h>
 #include <stdio.h>
 
 namespace {
 
-constexpr int ROW_LOADS = 4;              // 16-byte loads that a thread has in flight
+// 16-byte loads that a thread has in flight.  8192 rows of 50257 bf16 logits: sums 116 us with four (6.7 TB/s), gradient 249 us with four, 245
+// with eight and two thirds of the threads per SM (6.5 TB/s), 252 with two.
+constexpr int ROW_LOADS = 4, GRAD_LOADS = 8;
 constexpr size_t LONG_ROW = 32768;        // bytes from which a row gets more threads
 
 // dynamic shared memory next to a kernel's few static bytes: of one CTA per SM, and of each of two
@@ -181,15 +184,24 @@ __device__ __forceinline__ void soft_whole_row(const T* x, int n, K2 k, float& r
   if (threadIdx.x < 32 && isinf(r)) { const float2 e = soft_row_extreme(x, n); r = e.x; s = e.y; }
 }
 
-// -g softmax of a chunk of logits (ng = -g / s)
-template <typename T> __device__ __forceinline__ void grad_chunk(uint4* d, const uint4& q, K2 k, float r, float ng) {
+// -g softmax_j = ng 2^(k x_j - r).  Here k rounded to 32 bits will do: with what the rounding took at the largest logit (about r / k) in
+// the factor, an entry is off by 1.3e-8 of its distance from the largest, in units of the exponent.
+struct GradRow { float k, r, ng; };
+__device__ __forceinline__ GradRow grad_factors(float g, K2 k, float r, float s) {
+  const float k1 = k.hi + k.lo;
+  return {k1, r, -g / s * ex2(((k.hi - k1) + k.lo) * (r / k1))};
+}
+// The target's entry, g (1 - softmax_t): with the arithmetic of the sum, so that nothing is left of a certain target
+__device__ __forceinline__ float grad_target(float g, float xt, K2 k, float r, float s) { return fmaf(-g / s, ex2(expo(xt, k, r)), g); }
+__device__ __forceinline__ float grad_entry(const GradRow& w, float x) { return w.ng * ex2(fmaf(x, w.k, -w.r)); }
+template <typename T> __device__ __forceinline__ void grad_chunk(uint4* d, const uint4& q, const GradRow& w) {
   constexpr int VEC = Elem<T>::VEC;
   float f[VEC];
   Elem<T>::unpack(q, f);
 #pragma unroll
   for (int i = 0; i < VEC; i += 2) {
-    const float2 e = expo2(make_float2(f[i], f[i + 1]), k, r);
-    const float2 m = bb::mul2(make_float2(ex2(e.x), ex2(e.y)), make_float2(ng, ng));
+    const float2 e = bb::fma2(make_float2(f[i], f[i + 1]), make_float2(w.k, w.k), make_float2(-w.r, -w.r));
+    const float2 m = bb::mul2(make_float2(ex2(e.x), ex2(e.y)), make_float2(w.ng, w.ng));
     f[i] = m.x; f[i + 1] = m.y;
   }
   *d = Elem<T>::pack(f);
@@ -197,15 +209,15 @@ template <typename T> __device__ __forceinline__ void grad_chunk(uint4* d, const
 // What follows the chunks [0, whole): the target's entry (xt its logit, read before d, which may be x, was written; by the thread
 // that wrote its chunk), the chunk that the padding begins in, the padding, and the elements around the 16-byte boundaries
 template <typename T, int THREADS>
-__device__ __forceinline__ void grad_rest(const T* x, float xt, T* d, int lead, int whole, int V, int cols, int t, float g, float ng, K2 k, float r) {
+__device__ __forceinline__ void grad_rest(const T* x, float xt, T* d, int lead, int whole, int V, int cols, int t, float g, K2 k, float s, const GradRow& w) {
   constexpr int VEC = Elem<T>::VEC;
   if (t >= lead) {
     const int tc = (t - lead) / VEC;
-    if (tc < whole && tc % THREADS == (int)threadIdx.x) Elem<T>::put(d + t, ng * ex2(expo(xt, k, r)) + g);
+    if (tc < whole && tc % THREADS == (int)threadIdx.x) Elem<T>::put(d + t, grad_target(g, xt, k, w.r, s));
   }
   auto one = [&](int j) {
     float v = 0.f;
-    if (j < V) { v = ng * ex2(expo(Elem<T>::get(x + j), k, r)); if (j == t) v += g; }
+    if (j < V) { const float f = Elem<T>::get(x + j); v = j == t ? grad_target(g, f, k, w.r, s) : grad_entry(w, f); }
     Elem<T>::put(d + j, v);
   };
   const int nvec = (cols - lead) / VEC, tail = lead + nvec * VEC;
@@ -229,14 +241,14 @@ __device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int 
     for (int j = threadIdx.x; j < sp.lead + cols - sp.tail; j += THREADS) Elem<T>::put(d + (j < sp.lead ? j : sp.tail + j - sp.lead), 0.f);
     return;
   }
-  const float ng = -g / s;
+  const GradRow w = grad_factors(g, k, s < 0.f ? 0.f : r, s);
   if (s < 0.f || (((uintptr_t)x ^ (uintptr_t)d) & 15) != 0) {      // element by element
     for (int j = threadIdx.x; j < cols; j += THREADS) {
       float v = 0.f;
       if (j < V) {
         const float f = Elem<T>::get(x + j);
-        v = s < 0.f ? (f == r ? -ng : 0.f) : ng * ex2(expo(f, k, r));
-        if (j == t) v += g;
+        if (s < 0.f) v = (f == r ? g / s : 0.f) + (j == t ? g : 0.f);
+        else v = j == t ? grad_target(g, f, k, r, s) : grad_entry(w, f);
       }
       Elem<T>::put(d + j, v);
     }
@@ -253,10 +265,10 @@ __device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int 
 #pragma unroll
     for (int u = 0; u < U; ++u) q[u] = xv[c + u * THREADS];
 #pragma unroll
-    for (int u = 0; u < U; ++u) grad_chunk<T>(dv + c + u * THREADS, q[u], k, r, ng);
+    for (int u = 0; u < U; ++u) grad_chunk<T>(dv + c + u * THREADS, q[u], w);
   }
-  for (; c < whole; c += THREADS) grad_chunk<T>(dv + c, xv[c], k, r, ng);
-  grad_rest<T, THREADS>(x, xt, d, sp.lead, whole, V, cols, t, g, ng, k, r);
+  for (; c < whole; c += THREADS) grad_chunk<T>(dv + c, xv[c], w);
+  grad_rest<T, THREADS>(x, xt, d, sp.lead, whole, V, cols, t, g, k, s, w);
 }
 
 // ------------------------------------------------------------------ sums of a block
@@ -294,7 +306,7 @@ token_logprob_fwd_kernel(const T* logits, long long ld, const long long* targets
     if (threadIdx.x == 0) {
       if (t != ignore_index) atomicCAS(status, 0, BB_ERR_INVALID_ARG);
       logp[row] = 0.f;
-      stats[row] = make_float2(0.f, 0.f);
+      if (stats) stats[row] = make_float2(0.f, 0.f);
     }
     return;
   }
@@ -303,12 +315,12 @@ token_logprob_fwd_kernel(const T* logits, long long ld, const long long* targets
   soft_whole_row<T, THREADS, ROW_LOADS>(x, V, k, r, s, smem);
   if (threadIdx.x == 0) {
     logp[row] = (float)row_logp(Elem<T>::get(x + t), k, r, s);
-    stats[row] = make_float2(r, s);
+    if (stats) stats[row] = make_float2(r, s);
   }
 }
 
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 4)
 token_logprob_bwd_kernel(const T* logits, long long ld, const long long* targets, const float2* stats, const float* row_grad,
                          const float* gscale_dev, float gscale, K2 k, T* dlogits, long long ldd, int V, int cols,
                          long long ignore_index, const double* pair_loss, int pairs, float* loss) {
@@ -319,7 +331,7 @@ token_logprob_bwd_kernel(const T* logits, long long ld, const long long* targets
   const float2 st = stats[row];
   const bool counted = t != ignore_index && t >= 0 && t < V;
   const float g = counted ? row_grad[row] * (gscale_dev ? gscale_dev[0] : 1.f) * gscale : 0.f;
-  grad_row<T, THREADS, ROW_LOADS>(logits + (size_t)row * ld, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, st.x, st.y);
+  grad_row<T, THREADS, GRAD_LOADS>(logits + (size_t)row * ld, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, st.x, st.y);
 }
 
 // Tokens [a, b) of sequence q: rows of `seq_len` tokens, or between two offsets.  Offsets that do not ascend within [0, tokens]
@@ -442,6 +454,19 @@ __device__ __forceinline__ PolicyToken policy_token(const PolicyParams& p, const
   return o;
 }
 
+// The slope alone, from a row's softmax sums, in 32 bits: what the row kernels wait for between their halves (a log-probability in 64
+// bits takes a thousand cycles; 32 bits put 5e-7 on the ratio)
+__device__ __forceinline__ float policy_slope(const PolicyParams& p, const PolicyInput& in, float xt, K2 k, float r, float s) {
+  float lp;
+  if (s > 0.f) lp = (expo(xt, k, r) - log2f(s)) * 0.693147181f;
+  else lp = (float)row_logp(xt, k, r, s);
+  const float ratio = p.old_logp ? expf(lp - in.old) : 1.f;
+  const float plain = in.adv == 0.f ? 0.f : ratio * in.adv, bounded = fminf(fmaxf(ratio, p.low), p.high) * in.adv;
+  float slope = bounded < plain ? 0.f : -plain;
+  if (p.ref) slope -= p.kl_coef * expm1f(in.ref - lp);
+  return slope;
+}
+
 // Counted tokens of each of `gridDim.x` pieces of the targets (sequences, or equal pieces when weight is NULL) and, per sequence,
 // the weight 1 / (sequences * counted) of its tokens
 __global__ void __launch_bounds__(256)
@@ -460,6 +485,8 @@ policy_count_kernel(const long long* targets, const long long* offsets, long lon
   for (long long i = a + threadIdx.x; i < b; i += 256) count += targets[i] != ignore_index;
   const double n = block_sum<256>((double)count, smem);
   if (threadIdx.x == 0) counts[blockIdx.x] = (int)n;
+  // rows drawn by policy_ring_kernel, CTAs of policy_token_kernel that are done
+  if (threadIdx.x == 0 && blockIdx.x == 0) counts[gridDim.x] = counts[gridDim.x + 1] = 0;
   if (!weight) return;
   const float w = (float)(1.0 / ((double)gridDim.x * (n > 1.0 ? n : 1.0)));
   for (long long i = a + threadIdx.x; i < b; i += 256) weight[i] = w;
@@ -473,38 +500,62 @@ __device__ __forceinline__ float policy_weight(const PolicyParams& p, long long 
   return (float)(1.0 / (n > 1.0 ? n : 1.0));
 }
 
-// Token by token: row_grad, and the sums of a CTA's tokens: weighted loss, KL, clipped
+// Token by token: row_grad (from log-probabilities), or the log-probability (from rows: the softmax sums and the target's logit that a row
+// kernel left; a row with sums of 0 and a logit of 0 does not count).  The sums of a CTA's tokens - weighted loss, KL, clipped -
+// meet in the CTA that finishes last, in the order of the CTAs: loss[0], and stats = mean KL and share of clipped among counted tokens.
+struct PolicyRow { float r, s, xt, counts; };
+template <bool FROM_ROWS>
 __global__ void __launch_bounds__(256)
-policy_token_kernel(const float* logp, const long long* targets, const PolicyParams p, long long tokens, long long ignore_index,
-                    float* row_grad, double* partial) {
+policy_token_kernel(float* logp, const PolicyRow* row_sums, K2 k, const long long* targets, const PolicyParams p, long long tokens, long long ignore_index,
+                    float* row_grad, double* partial, int* done, float* loss, float* stats) {
   __shared__ double smem[8];
+  __shared__ int s_last;
   bb::pdl_sync();
-  double loss = 0.0, kl = 0.0, clipped = 0.0;
+  double v[3] = {0.0, 0.0, 0.0};
   const float whole = p.weight ? 0.f : policy_weight(p, 0);
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < tokens; i += (long long)gridDim.x * 256) {
     const float w = p.weight ? p.weight[i] : whole;
-    if (targets[i] == ignore_index || w == 0.f) { row_grad[i] = 0.f; continue; }
-    const PolicyToken o = policy_token(p, policy_input(p, i), (double)logp[i]);
-    row_grad[i] = o.slope * w;
-    loss += (double)o.loss * w; kl += o.kl; clipped += o.clipped;
+    double lp;
+    if constexpr (FROM_ROWS) {
+      const PolicyRow q = row_sums[i];
+      if (q.counts == 0.f) { logp[i] = 0.f; continue; }
+      lp = row_logp(q.xt, k, q.r, q.s);
+      logp[i] = (float)lp;
+    } else {
+      if (targets[i] == ignore_index || w == 0.f) { row_grad[i] = 0.f; continue; }
+      lp = (double)logp[i];
+    }
+    const PolicyToken o = policy_token(p, policy_input(p, i), lp);
+    if constexpr (!FROM_ROWS) row_grad[i] = o.slope * w;
+    v[0] += (double)o.loss * w; v[1] += o.kl; v[2] += o.clipped;
   }
-  loss = block_sum<256>(loss, smem); kl = block_sum<256>(kl, smem); clipped = block_sum<256>(clipped, smem);
-  if (threadIdx.x == 0) { partial[3 * blockIdx.x] = loss; partial[3 * blockIdx.x + 1] = kl; partial[3 * blockIdx.x + 2] = clipped; }
+  for (int c = 0; c < 3; ++c) v[c] = block_sum<256>(v[c], smem);
+  if (threadIdx.x == 0) {
+    for (int c = 0; c < 3; ++c) __stcg(partial + 3 * blockIdx.x + c, v[c]);
+    __threadfence();
+    s_last = atomicAdd(done, 1) == (int)gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  for (int c = 0; c < 3; ++c) v[c] = 0.0;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += 256)
+    for (int c = 0; c < 3; ++c) v[c] += __ldcg(partial + 3 * i + c);
+  double total = 0.0;
+  for (int i = threadIdx.x; i < p.num_counts; i += 256) total += (double)p.counts[i];
+  for (int c = 0; c < 3; ++c) v[c] = block_sum<256>(v[c], smem);
+  total = block_sum<256>(total, smem);
+  if (threadIdx.x == 0) {
+    if (total < 1.0) total = 1.0;
+    loss[0] = (float)v[0]; stats[0] = (float)(v[1] / total); stats[1] = (float)(v[2] / total);
+  }
 }
 
-// What thread 0 does between the two halves of a row
+// What thread 0 does between the two halves of a row; the token's loss follows in policy_token_kernel
 __device__ __forceinline__ void policy_row_finish(const PolicyParams& p, const PolicyInput& in, int row, float xt, K2 k, float r, float s, float weight, float gscale,
-                                                  float* s_row, float* logp, double* partial) {
-  const double lp = row_logp(xt, k, r, s);
-  const PolicyToken o = policy_token(p, in, lp);
-  s_row[0] = r; s_row[1] = s; s_row[2] = o.slope * weight * gscale; s_row[3] = xt;
-  logp[row] = (float)lp;
-  partial[3LL * row] = (double)o.loss * weight; partial[3LL * row + 1] = o.kl; partial[3LL * row + 2] = o.clipped;
-}
-__device__ __forceinline__ void policy_row_skip(int row, bool bad, float* logp, double* partial, int* status) {
-  if (bad) atomicCAS(status, 0, BB_ERR_INVALID_ARG);
-  logp[row] = 0.f;
-  partial[3LL * row] = 0.0; partial[3LL * row + 1] = 0.0; partial[3LL * row + 2] = 0.0;
+                                                  float* s_row, PolicyRow* row_sums) {
+  s_row[0] = r; s_row[1] = s; s_row[2] = policy_slope(p, in, xt, k, r, s) * weight * gscale;
+  row_sums[row] = {r, s, xt, 1.f};
 }
 
 // One CTA per row of logits: log-probability, the token's loss and, because a row's gradient needs nothing of the other rows (the
@@ -513,9 +564,9 @@ __device__ __forceinline__ void policy_row_skip(int row, bool bad, float* logp, 
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS)
 policy_row_kernel(const T* logits, long long ld, const long long* targets, const PolicyParams p, K2 k, float gscale,
-                  T* dlogits, long long ldd, int rows, int V, int cols, long long ignore_index, float* logp, double* partial, int* status) {
+                  T* dlogits, long long ldd, int rows, int V, int cols, long long ignore_index, PolicyRow* row_sums, int* status) {
   __shared__ float2 smem[THREADS / 32];
-  __shared__ float s_row[4];
+  __shared__ float s_row[3];
   bb::pdl_sync();
   const int row = blockIdx.x;
   const long long t = targets[row];
@@ -528,104 +579,140 @@ policy_row_kernel(const T* logits, long long ld, const long long* targets, const
     float xt = 0.f, weight = 0.f;
     if (threadIdx.x == 0) { in = policy_input(p, row); xt = Elem<T>::get(x + t); weight = policy_weight(p, row); }
     soft_whole_row<T, THREADS, ROW_LOADS>(x, V, k, r, s, smem);
-    if (threadIdx.x == 0) policy_row_finish(p, in, row, xt, k, r, s, weight, gscale, s_row, logp, partial);
+    if (threadIdx.x == 0) policy_row_finish(p, in, row, xt, k, r, s, weight, gscale, s_row, row_sums);
     __syncthreads();            // also: every thread is past its reads of the row before it may be overwritten
     r = s_row[0]; s = s_row[1]; g = s_row[2];
   } else if (threadIdx.x == 0) {
-    policy_row_skip(row, !valid && t != ignore_index, logp, partial, status);
+    if (!valid && t != ignore_index) atomicCAS(status, 0, BB_ERR_INVALID_ARG);
+    row_sums[row] = {0.f, 0.f, 0.f, 0.f};
   }
   grad_row<T, THREADS, ROW_LOADS>(x, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, r, s);
 }
 
-// The same for long rows, each read from memory once.  A row lands in shared memory (a ring of stages of 16 bytes per thread that holds
-// one row; bulk copies by a warp of their own), stays there for its gradient, and as that consumes stage after stage the next row
+// What the feeding warp of policy_ring_kernel hands over with a row; row < 0: no more
+struct PolicyTurn { int row, t; PolicyInput in; float weight, xt; };
+constexpr int TURNS = 4;
+
+// The same for long rows, each read from memory once.  A row lands in shared memory (a ring of stages of four chunks per thread that
+// holds one row; bulk copies by a warp of their own), stays there for its gradient, and as that consumes stage after stage the next row
 // follows into them.  Two CTAs per SM fill each other's turns: a row takes a CTA (V = 50257, bf16) about 1.7 us of ex2
 // for the sum and again for the gradient, one between them for the sum's barrier and the token's arithmetic, and an SM's
-// share of the memory rate is a row in 4.5 us.
-constexpr int RING_THREADS = 512, RING_STAGE = RING_THREADS * 16;
+// share of the memory rate is a row in 4.5 us.  Rows that do not count cost a CTA a fraction of the others and come in
+// runs (prompts), so rows are drawn from a counter.
+constexpr int RING_THREADS = 512, RING_CHUNKS = 4, RING_STAGE = RING_THREADS * RING_CHUNKS * 16, RING_STAGES = (int)(MAX_RING + RING_STAGE - 1) / RING_STAGE;
 template <typename T>
 __global__ void __launch_bounds__(RING_THREADS + 32, 2)
 policy_ring_kernel(const T* logits, long long ld, const long long* targets, const PolicyParams p, K2 k, float gscale,
-                   T* dlogits, long long ldd, int rows, int V, int cols, long long ignore_index, float* logp, double* partial, int* status, int stages) {
-  constexpr int VEC = Elem<T>::VEC, THREADS = RING_THREADS;
+                   T* dlogits, long long ldd, int rows, int V, int cols, long long ignore_index, PolicyRow* row_sums, int* status, int stages, int* ticket) {
+  constexpr int VEC = Elem<T>::VEC, THREADS = RING_THREADS, U = RING_CHUNKS, STAGE = THREADS * U;
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ float2 smem[THREADS / 32];
-  __shared__ float s_row[4];
-  __shared__ int s_abort;
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + stages * THREADS);
-  uint64_t* empty = full + stages;
+  __shared__ float s_row[3];
+  __shared__ PolicyTurn turns[TURNS];
+  __shared__ uint64_t turn_full[TURNS], turn_empty[TURNS];
+  __shared__ int s_abort, s_dead;
+  __shared__ uint64_t full[RING_STAGES], empty[RING_STAGES];
   volatile int* abort_flag = &s_abort;
-  const int warp = bb::warp_index();
+  const int warp = bb::warp_index(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    s_abort = 0;
+    s_abort = s_dead = 0;
     for (int j = 0; j < stages; ++j) { bb::mbar_init(&full[j], 1); bb::mbar_init(&empty[j], THREADS / 32); }
+    for (int j = 0; j < TURNS; ++j) { bb::mbar_init(&turn_full[j], 1); bb::mbar_init(&turn_empty[j], THREADS / 32); }
     bb::fence_barrier_init();
   }
   __syncthreads();
   bb::pdl_sync();
   if (warp == THREADS / 32) {
-    // ---- the warp that loads: stage j of a counted row follows the gradient of the row before it into the same place
+    // ---- the warp that feeds: draws rows, fetches what their tokens bring along, and lets the chunks of a counted row follow the gradient
+    // of the row before it into the same places
+    const float whole = p.weight ? 0.f : policy_weight(p, 0);
     bool alive = true;
     uint32_t phase = 0;
-    for (int row = blockIdx.x; row < rows && alive; row += gridDim.x) {
-      const long long t = targets[row];
-      if (t == ignore_index || t < 0 || t >= V || (p.weight && p.weight[row] == 0.f)) continue;
-      const T* x = logits + (size_t)row * ld;
-      const Span<T> sp(x, V);
-      for (int j = 0; j < stages; ++j) {
-        alive = bb::mbar_wait_warp(&empty[j], phase ^ 1, abort_flag, status);
-        if (!alive) break;
-        const int left = sp.nvec - j * THREADS;
-        const int bytes = left <= 0 ? 0 : (left < THREADS ? left : THREADS) * 16;
-        if (bb::elect_one()) {
-          bb::mbar_arrive_expect_tx(&full[j], bytes);
-          if (bytes) bb::bulk_load(ring + j * THREADS, x + sp.lead + (size_t)j * THREADS * VEC, bytes, &full[j]);
-        }
-        __syncwarp();
+    int row = blockIdx.x;
+    for (int it = 0; alive; ++it) {
+      const bool more = row < rows;
+      // (the next draw is under way while this row's copies are issued)
+      const int drawn = more && lane == 0 ? (int)gridDim.x + atomicAdd(ticket, 1) : 0;
+      PolicyTurn turn = {-1, -1, {}, 0.f, 0.f};
+      const T* x = logits;
+      if (more) {
+        x += (size_t)row * ld;
+        const long long t = targets[row];
+        const bool valid = t != ignore_index && t >= 0 && t < V;
+        turn.row = row;
+        turn.weight = p.weight ? p.weight[row] : whole;
+        turn.in = policy_input(p, row);
+        if (valid && turn.weight != 0.f) { turn.t = (int)t; turn.xt = Elem<T>::get(x + t); }
+        if (!valid && t != ignore_index && lane == 0) atomicCAS(status, 0, BB_ERR_INVALID_ARG);
       }
-      phase ^= 1;
+      const int at = it % TURNS;
+      alive = bb::mbar_wait_warp(&turn_empty[at], ((it / TURNS) & 1) ^ 1, abort_flag, status);
+      if (!alive) break;
+      if (lane == 0) { turns[at] = turn; bb::mbar_arrive(&turn_full[at]); }
+      __syncwarp();
+      if (!more) break;
+      if (turn.t >= 0) {
+        const Span<T> sp(x, V);
+        for (int j = 0; j < stages; ++j) {
+          alive = bb::mbar_wait_warp(&empty[j], phase ^ 1, abort_flag, status);
+          if (!alive) break;
+          const int left = (sp.nvec - j * STAGE) * 16, bytes = left <= 0 ? 0 : left < RING_STAGE ? left : RING_STAGE;
+          if (bb::elect_one()) {
+            bb::mbar_arrive_expect_tx(&full[j], bytes);
+            if (bytes) bb::bulk_load(ring + j * STAGE, x + sp.lead + (size_t)j * STAGE * VEC, bytes, &full[j]);
+          }
+          __syncwarp();
+        }
+        phase ^= 1;
+      }
+      row = __shfl_sync(0xffffffffu, drawn, 0);
     }
     return;
   }
-  const float whole_weight = p.weight || threadIdx.x ? 0.f : policy_weight(p, 0);
-  long long t = targets[blockIdx.x];
-  float w = p.weight ? p.weight[blockIdx.x] : 1.f;
-  PolicyInput in = {};
-  if (threadIdx.x == 0) in = policy_input(p, blockIdx.x);
-  bool alive = true;                 // (after a wait that ran out the rows go on without waiting: barriers stay matched)
+  bool alive = true;
   uint32_t phase = 0;
-  for (int row = blockIdx.x; row < rows;) {
-    const int next = row + gridDim.x;
-    long long t_next = ignore_index;
-    float w_next = 1.f;
-    PolicyInput in_next = {};
-    if (next < rows) {               // what the next row's token brings along, a row ahead
-      t_next = targets[next];
-      if (p.weight) w_next = p.weight[next];
-      if (threadIdx.x == 0) in_next = policy_input(p, next);
-    }
+  for (int it = 0;; ++it) {
+    const int at = it % TURNS;
+    alive = alive && bb::mbar_wait_warp(&turn_full[at], (it / TURNS) & 1, abort_flag, status);
+    const PolicyTurn turn = turns[at];
+    __syncwarp();
+    if (lane == 0) bb::mbar_arrive(&turn_empty[at]);
+    const int row = turn.row, t = turn.t;
+    // a wait that ran out in one warp ends the loop for all of them here, where their barriers match
+    if (!alive) s_dead = 1;
+    row_barrier<THREADS, true>();
+    if (s_dead || row < 0) break;
     const T* x = logits + (size_t)row * ld;
     T* d = dlogits + (size_t)row * ldd;
-    const bool valid = t != ignore_index && t >= 0 && t < V;
-    if (!valid || w == 0.f) {
-      if (threadIdx.x == 0) policy_row_skip(row, !valid && t != ignore_index, logp, partial, status);
+    if (t < 0) {
+      if (threadIdx.x == 0) row_sums[row] = {0.f, 0.f, 0.f, 0.f};
       grad_row<T, THREADS, ROW_LOADS>(x, d, V, cols, 0, 0.f, k, 0.f, 0.f);
-      row = next; t = t_next; w = w_next; in = in_next;
       continue;
     }
     // ---- sum
     const Span<T> sp(x, V);
-    float xt = threadIdx.x == 0 ? Elem<T>::get(x + t) : 0.f;
+    const float xt = turn.xt;
     float r = -INFINITY, s = 0.f;
     float2 sum = make_float2(0.f, 0.f);
     for (int j = 0; j < stages; ++j) {
       if (alive) alive = bb::mbar_wait_warp(&full[j], phase, abort_flag, status);
-      const int c = j * THREADS + threadIdx.x;
-      if (c < sp.nvec) {
-        float f[VEC];
-        Elem<T>::unpack(ring[c], f);
-        if (j == 0) soft_add<VEC>(r, s, f, k);
-        else soft_chunk<VEC>(sum, f, k, r);
+      const int c = j * STAGE + threadIdx.x;
+      float f[VEC];
+      if (c + (U - 1) * THREADS < sp.nvec) {
+        uint4 q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u] = ring[c + u * THREADS];
+        if (j == 0) { Elem<T>::unpack(q[0], f); soft_add<VEC>(r, s, f, k); }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u > 0 || j > 0) { Elem<T>::unpack(q[u], f); soft_chunk<VEC>(sum, f, k, r); }
+      } else {
+        for (int u = 0; u < U; ++u) {
+          if (c + u * THREADS >= sp.nvec) break;
+          Elem<T>::unpack(ring[c + u * THREADS], f);
+          if (j == 0 && u == 0) soft_add<VEC>(r, s, f, k);
+          else soft_chunk<VEC>(sum, f, k, r);
+        }
       }
     }
     s += sum.x + sum.y;
@@ -633,28 +720,29 @@ policy_ring_kernel(const T* logits, long long ld, const long long* targets, cons
     soft_edges<T, THREADS>(x, sp, V, k, r, s);
     soft_block<THREADS, true>(r, s, smem);
     if (threadIdx.x < 32 && isinf(r)) { const float2 e = soft_row_extreme(x, V); r = e.x; s = e.y; }
-    if (threadIdx.x == 0) policy_row_finish(p, in, row, xt, k, r, s, p.weight ? w : whole_weight, gscale, s_row, logp, partial);
+    if (threadIdx.x == 0) policy_row_finish(p, turn.in, row, xt, k, r, s, turn.weight, gscale, s_row, row_sums);
     row_barrier<THREADS, true>();    // also: every thread is past its reads of the row before it may be overwritten
-    r = s_row[0]; s = s_row[1]; xt = s_row[3];
+    r = s_row[0]; s = s_row[1];
     float g = s_row[2];
     if (s == 0.f) g = 0.f;
     // ---- gradient; a stage is handed back by the warps that have taken their chunks out of it
     const bool plain = g == 0.f || s < 0.f || (((uintptr_t)x ^ (uintptr_t)d) & 15) != 0;
-    const float ng = plain ? 0.f : -g / s;
+    const GradRow gw = grad_factors(g, k, plain ? 0.f : r, s);
     const int whole = plain ? 0 : (V - sp.lead) / VEC;         // chunks of vocabulary entries only
     uint4* dv = reinterpret_cast<uint4*>(d + sp.lead);
     for (int j = 0; j < stages; ++j) {
-      const int c = j * THREADS + threadIdx.x;
-      uint4 q = make_uint4(0, 0, 0, 0);
-      if (c < whole) q = ring[c];
+      const int c = j * STAGE + threadIdx.x;
+      uint4 q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) q[u] = c + u * THREADS < whole ? ring[c + u * THREADS] : make_uint4(0, 0, 0, 0);
       __syncwarp();
-      if ((threadIdx.x & 31) == 0) bb::mbar_arrive(&empty[j]);
-      if (c < whole) grad_chunk<T>(dv + c, q, k, r, ng);
+      if (lane == 0) bb::mbar_arrive(&empty[j]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) if (c + u * THREADS < whole) grad_chunk<T>(dv + c + u * THREADS, q[u], gw);
     }
-    if (plain) grad_row<T, THREADS, ROW_LOADS>(x, d, V, cols, (int)t, g, k, r, s);
-    else grad_rest<T, THREADS>(x, xt, d, sp.lead, whole, V, cols, (int)t, g, ng, k, r);
+    if (plain) grad_row<T, THREADS, ROW_LOADS>(x, d, V, cols, t, g, k, r, s);
+    else grad_rest<T, THREADS>(x, xt, d, sp.lead, whole, V, cols, t, g, k, s, gw);
     phase ^= 1;
-    row = next; t = t_next; w = w_next; in = in_next;
   }
   if (!alive) {
     // copies that may still be in flight land before the CTA's shared memory is released (bounded)
@@ -688,27 +776,13 @@ rescale_kernel(T* d, long long ld, int cols, const float* grad, float made_for) 
   }
 }
 
-// loss[0] = sum of the weighted losses; stats = mean KL and share of clipped among counted tokens
-__global__ void __launch_bounds__(1024)
-policy_finish_kernel(const double* partial, long long n, const int* counts, int num_counts, float* loss, float* stats) {
-  __shared__ double smem[32];
-  bb::pdl_sync();
-  double v[3] = {0.0, 0.0, 0.0};
-  for (long long i = threadIdx.x; i < n; i += 1024)
-    for (int c = 0; c < 3; ++c) v[c] += partial[3 * i + c];
-  double total = 0.0;
-  for (int i = threadIdx.x; i < num_counts; i += 1024) total += (double)counts[i];
-  for (int c = 0; c < 3; ++c) v[c] = block_sum<1024>(v[c], smem);
-  total = block_sum<1024>(total, smem);
-  if (threadIdx.x == 0) {
-    if (total < 1.0) total = 1.0;
-    loss[0] = (float)v[0]; stats[0] = (float)(v[1] / total); stats[1] = (float)(v[2] / total);
-  }
-}
-
 // ------------------------------------------------------------------ gradient norm, clipping
 constexpr int LIST_TENSORS = 128;             // tensors of one launch: their table travels as a kernel argument
-constexpr int NORM_THREADS = 512;
+// Both passes deal the list out in small pieces, most of them one per CTA: a CTA that walks a grid's share of a large list keeps
+// fewer requests in flight between its pieces.  153 M bf16 values: sum 52 us (5.9 TB/s), scaling 93 us (6.6 TB/s) in pieces of 16384
+// elements, 108 in pieces of 8192 or with four CTAs per SM that walk.
+constexpr int NORM_THREADS = 512, NORM_LOADS = 4, NORM_CTAS = 8192;
+constexpr long long SUM_PIECE = 32768, CLIP_PIECE = 16384;
 struct TensorTable {
   void* data[LIST_TENSORS];
   long long numel[LIST_TENSORS];
@@ -729,18 +803,30 @@ __device__ __forceinline__ int table_find(const TensorTable& t, int piece, long 
   return lo;
 }
 
-template <typename T> __device__ __forceinline__ double sumsq_piece(const T* x, int n) {
+template <typename T> __device__ __forceinline__ float sumsq_chunk(const uint4& q) {
   constexpr int VEC = Elem<T>::VEC;
+  float f[VEC];
+  float2 sum = make_float2(0.f, 0.f);
+  Elem<T>::unpack(q, f);
+#pragma unroll
+  for (int i = 0; i < VEC; i += 2) sum = bb::fma2(make_float2(f[i], f[i + 1]), make_float2(f[i], f[i + 1]), sum);
+  return sum.x + sum.y;
+}
+// (a chunk's squares in 32 bits, everything above in 64)
+template <typename T> __device__ __forceinline__ double sumsq_piece(const T* x, int n) {
+  constexpr int U = NORM_LOADS;
   const Span<T> sp(x, n);
   const uint4* v = reinterpret_cast<const uint4*>(x + sp.lead);
   double sum = 0.0;
-  for (int c = threadIdx.x; c < sp.nvec; c += NORM_THREADS) {
-    float f[VEC], q = 0.f;
-    Elem<T>::unpack(v[c], f);
+  int c = threadIdx.x;
+  for (; c + (U - 1) * NORM_THREADS < sp.nvec; c += U * NORM_THREADS) {
+    uint4 q[U];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) q = fmaf(f[i], f[i], q);
-    sum += (double)q;
+    for (int u = 0; u < U; ++u) q[u] = v[c + u * NORM_THREADS];
+#pragma unroll
+    for (int u = 0; u < U; ++u) sum += (double)sumsq_chunk<T>(q[u]);
   }
+  for (; c < sp.nvec; c += NORM_THREADS) sum += (double)sumsq_chunk<T>(v[c]);
   for (int j = threadIdx.x; j < sp.lead + n - sp.tail; j += NORM_THREADS) {
     const float f = Elem<T>::get(x + (j < sp.lead ? j : sp.tail + j - sp.lead));
     sum += (double)(f * f);
@@ -748,10 +834,12 @@ template <typename T> __device__ __forceinline__ double sumsq_piece(const T* x, 
   return sum;
 }
 
-// partial[blockIdx.x] = sum of squares of the CTA's pieces (every gridDim.x-th), in a fixed order
+// total[0] (+)= sum of squares of the list: every CTA sums its pieces (each gridDim.x-th), the CTA that finishes last adds the CTAs' sums in
+// their order.  `done` returns to zero by itself.
 __global__ void __launch_bounds__(NORM_THREADS)
-grad_sumsq_kernel(const __grid_constant__ TensorTable t, double* partial) {
+grad_sumsq_kernel(const __grid_constant__ TensorTable t, double* partial, double* total, int add, unsigned int* done) {
   __shared__ double smem[NORM_THREADS / 32];
+  __shared__ int s_last;
   bb::pdl_sync();
   double sum = 0.0;
   for (int piece = blockIdx.x; piece < t.first[t.count]; piece += gridDim.x) {
@@ -761,81 +849,106 @@ grad_sumsq_kernel(const __grid_constant__ TensorTable t, double* partial) {
                                       : sumsq_piece(reinterpret_cast<const __nv_bfloat16*>(t.data[i]) + a, (int)n);
   }
   sum = block_sum<NORM_THREADS>(sum, smem);
-  if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+  if (threadIdx.x == 0) {
+    __stcg(partial + blockIdx.x, sum);
+    __threadfence();
+    s_last = atomicInc(done, gridDim.x - 1) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  sum = 0.0;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += NORM_THREADS) sum += __ldcg(partial + i);
+  sum = block_sum<NORM_THREADS>(sum, smem);
+  if (threadIdx.x == 0) total[0] = add ? total[0] + sum : sum;
 }
 
-// norm = pre_scale * sqrt(sum of partials); min(1, max_norm / (norm + 1e-6)), NaN for a NaN norm
-template <int THREADS> __device__ __forceinline__ float clip_coef(const double* partial, int n, double pre_scale, double max_norm, double* smem,
-                                                                 float* norm_out) {
-  double sum = 0.0;
-  for (int i = threadIdx.x; i < n; i += THREADS) sum += partial[i];
-  const double norm = pre_scale * sqrt(block_sum<THREADS>(sum, smem));
-  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = (float)norm;
-  const double coef = max_norm / (norm + 1e-6);
-  return coef >= 1.0 ? 1.f : (float)coef;
+// norm = pre_scale * sqrt(sum of squares); min(1, max_norm / (norm + 1e-6)), NaN for a NaN norm
+__device__ __forceinline__ float clip_coef(const double* sumsq, double pre_scale, double max_norm, float* norm_out) {
+  __shared__ float s_coef;
+  if (threadIdx.x == 0) {
+    const double norm = pre_scale * sqrt(sumsq[0]), coef = max_norm / (norm + 1e-6);
+    if (blockIdx.x == 0) norm_out[0] = (float)norm;
+    s_coef = coef >= 1.0 ? 1.f : (float)coef;
+  }
+  __syncthreads();
+  return s_coef;
 }
 
-template <typename T> __device__ __forceinline__ void scale_piece(T* x, int n, float c) {
+template <typename T> __device__ __forceinline__ uint4 scale_chunk(const uint4& q, float c) {
   constexpr int VEC = Elem<T>::VEC;
+  float f[VEC];
+  Elem<T>::unpack(q, f);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) f[e] *= c;
+  return Elem<T>::pack(f);
+}
+template <typename T> __device__ __forceinline__ void scale_piece(T* x, int n, float c) {
+  constexpr int U = NORM_LOADS;
   const Span<T> sp(x, n);
   uint4* v = reinterpret_cast<uint4*>(x + sp.lead);
-  for (int i = threadIdx.x; i < sp.nvec; i += NORM_THREADS) {
-    float f[VEC];
-    Elem<T>::unpack(v[i], f);
+  int i = threadIdx.x;
+  for (; i + (U - 1) * NORM_THREADS < sp.nvec; i += U * NORM_THREADS) {
+    uint4 q[U];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] *= c;
-    v[i] = Elem<T>::pack(f);
+    for (int u = 0; u < U; ++u) q[u] = v[i + u * NORM_THREADS];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[i + u * NORM_THREADS] = scale_chunk<T>(q[u], c);
   }
+  for (; i < sp.nvec; i += NORM_THREADS) v[i] = scale_chunk<T>(v[i], c);
   for (int j = threadIdx.x; j < sp.lead + n - sp.tail; j += NORM_THREADS) {
     T* p = x + (j < sp.lead ? j : sp.tail + j - sp.lead);
     Elem<T>::put(p, Elem<T>::get(p) * c);
   }
 }
 
+// One piece per CTA
 __global__ void __launch_bounds__(NORM_THREADS)
-grad_clip_kernel(const __grid_constant__ TensorTable t, const double* partial, int num_partials, double max_norm, float* norm_out) {
-  __shared__ double smem[NORM_THREADS / 32];
+grad_clip_kernel(const __grid_constant__ TensorTable t, const double* sumsq, double max_norm, float* norm_out) {
   bb::pdl_sync();
-  const float c = clip_coef<NORM_THREADS>(partial, num_partials, 1.0, max_norm, smem, norm_out);
+  const float c = clip_coef(sumsq, 1.0, max_norm, norm_out);
   if (c == 1.f) return;                         // within the norm: the gradients stay as they are
-  for (int piece = blockIdx.x; piece < t.first[t.count]; piece += gridDim.x) {
-    long long a, n;
-    const int i = table_find(t, piece, a, n);
-    if (t.dtype[i] == BB_DTYPE_F32) scale_piece(reinterpret_cast<float*>(t.data[i]) + a, (int)n, c);
-    else scale_piece(reinterpret_cast<__nv_bfloat16*>(t.data[i]) + a, (int)n, c);
-  }
+  long long a, n;
+  // last pieces first: the sum read them last, and what of them is still in L2 need not come from memory again (sum and scaling of
+  // those 153 M values 156 -> 153 us)
+  const int i = table_find(t, gridDim.x - 1 - blockIdx.x, a, n);
+  if (t.dtype[i] == BB_DTYPE_F32) scale_piece(reinterpret_cast<float*>(t.data[i]) + a, (int)n, c);
+  else scale_piece(reinterpret_cast<__nv_bfloat16*>(t.data[i]) + a, (int)n, c);
 }
 
-// Adam on the clipped gradient; what the host can fold is folded there in 64 bits (1 - beta, bias corrections)
+// Adam on the clipped gradient; what the host can fold is folded there in 64 bits (1 - beta, bias corrections).  102.9 M parameters:
+// 513 us at 6.8 TB/s (34 bytes each) with four elements per thread and CTAs of 256, which all come and go; 590 us in CTAs that
+// walk, six per SM.
 struct AdamParams { float lr, b1, omb1, b2, omb2, eps, inv_bc1, inv_bc2, decay; int decoupled, zero_grad; };
 
 __global__ void __launch_bounds__(256)
-adam_clip_kernel(float* p, float* g, float* m, float* v, __nv_bfloat16* lp, long long n, const AdamParams a, const double* partial,
-                 int num_partials, double pre_scale, double max_norm, float* norm_out) {
-  __shared__ double smem[8];
+adam_clip_kernel(float* p, float* g, float* m, float* v, __nv_bfloat16* lp, long long n, const AdamParams a, const double* sumsq,
+                 double pre_scale, double max_norm, float* norm_out) {
   bb::pdl_sync();
-  const float c = clip_coef<256>(partial, num_partials, pre_scale, max_norm, smem, norm_out) * (float)pre_scale;
-  const long long n4 = n >> 2, stride = (long long)gridDim.x * 256;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n4; i += stride) {
-    const float4 P = reinterpret_cast<float4*>(p)[i], G = reinterpret_cast<float4*>(g)[i];
-    const float4 M = reinterpret_cast<float4*>(m)[i], W = reinterpret_cast<float4*>(v)[i];
-    float pp[4] = {P.x, P.y, P.z, P.w}, gg[4] = {G.x, G.y, G.z, G.w}, mm[4] = {M.x, M.y, M.z, M.w}, vv[4] = {W.x, W.y, W.z, W.w};
+  // four elements per thread, last ones first (see grad_clip_kernel)
+  const long long i = (gridDim.x - 1 - blockIdx.x) * 256LL + threadIdx.x;
+  const bool some = i < n >> 2;
+  const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4 P = some ? reinterpret_cast<float4*>(p)[i] : none, G = some ? reinterpret_cast<float4*>(g)[i] : none;
+  const float4 M = some ? reinterpret_cast<float4*>(m)[i] : none, W = some ? reinterpret_cast<float4*>(v)[i] : none;
+  float pp[4] = {P.x, P.y, P.z, P.w}, gg[4] = {G.x, G.y, G.z, G.w}, mm[4] = {M.x, M.y, M.z, M.w}, vv[4] = {W.x, W.y, W.z, W.w};
+  const float c = clip_coef(sumsq, pre_scale, max_norm, norm_out) * (float)pre_scale;
+  if (!some) return;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float x = gg[e] * c;
-      if (!a.decoupled) x = fmaf(a.decay, pp[e], x);
-      mm[e] = fmaf(a.b1, mm[e], a.omb1 * x);
-      vv[e] = fmaf(a.b2, vv[e], a.omb2 * x * x);
-      float step = (mm[e] * a.inv_bc1) / (sqrtf(vv[e] * a.inv_bc2) + a.eps);
-      if (a.decoupled) step = fmaf(a.decay, pp[e], step);
-      pp[e] = fmaf(-a.lr, step, pp[e]);
-    }
-    reinterpret_cast<float4*>(p)[i] = make_float4(pp[0], pp[1], pp[2], pp[3]);
-    reinterpret_cast<float4*>(m)[i] = make_float4(mm[0], mm[1], mm[2], mm[3]);
-    reinterpret_cast<float4*>(v)[i] = make_float4(vv[0], vv[1], vv[2], vv[3]);
-    if (a.zero_grad) reinterpret_cast<float4*>(g)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (lp) reinterpret_cast<uint2*>(lp)[i] = make_uint2(bb::pack_bf16x2(pp[0], pp[1]), bb::pack_bf16x2(pp[2], pp[3]));
+  for (int e = 0; e < 4; ++e) {
+    float x = gg[e] * c;
+    if (!a.decoupled) x = fmaf(a.decay, pp[e], x);
+    mm[e] = fmaf(a.b1, mm[e], a.omb1 * x);
+    vv[e] = fmaf(a.b2, vv[e], a.omb2 * x * x);
+    float step = (mm[e] * a.inv_bc1) / (sqrtf(vv[e] * a.inv_bc2) + a.eps);
+    if (a.decoupled) step = fmaf(a.decay, pp[e], step);
+    pp[e] = fmaf(-a.lr, step, pp[e]);
   }
+  reinterpret_cast<float4*>(p)[i] = make_float4(pp[0], pp[1], pp[2], pp[3]);
+  reinterpret_cast<float4*>(m)[i] = make_float4(mm[0], mm[1], mm[2], mm[3]);
+  reinterpret_cast<float4*>(v)[i] = make_float4(vv[0], vv[1], vv[2], vv[3]);
+  if (a.zero_grad) reinterpret_cast<float4*>(g)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (lp) reinterpret_cast<uint2*>(lp)[i] = make_uint2(bb::pack_bf16x2(pp[0], pp[1]), bb::pack_bf16x2(pp[2], pp[3]));
 }
 
 // ------------------------------------------------------------------ host side
@@ -863,33 +976,29 @@ bool bad_output(const void* logits, long long ld, const void* dlogits, long long
 int refuse(const char* msg) { bb_set_last_error_msg(msg); return BB_ERR_INVALID_ARG; }
 
 // counts of counted tokens, and the weights of the sequence reduction; both at the front of the workspace
-struct PolicyPlan { int num_counts; long long piece; size_t weight_at, partial_at, logp_at, bytes; };
-PolicyPlan policy_plan(long long tokens, int n_seq, int by_sequence, long long partials, bool logp) {
+struct PolicyPlan { int num_counts; long long piece; size_t weight_at, rows_at, partial_at, bytes; };
+int policy_token_ctas(long long tokens) {
+  const long long want = (tokens + 255) / 256, cap = 4LL * bb_num_sms();
+  return (int)(want < cap ? want : cap);
+}
+PolicyPlan policy_plan(long long tokens, int n_seq, bool by_sequence) {
   PolicyPlan pl;
   // (64 pieces at most: every CTA of the next kernel adds them up)
   pl.piece = (tokens + 63) / 64 > 2048 ? (tokens + 63) / 64 : 2048;
   pl.num_counts = by_sequence ? n_seq : (int)((tokens + pl.piece - 1) / pl.piece);
-  size_t at = ((size_t)pl.num_counts * 4 + 15) & ~(size_t)15;
+  size_t at = ((size_t)(pl.num_counts + 2) * 4 + 15) & ~(size_t)15;       // (two more: counters)
   pl.weight_at = at; at += by_sequence ? (size_t)tokens * 4 : 0;
   at = (at + 15) & ~(size_t)15;
-  pl.logp_at = at; at += logp ? (size_t)tokens * 4 : 0;
-  at = (at + 15) & ~(size_t)15;
-  pl.partial_at = at; at += (size_t)partials * 24;
+  pl.rows_at = at; at += (size_t)tokens * sizeof(PolicyRow);
+  pl.partial_at = at; at += (size_t)policy_token_ctas(tokens) * 24;
   pl.bytes = at;
   return pl;
 }
-int policy_token_ctas(long long tokens) {
-  const long long want = (tokens + 1023) / 1024, cap = 4LL * bb_num_sms();
-  return (int)(want < cap ? want : cap);
-}
-
-// Pieces of the list's tensors dealt over the machine: enough for every SM, none below 4096 elements
-int table_fill(TensorTable& t, const bb_grad_tensor* list, int count) {
+// The list's tensors in pieces of `piece` elements, more where there would be too many
+int table_fill(TensorTable& t, const bb_grad_tensor* list, int count, long long piece) {
   long long total = 0;
   for (int i = 0; i < count; ++i) total += list[i].numel;
-  long long piece = (total / (4LL * bb_num_sms()) + 4095) / 4096 * 4096;
-  piece = piece < 4096 ? 4096 : piece > 65536 ? 65536 : piece;
-  while (total / piece + count > INT_MAX / 2) piece *= 2;
+  while (total / piece + count > (1 << 24)) piece *= 2;
   t.piece = (int)piece;
   t.count = count;
   int pieces = 0;
@@ -901,7 +1010,29 @@ int table_fill(TensorTable& t, const bb_grad_tensor* list, int count) {
   t.first[count] = pieces;
   return pieces;
 }
-int norm_ctas() { return 4 * bb_num_sms(); }
+// Pieces of the sum: enough for every SM, none below 4096 elements
+long long sum_piece(const bb_grad_tensor* list, int count) {
+  long long total = 0;
+  for (int i = 0; i < count; ++i) total += list[i].numel;
+  const long long piece = (total / (4LL * bb_num_sms()) + 4095) / 4096 * 4096;
+  return piece < 4096 ? 4096 : piece > SUM_PIECE ? SUM_PIECE : piece;
+}
+
+// Counters of the CTAs that are done, one per launch in turn; each is zero again when its launch is over
+constexpr unsigned DONE_SLOTS = 1u << 12;
+__device__ unsigned int g_norm_done[DONE_SLOTS];
+unsigned int* norm_done() {
+  static unsigned int* table[64] = {nullptr};
+  static std::atomic<unsigned> next{0};
+  const int dev = bb_current_device();
+  if (dev < 0) return nullptr;
+  if (!table[dev]) {
+    void* ptr = nullptr;
+    if (cudaGetSymbolAddress(&ptr, g_norm_done) != cudaSuccess) return nullptr;
+    table[dev] = static_cast<unsigned int*>(ptr);
+  }
+  return table[dev] + next.fetch_add(1u) % DONE_SLOTS;
+}
 
 bool bad_list(const bb_grad_tensor* list, int count) {
   if (!list || count <= 0) return true;
@@ -955,7 +1086,7 @@ int logprob_bwd(const void* logits, int dtype, long long ld, const long long* ta
 extern "C" int bb_token_logprob_fwd(const void* logits, int dtype, long long ld, const long long* targets, double scale, float* logp,
                                     float* stats, long long rows, int vocab, long long ignore_index, void* stream) {
   if (bad_logits("bb_token_logprob_fwd", logits, dtype, ld, targets, rows, vocab, scale)) return BB_ERR_INVALID_ARG;
-  if (!logp || !stats || ((uintptr_t)stats & 7)) return refuse("bb_token_logprob_fwd: logp and stats (8-byte aligned) are needed");
+  if (!logp || ((uintptr_t)stats & 7)) return refuse("bb_token_logprob_fwd: logp is needed, and stats 8-byte aligned");
   return logprob_fwd(logits, dtype, ld, targets, scale, logp, stats, rows, vocab, ignore_index, (cudaStream_t)stream);
 }
 
@@ -1058,32 +1189,39 @@ int policy_front(const bb_policy_desc* d, const PolicyPlan& pl, const long long*
 namespace {
 struct PolicyRowCall {
   long long ld; const long long* targets; PolicyParams p; K2 k; float gscale; long long ldd; int V, cols; long long ignore_index;
-  float* logp; double* partial; int* status; int rows; cudaStream_t stream;
+  PolicyRow* row_sums; int* status; int rows; int* ticket; cudaStream_t stream;
 };
 template <typename T, int THREADS> int policy_rows_as(const T* logits, T* dlogits, const PolicyRowCall& c) {
   BB_CUDA_CHECK(bb_launch(policy_row_kernel<T, THREADS>, c.rows, THREADS, 0, c.stream, logits, c.ld, c.targets, c.p, c.k, c.gscale, dlogits, c.ldd, c.rows, c.V, c.cols,
-                          c.ignore_index, c.logp, c.partial, c.status));
+                          c.ignore_index, c.row_sums, c.status));
   return BB_OK;
 }
 template <typename T> int policy_rows(const T* logits, T* dlogits, const PolicyRowCall& c) {
   const size_t bytes = (size_t)c.V * sizeof(T);
   if (bytes <= LONG_ROW) return policy_rows_as<T, 256>(logits, dlogits, c);
-  const int stages = (int)((bytes / 16 + RING_THREADS - 1) / RING_THREADS);
-  const size_t smem = (size_t)stages * (RING_STAGE + 16);
+  const size_t smem = bytes / 16 * 16;
+  const int stages = (int)((smem + RING_STAGE - 1) / RING_STAGE);
   if (smem > MAX_RING) return policy_rows_as<T, 512>(logits, dlogits, c);
   BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(policy_ring_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_RING)));
   // as many CTAs as the machine holds
   const int per_sm = smem <= PAIR_RING ? 2 : 1, most = per_sm * bb_num_sms();
   BB_CUDA_CHECK(bb_launch(policy_ring_kernel<T>, c.rows < most ? c.rows : most, RING_THREADS + 32, smem, c.stream, logits, c.ld, c.targets, c.p, c.k, c.gscale, dlogits,
-                          c.ldd, c.rows, c.V, c.cols, c.ignore_index, c.logp, c.partial, c.status, stages));
+                          c.ldd, c.rows, c.V, c.cols, c.ignore_index, c.row_sums, c.status, stages, c.ticket));
+  return BB_OK;
+}
+template <bool FROM_ROWS>
+int policy_tokens(const bb_policy_desc* d, const PolicyPlan& pl, float* logp, K2 k, const long long* targets, const PolicyParams& p, float* row_grad, float* loss,
+                  float* stats, void* workspace, cudaStream_t s) {
+  char* ws = (char*)workspace;
+  BB_CUDA_CHECK(bb_launch(policy_token_kernel<FROM_ROWS>, policy_token_ctas(d->tokens), 256, 0, s, logp, (const PolicyRow*)(ws + pl.rows_at), k, targets, p, d->tokens,
+                          d->ignore_index, row_grad, (double*)(ws + pl.partial_at), (int*)ws + pl.num_counts + 1, loss, stats));
   return BB_OK;
 }
 }  // namespace
 
 extern "C" long long bb_policy_workspace_bytes(const bb_policy_desc* d) {
   if (!d || d->tokens <= 0 || d->sequences <= 0) return -1;
-  const long long partials = d->tokens > policy_token_ctas(d->tokens) ? d->tokens : policy_token_ctas(d->tokens);
-  return (long long)policy_plan(d->tokens, d->sequences, d->reduction == BB_POLICY_SEQUENCE, partials, true).bytes;
+  return (long long)policy_plan(d->tokens, d->sequences, d->reduction == BB_POLICY_SEQUENCE).bytes;
 }
 
 extern "C" int bb_policy_loss(const bb_policy_desc* d, const float* logp, const float* old_logp, const float* advantages, const float* ref,
@@ -1093,15 +1231,11 @@ extern "C" int bb_policy_loss(const bb_policy_desc* d, const float* logp, const 
   if (!logp || !row_grad) return refuse("bb_policy_loss: logp and row_grad are needed");
   if (workspace_bytes < bb_policy_workspace_bytes(d)) return refuse("bb_policy_loss: workspace smaller than bb_policy_workspace_bytes()");
   cudaStream_t s = (cudaStream_t)stream;
-  const int ctas = policy_token_ctas(d->tokens);
-  const PolicyPlan pl = policy_plan(d->tokens, d->sequences, d->reduction == BB_POLICY_SEQUENCE, ctas, false);
-  double* partial = (double*)((char*)workspace + pl.partial_at);
+  const PolicyPlan pl = policy_plan(d->tokens, d->sequences, d->reduction == BB_POLICY_SEQUENCE);
   PolicyParams p;
   BackToBack overlap;
   if (int rc = policy_front(d, pl, targets, offsets, old_logp, advantages, ref, workspace, p, s)) return rc;
-  BB_CUDA_CHECK(bb_launch(policy_token_kernel, ctas, 256, 0, s, logp, targets, p, d->tokens, d->ignore_index, row_grad, partial));
-  BB_CUDA_CHECK(bb_launch(policy_finish_kernel, 1, 1024, 0, s, (const double*)partial, (long long)ctas, p.counts, p.num_counts, loss, stats));
-  return BB_OK;
+  return policy_tokens<false>(d, pl, const_cast<float*>(logp), K2{}, targets, p, row_grad, loss, stats, workspace, s);
 }
 
 extern "C" int bb_policy_loss_logits(const bb_policy_desc* d, const void* logits, int dtype, long long ld, double scale, int vocab, int cols,
@@ -1114,19 +1248,17 @@ extern "C" int bb_policy_loss_logits(const bb_policy_desc* d, const void* logits
     return refuse("bb_policy_loss_logits: null pointer, columns that do not cover the vocabulary, or a gradient that overlaps the logits without being in place");
   if (workspace_bytes < bb_policy_workspace_bytes(d)) return refuse("bb_policy_loss_logits: workspace smaller than bb_policy_workspace_bytes()");
   cudaStream_t s = (cudaStream_t)stream;
-  const PolicyPlan pl = policy_plan(d->tokens, d->sequences, d->reduction == BB_POLICY_SEQUENCE, d->tokens, false);
-  double* partial = (double*)((char*)workspace + pl.partial_at);
+  const PolicyPlan pl = policy_plan(d->tokens, d->sequences, d->reduction == BB_POLICY_SEQUENCE);
   const K2 k = split_k(scale);
   const float g = (float)(scale * grad_scale);
   int* status = bb_device_status_word();
   PolicyParams p;
   BackToBack overlap;
   if (int rc = policy_front(d, pl, targets, offsets, old_logp, advantages, ref, workspace, p, s)) return rc;
-  const PolicyRowCall c = {ld, targets, p, k, g, ldd, vocab, cols, d->ignore_index, logp, partial, status, (int)d->tokens, s};
+  const PolicyRowCall c = {ld, targets, p, k, g, ldd, vocab, cols, d->ignore_index, (PolicyRow*)((char*)workspace + pl.rows_at), status, (int)d->tokens, (int*)workspace + pl.num_counts, s};
   if (int rc = dtype == BB_DTYPE_BF16 ? policy_rows((const __nv_bfloat16*)logits, (__nv_bfloat16*)dlogits, c) : policy_rows((const float*)logits, (float*)dlogits, c))
     return rc;
-  BB_CUDA_CHECK(bb_launch(policy_finish_kernel, 1, 1024, 0, s, (const double*)partial, d->tokens, p.counts, p.num_counts, loss, stats));
-  return BB_OK;
+  return policy_tokens<true>(d, pl, logp, k, targets, p, nullptr, loss, stats, workspace, s);
 }
 
 extern "C" int bb_rescale_grad(void* grad, int dtype, long long ld, long long rows, int cols, const float* upstream, float made_for, void* stream) {
@@ -1140,56 +1272,68 @@ extern "C" int bb_rescale_grad(void* grad, int dtype, long long ld, long long ro
   return BB_OK;
 }
 
-extern "C" int bb_grad_norm_partials(int count) { return count > 0 ? (count + LIST_TENSORS - 1) / LIST_TENSORS * norm_ctas() : 0; }
+extern "C" long long bb_grad_norm_workspace_bytes(void) { return 8LL * (1 + NORM_CTAS); }
 
-extern "C" int bb_grad_sumsq(const bb_grad_tensor* tensors, int count, double* partials, void* stream) {
-  if (bad_list(tensors, count) || !partials) return refuse("bb_grad_sumsq: null pointer, an empty tensor, or a type other than bf16 and fp32");
+namespace {
+// Sum of squares of the list into the workspace's first value
+int list_sumsq(const bb_grad_tensor* tensors, int count, double* workspace, cudaStream_t s) {
   for (int at = 0; at < count; at += LIST_TENSORS) {
+    const int n = count - at < LIST_TENSORS ? count - at : LIST_TENSORS;
     TensorTable t;
-    table_fill(t, tensors + at, count - at < LIST_TENSORS ? count - at : LIST_TENSORS);
-    BB_CUDA_CHECK(bb_launch(grad_sumsq_kernel, norm_ctas(), NORM_THREADS, 0, (cudaStream_t)stream, t, partials + (long long)(at / LIST_TENSORS) * norm_ctas()));
+    const int pieces = table_fill(t, tensors + at, n, sum_piece(tensors + at, n));
+    unsigned int* done = norm_done();
+    if (!done) { bb_set_last_error_msg("bb_grad_sumsq: counters unavailable on this device"); return BB_ERR_CUDA; }
+    BB_CUDA_CHECK(bb_launch(grad_sumsq_kernel, pieces < NORM_CTAS ? pieces : NORM_CTAS, NORM_THREADS, 0, s, t, workspace + 1, workspace, at > 0 ? 1 : 0, done));
   }
   return BB_OK;
 }
+bool bad_workspace(const void* workspace, long long bytes) { return !workspace || ((uintptr_t)workspace & 7) || bytes < bb_grad_norm_workspace_bytes(); }
+}  // namespace
 
-extern "C" int bb_grad_clip(const bb_grad_tensor* tensors, int count, double* partials, int num_partials, double max_norm, float* norm,
-                            void* stream) {
-  if (bad_list(tensors, count) || !partials || num_partials < 0 || !norm || !(max_norm > 0.0))
-    return refuse("bb_grad_clip: null pointer, an empty tensor, a type other than bf16 and fp32, or a norm that is not positive");
+extern "C" int bb_grad_sumsq(const bb_grad_tensor* tensors, int count, void* workspace, long long workspace_bytes, void* stream) {
+  if (bad_list(tensors, count) || bad_workspace(workspace, workspace_bytes))
+    return refuse("bb_grad_sumsq: an empty tensor, a type other than bf16 and fp32, or a workspace smaller than bb_grad_norm_workspace_bytes()");
+  return list_sumsq(tensors, count, (double*)workspace, (cudaStream_t)stream);
+}
+
+extern "C" int bb_grad_clip(const bb_grad_tensor* tensors, int count, const double* sumsq, double max_norm, float* norm, void* workspace,
+                            long long workspace_bytes, void* stream) {
+  if (bad_list(tensors, count) || !norm || !(max_norm > 0.0) || (!sumsq && bad_workspace(workspace, workspace_bytes)))
+    return refuse("bb_grad_clip: an empty tensor, a type other than bf16 and fp32, a norm that is not positive, or a workspace that is too small");
   BackToBack overlap;
-  if (num_partials == 0) {
-    if (int rc = bb_grad_sumsq(tensors, count, partials, stream)) return rc;
-    num_partials = bb_grad_norm_partials(count);
+  if (!sumsq) {
+    if (int rc = list_sumsq(tensors, count, (double*)workspace, (cudaStream_t)stream)) return rc;
+    sumsq = (const double*)workspace;
   }
   for (int at = 0; at < count; at += LIST_TENSORS) {
     TensorTable t;
-    const int pieces = table_fill(t, tensors + at, count - at < LIST_TENSORS ? count - at : LIST_TENSORS);
-    const int grid = pieces < norm_ctas() ? pieces : norm_ctas();
-    BB_CUDA_CHECK(bb_launch(grad_clip_kernel, grid, NORM_THREADS, 0, (cudaStream_t)stream, t, (const double*)partials, num_partials, max_norm, norm));
+    const int pieces = table_fill(t, tensors + at, count - at < LIST_TENSORS ? count - at : LIST_TENSORS, CLIP_PIECE);
+    BB_CUDA_CHECK(bb_launch(grad_clip_kernel, pieces, NORM_THREADS, 0, (cudaStream_t)stream, t, sumsq, max_norm, norm));
   }
   return BB_OK;
 }
 
 extern "C" int bb_adam_step_clipped(float* master, float* grad, float* exp_avg, float* exp_avg_sq, void* param_bf16, long long n, double lr,
                                     double beta1, double beta2, double eps, int step, int adam_w_mode, int bias_correction,
-                                    double weight_decay, double grad_scale, int zero_grad, double* partials, int num_partials,
-                                    double max_norm, float* norm, void* stream) {
-  if (!master || !grad || !exp_avg || !exp_avg_sq || n <= 0 || (n & 3) || step < 1 || !partials || num_partials < 0 || !norm || !(max_norm > 0.0) ||
+                                    double weight_decay, double grad_scale, int zero_grad, const double* sumsq, double max_norm,
+                                    float* norm, void* workspace, long long workspace_bytes, void* stream) {
+  if (!master || !grad || !exp_avg || !exp_avg_sq || n <= 0 || (n & 3) || step < 1 || (!sumsq && bad_workspace(workspace, workspace_bytes)) || !norm || !(max_norm > 0.0) ||
       (((uintptr_t)master | (uintptr_t)grad | (uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & 15) || ((uintptr_t)param_bf16 & 7))
-    return refuse("bb_adam_step_clipped: null or unaligned pointer, n not a multiple of 4, step < 1, or a norm that is not positive");
+    return refuse("bb_adam_step_clipped: null or unaligned pointer, n not a multiple of 4, step < 1, a norm that is not positive, or a workspace that is too small");
   AdamParams a;
   a.lr = (float)lr; a.b1 = (float)beta1; a.omb1 = (float)(1.0 - beta1); a.b2 = (float)beta2; a.omb2 = (float)(1.0 - beta2); a.eps = (float)eps;
   a.inv_bc1 = bias_correction ? (float)(1.0 / (1.0 - pow(beta1, step))) : 1.f;
   a.inv_bc2 = bias_correction ? (float)(1.0 / (1.0 - pow(beta2, step))) : 1.f;
   a.decay = (float)weight_decay; a.decoupled = adam_w_mode ? 1 : 0; a.zero_grad = zero_grad;
   BackToBack overlap;
-  if (num_partials == 0) {
+  if (!sumsq) {
     const bb_grad_tensor t = {grad, n, BB_DTYPE_F32};
-    if (int rc = bb_grad_sumsq(&t, 1, partials, stream)) return rc;
-    num_partials = bb_grad_norm_partials(1);
+    if (int rc = list_sumsq(&t, 1, (double*)workspace, (cudaStream_t)stream)) return rc;
+    sumsq = (const double*)workspace;
   }
-  const long long want = ((n >> 2) + 255) / 256, cap = 8LL * bb_num_sms();
-  BB_CUDA_CHECK(bb_launch(adam_clip_kernel, (int)(want < cap ? want : cap), 256, 0, (cudaStream_t)stream, master, grad, exp_avg, exp_avg_sq,
-                          (__nv_bfloat16*)param_bf16, n, a, (const double*)partials, num_partials, grad_scale, max_norm, norm));
+  const long long ctas = ((n >> 2) + 255) / 256;
+  if (ctas > INT_MAX) return refuse("bb_adam_step_clipped: more elements than one launch covers");
+  BB_CUDA_CHECK(bb_launch(adam_clip_kernel, (int)ctas, 256, 0, (cudaStream_t)stream, master, grad, exp_avg, exp_avg_sq, (__nv_bfloat16*)param_bf16, n, a, sumsq,
+                          grad_scale, max_norm, norm));
   return BB_OK;
 }

@@ -145,9 +145,10 @@ def load():
         lib.bb_head_logprob_fwd.argtypes = [vp] * 7 + [ll, vp]
         lib.bb_head_logprob_grad.argtypes = [vp] * 7 + [f, i, i, vp, ll, vp]
         lib.bb_rescale_grad.argtypes = [vp, i, ll, ll, i, vp, f, vp]
-        lib.bb_grad_sumsq.argtypes = [vp, i, vp, vp]
-        lib.bb_grad_clip.argtypes = [vp, i, vp, i, d, vp, vp]
-        lib.bb_adam_step_clipped.argtypes = [vp] * 5 + [ll, d, d, d, d, i, i, i, d, d, i, vp, i, d, vp, vp]
+        lib.bb_grad_norm_workspace_bytes.restype = ll
+        lib.bb_grad_sumsq.argtypes = [vp, i, vp, ll, vp]
+        lib.bb_grad_clip.argtypes = [vp, i, vp, d, vp, vp, ll, vp]
+        lib.bb_adam_step_clipped.argtypes = [vp] * 5 + [ll, d, d, d, d, i, i, i, d, d, i, vp, d, vp, vp, ll, vp]
         _lib = lib
     return _lib
 
@@ -584,21 +585,33 @@ def conv_bn_bwd(desc, x, y, z, mean, rstd, dz, dx, dres, scratch, residual=True,
 
 
 # ---------------------------------------------------------------------------- post-training
+class _DtypeCodes(dict):
+    """torch.dtype -> BB_DTYPE_*, filled when first asked (this module does not import torch by itself)."""
+
+    def get(self, key, default=None):
+        if not self:
+            import torch
+            self.update({torch.bfloat16: 0, torch.float32: 1})
+        return dict.get(self, key, default)
+
+
+DTYPE_CODES = _DtypeCodes()
+
+
 def _dtype(t, what):
-    import torch
-    if t.dtype == torch.bfloat16:
-        return 0
-    if t.dtype == torch.float32:
-        return 1
-    raise BambooNativeError(f"{what}: bf16 or fp32 expected, got {t.dtype}")
+    code = DTYPE_CODES.get(t.dtype)
+    if code is None:
+        raise BambooNativeError(f"{what}: bf16 or fp32 expected, got {t.dtype}")
+    return code
 
 
 def token_logprob_fwd(logits, targets, logp, stats, vocab, scale=1.0, ignore_index=-100):
-    """logits: [rows, cols] bf16 / fp32, unit inner stride; targets [rows] int64; logp [rows], stats [rows, 2] fp32."""
+    """logits: [rows, cols] bf16 / fp32, unit inner stride; targets [rows] int64; logp [rows], stats [rows, 2] fp32 (None:
+    no backward pass follows)."""
     global LAUNCHES
     LAUNCHES += 1
     check(load().bb_token_logprob_fwd(logits.data_ptr(), _dtype(logits, "logits"), logits.stride(0), targets.data_ptr(), scale, logp.data_ptr(),
-                                      stats.data_ptr(), logits.shape[0], vocab, ignore_index, _raw_stream()), "bb_token_logprob_fwd")
+                                      _addr(stats), logits.shape[0], vocab, ignore_index, _raw_stream()), "bb_token_logprob_fwd")
     return logp
 
 
@@ -656,7 +669,7 @@ def preference_loss_logits(desc, logits, targets, vocab, ref, offsets, loss, rew
 
 def policy_loss(desc, logp, old_logp, advantages, ref, targets, offsets, loss, stats, row_grad):
     global LAUNCHES
-    LAUNCHES += 3
+    LAUNCHES += 2
     lib = load()
     ws = workspace(max(0, lib.bb_policy_workspace_bytes(ctypes.byref(desc))), "post_training")
     check(lib.bb_policy_loss(ctypes.byref(desc), logp.data_ptr(), _addr(old_logp), advantages.data_ptr(), _addr(ref), targets.data_ptr(),
@@ -692,39 +705,47 @@ def _tensor_table(n):
     return struct.Struct("QqiI" * n)        # bb_grad_tensor[n]
 
 
-def grad_tensors(tensors):
-    """bb_grad_tensor[len(tensors)]: every tensor fills its memory without gaps."""
-    flat = []
-    for t in tensors:
-        flat += (t.data_ptr(), t.numel(), _dtype(t, "gradient"), 0)
-    return _tensor_table(len(tensors)).pack(*flat)
+def grad_tensors(fields):
+    """bb_grad_tensor[] from (address, elements, type, 0) of every tensor, one after the other."""
+    return _tensor_table(len(fields) // 4).pack(*fields)
 
 
-def grad_norm_partials(count):
-    return load().bb_grad_norm_partials(count)
+_norm_bytes = None
 
 
-def grad_sumsq(table, count, partials):
-    """Partial sums of squares of a list (``grad_tensors``) into ``partials`` (fp64, ``grad_norm_partials(count)`` values)."""
+def grad_norm_workspace():
+    global _norm_bytes
+    if _norm_bytes is None:
+        _norm_bytes = load().bb_grad_norm_workspace_bytes()
+    return workspace(_norm_bytes, "grad_norm")
+
+
+def grad_sumsq(table, count):
+    """Sum of squares of a list (``grad_tensors``): fp64 [1], in scratch that the next call on this stream overwrites."""
     global LAUNCHES
     LAUNCHES += (count + 127) // 128
-    check(load().bb_grad_sumsq(table, count, _addr(partials), _raw_stream()), "bb_grad_sumsq")
+    ws = grad_norm_workspace()
+    check(load().bb_grad_sumsq(table, count, ws.data_ptr(), ws.numel(), _raw_stream()), "bb_grad_sumsq")
+    import torch
+    return ws[:8].view(torch.float64)
 
 
-def grad_clip(table, count, partials, max_norm, norm, num_partials=0):
-    """``num_partials`` 0: the norm is over this list, and made by this call (``partials``: room for it)."""
+def grad_clip(table, count, max_norm, norm, sumsq=None):
+    """``sumsq`` (fp64 [1], device): what the norm is over; None: this list."""
     global LAUNCHES
-    LAUNCHES += (count + 127) // 128 * (1 if num_partials else 2)
-    check(load().bb_grad_clip(table, count, _addr(partials), num_partials, max_norm, norm.data_ptr(), _raw_stream()), "bb_grad_clip")
+    LAUNCHES += (count + 127) // 128 * (1 if sumsq is not None else 2)
+    ws = grad_norm_workspace()
+    check(load().bb_grad_clip(table, count, _addr(sumsq), max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream()), "bb_grad_clip")
     return norm
 
 
 def adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, *, lr, beta1=0.9, beta2=0.999, eps=1e-8, step, adam_w_mode=True,
-                      bias_correction=True, weight_decay=0.0, grad_scale=1.0, zero_grad=True, partials, num_partials=0, max_norm, norm):
-    """``num_partials`` 0: the norm is over ``grad``, and made by this call (``partials``: room for ``grad_norm_partials(1)`` values)."""
+                      bias_correction=True, weight_decay=0.0, grad_scale=1.0, zero_grad=True, max_norm, norm, sumsq=None):
+    """``sumsq`` (fp64 [1], device): what the norm is over, before ``grad_scale``; None: ``grad``."""
     global LAUNCHES
-    LAUNCHES += 1 if num_partials else 2
+    LAUNCHES += 1 if sumsq is not None else 2
+    ws = grad_norm_workspace()
     check(load().bb_adam_step_clipped(master.data_ptr(), grad.data_ptr(), exp_avg.data_ptr(), exp_avg_sq.data_ptr(), _addr(param_lp), master.numel(),
                                       lr, beta1, beta2, eps, step, int(adam_w_mode), int(bias_correction), weight_decay, grad_scale, int(zero_grad),
-                                      _addr(partials), num_partials, max_norm, norm.data_ptr(), _raw_stream()), "bb_adam_step_clipped")
+                                      _addr(sumsq), max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream()), "bb_adam_step_clipped")
     return norm

@@ -30,7 +30,7 @@ def _rows(logits, vocab):
     vocab = cols if vocab is None else vocab
     if not 0 < vocab <= cols:
         raise ValueError(f"vocab {vocab} does not fit logits with {cols} columns")
-    lg = logits.detach().reshape(-1, cols)
+    lg = logits.detach() if logits.dim() == 2 else logits.detach().reshape(-1, cols)
     if lg.stride(1) != 1 or (lg.shape[0] > 1 and lg.stride(0) < cols):
         lg = lg.contiguous()
     return lg, vocab
@@ -74,10 +74,12 @@ def _wants_grad(t):
 
 
 # ----------------------------------------------------------------------------------- token log-probabilities
-def _logprobs(lg, tg, vocab, scale, ignore_index):
-    logp = torch.empty(lg.shape[0], dtype=torch.float32, device=lg.device)
-    stats = torch.empty(lg.shape[0], 2, dtype=torch.float32, device=lg.device)
-    if lg.shape[0]:
+def _logprobs(lg, tg, vocab, scale, ignore_index, shape=None, keep=True):
+    """(log-probabilities, softmax sums for the backward pass unless ``keep`` is off)"""
+    rows = lg.shape[0]
+    logp = torch.empty(rows if shape is None else shape, dtype=torch.float32, device=lg.device)
+    stats = torch.empty(rows, 2, dtype=torch.float32, device=lg.device) if keep else None
+    if rows:
         L.token_logprob_fwd(lg, tg, logp, stats, vocab, scale, ignore_index)
     return logp, stats
 
@@ -87,10 +89,10 @@ class _TokenLogprobsFn(torch.autograd.Function):
     def forward(ctx, logits, targets, vocab, scale, ignore_index, inplace):
         lg, vocab = _rows(logits, vocab)
         tg = _flat(targets, "targets", lg.shape[0], torch.int64, lg.device)
-        logp, stats = _logprobs(lg, tg, vocab, scale, ignore_index)
+        logp, stats = _logprobs(lg, tg, vocab, scale, ignore_index, targets.shape)
         ctx.args, ctx.shape, ctx.inplace = (vocab, scale, ignore_index), logits.shape, inplace
         ctx.save_for_backward(lg, tg, stats)
-        return logp.view(targets.shape)
+        return logp
 
     @staticmethod
     def backward(ctx, grad):
@@ -112,7 +114,8 @@ def token_logprobs(logits, targets, vocab=None, *, temperature=1.0, ignore_index
     if _wants_grad(logits):
         return _TokenLogprobsFn.apply(logits, targets, vocab, scale, ignore_index, inplace)
     lg, vocab = _rows(logits, vocab)
-    return _logprobs(lg, _flat(targets, "targets", lg.shape[0], torch.int64, lg.device), vocab, scale, ignore_index)[0].view(targets.shape)
+    tg = _flat(targets, "targets", lg.shape[0], torch.int64, lg.device)
+    return _logprobs(lg, tg, vocab, scale, ignore_index, targets.shape, keep=False)[0]
 
 
 # ----------------------------------------------------------------------------------- through the vocabulary projection
@@ -419,7 +422,7 @@ class PolicyLoss:
         if _wants_grad(logits):
             return _LogitsLossFn.apply(logits, self, labels, offsets)
         lg, vocab, desc, (old, advantages, ref, tg), offsets = self._prepare(logits, labels, offsets)
-        logp, _ = _logprobs(lg, tg, vocab, self.scale, self.ignore_index)
+        logp, _ = _logprobs(lg, tg, vocab, self.scale, self.ignore_index, keep=False)
         loss, self.stats = torch.empty((), dtype=torch.float32, device=lg.device), torch.empty(2, dtype=torch.float32, device=lg.device)
         return L.policy_loss(desc, logp, old, advantages, ref, tg, offsets, loss, self.stats, torch.empty_like(logp))
 
@@ -445,39 +448,43 @@ def _dense(t):
 
 
 def _gradients(tensors):
-    """The gradients of parameters (``main_grad`` of an arena's, else ``grad``), other tensors as they are; empty ones left out."""
-    tensors = [tensors] if isinstance(tensors, torch.Tensor) else tensors
-    grads = []
-    for t in tensors:
-        if isinstance(t, nn.Parameter):
-            t = t.main_grad if getattr(t, "main_grad", None) is not None else t.grad
-        if t is None or t.numel() == 0:
+    """(tensors for the kernels, [(gradient, its copy without gaps)], bb_grad_tensor fields) of a list: the gradients of parameters
+    (``main_grad`` of an arena's, else ``grad``), other tensors as they are, empty ones left out."""
+    grads, staged, fields, device = [], [], [], None
+    for t in ((tensors,) if isinstance(tensors, torch.Tensor) else tensors):
+        if type(t) is not torch.Tensor:
+            if isinstance(t, nn.Parameter):
+                main = getattr(t, "main_grad", None)
+                t = t.grad if main is None else main
+            if t is None:
+                continue
+        n = t.numel()
+        if n == 0:
             continue
-        if not t.is_cuda or (grads and t.device != grads[0].device):
+        where = t.get_device()
+        if where < 0 or (device is not None and where != device):
             raise L.BambooNativeError("gradients: CUDA tensors of one device are expected; the sm_100a kernels have no CPU fallback")
-        grads.append(t.detach() if t.requires_grad else t)
-    return grads
-
-
-def _partials(grads):
-    n = L.grad_norm_partials(len(grads))
-    return L.workspace(8 * n, "grad_norm"), n
+        device = where
+        if not t.is_contiguous() and not _dense(t):
+            gradient, t = t.detach(), t.detach().contiguous()
+            staged.append((gradient, t))
+        fields += (t.data_ptr(), n, L.DTYPE_CODES.get(t.dtype, -1), 0)
+        grads.append(t)
+    return grads, staged, fields
 
 
 def grad_sumsq(tensors):
     """Sum of squares over all gradients together (fp64 [1] on their device)."""
-    grads = [g if _dense(g) else g.contiguous() for g in _gradients(tensors)]
-    partials, n = _partials(grads)
-    L.grad_sumsq(L.grad_tensors(grads), len(grads), partials)
-    return partials[:8 * n].view(torch.float64).sum().reshape(1)
+    grads, _, fields = _gradients(tensors)
+    return L.grad_sumsq(L.grad_tensors(fields), len(grads)).clone()
 
 
 def global_grad_norm(tensors):
     """2-norm over all gradients together (fp32 scalar on their device); nothing is changed."""
-    grads = _gradients(tensors)
-    if not grads:
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not _gradients(tensors)[0]:
         return torch.zeros(())
-    return grad_sumsq(grads).sqrt().float().reshape(())
+    return grad_sumsq(tensors).sqrt().float().reshape(())
 
 
 def clip_grad_norm_(tensors, max_norm):
@@ -487,17 +494,12 @@ def clip_grad_norm_(tensors, max_norm):
     within the norm nothing is written."""
     if not max_norm > 0:
         raise ValueError(f"max_norm has to be positive, got {max_norm}")
-    grads = _gradients(tensors)
+    grads, staged, fields = _gradients(tensors)
     if not grads:
         return torch.zeros(())
-    staged = [g if _dense(g) else g.contiguous() for g in grads]
-    partials, _ = _partials(staged)
-    table = L.grad_tensors(staged)
-    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    L.grad_clip(table, len(staged), partials, max_norm, norm)
-    for g, s in zip(grads, staged):
-        if s is not g:
-            g.copy_(s)
+    norm = L.grad_clip(L.grad_tensors(fields), len(grads), max_norm, torch.empty((), dtype=torch.float32, device=grads[0].device))
+    for gradient, copy in staged:
+        gradient.copy_(copy)
     return norm
 
 
@@ -512,6 +514,4 @@ def adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, *, max_norm, 
         if not t.is_cuda or t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != master.numel():
             raise L.BambooNativeError("adam_step_clipped: contiguous fp32 CUDA tensors of one size are expected")
     norm = torch.empty((), dtype=torch.float32, device=master.device)
-    partials, n = (_partials([grad])[0], 0) if sumsq is None else (sumsq, 1)
-    return L.adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, grad_scale=grad_scale, partials=partials, num_partials=n,
-                               max_norm=max_norm, norm=norm, **adam)
+    return L.adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, grad_scale=grad_scale, sumsq=sumsq, max_norm=max_norm, norm=norm, **adam)

@@ -308,7 +308,7 @@ enum { BB_DTYPE_BF16 = 0, BB_DTYPE_F32 = 1 };
 
 /* logp[r] = log softmax(scale * logits[r, :vocab])[targets[r]], 0 for rows whose target is ignore_index (such rows are not
  * read).  Rows start anywhere (ld >= vocab elements, no alignment beyond the type's).  stats [rows, 2], 8-byte aligned, keeps
- * what the backward call needs of each row's softmax.  A row without a finite logit gives -inf and a zero gradient; a
+ * what the backward call needs of each row's softmax (NULL: none follows).  A row without a finite logit gives -inf and a zero gradient; a
  * target outside [0, vocab) sets the status word to BB_ERR_INVALID_ARG and counts as ignored. */
 int bb_token_logprob_fwd(const void* logits, int dtype, long long ld, const long long* targets, double scale, float* logp,
                          float* stats, long long rows, int vocab, long long ignore_index, void* stream);
@@ -392,21 +392,21 @@ int bb_policy_loss_logits(const bb_policy_desc* d, const void* logits, int dtype
 int bb_rescale_grad(void* grad, int dtype, long long ld, long long rows, int cols, const float* upstream, float made_for,
                     void* stream);
 
-/* Global norm of a list of gradients and clipping.  bb_grad_sumsq writes bb_grad_norm_partials(count) partial sums of squares
- * (64-bit); their sum, over whatever else the caller adds (other pipeline stages), is the squared norm.  The consumers take
- * `num_partials` such values (0: they make them first, from their own gradients, in the room for
- * bb_grad_norm_partials(count) values at `partials`; 1 tensor for the Adam step), norm = grad_scale * sqrt(sum), coefficient = min(1, max_norm / (norm + 1e-6)), and write the
- * norm before clipping to `norm` (device).  bb_grad_clip scales the tensors in place (not at all within the norm);
- * bb_adam_step_clipped is an Adam step on coefficient * grad_scale * grad.  A norm that is NaN makes everything NaN. */
+/* Global norm of a list of gradients and clipping.  bb_grad_sumsq writes the sum of squares (64-bit) to the first 8 bytes of
+ * the workspace (bb_grad_norm_workspace_bytes()).  The consumers take such a sum - over whatever the caller lets the norm be
+ * over, e.g. other pipeline stages - or, with sumsq NULL, make it first from their own gradients: norm = grad_scale *
+ * sqrt(sumsq), coefficient = min(1, max_norm / (norm + 1e-6)); the norm before clipping goes to `norm` (device).  bb_grad_clip
+ * scales the tensors in place (not at all within the norm); bb_adam_step_clipped is an Adam step on coefficient * grad_scale
+ * * grad.  A norm that is NaN makes everything NaN.  Squares are taken in 32 bits: values up to 1e19. */
 typedef struct bb_grad_tensor { void* data; long long numel; int dtype; } bb_grad_tensor;
-int bb_grad_norm_partials(int count);
-int bb_grad_sumsq(const bb_grad_tensor* tensors, int count, double* partials, void* stream);
-int bb_grad_clip(const bb_grad_tensor* tensors, int count, double* partials, int num_partials, double max_norm, float* norm,
-                 void* stream);
+long long bb_grad_norm_workspace_bytes(void);
+int bb_grad_sumsq(const bb_grad_tensor* tensors, int count, void* workspace, long long workspace_bytes, void* stream);
+int bb_grad_clip(const bb_grad_tensor* tensors, int count, const double* sumsq, double max_norm, float* norm, void* workspace,
+                 long long workspace_bytes, void* stream);
 int bb_adam_step_clipped(float* master, float* grad, float* exp_avg, float* exp_avg_sq, void* param_bf16, long long n, double lr,
                          double beta1, double beta2, double eps, int step, int adam_w_mode, int bias_correction,
-                         double weight_decay, double grad_scale, int zero_grad, double* partials, int num_partials,
-                         double max_norm, float* norm, void* stream);
+                         double weight_decay, double grad_scale, int zero_grad, const double* sumsq, double max_norm,
+                         float* norm, void* workspace, long long workspace_bytes, void* stream);
 
 /* ---- inter-stage transfer --------------------------------------------------------- */
 /* Set-up (these four are the only entry points that allocate or map device memory; call

@@ -150,11 +150,16 @@ def test_native_refusals_do_not_need_a_gpu():
         return handle.bb_head_logprob_fwd(ctypes.byref(lib.HeadDesc(**{**h, **kw})), states, at, at, at, at, at, ws, None)
     for bad in (dict(rows=0), dict(vocab=0), dict(hidden=0), dict(ld_hidden=63), dict(ld_weight=56), dict(scale=-1.0), dict(states=at + 8), dict(ws=8)):
         refused(head(**bad), b"bb_head_logprob_fwd")
-    refused(handle.bb_grad_sumsq(None, 1, at, None), b"bb_grad_sumsq")
-    refused(handle.bb_grad_clip(lib._tensor_table(1).pack(at, 4, 1, 0), 1, at, 1, 0.0, at, None), b"bb_grad_clip")
-    refused(handle.bb_grad_clip(lib._tensor_table(1).pack(at, 0, 1, 0), 1, at, 1, 1.0, at, None), b"bb_grad_clip")
-    refused(handle.bb_grad_clip(lib._tensor_table(1).pack(at + 2, 4, 1, 0), 1, at, 1, 1.0, at, None), b"bb_grad_clip")
-    refused(handle.bb_adam_step_clipped(at, at, at, at, None, 6, 1e-3, 0.9, 0.999, 1e-8, 1, 1, 1, 0.0, 1.0, 1, at, 1, 1.0, at, None), b"bb_adam_step_clipped")
+    room = handle.bb_grad_norm_workspace_bytes()
+    one = lambda *fields: lib._tensor_table(1).pack(*fields)  # noqa: E731
+    refused(handle.bb_grad_sumsq(None, 1, at, room, None), b"bb_grad_sumsq")
+    refused(handle.bb_grad_sumsq(one(at, 4, 1, 0), 1, at, room - 1, None), b"bb_grad_sumsq")
+    for fields, limit, ws in (((at, 4, 1, 0), 0.0, room), ((at, 0, 1, 0), 1.0, room), ((at + 2, 4, 1, 0), 1.0, room), ((at, 4, 2, 0), 1.0, room),
+                              ((0, 4, 1, 0), 1.0, room), ((at, 4, 1, 0), 1.0, 8), ((at, 4, 1, 0), math.nan, room)):
+        refused(handle.bb_grad_clip(one(*fields), 1, None, limit, at, at, ws, None), b"bb_grad_clip")
+    for n, limit, ws in ((6, 1.0, room), (8, 0.0, room), (8, 1.0, 8)):
+        refused(handle.bb_adam_step_clipped(at, at, at, at, None, n, 1e-3, 0.9, 0.999, 1e-8, 1, 1, 1, 0.0, 1.0, 1, None, limit, at, at, ws, None),
+                b"bb_adam_step_clipped")
 
 
 def test_descriptors_match_the_header():
