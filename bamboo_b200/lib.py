@@ -605,6 +605,14 @@ def _dtype(t, what):
     return code
 
 
+def _bytes_of(desc, ask):
+    """Workspace bytes of a descriptor, asked once (0 where the native side refuses it: the call itself then says why)."""
+    n = desc.__dict__.get("_bytes")
+    if n is None:
+        n = desc._bytes = max(0, ask(ctypes.byref(desc)))
+    return n
+
+
 def token_logprob_fwd(logits, targets, logp, stats, vocab, scale=1.0, ignore_index=-100):
     """logits: [rows, cols] bf16 / fp32, unit inner stride; targets [rows] int64; logp [rows], stats [rows, 2] fp32 (None:
     no backward pass follows)."""
@@ -630,7 +638,7 @@ def head_logprob_fwd(desc, hidden, weight, targets, logp, stats):
     global LAUNCHES
     LAUNCHES += 2
     lib = load()
-    ws = workspace(max(0, lib.bb_head_logprob_workspace_bytes(ctypes.byref(desc))), "post_training")
+    ws = workspace(_bytes_of(desc, lib.bb_head_logprob_workspace_bytes), "post_training")
     check(lib.bb_head_logprob_fwd(ctypes.byref(desc), hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), logp.data_ptr(), stats.data_ptr(),
                                   ws.data_ptr(), ws.numel(), _raw_stream()), "bb_head_logprob_fwd")
     return logp
@@ -650,7 +658,7 @@ def preference_loss(desc, logp, ref, targets, offsets, loss, rewards, row_grad):
     global LAUNCHES
     LAUNCHES += 2
     lib = load()
-    ws = workspace(max(0, lib.bb_preference_workspace_bytes(ctypes.byref(desc))), "post_training")
+    ws = workspace(_bytes_of(desc, lib.bb_preference_workspace_bytes), "post_training")
     check(lib.bb_preference_loss(ctypes.byref(desc), logp.data_ptr(), _addr(ref), targets.data_ptr(), _addr(offsets), loss.data_ptr(),
                                  rewards.data_ptr(), row_grad.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream()), "bb_preference_loss")
     return loss
@@ -660,7 +668,7 @@ def preference_loss_logits(desc, logits, targets, vocab, ref, offsets, loss, rew
     global LAUNCHES
     LAUNCHES += 3
     lib = load()
-    ws = workspace(max(0, lib.bb_preference_workspace_bytes(ctypes.byref(desc))), "post_training")
+    ws = workspace(_bytes_of(desc, lib.bb_preference_workspace_bytes), "post_training")
     check(lib.bb_preference_loss_logits(ctypes.byref(desc), logits.data_ptr(), _dtype(logits, "logits"), logits.stride(0), scale, vocab, logits.shape[1],
                                         _addr(ref), targets.data_ptr(), _addr(offsets), loss.data_ptr(), rewards.data_ptr(), dlogits.data_ptr(),
                                         dlogits.stride(0), grad_scale, ws.data_ptr(), ws.numel(), _raw_stream()), "bb_preference_loss_logits")
@@ -671,7 +679,7 @@ def policy_loss(desc, logp, old_logp, advantages, ref, targets, offsets, loss, s
     global LAUNCHES
     LAUNCHES += 2
     lib = load()
-    ws = workspace(max(0, lib.bb_policy_workspace_bytes(ctypes.byref(desc))), "post_training")
+    ws = workspace(_bytes_of(desc, lib.bb_policy_workspace_bytes), "post_training")
     check(lib.bb_policy_loss(ctypes.byref(desc), logp.data_ptr(), _addr(old_logp), advantages.data_ptr(), _addr(ref), targets.data_ptr(),
                              _addr(offsets), loss.data_ptr(), stats.data_ptr(), row_grad.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream()),
           "bb_policy_loss")
@@ -682,7 +690,7 @@ def policy_loss_logits(desc, logits, targets, vocab, old_logp, advantages, ref, 
     global LAUNCHES
     LAUNCHES += 3
     lib = load()
-    ws = workspace(max(0, lib.bb_policy_workspace_bytes(ctypes.byref(desc))), "post_training")
+    ws = workspace(_bytes_of(desc, lib.bb_policy_workspace_bytes), "post_training")
     check(lib.bb_policy_loss_logits(ctypes.byref(desc), logits.data_ptr(), _dtype(logits, "logits"), logits.stride(0), scale, vocab, logits.shape[1],
                                     _addr(old_logp), advantages.data_ptr(), _addr(ref), targets.data_ptr(), _addr(offsets), loss.data_ptr(),
                                     stats.data_ptr(), logp.data_ptr(), dlogits.data_ptr(), dlogits.stride(0), grad_scale, ws.data_ptr(), ws.numel(),

@@ -15,6 +15,8 @@ Formulas stand beside the kernels' declarations (``include/bamboo_b200.h``) and 
 advantages may be anything, NaN and infinities included.  Everything runs on the current stream, nothing synchronises, and there is no
 fallback: CPU tensors are refused.
 """
+import functools
+
 import torch
 from torch import nn
 
@@ -210,6 +212,8 @@ def head_logprobs(hidden, weight, targets, vocab=None, *, temperature=1.0, ignor
 
 
 # ----------------------------------------------------------------------------------- losses over log-probabilities
+# (descriptors are kept: making one costs the host as much as a launch)
+@functools.lru_cache(maxsize=256)
 def _preference_desc(tokens, sequences, beta, form, label_smoothing, average, ignore_index):
     if form not in L.PREFERENCE_FORMS:
         raise ValueError(f"form {form!r}: one of {sorted(L.PREFERENCE_FORMS)}")
@@ -219,10 +223,11 @@ def _preference_desc(tokens, sequences, beta, form, label_smoothing, average, ig
                             average=int(average), ignore_index=ignore_index)
 
 
+@functools.lru_cache(maxsize=256)
 def _policy_desc(tokens, sequences, advantages, clip_low, clip_high, kl_coef, reduction, ignore_index):
     if reduction not in L.POLICY_REDUCTIONS:
         raise ValueError(f"reduction {reduction!r}: one of {sorted(L.POLICY_REDUCTIONS)}")
-    per_sequence = advantages.numel() == sequences and tokens != sequences
+    per_sequence = advantages == sequences and tokens != sequences
     return L.PolicyDesc(tokens=tokens, sequences=sequences, reduction=L.POLICY_REDUCTIONS[reduction], clip_low=clip_low, clip_high=clip_high,
                         kl_coef=kl_coef, advantage_per_sequence=int(per_sequence), ignore_index=ignore_index)
 
@@ -280,7 +285,7 @@ def policy_loss(logps, old_logps, advantages, targets, *, ref_logps=None, clip_l
     lp = _flat(logps, "logps", targets.numel(), torch.float32, targets.device)
     if not lp.is_cuda:
         raise L.BambooNativeError("logps: expected a CUDA tensor; the sm_100a kernels have no CPU fallback")
-    desc = _policy_desc(lp.numel(), sequences, advantages, clip_low, clip_high, kl_coef, reduction, ignore_index)
+    desc = _policy_desc(lp.numel(), sequences, advantages.numel(), clip_low, clip_high, kl_coef, reduction, ignore_index)
     loss, stats = torch.empty((), dtype=torch.float32, device=lp.device), torch.empty(2, dtype=torch.float32, device=lp.device)
     row_grad = torch.empty_like(lp)
     L.policy_loss(desc, lp, *_policy_inputs(desc, old_logps, advantages, ref_logps, targets, lp.device), offsets, loss, stats, row_grad)
@@ -398,7 +403,7 @@ class PolicyLoss:
         ref = labels[3] if len(labels) > 3 else None
         lg, vocab = _rows(logits, self.vocab)
         sequences, offsets = _geometry(targets, offsets)
-        desc = _policy_desc(lg.shape[0], sequences, advantages, *self.form, self.ignore_index)
+        desc = _policy_desc(lg.shape[0], sequences, advantages.numel(), *self.form, self.ignore_index)
         return lg, vocab, desc, _policy_inputs(desc, old, advantages, ref, targets, lg.device), offsets
 
     def _both(self, lg, vocab, desc, inputs, offsets, d, grad_scale):
