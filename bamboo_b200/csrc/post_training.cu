@@ -566,9 +566,9 @@ policy_token_kernel(float* logp, const PolicyRow* row_sums, K2 k, const long lon
     double lp;
     if constexpr (FROM_ROWS) {
       const PolicyRow q = row_sums[i];
-      if (q.counts == 0.f) { logp[i] = 0.f; continue; }
-      lp = row_logp(q.xt, k, q.r, q.s);
-      logp[i] = (float)lp;
+      lp = q.counts == 0.f ? 0.0 : row_logp(q.xt, k, q.r, q.s);
+      if (logp) logp[i] = (float)lp;
+      if (q.counts == 0.f) continue;
     } else {
       if (targets[i] == ignore_index || w == 0.f) { row_grad[i] = 0.f; continue; }
       lp = (double)logp[i];
@@ -1313,8 +1313,8 @@ extern "C" int bb_policy_loss_logits(const bb_policy_desc* d, const void* logits
                                      float grad_scale, void* workspace, long long workspace_bytes, void* stream) {
   if (int rc = policy_check(d, targets, offsets, advantages, loss, stats, workspace)) return rc;
   if (bad_logits("bb_policy_loss_logits", logits, dtype, ld, targets, d->tokens, vocab, scale)) return BB_ERR_INVALID_ARG;
-  if (!logp || bad_output(logits, ld, dlogits, ldd, dtype, d->tokens, vocab, cols))
-    return refuse("bb_policy_loss_logits: null pointer, columns that do not cover the vocabulary, or a gradient that overlaps the logits without being in place");
+  if (bad_output(logits, ld, dlogits, ldd, dtype, d->tokens, vocab, cols))
+    return refuse("bb_policy_loss_logits: columns that do not cover the vocabulary, or a gradient that overlaps the logits without being in place");
   if (workspace_bytes < bb_policy_workspace_bytes(d)) return refuse("bb_policy_loss_logits: workspace smaller than bb_policy_workspace_bytes()");
   cudaStream_t s = (cudaStream_t)stream;
   const PolicyPlan pl = policy_plan(d->tokens, d->sequences, d->reduction == BB_POLICY_SEQUENCE);

@@ -585,21 +585,19 @@ def conv_bn_bwd(desc, x, y, z, mean, rstd, dz, dx, dres, scratch, residual=True,
 
 
 # ---------------------------------------------------------------------------- post-training
-class _DtypeCodes(dict):
-    """torch.dtype -> BB_DTYPE_*, filled when first asked (this module does not import torch by itself)."""
-
-    def get(self, key, default=None):
-        if not self:
-            import torch
-            self.update({torch.bfloat16: 0, torch.float32: 1})
-        return dict.get(self, key, default)
+_dtype_codes = {}
 
 
-DTYPE_CODES = _DtypeCodes()
+def dtype_codes():
+    """torch.dtype -> BB_DTYPE_* (this module does not import torch by itself)."""
+    if not _dtype_codes:
+        import torch
+        _dtype_codes.update({torch.bfloat16: 0, torch.float32: 1})
+    return _dtype_codes
 
 
 def _dtype(t, what):
-    code = DTYPE_CODES.get(t.dtype)
+    code = dtype_codes().get(t.dtype)
     if code is None:
         raise BambooNativeError(f"{what}: bf16 or fp32 expected, got {t.dtype}")
     return code
@@ -613,23 +611,29 @@ def _bytes_of(desc, ask):
     return n
 
 
+def _ld(t):
+    """Elements from one row (last dimension) to the next, of a contiguous tensor of any shape or a 2-D one with unit inner stride."""
+    return t.shape[-1] if t.is_contiguous() else t.stride(-2)
+
+
 def token_logprob_fwd(logits, targets, logp, stats, vocab, scale=1.0, ignore_index=-100):
-    """logits: [rows, cols] bf16 / fp32, unit inner stride; targets [rows] int64; logp [rows], stats [rows, 2] fp32 (None:
-    no backward pass follows)."""
+    """logits: contiguous [..., cols], or [rows, cols] with unit inner stride, bf16 / fp32; targets [rows] int64; logp [rows], stats
+    [rows, 2] fp32 (None: no backward pass follows)."""
     global LAUNCHES
     LAUNCHES += 1
-    check(load().bb_token_logprob_fwd(logits.data_ptr(), _dtype(logits, "logits"), logits.stride(0), targets.data_ptr(), scale, logp.data_ptr(),
-                                      _addr(stats), logits.shape[0], vocab, ignore_index, _raw_stream()), "bb_token_logprob_fwd")
+    check((_lib or load()).bb_token_logprob_fwd(logits.data_ptr(), _dtype(logits, "logits"), _ld(logits), targets.data_ptr(), scale, logp.data_ptr(),
+                                                _addr(stats), logits.numel() // logits.shape[-1], vocab, ignore_index, _raw_stream()),
+          "bb_token_logprob_fwd")
     return logp
 
 
 def token_logprob_bwd(logits, targets, stats, row_grad, dlogits, vocab, scale=1.0, ignore_index=-100, grad_scale=1.0, grad_scale_dev=None):
     global LAUNCHES
     LAUNCHES += 1
-    rows, cols = logits.shape
-    check(load().bb_token_logprob_bwd(logits.data_ptr(), _dtype(logits, "logits"), logits.stride(0), targets.data_ptr(), scale, stats.data_ptr(),
-                                      row_grad.data_ptr(), _addr(grad_scale_dev), grad_scale, dlogits.data_ptr(), dlogits.stride(0), rows, vocab,
-                                      cols, ignore_index, _raw_stream()), "bb_token_logprob_bwd")
+    cols = logits.shape[-1]
+    check((_lib or load()).bb_token_logprob_bwd(logits.data_ptr(), _dtype(logits, "logits"), _ld(logits), targets.data_ptr(), scale, stats.data_ptr(),
+                                                row_grad.data_ptr(), _addr(grad_scale_dev), grad_scale, dlogits.data_ptr(), _ld(dlogits),
+                                                logits.numel() // cols, vocab, cols, ignore_index, _raw_stream()), "bb_token_logprob_bwd")
     return dlogits
 
 
@@ -669,9 +673,9 @@ def preference_loss_logits(desc, logits, targets, vocab, ref, offsets, loss, rew
     LAUNCHES += 3
     lib = load()
     ws = workspace(_bytes_of(desc, lib.bb_preference_workspace_bytes), "post_training")
-    check(lib.bb_preference_loss_logits(ctypes.byref(desc), logits.data_ptr(), _dtype(logits, "logits"), logits.stride(0), scale, vocab, logits.shape[1],
+    check(lib.bb_preference_loss_logits(ctypes.byref(desc), logits.data_ptr(), _dtype(logits, "logits"), _ld(logits), scale, vocab, logits.shape[-1],
                                         _addr(ref), targets.data_ptr(), _addr(offsets), loss.data_ptr(), rewards.data_ptr(), dlogits.data_ptr(),
-                                        dlogits.stride(0), grad_scale, ws.data_ptr(), ws.numel(), _raw_stream()), "bb_preference_loss_logits")
+                                        _ld(dlogits), grad_scale, ws.data_ptr(), ws.numel(), _raw_stream()), "bb_preference_loss_logits")
     return loss
 
 
@@ -691,9 +695,9 @@ def policy_loss_logits(desc, logits, targets, vocab, old_logp, advantages, ref, 
     LAUNCHES += 3
     lib = load()
     ws = workspace(_bytes_of(desc, lib.bb_policy_workspace_bytes), "post_training")
-    check(lib.bb_policy_loss_logits(ctypes.byref(desc), logits.data_ptr(), _dtype(logits, "logits"), logits.stride(0), scale, vocab, logits.shape[1],
+    check(lib.bb_policy_loss_logits(ctypes.byref(desc), logits.data_ptr(), _dtype(logits, "logits"), _ld(logits), scale, vocab, logits.shape[-1],
                                     _addr(old_logp), advantages.data_ptr(), _addr(ref), targets.data_ptr(), _addr(offsets), loss.data_ptr(),
-                                    stats.data_ptr(), logp.data_ptr(), dlogits.data_ptr(), dlogits.stride(0), grad_scale, ws.data_ptr(), ws.numel(),
+                                    stats.data_ptr(), _addr(logp), dlogits.data_ptr(), _ld(dlogits), grad_scale, ws.data_ptr(), ws.numel(),
                                     _raw_stream()), "bb_policy_loss_logits")
     return loss
 
@@ -702,8 +706,8 @@ def rescale(grad, upstream, made_for):
     """``grad`` [rows, cols], made for an upstream gradient of ``made_for``, times ``upstream`` (device) / made_for."""
     global LAUNCHES
     LAUNCHES += 1
-    rows, cols = grad.shape
-    check(load().bb_rescale_grad(grad.data_ptr(), _dtype(grad, "gradient"), grad.stride(0), rows, cols, upstream.data_ptr(), made_for, _raw_stream()),
+    cols = grad.shape[-1]
+    check(load().bb_rescale_grad(grad.data_ptr(), _dtype(grad, "gradient"), _ld(grad), grad.numel() // cols, cols, upstream.data_ptr(), made_for, _raw_stream()),
           "bb_rescale_grad")
     return grad
 

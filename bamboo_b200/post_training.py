@@ -25,17 +25,20 @@ from . import lib as L
 
 # ----------------------------------------------------------------------------------- arguments
 def _rows(logits, vocab):
-    """logits [..., cols] as [rows, cols] with unit inner stride (a copy only where strides ask for one)."""
+    """(logits, rows, vocab): contiguous logits [..., cols] as they are, others as [rows, cols] with unit inner stride (a copy only where
+    their strides ask for one)."""
     if not logits.is_cuda:
         raise L.BambooNativeError("logits: expected a CUDA tensor; the sm_100a kernels have no CPU fallback")
     cols = logits.shape[-1]
-    vocab = cols if vocab is None else vocab
+    if vocab is None:
+        vocab = cols
     if not 0 < vocab <= cols:
         raise ValueError(f"vocab {vocab} does not fit logits with {cols} columns")
-    lg = logits.detach() if logits.dim() == 2 else logits.detach().reshape(-1, cols)
-    if lg.stride(1) != 1 or (lg.shape[0] > 1 and lg.stride(0) < cols):
-        lg = lg.contiguous()
-    return lg, vocab
+    if not logits.is_contiguous():
+        logits = logits.detach().reshape(-1, cols)
+        if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < cols):
+            logits = logits.contiguous()
+    return logits, logits.numel() // cols, vocab
 
 
 def _flat(t, name, numel, dtype, device):
@@ -76,9 +79,8 @@ def _wants_grad(t):
 
 
 # ----------------------------------------------------------------------------------- token log-probabilities
-def _logprobs(lg, tg, vocab, scale, ignore_index, shape=None, keep=True):
+def _logprobs(lg, rows, tg, vocab, scale, ignore_index, shape=None, keep=True):
     """(log-probabilities, softmax sums for the backward pass unless ``keep`` is off)"""
-    rows = lg.shape[0]
     logp = torch.empty(rows if shape is None else shape, dtype=torch.float32, device=lg.device)
     stats = torch.empty(rows, 2, dtype=torch.float32, device=lg.device) if keep else None
     if rows:
@@ -89,20 +91,20 @@ def _logprobs(lg, tg, vocab, scale, ignore_index, shape=None, keep=True):
 class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, vocab, scale, ignore_index, inplace):
-        lg, vocab = _rows(logits, vocab)
-        tg = _flat(targets, "targets", lg.shape[0], torch.int64, lg.device)
-        logp, stats = _logprobs(lg, tg, vocab, scale, ignore_index, targets.shape)
-        ctx.args, ctx.shape, ctx.inplace = (vocab, scale, ignore_index), logits.shape, inplace
-        ctx.save_for_backward(lg, tg, stats)
+        lg, rows, vocab = _rows(logits, vocab)
+        tg = _flat(targets, "targets", rows, torch.int64, lg.device)
+        logp, stats = _logprobs(lg, rows, tg, vocab, scale, ignore_index, targets.shape)
+        ctx.args, ctx.shape, ctx.inplace = (rows, vocab, scale, ignore_index), logits.shape, inplace
+        ctx.save_for_backward(lg.detach(), tg, stats)
         return logp
 
     @staticmethod
     def backward(ctx, grad):
         lg, tg, stats = ctx.saved_tensors
-        vocab, scale, ignore_index = ctx.args
+        rows, vocab, scale, ignore_index = ctx.args
         out = lg if ctx.inplace else torch.empty(lg.shape, dtype=lg.dtype, device=lg.device)
-        if lg.shape[0]:
-            row_grad = _flat(grad, "gradient", lg.shape[0], torch.float32, lg.device)
+        if rows:
+            row_grad = _flat(grad, "gradient", rows, torch.float32, lg.device)
             L.token_logprob_bwd(lg, tg, stats, row_grad, out, vocab, scale, ignore_index)
         return out.view(ctx.shape), None, None, None, None, None
 
@@ -115,9 +117,9 @@ def token_logprobs(logits, targets, vocab=None, *, temperature=1.0, ignore_index
     scale = _inverse(temperature)
     if _wants_grad(logits):
         return _TokenLogprobsFn.apply(logits, targets, vocab, scale, ignore_index, inplace)
-    lg, vocab = _rows(logits, vocab)
-    tg = _flat(targets, "targets", lg.shape[0], torch.int64, lg.device)
-    return _logprobs(lg, tg, vocab, scale, ignore_index, targets.shape, keep=False)[0]
+    lg, rows, vocab = _rows(logits, vocab)
+    tg = _flat(targets, "targets", rows, torch.int64, lg.device)
+    return _logprobs(lg, rows, tg, vocab, scale, ignore_index, targets.shape, keep=False)[0]
 
 
 # ----------------------------------------------------------------------------------- through the vocabulary projection
@@ -333,16 +335,16 @@ class PreferenceLoss:
 
     def _prepare(self, logits, labels, offsets):
         targets, ref = labels if isinstance(labels, (tuple, list)) else (labels, None)
-        lg, vocab = _rows(logits, self.vocab)
+        lg, rows, vocab = _rows(logits, self.vocab)
         sequences, offsets = _geometry(targets, offsets)
-        tg = _flat(targets, "targets", lg.shape[0], torch.int64, lg.device)
-        return lg, vocab, tg, ref, offsets, _preference_desc(lg.shape[0], sequences, *self.form, self.ignore_index)
+        tg = _flat(targets, "targets", rows, torch.int64, lg.device)
+        return lg, vocab, tg, ref, offsets, _preference_desc(rows, sequences, *self.form, self.ignore_index)
 
     def _losses(self, logits, labels, offsets):
         lg, vocab, tg, ref, offsets, desc = self._prepare(logits, labels, offsets)
-        logp, stats = _logprobs(lg, tg, vocab, self.scale, self.ignore_index)
+        logp, stats = _logprobs(lg, desc.tokens, tg, vocab, self.scale, self.ignore_index)
         loss, self.rewards, row_grad = _preference(logp, ref, tg, offsets, desc)
-        return lg, tg, stats, row_grad, loss
+        return lg.detach(), tg, stats, row_grad, loss
 
     def _forward(self, logits, labels, offsets):
         *saved, loss = self._losses(logits, labels, offsets)
@@ -362,23 +364,23 @@ class PreferenceLoss:
         """(loss, rewards, gradient of the logits times ``grad_scale``) without autograd; ``out`` receives the gradient (the logits
         themselves are allowed)."""
         lg, vocab, tg, ref, offsets, desc = self._prepare(logits, labels, offsets)
-        ref = None if ref is None else _flat(ref, "ref_logps", lg.shape[0], torch.float32, lg.device)
+        ref = None if ref is None else _flat(ref, "ref_logps", desc.tokens, torch.float32, lg.device)
         loss = torch.empty((), dtype=torch.float32, device=lg.device)
         self.rewards = torch.empty(desc.sequences, dtype=torch.float32, device=lg.device)
-        d, grad = _gradient_buffer(lg, logits, out)
+        d, grad = _gradient_buffer(logits, out)
         L.preference_loss_logits(desc, lg, tg, vocab, ref, offsets, loss, self.rewards, d, self.scale, grad_scale)
         return loss, self.rewards, grad
 
 
-def _gradient_buffer(lg, logits, out):
-    """(rows view for the kernels, tensor for the caller) of the gradient."""
+def _gradient_buffer(logits, out):
+    """(tensor for the kernels, tensor for the caller) of the gradient."""
     if out is None:
-        d = torch.empty(lg.shape, dtype=lg.dtype, device=lg.device)
-        return d, d.view(logits.shape)
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        return out, out
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
         raise ValueError("out: a tensor like the logits is expected")
-    d = out.detach().view(-1, out.shape[-1])
-    if d.stride(1) != 1:
+    d = out.detach() if out.is_contiguous() else out.detach().view(-1, out.shape[-1])
+    if d.stride(-1) != 1:
         raise ValueError("out: rows with unit stride are expected")
     return d, out
 
@@ -401,21 +403,21 @@ class PolicyLoss:
     def _prepare(self, logits, labels, offsets):
         targets, old, advantages = labels[:3]
         ref = labels[3] if len(labels) > 3 else None
-        lg, vocab = _rows(logits, self.vocab)
+        lg, rows, vocab = _rows(logits, self.vocab)
         sequences, offsets = _geometry(targets, offsets)
-        desc = _policy_desc(lg.shape[0], sequences, advantages.numel(), *self.form, self.ignore_index)
+        desc = _policy_desc(rows, sequences, advantages.numel(), *self.form, self.ignore_index)
         return lg, vocab, desc, _policy_inputs(desc, old, advantages, ref, targets, lg.device), offsets
 
     def _both(self, lg, vocab, desc, inputs, offsets, d, grad_scale):
         old, advantages, ref, tg = inputs
         loss = torch.empty((), dtype=torch.float32, device=lg.device)
-        logp = torch.empty(lg.shape[0], dtype=torch.float32, device=lg.device)
         self.stats = torch.empty(2, dtype=torch.float32, device=lg.device)
-        L.policy_loss_logits(desc, lg, tg, vocab, old, advantages, ref, offsets, loss, self.stats, logp, d, self.scale, grad_scale)
+        L.policy_loss_logits(desc, lg, tg, vocab, old, advantages, ref, offsets, loss, self.stats, None, d, self.scale, grad_scale)
         return loss
 
     def _forward(self, logits, labels, offsets):
         lg, *rest = self._prepare(logits, labels, offsets)
+        lg = lg.detach()
         d = lg if self.inplace else torch.empty(lg.shape, dtype=lg.dtype, device=lg.device)
         return self._both(lg, *rest, d, self.grad_scale), (d,), (self.grad_scale,)
 
@@ -427,7 +429,7 @@ class PolicyLoss:
         if _wants_grad(logits):
             return _LogitsLossFn.apply(logits, self, labels, offsets)
         lg, vocab, desc, (old, advantages, ref, tg), offsets = self._prepare(logits, labels, offsets)
-        logp, _ = _logprobs(lg, tg, vocab, self.scale, self.ignore_index, keep=False)
+        logp, _ = _logprobs(lg, desc.tokens, tg, vocab, self.scale, self.ignore_index, keep=False)
         loss, self.stats = torch.empty((), dtype=torch.float32, device=lg.device), torch.empty(2, dtype=torch.float32, device=lg.device)
         return L.policy_loss(desc, logp, old, advantages, ref, tg, offsets, loss, self.stats, torch.empty_like(logp))
 
@@ -435,7 +437,7 @@ class PolicyLoss:
         """(loss, stats, gradient of the logits times ``grad_scale``) without autograd; ``out`` receives the gradient (the logits
         themselves are allowed)."""
         lg, *rest = self._prepare(logits, labels, offsets)
-        d, grad = _gradient_buffer(lg, logits, out)
+        d, grad = _gradient_buffer(logits, out)
         return self._both(lg, *rest, d, grad_scale), self.stats, grad
 
 
@@ -455,7 +457,7 @@ def _dense(t):
 def _gradients(tensors):
     """(tensors for the kernels, [(gradient, its copy without gaps)], bb_grad_tensor fields) of a list: the gradients of parameters
     (``main_grad`` of an arena's, else ``grad``), other tensors as they are, empty ones left out."""
-    grads, staged, fields, device = [], [], [], None
+    grads, staged, fields, device, codes = [], [], [], None, L.dtype_codes()
     for t in ((tensors,) if isinstance(tensors, torch.Tensor) else tensors):
         if type(t) is not torch.Tensor:
             if isinstance(t, nn.Parameter):
@@ -473,7 +475,7 @@ def _gradients(tensors):
         if not t.is_contiguous() and not _dense(t):
             gradient, t = t.detach(), t.detach().contiguous()
             staged.append((gradient, t))
-        fields += (t.data_ptr(), n, L.DTYPE_CODES.get(t.dtype, -1), 0)
+        fields += (t.data_ptr(), n, codes.get(t.dtype, -1), 0)
         grads.append(t)
     return grads, staged, fields
 

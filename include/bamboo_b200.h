@@ -381,7 +381,7 @@ int bb_policy_loss(const bb_policy_desc* d, const float* logp, const float* old_
                    const long long* targets, const long long* offsets, float* loss, float* stats, float* row_grad,
                    void* workspace, long long workspace_bytes, void* stream);
 /* The same from logits, with their gradient (times grad_scale) in the same pass: a row's gradient needs nothing of the other
- * rows.  logp [tokens] receives the log-probabilities; arguments otherwise as above and in bb_token_logprob_*. */
+ * rows.  logp [tokens] (may be NULL) receives the log-probabilities; arguments otherwise as above and in bb_token_logprob_*. */
 int bb_policy_loss_logits(const bb_policy_desc* d, const void* logits, int dtype, long long ld, double scale, int vocab, int cols,
                           const float* old_logp, const float* advantages, const float* ref, const long long* targets,
                           const long long* offsets, float* loss, float* stats, float* logp, void* dlogits, long long ldd,

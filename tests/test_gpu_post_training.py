@@ -130,6 +130,9 @@ def test_other_strides_and_shapes(pt):
     near(pt.token_logprobs(x[:, 1:], t[:, 1:]), want[:, 1:], 1e-6, 1e-6)
     near(pt.token_logprobs(x[:1].expand(6, 5, 77), t[:1].expand(6, 5)), want[:1].expand(6, 5), 1e-6, 1e-6)
     assert pt.token_logprobs(x[:0], t[:0]).shape == (0, 5)
+    near(pt.token_logprobs(x[:, 2:3], t[:, 2:3]), want[:, 2:3], 1e-6, 1e-6)                            # one token of each sequence
+    near(pt.token_logprobs(x[:, 2], t[:, 2]), want[:, 2], 1e-6, 1e-6)
+    near(pt.token_logprobs(x[3, 2], t[3, 2]).reshape(1), want[3, 2].reshape(1), 1e-6, 1e-6)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
