@@ -1602,9 +1602,10 @@ namespace {
 __global__ void __launch_bounds__(1024)
 head_combine_kernel(const float2* partial, int num, int rows, const float* target_logit, const long long* targets, long long ignore_index,
                     int vocab, K2 k, float* logp, float2* stats, int* status) {
-  __shared__ float2 sums[32][32];
+  __shared__ float2 sums[32][33];
   bb::pdl_sync();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int row = blockIdx.x * 32 + lane;
   float r = -INFINITY, s = 0.f;
   if (row < rows) {
 #pragma unroll 4
@@ -1613,10 +1614,19 @@ head_combine_kernel(const float2* partial, int num, int rows, const float* targe
       bb::soft_merge(r, s, q.x, q.y);
     }
   }
-  sums[warp][lane] = make_float2(r, s);
+  sums[lane][warp] = make_float2(r, s);
   __syncthreads();
-  if (warp != 0 || row >= rows) return;
-  for (int w = 1; w < 32; ++w) bb::soft_merge(r, s, sums[w][lane].x, sums[w][lane].y);
+  // the warps' sums of row `warp` of the CTA, one per lane
+  row = blockIdx.x * 32 + warp;
+  const float2 q = sums[warp][lane];
+  float top = q.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  r = top;
+  s = q.x == top ? q.y : q.y * bb::ex2(q.x - top);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane != 0 || row >= rows) return;
   const long long t = targets[row];
   const bool counted = t != ignore_index && t >= 0 && t < vocab;
   if (!counted && t != ignore_index) atomicCAS(status, 0, BB_ERR_INVALID_ARG);
@@ -1697,6 +1707,39 @@ extern "C" int bb_head_logprob_grad(const bb_head_desc* d, const void* hidden_st
   HeadParams h = head_params(d, targets);
   h.col0 = col0; h.stats = (const float2*)stats; h.row_grad = row_grad; h.gscale_dev = grad_scale_dev; h.gscale = (float)(d->scale * grad_scale);
   return head_launch<HEAD_GRAD>(g, h, (cudaStream_t)stream);
+}
+
+extern "C" int bb_head_logprob_bwd(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets, const float* stats,
+                                   const float* row_grad, void* d_hidden, float* d_hidden_f32, void* d_weight, float* d_weight_accum, int piece,
+                                   void* dlogits, long long ldd, void* stream) {
+  if (int rc = head_check("bb_head_logprob_bwd", d, hidden_states, weight, targets)) return rc;
+  const bool whole = piece >= d->vocab;
+  if (!dlogits || piece <= 0 || piece % 8 || ldd < (whole ? d->vocab : piece) || (d_weight && d_weight_accum) || (d_hidden && !whole && !d_hidden_f32)) {
+    bb_set_last_error_msg("bb_head_logprob_bwd: pieces are multiples of 8 entries that fit the buffer, several pieces need the fp32 buffer of d_hidden, and there is one weight gradient");
+    return BB_ERR_INVALID_ARG;
+  }
+  cudaStream_t s = (cudaStream_t)stream;
+  if (d_hidden && !whole) BB_CUDA_CHECK(cudaMemsetAsync(d_hidden_f32, 0, (size_t)d->rows * d->hidden * 4, s));
+  BackToBack overlap;
+  for (int col0 = 0; col0 < d->vocab; col0 += piece) {
+    const int cols = piece < d->vocab - col0 ? piece : d->vocab - col0;
+    if (int rc = bb_head_logprob_grad(d, hidden_states, weight, targets, stats, row_grad, nullptr, 1.f, col0, cols, dlogits, ldd, stream)) return rc;
+    bb_gemm_desc g = {};
+    g.A = dlogits; g.lda = ldd;
+    if (d_hidden) {
+      g.M = d->rows; g.N = d->hidden; g.K = cols; g.B = (const __nv_bfloat16*)weight + (long long)col0 * d->ld_weight; g.ldb = d->ld_weight; g.b_mn_major = 1;
+      g.D = whole ? d_hidden : (void*)d_hidden_f32; g.ldd = d->hidden; g.epilogue = whole ? BB_EPI_STORE : BB_EPI_ACCUM_F32;
+      if (int rc = bb_gemm_bf16(&g, stream)) return rc;
+    }
+    if (d_weight || d_weight_accum) {
+      g.M = cols; g.N = d->hidden; g.K = d->rows; g.a_mn_major = 1; g.B = hidden_states; g.ldb = d->ld_hidden; g.b_mn_major = 1; g.ldd = d->hidden;
+      g.D = d_weight ? (void*)((__nv_bfloat16*)d_weight + (long long)col0 * d->hidden) : (void*)(d_weight_accum + (long long)col0 * d->hidden);
+      g.epilogue = d_weight ? BB_EPI_STORE : BB_EPI_ACCUM_F32;
+      if (int rc = bb_gemm_bf16(&g, stream)) return rc;
+    }
+  }
+  if (d_hidden && !whole) return bb_cast_f32_to_bf16(d_hidden_f32, d_hidden, (long long)d->rows * d->hidden, stream);
+  return BB_OK;
 }
 
 double bb_gemm_store_us(long long M, long long N, long long K, int max_ctas) {

@@ -13,7 +13,12 @@ namespace {
 // with eight and two thirds of the threads per SM (6.5 TB/s), 252 with two.
 constexpr int ROW_LOADS = 4, GRAD_LOADS = 8;
 constexpr int MAX_PARTS = 8;              // CTAs of a cluster that share a row
-constexpr size_t LONG_ROW = 32768;        // bytes from which a row gets more threads
+// How many threads share a row.  A warp of its own where rows are short and there are enough of them for every warp of the machine to be
+// waiting for one (sum / gradient in us, a block of 256 | a warp: 11840 rows of 2.4 KB 25 / 40 | 14 / 13, 5515 of 7.6 KB 18 / 29 |
+// 13 / 18, 2876 of 14 KB 13 / 22 | 18 / 14, 1500 of 28 KB 12 / 20 | 26 / 20; few rows: 600 of 7.6 KB 4 / 4 | 5 / 5); from LONG_ROW on the
+// policy loss's ring (1500 rows of 28 KB 35 -> 26 us against 16 KB as the limit).
+constexpr size_t WARP_SUM = 8192, WARP_GRAD = 16384, TINY_ROW = 1024, LONG_ROW = 32768;
+constexpr int WARP_ROWS = 1024;
 
 // dynamic shared memory next to a kernel's few static bytes: of one CTA per SM, and of each of two
 constexpr size_t MAX_RING = 226 * 1024, PAIR_RING = 112 * 1024;
@@ -63,6 +68,11 @@ template <typename T> struct Span {
   }
 };
 
+// A row is worked on by a block, by its first THREADS threads (a warp more feeds them), or (THREADS = 32) by a warp of its own
+template <int THREADS> __device__ __forceinline__ int row_thread() { return THREADS == 32 ? (int)(threadIdx.x & 31) : (int)threadIdx.x; }
+template <int THREADS> constexpr int ROWS_OF_BLOCK = THREADS == 32 ? 8 : 1;
+template <int THREADS> constexpr int BLOCK = THREADS == 32 ? 256 : THREADS;
+
 // (r, s) of a warp's lanes merged: the largest reference first, one scaling, then plain sums
 __device__ __forceinline__ void soft_warp(float& r, float& s) {
   float top = r;
@@ -94,7 +104,7 @@ template <int THREADS, bool FED = false> __device__ __forceinline__ void soft_bl
 template <typename T, int THREADS> __device__ __noinline__ float2 soft_share_exact(const uint4* v, int nvec, K2 k) {
   constexpr int VEC = Elem<T>::VEC;
   float r = -INFINITY, s = 0.f;
-  for (int c = threadIdx.x; c < nvec; c += THREADS) {
+  for (int c = row_thread<THREADS>(); c < nvec; c += THREADS) {
     float f[VEC];
     Elem<T>::unpack(v[c], f);
     soft_add<VEC>(r, s, f, k);
@@ -112,7 +122,7 @@ template <int VEC> __device__ __forceinline__ void soft_chunk(float2& sum, const
 }
 // the elements of a row in front of its first 16-byte boundary and behind its last
 template <typename T, int THREADS> __device__ __forceinline__ void soft_edges(const T* x, const Span<T>& sp, int n, K2 k, float& r, float& s) {
-  for (int j = threadIdx.x; j < sp.lead + n - sp.tail; j += THREADS) {
+  for (int j = row_thread<THREADS>(); j < sp.lead + n - sp.tail; j += THREADS) {
     const float f = Elem<T>::get(x + (j < sp.lead ? j : sp.tail + j - sp.lead));
     soft_add<1>(r, s, &f, k);
   }
@@ -125,7 +135,7 @@ template <typename T, int THREADS, int U>
 __device__ __forceinline__ void soft_share(const uint4* v, int nvec, K2 k, float& r, float& s) {
   constexpr int VEC = Elem<T>::VEC;
   r = -INFINITY; s = 0.f;
-  int c = threadIdx.x;
+  int c = row_thread<THREADS>();
   float2 sum = make_float2(0.f, 0.f);
   float f[VEC];
   if (c < nvec) {
@@ -158,7 +168,7 @@ __device__ __forceinline__ void soft_share(const uint4* v, int nvec, K2 k, float
 template <typename T> __device__ __noinline__ float2 soft_row_extreme(const T* x, int n) {
   float top = -INFINITY;
   int count = 0, bad = 0;
-  for (int j = threadIdx.x; j < n; j += 32) {
+  for (int j = threadIdx.x & 31; j < n; j += 32) {
     const float f = Elem<T>::get(x + j);
     bad |= f != f || f == INFINITY;
     if (f > top) { top = f; count = 1; } else if (f == top) ++count;
@@ -174,14 +184,15 @@ template <typename T> __device__ __noinline__ float2 soft_row_extreme(const T* x
   return make_float2(top, top == -INFINITY ? 0.f : -(float)count);
 }
 
-// The row's (r, s), in the first warp
+// The row's (r, s), in the row's first warp
 template <typename T, int THREADS, int U>
 __device__ __forceinline__ void soft_whole_row(const T* x, int n, K2 k, float& r, float& s, float2* smem) {
   const Span<T> sp(x, n);
   soft_share<T, THREADS, U>(reinterpret_cast<const uint4*>(x + sp.lead), sp.nvec, k, r, s);
   soft_edges<T, THREADS>(x, sp, n, k, r, s);
-  soft_block<THREADS>(r, s, smem);
-  if (threadIdx.x < 32 && isinf(r)) { const float2 e = soft_row_extreme(x, n); r = e.x; s = e.y; }
+  if constexpr (THREADS == 32) soft_warp(r, s);
+  else soft_block<THREADS>(r, s, smem);
+  if (row_thread<THREADS>() < 32 && isinf(r)) { const float2 e = soft_row_extreme(x, n); r = e.x; s = e.y; }
 }
 
 // -g softmax_j = ng 2^(k x_j - r).  Here k rounded to 32 bits will do: with what the rounding took at the largest logit (about r / k) in
@@ -213,7 +224,7 @@ __device__ __forceinline__ void grad_rest(const T* x, float xt, T* d, int lead, 
   constexpr int VEC = Elem<T>::VEC;
   if (t >= lead) {
     const int tc = (t - lead) / VEC;
-    if (tc < whole && tc % THREADS == (int)threadIdx.x) Elem<T>::put(d + t, grad_target(g, xt, k, w.r, s));
+    if (tc < whole && tc % THREADS == row_thread<THREADS>()) Elem<T>::put(d + t, grad_target(g, xt, k, w.r, s));
   }
   auto one = [&](int j) {
     float v = 0.f;
@@ -221,29 +232,30 @@ __device__ __forceinline__ void grad_rest(const T* x, float xt, T* d, int lead, 
     Elem<T>::put(d + j, v);
   };
   const int nvec = (cols - lead) / VEC, tail = lead + nvec * VEC;
-  for (int c = whole + threadIdx.x; c < nvec; c += THREADS) {
+  for (int c = whole + row_thread<THREADS>(); c < nvec; c += THREADS) {
     const int j0 = lead + c * VEC;
     if (j0 >= V) *reinterpret_cast<uint4*>(d + j0) = make_uint4(0, 0, 0, 0);
     else for (int i = 0; i < VEC; ++i) one(j0 + i);
   }
-  for (int j = threadIdx.x; j < lead + cols - tail; j += THREADS) one(j < lead ? j : tail + j - lead);
+  for (int j = row_thread<THREADS>(); j < lead + cols - tail; j += THREADS) one(j < lead ? j : tail + j - lead);
 }
 
 // d[j] = g * ([j == t] - softmax_j) for j < V, 0 in [V, cols); zeros throughout when g == 0 (nothing is read then)
 template <typename T, int THREADS, int U>
 __device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int t, float g, K2 k, float r, float s) {
   constexpr int VEC = Elem<T>::VEC;
+  const int tid = row_thread<THREADS>();
   if (s == 0.f) g = 0.f;
   if (g == 0.f) {
     const Span<T> sp(d, cols);
     uint4* dv = reinterpret_cast<uint4*>(d + sp.lead);
-    for (int c = threadIdx.x; c < sp.nvec; c += THREADS) dv[c] = make_uint4(0, 0, 0, 0);
-    for (int j = threadIdx.x; j < sp.lead + cols - sp.tail; j += THREADS) Elem<T>::put(d + (j < sp.lead ? j : sp.tail + j - sp.lead), 0.f);
+    for (int c = tid; c < sp.nvec; c += THREADS) dv[c] = make_uint4(0, 0, 0, 0);
+    for (int j = tid; j < sp.lead + cols - sp.tail; j += THREADS) Elem<T>::put(d + (j < sp.lead ? j : sp.tail + j - sp.lead), 0.f);
     return;
   }
   const GradRow w = grad_factors(g, k, s < 0.f ? 0.f : r, s);
   if (s < 0.f || (((uintptr_t)x ^ (uintptr_t)d) & 15) != 0) {      // element by element
-    for (int j = threadIdx.x; j < cols; j += THREADS) {
+    for (int j = tid; j < cols; j += THREADS) {
       float v = 0.f;
       if (j < V) {
         const float f = Elem<T>::get(x + j);
@@ -258,8 +270,8 @@ __device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int 
   const uint4* xv = reinterpret_cast<const uint4*>(x + sp.lead);
   uint4* dv = reinterpret_cast<uint4*>(d + sp.lead);
   const int whole = sp.nvec;                            // chunks of vocabulary entries only
-  const float xt = t >= sp.lead && (t - sp.lead) / VEC % THREADS == (int)threadIdx.x ? Elem<T>::get(x + t) : 0.f;
-  int c = threadIdx.x;
+  const float xt = t >= sp.lead && (t - sp.lead) / VEC % THREADS == tid ? Elem<T>::get(x + t) : 0.f;
+  int c = tid;
   for (; c + (U - 1) * THREADS < whole; c += U * THREADS) {
     uint4 q[U];
 #pragma unroll
@@ -284,6 +296,25 @@ template <int THREADS> __device__ __forceinline__ double block_sum(double v, dou
   return v;
 }
 
+// The same for N values at once; every thread gets the sums
+template <int THREADS, int N> __device__ __forceinline__ void block_sums(double* v, double (*smem)[N] /*[THREADS/32]*/) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i) smem[threadIdx.x >> 5][i] = v[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = 0.0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) v[i] += smem[w][i];
+  }
+}
+
 // loss = mean of pair_loss, in a fixed order; by a block
 template <int THREADS> __device__ __forceinline__ void mean_of(const double* pair_loss, int pairs, float* loss) {
   __shared__ double smem[THREADS / 32];
@@ -295,15 +326,16 @@ template <int THREADS> __device__ __forceinline__ void mean_of(const double* pai
 
 // ------------------------------------------------------------------ token log-probabilities
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(BLOCK<THREADS>)
 token_logprob_fwd_kernel(const T* logits, long long ld, const long long* targets, K2 k, float* logp, float2* stats,
-                         int V, long long ignore_index, int* status) {
-  __shared__ float2 smem[THREADS / 32];
+                         int rows, int V, long long ignore_index, int* status) {
+  __shared__ float2 smem[BLOCK<THREADS> / 32];
   bb::pdl_sync();
-  const int row = blockIdx.x;
+  const int row = THREADS == 32 ? (int)blockIdx.x * ROWS_OF_BLOCK<THREADS> + (int)(threadIdx.x >> 5) : (int)blockIdx.x;
+  if (row >= rows) return;
   const long long t = targets[row];
   if (t == ignore_index || t < 0 || t >= V) {
-    if (threadIdx.x == 0) {
+    if (row_thread<THREADS>() == 0) {
       if (t != ignore_index) atomicCAS(status, 0, BB_ERR_INVALID_ARG);
       logp[row] = 0.f;
       if (stats) stats[row] = make_float2(0.f, 0.f);
@@ -312,9 +344,10 @@ token_logprob_fwd_kernel(const T* logits, long long ld, const long long* targets
   }
   const T* x = logits + (size_t)row * ld;
   float r, s;
+  const float xt = row_thread<THREADS>() == 0 ? Elem<T>::get(x + t) : 0.f;
   soft_whole_row<T, THREADS, ROW_LOADS>(x, V, k, r, s, smem);
-  if (threadIdx.x == 0) {
-    logp[row] = (float)row_logp(Elem<T>::get(x + t), k, r, s);
+  if (row_thread<THREADS>() == 0) {
+    logp[row] = (float)row_logp(xt, k, r, s);
     if (stats) stats[row] = make_float2(r, s);
   }
 }
@@ -368,18 +401,20 @@ token_logprob_fwd_cluster_kernel(const T* logits, long long ld, const long long*
 }
 
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS, 4)
+__global__ void __launch_bounds__(BLOCK<THREADS>, 4)
 token_logprob_bwd_kernel(const T* logits, long long ld, const long long* targets, const float2* stats, const float* row_grad,
-                         const float* gscale_dev, float gscale, K2 k, T* dlogits, long long ldd, int V, int cols,
+                         const float* gscale_dev, float gscale, K2 k, T* dlogits, long long ldd, int rows, int V, int cols,
                          long long ignore_index, const double* pair_loss, int pairs, float* loss) {
   bb::pdl_sync();
-  if (pair_loss && blockIdx.x == 0) mean_of<THREADS>(pair_loss, pairs, loss);     // (the preference loss: one launch less)
-  const int row = gridDim.x - 1 - blockIdx.x;     // the rows that the forward pass read last may still be in L2
+  if (pair_loss && blockIdx.x == 0) mean_of<BLOCK<THREADS>>(pair_loss, pairs, loss);     // (the preference loss: one launch less)
+  const int block = gridDim.x - 1 - blockIdx.x;     // the rows that the forward pass read last may still be in L2
+  const int row = THREADS == 32 ? block * ROWS_OF_BLOCK<THREADS> + (int)(threadIdx.x >> 5) : block;
+  if (row >= rows) return;
   const long long t = targets[row];
   const float2 st = stats[row];
   const bool counted = t != ignore_index && t >= 0 && t < V;
   const float g = counted ? row_grad[row] * (gscale_dev ? gscale_dev[0] : 1.f) * gscale : 0.f;
-  grad_row<T, THREADS, GRAD_LOADS>(logits + (size_t)row * ld, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, st.x, st.y);
+  grad_row<T, THREADS, THREADS == 32 ? ROW_LOADS : GRAD_LOADS>(logits + (size_t)row * ld, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, st.x, st.y);
 }
 
 // Tokens [a, b) of sequence q: rows of `seq_len` tokens, or between two offsets.  Offsets that do not ascend within [0, tokens]
@@ -413,24 +448,30 @@ __global__ void __launch_bounds__(256)
 preference_pair_kernel(const float* logp, const float* ref, const long long* targets, const long long* offsets, long long seq_len,
                        long long tokens, int pairs, int form, double beta, double smoothing, int average, long long ignore_index,
                        double* pair_loss, float* rewards, float* row_grad, int* status) {
-  __shared__ double smem[8];
+  __shared__ double smem[8][4];
   bb::pdl_sync();
   const int pair = blockIdx.x;
-  double score[2], length[2];
+  double score[2], length[2], sums[4] = {0.0, 0.0, 0.0, 0.0};
   long long a[2], b[2];
+#pragma unroll
   for (int w = 0; w < 2; ++w) {
     sequence(offsets, seq_len, tokens, 2 * pair + w, a[w], b[w], status);
-    double sum = 0.0;
     int count = 0;
+#pragma unroll 4
     for (long long i = a[w] + threadIdx.x; i < b[w]; i += 256) {
-      if (targets[i] == ignore_index) continue;
-      sum += (double)logp[i] - (ref ? (double)ref[i] : 0.0);
-      ++count;
+      // (read without waiting for the target: what stands at a place that does not count is dropped, whatever it is)
+      const double d = (double)logp[i] - (ref ? (double)ref[i] : 0.0);
+      const bool counted = targets[i] != ignore_index;
+      sums[w] += counted ? d : 0.0;
+      count += counted;
     }
-    score[w] = block_sum<256>(sum, smem);
-    const double n = block_sum<256>((double)count, smem);
-    length[w] = average ? (n > 1.0 ? n : 1.0) : 1.0;
-    score[w] /= length[w];
+    sums[2 + w] = (double)count;
+  }
+  block_sums<256, 4>(sums, smem);
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    length[w] = average ? fmax(sums[2 + w], 1.0) : 1.0;
+    score[w] = sums[w] / length[w];
   }
   const double h = beta * (score[0] - score[1]);
   double loss, slope;
@@ -556,10 +597,10 @@ template <bool FROM_ROWS>
 __global__ void __launch_bounds__(256)
 policy_token_kernel(float* logp, const PolicyRow* row_sums, K2 k, const long long* targets, const PolicyParams p, long long tokens, long long ignore_index,
                     float* row_grad, double* partial, int* done, float* loss, float* stats) {
-  __shared__ double smem[8];
+  __shared__ double smem[8][4];
   __shared__ int s_last;
   bb::pdl_sync();
-  double v[3] = {0.0, 0.0, 0.0};
+  double v[4] = {0.0, 0.0, 0.0, 0.0};
   const float whole = p.weight ? 0.f : policy_weight(p, 0);
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < tokens; i += (long long)gridDim.x * 256) {
     const float w = p.weight ? p.weight[i] : whole;
@@ -577,24 +618,25 @@ policy_token_kernel(float* logp, const PolicyRow* row_sums, K2 k, const long lon
     if constexpr (!FROM_ROWS) row_grad[i] = o.slope * w;
     v[0] += (double)o.loss * w; v[1] += o.kl; v[2] += o.clipped;
   }
-  for (int c = 0; c < 3; ++c) v[c] = block_sum<256>(v[c], smem);
-  if (threadIdx.x == 0) {
-    for (int c = 0; c < 3; ++c) __stcg(partial + 3 * blockIdx.x + c, v[c]);
+  if (gridDim.x > 1) {
+    block_sums<256, 4>(v, smem);
+    if (threadIdx.x == 0) {
+      for (int c = 0; c < 3; ++c) __stcg(partial + 3 * blockIdx.x + c, v[c]);
+      __threadfence();
+      s_last = atomicAdd(done, 1) == (int)gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!s_last) return;
     __threadfence();
-    s_last = atomicAdd(done, 1) == (int)gridDim.x - 1;
+    for (int c = 0; c < 3; ++c) v[c] = 0.0;
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += 256)
+      for (int c = 0; c < 3; ++c) v[c] += __ldcg(partial + 3 * i + c);
   }
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  for (int c = 0; c < 3; ++c) v[c] = 0.0;
-  for (int i = threadIdx.x; i < (int)gridDim.x; i += 256)
-    for (int c = 0; c < 3; ++c) v[c] += __ldcg(partial + 3 * i + c);
-  double total = 0.0;
-  for (int i = threadIdx.x; i < p.num_counts; i += 256) total += (double)p.counts[i];
-  for (int c = 0; c < 3; ++c) v[c] = block_sum<256>(v[c], smem);
-  total = block_sum<256>(total, smem);
+  v[3] = 0.0;
+  for (int i = threadIdx.x; i < p.num_counts; i += 256) v[3] += (double)p.counts[i];
+  block_sums<256, 4>(v, smem);
   if (threadIdx.x == 0) {
-    if (total < 1.0) total = 1.0;
+    const double total = fmax(v[3], 1.0);
     loss[0] = (float)v[0]; stats[0] = (float)(v[1] / total); stats[1] = (float)(v[2] / total);
   }
 }
@@ -610,13 +652,16 @@ __device__ __forceinline__ void policy_row_finish(const PolicyParams& p, const P
 // weights follow from the targets), that gradient too.  For rows that are short, or too long for policy_ring_kernel: the second half reads
 // the row again, from L1 or L2.
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(BLOCK<THREADS>)
 policy_row_kernel(const T* logits, long long ld, const long long* targets, const PolicyParams p, K2 k, float gscale,
                   T* dlogits, long long ldd, int rows, int V, int cols, long long ignore_index, PolicyRow* row_sums, int* status) {
-  __shared__ float2 smem[THREADS / 32];
-  __shared__ float s_row[3];
+  __shared__ float2 smem[BLOCK<THREADS> / 32];
+  __shared__ float s_row[BLOCK<THREADS> / 32][3];
   bb::pdl_sync();
-  const int row = blockIdx.x;
+  const int row = THREADS == 32 ? (int)blockIdx.x * ROWS_OF_BLOCK<THREADS> + (int)(threadIdx.x >> 5) : (int)blockIdx.x;
+  if (row >= rows) return;
+  float* mine = s_row[THREADS == 32 ? threadIdx.x >> 5 : 0];
+  const bool first = row_thread<THREADS>() == 0;
   const long long t = targets[row];
   const T* x = logits + (size_t)row * ld;
   const bool valid = t != ignore_index && t >= 0 && t < V, counted = valid && !(p.weight && p.weight[row] == 0.f);
@@ -625,12 +670,14 @@ policy_row_kernel(const T* logits, long long ld, const long long* targets, const
     // (in flight while the row is read: one after the other their latencies would stand between the two halves)
     PolicyInput in = {};
     float xt = 0.f, weight = 0.f;
-    if (threadIdx.x == 0) { in = policy_input(p, row); xt = Elem<T>::get(x + t); weight = policy_weight(p, row); }
+    if (first) { in = policy_input(p, row); xt = Elem<T>::get(x + t); weight = policy_weight(p, row); }
     soft_whole_row<T, THREADS, ROW_LOADS>(x, V, k, r, s, smem);
-    if (threadIdx.x == 0) policy_row_finish(p, in, row, xt, k, r, s, weight, gscale, s_row, row_sums);
-    __syncthreads();            // also: every thread is past its reads of the row before it may be overwritten
-    r = s_row[0]; s = s_row[1]; g = s_row[2];
-  } else if (threadIdx.x == 0) {
+    if (first) policy_row_finish(p, in, row, xt, k, r, s, weight, gscale, mine, row_sums);
+    // also: every thread is past its reads of the row before it may be overwritten
+    if constexpr (THREADS == 32) __syncwarp();
+    else __syncthreads();
+    r = mine[0]; s = mine[1]; g = mine[2];
+  } else if (first) {
     if (!valid && t != ignore_index) atomicCAS(status, 0, BB_ERR_INVALID_ARG);
     row_sums[row] = {0.f, 0.f, 0.f, 0.f};
   }
@@ -1097,8 +1144,12 @@ bool bad_list(const bb_grad_tensor* list, int count) {
 }
 
 template <typename T> struct FwdCall { const T* logits; long long ld; const long long* targets; K2 k; float* logp; float2* stats; int rows, V; long long ignore; int* status; cudaStream_t s; };
+// Blocks of a launch whose rows are worked on by THREADS threads each
+template <int THREADS> int row_blocks(int rows) { return (rows + ROWS_OF_BLOCK<THREADS> - 1) / ROWS_OF_BLOCK<THREADS>; }
+bool by_warps(size_t bytes, int rows, size_t limit) { return bytes <= TINY_ROW || (bytes <= limit && rows >= WARP_ROWS); }
 template <typename T, int THREADS> int fwd_rows(const FwdCall<T>& c) {
-  BB_CUDA_CHECK(bb_launch(token_logprob_fwd_kernel<T, THREADS>, c.rows, THREADS, 0, c.s, c.logits, c.ld, c.targets, c.k, c.logp, c.stats, c.V, c.ignore, c.status));
+  BB_CUDA_CHECK(bb_launch(token_logprob_fwd_kernel<T, THREADS>, row_blocks<THREADS>(c.rows), BLOCK<THREADS>, 0, c.s, c.logits, c.ld, c.targets, c.k, c.logp,
+                          c.stats, c.rows, c.V, c.ignore, c.status));
   return BB_OK;
 }
 // CTAs per row: while there are fewer rows than SMs, as many as keep every SM to one and a part above a chunk per thread
@@ -1109,7 +1160,7 @@ template <typename T> int fwd_parts(int rows, int V) {
 }
 template <typename T> int fwd_call(const FwdCall<T>& c) {
   const int parts = fwd_parts<T>(c.rows, c.V);
-  if (parts == 1) return fwd_rows<T, 256>(c);
+  if (parts == 1) return by_warps(c.V * sizeof(T), c.rows, WARP_SUM) ? fwd_rows<T, 32>(c) : fwd_rows<T, 256>(c);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(c.rows * parts); cfg.blockDim = dim3(256); cfg.stream = c.s;
   cudaLaunchAttribute attr[2];
@@ -1133,11 +1184,11 @@ template <typename T> struct BwdCall {
   long long ldd; int rows, V, cols; long long ignore; const double* pair_loss; int pairs; float* loss; cudaStream_t s;
 };
 template <typename T, int THREADS> int bwd_rows(const BwdCall<T>& c) {
-  BB_CUDA_CHECK(bb_launch(token_logprob_bwd_kernel<T, THREADS>, c.rows, THREADS, 0, c.s, c.logits, c.ld, c.targets, c.stats, c.row_grad, c.gscale_dev, c.gscale, c.k,
-                          c.dlogits, c.ldd, c.V, c.cols, c.ignore, c.pair_loss, c.pairs, c.loss));
+  BB_CUDA_CHECK(bb_launch(token_logprob_bwd_kernel<T, THREADS>, row_blocks<THREADS>(c.rows), BLOCK<THREADS>, 0, c.s, c.logits, c.ld, c.targets, c.stats, c.row_grad,
+                          c.gscale_dev, c.gscale, c.k, c.dlogits, c.ldd, c.rows, c.V, c.cols, c.ignore, c.pair_loss, c.pairs, c.loss));
   return BB_OK;
 }
-template <typename T> int bwd_call(const BwdCall<T>& c) { return bwd_rows<T, 256>(c); }
+template <typename T> int bwd_call(const BwdCall<T>& c) { return by_warps(c.V * sizeof(T), c.rows, WARP_GRAD) ? bwd_rows<T, 32>(c) : bwd_rows<T, 256>(c); }
 int logprob_bwd(const void* logits, int dtype, long long ld, const long long* targets, double scale, const float* stats, const float* row_grad,
                 const float* grad_scale_dev, float grad_scale, void* dlogits, long long ldd, long long rows, int vocab, int cols, long long ignore_index,
                 const double* pair_loss, int pairs, float* loss, cudaStream_t s) {
@@ -1261,12 +1312,13 @@ struct PolicyRowCall {
   PolicyRow* row_sums; int* status; int rows; int* ticket; cudaStream_t stream;
 };
 template <typename T, int THREADS> int policy_rows_as(const T* logits, T* dlogits, const PolicyRowCall& c) {
-  BB_CUDA_CHECK(bb_launch(policy_row_kernel<T, THREADS>, c.rows, THREADS, 0, c.stream, logits, c.ld, c.targets, c.p, c.k, c.gscale, dlogits, c.ldd, c.rows, c.V, c.cols,
+  BB_CUDA_CHECK(bb_launch(policy_row_kernel<T, THREADS>, row_blocks<THREADS>(c.rows), BLOCK<THREADS>, 0, c.stream, logits, c.ld, c.targets, c.p, c.k, c.gscale, dlogits, c.ldd, c.rows, c.V, c.cols,
                           c.ignore_index, c.row_sums, c.status));
   return BB_OK;
 }
 template <typename T> int policy_rows(const T* logits, T* dlogits, const PolicyRowCall& c) {
   const size_t bytes = (size_t)c.V * sizeof(T);
+  if (by_warps(bytes, c.rows, WARP_SUM)) return policy_rows_as<T, 32>(logits, dlogits, c);
   if (bytes <= LONG_ROW) return policy_rows_as<T, 256>(logits, dlogits, c);
   const size_t smem = bytes / 16 * 16;
   const int stages = (int)((smem + RING_STAGE - 1) / RING_STAGE);

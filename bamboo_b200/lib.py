@@ -144,6 +144,7 @@ def load():
         lib.bb_head_logprob_workspace_bytes.restype = ll
         lib.bb_head_logprob_fwd.argtypes = [vp] * 7 + [ll, vp]
         lib.bb_head_logprob_grad.argtypes = [vp] * 7 + [f, i, i, vp, ll, vp]
+        lib.bb_head_logprob_bwd.argtypes = [vp] * 10 + [i, vp, ll, vp]
         lib.bb_rescale_grad.argtypes = [vp, i, ll, ll, i, vp, f, vp]
         lib.bb_grad_norm_workspace_bytes.restype = ll
         lib.bb_grad_sumsq.argtypes = [vp, i, vp, ll, vp]
@@ -656,6 +657,16 @@ def head_logprob_grad(desc, hidden, weight, targets, stats, row_grad, col0, cols
                                       row_grad.data_ptr(), _addr(grad_scale_dev), grad_scale, col0, cols, dlogits.data_ptr(), dlogits.stride(0),
                                       _raw_stream()), "bb_head_logprob_grad")
     return dlogits
+
+
+def head_logprob_bwd(desc, hidden, weight, targets, stats, row_grad, d_hidden, d_hidden_f32, d_weight, d_weight_accum, piece, dlogits):
+    """Gradients of hidden states (bf16) and weight (bf16, or added to fp32), each None where it is not wanted; ``dlogits``: room for a piece."""
+    global LAUNCHES
+    pieces = -(-desc.vocab // piece)
+    LAUNCHES += pieces * (1 + (d_hidden is not None) + (d_weight is not None or d_weight_accum is not None)) + (d_hidden is not None and pieces > 1)
+    check((_lib or load()).bb_head_logprob_bwd(ctypes.byref(desc), hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), stats.data_ptr(),
+                                               row_grad.data_ptr(), _addr(d_hidden), _addr(d_hidden_f32), _addr(d_weight), _addr(d_weight_accum), piece,
+                                               dlogits.data_ptr(), dlogits.stride(0), _raw_stream()), "bb_head_logprob_bwd")
 
 
 def preference_loss(desc, logp, ref, targets, offsets, loss, rewards, row_grad):

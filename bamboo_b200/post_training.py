@@ -127,6 +127,21 @@ def token_logprobs(logits, targets, vocab=None, *, temperature=1.0, ignore_index
 HEAD_GRAD_BYTES = 256 << 20
 
 
+@functools.lru_cache(maxsize=256)
+def _head_desc(rows, vocab, hidden, ld_hidden, ld_weight, scale, ignore_index):
+    return L.HeadDesc(rows=rows, vocab=vocab, hidden=hidden, ld_hidden=ld_hidden, ld_weight=ld_weight, scale=scale, ignore_index=ignore_index)
+
+
+def _aligned_rows(t, n):
+    """``t`` as [rows, n] with 16-byte rows (a copy only where its layout asks for one)."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t, n
+    t = t.detach().reshape(-1, n)
+    if t.stride(1) != 1 or t.stride(0) % 8 or t.stride(0) < n or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride(0)
+
+
 def _head_operands(hidden, weight, targets, vocab, scale, ignore_index):
     for name, t in (("hidden", hidden), ("weight", weight)):
         if not t.is_cuda:
@@ -134,71 +149,55 @@ def _head_operands(hidden, weight, targets, vocab, scale, ignore_index):
         if t.dtype != torch.bfloat16:
             raise L.BambooNativeError(f"{name}: bf16 expected, got {t.dtype}")
     n = hidden.shape[-1]
-    if weight.dim() != 2 or weight.shape[1] != n or weight.device != hidden.device:
+    if weight.dim() != 2 or weight.shape[1] != n or weight.get_device() != hidden.get_device():
         raise ValueError(f"weight {tuple(weight.shape)} on {weight.device} for hidden states of {n} on {hidden.device}")
-    vocab = weight.shape[0] if vocab is None else vocab
+    if vocab is None:
+        vocab = weight.shape[0]
     if not 0 < vocab <= weight.shape[0]:
         raise ValueError(f"vocab {vocab} does not fit a weight of {weight.shape[0]} rows")
-    if n % 8:
+    if n == 0 or n % 8:
         raise ValueError(f"hidden size {n}: a multiple of 8 is needed (16-byte rows)")
-
-    def rows_of(t):
-        ok = t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= n and t.data_ptr() % 16 == 0
-        return t if ok else t.clone(memory_format=torch.contiguous_format)
-    h2, w = rows_of(hidden.detach().reshape(-1, n)), rows_of(weight.detach())
-    tg = _flat(targets, "targets", h2.shape[0], torch.int64, h2.device)
-    desc = L.HeadDesc(rows=h2.shape[0], vocab=vocab, hidden=n, ld_hidden=h2.stride(0), ld_weight=w.stride(0), scale=scale, ignore_index=ignore_index)
-    return desc, h2, w, tg
+    (h, ld_h), (w, ld_w) = _aligned_rows(hidden, n), _aligned_rows(weight, n)
+    rows = h.numel() // n
+    return _head_desc(rows, vocab, n, ld_h, ld_w, scale, ignore_index), h, w, _flat(targets, "targets", rows, torch.int64, h.device)
 
 
-def _head_forward(desc, h2, w, tg):
-    logp = torch.empty(desc.rows, dtype=torch.float32, device=h2.device)
-    stats = torch.empty(desc.rows, 2, dtype=torch.float32, device=h2.device)
+def _head_forward(desc, h, w, tg, shape):
+    logp = torch.empty(shape, dtype=torch.float32, device=h.device)
+    stats = torch.empty(desc.rows, 2, dtype=torch.float32, device=h.device)
     if desc.rows:
-        L.head_logprob_fwd(desc, h2, w, tg, logp, stats)
+        L.head_logprob_fwd(desc, h, w, tg, logp, stats)
     return logp, stats
 
 
 class _HeadLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, vocab, scale, ignore_index):
-        desc, h2, w, tg = _head_operands(hidden, weight, targets, vocab, scale, ignore_index)
-        logp, stats = _head_forward(desc, h2, w, tg)
+        desc, h, w, tg = _head_operands(hidden, weight, targets, vocab, scale, ignore_index)
+        logp, stats = _head_forward(desc, h, w, tg, targets.shape)
         ctx.desc, ctx.weight, ctx.shape = desc, weight, hidden.shape
-        ctx.save_for_backward(h2, w, tg, stats)
-        return logp.view(targets.shape)
+        ctx.save_for_backward(h.detach(), w.detach(), tg, stats)
+        return logp
 
     @staticmethod
     def backward(ctx, grad):
-        h2, w, tg, stats = ctx.saved_tensors
-        desc, weight, dev = ctx.desc, ctx.weight, h2.device
+        h, w, tg, stats = ctx.saved_tensors
+        desc, weight, dev = ctx.desc, ctx.weight, h.device
         rows, n, vocab = desc.rows, desc.hidden, desc.vocab
         need_h, need_w = ctx.needs_input_grad[:2]
-        main = getattr(weight, "main_grad", None)
-        dh = torch.empty(rows, n, dtype=torch.bfloat16, device=dev) if need_h else None
+        main = getattr(weight, "main_grad", None) if need_w else None
+        dh = torch.empty(ctx.shape, dtype=torch.bfloat16, device=dev) if need_h else None
         dw = torch.empty(weight.shape, dtype=torch.bfloat16, device=dev) if need_w and main is None else None
-        if dw is not None:
+        if dw is not None and (vocab < dw.shape[0] or not rows):
             dw[vocab if rows else 0:].zero_()
-        if not rows:
-            return (None if dh is None else dh.view(ctx.shape)), dw, None, None, None, None
-        row_grad = _flat(grad, "gradient", rows, torch.float32, dev)
-        # vocabulary entries in pieces, so that the gradient of the logits never exists whole; a multiple of 256, the widest tile
-        piece = min(vocab, max(2048, HEAD_GRAD_BYTES // (2 * rows) // 256 * 256))
-        whole = piece >= vocab
-        acc = torch.zeros(rows, n, dtype=torch.float32, device=dev) if need_h and not whole else None
-        buffer = torch.empty(rows, (piece + 7) // 8 * 8, dtype=torch.bfloat16, device=dev)
-        for col0 in range(0, vocab, piece):
-            cols = min(piece, vocab - col0)
-            d = L.head_logprob_grad(desc, h2, w, tg, stats, row_grad, col0, cols, buffer)
-            if need_h:
-                L.gemm(d, w[col0:], dh if whole else acc, b_mn=True, epilogue=L.EPI_STORE if whole else L.EPI_ACCUM_F32, M=rows, N=n, K=cols)
-            if dw is not None:
-                L.gemm(d, h2, dw[col0:], a_mn=True, b_mn=True, M=cols, N=n, K=rows)
-            elif need_w:
-                L.gemm(d, h2, main[col0:], a_mn=True, b_mn=True, epilogue=L.EPI_ACCUM_F32, M=cols, N=n, K=rows)
-        if acc is not None:
-            L.cast_f32_to_bf16(acc, dh)
-        return (None if dh is None else dh.view(ctx.shape)), dw, None, None, None, None
+        if rows:
+            # vocabulary entries in pieces, so that the gradient of the logits never exists whole; a multiple of 256, the widest tile
+            piece = max(2048, HEAD_GRAD_BYTES // (2 * rows) // 256 * 256)
+            width = (min(piece, vocab) + 7) // 8 * 8
+            acc = torch.empty(rows, n, dtype=torch.float32, device=dev) if need_h and piece < vocab else None
+            L.head_logprob_bwd(desc, h, w, tg, stats, _flat(grad, "gradient", rows, torch.float32, dev), dh, acc, dw, main, piece,
+                               torch.empty(rows, width, dtype=torch.bfloat16, device=dev))
+        return dh, dw, None, None, None, None
 
 
 def head_logprobs(hidden, weight, targets, vocab=None, *, temperature=1.0, ignore_index=-100):
@@ -210,7 +209,7 @@ def head_logprobs(hidden, weight, targets, vocab=None, *, temperature=1.0, ignor
     scale = _inverse(temperature)
     if _wants_grad(hidden) or _wants_grad(weight):
         return _HeadLogprobsFn.apply(hidden, weight, targets, vocab, scale, ignore_index)
-    return _head_forward(*_head_operands(hidden, weight, targets, vocab, scale, ignore_index))[0].view(targets.shape)
+    return _head_forward(*_head_operands(hidden, weight, targets, vocab, scale, ignore_index), targets.shape)[0]
 
 
 # ----------------------------------------------------------------------------------- losses over log-probabilities
