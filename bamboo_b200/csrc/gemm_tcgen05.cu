@@ -99,7 +99,7 @@ struct HeadParams {
   float2* partial;            // SUMS: (r, s) of each half of a tile's columns, [2 * column tiles][M]
   float* target_logit;        // SUMS: logit of the target, [M]
   const float2* stats;        // GRAD: (r, s) per row
-  const float* row_grad; const float* gscale_dev; float gscale;
+  const float* row_grad; float gscale;
 };
 // The tensor core's fp32 additions truncate, so a sum's error grows with the number of its k-blocks (a logit of 4096 products
 // 4.6e-5 off, of 1024 products 2.4e-6).  Projections from more than 2048 columns sum the halves of the reduction into the two
@@ -576,7 +576,7 @@ template <int HEAD> struct HeadRow {
       if (target < 0) return;
       const float2 st = h.stats[row];
       r = st.x; s = st.y;
-      g = s == 0.f ? 0.f : h.row_grad[row] * (h.gscale_dev ? h.gscale_dev[0] : 1.f) * h.gscale;
+      g = s == 0.f ? 0.f : h.row_grad[row] * h.gscale;
     }
   }
   __device__ __forceinline__ void sums(const HeadParams& h, int nb, int N, int row, int M, float* v) {
@@ -1691,39 +1691,37 @@ extern "C" int bb_head_logprob_fwd(const bb_head_desc* d, const void* hidden_sta
   return BB_OK;
 }
 
-extern "C" int bb_head_logprob_grad(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets, const float* stats,
-                                    const float* row_grad, const float* grad_scale_dev, float grad_scale, int col0, int cols, void* dlogits,
-                                    long long ldd, void* stream) {
-  if (int rc = head_check("bb_head_logprob_grad", d, hidden_states, weight, targets)) return rc;
-  if (!stats || ((uintptr_t)stats & 7) || !row_grad || !dlogits || ((uintptr_t)dlogits & 15) || ldd % 8 || col0 < 0 || cols <= 0 || cols > d->vocab - col0 || ldd < cols) {
-    bb_set_last_error_msg("bb_head_logprob_grad: null or unaligned pointer, or columns that are no part of the vocabulary");
-    return BB_ERR_INVALID_ARG;
-  }
-  if (int rc = bbhost::bind_context()) return rc;
+namespace {
+// Gradient of the logits of vocabulary entries [col0, col0 + cols): the projection again, with an epilogue of its own
+int head_logits_grad(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets, const float* stats, const float* row_grad,
+                     int col0, int cols, void* dlogits, long long ldd, cudaStream_t s) {
   bb_gemm_desc g = {};
   g.M = d->rows; g.N = cols; g.K = d->hidden; g.A = hidden_states; g.lda = d->ld_hidden;
   g.B = (const __nv_bfloat16*)weight + (long long)col0 * d->ld_weight; g.ldb = d->ld_weight;
   g.D = dlogits; g.ldd = ldd; g.epilogue = BB_EPI_STORE;
   HeadParams h = head_params(d, targets);
-  h.col0 = col0; h.stats = (const float2*)stats; h.row_grad = row_grad; h.gscale_dev = grad_scale_dev; h.gscale = (float)(d->scale * grad_scale);
-  return head_launch<HEAD_GRAD>(g, h, (cudaStream_t)stream);
+  h.col0 = col0; h.stats = (const float2*)stats; h.row_grad = row_grad; h.gscale = (float)d->scale;
+  return head_launch<HEAD_GRAD>(g, h, s);
 }
+}  // namespace
 
 extern "C" int bb_head_logprob_bwd(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets, const float* stats,
                                    const float* row_grad, void* d_hidden, float* d_hidden_f32, void* d_weight, float* d_weight_accum, int piece,
                                    void* dlogits, long long ldd, void* stream) {
   if (int rc = head_check("bb_head_logprob_bwd", d, hidden_states, weight, targets)) return rc;
   const bool whole = piece >= d->vocab;
-  if (!dlogits || piece <= 0 || piece % 8 || ldd < (whole ? d->vocab : piece) || (d_weight && d_weight_accum) || (d_hidden && !whole && !d_hidden_f32)) {
-    bb_set_last_error_msg("bb_head_logprob_bwd: pieces are multiples of 8 entries that fit the buffer, several pieces need the fp32 buffer of d_hidden, and there is one weight gradient");
+  if (!stats || ((uintptr_t)stats & 7) || !row_grad || !dlogits || (((uintptr_t)dlogits | (uintptr_t)d_hidden | (uintptr_t)d_hidden_f32 | (uintptr_t)d_weight | (uintptr_t)d_weight_accum) & 15) ||
+      piece <= 0 || piece % 8 || ldd % 8 || ldd < (whole ? d->vocab : piece) || (d_weight && d_weight_accum) || (d_hidden && !whole && !d_hidden_f32)) {
+    bb_set_last_error_msg("bb_head_logprob_bwd: null or unaligned pointer, pieces that are no multiple of 8 or do not fit the buffer, no fp32 buffer for d_hidden over several pieces, or two weight gradients");
     return BB_ERR_INVALID_ARG;
   }
+  if (int rc = bbhost::bind_context()) return rc;
   cudaStream_t s = (cudaStream_t)stream;
   if (d_hidden && !whole) BB_CUDA_CHECK(cudaMemsetAsync(d_hidden_f32, 0, (size_t)d->rows * d->hidden * 4, s));
   BackToBack overlap;
   for (int col0 = 0; col0 < d->vocab; col0 += piece) {
     const int cols = piece < d->vocab - col0 ? piece : d->vocab - col0;
-    if (int rc = bb_head_logprob_grad(d, hidden_states, weight, targets, stats, row_grad, nullptr, 1.f, col0, cols, dlogits, ldd, stream)) return rc;
+    if (int rc = head_logits_grad(d, hidden_states, weight, targets, stats, row_grad, col0, cols, dlogits, ldd, s)) return rc;
     bb_gemm_desc g = {};
     g.A = dlogits; g.lda = ldd;
     if (d_hidden) {

@@ -42,6 +42,7 @@ from .config import PipeConfig
 from .module import PipelineModule
 from .p2p import ACT, GRAD, DistTransport, NullTransport, PeerTimeout
 from .partition import get_redundant_stage_ids, get_redundant_user_stage_ids
+from .post_training import PolicyLoss
 
 should_stop = False
 _live_stores = []
@@ -271,8 +272,8 @@ class PipelineEngine:
         self.total_loss = None
         self.agg_train_loss = None
         self.loss_model = self.module.loss_fn
-        if hasattr(self.loss_model, "grad_scale"):
-            # a loss that makes its gradient with its value: every micro-batch contributes loss / GAS
+        if isinstance(self.loss_model, PolicyLoss):
+            # it makes its gradient with its value: every micro-batch contributes loss / GAS
             self.loss_model.grad_scale = 1.0 / self.micro_batches
         self._global_grad_norm, self._clip_epoch = None, 0
         self._compute_loss = True

@@ -143,7 +143,6 @@ def load():
         lib.bb_policy_loss_logits.argtypes = [vp, vp, i, ll, d, i, i] + [vp] * 9 + [ll, f, vp, ll, vp]
         lib.bb_head_logprob_workspace_bytes.restype = ll
         lib.bb_head_logprob_fwd.argtypes = [vp] * 7 + [ll, vp]
-        lib.bb_head_logprob_grad.argtypes = [vp] * 7 + [f, i, i, vp, ll, vp]
         lib.bb_head_logprob_bwd.argtypes = [vp] * 10 + [i, vp, ll, vp]
         lib.bb_rescale_grad.argtypes = [vp, i, ll, ll, i, vp, f, vp]
         lib.bb_grad_norm_workspace_bytes.restype = ll
@@ -647,16 +646,6 @@ def head_logprob_fwd(desc, hidden, weight, targets, logp, stats):
     check(lib.bb_head_logprob_fwd(ctypes.byref(desc), hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), logp.data_ptr(), stats.data_ptr(),
                                   ws.data_ptr(), ws.numel(), _raw_stream()), "bb_head_logprob_fwd")
     return logp
-
-
-def head_logprob_grad(desc, hidden, weight, targets, stats, row_grad, col0, cols, dlogits, grad_scale=1.0, grad_scale_dev=None):
-    """Gradient of the logits of vocabulary entries [col0, col0 + cols) into dlogits [rows, >= cols] bf16."""
-    global LAUNCHES
-    LAUNCHES += 1
-    check(load().bb_head_logprob_grad(ctypes.byref(desc), hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), stats.data_ptr(),
-                                      row_grad.data_ptr(), _addr(grad_scale_dev), grad_scale, col0, cols, dlogits.data_ptr(), dlogits.stride(0),
-                                      _raw_stream()), "bb_head_logprob_grad")
-    return dlogits
 
 
 def head_logprob_bwd(desc, hidden, weight, targets, stats, row_grad, d_hidden, d_hidden_f32, d_weight, d_weight_accum, piece, dlogits):

@@ -24,11 +24,19 @@ from . import lib as L
 
 
 # ----------------------------------------------------------------------------------- arguments
+def _on_current(t, name):
+    """The kernels run on the current device's stream: tensors of another device are refused, as are CPU tensors."""
+    where = t.get_device()
+    if where < 0:
+        raise L.BambooNativeError(f"{name}: expected a CUDA tensor; the sm_100a kernels have no CPU fallback")
+    if where != torch._C._cuda_getDevice():
+        raise L.BambooNativeError(f"{name}: on cuda:{where}, but cuda:{torch._C._cuda_getDevice()} is the current device")
+
+
 def _rows(logits, vocab):
     """(logits, rows, vocab): contiguous logits [..., cols] as they are, others as [rows, cols] with unit inner stride (a copy only where
     their strides ask for one)."""
-    if not logits.is_cuda:
-        raise L.BambooNativeError("logits: expected a CUDA tensor; the sm_100a kernels have no CPU fallback")
+    _on_current(logits, "logits")
     cols = logits.shape[-1]
     if vocab is None:
         vocab = cols
@@ -144,13 +152,12 @@ def _aligned_rows(t, n):
 
 def _head_operands(hidden, weight, targets, vocab, scale, ignore_index):
     for name, t in (("hidden", hidden), ("weight", weight)):
-        if not t.is_cuda:
-            raise L.BambooNativeError(f"{name}: expected a CUDA tensor; the sm_100a kernels have no CPU fallback")
+        _on_current(t, name)
         if t.dtype != torch.bfloat16:
             raise L.BambooNativeError(f"{name}: bf16 expected, got {t.dtype}")
     n = hidden.shape[-1]
-    if weight.dim() != 2 or weight.shape[1] != n or weight.get_device() != hidden.get_device():
-        raise ValueError(f"weight {tuple(weight.shape)} on {weight.device} for hidden states of {n} on {hidden.device}")
+    if weight.dim() != 2 or weight.shape[1] != n:
+        raise ValueError(f"weight {tuple(weight.shape)} for hidden states of {n}")
     if vocab is None:
         vocab = weight.shape[0]
     if not 0 < vocab <= weight.shape[0]:
@@ -264,8 +271,7 @@ def preference_loss(logps, ref_logps, targets, *, beta=0.1, form="sigmoid", labe
 
 
 def _preference(lp, ref, targets, offsets, desc):
-    if not lp.is_cuda:
-        raise L.BambooNativeError("logps: expected a CUDA tensor; the sm_100a kernels have no CPU fallback")
+    _on_current(lp, "logps")
     n, dev = desc.tokens, lp.device
     tg = _flat(targets, "targets", n, torch.int64, dev)
     ref = None if ref is None else _flat(ref, "ref_logps", n, torch.float32, dev)
@@ -284,8 +290,7 @@ def policy_loss(logps, old_logps, advantages, targets, *, ref_logps=None, clip_l
     2-D ``targets``.  ``reduction``: "token" averages over all counted tokens, "sequence" averages the sequences' means."""
     sequences, offsets = _geometry(targets, offsets)
     lp = _flat(logps, "logps", targets.numel(), torch.float32, targets.device)
-    if not lp.is_cuda:
-        raise L.BambooNativeError("logps: expected a CUDA tensor; the sm_100a kernels have no CPU fallback")
+    _on_current(lp, "logps")
     desc = _policy_desc(lp.numel(), sequences, advantages.numel(), clip_low, clip_high, kl_coef, reduction, ignore_index)
     loss, stats = torch.empty((), dtype=torch.float32, device=lp.device), torch.empty(2, dtype=torch.float32, device=lp.device)
     row_grad = torch.empty_like(lp)
@@ -467,10 +472,9 @@ def _gradients(tensors):
         n = t.numel()
         if n == 0:
             continue
-        where = t.get_device()
-        if where < 0 or (device is not None and where != device):
-            raise L.BambooNativeError("gradients: CUDA tensors of one device are expected; the sm_100a kernels have no CPU fallback")
-        device = where
+        if t.get_device() != device:
+            _on_current(t, "gradients")
+            device = t.get_device()
         if not t.is_contiguous() and not _dense(t):
             gradient, t = t.detach(), t.detach().contiguous()
             staged.append((gradient, t))
@@ -517,7 +521,13 @@ def adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, *, max_norm, 
     if not max_norm > 0:
         raise ValueError(f"max_norm has to be positive, got {max_norm}")
     for t in (master, grad, exp_avg, exp_avg_sq):
-        if not t.is_cuda or t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != master.numel():
+        _on_current(t, "adam_step_clipped")
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != master.numel():
             raise L.BambooNativeError("adam_step_clipped: contiguous fp32 CUDA tensors of one size are expected")
+    if param_lp is not None and (param_lp.get_device() != master.get_device() or param_lp.dtype != torch.bfloat16 or
+                                 not param_lp.is_contiguous() or param_lp.numel() != master.numel()):
+        raise L.BambooNativeError("adam_step_clipped: the working copy is contiguous bf16, of the arena's size")
+    if sumsq is not None and (sumsq.get_device() != master.get_device() or sumsq.dtype != torch.float64):
+        raise L.BambooNativeError("adam_step_clipped: sumsq is fp64, on the arena's device")
     norm = torch.empty((), dtype=torch.float32, device=master.device)
     return L.adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, grad_scale=grad_scale, sumsq=sumsq, max_norm=max_norm, norm=norm, **adam)

@@ -319,10 +319,9 @@ int bb_token_logprob_bwd(const void* logits, int dtype, long long ld, const long
                          long long rows, int vocab, int cols, long long ignore_index, void* stream);
 
 /* The same from hidden states, through the vocabulary projection, without storing the logits: logits = hidden_states [rows,
- * hidden] * weight [vocab, hidden]^T (bf16, rows 16-byte aligned; fp32 accumulation, the logits are not rounded).  _fwd: one
- * GEMM whose epilogue keeps softmax sums, and a small kernel that joins them.  _grad: the gradient of the logits for vocabulary entries
- * [col0, col0 + cols) (bf16 [rows, cols], row stride ldd), from a second GEMM over the same operands; the input and weight
- * gradients are bb_gemm_bf16 products of it.  A logit so large that scale * log2(e) * logit overflows counts as infinite here. */
+ * hidden] * weight [vocab, hidden]^T (bf16, rows 16-byte aligned; fp32 accumulation, the logits are not rounded): one GEMM
+ * whose epilogue keeps softmax sums, and a small kernel that joins them.  A logit so large that scale * log2(e) * logit
+ * overflows counts as infinite here. */
 typedef struct bb_head_desc {
   int rows, vocab, hidden;
   long long ld_hidden, ld_weight;
@@ -332,11 +331,8 @@ typedef struct bb_head_desc {
 long long bb_head_logprob_workspace_bytes(const bb_head_desc* d);
 int bb_head_logprob_fwd(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets, float* logp,
                         float* stats, void* workspace, long long workspace_bytes, void* stream);
-int bb_head_logprob_grad(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets,
-                         const float* stats, const float* row_grad, const float* grad_scale_dev, float grad_scale, int col0,
-                         int cols, void* dlogits, long long ldd, void* stream);
-/* The backward pass in one call: pieces of `piece` vocabulary entries (a multiple of 8), of each the gradient of the logits
- * into `dlogits` (bf16 [rows, ldd]) and its products into the input gradient d_hidden (bf16 [rows, hidden]; over several pieces
+/* The backward pass computes the logits again, in pieces of `piece` vocabulary entries (a multiple of 8): of each the gradient
+ * of the logits into `dlogits` (bf16 [rows, ldd]) and its products into the input gradient d_hidden (bf16 [rows, hidden]; over several pieces
  * through the fp32 buffer d_hidden_f32 of the same shape) and the weight gradient: d_weight (bf16 [vocab, hidden]), or
  * d_weight_accum (fp32, +=).  A gradient that is not wanted is NULL. */
 int bb_head_logprob_bwd(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets,

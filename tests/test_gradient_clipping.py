@@ -173,7 +173,7 @@ def test_descriptors_match_the_header():
     assert lib._tensor_table(3).size == 3 * 24
 
 
-def test_cpu_tensors_are_refused():
+def test_cpu_tensors_are_refused(monkeypatch):
     from bamboo_b200 import lib, post_training as pt
     x, t = torch.zeros(4, 16), torch.zeros(4, dtype=torch.int64)
     calls = (lambda: pt.token_logprobs(x, t), lambda: pt.head_logprobs(x.bfloat16(), x.bfloat16(), t),
@@ -183,6 +183,9 @@ def test_cpu_tensors_are_refused():
     for call in calls:
         with pytest.raises(lib.BambooNativeError):
             call()
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0)
+    with pytest.raises(lib.BambooNativeError, match="current device"):         # another device's tensor is refused before a launch
+        pt._on_current(type("OnThird", (), {"get_device": lambda self: 3})(), "x")
     import deepspeed.runtime.utils as ds_utils
     with pytest.raises(NotImplementedError):
         ds_utils.clip_grad_norm_([x], 1.0, norm_type=1)
