@@ -1607,17 +1607,27 @@ head_combine_kernel(const float2* partial, int num, int rows, const float* targe
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int row = blockIdx.x * 32 + lane;
   float r = -INFINITY, s = 0.f;
+  // (what the row's last step needs, under way while the sums are read)
+  const int own = blockIdx.x * 32 + warp;
+  long long t = ignore_index;
+  float xt = 0.f;
+  if (lane == 0 && own < rows) {
+    t = targets[own];
+    if (t != ignore_index && t >= 0 && t < vocab) xt = target_logit[own];
+  }
   if (row < rows) {
-#pragma unroll 4
-    for (int i = warp; i < num; i += 32) {
-      const float2 q = __ldcg(partial + (long long)i * rows + row);
-      bb::soft_merge(r, s, q.x, q.y);
+    for (int i = warp; i < num; i += 32 * 8) {
+      float2 q[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) q[u] = i + 32 * u < num ? __ldcg(partial + (long long)(i + 32 * u) * rows + row) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) bb::soft_merge(r, s, q[u].x, q[u].y);
     }
   }
   sums[lane][warp] = make_float2(r, s);
   __syncthreads();
   // the warps' sums of row `warp` of the CTA, one per lane
-  row = blockIdx.x * 32 + warp;
+  row = own;
   const float2 q = sums[warp][lane];
   float top = q.x;
 #pragma unroll
@@ -1627,10 +1637,9 @@ head_combine_kernel(const float2* partial, int num, int rows, const float* targe
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane != 0 || row >= rows) return;
-  const long long t = targets[row];
   const bool counted = t != ignore_index && t >= 0 && t < vocab;
   if (!counted && t != ignore_index) atomicCAS(status, 0, BB_ERR_INVALID_ARG);
-  logp[row] = counted ? (float)bb::row_logp(target_logit[row], k, r, s) : 0.f;
+  logp[row] = counted ? (float)bb::row_logp(xt, k, r, s) : 0.f;
   stats[row] = counted ? make_float2(r, s) : make_float2(0.f, 0.f);
 }
 
