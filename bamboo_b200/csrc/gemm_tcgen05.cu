@@ -1643,6 +1643,19 @@ head_combine_kernel(const float2* partial, int num, int rows, const float* targe
   stats[row] = counted ? make_float2(r, s) : make_float2(0.f, 0.f);
 }
 
+// out = hidden states, with zeros for the rows that do not count: the gradient of their logits is zero, but zero times what stands there
+// (NaN of a padded position) would be NaN in the weight gradient.  16 MB of 4096 x 1024: 5 us beside 1.15 ms.
+__global__ void __launch_bounds__(128)
+head_counted_rows_kernel(const __nv_bfloat16* h, long long ld, const long long* targets, long long ignore_index, int vocab, int hidden, __nv_bfloat16* out) {
+  bb::pdl_sync();
+  const int row = blockIdx.x;
+  const long long t = targets[row];
+  const bool counted = t != ignore_index && t >= 0 && t < vocab;
+  const uint4* src = reinterpret_cast<const uint4*>(h + (long long)row * ld);
+  uint4* dst = reinterpret_cast<uint4*>(out + (long long)row * hidden);
+  for (int c = threadIdx.x; c < hidden >> 3; c += 128) dst[c] = counted ? src[c] : make_uint4(0, 0, 0, 0);
+}
+
 // Tile of the projection, from the same expected times as any stored product (its epilogue stores nothing, but the main loop
 // is what the tile is chosen by)
 StorePlan head_plan(int rows, int vocab, int hidden) { return plan_store(rows, vocab, hidden, 0, true); }
@@ -1715,19 +1728,22 @@ int head_logits_grad(const bb_head_desc* d, const void* hidden_states, const voi
 }  // namespace
 
 extern "C" int bb_head_logprob_bwd(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets, const float* stats,
-                                   const float* row_grad, void* d_hidden, float* d_hidden_f32, void* d_weight, float* d_weight_accum, int piece,
-                                   void* dlogits, long long ldd, void* stream) {
+                                   const float* row_grad, void* d_hidden, float* d_hidden_f32, void* d_weight, float* d_weight_accum, void* counted_hidden,
+                                   int piece, void* dlogits, long long ldd, void* stream) {
   if (int rc = head_check("bb_head_logprob_bwd", d, hidden_states, weight, targets)) return rc;
   const bool whole = piece >= d->vocab;
-  if (!stats || ((uintptr_t)stats & 7) || !row_grad || !dlogits || (((uintptr_t)dlogits | (uintptr_t)d_hidden | (uintptr_t)d_hidden_f32 | (uintptr_t)d_weight | (uintptr_t)d_weight_accum) & 15) ||
-      piece <= 0 || piece % 8 || ldd % 8 || ldd < (whole ? d->vocab : piece) || (d_weight && d_weight_accum) || (d_hidden && !whole && !d_hidden_f32)) {
-    bb_set_last_error_msg("bb_head_logprob_bwd: null or unaligned pointer, pieces that are no multiple of 8 or do not fit the buffer, no fp32 buffer for d_hidden over several pieces, or two weight gradients");
+  if (!stats || ((uintptr_t)stats & 7) || !row_grad || !dlogits || (((uintptr_t)dlogits | (uintptr_t)d_hidden | (uintptr_t)d_hidden_f32 | (uintptr_t)d_weight | (uintptr_t)d_weight_accum | (uintptr_t)counted_hidden) & 15) ||
+      piece <= 0 || piece % 8 || ldd % 8 || ldd < (whole ? d->vocab : piece) || (d_weight && d_weight_accum) || ((d_weight || d_weight_accum) && !counted_hidden) || (d_hidden && !whole && !d_hidden_f32)) {
+    bb_set_last_error_msg("bb_head_logprob_bwd: null or unaligned pointer, pieces that are no multiple of 8 or do not fit the buffer, no fp32 buffer for d_hidden over several pieces, two weight gradients, or no counted_hidden for one");
     return BB_ERR_INVALID_ARG;
   }
   if (int rc = bbhost::bind_context()) return rc;
   cudaStream_t s = (cudaStream_t)stream;
   if (d_hidden && !whole) BB_CUDA_CHECK(cudaMemsetAsync(d_hidden_f32, 0, (size_t)d->rows * d->hidden * 4, s));
   BackToBack overlap;
+  if (d_weight || d_weight_accum)
+    BB_CUDA_CHECK(bb_launch(head_counted_rows_kernel, d->rows, 128, 0, s, (const __nv_bfloat16*)hidden_states, d->ld_hidden, targets, d->ignore_index, d->vocab, d->hidden,
+                            (__nv_bfloat16*)counted_hidden));
   for (int col0 = 0; col0 < d->vocab; col0 += piece) {
     const int cols = piece < d->vocab - col0 ? piece : d->vocab - col0;
     if (int rc = head_logits_grad(d, hidden_states, weight, targets, stats, row_grad, col0, cols, dlogits, ldd, s)) return rc;
@@ -1739,7 +1755,7 @@ extern "C" int bb_head_logprob_bwd(const bb_head_desc* d, const void* hidden_sta
       if (int rc = bb_gemm_bf16(&g, stream)) return rc;
     }
     if (d_weight || d_weight_accum) {
-      g.M = cols; g.N = d->hidden; g.K = d->rows; g.a_mn_major = 1; g.B = hidden_states; g.ldb = d->ld_hidden; g.b_mn_major = 1; g.ldd = d->hidden;
+      g.M = cols; g.N = d->hidden; g.K = d->rows; g.a_mn_major = 1; g.B = counted_hidden; g.ldb = d->hidden; g.b_mn_major = 1; g.ldd = d->hidden;
       g.D = d_weight ? (void*)((__nv_bfloat16*)d_weight + (long long)col0 * d->hidden) : (void*)(d_weight_accum + (long long)col0 * d->hidden);
       g.epilogue = d_weight ? BB_EPI_STORE : BB_EPI_ACCUM_F32;
       if (int rc = bb_gemm_bf16(&g, stream)) return rc;

@@ -279,11 +279,16 @@ def test_head_rows_that_do_not_count_and_refusals(pt):
     t = torch.tensor([3, IGNORE, 99, IGNORE, 0], device="cuda")
     want = ref_head(h, w, t, 100, 1.0)
     h[1], h[3] = math.nan, math.inf
-    hl = h.clone().requires_grad_(True)
-    out = pt.head_logprobs(hl, w, t)
+    hl, wl = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    out = pt.head_logprobs(hl, wl, t)
     near(out.detach(), want, 1e-6, 2e-5)
     out.sum().backward()
     assert torch.isfinite(hl.grad).all() and torch.all(hl.grad[[1, 3]] == 0)
+    assert torch.isfinite(wl.grad).all()                  # zero times NaN of a row that does not count stays out of it
+    p = torch.nn.Parameter(w.clone())
+    p.main_grad = torch.zeros(100, 64, device="cuda")
+    pt.head_logprobs(h, p, t).sum().backward()
+    near(p.main_grad.bfloat16(), wl.grad.double(), 2 ** -7, 1e-6)
     out = pt.head_logprobs(h, w, torch.tensor([3, 100, -7, IGNORE, 0], device="cuda"))
     torch.cuda.synchronize()
     assert lib.read_status() < 0 and torch.all(out[1:4] == 0)
@@ -531,6 +536,48 @@ def test_policy_loss_from_logits(pt, dtype, reduction, vocab, cols, lengths):
             near(leaf.grad, 0.5 * grad.double(), 2 ** -8 if dtype == torch.bfloat16 else 2 ** -23, 1e-38)
     over = x.clone()
     assert torch.equal(loss_fn.loss_and_grad(over, (t, old, adv, ref), offsets=offsets, out=over, grad_scale=0.5)[2], grad)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("offset", [0, 1, 3])
+@pytest.mark.parametrize("vocab", [1003, 30011])
+def test_losses_on_rows_that_start_anywhere(pt, vocab, offset, dtype):
+    """Windows of a wider matrix: gradients beside them (another alignment) and over them, with nothing around touched."""
+    rows, ld = 24, vocab + 18
+    whole = logits_of(rows, ld, ld, dtype, 45)
+    x, t = whole[:, offset:offset + vocab], targets_of(rows, vocab, 46)
+    lp, _, _ = ref_logps(x, t, vocab)
+    old, adv, ref = policy_inputs(lp, 47)
+    offsets = torch.tensor([0, 5, 12, 13, 24], device="cuda")
+    for fn, labels in ((pt.PolicyLoss(vocab, clip_high=0.3, kl_coef=0.05), (t, old, adv, ref)), (pt.PreferenceLoss(vocab), (t, ref))):
+        loss, extra, want = fn.loss_and_grad(x.contiguous(), labels, offsets=offsets)
+        beside = fn.loss_and_grad(x, labels, offsets=offsets)
+        near(beside[0].reshape(1), loss.double().reshape(1), 1e-6, 1e-6)
+        # (rows that start elsewhere are summed in another order: a unit or two in the last place of the sums)
+        near(beside[2], want.double(), 2 ** -7 if dtype == torch.bfloat16 else 4e-6, 1e-7)
+        over = whole.clone()
+        got = fn.loss_and_grad(over[:, offset:offset + vocab], labels, offsets=offsets, out=over[:, offset:offset + vocab])[2]
+        assert torch.equal(got, beside[2])
+        assert torch.equal(over[:, :offset], whole[:, :offset]) and torch.equal(over[:, offset + vocab:], whole[:, offset + vocab:])
+
+
+def test_more_than_two_to_the_31_logits(pt):
+    rows, vocab, cols = 43000, 50257, 50304
+    x = torch.empty(rows, cols, device="cuda", dtype=torch.bfloat16)
+    x[:-3] = 0
+    x[-3:] = logits_of(3, cols, cols, torch.bfloat16, 48)
+    t = torch.full((rows,), IGNORE, device="cuda")
+    t[-3:] = torch.tensor([50256, 0, 777], device="cuda")
+    tail = x[-3:].clone()
+    lp, probs, counted = ref_logps(tail, t[-3:], vocab)
+    near(pt.token_logprobs(x, t, vocab)[-3:], lp, 1e-6, 1e-6)
+    fn = pt.PolicyLoss(vocab, inplace=True)
+    labels = (t.view(1, -1), None, torch.ones(rows, device="cuda").view(1, -1))
+    loss, _, grad = fn.loss_and_grad(x.view(1, rows, cols), labels, out=x.view(1, rows, cols))
+    near(loss.reshape(1), torch.tensor([-1.0], dtype=torch.float64, device="cuda"), 1e-6, 0)
+    want = ref_dlogits(probs, counted, t[-3:], torch.full((3,), -1 / 3, device="cuda"), cols)
+    near(grad[0, -3:], want, 2 ** -8, 1e-7)
+    assert torch.all(x[:-3] == 0)
 
 
 # ----------------------------------------------------------------------------------- gradient norm and clipping
