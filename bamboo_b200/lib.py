@@ -137,7 +137,7 @@ def load():
         lib.bb_token_logprob_bwd.argtypes = [vp, i, ll, vp, d, vp, vp, vp, f, vp, ll, ll, i, i, ll, vp]
         lib.bb_preference_workspace_bytes.restype = ll
         lib.bb_preference_loss.argtypes = [vp] * 9 + [ll, vp]
-        lib.bb_preference_loss_logits.argtypes = [vp, vp, i, ll, d, i, i] + [vp] * 6 + [ll, f, vp, ll, vp]
+        lib.bb_preference_loss_logits.argtypes = [vp, vp, i, ll, d, i, i] + [vp] * 8 + [ll, f, vp, ll, vp]
         lib.bb_policy_workspace_bytes.restype = ll
         lib.bb_policy_loss.argtypes = [vp] * 11 + [ll, vp]
         lib.bb_policy_loss_logits.argtypes = [vp, vp, i, ll, d, i, i] + [vp] * 9 + [ll, f, vp, ll, vp]
@@ -670,14 +670,15 @@ def preference_loss(desc, logp, ref, targets, offsets, loss, rewards, row_grad):
     return loss
 
 
-def preference_loss_logits(desc, logits, targets, vocab, ref, offsets, loss, rewards, dlogits, scale=1.0, grad_scale=1.0):
+def preference_loss_logits(desc, logits, targets, vocab, ref, offsets, loss, rewards, dlogits, scale=1.0, grad_scale=1.0, stats=None, row_grad=None):
+    """dlogits None: loss and rewards alone, and what the backward pass needs into stats [tokens, 2] and row_grad [tokens], where given."""
     global LAUNCHES
     LAUNCHES += 3
     lib = load()
     ws = workspace(_bytes_of(desc, lib.bb_preference_workspace_bytes), "post_training")
     check(lib.bb_preference_loss_logits(ctypes.byref(desc), logits.data_ptr(), _dtype(logits, "logits"), _ld(logits), scale, vocab, logits.shape[-1],
-                                        _addr(ref), targets.data_ptr(), _addr(offsets), loss.data_ptr(), rewards.data_ptr(), dlogits.data_ptr(),
-                                        _ld(dlogits), grad_scale, ws.data_ptr(), ws.numel(), _raw_stream()), "bb_preference_loss_logits")
+                                        _addr(ref), targets.data_ptr(), _addr(offsets), loss.data_ptr(), rewards.data_ptr(), _addr(stats), _addr(row_grad),
+                                        _addr(dlogits), 0 if dlogits is None else _ld(dlogits), grad_scale, ws.data_ptr(), ws.numel(), _raw_stream()), "bb_preference_loss_logits")
     return loss
 
 

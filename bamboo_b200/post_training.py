@@ -311,7 +311,7 @@ def _policy_inputs(desc, old, advantages, ref, targets, dev):
 
 # ----------------------------------------------------------------------------------- losses from logits
 class _LogitsLossFn(torch.autograd.Function):
-    """loss_fn(logits, labels) with the gradient made by ``loss.forward_for_backward`` / ``loss.gradient``."""
+    """loss_fn(logits, labels) whose gradient the loss function makes itself (``_forward``, ``_backward``)."""
 
     @staticmethod
     def forward(ctx, logits, loss_fn, labels, offsets):
@@ -343,17 +343,19 @@ class PreferenceLoss:
         lg, rows, vocab = _rows(logits, self.vocab)
         sequences, offsets = _geometry(targets, offsets)
         tg = _flat(targets, "targets", rows, torch.int64, lg.device)
+        ref = None if ref is None else _flat(ref, "ref_logps", rows, torch.float32, lg.device)
         return lg, vocab, tg, ref, offsets, _preference_desc(rows, sequences, *self.form, self.ignore_index)
 
-    def _losses(self, logits, labels, offsets):
-        lg, vocab, tg, ref, offsets, desc = self._prepare(logits, labels, offsets)
-        logp, stats = _logprobs(lg, desc.tokens, tg, vocab, self.scale, self.ignore_index)
-        loss, self.rewards, row_grad = _preference(logp, ref, tg, offsets, desc)
-        return lg.detach(), tg, stats, row_grad, loss
+    def _run(self, lg, vocab, tg, ref, offsets, desc, dlogits=None, grad_scale=1.0, stats=None, row_grad=None):
+        loss = torch.empty((), dtype=torch.float32, device=lg.device)
+        self.rewards = torch.empty(desc.sequences, dtype=torch.float32, device=lg.device)
+        return L.preference_loss_logits(desc, lg, tg, vocab, ref, offsets, loss, self.rewards, dlogits, self.scale, grad_scale, stats, row_grad)
 
     def _forward(self, logits, labels, offsets):
-        *saved, loss = self._losses(logits, labels, offsets)
-        return loss, saved, ()
+        lg, vocab, tg, *rest = self._prepare(logits, labels, offsets)
+        lg, n = lg.detach(), tg.numel()
+        stats, row_grad = torch.empty(n, 2, dtype=torch.float32, device=lg.device), torch.empty(n, dtype=torch.float32, device=lg.device)
+        return self._run(lg, vocab, tg, *rest, stats=stats, row_grad=row_grad), (lg, tg, stats, row_grad), ()
 
     def _backward(self, saved, args, grad):
         lg, tg, stats, row_grad = saved
@@ -363,18 +365,14 @@ class PreferenceLoss:
     def __call__(self, logits, labels, offsets=None):
         if _wants_grad(logits):
             return _LogitsLossFn.apply(logits, self, labels, offsets)
-        return self._losses(logits, labels, offsets)[-1]
+        return self._run(*self._prepare(logits, labels, offsets))
 
     def loss_and_grad(self, logits, labels, *, offsets=None, out=None, grad_scale=1.0):
         """(loss, rewards, gradient of the logits times ``grad_scale``) without autograd; ``out`` receives the gradient (the logits
         themselves are allowed)."""
-        lg, vocab, tg, ref, offsets, desc = self._prepare(logits, labels, offsets)
-        ref = None if ref is None else _flat(ref, "ref_logps", desc.tokens, torch.float32, lg.device)
-        loss = torch.empty((), dtype=torch.float32, device=lg.device)
-        self.rewards = torch.empty(desc.sequences, dtype=torch.float32, device=lg.device)
+        args = self._prepare(logits, labels, offsets)
         d, grad = _gradient_buffer(logits, out)
-        L.preference_loss_logits(desc, lg, tg, vocab, ref, offsets, loss, self.rewards, d, self.scale, grad_scale)
-        return loss, self.rewards, grad
+        return self._run(*args, d, grad_scale), self.rewards, grad
 
 
 def _gradient_buffer(logits, out):

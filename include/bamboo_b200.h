@@ -361,10 +361,11 @@ int bb_preference_loss(const bb_preference_desc* d, const float* logp, const flo
                        const long long* offsets, float* loss, float* rewards, float* row_grad, void* workspace,
                        long long workspace_bytes, void* stream);
 /* The same from logits, and their gradient times grad_scale: the three passes in one call; arguments otherwise as in
- * bb_token_logprob_*. */
+ * bb_token_logprob_*.  The log-probabilities enter the scores unrounded.  Without dlogits (NULL) the first two passes alone, and stats
+ * and row_grad receive what bb_token_logprob_bwd takes (either may be NULL: kept in the workspace for this call). */
 int bb_preference_loss_logits(const bb_preference_desc* d, const void* logits, int dtype, long long ld, double scale, int vocab,
                               int cols, const float* ref, const long long* targets, const long long* offsets, float* loss,
-                              float* rewards, void* dlogits, long long ldd, float grad_scale, void* workspace,
+                              float* rewards, float* stats, float* row_grad, void* dlogits, long long ldd, float grad_scale, void* workspace,
                               long long workspace_bytes, void* stream);
 
 /* Clipped policy loss.  Per counted token: ratio = exp(logp - old) (old NULL: 1), surrogate = min(ratio A, clamp(ratio, 1 -

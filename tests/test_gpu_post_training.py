@@ -410,6 +410,19 @@ def test_preference_loss_from_logits(pt, dtype, vocab, cols, shape):
     assert out is over and torch.equal(over.view(rows, cols), grad.view(rows, cols))
 
 
+@pytest.mark.parametrize("vocab", [257, 32000])
+def test_rewards_of_a_policy_that_is_its_reference(pt, vocab):
+    # The reference's log-probabilities are the policy's own, rounded to fp32: the rewards are what that rounding left out.  A sum of
+    # vocab ex2 results, 2^-22 at most each and of either sign, is some 2^-24 off; rounding the policy's values too would add 3e-7.
+    rows = 512
+    x, t = logits_of(rows, vocab, vocab, torch.float32, 37), targets_of(rows, vocab, 38, 0.0)
+    lp, _, _ = ref_logps(x, t, vocab)
+    loss, rewards, _ = pt.PreferenceLoss(vocab, beta=1.0, inplace=False).loss_and_grad(x.view(rows, 1, vocab), (t.view(rows, 1), lp.float().view(rows, 1)))
+    off = rewards.double() - (lp - lp.float().double())
+    assert off.square().mean().sqrt().item() <= 2 ** -23
+    near(loss.reshape(1), torch.tensor([math.log(2)], dtype=torch.float64, device="cuda"), 1e-6, 0)
+
+
 # ----------------------------------------------------------------------------------- policy loss
 def ref_policy(lp, old, adv, ref, counted, spans, low, high, kl_coef, reduction):
     zero = torch.zeros((), dtype=torch.float64, device="cuda")
