@@ -13,12 +13,25 @@ namespace {
 // with eight and two thirds of the threads per SM (6.5 TB/s), 252 with two.
 constexpr int ROW_LOADS = 4, GRAD_LOADS = 8;
 constexpr int MAX_PARTS = 8;              // CTAs of a cluster that share a row
-// How many threads share a row.  A warp of its own where rows are short and there are enough of them for every warp of the machine to be
-// waiting for one (sum / gradient in us, a block of 256 | a warp: 11840 rows of 2.4 KB 25 / 40 | 14 / 13, 5515 of 7.6 KB 18 / 29 |
-// 13 / 18, 2876 of 14 KB 13 / 22 | 18 / 14, 1500 of 28 KB 12 / 20 | 26 / 20; few rows: 600 of 7.6 KB 4 / 4 | 5 / 5); from LONG_ROW on the
-// policy loss's ring (1500 rows of 28 KB 35 -> 26 us against 16 KB as the limit).
-constexpr size_t WARP_SUM = 8192, WARP_GRAD = 16384, TINY_ROW = 1024, LONG_ROW = 32768;
-constexpr int WARP_ROWS = 1024;
+// How many threads share a row: with its bytes a thread's loads, barriers and start are spread over more of them, and with few rows
+// more of them are needed to fill the machine (TEAM_THREADS; 148 SMs hold 303104).  us, bf16, per row a warp | 64 | 128 | 256 threads:
+//   sums      16384 rows of 8 KB 29 | 29 | 38 | 64, of 16 KB 52 | 49 | 50 | 73, of 49 KB 137 | 128 | 122 | 140;  1024 of 16 KB 17 | 9 | 7 | 9
+//   gradient  16384 rows of 4 KB 28 | 32 | 44 | 76, of 16 KB 91 | 88 | 92 | 111, of 32 KB 176 | 173 | 165 | 176;  1024 of 16 KB 11 | 8 | 7 | 8
+//   policy    16384 rows of 4 KB 41 | 44 | 61 | 86, of 12 KB 94 | 81 | 92 | 123, of 24 KB 187 | 178 | 145 | 172;  1024 of 16 KB 21 | 18 | 15 | 19
+// (fp32 within 10 % of the same ratios.)
+constexpr size_t TINY_ROW = 1024;
+constexpr long long TEAM_THREADS = 131072;
+struct Teams { size_t warp, two, four; };
+constexpr Teams SUM_TEAMS = {8192, 16384, 65536}, GRAD_TEAMS = {4096, 16384, 40960}, POLICY_TEAMS = {4096, 12288, 32768};
+// From here on the policy loss keeps a row in shared memory instead of reading it twice (16384 rows, us, twice | kept: bf16 of 38 KB 238 | 285, of
+// 49 KB 284 | 334, of 63 KB 373 | 383; fp32 of 32 KB 204 | 232, of 38 KB 253 | 248, of 49 KB 313 | 289).
+template <typename T> constexpr size_t LONG_ROW = sizeof(T) == 2 ? 65536 : 32768;
+int team_of(size_t bytes, long long rows, const Teams& by) {
+  if (bytes <= TINY_ROW) return 32;
+  int threads = bytes <= by.warp ? 32 : bytes <= by.two ? 64 : bytes <= by.four ? 128 : 256;
+  while (threads < 256 && threads * rows < TEAM_THREADS) threads *= 2;
+  return threads;
+}
 
 // dynamic shared memory next to a kernel's few static bytes: of one CTA per SM, and of each of two
 constexpr size_t MAX_RING = 226 * 1024, PAIR_RING = 112 * 1024;
@@ -240,8 +253,9 @@ __device__ __forceinline__ void grad_rest(const T* x, float xt, T* d, int lead, 
   for (int j = row_thread<THREADS>(); j < lead + cols - tail; j += THREADS) one(j < lead ? j : tail + j - lead);
 }
 
-// d[j] = g * ([j == t] - softmax_j) for j < V, 0 in [V, cols); zeros throughout when g == 0 (nothing is read then)
-template <typename T, int THREADS, int U>
+// d[j] = g * ([j == t] - softmax_j) for j < V, 0 in [V, cols); zeros throughout when g == 0 (nothing is read then).  FAR: the row comes
+// from memory, not from a cache that has just seen it
+template <typename T, int THREADS, int U, bool FAR = false>
 __device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int t, float g, K2 k, float r, float s) {
   constexpr int VEC = Elem<T>::VEC;
   const int tid = row_thread<THREADS>();
@@ -279,7 +293,15 @@ __device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int 
 #pragma unroll
     for (int u = 0; u < U; ++u) grad_chunk<T>(dv + c + u * THREADS, q[u], w);
   }
-  for (; c < whole; c += THREADS) grad_chunk<T>(dv + c, xv[c], w);
+  if constexpr (FAR) {        // up to U - 1 more, their loads together as well
+    uint4 q[U - 1];
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u) if (c + u * THREADS < whole) q[u] = xv[c + u * THREADS];
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u) if (c + u * THREADS < whole) grad_chunk<T>(dv + c + u * THREADS, q[u], w);
+  } else {
+    for (; c < whole; c += THREADS) grad_chunk<T>(dv + c, xv[c], w);
+  }
   grad_rest<T, THREADS>(x, xt, d, sp.lead, whole, V, cols, t, g, k, s, w);
 }
 
@@ -333,8 +355,11 @@ __device__ inline void put_logp(double lp, int row, float* logp, float* rest) {
   if (rest) rest[row] = isinf(lp) ? 0.f : (float)(lp - (double)(float)lp);
 }
 
+// Registers for a full SM (32 a thread): bf16 sums with 34 take 5 to 25 % longer (2048 rows of 32 KB 17.8 us, with 32 14.5).  fp32 rows of
+// a warp have 32 unasked, and lose 12 % when asked.
+template <typename T, int THREADS> constexpr int SUM_BLOCKS = THREADS == 32 && sizeof(T) == 4 ? 0 : 2048 / BLOCK<THREADS>;
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(BLOCK<THREADS>)
+__global__ void __launch_bounds__(BLOCK<THREADS>, SUM_BLOCKS<T, THREADS>)
 token_logprob_fwd_kernel(const T* logits, long long ld, const long long* targets, K2 k, float* logp, float* rest, float2* stats,
                          int rows, int V, long long ignore_index, int* status) {
   __shared__ float2 smem[BLOCK<THREADS> / 32];
@@ -408,8 +433,11 @@ token_logprob_fwd_cluster_kernel(const T* logits, long long ld, const long long*
   }
 }
 
+// Threads of an SM that the registers leave room for: short rows gain from more of them (16384 bf16 rows of 16 KB 92 us with 1024, 84 with
+// 1536), long ones from the loads that they would hold in registers instead.
+template <int THREADS> constexpr int GRAD_BLOCKS = (THREADS <= 64 ? 1536 : THREADS == 128 ? 1280 : 1024) / BLOCK<THREADS>;
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(BLOCK<THREADS>, 4)
+__global__ void __launch_bounds__(BLOCK<THREADS>, GRAD_BLOCKS<THREADS>)
 token_logprob_bwd_kernel(const T* logits, long long ld, const long long* targets, const float2* stats, const float* row_grad,
                          const float* gscale_dev, float gscale, K2 k, T* dlogits, long long ldd, int rows, int V, int cols,
                          long long ignore_index, const double* pair_loss, int pairs, float* loss) {
@@ -422,7 +450,7 @@ token_logprob_bwd_kernel(const T* logits, long long ld, const long long* targets
   const float2 st = stats[row];
   const bool counted = t != ignore_index && t >= 0 && t < V;
   const float g = counted ? row_grad[row] * (gscale_dev ? gscale_dev[0] : 1.f) * gscale : 0.f;
-  grad_row<T, THREADS, THREADS == 32 ? ROW_LOADS : GRAD_LOADS>(logits + (size_t)row * ld, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, st.x, st.y);
+  grad_row<T, THREADS, THREADS < 256 ? ROW_LOADS : GRAD_LOADS, true>(logits + (size_t)row * ld, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, st.x, st.y);
 }
 
 // Tokens [a, b) of sequence q: rows of `seq_len` tokens, or between two offsets.  Offsets that do not ascend within [0, tokens]
@@ -1155,7 +1183,6 @@ bool bad_list(const bb_grad_tensor* list, int count) {
 template <typename T> struct FwdCall { const T* logits; long long ld; const long long* targets; K2 k; float *logp, *rest; float2* stats; int rows, V; long long ignore; int* status; cudaStream_t s; };
 // Blocks of a launch whose rows are worked on by THREADS threads each
 template <int THREADS> int row_blocks(int rows) { return (rows + ROWS_OF_BLOCK<THREADS> - 1) / ROWS_OF_BLOCK<THREADS>; }
-bool by_warps(size_t bytes, int rows, size_t limit) { return bytes <= TINY_ROW || (bytes <= limit && rows >= WARP_ROWS); }
 template <typename T, int THREADS> int fwd_rows(const FwdCall<T>& c) {
   BB_CUDA_CHECK(bb_launch(token_logprob_fwd_kernel<T, THREADS>, row_blocks<THREADS>(c.rows), BLOCK<THREADS>, 0, c.s, c.logits, c.ld, c.targets, c.k, c.logp,
                           c.rest, c.stats, c.rows, c.V, c.ignore, c.status));
@@ -1170,7 +1197,10 @@ template <typename T> int fwd_parts(int rows, int V) {
 }
 template <typename T> int fwd_call(const FwdCall<T>& c) {
   const int parts = fwd_parts<T>(c.rows, c.V);
-  if (parts == 1) return by_warps(c.V * sizeof(T), c.rows, WARP_SUM) ? fwd_rows<T, 32>(c) : fwd_rows<T, 256>(c);
+  if (parts == 1) {
+    const int threads = team_of(c.V * sizeof(T), c.rows, SUM_TEAMS);
+    return threads == 32 ? fwd_rows<T, 32>(c) : threads == 64 ? fwd_rows<T, 64>(c) : threads == 128 ? fwd_rows<T, 128>(c) : fwd_rows<T, 256>(c);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(c.rows * parts); cfg.blockDim = dim3(256); cfg.stream = c.s;
   cudaLaunchAttribute attr[2];
@@ -1198,7 +1228,10 @@ template <typename T, int THREADS> int bwd_rows(const BwdCall<T>& c) {
                           c.gscale_dev, c.gscale, c.k, c.dlogits, c.ldd, c.rows, c.V, c.cols, c.ignore, c.pair_loss, c.pairs, c.loss));
   return BB_OK;
 }
-template <typename T> int bwd_call(const BwdCall<T>& c) { return by_warps(c.V * sizeof(T), c.rows, WARP_GRAD) ? bwd_rows<T, 32>(c) : bwd_rows<T, 256>(c); }
+template <typename T> int bwd_call(const BwdCall<T>& c) {
+  const int threads = team_of(c.V * sizeof(T), c.rows, GRAD_TEAMS);
+  return threads == 32 ? bwd_rows<T, 32>(c) : threads == 64 ? bwd_rows<T, 64>(c) : threads == 128 ? bwd_rows<T, 128>(c) : bwd_rows<T, 256>(c);
+}
 int logprob_bwd(const void* logits, int dtype, long long ld, const long long* targets, double scale, const float* stats, const float* row_grad,
                 const float* grad_scale_dev, float grad_scale, void* dlogits, long long ldd, long long rows, int vocab, int cols, long long ignore_index,
                 const double* pair_loss, int pairs, float* loss, cudaStream_t s) {
@@ -1335,8 +1368,11 @@ template <typename T, int THREADS> int policy_rows_as(const T* logits, T* dlogit
 }
 template <typename T> int policy_rows(const T* logits, T* dlogits, const PolicyRowCall& c) {
   const size_t bytes = (size_t)c.V * sizeof(T);
-  if (by_warps(bytes, c.rows, WARP_SUM)) return policy_rows_as<T, 32>(logits, dlogits, c);
-  if (bytes <= LONG_ROW) return policy_rows_as<T, 256>(logits, dlogits, c);
+  if (bytes <= LONG_ROW<T>) {
+    const int threads = team_of(bytes, c.rows, POLICY_TEAMS);
+    return threads == 32 ? policy_rows_as<T, 32>(logits, dlogits, c) : threads == 64 ? policy_rows_as<T, 64>(logits, dlogits, c)
+         : threads == 128 ? policy_rows_as<T, 128>(logits, dlogits, c) : policy_rows_as<T, 256>(logits, dlogits, c);
+  }
   const size_t smem = bytes / 16 * 16;
   const int stages = (int)((smem + RING_STAGE - 1) / RING_STAGE);
   if (smem > MAX_RING) return policy_rows_as<T, 512>(logits, dlogits, c);
