@@ -23,6 +23,10 @@ constexpr size_t TINY_ROW = 1024;
 constexpr long long TEAM_THREADS = 131072;
 struct Teams { size_t warp, two, four; };
 constexpr Teams SUM_TEAMS = {8192, 16384, 65536}, GRAD_TEAMS = {4096, 16384, 40960}, POLICY_TEAMS = {4096, 12288, 32768};
+// Gradients of many long rows: 512 threads with four loads instead of 256 with eight (bf16, us: 16384 rows of 65 KB 330 | 328, of 98 KB 490 | 499, of 196 KB
+// 1009 | 1026; 2048 of 98 KB 67 | 70; 512 of 98 KB 23.5 | 21.7).
+constexpr size_t GRAD_EIGHT = 81920;
+constexpr int GRAD_EIGHT_ROWS = 2048;
 // From here on the policy loss keeps a row in shared memory instead of reading it twice (16384 rows, us, twice | kept: bf16 of 38 KB 238 | 285, of
 // 49 KB 284 | 334, of 63 KB 373 | 383; fp32 of 32 KB 204 | 232, of 38 KB 253 | 248, of 49 KB 313 | 289).
 template <typename T> constexpr size_t LONG_ROW = sizeof(T) == 2 ? 65536 : 32768;
@@ -435,7 +439,7 @@ token_logprob_fwd_cluster_kernel(const T* logits, long long ld, const long long*
 
 // Threads of an SM that the registers leave room for: short rows gain from more of them (16384 bf16 rows of 16 KB 92 us with 1024, 84 with
 // 1536), long ones from the loads that they would hold in registers instead.
-template <int THREADS> constexpr int GRAD_BLOCKS = (THREADS <= 64 ? 1536 : THREADS == 128 ? 1280 : 1024) / BLOCK<THREADS>;
+template <int THREADS> constexpr int GRAD_BLOCKS = (THREADS == 256 ? 1024 : THREADS == 128 ? 1280 : 1536) / BLOCK<THREADS>;
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(BLOCK<THREADS>, GRAD_BLOCKS<THREADS>)
 token_logprob_bwd_kernel(const T* logits, long long ld, const long long* targets, const float2* stats, const float* row_grad,
@@ -450,7 +454,7 @@ token_logprob_bwd_kernel(const T* logits, long long ld, const long long* targets
   const float2 st = stats[row];
   const bool counted = t != ignore_index && t >= 0 && t < V;
   const float g = counted ? row_grad[row] * (gscale_dev ? gscale_dev[0] : 1.f) * gscale : 0.f;
-  grad_row<T, THREADS, THREADS < 256 ? ROW_LOADS : GRAD_LOADS, true>(logits + (size_t)row * ld, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, st.x, st.y);
+  grad_row<T, THREADS, THREADS == 256 ? GRAD_LOADS : ROW_LOADS, true>(logits + (size_t)row * ld, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, st.x, st.y);
 }
 
 // Tokens [a, b) of sequence q: rows of `seq_len` tokens, or between two offsets.  Offsets that do not ascend within [0, tokens]
@@ -1229,7 +1233,9 @@ template <typename T, int THREADS> int bwd_rows(const BwdCall<T>& c) {
   return BB_OK;
 }
 template <typename T> int bwd_call(const BwdCall<T>& c) {
-  const int threads = team_of(c.V * sizeof(T), c.rows, GRAD_TEAMS);
+  const size_t bytes = c.V * sizeof(T);
+  if (bytes > GRAD_EIGHT && c.rows >= GRAD_EIGHT_ROWS) return bwd_rows<T, 512>(c);
+  const int threads = team_of(bytes, c.rows, GRAD_TEAMS);
   return threads == 32 ? bwd_rows<T, 32>(c) : threads == 64 ? bwd_rows<T, 64>(c) : threads == 128 ? bwd_rows<T, 128>(c) : bwd_rows<T, 256>(c);
 }
 int logprob_bwd(const void* logits, int dtype, long long ld, const long long* targets, double scale, const float* stats, const float* row_grad,
