@@ -551,6 +551,40 @@ def test_policy_loss_from_logits(pt, dtype, reduction, vocab, cols, lengths):
     assert torch.equal(loss_fn.loss_and_grad(over, (t, old, adv, ref), offsets=offsets, out=over, grad_scale=0.5)[2], grad)
 
 
+# Rows that 32, 64, 128, 256 and 512 threads work on (the last for gradients)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab,cols", [(4100, 1000, 1003), (2100, 5001, 5001), (1100, 12001, 12008), (700, 12001, 12001), (2050, 41003, 41003)])
+def test_many_rows_of_every_size(pt, rows, vocab, cols, dtype):
+    x, t = logits_of(rows, vocab, cols, dtype, 61), targets_of(rows, vocab, 62)
+    t[:2] = 7
+    x[0, :vocab] = torch.finfo(dtype).min
+    x[1, :vocab] = -math.inf
+    g = torch.randn(rows, device="cuda", generator=gen(63))
+    lp, probs, counted = ref_logps(x, t, vocab, 0.9)
+    want = ref_dlogits(probs, counted, t, g, cols, 0.9)
+    lp[1], want[1] = -math.inf, 0.0
+    leaf = x.clone().requires_grad_(True)
+    out = pt.token_logprobs(leaf, t, vocab, temperature=0.9)
+    near(out.detach(), lp, 1e-6, 1e-6)
+    near(pt.token_logprobs(x, t, vocab, temperature=0.9), lp, 1e-6, 1e-6)
+    out.backward(g)
+    near(leaf.grad, want, 4e-6 if dtype == torch.float32 else 2 ** -8, 1e-7 * g.abs().max().item() / 0.9)
+    del leaf, want
+    # the policy loss on all but the first two
+    t[:2] = IGNORE
+    counted[:2] = False
+    lp[:2] = 0.0
+    old, adv, ref = policy_inputs(lp, 64)
+    exact = lp.clone().requires_grad_(True)
+    loss, _ = ref_policy(exact, old.double(), adv.double(), ref.double(), t != IGNORE, spans_of([rows]), 0.2, 0.3, 0.05, "token")
+    (row_grad,) = torch.autograd.grad(loss, exact)
+    err, size = 1e-6 * (1 + lp.abs().max().item()), row_grad.abs().max().item()
+    loss_fn = pt.PolicyLoss(vocab, clip_low=0.2, clip_high=0.3, kl_coef=0.05, temperature=0.9, inplace=False)
+    got, _, grad = loss_fn.loss_and_grad(x, (t, old, adv, ref), offsets=torch.tensor([0, rows], device="cuda"))
+    near(got.reshape(1), loss.detach().reshape(1), 2e-6, 2 * err)
+    near(grad, ref_dlogits(probs, counted, t, row_grad, cols, 0.9), (4e-6 if dtype == torch.float32 else 2 ** -8) + 4 * err, 4 * err * size)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("offset", [0, 1, 3])
 @pytest.mark.parametrize("vocab", [1003, 30011])
