@@ -89,7 +89,10 @@ template <bool CONV> struct ConvArg { typedef NoConv type; };
 template <> struct ConvArg<true> { typedef ConvParams type; };
 
 // A vocabulary projection whose logits are not stored (template parameter HEAD): the epilogue turns them into partial softmax sums
-// (HEAD_SUMS), or into the gradient of the targets' log-probabilities (HEAD_GRAD, the bf16 output).
+// (HEAD_SUMS), or into the gradient of the targets' log-probabilities (HEAD_GRAD, the bf16 output).  The tensor core bounds both: 4096 rows of
+// 1024 against 50257 entries 257 us with sums (1.64 PFLOP/s), 185 us for the gradient of 32768 of them (1.49: it writes 268 MB).  That gradient
+// is rounded to bf16 because the two products that follow take bf16 operands; an entry is off by 2^-9 of itself, which a row's input
+// gradient feels most where one entry outweighs the others (0.25 % of its norm in place of the 0.17 % of its own rounding; 0.35 % with two rows in all).
 constexpr int HEAD_NONE = 0, HEAD_SUMS = 1, HEAD_GRAD = 2;
 struct HeadParams {
   const long long* targets;   // per row

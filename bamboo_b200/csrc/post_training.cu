@@ -9,8 +9,9 @@
 
 namespace {
 
-// 16-byte loads that a thread has in flight.  8192 rows of 50257 bf16 logits: sums 116 us with four (6.7 TB/s), gradient 249 us with four, 245
-// with eight and two thirds of the threads per SM (6.5 TB/s), 252 with two.
+// 16-byte loads that a thread has in flight (GRAD_LOADS: in a gradient by 256 threads).  8192 rows of 50257 bf16 logits, a sixteenth of them
+// ignored: sums 120 us with four (6.4 TB/s), gradient by 256 threads 249 us with four, 246 with eight and two thirds of the threads per SM, 252
+// with two; by 512 with four 242 (6.6 TB/s).
 constexpr int ROW_LOADS = 4, GRAD_LOADS = 8;
 constexpr int MAX_PARTS = 8;              // CTAs of a cluster that share a row
 // How many threads share a row: with its bytes a thread's loads, barriers and start are spread over more of them, and with few rows
@@ -390,7 +391,7 @@ token_logprob_fwd_kernel(const T* logits, long long ld, const long long* targets
 }
 
 // Few rows: a cluster per row, the chunks dealt out in equal parts; the parts' sums meet in the first CTA.  Three rows of 50257 fp32
-// logits 6.6 -> 3.9 us in a graph.
+// logits 6.6 -> 4.2 us in a graph.
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS)
 token_logprob_fwd_cluster_kernel(const T* logits, long long ld, const long long* targets, K2 k, float* logp, float* rest, float2* stats, int V, long long ignore_index,
