@@ -93,7 +93,11 @@ template <> struct ConvArg<true> { typedef ConvParams type; };
 // 1024 against 50257 entries 257 us with sums (1.64 PFLOP/s), 185 us for the gradient of 32768 of them (1.49: it writes 268 MB).  That gradient
 // is rounded to bf16 because the two products that follow take bf16 operands; an entry is off by 2^-9 of itself, which a row's input
 // gradient feels most where one entry outweighs the others (0.25 % of its norm in place of the 0.17 % of its own rounding; 0.35 % with two rows in all).
-constexpr int HEAD_NONE = 0, HEAD_SUMS = 1, HEAD_GRAD = 2;
+// HEAD_PARTS: the input gradient's product, whose reduction is the vocabulary: fp32 outputs, part s of a split reduction into a buffer of
+// its own (`stride` values after part s - 1), so that they are added up in one order.
+constexpr int HEAD_NONE = 0, HEAD_SUMS = 1, HEAD_GRAD = 2, HEAD_PARTS = 3;
+template <int HEAD> constexpr bool HEAD_LOGITS = HEAD == HEAD_SUMS || HEAD == HEAD_GRAD;
+struct PartsParams { long long stride; };
 struct HeadParams {
   const long long* targets;   // per row
   long long ignore_index;
@@ -108,9 +112,11 @@ struct HeadParams {
 // 4.6e-5 off, of 1024 products 2.4e-6).  Projections from more than 2048 columns sum the halves of the reduction into the two
 // accumulators and add those in the epilogue; the main loop of the next tile then covers less of the epilogue.
 constexpr int HEAD_WHOLE_KB = 2048 / BK;
+constexpr long long PARTS_VALUES = 1LL << 26;   // in all parts of an input gradient (256 MiB)
 struct NoHead {};
 template <int HEAD> struct HeadArg { typedef HeadParams type; };
 template <> struct HeadArg<HEAD_NONE> { typedef NoHead type; };
+template <> struct HeadArg<HEAD_PARTS> { typedef PartsParams type; };
 
 __device__ __forceinline__ void unpack8(const uint4& q, float* f) {
   f[0] = bb::bf16_lo(q.x); f[1] = bb::bf16_hi(q.x); f[2] = bb::bf16_lo(q.y); f[3] = bb::bf16_hi(q.y);
@@ -611,6 +617,7 @@ template <int HEAD> struct HeadRow {
   }
 };
 template <> struct HeadRow<HEAD_NONE> {};
+template <> struct HeadRow<HEAD_PARTS> {};
 
 template <int BN, bool PAIR, int EW, bool CONV, int HEAD>
 __global__ void __launch_bounds__(num_threads(EW), 1)
@@ -778,7 +785,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
       int mi, ni, ks;
       unit_coords(p, tile, mi, ni, ks);
       int num_kb = min(total_kb, (ks + 1) * p.kb_per_split) - ks * p.kb_per_split;
-      if constexpr (HEAD != HEAD_NONE) {
+      if constexpr (HEAD_LOGITS<HEAD>) {
         if (total_kb > HEAD_WHOLE_KB) {         // first half here (accumulator 0), the second below
           const int first = num_kb >> 1;
           if (!issue_mmas<BN, PAIR>(p, sA, sB, full_bar, empty_bar, &tmem_full[0], abort_flag, 3, tmem_base, first, s, phase)) { alive = false; break; }
@@ -801,8 +808,8 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
     // another warp or on the TMA queue, which the producer keeps full of operand loads.
     const int eg = (warp - EPI_WARP) >> 2;         // which of the quarter's EW warps
     const int quarter = warp & 3;
-    const int epi = HEAD == HEAD_NONE ? p.epi : (int)BB_EPI_STORE;
-    const bool f32 = (epi == BB_EPI_ACCUM_F32 || epi == BB_EPI_STORE_F32);
+    const int epi = HEAD_LOGITS<HEAD> ? (int)BB_EPI_STORE : p.epi;
+    const bool f32 = HEAD == HEAD_PARTS || (epi == BB_EPI_ACCUM_F32 || epi == BB_EPI_STORE_F32);
     const bool dual = (epi == BB_EPI_BIAS_GELU);
     const bool has_aux = (epi == BB_EPI_MUL_DGELU || epi == BB_EPI_BIAS_RESIDUAL);
     int acc = 0; uint32_t acc_phase = 0;
@@ -860,12 +867,12 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
       const int m0 = mi * C::TILE_M + (int)rank * BM, n0 = ni * BN;
       const int r0 = m0 + quarter * 32;            // first output row of this warp
       HeadRow<HEAD> head;
-      if constexpr (HEAD != HEAD_NONE) head.load(hd, r0 + lane, p.M);      // in flight while the accumulator is waited for
+      if constexpr (HEAD_LOGITS<HEAD>) head.load(hd, r0 + lane, p.M);      // in flight while the accumulator is waited for
       const bool got = bb::mbar_wait(&tmem_full[acc], acc_phase, abort_flag, p.status);
       if (!__all_sync(0xffffffffu, got)) { alive = false; break; }
       bb::tc_fence_after_sync();
       bool halves = false;                         // the reduction's second half is in accumulator 1
-      if constexpr (HEAD != HEAD_NONE) {
+      if constexpr (HEAD_LOGITS<HEAD>) {
         halves = total_kb > HEAD_WHOLE_KB;
         if (halves) {
           const bool both = bb::mbar_wait(&tmem_full[1], acc_phase, abort_flag, p.status);
@@ -900,7 +907,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[32 + i] = __uint_as_float(r[i]);
           }
-          if constexpr (HEAD != HEAD_NONE) {
+          if constexpr (HEAD_LOGITS<HEAD>) {
             if (halves) {
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
@@ -931,8 +938,10 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
         if (f32) {
           panel_store_row_f32(slab, lane, v);
           __syncwarp();
-          if (epi == BB_EPI_ACCUM_F32) slab_flush_f32<true>(slab, reinterpret_cast<float*>(p.D), p.ldd, r0, nb, p.M, p.N, lane);
-          else slab_flush_f32<false>(slab, reinterpret_cast<float*>(p.D), p.ldd, r0, nb, p.M, p.N, lane);
+          float* out = reinterpret_cast<float*>(p.D);
+          if constexpr (HEAD == HEAD_PARTS) out += ks * hd.stride;
+          if (epi == BB_EPI_ACCUM_F32) slab_flush_f32<true>(slab, out, p.ldd, r0, nb, p.M, p.N, lane);
+          else slab_flush_f32<false>(slab, out, p.ldd, r0, nb, p.M, p.N, lane);
           __syncwarp();
           continue;
         }
@@ -962,7 +971,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
       if constexpr (HEAD == HEAD_SUMS) {
         if (r0 + lane < p.M) hd.partial[(long long)(2 * ni + eg) * p.M + r0 + lane] = make_float2(head.r, head.s);
       }
-      if constexpr (HEAD != HEAD_NONE) {
+      if constexpr (HEAD_LOGITS<HEAD>) {
         if (halves) { acc_phase ^= 1; continue; }
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
@@ -1261,7 +1270,7 @@ int launch(const bb_gemm_desc* g, cudaStream_t stream, const bb_conv_gemm_args* 
   const int mn_tiles = ((g->M + C::TILE_M - 1) / C::TILE_M) * ((g->N + BN - 1) / BN);
   const int workers_max = PAIR ? bb_num_sms() / 2 : bb_num_sms();
   int ksplit = 1;
-  if (g->epilogue == BB_EPI_ACCUM_F32) {
+  if (g->epilogue == BB_EPI_ACCUM_F32 || HEAD == HEAD_PARTS) {
     if (g->split_k > 0) {
       ksplit = g->split_k;
     } else {
@@ -1669,6 +1678,54 @@ template <int HEAD> int head_launch(const bb_gemm_desc& g, const HeadParams& hd,
   return pl.bn == 256 ? launch<256, false, 2, false, HEAD>(&g, s, nullptr, hd) : launch<128, false, 2, false, HEAD>(&g, s, nullptr, hd);
 }
 
+// The input gradient [M, N] sums over the vocabulary entries of a piece [K], many more than the machine has use for in one unit: tile,
+// pairing and the number of parts by the expected time (the constants of the add-reductions, and the parts' way through memory).  us, one
+// product stored | in parts with their sum: 64 x 768 from 50257 entries 34 | 23, 411 x 792 from 36348 55 | 36, 1999 x 768 from 32000 86 | 76, 1500 x 1024 from
+// 50257 136 | 115; 106 x 1536 from 47650 32 | 32, 770 x 1264 from 15415 38 | 40 and 2502 x 1752 from 4407 38 | 45 (stored).
+struct PartsPlan { int bn; bool pair; int parts; double us; };
+PartsPlan plan_parts(int M, int N, int K) {
+  static const struct { int bn; bool pair; double kblock, tile, once; } kinds[3] = {
+      {256, true, 0.316, 4.6, 3.2}, {256, false, 0.365, 4.6, 1.9}, {128, false, 0.282, 1.75, 3.1}};
+  const long long kb = (K + BK - 1) / BK;
+  const double part_us = (double)M * N * 4 / 4.5e6;
+  PartsPlan best = {0, false, 0, 0};
+  for (const auto& k : kinds) {
+    if ((k.bn == 256 && N <= 128) || (k.pair && M <= BM)) continue;
+    const long long tm = k.pair ? 2 * BM : BM, tiles = ((M + tm - 1) / tm) * ((N + k.bn - 1) / k.bn);
+    const long long workers = k.pair ? bb_num_sms() / 2 : bb_num_sms();
+    const long long widest = workers / tiles > 8 ? workers / tiles : 8;
+    for (long long s = 1; s <= widest; ++s) {
+      const long long kbs = (kb + s - 1) / s, parts = (kb + kbs - 1) / kbs;
+      if (s > 1 && (kbs < 8 || parts * M * N > PARTS_VALUES)) break;
+      if (parts != s) continue;
+      const double us = (double)((tiles * s + workers - 1) / workers) * ((double)kbs * k.kblock + k.tile) + k.once + 2.5 + part_us * (double)s;
+      if (best.parts == 0 || us < best.us) best = {k.bn, k.pair, (int)s, us};
+    }
+  }
+  return best;
+}
+// ... for a backward pass: no parts where the whole vocabulary is one piece and its product stored directly is expected to be no slower (the
+// estimate of the parts is up to a tenth low)
+PartsPlan head_parts(const bb_head_desc* d, int piece) {
+  PartsPlan pl = plan_parts(d->rows, d->hidden, piece < d->vocab ? piece : d->vocab);
+  if (piece >= d->vocab && bb_gemm_store_us(d->rows, d->hidden, d->vocab, 0) <= 1.03 * pl.us + 3.0) pl.parts = 0;
+  return pl;
+}
+// out = sum of the parts, one after the other
+__global__ void __launch_bounds__(256)
+head_sum_parts_kernel(const float4* parts, int num, long long n4, uint2* out) {
+  bb::pdl_sync();
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n4) return;
+  float4 sum = __ldcg(parts + i);
+#pragma unroll 8
+  for (int s = 1; s < num; ++s) {
+    const float4 q = __ldcg(parts + s * n4 + i);
+    sum.x += q.x; sum.y += q.y; sum.z += q.z; sum.w += q.w;
+  }
+  out[i] = make_uint2(bb::pack_bf16x2(sum.x, sum.y), bb::pack_bf16x2(sum.z, sum.w));
+}
+
 int head_check(const char* who, const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets) {
   const bool ok = d && hidden_states && weight && targets && d->rows > 0 && d->vocab > 0 && d->hidden > 0 && d->ld_hidden % 8 == 0 && d->ld_weight % 8 == 0 &&
                   d->ld_hidden >= d->hidden && d->ld_weight >= d->hidden && !((uintptr_t)hidden_states & 15) && !((uintptr_t)weight & 15) &&
@@ -1730,19 +1787,25 @@ int head_logits_grad(const bb_head_desc* d, const void* hidden_states, const voi
 }
 }  // namespace
 
+// fp32 buffers of [rows, hidden] that the backward pass with pieces of `piece` entries needs for the input gradient
+extern "C" int bb_head_logprob_bwd_parts(const bb_head_desc* d, int piece) {
+  if (!d || d->rows <= 0 || d->vocab <= 0 || d->hidden <= 0 || piece <= 0) return -1;
+  return head_parts(d, piece).parts;
+}
+
 extern "C" int bb_head_logprob_bwd(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets, const float* stats,
-                                   const float* row_grad, void* d_hidden, float* d_hidden_f32, void* d_weight, float* d_weight_accum, void* counted_hidden,
+                                   const float* row_grad, void* d_hidden, float* d_hidden_parts, void* d_weight, float* d_weight_accum, void* counted_hidden,
                                    int piece, void* dlogits, long long ldd, void* stream) {
   if (int rc = head_check("bb_head_logprob_bwd", d, hidden_states, weight, targets)) return rc;
   const bool whole = piece >= d->vocab;
-  if (!stats || ((uintptr_t)stats & 7) || !row_grad || !dlogits || (((uintptr_t)dlogits | (uintptr_t)d_hidden | (uintptr_t)d_hidden_f32 | (uintptr_t)d_weight | (uintptr_t)d_weight_accum | (uintptr_t)counted_hidden) & 15) ||
-      piece <= 0 || piece % 8 || ldd % 8 || ldd < (whole ? d->vocab : piece) || (d_weight && d_weight_accum) || ((d_weight || d_weight_accum) && !counted_hidden) || (d_hidden && !whole && !d_hidden_f32)) {
-    bb_set_last_error_msg("bb_head_logprob_bwd: null or unaligned pointer, pieces that are no multiple of 8 or do not fit the buffer, no fp32 buffer for d_hidden over several pieces, two weight gradients, or no counted_hidden for one");
+  const PartsPlan parts = d_hidden && piece > 0 ? head_parts(d, piece) : PartsPlan{};
+  if (!stats || ((uintptr_t)stats & 7) || !row_grad || !dlogits || (((uintptr_t)dlogits | (uintptr_t)d_hidden | (uintptr_t)d_hidden_parts | (uintptr_t)d_weight | (uintptr_t)d_weight_accum | (uintptr_t)counted_hidden) & 15) ||
+      piece <= 0 || piece % 8 || ldd % 8 || ldd < (whole ? d->vocab : piece) || (d_weight && d_weight_accum) || ((d_weight || d_weight_accum) && !counted_hidden) || (parts.parts > 0 && !d_hidden_parts)) {
+    bb_set_last_error_msg("bb_head_logprob_bwd: null or unaligned pointer, pieces that are no multiple of 8 or do not fit the buffer, no fp32 buffer for the parts of d_hidden, two weight gradients, or no counted_hidden for one");
     return BB_ERR_INVALID_ARG;
   }
   if (int rc = bbhost::bind_context()) return rc;
   cudaStream_t s = (cudaStream_t)stream;
-  if (d_hidden && !whole) BB_CUDA_CHECK(cudaMemsetAsync(d_hidden_f32, 0, (size_t)d->rows * d->hidden * 4, s));
   BackToBack overlap;
   if (d_weight || d_weight_accum)
     BB_CUDA_CHECK(bb_launch(head_counted_rows_kernel, d->rows, 128, 0, s, (const __nv_bfloat16*)hidden_states, d->ld_hidden, targets, d->ignore_index, d->vocab, d->hidden,
@@ -1754,8 +1817,17 @@ extern "C" int bb_head_logprob_bwd(const bb_head_desc* d, const void* hidden_sta
     g.A = dlogits; g.lda = ldd;
     if (d_hidden) {
       g.M = d->rows; g.N = d->hidden; g.K = cols; g.B = (const __nv_bfloat16*)weight + (long long)col0 * d->ld_weight; g.ldb = d->ld_weight; g.b_mn_major = 1;
-      g.D = whole ? d_hidden : (void*)d_hidden_f32; g.ldd = d->hidden; g.epilogue = whole ? BB_EPI_STORE : BB_EPI_ACCUM_F32;
-      if (int rc = bb_gemm_bf16(&g, stream)) return rc;
+      g.ldd = d->hidden;
+      if (parts.parts == 0) {
+        g.D = d_hidden; g.epilogue = BB_EPI_STORE;
+        if (int rc = bb_gemm_bf16(&g, stream)) return rc;
+      } else {
+        g.D = d_hidden_parts; g.epilogue = col0 == 0 ? BB_EPI_STORE_F32 : BB_EPI_ACCUM_F32; g.split_k = parts.parts;
+        const PartsParams pp = {(long long)d->rows * d->hidden};
+        if (int rc = parts.pair ? launch<256, true, 2, false, HEAD_PARTS>(&g, s, nullptr, pp)
+                   : parts.bn == 256 ? launch<256, false, 2, false, HEAD_PARTS>(&g, s, nullptr, pp) : launch<128, false, 2, false, HEAD_PARTS>(&g, s, nullptr, pp)) return rc;
+        g.split_k = 0;
+      }
     }
     if (d_weight || d_weight_accum) {
       g.M = cols; g.N = d->hidden; g.K = d->rows; g.a_mn_major = 1; g.B = counted_hidden; g.ldb = d->hidden; g.b_mn_major = 1; g.ldd = d->hidden;
@@ -1764,7 +1836,10 @@ extern "C" int bb_head_logprob_bwd(const bb_head_desc* d, const void* hidden_sta
       if (int rc = bb_gemm_bf16(&g, stream)) return rc;
     }
   }
-  if (d_hidden && !whole) return bb_cast_f32_to_bf16(d_hidden_f32, d_hidden, (long long)d->rows * d->hidden, stream);
+  if (parts.parts > 0) {
+    const long long n4 = (long long)d->rows * d->hidden / 4;
+    BB_CUDA_CHECK(bb_launch(head_sum_parts_kernel, (int)((n4 + 255) / 256), 256, 0, s, (const float4*)d_hidden_parts, parts.parts, n4, (uint2*)d_hidden));
+  }
   return BB_OK;
 }
 

@@ -143,6 +143,7 @@ def load():
         lib.bb_policy_loss_logits.argtypes = [vp, vp, i, ll, d, i, i] + [vp] * 9 + [ll, f, vp, ll, vp]
         lib.bb_head_logprob_workspace_bytes.restype = ll
         lib.bb_head_logprob_fwd.argtypes = [vp] * 7 + [ll, vp]
+        lib.bb_head_logprob_bwd_parts.argtypes = [vp, i]
         lib.bb_head_logprob_bwd.argtypes = [vp] * 11 + [i, vp, ll, vp]
         lib.bb_rescale_grad.argtypes = [vp, i, ll, ll, i, vp, f, vp]
         lib.bb_grad_norm_workspace_bytes.restype = ll
@@ -648,14 +649,19 @@ def head_logprob_fwd(desc, hidden, weight, targets, logp, stats):
     return logp
 
 
-def head_logprob_bwd(desc, hidden, weight, targets, stats, row_grad, d_hidden, d_hidden_f32, d_weight, d_weight_accum, counted, piece, dlogits):
+def head_bwd_parts(desc, piece):
+    """fp32 buffers [rows, hidden] that head_logprob_bwd needs for the input gradient (0: none)"""
+    return (_lib or load()).bb_head_logprob_bwd_parts(ctypes.byref(desc), piece)
+
+
+def head_logprob_bwd(desc, hidden, weight, targets, stats, row_grad, d_hidden, d_hidden_parts, d_weight, d_weight_accum, counted, piece, dlogits):
     """Gradients of hidden states (bf16) and weight (bf16, or added to fp32), each None where it is not wanted; ``dlogits``: room for a piece;
     ``counted``: room for a copy of the hidden states, where there is a weight gradient."""
     global LAUNCHES
     pieces, wgrad = -(-desc.vocab // piece), d_weight is not None or d_weight_accum is not None
-    LAUNCHES += pieces * (1 + (d_hidden is not None) + wgrad) + (d_hidden is not None and pieces > 1) + wgrad
+    LAUNCHES += pieces * (1 + (d_hidden is not None) + wgrad) + (d_hidden_parts is not None) + wgrad
     check((_lib or load()).bb_head_logprob_bwd(ctypes.byref(desc), hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), stats.data_ptr(),
-                                               row_grad.data_ptr(), _addr(d_hidden), _addr(d_hidden_f32), _addr(d_weight), _addr(d_weight_accum),
+                                               row_grad.data_ptr(), _addr(d_hidden), _addr(d_hidden_parts), _addr(d_weight), _addr(d_weight_accum),
                                                _addr(counted), piece,
                                                dlogits.data_ptr(), dlogits.stride(0), _raw_stream()), "bb_head_logprob_bwd")
 

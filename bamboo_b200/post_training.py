@@ -201,7 +201,8 @@ class _HeadLogprobsFn(torch.autograd.Function):
             # vocabulary entries in pieces, so that the gradient of the logits never exists whole; a multiple of 256, the widest tile
             piece = max(2048, HEAD_GRAD_BYTES // (2 * rows) // 256 * 256)
             width = (min(piece, vocab) + 7) // 8 * 8
-            acc = torch.empty(rows, n, dtype=torch.float32, device=dev) if need_h and piece < vocab else None
+            parts = L.head_bwd_parts(desc, piece) if need_h else 0
+            acc = torch.empty(parts, rows, n, dtype=torch.float32, device=dev) if parts else None
             counted = torch.empty(rows, n, dtype=torch.bfloat16, device=dev) if need_w else None
             L.head_logprob_bwd(desc, h, w, tg, stats, _flat(grad, "gradient", rows, torch.float32, dev), dh, acc, dw, main, counted, piece,
                                torch.empty(rows, width, dtype=torch.bfloat16, device=dev))

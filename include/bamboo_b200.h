@@ -332,12 +332,13 @@ long long bb_head_logprob_workspace_bytes(const bb_head_desc* d);
 int bb_head_logprob_fwd(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets, float* logp,
                         float* stats, void* workspace, long long workspace_bytes, void* stream);
 /* The backward pass computes the logits again, in pieces of `piece` vocabulary entries (a multiple of 8): of each the gradient
- * of the logits into `dlogits` (bf16 [rows, ldd]) and its products into the input gradient d_hidden (bf16 [rows, hidden]; over several pieces
- * through the fp32 buffer d_hidden_f32 of the same shape) and the weight gradient: d_weight (bf16 [vocab, hidden]), or
+ * of the logits into `dlogits` (bf16 [rows, ldd]) and its products into the input gradient d_hidden (bf16 [rows, hidden]; where
+ * bb_head_logprob_bwd_parts says so, through that many fp32 buffers of its shape at d_hidden_parts, which are added up in one order) and the weight gradient: d_weight (bf16 [vocab, hidden]), or
  * d_weight_accum (fp32, +=), through a copy of the rows that count (counted_hidden, bf16 [rows, hidden]).  A gradient that is
  * not wanted is NULL. */
+int bb_head_logprob_bwd_parts(const bb_head_desc* d, int piece);
 int bb_head_logprob_bwd(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets,
-                        const float* stats, const float* row_grad, void* d_hidden, float* d_hidden_f32, void* d_weight,
+                        const float* stats, const float* row_grad, void* d_hidden, float* d_hidden_parts, void* d_weight,
                         float* d_weight_accum, void* counted_hidden, int piece, void* dlogits, long long ldd, void* stream);
 
 /* Paired preference loss over token log-probabilities.  Sequences 2i (preferred) and 2i + 1 (rejected) form pair i; sequence q is

@@ -241,6 +241,28 @@ def test_head_backward_in_pieces_and_into_an_arena(pt, monkeypatch):
     near((p.main_grad - 1).bfloat16(), whole[1].double(), 2 ** -7, 1e-6)
 
 
+@pytest.mark.parametrize("rows,hidden,vocab,parts", [(64, 768, 50257, True), (411, 792, 36348, True), (1999, 768, 32000, True), (130, 2304, 600, False)])
+def test_head_gradient_in_parts_of_the_vocabulary(pt, rows, hidden, vocab, parts, monkeypatch):
+    from bamboo_b200 import lib
+    desc = lib.HeadDesc(rows=rows, vocab=vocab, hidden=hidden, ld_hidden=hidden, ld_weight=hidden, scale=1.0, ignore_index=IGNORE)
+    assert (lib.head_bwd_parts(desc, (vocab + 7) // 8 * 8) > 1) == parts and lib.head_bwd_parts(desc, 256) >= 1
+    h = torch.randn(rows, hidden, device="cuda", generator=gen(81)).bfloat16()
+    w = (torch.randn(vocab, hidden, device="cuda", generator=gen(82)) / hidden ** 0.5).bfloat16()
+    t, g = targets_of(rows, vocab, 83), torch.randn(rows, device="cuda", generator=gen(84))
+    dh = ref_head(h, w, t, vocab, 1.0, g)[1]
+    size = ref_dlogits(*ref_logps(h.double() @ w.double().t(), t, vocab)[1:], t, g, vocab).abs() @ w.double().abs()
+    whole = None
+    for limit in (256 << 20, 2 * rows * 4096):          # the vocabulary at once, and in pieces of 4096
+        monkeypatch.setattr(pt, "HEAD_GRAD_BYTES", limit)
+        for _ in range(3):
+            leaf = h.clone().requires_grad_(True)
+            pt.head_logprobs(leaf, w, t, vocab).backward(g)
+            assert ((leaf.grad.double() - dh).abs() <= 2 ** -8 * dh.abs() + 2 ** -7 * size + 1e-6).all()
+            assert whole is None or torch.equal(leaf.grad, whole)      # parts are added up in one order
+            whole = leaf.grad
+        whole = None
+
+
 def test_head_operands_of_other_layouts(pt):
     h = torch.randn(4, 9, 96, device="cuda", generator=gen(109)).bfloat16()
     w = (torch.randn(400, 104, device="cuda", generator=gen(110)) * 0.2).bfloat16()
