@@ -1658,13 +1658,13 @@ head_combine_kernel(const float2* partial, int num, int rows, const float* targe
 // out = hidden states, with zeros for the rows that do not count: the gradient of their logits is zero, but zero times what stands there
 // (NaN of a padded position) would be NaN in the weight gradient.  16 MB of 4096 x 1024: 5 us beside 1.15 ms.
 __global__ void __launch_bounds__(128)
-head_counted_rows_kernel(const __nv_bfloat16* h, long long ld, const long long* targets, long long ignore_index, int vocab, int hidden, __nv_bfloat16* out) {
+head_counted_rows_kernel(const __nv_bfloat16* h, long long ld, const long long* targets, long long ignore_index, int vocab, int hidden, __nv_bfloat16* out, long long ldo) {
   bb::pdl_sync();
   const int row = blockIdx.x;
   const long long t = targets[row];
   const bool counted = t != ignore_index && t >= 0 && t < vocab;
   const uint4* src = reinterpret_cast<const uint4*>(h + (long long)row * ld);
-  uint4* dst = reinterpret_cast<uint4*>(out + (long long)row * hidden);
+  uint4* dst = reinterpret_cast<uint4*>(out + (long long)row * ldo);
   for (int c = threadIdx.x; c < hidden >> 3; c += 128) dst[c] = counted ? src[c] : make_uint4(0, 0, 0, 0);
 }
 
@@ -1707,8 +1707,14 @@ PartsPlan plan_parts(int M, int N, int K) {
 // ... for a backward pass: no parts where the whole vocabulary is one piece and its product stored directly is expected to be no slower (the
 // estimate of the parts is up to a tenth low)
 PartsPlan head_parts(const bb_head_desc* d, int piece) {
+  // (a thread's recent plans: going through the splits takes the host some microseconds)
+  static thread_local struct { int rows = 0, hidden = 0, vocab = 0, piece = 0, dev = -1; PartsPlan pl = {}; } memo[32];
+  auto& e = memo[((unsigned)d->rows * 2654435761u ^ (unsigned)d->hidden * 2246822519u ^ (unsigned)d->vocab * 3266489917u) >> 27];
+  const int dev = bb_current_device();
+  if (dev >= 0 && e.rows == d->rows && e.hidden == d->hidden && e.vocab == d->vocab && e.piece == piece && e.dev == dev) return e.pl;
   PartsPlan pl = plan_parts(d->rows, d->hidden, piece < d->vocab ? piece : d->vocab);
   if (piece >= d->vocab && bb_gemm_store_us(d->rows, d->hidden, d->vocab, 0) <= 1.03 * pl.us + 3.0) pl.parts = 0;
+  e.rows = d->rows; e.hidden = d->hidden; e.vocab = d->vocab; e.piece = piece; e.dev = dev; e.pl = pl;
   return pl;
 }
 // out = sum of the parts, one after the other
@@ -1807,9 +1813,10 @@ extern "C" int bb_head_logprob_bwd(const bb_head_desc* d, const void* hidden_sta
   if (int rc = bbhost::bind_context()) return rc;
   cudaStream_t s = (cudaStream_t)stream;
   BackToBack overlap;
+  const long long ldc = (d->hidden + 63) / 64 * 64;          // rows on lines of their own
   if (d_weight || d_weight_accum)
     BB_CUDA_CHECK(bb_launch(head_counted_rows_kernel, d->rows, 128, 0, s, (const __nv_bfloat16*)hidden_states, d->ld_hidden, targets, d->ignore_index, d->vocab, d->hidden,
-                            (__nv_bfloat16*)counted_hidden));
+                            (__nv_bfloat16*)counted_hidden, ldc));
   for (int col0 = 0; col0 < d->vocab; col0 += piece) {
     const int cols = piece < d->vocab - col0 ? piece : d->vocab - col0;
     if (int rc = head_logits_grad(d, hidden_states, weight, targets, stats, row_grad, col0, cols, dlogits, ldd, s)) return rc;
@@ -1830,7 +1837,7 @@ extern "C" int bb_head_logprob_bwd(const bb_head_desc* d, const void* hidden_sta
       }
     }
     if (d_weight || d_weight_accum) {
-      g.M = cols; g.N = d->hidden; g.K = d->rows; g.a_mn_major = 1; g.B = counted_hidden; g.ldb = d->hidden; g.b_mn_major = 1; g.ldd = d->hidden;
+      g.M = cols; g.N = d->hidden; g.K = d->rows; g.a_mn_major = 1; g.B = counted_hidden; g.ldb = ldc; g.b_mn_major = 1; g.ldd = d->hidden;
       g.D = d_weight ? (void*)((__nv_bfloat16*)d_weight + (long long)col0 * d->hidden) : (void*)(d_weight_accum + (long long)col0 * d->hidden);
       g.epilogue = d_weight ? BB_EPI_STORE : BB_EPI_ACCUM_F32;
       if (int rc = bb_gemm_bf16(&g, stream)) return rc;

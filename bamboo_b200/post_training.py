@@ -200,12 +200,10 @@ class _HeadLogprobsFn(torch.autograd.Function):
         if rows:
             # vocabulary entries in pieces, so that the gradient of the logits never exists whole; a multiple of 256, the widest tile
             piece = max(2048, HEAD_GRAD_BYTES // (2 * rows) // 256 * 256)
-            width = (min(piece, vocab) + 7) // 8 * 8
+            width = (min(piece, vocab) + 63) // 64 * 64        # rows on lines of their own
             parts = L.head_bwd_parts(desc, piece) if need_h else 0
-            acc = torch.empty(parts, rows, n, dtype=torch.float32, device=dev) if parts else None
-            counted = torch.empty(rows, n, dtype=torch.bfloat16, device=dev) if need_w else None
-            L.head_logprob_bwd(desc, h, w, tg, stats, _flat(grad, "gradient", rows, torch.float32, dev), dh, acc, dw, main, counted, piece,
-                               torch.empty(rows, width, dtype=torch.bfloat16, device=dev))
+            scratch = torch.empty(L.head_bwd_scratch(desc, width, need_w, parts)[2], dtype=torch.uint8, device=dev)
+            L.head_logprob_bwd(desc, h, w, tg, stats, _flat(grad, "gradient", rows, torch.float32, dev), dh, parts, dw, main, piece, width, scratch)
         return dh, dw, None, None, None, None
 
 
