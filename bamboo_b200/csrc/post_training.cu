@@ -811,9 +811,11 @@ policy_ring_kernel(const T* logits, long long ld, const long long* targets, cons
   for (int it = 0;; ++it) {
     const int at = it % TURNS;
     alive = alive && bb::mbar_wait_warp(&turn_full[at], (it / TURNS) & 1, abort_flag, status);
-    const PolicyTurn turn = turns[at];
-    __syncwarp();
-    if (lane == 0) bb::mbar_arrive(&turn_empty[at]);
+    const PolicyTurn turn = turns[at];         // (handed back when the row is done, for the same reason as the stages)
+    auto turn_done = [&] {
+      __syncwarp();
+      if (lane == 0) bb::mbar_arrive(&turn_empty[at]);
+    };
     const int row = turn.row, t = turn.t;
     // a wait that ran out in one warp ends the loop for all of them here, where their barriers match
     if (!alive) s_dead = 1;
@@ -824,6 +826,7 @@ policy_ring_kernel(const T* logits, long long ld, const long long* targets, cons
     if (t < 0) {
       if (threadIdx.x == 0) row_sums[row] = {0.f, 0.f, 0.f, 0.f};
       grad_row<T, THREADS, ROW_LOADS>(x, d, V, cols, 0, 0.f, k, 0.f, 0.f);
+      turn_done();
       continue;
     }
     // ---- sum
@@ -862,7 +865,9 @@ policy_ring_kernel(const T* logits, long long ld, const long long* targets, cons
     r = s_row[0]; s = s_row[1];
     float g = s_row[2];
     if (s == 0.f) g = 0.f;
-    // ---- gradient; a stage is handed back by the warps that have taken their chunks out of it
+    // ---- gradient; a stage is handed back by the warps that have taken their chunks out of it, which is certain once what was made of them
+    // is on its way: an arrival right behind the loads may pass them (they queue behind stores of earlier stages), and the next
+    // row's first lines land in what is still to be read
     const bool plain = g == 0.f || s < 0.f || (((uintptr_t)x ^ (uintptr_t)d) & 15) != 0;
     const GradRow gw = grad_factors(g, k, plain ? 0.f : r, s);
     const int whole = plain ? 0 : (V - sp.lead) / VEC;         // chunks of vocabulary entries only
@@ -872,13 +877,14 @@ policy_ring_kernel(const T* logits, long long ld, const long long* targets, cons
       uint4 q[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) q[u] = c + u * THREADS < whole ? ring[c + u * THREADS] : make_uint4(0, 0, 0, 0);
-      __syncwarp();
-      if (lane == 0) bb::mbar_arrive(&empty[j]);
 #pragma unroll
       for (int u = 0; u < U; ++u) if (c + u * THREADS < whole) grad_chunk<T>(dv + c + u * THREADS, q[u], gw);
+      __syncwarp();
+      if (lane == 0) bb::mbar_arrive(&empty[j]);
     }
     if (plain) grad_row<T, THREADS, ROW_LOADS>(x, d, V, cols, t, g, k, r, s);
     else grad_rest<T, THREADS>(x, xt, d, sp.lead, whole, V, cols, t, g, k, s, gw);
+    turn_done();
     phase ^= 1;
   }
   if (!alive) {

@@ -607,6 +607,19 @@ def test_many_rows_of_every_size(pt, rows, vocab, cols, dtype):
     near(grad, ref_dlogits(probs, counted, t, row_grad, cols, 0.9), (4e-6 if dtype == torch.float32 else 2 ** -8) + 4 * err, 4 * err * size)
 
 
+@pytest.mark.parametrize("rows,vocab,dtype", [(2050, 41003, torch.bfloat16), (3000, 50257, torch.bfloat16), (1100, 12001, torch.float32)])
+def test_policy_rows_wait_for_their_readers(pt, rows, vocab, dtype):
+    """Rows that follow one another through shared memory: the same result every time."""
+    x, t = logits_of(rows, vocab, vocab, dtype, 71), targets_of(rows, vocab, 72)
+    old, adv, ref = policy_inputs(pt.token_logprobs(x, t).double(), 73)
+    loss_fn = pt.PolicyLoss(vocab, clip_low=0.2, clip_high=0.3, kl_coef=0.05, temperature=0.9, inplace=False)
+    offsets, first = torch.tensor([0, rows], device="cuda"), None
+    for _ in range(25):
+        loss, stats, grad = loss_fn.loss_and_grad(x, (t, old, adv, ref), offsets=offsets)
+        assert first is None or (torch.equal(grad, first[2]) and torch.equal(stats, first[1]) and loss == first[0])
+        first = first or (loss, stats, grad)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("offset", [0, 1, 3])
 @pytest.mark.parametrize("vocab", [1003, 30011])
