@@ -65,6 +65,11 @@ def _flat(t, name, numel, dtype, device):
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _row_grad(grad, rows):
+    """What autograd hands to a backward pass, as contiguous fp32."""
+    return grad if grad.is_contiguous() and grad.dtype is torch.float32 else _flat(grad, "gradient", rows, torch.float32, grad.device)
+
+
 def _geometry(targets, offsets):
     """(sequences, offsets as int64): the rows of 2-D targets, or what the offsets delimit in 1-D ones."""
     if offsets is not None:
@@ -102,19 +107,18 @@ class _TokenLogprobsFn(torch.autograd.Function):
         lg, rows, vocab = _rows(logits, vocab)
         tg = _flat(targets, "targets", rows, torch.int64, lg.device)
         logp, stats = _logprobs(lg, rows, tg, vocab, scale, ignore_index, targets.shape)
-        ctx.args, ctx.shape, ctx.inplace = (rows, vocab, scale, ignore_index), logits.shape, inplace
-        ctx.save_for_backward(lg.detach(), tg, stats)
+        ctx.args = rows, vocab, scale, ignore_index, inplace, stats, None if lg is logits else logits.shape
+        ctx.save_for_backward(lg, tg)
         return logp
 
     @staticmethod
     def backward(ctx, grad):
-        lg, tg, stats = ctx.saved_tensors
-        rows, vocab, scale, ignore_index = ctx.args
-        out = lg if ctx.inplace else torch.empty(lg.shape, dtype=lg.dtype, device=lg.device)
+        lg, tg = ctx.saved_tensors
+        rows, vocab, scale, ignore_index, inplace, stats, shape = ctx.args
+        out = lg.detach() if inplace else torch.empty_like(lg)
         if rows:
-            row_grad = _flat(grad, "gradient", rows, torch.float32, lg.device)
-            L.token_logprob_bwd(lg, tg, stats, row_grad, out, vocab, scale, ignore_index)
-        return out.view(ctx.shape), None, None, None, None, None
+            L.token_logprob_bwd(lg, tg, stats, _row_grad(grad, rows), out, vocab, scale, ignore_index)
+        return out if shape is None else out.view(shape), None, None, None, None, None
 
 
 def token_logprobs(logits, targets, vocab=None, *, temperature=1.0, ignore_index=-100, inplace=False):
@@ -182,18 +186,18 @@ class _HeadLogprobsFn(torch.autograd.Function):
     def forward(ctx, hidden, weight, targets, vocab, scale, ignore_index):
         desc, h, w, tg = _head_operands(hidden, weight, targets, vocab, scale, ignore_index)
         logp, stats = _head_forward(desc, h, w, tg, targets.shape)
-        ctx.desc, ctx.weight, ctx.shape = desc, weight, hidden.shape
-        ctx.save_for_backward(h.detach(), w.detach(), tg, stats)
+        ctx.args = desc, weight, hidden.shape, stats
+        ctx.save_for_backward(h, w, tg)
         return logp
 
     @staticmethod
     def backward(ctx, grad):
-        h, w, tg, stats = ctx.saved_tensors
-        desc, weight, dev = ctx.desc, ctx.weight, h.device
-        rows, n, vocab = desc.rows, desc.hidden, desc.vocab
+        h, w, tg = ctx.saved_tensors
+        desc, weight, shape, stats = ctx.args
+        dev, rows, n, vocab = h.device, desc.rows, desc.hidden, desc.vocab
         need_h, need_w = ctx.needs_input_grad[:2]
         main = getattr(weight, "main_grad", None) if need_w else None
-        dh = torch.empty(ctx.shape, dtype=torch.bfloat16, device=dev) if need_h else None
+        dh = torch.empty(shape, dtype=torch.bfloat16, device=dev) if need_h else None
         dw = torch.empty(weight.shape, dtype=torch.bfloat16, device=dev) if need_w and main is None else None
         if dw is not None and (vocab < dw.shape[0] or not rows):
             dw[vocab if rows else 0:].zero_()
@@ -203,7 +207,7 @@ class _HeadLogprobsFn(torch.autograd.Function):
             width = (min(piece, vocab) + 63) // 64 * 64        # rows on lines of their own
             parts = L.head_bwd_parts(desc, piece) if need_h else 0
             scratch = torch.empty(L.head_bwd_scratch(desc, width, need_w, parts)[2], dtype=torch.uint8, device=dev)
-            L.head_logprob_bwd(desc, h, w, tg, stats, _flat(grad, "gradient", rows, torch.float32, dev), dh, parts, dw, main, piece, width, scratch)
+            L.head_logprob_bwd(desc, h, w, tg, stats, _row_grad(grad, rows), dh, parts, dw, main, piece, width, scratch)
         return dh, dw, None, None, None, None
 
 
