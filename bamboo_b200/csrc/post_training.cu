@@ -1164,12 +1164,16 @@ long long sum_piece(const bb_grad_tensor* list, int count) {
   return piece < 4096 ? 4096 : piece > SUM_PIECE ? SUM_PIECE : piece;
 }
 
-// Counters of the CTAs that are done, one per launch in turn; each is zero again when its launch is over
-constexpr unsigned DONE_SLOTS = 1u << 16;
-__device__ unsigned int g_norm_done[DONE_SLOTS];
-unsigned int* norm_done() {
+// Counters of the CTAs that are done, one per launch in turn; each is zero again when its launch is over.  A launch that is being captured
+// keeps its counter for good, so those have a half of their own: a graph's replay never meets a launch that came round to the same one.
+constexpr unsigned DONE_SLOTS = 1u << 15;
+__device__ unsigned int g_norm_done[2 * DONE_SLOTS];
+unsigned int* norm_done(cudaStream_t stream) {
   static unsigned int* table[64] = {nullptr};
-  static std::atomic<unsigned> next{0};
+  static std::atomic<unsigned> next[2];
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &status) != cudaSuccess) (void)cudaGetLastError();
+  const int half = status == cudaStreamCaptureStatusNone ? 0 : 1;
   const int dev = bb_current_device();
   if (dev < 0) return nullptr;
   if (!table[dev]) {
@@ -1177,7 +1181,7 @@ unsigned int* norm_done() {
     if (cudaGetSymbolAddress(&ptr, g_norm_done) != cudaSuccess) return nullptr;
     table[dev] = static_cast<unsigned int*>(ptr);
   }
-  return table[dev] + next.fetch_add(1u) % DONE_SLOTS;
+  return table[dev] + half * DONE_SLOTS + next[half].fetch_add(1u) % DONE_SLOTS;
 }
 
 bool bad_list(const bb_grad_tensor* list, int count) {
@@ -1469,7 +1473,7 @@ int list_sumsq(const bb_grad_tensor* tensors, int count, double* workspace, cuda
     const int n = count - at < LIST_TENSORS ? count - at : LIST_TENSORS;
     TensorTable t;
     const int pieces = table_fill(t, tensors + at, n, sum_piece(tensors + at, n));
-    unsigned int* done = norm_done();
+    unsigned int* done = norm_done(s);
     if (!done) { bb_set_last_error_msg("bb_grad_sumsq: counters unavailable on this device"); return BB_ERR_CUDA; }
     BB_CUDA_CHECK(bb_launch(grad_sumsq_kernel, pieces < NORM_CTAS ? pieces : NORM_CTAS, NORM_THREADS, 0, s, t, workspace + 2, workspace, at > 0 ? 1 : 0, done,
                             at + n < count ? ClipTo{} : clip));

@@ -815,3 +815,22 @@ def test_offsets_that_do_not_ascend_are_reported(pt):
         pt.policy_loss(lp, lp, lp, t, offsets=off, reduction="sequence")
         torch.cuda.synchronize()
         assert lib.read_status() < 0
+
+
+def test_gradient_clipping_in_a_graph_beside_other_calls(pt):
+    """A captured norm replayed between calls that are launched one by one: counters of their own, the same results."""
+    grads = [torch.randn(n, device="cuda", generator=gen(200 + n)) for n in (70001, 5, 300000)]
+    want = torch.sqrt(sum(g.double().square().sum() for g in grads))
+    keep, other = [g.clone() for g in grads], [torch.ones(50000, device="cuda")]
+    pt.global_grad_norm(grads)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = pt.clip_grad_norm_(grads, 0.25)
+    for _ in range(4):
+        for g, k in zip(grads, keep):
+            g.copy_(k)
+        graph.replay()
+        near(pt.global_grad_norm(other).reshape(1), torch.tensor([50000 ** 0.5], dtype=torch.float64, device="cuda"), 1e-6, 0)
+        near(norm.reshape(1), want.reshape(1), 1e-6, 0)
+        for g, k in zip(grads, keep):
+            near(g, k.double() * (0.25 / (want + 1e-6)), 1e-6, 0)
