@@ -735,9 +735,9 @@ def _tensor_table(n):
     return struct.Struct("QqiI" * n)        # bb_grad_tensor[n]
 
 
-def grad_tensors(fields):
-    """bb_grad_tensor[] from (address, elements, type, 0) of every tensor, one after the other."""
-    return _tensor_table(len(fields) // 4).pack(*fields)
+def grad_tensors(fields, count):
+    """bb_grad_tensor[count] from (address, elements, type, 0) of every tensor, one after the other."""
+    return _tensor_table(count).pack(*fields)
 
 
 _norm_bytes = None

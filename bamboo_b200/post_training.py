@@ -16,6 +16,8 @@ advantages may be anything, NaN and infinities included.  Everything runs on the
 fallback: CPU tensors are refused.
 """
 import functools
+import itertools
+import operator
 
 import torch
 from torch import nn
@@ -460,35 +462,44 @@ def _dense(t):
     return True
 
 
+_dtype_of = operator.attrgetter("dtype")
+
+
+def _gradient_of(t):
+    """The gradient of a parameter (``main_grad`` of an arena's, else ``grad``), another tensor as it is."""
+    if isinstance(t, nn.Parameter):
+        main = getattr(t, "main_grad", None)
+        return t.grad if main is None else main
+    return t
+
+
 def _gradients(tensors):
-    """(tensors for the kernels, [(gradient, its copy without gaps)], bb_grad_tensor fields) of a list: the gradients of parameters
-    (``main_grad`` of an arena's, else ``grad``), other tensors as they are, empty ones left out."""
-    grads, staged, fields, device, codes = [], [], [], None, L.dtype_codes()
-    for t in ((tensors,) if isinstance(tensors, torch.Tensor) else tensors):
-        if type(t) is not torch.Tensor:
-            if isinstance(t, nn.Parameter):
-                main = getattr(t, "main_grad", None)
-                t = t.grad if main is None else main
-            if t is None:
-                continue
-        n = t.numel()
-        if n == 0:
-            continue
-        if t.get_device() != device:
-            _on_current(t, "gradients")
-            device = t.get_device()
-        if not t.is_contiguous() and not _dense(t):
-            gradient, t = t.detach(), t.detach().contiguous()
-            staged.append((gradient, t))
-        fields += (t.data_ptr(), n, codes.get(t.dtype, -1), 0)
-        grads.append(t)
-    return grads, staged, fields
+    """(tensors for the kernels, [(gradient, its copy without gaps)], bb_grad_tensor fields) of a list, empty tensors left out.  (The list is
+    gone through property by property: 60 ns each.)"""
+    grads = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if set(map(type, grads)) != {torch.Tensor}:
+        grads = [t for t in map(_gradient_of, grads) if t is not None]
+    sizes = list(map(torch.Tensor.numel, grads))
+    if not all(sizes):
+        grads, sizes = [t for t, n in zip(grads, sizes) if n], [n for n in sizes if n]
+    staged = []
+    here = torch._C._cuda_getDevice() if grads else None
+    for at, where in enumerate(map(torch.Tensor.get_device, grads)):
+        if where != here:
+            _on_current(grads[at], "gradients")
+    if not all(map(torch.Tensor.is_contiguous, grads)):
+        for at, t in enumerate(grads):
+            if not _dense(t):
+                grads[at] = t.detach().contiguous()
+                staged.append((t.detach(), grads[at]))
+    codes = map(L.dtype_codes().get, map(_dtype_of, grads), itertools.repeat(-1))
+    return grads, staged, itertools.chain.from_iterable(zip(map(torch.Tensor.data_ptr, grads), sizes, codes, itertools.repeat(0)))
 
 
 def grad_sumsq(tensors):
     """Sum of squares over all gradients together (fp64 [1] on their device)."""
     grads, _, fields = _gradients(tensors)
-    return L.grad_sumsq(L.grad_tensors(fields), len(grads)).clone()
+    return L.grad_sumsq(L.grad_tensors(fields, len(grads)), len(grads)).clone()
 
 
 def global_grad_norm(tensors):
@@ -509,7 +520,7 @@ def clip_grad_norm_(tensors, max_norm):
     grads, staged, fields = _gradients(tensors)
     if not grads:
         return torch.zeros(())
-    norm = L.grad_clip(L.grad_tensors(fields), len(grads), max_norm, torch.empty((), dtype=torch.float32, device=grads[0].device))
+    norm = L.grad_clip(L.grad_tensors(fields, len(grads)), len(grads), max_norm, torch.empty((), dtype=torch.float32, device=grads[0].device))
     for gradient, copy in staged:
         gradient.copy_(copy)
     return norm
