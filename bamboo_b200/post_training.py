@@ -483,10 +483,9 @@ def _gradients(tensors):
     if not all(sizes):
         grads, sizes = [t for t, n in zip(grads, sizes) if n], [n for n in sizes if n]
     staged = []
-    here = torch._C._cuda_getDevice() if grads else None
-    for at, where in enumerate(map(torch.Tensor.get_device, grads)):
-        if where != here:
-            _on_current(grads[at], "gradients")
+    devices = list(map(torch.Tensor.get_device, grads))
+    for device in set(devices):
+        _on_current(grads[devices.index(device)], "gradients")
     if not all(map(torch.Tensor.is_contiguous, grads)):
         for at, t in enumerate(grads):
             if not _dense(t):
