@@ -147,8 +147,11 @@ template <typename T, int THREADS> __device__ __forceinline__ void soft_edges(co
 }
 
 // (r, s) of this thread's share of a row's chunks.  The reference comes from the thread's first chunk and stays: a later logit may be larger,
-// 2^(k x - r) is a float all the same as long as it is below 2^127, so the loop needs no maximum; a share whose first chunk
-// is all -inf or whose sum did overflow is taken (again) in the exact form.  U loads are in flight per thread.
+// 2^(k x - r) is a float all the same, so the loop needs no maximum; a share whose first chunk is all -inf or whose sum reaches SHARE_MOST
+// is taken (again) in the exact form.  That bound keeps what the merges make of the shares: 8 x 512 of them add up to less than 2^76, far from
+// overflow; a share that a difference of 127 between references flushes to zero was below 2^-63 of the sum; and 1 / s is no denormal
+// number.  U loads are in flight per thread.
+constexpr float SHARE_MOST = 0x1p64f;
 template <typename T, int THREADS, int U>
 __device__ __forceinline__ void soft_share(const uint4* v, int nvec, K2 k, float& r, float& s) {
   constexpr int VEC = Elem<T>::VEC;
@@ -177,7 +180,7 @@ __device__ __forceinline__ void soft_share(const uint4* v, int nvec, K2 k, float
   }
   s += sum.x + sum.y;
   // (with r = -inf the loop has added NaN or +inf)
-  if (!(s < INFINITY)) { const float2 e = soft_share_exact<T, THREADS>(v, nvec, k); r = e.x; s = e.y; }
+  if (!(s < SHARE_MOST)) { const float2 e = soft_share_exact<T, THREADS>(v, nvec, k); r = e.x; s = e.y; }
 }
 
 // A row whose largest logit is so far from zero that k x is not finite (a row of the type's lowest value): differences at that
@@ -856,7 +859,7 @@ policy_ring_kernel(const T* logits, long long ld, const long long* targets, cons
       }
     }
     s += sum.x + sum.y;
-    if (!(s < INFINITY)) { const float2 e = soft_share_exact<T, THREADS>(ring, sp.nvec, k); r = e.x; s = e.y; }
+    if (!(s < SHARE_MOST)) { const float2 e = soft_share_exact<T, THREADS>(ring, sp.nvec, k); r = e.x; s = e.y; }
     soft_edges<T, THREADS>(x, sp, V, k, r, s);
     soft_block<THREADS, true>(r, s, smem);
     if (threadIdx.x < 32 && isinf(r)) { const float2 e = soft_row_extreme(x, V); r = e.x; s = e.y; }

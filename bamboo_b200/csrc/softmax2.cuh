@@ -1,5 +1,6 @@
-// Softmax in base 2.  With k = scale * log2(e) the kernels sum 2^(k x - r) for an INTEGER reference r >= max(k x): partial sums with
-// different references meet exactly (powers of two).  A row is kept as the pair (r, s): softmax_j = 2^(k x_j - r) / s, log
+// Softmax in base 2.  With k = scale * log2(e) the kernels sum 2^(k x - r) for an INTEGER reference r: partial sums with different references
+// meet exactly (powers of two).  soft_add keeps r >= max(k x); where r is the maximum of a part of the logits only, the caller bounds
+// the sum that may come of it.  A row is kept as the pair (r, s): softmax_j = 2^(k x_j - r) / s, log
 // softmax_j = (k x_j - r - log2 s) ln 2, the latter once per row in 64 bits.  k comes in two parts (K2): rounded to 32 bits it would
 // be another temperature, 1.3e-8 off, which moves every log-probability of a sequence to the same side (measured on four
 // sequences of 1024 tokens: the sum of log-ratios 2.7e-5 off, in two parts 2e-6, which is the rounding of the log-probabilities).
