@@ -239,12 +239,14 @@ template <typename T> __device__ __forceinline__ void grad_chunk(uint4* d, const
   *d = Elem<T>::pack(f);
 }
 // What follows the chunks [0, whole): the target's entry (xt its logit, read before d, which may be x, was written; by the thread
-// that wrote its chunk), the chunk that the padding begins in, the padding, and the elements around the 16-byte boundaries
+// that wrote its chunk), the chunk that the padding begins in, the padding, and the elements around the 16-byte boundaries.  The chunks here are
+// those of all columns: a vocabulary that ends before the first boundary has none, while the padding behind it goes on past it.
 template <typename T, int THREADS>
-__device__ __forceinline__ void grad_rest(const T* x, float xt, T* d, int lead, int whole, int V, int cols, int t, float g, K2 k, float s, const GradRow& w) {
+__device__ __forceinline__ void grad_rest(const T* x, float xt, T* d, int whole, int V, int cols, int t, float g, K2 k, float s, const GradRow& w) {
   constexpr int VEC = Elem<T>::VEC;
-  if (t >= lead) {
-    const int tc = (t - lead) / VEC;
+  const Span<T> sp(d, cols);
+  if (t >= sp.lead) {
+    const int tc = (t - sp.lead) / VEC;
     if (tc < whole && tc % THREADS == row_thread<THREADS>()) Elem<T>::put(d + t, grad_target(g, xt, k, w.r, s));
   }
   auto one = [&](int j) {
@@ -252,13 +254,12 @@ __device__ __forceinline__ void grad_rest(const T* x, float xt, T* d, int lead, 
     if (j < V) { const float f = Elem<T>::get(x + j); v = j == t ? grad_target(g, f, k, w.r, s) : grad_entry(w, f); }
     Elem<T>::put(d + j, v);
   };
-  const int nvec = (cols - lead) / VEC, tail = lead + nvec * VEC;
-  for (int c = whole + row_thread<THREADS>(); c < nvec; c += THREADS) {
-    const int j0 = lead + c * VEC;
+  for (int c = whole + row_thread<THREADS>(); c < sp.nvec; c += THREADS) {
+    const int j0 = sp.lead + c * VEC;
     if (j0 >= V) *reinterpret_cast<uint4*>(d + j0) = make_uint4(0, 0, 0, 0);
     else for (int i = 0; i < VEC; ++i) one(j0 + i);
   }
-  for (int j = row_thread<THREADS>(); j < lead + cols - tail; j += THREADS) one(j < lead ? j : tail + j - lead);
+  for (int j = row_thread<THREADS>(); j < sp.lead + cols - sp.tail; j += THREADS) one(j < sp.lead ? j : sp.tail + j - sp.lead);
 }
 
 // d[j] = g * ([j == t] - softmax_j) for j < V, 0 in [V, cols); zeros throughout when g == 0 (nothing is read then).  FAR: the row comes
@@ -310,7 +311,7 @@ __device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int 
   } else {
     for (; c < whole; c += THREADS) grad_chunk<T>(dv + c, xv[c], w);
   }
-  grad_rest<T, THREADS>(x, xt, d, sp.lead, whole, V, cols, t, g, k, s, w);
+  grad_rest<T, THREADS>(x, xt, d, whole, V, cols, t, g, k, s, w);
 }
 
 // ------------------------------------------------------------------ sums of a block
@@ -886,7 +887,7 @@ policy_ring_kernel(const T* logits, long long ld, const long long* targets, cons
       if (lane == 0) bb::mbar_arrive(&empty[j]);
     }
     if (plain) grad_row<T, THREADS, ROW_LOADS>(x, d, V, cols, t, g, k, r, s);
-    else grad_rest<T, THREADS>(x, xt, d, sp.lead, whole, V, cols, t, g, k, s, gw);
+    else grad_rest<T, THREADS>(x, xt, d, whole, V, cols, t, g, k, s, gw);
     turn_done();
     phase ^= 1;
   }

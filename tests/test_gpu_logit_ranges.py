@@ -116,3 +116,39 @@ def test_losses_and_their_gradients(pt, rows, vocab, dtype, pattern):
     want = -row * probs[:even]
     want[torch.arange(even, device="cuda"), t[:even]] += row[:, 0]
     near(grad, want, 1.5e-5 if dtype == F32 else 2 ** -8 + 2e-6, 1e-7 * row.abs().max().item())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_vocabularies_shorter_than_the_way_to_a_boundary(pt, dtype):
+    """Rows that start anywhere, a vocabulary that ends before their first 16-byte boundary, and padding that goes on past it."""
+    gen = torch.Generator(device="cuda").manual_seed(35)
+    for vocab in range(1, 9):
+        for cols in (vocab, vocab + 1, 9, 13, 17, 23, 40):
+            if cols < vocab:
+                continue
+            rows = 19
+            x = torch.randn(rows, cols, device="cuda", generator=gen).to(dtype)
+            x[:, vocab:] = math.nan
+            t = torch.randint(0, vocab, (rows,), device="cuda", generator=gen)
+            g = torch.randn(rows, device="cuda", generator=gen)
+            lp, probs = reference(x[:, :vocab], t, 1.0)
+            want = -g.double()[:, None] * probs
+            want[torch.arange(rows, device="cuda"), t] += g.double()
+            want = torch.nn.functional.pad(want, (0, cols - vocab))
+            rel, floor = 1.2e-5 if dtype == F32 else 2 ** -8, 1e-7 * g.abs().max().item()
+            for inplace in (False, True):
+                leaf = x.clone().requires_grad_(True)
+                out = pt.token_logprobs(leaf, t, vocab, inplace=inplace)
+                near(out.detach(), lp, 1e-6, 4e-6)
+                near(torch.autograd.grad(out, leaf, g)[0], want, rel, floor)
+            y = x.clone()
+            _, _, grad = pt.PolicyLoss(vocab).loss_and_grad(y, (t.view(1, -1), None, g), out=y)
+            near(grad, -want / rows, rel, floor)
+            y = x[:18].clone()
+            _, _, grad = pt.PreferenceLoss(vocab, beta=1.0, form="hinge").loss_and_grad(y, t[:18].view(18, 1), out=y)
+            h = lp[0:18:2] - lp[1:18:2]
+            slope = torch.where(h < 1, -1.0, 0.0).double() / 9
+            row = torch.stack((slope, -slope), 1).reshape(-1, 1)
+            want = -row * probs[:18]
+            want[torch.arange(18, device="cuda"), t[:18]] += row[:, 0]
+            near(grad, torch.nn.functional.pad(want, (0, cols - vocab)), rel, 1e-7)
