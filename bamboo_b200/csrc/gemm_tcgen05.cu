@@ -108,6 +108,8 @@ struct HeadParams {
   const float2* stats;        // GRAD: (r, s) per row
   const float* row_grad; float gscale;
 };
+// Logits whose exponent reaches this count as infinite: the row cannot be looked at again (see soft_add)
+constexpr float HEAD_FAR = 0x1p31f;
 // The tensor core's fp32 additions truncate, so a sum's error grows with the number of its k-blocks (a logit of 4096 products
 // 4.6e-5 off, of 1024 products 2.4e-6).  Projections from more than 2048 columns sum the halves of the reduction into the two
 // accumulators and add those in the epilogue; the main loop of the next tile then covers less of the epilogue.
@@ -599,7 +601,7 @@ template <int HEAD> struct HeadRow {
 #pragma unroll
       for (int i = 0; i < 64; ++i) if (nb + i >= N) v[i] = -INFINITY;
     }
-    bb::soft_add<64>(r, s, v, h.k);
+    bb::soft_add<64>(r, s, v, h.k, -HEAD_FAR);
   }
   __device__ __forceinline__ void gradient(const HeadParams& h, int nb, float* v) {
     const float ng = -g / s;
@@ -1649,6 +1651,7 @@ head_combine_kernel(const float2* partial, int num, int rows, const float* targe
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane != 0 || row >= rows) return;
+  if (r >= HEAD_FAR) s = NAN;
   const bool counted = t != ignore_index && t >= 0 && t < vocab;
   if (!counted && t != ignore_index) atomicCAS(status, 0, BB_ERR_INVALID_ARG);
   logp[row] = counted ? (float)bb::row_logp(xt, k, r, s) : 0.f;

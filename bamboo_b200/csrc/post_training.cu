@@ -125,7 +125,7 @@ template <typename T, int THREADS> __device__ __noinline__ float2 soft_share_exa
   for (int c = row_thread<THREADS>(); c < nvec; c += THREADS) {
     float f[VEC];
     Elem<T>::unpack(v[c], f);
-    soft_add<VEC>(r, s, f, k);
+    soft_add<VEC>(r, s, f, k, -bb::SOFT_FAR);
   }
   return make_float2(r, s);
 }
@@ -142,13 +142,13 @@ template <int VEC> __device__ __forceinline__ void soft_chunk(float2& sum, const
 template <typename T, int THREADS> __device__ __forceinline__ void soft_edges(const T* x, const Span<T>& sp, int n, K2 k, float& r, float& s) {
   for (int j = row_thread<THREADS>(); j < sp.lead + n - sp.tail; j += THREADS) {
     const float f = Elem<T>::get(x + (j < sp.lead ? j : sp.tail + j - sp.lead));
-    soft_add<1>(r, s, &f, k);
+    soft_add<1>(r, s, &f, k, -bb::SOFT_FAR);
   }
 }
 
 // (r, s) of this thread's share of a row's chunks.  The reference comes from the thread's first chunk and stays: a later logit may be larger,
-// 2^(k x - r) is a float all the same, so the loop needs no maximum; a share whose first chunk is all -inf or whose sum reaches SHARE_MOST
-// is taken (again) in the exact form.  That bound keeps what the merges make of the shares: 8 x 512 of them add up to less than 2^76, far from
+// 2^(k x - r) is a float all the same, so the loop needs no maximum; a share whose sum reaches SHARE_MOST (above a first
+// chunk that is masked, for one) is taken (again) in the exact form.  That bound keeps what the merges make of the shares: 8 x 512 of them add up to less than 2^76, far from
 // overflow; a share that a difference of 127 between references flushes to zero was below 2^-63 of the sum; and 1 / s is no denormal
 // number.  U loads are in flight per thread.
 constexpr float SHARE_MOST = 0x1p64f;
@@ -161,7 +161,7 @@ __device__ __forceinline__ void soft_share(const uint4* v, int nvec, K2 k, float
   float f[VEC];
   if (c < nvec) {
     Elem<T>::unpack(v[c], f);
-    soft_add<VEC>(r, s, f, k);
+    soft_add<VEC>(r, s, f, k, -bb::SOFT_FAR);
     c += THREADS;
   }
   for (; c + (U - 1) * THREADS < nvec; c += U * THREADS) {
@@ -179,31 +179,32 @@ __device__ __forceinline__ void soft_share(const uint4* v, int nvec, K2 k, float
     for (int u = 0; u < U - 1; ++u) { Elem<T>::unpack(q[u], f); soft_chunk<VEC>(sum, f, k, r); }
   }
   s += sum.x + sum.y;
-  // (with r = -inf the loop has added NaN or +inf)
   if (!(s < SHARE_MOST)) { const float2 e = soft_share_exact<T, THREADS>(v, nvec, k); r = e.x; s = e.y; }
 }
 
-// A row whose largest logit is so far from zero that k x is not finite (a row of the type's lowest value): differences at that
-// magnitude leave all of the softmax to the logits that equal the largest.  Kept as (largest, -how many of them there are);
-// (NaN, NaN) with a NaN or +inf in the row, (-inf, 0) when every logit is -inf.  Called by the first warp where r is infinite.
-template <typename T> __device__ __noinline__ float2 soft_row_extreme(const T* x, int n) {
+// A row whose largest logit is so far from zero that integer references are too coarse (a row masked whole by a large negative value): kept as
+// (largest, -sum of 2^(k (x - largest))), so that what is rounded is a difference; (NaN, NaN) with a NaN or +inf in the row, (-inf, 0)
+// when every logit is -inf.  Called by the first warp.
+template <typename T> __device__ __noinline__ float2 soft_row_far(const T* x, int n, K2 k) {
   float top = -INFINITY;
-  int count = 0, bad = 0;
+  int bad = 0;
   for (int j = threadIdx.x & 31; j < n; j += 32) {
     const float f = Elem<T>::get(x + j);
     bad |= f != f || f == INFINITY;
-    if (f > top) { top = f; count = 1; } else if (f == top) ++count;
+    top = fmaxf(top, f);
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float t2 = __shfl_xor_sync(0xffffffffu, top, o);
-    const int c2 = __shfl_xor_sync(0xffffffffu, count, o);
-    count = (top >= t2 ? count : 0) + (t2 >= top ? c2 : 0);
-    top = fmaxf(top, t2);
-  }
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (__any_sync(0xffffffffu, bad)) return make_float2(NAN, NAN);
-  return make_float2(top, top == -INFINITY ? 0.f : -(float)count);
+  if (top == -INFINITY) return make_float2(top, 0.f);
+  float sum = 0.f;
+  for (int j = threadIdx.x & 31; j < n; j += 32) sum += ex2(bb::expo_gap(Elem<T>::get(x + j) - top, k));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return make_float2(top, -sum);
 }
+
+__device__ __forceinline__ bool soft_far(float r) { return fabsf(r) >= bb::SOFT_FAR; }
 
 // The row's (r, s), in the row's first warp
 template <typename T, int THREADS, int U>
@@ -213,7 +214,7 @@ __device__ __forceinline__ void soft_whole_row(const T* x, int n, K2 k, float& r
   soft_edges<T, THREADS>(x, sp, n, k, r, s);
   if constexpr (THREADS == 32) soft_warp(r, s);
   else soft_block<THREADS>(r, s, smem);
-  if (row_thread<THREADS>() < 32 && isinf(r)) { const float2 e = soft_row_extreme(x, n); r = e.x; s = e.y; }
+  if (row_thread<THREADS>() < 32 && soft_far(r)) { const float2 e = soft_row_far(x, n, k); r = e.x; s = e.y; }
 }
 
 // -g softmax_j = ng 2^(k x_j - r).  Here k rounded to 32 bits will do: with what the rounding took at the largest logit (about r / k) in
@@ -282,7 +283,7 @@ __device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int 
       float v = 0.f;
       if (j < V) {
         const float f = Elem<T>::get(x + j);
-        if (s < 0.f) v = (f == r ? g / s : 0.f) + (j == t ? g : 0.f);
+        if (s < 0.f) v = fmaf(g / s, ex2(bb::expo_gap(f - r, k)), j == t ? g : 0.f);
         else v = j == t ? grad_target(g, f, k, r, s) : grad_entry(w, f);
       }
       Elem<T>::put(d + j, v);
@@ -439,7 +440,7 @@ token_logprob_fwd_cluster_kernel(const T* logits, long long ld, const long long*
   const float2 q = (int)threadIdx.x < size ? parts[threadIdx.x] : make_float2(-INFINITY, 0.f);
   r = q.x; s = q.y;
   soft_warp(r, s);
-  if (isinf(r)) { const float2 e = soft_row_extreme(x, V); r = e.x; s = e.y; }
+  if (soft_far(r)) { const float2 e = soft_row_far(x, V, k); r = e.x; s = e.y; }
   if (threadIdx.x == 0) {
     put_logp(row_logp(xt, k, r, s), row, logp, rest);
     if (stats) stats[row] = make_float2(r, s);
@@ -850,7 +851,7 @@ policy_ring_kernel(const T* logits, long long ld, const long long* targets, cons
         uint4 q[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) q[u] = ring[c + u * THREADS];
-        if (j == 0) { Elem<T>::unpack(q[0], f); soft_add<VEC>(r, s, f, k); }
+        if (j == 0) { Elem<T>::unpack(q[0], f); soft_add<VEC>(r, s, f, k, -bb::SOFT_FAR); }
 #pragma unroll
         for (int u = 0; u < U; ++u)
           if (u > 0 || j > 0) { Elem<T>::unpack(q[u], f); soft_chunk<VEC>(sum, f, k, r); }
@@ -858,7 +859,7 @@ policy_ring_kernel(const T* logits, long long ld, const long long* targets, cons
         for (int u = 0; u < U; ++u) {
           if (c + u * THREADS >= sp.nvec) break;
           Elem<T>::unpack(ring[c + u * THREADS], f);
-          if (j == 0 && u == 0) soft_add<VEC>(r, s, f, k);
+          if (j == 0 && u == 0) soft_add<VEC>(r, s, f, k, -bb::SOFT_FAR);
           else soft_chunk<VEC>(sum, f, k, r);
         }
       }
@@ -867,7 +868,7 @@ policy_ring_kernel(const T* logits, long long ld, const long long* targets, cons
     if (!(s < SHARE_MOST)) { const float2 e = soft_share_exact<T, THREADS>(ring, sp.nvec, k); r = e.x; s = e.y; }
     soft_edges<T, THREADS>(x, sp, V, k, r, s);
     soft_block<THREADS, true>(r, s, smem);
-    if (threadIdx.x < 32 && isinf(r)) { const float2 e = soft_row_extreme(x, V); r = e.x; s = e.y; }
+    if (threadIdx.x < 32 && soft_far(r)) { const float2 e = soft_row_far(x, V, k); r = e.x; s = e.y; }
     if (threadIdx.x == 0) policy_row_finish(p, turn.in, row, xt, k, r, s, turn.weight, gscale, s_row, row_sums);
     row_barrier<THREADS, true>();    // also: every thread is past its reads of the row before it may be overwritten
     r = s_row[0]; s = s_row[1];

@@ -34,39 +34,46 @@ __device__ __forceinline__ float2 expo2(float2 x, K2 k, float r) {
   return fma2(x, make_float2(k.lo, k.lo), fma2(x, make_float2(k.hi, k.hi), make_float2(-r, -r)));
 }
 
-// Partial sums (r, s), r an integer or -inf (nothing yet, or only -inf logits)
+// Partial sums (r, s), r an integer or -inf (nothing yet)
 __device__ __forceinline__ void soft_merge(float& r, float& s, float r2, float s2) {
   const float rn = fmaxf(r, r2);
   // (equal references add as they are: -inf - -inf would be NaN)
   s = (r == rn ? s : s * ex2(r - rn)) + (r2 == rn ? s2 : s2 * ex2(r2 - rn));
   r = rn;
 }
-// N (even, or 1) logits added to (r, s)
-template <int N> __device__ __forceinline__ void soft_add(float& r, float& s, const float* f, K2 k) {
+// N (even, or 1) logits added to (r, s).  The reference is an integer only as far as a float's integers go: at 2^20 the rounding of k x
+// to the reference's grid costs the exponent 2^-20, at 2^31 all of it (a mask of -1e10 would be 2^0 or 2^300, by chance).  So it is not taken from below
+// `lowest`: logits down there add nothing to what stands above, and rows without any other are the caller's to look at again.
+constexpr float SOFT_FAR = 0x1p20f;
+template <int N> __device__ __forceinline__ void soft_add(float& r, float& s, const float* f, K2 k, float lowest) {
   float top = f[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) top = fmaxf(top, f[i]);
-  const float rn = ceilf(expo(top, k, 0.f));
-  if (rn > r) { s = r == -INFINITY ? s : s * ex2(r - rn); r = rn; }
-  const float ref = r == -INFINITY ? 0.f : r;          // only -inf so far: 2^-inf = 0 is added, NaN stays NaN
+  const float rn = fmaxf(ceilf(expo(top, k, 0.f)), lowest);
+  if (rn > r) { s *= ex2(r - rn); r = rn; }            // (nothing yet: 0 * 2^-inf)
   if constexpr (N == 1) {
-    s += ex2(expo(f[0], k, ref));
+    s += ex2(expo(f[0], k, r));
   } else {
     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-      const float2 t = expo2(make_float2(f[i], f[i + 1]), k, ref);
+      const float2 t = expo2(make_float2(f[i], f[i + 1]), k, r);
       sum = add2(sum, make_float2(ex2(t.x), ex2(t.y)));
     }
     s += sum.x + sum.y;
   }
 }
 
-// log softmax of logit x in 64 bits; a row without any finite logit (s = 0) has no distribution: -inf; s < 0: see soft_row_extreme
+// k d for a difference of logits, which may be -inf
+__device__ __forceinline__ float expo_gap(float d, K2 k) { return fmaf(d, k.lo, d * k.hi); }
+
+// log softmax of logit x in 64 bits; a row without any finite logit (s = 0) has no distribution: -inf; s < 0: a row kept as its largest logit and
+// the sum over differences from it
 __device__ __forceinline__ double row_logp(float x, K2 k, float r, float s) {
+  const double k2 = (double)k.hi + (double)k.lo;
   if (s == 0.f) return -INFINITY;
-  if (s < 0.f) return x == r ? -log((double)-s) : -INFINITY;
-  return ((double)x * ((double)k.hi + (double)k.lo) - ((double)r + log2((double)s))) * 0.69314718055994531;
+  if (s < 0.f) return ((double)x - (double)r) * k2 * 0.69314718055994531 - log((double)-s);
+  return ((double)x * k2 - ((double)r + log2((double)s))) * 0.69314718055994531;
 }
 
 }  // namespace bb

@@ -320,8 +320,8 @@ int bb_token_logprob_bwd(const void* logits, int dtype, long long ld, const long
 
 /* The same from hidden states, through the vocabulary projection, without storing the logits: logits = hidden_states [rows,
  * hidden] * weight [vocab, hidden]^T (bf16, rows 16-byte aligned; fp32 accumulation, the logits are not rounded): one GEMM
- * whose epilogue keeps softmax sums, and a small kernel that joins them.  A logit so large that scale * log2(e) * logit
- * overflows counts as infinite here. */
+ * whose epilogue keeps softmax sums, and a small kernel that joins them.  A logit so large that scale * log2(e) * |logit|
+ * reaches 2^31 counts as infinite here. */
 typedef struct bb_head_desc {
   int rows, vocab, hidden;
   long long ld_hidden, ld_weight;

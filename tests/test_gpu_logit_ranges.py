@@ -1,5 +1,5 @@
-"""The row sums where the logits are far from a bell around zero: a low head of the vocabulary, low temperatures, against the
-definitions in 64 bits, for every number of threads that a row is given, the cluster per row and the ring.
+"""The row sums where the logits are far from a bell around zero: a low head of the vocabulary, low temperatures, large finite masks, against
+the definitions in 64 bits, for every number of threads that a row is given, the cluster per row and the ring.
 
 Tolerances.  A sum's reference may lie 2^64 below its terms, so arguments reach 64 in front of ex2: two roundings of 2^-19 each, 2.7e-6 of a
 term after the factor ln 2, and ex2 and the sum as elsewhere (1e-6): log-probabilities 4e-6 + 1e-6 of their magnitude.  A gradient has
@@ -152,3 +152,62 @@ def test_vocabularies_shorter_than_the_way_to_a_boundary(pt, dtype):
             want = -row * probs[:18]
             want[torch.arange(18, device="cuda"), t[:18]] += row[:, 0]
             near(grad, torch.nn.functional.pad(want, (0, cols - vocab)), rel, 1e-7)
+
+
+MASKS = [-1e5, -1e6, -1e9, -3e9, -1e10, -1e30, "half", "lowest"]
+
+
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("rows,vocab,dtype", ROWS)
+def test_large_finite_masks(pt, rows, vocab, dtype, mask):
+    """Finite values that stand for "not this one", in parts of a row and in all of it, and their opposites.  Rows that lie whole
+    beyond 2^20 in the exponent are summed over differences from their largest logit; below that the reference costs 2^-40 of the exponent."""
+    lowest = torch.finfo(dtype).min
+    value = {"half": lowest / 2, "lowest": lowest}.get(mask, mask)
+    value = torch.tensor(value).to(dtype).item()
+    temperature = 2.0 if MASKS.index(mask) % 2 else 1.0
+    gen = torch.Generator(device="cuda").manual_seed(41)
+    x = (torch.randn(rows, vocab, device="cuda", generator=gen) * 3).to(dtype)
+    t = torch.randint(vocab // 2, vocab, (rows,), device="cuda", generator=gen)
+    kind = torch.arange(rows, device="cuda") % 8
+    if rows < 8:
+        kind = (kind + MASKS.index(mask) * rows) % 8
+    column = torch.arange(vocab, device="cuda")
+    full = torch.full((), value, dtype=dtype, device="cuda")
+    where = torch.where
+    x = where((kind == 0)[:, None] & (column < vocab // 2), full, x)                   # the head
+    x = where((kind == 1)[:, None] & (column != t[:, None]), full, x)                  # all but the target
+    x = where((kind == 2)[:, None], full, x)                                           # all of it
+    x = where((kind == 3)[:, None] & (column == t[:, None]), full, x)                  # the target
+    x = where((kind == 4)[:, None] & (column // 64 % 2 == 0), full, x)                 # every other 64
+    x = where((kind == 5)[:, None], torch.nextafter(full, -full) if dtype == F32 else full * 0.75, x)     # all, the target one step lower
+    x = where((kind == 5)[:, None] & (column == t[:, None]), full, x)
+    x = where((kind == 6)[:, None], -full, x)                                          # all of it, far above zero
+    x = where((kind == 7)[:, None] & (column == t[:, None]), -full, x)                 # certain
+    lp, probs = reference(x, t, temperature)
+    near(pt.token_logprobs(x, t, temperature=temperature), lp, 1e-6, 4e-6)
+    g = torch.randn(rows, device="cuda", generator=gen)
+    leaf = x.requires_grad_(True)
+    pt.token_logprobs(leaf, t, temperature=temperature).backward(g)
+    want = probs.mul_(-g.double()[:, None] / temperature)
+    want[torch.arange(rows, device="cuda"), t] += g.double() / temperature
+    near(leaf.grad, want, 1.2e-5 if dtype == F32 else 2 ** -8, 1e-6 * g.abs().max().item() / temperature)
+    loss, _, grad = pt.PolicyLoss(vocab, temperature=temperature).loss_and_grad(leaf.detach(), (t.view(1, -1), None, g))
+    row = (-g.double() / rows / temperature)[:, None]
+    near(grad, want * (row / (g.double()[:, None] / temperature)), 1.2e-5 if dtype == F32 else 2 ** -8, 1e-6 * row.abs().max().item())
+    assert loss.item() == pytest.approx(-g.double().mean().item(), rel=1e-5, abs=1e-6)
+
+
+def test_projected_logits_beyond_the_range_count_as_infinite(pt):
+    """What a vocabulary projection's logits are from 2^31 in the exponent on: infinities of their sign, as the header states."""
+    h = torch.zeros(3, 64, device="cuda", dtype=BF16)
+    w = torch.zeros(300, 64, device="cuda", dtype=BF16)
+    w[:, 0], w[:, 1], w[7, 1], w[:, 2] = 1e6, 1e6, -1e6, torch.linspace(-1, 1, 300, device="cuda").to(BF16)
+    h[0, 0], h[1, 1], h[2, 2] = -1e6, -1e6, 1.0                  # all at -1e12; one at 1e12, the rest at -1e12; ordinary ones
+    t = torch.tensor([5, 7, 9], device="cuda")
+    hl = h.clone().requires_grad_(True)
+    got = pt.head_logprobs(hl, w, t)
+    assert got[0].item() == -math.inf and math.isnan(got[1].item())
+    near(got[2:].detach(), reference(h[2:].double() @ w.double().t(), t[2:], 1.0)[0], 1e-6, 2e-5)
+    got[0].backward()
+    assert torch.all(hl.grad[0] == 0)
