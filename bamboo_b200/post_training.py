@@ -89,6 +89,11 @@ def _inverse(temperature):
     return 1.0 / temperature
 
 
+def _overwritten(t):
+    """Tell autograd that a kernel wrote over ``t``: what kept it for a backward pass raises instead of reading something else."""
+    torch.autograd.graph.increment_version(t)
+
+
 def _wants_grad(t):
     return t.requires_grad and torch.is_grad_enabled()
 
@@ -120,6 +125,8 @@ class _TokenLogprobsFn(torch.autograd.Function):
         out = lg.detach() if inplace else torch.empty_like(lg)
         if rows:
             L.token_logprob_bwd(lg, tg, stats, _row_grad(grad, rows), out, vocab, scale, ignore_index)
+            if inplace:
+                _overwritten(lg)
         return out if shape is None else out.view(shape), None, None, None, None, None
 
 
@@ -321,21 +328,19 @@ class _LogitsLossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, loss_fn, labels, offsets):
         ctx.loss_fn, ctx.shape = loss_fn, logits.shape
-        loss, saved, ctx.args = loss_fn._forward(logits, labels, offsets)
-        ctx.save_for_backward(*saved)
-        return loss
+        return loss_fn._forward(ctx, logits, labels, offsets)
 
     @staticmethod
     def backward(ctx, grad):
-        out = ctx.loss_fn._backward(ctx.saved_tensors, ctx.args, grad.reshape(1).to(torch.float32).contiguous())
+        out = ctx.loss_fn._backward(ctx, grad.reshape(1).to(torch.float32).contiguous())
         return out.view(ctx.shape), None, None, None
 
 
 class PreferenceLoss:
     """Paired preference loss from logits: ``loss_fn(logits, (targets, ref_logps))`` for the last stage; reference-free with targets alone.
 
-    ``vocab``: real logit columns (the rest is padding).  The gradient overwrites the logits in the backward pass unless ``inplace`` is
-    off.  ``rewards`` keeps the last call's beta-scaled log-ratios per sequence (device)."""
+    ``vocab``: real logit columns (the rest is padding).  The gradient overwrites the logits in the backward pass (one, then) unless
+    ``inplace`` is off.  ``rewards`` keeps the last call's beta-scaled log-ratios per sequence (device)."""
 
     def __init__(self, vocab, *, beta=0.1, form="sigmoid", label_smoothing=0.0, average=False, temperature=1.0, ignore_index=-100,
                  inplace=True):
@@ -356,16 +361,24 @@ class PreferenceLoss:
         self.rewards = torch.empty(desc.sequences, dtype=torch.float32, device=lg.device)
         return L.preference_loss_logits(desc, lg, tg, vocab, ref, offsets, loss, self.rewards, dlogits, self.scale, grad_scale, stats, row_grad)
 
-    def _forward(self, logits, labels, offsets):
+    def _forward(self, ctx, logits, labels, offsets):
         lg, vocab, tg, *rest = self._prepare(logits, labels, offsets)
         lg, n = lg.detach(), tg.numel()
         stats, row_grad = torch.empty(n, 2, dtype=torch.float32, device=lg.device), torch.empty(n, dtype=torch.float32, device=lg.device)
-        return self._run(lg, vocab, tg, *rest, stats=stats, row_grad=row_grad), (lg, tg, stats, row_grad), ()
+        loss = self._run(lg, vocab, tg, *rest, stats=stats, row_grad=row_grad)
+        ctx.args = self.vocab, self.scale, self.ignore_index, self.inplace
+        ctx.save_for_backward(lg, tg, stats, row_grad)
+        return loss
 
-    def _backward(self, saved, args, grad):
-        lg, tg, stats, row_grad = saved
-        out = lg if self.inplace else torch.empty(lg.shape, dtype=lg.dtype, device=lg.device)
-        return L.token_logprob_bwd(lg, tg, stats, row_grad, out, self.vocab, self.scale, self.ignore_index, grad_scale_dev=grad)
+    @staticmethod
+    def _backward(ctx, grad):
+        lg, tg, stats, row_grad = ctx.saved_tensors
+        vocab, scale, ignore_index, inplace = ctx.args
+        out = lg if inplace else torch.empty(lg.shape, dtype=lg.dtype, device=lg.device)
+        L.token_logprob_bwd(lg, tg, stats, row_grad, out, vocab, scale, ignore_index, grad_scale_dev=grad)
+        if inplace:
+            _overwritten(lg)
+        return out
 
     def __call__(self, logits, labels, offsets=None):
         if _wants_grad(logits):
@@ -393,13 +406,23 @@ def _gradient_buffer(logits, out):
     return d, out
 
 
+def _policy_both(lg, vocab, desc, inputs, offsets, d, scale, grad_scale):
+    """(loss, stats) from logits, and their gradient into ``d``."""
+    old, advantages, ref, tg = inputs
+    loss = torch.empty((), dtype=torch.float32, device=lg.device)
+    stats = torch.empty(2, dtype=torch.float32, device=lg.device)
+    L.policy_loss_logits(desc, lg, tg, vocab, old, advantages, ref, offsets, loss, stats, None, d, scale, grad_scale)
+    return loss, stats
+
+
 class PolicyLoss:
     """Clipped policy loss from logits: ``loss_fn(logits, (targets, old_logps, advantages[, ref_logps]))`` for the last stage.
 
     The gradient of a row of logits needs that row alone, so loss and gradient come from one pass in the forward call, for an upstream
     gradient of ``grad_scale`` (the pipeline engine sets it to 1 / micro-batches); a different upstream gradient costs a pass
-    over the gradient in the backward call.  It overwrites the logits IN THE FORWARD call unless ``inplace`` is off.  ``stats`` keeps the
-    last call's mean KL and share of clipped tokens (device)."""
+    over the gradient in the backward call.  It overwrites the logits IN THE FORWARD call unless ``inplace`` is off; a second backward
+    pass over a kept graph is then an error, and makes the gradient again where it is off.  ``stats`` keeps the last call's mean KL and
+    share of clipped tokens (device)."""
 
     def __init__(self, vocab, *, clip_low=0.2, clip_high=0.2, kl_coef=0.0, reduction="token", temperature=1.0, ignore_index=-100,
                  inplace=True):
@@ -417,21 +440,39 @@ class PolicyLoss:
         return lg, vocab, desc, _policy_inputs(desc, old, advantages, ref, targets, lg.device), offsets
 
     def _both(self, lg, vocab, desc, inputs, offsets, d, grad_scale):
-        old, advantages, ref, tg = inputs
-        loss = torch.empty((), dtype=torch.float32, device=lg.device)
-        self.stats = torch.empty(2, dtype=torch.float32, device=lg.device)
-        L.policy_loss_logits(desc, lg, tg, vocab, old, advantages, ref, offsets, loss, self.stats, None, d, self.scale, grad_scale)
+        loss, self.stats = _policy_both(lg, vocab, desc, inputs, offsets, d, self.scale, grad_scale)
         return loss
 
-    def _forward(self, logits, labels, offsets):
-        lg, *rest = self._prepare(logits, labels, offsets)
+    def _forward(self, ctx, logits, labels, offsets):
+        lg, vocab, desc, inputs, offsets = self._prepare(logits, labels, offsets)
         lg = lg.detach()
+        ctx.args = vocab, desc, self.scale, self.grad_scale, self.inplace
         d = lg if self.inplace else torch.empty(lg.shape, dtype=lg.dtype, device=lg.device)
-        return self._both(lg, *rest, d, self.grad_scale), (d,), (self.grad_scale,)
+        loss = self._both(lg, vocab, desc, inputs, offsets, d, self.grad_scale)
+        if self.inplace:
+            _overwritten(lg)
+            ctx.save_for_backward(d)
+        else:
+            # (the first backward pass hands its gradient out; what further ones over a kept graph need to make theirs)
+            ctx.made = d
+            ctx.save_for_backward(lg, offsets, *inputs)
+        return loss
 
-    def _backward(self, saved, args, grad):
-        (d,) = saved
-        return L.rescale(d, grad, args[0])
+    @staticmethod
+    def _backward(ctx, grad):
+        vocab, desc, scale, made_for, inplace = ctx.args
+        if inplace:
+            (d,) = ctx.saved_tensors
+        else:
+            d, ctx.made = ctx.made, None
+            if d is None:
+                lg, offsets, *inputs = ctx.saved_tensors
+                d = torch.empty(lg.shape, dtype=lg.dtype, device=lg.device)
+                _policy_both(lg, vocab, desc, inputs, offsets, d, scale, made_for)
+        L.rescale(d, grad, made_for)
+        if inplace:
+            _overwritten(d)
+        return d
 
     def __call__(self, logits, labels, offsets=None):
         if _wants_grad(logits):
