@@ -339,7 +339,7 @@ class _LogitsLossFn(torch.autograd.Function):
 class PreferenceLoss:
     """Paired preference loss from logits: ``loss_fn(logits, (targets, ref_logps))`` for the last stage; reference-free with targets alone.
 
-    ``vocab``: real logit columns (the rest is padding).  The gradient overwrites the logits in the backward pass (one, then) unless
+    ``vocab``: real logit columns (the rest is padding; None: all).  The gradient overwrites the logits in the backward pass (one, then) unless
     ``inplace`` is off.  ``rewards`` keeps the last call's beta-scaled log-ratios per sequence (device)."""
 
     def __init__(self, vocab, *, beta=0.1, form="sigmoid", label_smoothing=0.0, average=False, temperature=1.0, ignore_index=-100,
@@ -366,7 +366,7 @@ class PreferenceLoss:
         lg, n = lg.detach(), tg.numel()
         stats, row_grad = torch.empty(n, 2, dtype=torch.float32, device=lg.device), torch.empty(n, dtype=torch.float32, device=lg.device)
         loss = self._run(lg, vocab, tg, *rest, stats=stats, row_grad=row_grad)
-        ctx.args = self.vocab, self.scale, self.ignore_index, self.inplace
+        ctx.args = vocab, self.scale, self.ignore_index, self.inplace
         ctx.save_for_backward(lg, tg, stats, row_grad)
         return loss
 

@@ -81,3 +81,26 @@ def test_graphs_that_are_not_overwritten_can_be_kept(pt):
         loss = call(leaf)
         one = torch.autograd.grad(loss, leaf, retain_graph=True)[0]
         assert torch.equal(torch.autograd.grad(loss, leaf)[0], one)
+
+
+def test_all_columns_are_the_vocabulary_where_none_is_given(pt):
+    x, t, adv = batch()
+    for make, labels in ((pt.PreferenceLoss, t), (pt.PolicyLoss, (t, None, adv))):
+        grads = []
+        for vocab in (300, None):
+            leaf = x.clone().requires_grad_(True)
+            make(vocab, inplace=False)(leaf, labels).backward()
+            grads.append(leaf.grad)
+        assert torch.equal(*grads)
+
+
+def test_a_backward_pass_is_that_of_its_own_call(pt):
+    """A loss whose vocabulary is changed for the next batch before the last one's backward pass."""
+    x, t, adv = batch()
+    t = t.clamp(max=199)
+    for make, labels in ((pt.PreferenceLoss, t), (pt.PolicyLoss, (t, None, adv))):
+        loss_fn = make(300, inplace=False)
+        want = torch.autograd.grad(loss_fn(leaf := x.clone().requires_grad_(True), labels), leaf)[0]
+        loss = loss_fn(leaf := x.clone().requires_grad_(True), labels)
+        loss_fn.vocab, loss_fn.scale = 200, 2.0
+        assert torch.equal(torch.autograd.grad(loss, leaf)[0], want)
