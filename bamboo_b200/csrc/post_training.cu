@@ -574,12 +574,13 @@ struct PolicyToken { float loss, kl, clipped, slope; };
 __device__ __forceinline__ PolicyInput policy_input(const PolicyParams& p, long long row) {
   return {p.old_logp ? p.old_logp[row] : 0.f, p.advantages[p.adv_div == 1 ? row : row / p.adv_div], p.ref ? p.ref[row] : 0.f};
 }
-__device__ __forceinline__ PolicyToken policy_token(const PolicyParams& p, const PolicyInput& in, double lp) {
+// `decided`: whether the token is clipped, where its gradient was made already (< 0: not yet)
+__device__ __forceinline__ PolicyToken policy_token(const PolicyParams& p, const PolicyInput& in, double lp, int decided = -1) {
   PolicyToken o;
   const float ratio = p.old_logp ? expf((float)(lp - (double)in.old)) : 1.f;
   // (an advantage of 0 has no part in the surrogate, whatever the ratio overflowed to)
   const float plain = in.adv == 0.f ? 0.f : ratio * in.adv, bounded = fminf(fmaxf(ratio, p.low), p.high) * in.adv;
-  const bool cut = bounded < plain;
+  const bool cut = decided < 0 ? bounded < plain : decided != 0;
   o.clipped = cut ? 1.f : 0.f;
   o.loss = cut ? -bounded : -plain;
   o.slope = cut ? 0.f : -plain;
@@ -593,17 +594,13 @@ __device__ __forceinline__ PolicyToken policy_token(const PolicyParams& p, const
   return o;
 }
 
-// The slope alone, from a row's softmax sums, in 32 bits: what the row kernels wait for between their halves (a log-probability in 64
-// bits takes a thousand cycles; 32 bits put 5e-7 on the ratio)
-__device__ __forceinline__ float policy_slope(const PolicyParams& p, const PolicyInput& in, float xt, K2 k, float r, float s) {
-  float lp;
-  if (s > 0.f) lp = (expo(xt, k, r) - log2f(s)) * 0.693147181f;
-  else lp = (float)row_logp(xt, k, r, s);
-  const float ratio = p.old_logp ? expf(lp - in.old) : 1.f;
-  const float plain = in.adv == 0.f ? 0.f : ratio * in.adv, bounded = fminf(fmaxf(ratio, p.low), p.high) * in.adv;
-  float slope = bounded < plain ? 0.f : -plain;
-  if (p.ref) slope -= p.kl_coef * expm1f(in.ref - lp);
-  return slope;
+// What the row kernels wait for between their halves: row_logp with the logarithm of the sum's mantissa in 32 bits (6e-8; one in 64 bits takes a
+// thousand cycles), everything else in 64, since a ratio at 32 bits of a log-probability of -150 is 1e-5 off
+__device__ __forceinline__ double row_logp_quick(float xt, K2 k, float r, float s) {
+  if (!(s > 0.f)) return row_logp(xt, k, r, s);
+  const int bits = __float_as_int(s), e = (bits >> 23) - 127;
+  const double log2_s = (double)e + (double)log2f(__int_as_float((bits & 0x7FFFFF) | 0x3F800000));
+  return ((double)xt * ((double)k.hi + (double)k.lo) - ((double)r + log2_s)) * 0.69314718055994531;
 }
 
 // Counted tokens of each of `gridDim.x` pieces of the targets (sequences, or equal pieces when weight is NULL) and, per sequence,
@@ -640,9 +637,10 @@ __device__ __forceinline__ float policy_weight(const PolicyParams& p, long long 
 }
 
 // Token by token: row_grad (from log-probabilities), or the log-probability (from rows: the softmax sums and the target's logit that a row
-// kernel left; a row with sums of 0 and a logit of 0 does not count).  The sums of a CTA's tokens - weighted loss, KL, clipped -
+// kernel left, and whether its gradient is that of a clipped token).  The sums of a CTA's tokens - weighted loss, KL, clipped -
 // meet in the CTA that finishes last, in the order of the CTAs: loss[0], and stats = mean KL and share of clipped among counted tokens.
-struct PolicyRow { float r, s, xt, counts; };
+struct PolicyRow { float r, s, xt; int kind; };
+constexpr int ROW_IGNORED = 0, ROW_COUNTS = 1, ROW_CLIPPED = 2;
 template <bool FROM_ROWS>
 __global__ void __launch_bounds__(256)
 policy_token_kernel(float* logp, const PolicyRow* row_sums, K2 k, const long long* targets, const PolicyParams p, long long tokens, long long ignore_index,
@@ -655,16 +653,18 @@ policy_token_kernel(float* logp, const PolicyRow* row_sums, K2 k, const long lon
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < tokens; i += (long long)gridDim.x * 256) {
     const float w = p.weight ? p.weight[i] : whole;
     double lp;
+    int decided = -1;
     if constexpr (FROM_ROWS) {
       const PolicyRow q = row_sums[i];
-      lp = q.counts == 0.f ? 0.0 : row_logp(q.xt, k, q.r, q.s);
+      lp = q.kind == ROW_IGNORED ? 0.0 : row_logp(q.xt, k, q.r, q.s);
       if (logp) logp[i] = (float)lp;
-      if (q.counts == 0.f) continue;
+      if (q.kind == ROW_IGNORED) continue;
+      decided = q.kind == ROW_CLIPPED;
     } else {
       if (targets[i] == ignore_index || w == 0.f) { row_grad[i] = 0.f; continue; }
       lp = (double)logp[i];
     }
-    const PolicyToken o = policy_token(p, policy_input(p, i), lp);
+    const PolicyToken o = policy_token(p, policy_input(p, i), lp, decided);
     if constexpr (!FROM_ROWS) row_grad[i] = o.slope * w;
     v[0] += (double)o.loss * w; v[1] += o.kl; v[2] += o.clipped;
   }
@@ -694,8 +694,9 @@ policy_token_kernel(float* logp, const PolicyRow* row_sums, K2 k, const long lon
 // What thread 0 does between the two halves of a row; the token's loss follows in policy_token_kernel
 __device__ __forceinline__ void policy_row_finish(const PolicyParams& p, const PolicyInput& in, int row, float xt, K2 k, float r, float s, float weight, float gscale,
                                                   float* s_row, PolicyRow* row_sums) {
-  s_row[0] = r; s_row[1] = s; s_row[2] = policy_slope(p, in, xt, k, r, s) * weight * gscale;
-  row_sums[row] = {r, s, xt, 1.f};
+  const PolicyToken o = policy_token(p, in, row_logp_quick(xt, k, r, s));
+  s_row[0] = r; s_row[1] = s; s_row[2] = o.slope * weight * gscale;
+  row_sums[row] = {r, s, xt, o.clipped != 0.f ? ROW_CLIPPED : ROW_COUNTS};
 }
 
 // One CTA per row of logits: log-probability, the token's loss and, because a row's gradient needs nothing of the other rows (the
@@ -729,7 +730,7 @@ policy_row_kernel(const T* logits, long long ld, const long long* targets, const
     r = mine[0]; s = mine[1]; g = mine[2];
   } else if (first) {
     if (!valid && t != ignore_index) atomicCAS(status, 0, BB_ERR_INVALID_ARG);
-    row_sums[row] = {0.f, 0.f, 0.f, 0.f};
+    row_sums[row] = {0.f, 0.f, 0.f, ROW_IGNORED};
   }
   grad_row<T, THREADS, ROW_LOADS>(x, dlogits + (size_t)row * ldd, V, cols, (int)t, g, k, r, s);
 }
@@ -833,7 +834,7 @@ policy_ring_kernel(const T* logits, long long ld, const long long* targets, cons
     const T* x = logits + (size_t)row * ld;
     T* d = dlogits + (size_t)row * ldd;
     if (t < 0) {
-      if (threadIdx.x == 0) row_sums[row] = {0.f, 0.f, 0.f, 0.f};
+      if (threadIdx.x == 0) row_sums[row] = {0.f, 0.f, 0.f, ROW_IGNORED};
       grad_row<T, THREADS, ROW_LOADS>(x, d, V, cols, 0, 0.f, k, 0.f, 0.f);
       turn_done();
       continue;
