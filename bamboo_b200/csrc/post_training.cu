@@ -574,6 +574,16 @@ struct PolicyToken { float loss, kl, clipped, slope; };
 __device__ __forceinline__ PolicyInput policy_input(const PolicyParams& p, long long row) {
   return {p.old_logp ? p.old_logp[row] : 0.f, p.advantages[p.adv_div == 1 ? row : row / p.adv_div], p.ref ? p.ref[row] : 0.f};
 }
+// e^gap - 1 - gap, e = e^gap - 1.  The difference of the two cancels near zero (at a gap of 1e-3 to 1e-4 of the result), so below a quarter it is the
+// series up to gap^8 / 8!, 4e-10 of the result short.
+__device__ __forceinline__ float kl_term(float gap, float e) {
+  if (!(fabsf(gap) < 0.25f)) return e - gap;
+  float c = 1.f / 8.f;
+#pragma unroll
+  for (int n = 7; n >= 3; --n) c = fmaf(c, gap, 1.f) * (1.f / (float)n);
+  return 0.5f * gap * gap * fmaf(c, gap, 1.f);
+}
+
 // `decided`: whether the token is clipped, where its gradient was made already (< 0: not yet)
 __device__ __forceinline__ PolicyToken policy_token(const PolicyParams& p, const PolicyInput& in, double lp, int decided = -1) {
   PolicyToken o;
@@ -586,8 +596,8 @@ __device__ __forceinline__ PolicyToken policy_token(const PolicyParams& p, const
   o.slope = cut ? 0.f : -plain;
   o.kl = 0.f;
   if (p.ref) {
-    const float gap = (float)((double)in.ref - lp), e = expm1f(gap);       // e^gap - gap - 1 without the cancellation
-    o.kl = e - gap;
+    const float gap = (float)((double)in.ref - lp), e = expm1f(gap);
+    o.kl = kl_term(gap, e);
     o.loss += p.kl_coef * o.kl;
     o.slope -= p.kl_coef * e;
   }

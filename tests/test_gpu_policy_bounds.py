@@ -1,4 +1,4 @@
-"""The clipped policy loss where a ratio stands at a bound."""
+"""The clipped policy loss where a ratio stands at a bound, and its KL term where policy and reference nearly agree."""
 import math
 
 import pytest
@@ -63,3 +63,15 @@ def test_slopes_of_improbable_tokens(pt, rows, vocab, dtype):
     got = grad.double().gather(1, t[:, None])[:, 0]
     err = (got - row * -torch.expm1(lp)).abs()
     assert (err <= 4e-6 / rows).all(), err.max().item() * rows
+
+
+@pytest.mark.parametrize("gap", [1e-4, 1e-3, 0.01, 0.1, 0.24, 0.26, 1.0, 3.0, -1e-4, -0.01, -0.24, -0.26, -1.0])
+def test_kl_of_a_policy_near_its_reference(pt, gap):
+    """e^gap - gap - 1 to 3e-6 of itself, from the gap between the 32-bit inputs (series below a quarter, the difference above)."""
+    gen = torch.Generator(device="cuda").manual_seed(63)
+    lp = -torch.rand(8, 40, device="cuda", generator=gen) * 3 - 1
+    ref = lp + gap
+    t = torch.zeros(8, 40, dtype=torch.int64, device="cuda")
+    _, stats = pt.policy_loss(lp, None, torch.zeros(8, 40, device="cuda"), t, ref_logps=ref, kl_coef=1.0)
+    g = ref.double() - lp.double()
+    assert stats[0].item() == pytest.approx((torch.expm1(g) - g).mean().item(), rel=3e-6)
