@@ -86,7 +86,7 @@ def _geometry(targets, offsets):
 def _inverse(temperature):
     if not temperature > 0:
         raise ValueError(f"temperature has to be positive, got {temperature}")
-    return 1.0 / temperature
+    return 1.0 / float(temperature)
 
 
 def _overwritten(t):
@@ -233,24 +233,33 @@ def head_logprobs(hidden, weight, targets, vocab=None, *, temperature=1.0, ignor
 
 
 # ----------------------------------------------------------------------------------- losses over log-probabilities
-# (descriptors are kept: making one costs the host as much as a launch)
+# (descriptors are kept: making one costs the host as much as a launch.  They are known by plain numbers: a constant that is a tensor may hold
+# another value at the next call)
 @functools.lru_cache(maxsize=256)
-def _preference_desc(tokens, sequences, beta, form, label_smoothing, average, ignore_index):
+def _kept_preference_desc(tokens, sequences, beta, form, label_smoothing, average, ignore_index):
     if form not in L.PREFERENCE_FORMS:
         raise ValueError(f"form {form!r}: one of {sorted(L.PREFERENCE_FORMS)}")
     if sequences % 2:
         raise ValueError(f"{sequences} sequences: preferences come in pairs (preferred, rejected)")
     return L.PreferenceDesc(tokens=tokens, sequences=sequences, form=L.PREFERENCE_FORMS[form], beta=beta, label_smoothing=label_smoothing,
-                            average=int(average), ignore_index=ignore_index)
+                            average=average, ignore_index=ignore_index)
+
+
+def _preference_desc(tokens, sequences, beta, form, label_smoothing, average, ignore_index):
+    return _kept_preference_desc(tokens, sequences, float(beta), form, float(label_smoothing), int(average), int(ignore_index))
 
 
 @functools.lru_cache(maxsize=256)
-def _policy_desc(tokens, sequences, advantages, clip_low, clip_high, kl_coef, reduction, ignore_index):
+def _kept_policy_desc(tokens, sequences, advantages, clip_low, clip_high, kl_coef, reduction, ignore_index):
     if reduction not in L.POLICY_REDUCTIONS:
         raise ValueError(f"reduction {reduction!r}: one of {sorted(L.POLICY_REDUCTIONS)}")
     per_sequence = advantages == sequences and tokens != sequences
     return L.PolicyDesc(tokens=tokens, sequences=sequences, reduction=L.POLICY_REDUCTIONS[reduction], clip_low=clip_low, clip_high=clip_high,
                         kl_coef=kl_coef, advantage_per_sequence=int(per_sequence), ignore_index=ignore_index)
+
+
+def _policy_desc(tokens, sequences, advantages, clip_low, clip_high, kl_coef, reduction, ignore_index):
+    return _kept_policy_desc(tokens, sequences, advantages, float(clip_low), float(clip_high), float(kl_coef), reduction, int(ignore_index))
 
 
 class _ScaledFn(torch.autograd.Function):
