@@ -515,9 +515,13 @@ def _dense(t):
 _dtype_of = operator.attrgetter("dtype")
 
 
+_needs_grad = operator.attrgetter("requires_grad")
+
+
 def _gradient_of(t):
-    """The gradient of a parameter (``main_grad`` of an arena's, else ``grad``), another tensor as it is."""
-    if isinstance(t, nn.Parameter):
+    """The gradient of a parameter (``main_grad`` of an arena's, else ``grad``), another tensor as it is.  A leaf that requires a gradient is a
+    parameter whatever its class; a gradient with a graph of its own (create_graph) is no leaf."""
+    if isinstance(t, nn.Parameter) or (t.requires_grad and t.is_leaf):
         main = getattr(t, "main_grad", None)
         return t.grad if main is None else main
     return t
@@ -527,7 +531,7 @@ def _gradients(tensors):
     """(tensors for the kernels, [(gradient, its copy without gaps)], bb_grad_tensor fields) of a list, empty tensors left out.  (The list is
     gone through property by property: 60 ns each.)"""
     grads = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    if set(map(type, grads)) != {torch.Tensor}:
+    if set(map(type, grads)) != {torch.Tensor} or any(map(_needs_grad, grads)):
         grads = [t for t in map(_gradient_of, grads) if t is not None]
     sizes = list(map(torch.Tensor.numel, grads))
     if not all(sizes):
@@ -562,7 +566,8 @@ def global_grad_norm(tensors):
 def clip_grad_norm_(tensors, max_norm):
     """Scale the gradients in place so that their global 2-norm is at most ``max_norm``; returns the norm before (fp32 scalar, device).
 
-    ``tensors``: parameters, or the gradients themselves (bf16 and fp32 may be mixed).  coefficient = min(1, max_norm / (norm + 1e-6));
+    ``tensors``: parameters (leaves that require a gradient), or the gradients themselves (bf16 and fp32 may be mixed).  coefficient = min(1,
+    max_norm / (norm + 1e-6));
     within the norm nothing is written."""
     if not max_norm > 0:
         raise ValueError(f"max_norm has to be positive, got {max_norm}")

@@ -23,4 +23,6 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2, mpu=None):
     ``deepspeed/runtime/utils.py:141-192``; ``bamboo_b200.post_training.clip_grad_norm_`` returns it without reading the device)."""
     if norm_type != 2 or mpu is not None:
         raise NotImplementedError("the 2-norm over one rank's gradients; a pipeline clips over its stages with `gradient_clipping`")
-    return float(post_training.clip_grad_norm_(parameters, max_norm))
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    grads = [p.grad if getattr(p, "main_grad", None) is None else p.main_grad for p in parameters]
+    return float(post_training.clip_grad_norm_([g for g in grads if g is not None], max_norm))

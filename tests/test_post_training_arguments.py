@@ -36,3 +36,34 @@ def test_constants_given_as_tensors_are_read_at_every_call(recorded):
         assert [seen[0][n] for n in ("kl_coef", "clip_low", "clip_high")] == [want] * 3
         assert [seen[1][n] for n in ("beta", "label_smoothing")] == [want] * 2
         assert (seen[2]["kl_coef"], seen[3]["beta"], seen[4]["scale"]) == (want, want, 1 / want)
+
+
+def test_which_tensor_is_clipped(recorded):
+    """A parameter of any class stands for its gradient, as in torch; a gradient for itself, one with a graph of its own included."""
+    pt, _ = recorded
+    parameter, leaf, arena, bare = torch.nn.Parameter(torch.ones(4)), torch.ones(4, requires_grad=True), torch.nn.Parameter(torch.ones(4)), torch.ones(4)
+    parameter.grad, leaf.grad, arena.main_grad = torch.full((4,), 2.0), torch.full((4,), 3.0), torch.full((4,), 4.0)
+    without = torch.ones(4, requires_grad=True)
+    made = torch.ones(4, requires_grad=True) * 5
+    assert not made.is_leaf
+    grads = pt._gradients([parameter, leaf, arena, bare, without, made])[0]
+    assert [g.data_ptr() for g in grads] == [t.data_ptr() for t in (parameter.grad, leaf.grad, arena.main_grad, bare, made)]
+    assert [g.data_ptr() for g in pt._gradients(leaf)[0]] == [leaf.grad.data_ptr()]
+    assert pt._gradients([without])[0] == []
+
+
+def test_the_facade_clips_what_parameters_have_as_gradient(recorded, monkeypatch):
+    import deepspeed.runtime.utils as ds_utils
+    pt, _ = recorded
+    seen = []
+    monkeypatch.setattr(pt, "clip_grad_norm_", lambda tensors, max_norm: seen.append(list(tensors)) or torch.zeros(()))
+    leaf, frozen, buffer = torch.ones(4, requires_grad=True), torch.nn.Parameter(torch.ones(4), requires_grad=False), torch.ones(4)
+    leaf.grad = torch.full((4,), 3.0)
+    arena = torch.nn.Parameter(torch.ones(4))
+    arena.main_grad = torch.full((4,), 4.0)
+    for given in ([leaf, frozen, buffer, arena], (p for p in (leaf, frozen, buffer, arena))):
+        seen.clear()
+        assert ds_utils.clip_grad_norm_(given, 1.0) == 0.0
+        assert [t.data_ptr() for t in seen[0]] == [leaf.grad.data_ptr(), arena.main_grad.data_ptr()]
+    ds_utils.clip_grad_norm_(leaf, 1.0)
+    assert [t.data_ptr() for t in seen[1]] == [leaf.grad.data_ptr()]
