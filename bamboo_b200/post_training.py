@@ -98,6 +98,31 @@ def _wants_grad(t):
     return t.requires_grad and torch.is_grad_enabled()
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    """A gradient as it is; an error where it is differentiated."""
+
+    @staticmethod
+    def forward(ctx, grad, anchor):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("the post-training functions are once_differentiable: their gradients have no gradient of their own")
+
+
+def _once_differentiable(backward):
+    """For a backward pass of kernels: under ``create_graph`` its gradients would count as constants.  (torch's decorator of that name lets them
+    where the incoming gradient is one.)"""
+    @functools.wraps(backward)
+    def once(ctx, grad):
+        if not torch.is_grad_enabled():
+            return backward(ctx, grad)
+        with torch.no_grad():
+            grads = backward(ctx, grad)
+        return tuple(g if g is None else _NoSecondDerivative.apply(g, torch.empty(0, requires_grad=True)) for g in grads)
+    return once
+
+
 # ----------------------------------------------------------------------------------- token log-probabilities
 def _logprobs(lg, rows, tg, vocab, scale, ignore_index, shape=None, keep=True):
     """(log-probabilities, softmax sums for the backward pass unless ``keep`` is off)"""
@@ -119,6 +144,7 @@ class _TokenLogprobsFn(torch.autograd.Function):
         return logp
 
     @staticmethod
+    @_once_differentiable
     def backward(ctx, grad):
         lg, tg = ctx.saved_tensors
         rows, vocab, scale, ignore_index, inplace, stats, shape = ctx.args
@@ -200,6 +226,7 @@ class _HeadLogprobsFn(torch.autograd.Function):
         return logp
 
     @staticmethod
+    @_once_differentiable
     def backward(ctx, grad):
         h, w, tg = ctx.saved_tensors
         desc, weight, shape, stats = ctx.args
@@ -271,6 +298,7 @@ class _ScaledFn(torch.autograd.Function):
         return loss.clone()
 
     @staticmethod
+    @_once_differentiable
     def backward(ctx, grad):
         (row_grad,) = ctx.saved_tensors
         return row_grad * grad, None, None
@@ -340,6 +368,7 @@ class _LogitsLossFn(torch.autograd.Function):
         return loss_fn._forward(ctx, logits, labels, offsets)
 
     @staticmethod
+    @_once_differentiable
     def backward(ctx, grad):
         out = ctx.loss_fn._backward(ctx, grad.reshape(1).to(torch.float32).contiguous())
         return out.view(ctx.shape), None, None, None
@@ -567,8 +596,7 @@ def clip_grad_norm_(tensors, max_norm):
     """Scale the gradients in place so that their global 2-norm is at most ``max_norm``; returns the norm before (fp32 scalar, device).
 
     ``tensors``: parameters (leaves that require a gradient), or the gradients themselves (bf16 and fp32 may be mixed).  coefficient = min(1,
-    max_norm / (norm + 1e-6));
-    within the norm nothing is written."""
+    max_norm / (norm + 1e-6)); within the norm nothing is written."""
     if not max_norm > 0:
         raise ValueError(f"max_norm has to be positive, got {max_norm}")
     grads, staged, fields = _gradients(tensors)

@@ -104,3 +104,17 @@ def test_a_backward_pass_is_that_of_its_own_call(pt):
         loss = loss_fn(leaf := x.clone().requires_grad_(True), labels)
         loss_fn.vocab, loss_fn.scale = 200, 2.0
         assert torch.equal(torch.autograd.grad(loss, leaf)[0], want)
+
+
+def test_second_derivatives_are_refused(pt):
+    """They are not implemented, and a gradient that autograd took for a constant would be a wrong one."""
+    x, t, adv = batch()
+    h, w = torch.randn(24, 64, device="cuda").bfloat16(), torch.randn(300, 64, device="cuda").bfloat16()
+    calls = ((lambda y: pt.token_logprobs(y, t).sum(), x), (lambda y: pt.PreferenceLoss(300, inplace=False)(y, t), x),
+             (lambda y: pt.PolicyLoss(300, inplace=False)(y, (t, None, adv)), x), (lambda y: pt.head_logprobs(y, w, t.view(-1)).sum(), h),
+             (lambda y: pt.preference_loss(y, None, t)[0], adv), (lambda y: pt.policy_loss(y, None, adv, t)[0], adv))
+    for call, value in calls:
+        leaf = value.clone().requires_grad_(True)
+        (grad,) = torch.autograd.grad(call(leaf * 1.0) * 2.0, leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            grad.float().square().sum().backward()
