@@ -1809,8 +1809,8 @@ extern "C" int bb_head_logprob_bwd(const bb_head_desc* d, const void* hidden_sta
   const bool whole = piece >= d->vocab;
   const PartsPlan parts = d_hidden && piece > 0 ? head_parts(d, piece) : PartsPlan{};
   if (!stats || ((uintptr_t)stats & 7) || !row_grad || !dlogits || (((uintptr_t)dlogits | (uintptr_t)d_hidden | (uintptr_t)d_hidden_parts | (uintptr_t)d_weight | (uintptr_t)d_weight_accum | (uintptr_t)counted_hidden) & 15) ||
-      piece <= 0 || piece % 8 || ldd % 8 || ldd < (whole ? d->vocab : piece) || (d_weight && d_weight_accum) || ((d_weight || d_weight_accum) && !counted_hidden) || (parts.parts > 0 && !d_hidden_parts)) {
-    bb_set_last_error_msg("bb_head_logprob_bwd: null or unaligned pointer, pieces that are no multiple of 8 or do not fit the buffer, no fp32 buffer for the parts of d_hidden, two weight gradients, or no counted_hidden for one");
+      d->hidden % 8 || piece <= 0 || piece % 8 || ldd % 8 || ldd < (whole ? d->vocab : piece) || (d_weight && d_weight_accum) || ((d_weight || d_weight_accum) && !counted_hidden) || (parts.parts > 0 && !d_hidden_parts)) {
+    bb_set_last_error_msg("bb_head_logprob_bwd: null or unaligned pointer, hidden no multiple of 8, pieces that are no multiple of 8 or do not fit the buffer, no fp32 buffer for the parts of d_hidden, two weight gradients, or no counted_hidden for one");
     return BB_ERR_INVALID_ARG;
   }
   if (int rc = bbhost::bind_context()) return rc;

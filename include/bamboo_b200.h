@@ -335,7 +335,7 @@ int bb_head_logprob_fwd(const bb_head_desc* d, const void* hidden_states, const 
  * of the logits into `dlogits` (bf16 [rows, ldd]) and its products into the input gradient d_hidden (bf16 [rows, hidden]; where
  * bb_head_logprob_bwd_parts says so, through that many fp32 buffers of its shape at d_hidden_parts, which are added up in one order) and the weight gradient: d_weight (bf16 [vocab, hidden]), or
  * d_weight_accum (fp32, +=), through a copy of the rows that count (counted_hidden, bf16 [rows, hidden rounded up to 64]).  A gradient that is
- * not wanted is NULL. */
+ * not wanted is NULL.  hidden has to be a multiple of 8. */
 int bb_head_logprob_bwd_parts(const bb_head_desc* d, int piece);
 int bb_head_logprob_bwd(const bb_head_desc* d, const void* hidden_states, const void* weight, const long long* targets,
                         const float* stats, const float* row_grad, void* d_hidden, float* d_hidden_parts, void* d_weight,

@@ -67,3 +67,13 @@ def test_the_facade_clips_what_parameters_have_as_gradient(recorded, monkeypatch
         assert [t.data_ptr() for t in seen[0]] == [leaf.grad.data_ptr(), arena.main_grad.data_ptr()]
     ds_utils.clip_grad_norm_(leaf, 1.0)
     assert [t.data_ptr() for t in seen[1]] == [leaf.grad.data_ptr()]
+
+
+def test_backward_pass_of_the_projection_refuses_rows_that_are_no_whole_vectors():
+    """d_hidden, its fp32 parts and the copy of the hidden states have rows of ``hidden`` values, which are stored 16 bytes at a time."""
+    from bamboo_b200 import lib
+    handle, at = lib.load(), 1 << 20
+    for hidden, weight_only in ((60, False), (12, False), (60, True), (1, False)):
+        desc = lib.HeadDesc(rows=4, vocab=100, hidden=hidden, ld_hidden=64, ld_weight=64, scale=1.0, ignore_index=-100)
+        rc = handle.bb_head_logprob_bwd(ctypes.byref(desc), at, at, at, at, at, None if weight_only else at, at, at, None, at, 104, at, 104, None)
+        assert rc == -1 and b"bb_head_logprob_bwd" in handle.bb_last_error(), (hidden, rc, handle.bb_last_error())
