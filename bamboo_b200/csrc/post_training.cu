@@ -106,6 +106,13 @@ template <int THREADS, bool FED = false> __device__ __forceinline__ void row_bar
   if constexpr (FED) asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
   else __syncthreads();
 }
+// The same for a block that is fed; whether `v` holds in any of those threads, the same answer for all of them
+template <int THREADS> __device__ __forceinline__ bool row_barrier_any(bool v) {
+  uint32_t any;
+  asm volatile("{\n\t.reg .pred P, Q;\n\tsetp.ne.u32 P, %1, 0;\n\tbar.red.or.pred Q, 1, %2, P;\n\tselp.u32 %0, 1, 0, Q;\n\t}"
+               : "=r"(any) : "r"((uint32_t)v), "n"(THREADS) : "memory");
+  return any != 0;
+}
 // (r, s) of the block's threads merged; the first warp gets the result
 template <int THREADS, bool FED = false> __device__ __forceinline__ void soft_block(float& r, float& s, float2* smem /*[THREADS/32]*/) {
   soft_warp(r, s);
@@ -767,12 +774,12 @@ policy_ring_kernel(const T* logits, long long ld, const long long* targets, cons
   __shared__ float s_row[3];
   __shared__ PolicyTurn turns[TURNS];
   __shared__ uint64_t turn_full[TURNS], turn_empty[TURNS];
-  __shared__ int s_abort, s_dead;
+  __shared__ int s_abort;
   __shared__ uint64_t full[RING_STAGES], empty[RING_STAGES];
   volatile int* abort_flag = &s_abort;
   const int warp = bb::warp_index(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    s_abort = s_dead = 0;
+    s_abort = 0;
     for (int j = 0; j < stages; ++j) { bb::mbar_init(&full[j], 1); bb::mbar_init(&empty[j], THREADS / 32); }
     for (int j = 0; j < TURNS; ++j) { bb::mbar_init(&turn_full[j], 1); bb::mbar_init(&turn_empty[j], THREADS / 32); }
     bb::fence_barrier_init();
@@ -837,10 +844,9 @@ policy_ring_kernel(const T* logits, long long ld, const long long* targets, cons
       if (lane == 0) bb::mbar_arrive(&turn_empty[at]);
     };
     const int row = turn.row, t = turn.t;
-    // a wait that ran out in one warp ends the loop for all of them here, where their barriers match
-    if (!alive) s_dead = 1;
-    row_barrier<THREADS, true>();
-    if (s_dead || row < 0) break;
+    // a wait that ran out in one warp ends the loop for all of them here, where their barriers match; the barrier itself says so (a flag beside it
+    // could be set for the next row, where this one does not count, before a slow warp has read it for this one)
+    if (row_barrier_any<THREADS>(!alive) || row < 0) break;
     const T* x = logits + (size_t)row * ld;
     T* d = dlogits + (size_t)row * ldd;
     if (t < 0) {
