@@ -285,8 +285,13 @@ def _kept_policy_desc(tokens, sequences, advantages, clip_low, clip_high, kl_coe
                         kl_coef=kl_coef, advantage_per_sequence=int(per_sequence), ignore_index=ignore_index)
 
 
-def _policy_desc(tokens, sequences, advantages, clip_low, clip_high, kl_coef, reduction, ignore_index):
-    return _kept_policy_desc(tokens, sequences, advantages, float(clip_low), float(clip_high), float(kl_coef), reduction, int(ignore_index))
+def _policy_desc(tokens, sequences, offsets, advantages, clip_low, clip_high, kl_coef, reduction, ignore_index):
+    count = advantages.numel()
+    if count != tokens and (count != sequences or offsets is not None):
+        how = ("one per token or per sequence" if offsets is None else
+               "one per token here (repeat_interleave those of the sequences); one per sequence goes with sequences of one length, as 2-D targets")
+        raise ValueError(f"advantages: {count} values for {tokens} tokens in {sequences} sequences; {how}")
+    return _kept_policy_desc(tokens, sequences, count, float(clip_low), float(clip_high), float(kl_coef), reduction, int(ignore_index))
 
 
 class _ScaledFn(torch.autograd.Function):
@@ -341,7 +346,7 @@ def policy_loss(logps, old_logps, advantages, targets, *, ref_logps=None, clip_l
     sequences, offsets = _geometry(targets, offsets)
     lp = _flat(logps, "logps", targets.numel(), torch.float32, targets.device)
     _on_current(lp, "logps")
-    desc = _policy_desc(lp.numel(), sequences, advantages.numel(), clip_low, clip_high, kl_coef, reduction, ignore_index)
+    desc = _policy_desc(lp.numel(), sequences, offsets, advantages, clip_low, clip_high, kl_coef, reduction, ignore_index)
     loss, stats = torch.empty((), dtype=torch.float32, device=lp.device), torch.empty(2, dtype=torch.float32, device=lp.device)
     row_grad = torch.empty_like(lp)
     L.policy_loss(desc, lp, *_policy_inputs(desc, old_logps, advantages, ref_logps, targets, lp.device), offsets, loss, stats, row_grad)
@@ -474,7 +479,7 @@ class PolicyLoss:
         ref = labels[3] if len(labels) > 3 else None
         lg, rows, vocab = _rows(logits, self.vocab)
         sequences, offsets = _geometry(targets, offsets)
-        desc = _policy_desc(rows, sequences, advantages.numel(), *self.form, self.ignore_index)
+        desc = _policy_desc(rows, sequences, offsets, advantages, *self.form, self.ignore_index)
         return lg, vocab, desc, _policy_inputs(desc, old, advantages, ref, targets, lg.device), offsets
 
     def _both(self, lg, vocab, desc, inputs, offsets, d, grad_scale):

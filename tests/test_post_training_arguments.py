@@ -77,3 +77,19 @@ def test_backward_pass_of_the_projection_refuses_rows_that_are_no_whole_vectors(
         desc = lib.HeadDesc(rows=4, vocab=100, hidden=hidden, ld_hidden=64, ld_weight=64, scale=1.0, ignore_index=-100)
         rc = handle.bb_head_logprob_bwd(ctypes.byref(desc), at, at, at, at, at, None if weight_only else at, at, at, None, at, 104, at, 104, None)
         assert rc == -1 and b"bb_head_logprob_bwd" in handle.bb_last_error(), (hidden, rc, handle.bb_last_error())
+
+
+def test_advantages_of_the_wrong_number_say_what_is_expected(recorded):
+    pt, seen = recorded
+    lp, t, offsets = torch.zeros(8), torch.zeros(8, dtype=torch.int64), torch.tensor([0, 3, 8])
+    for call in (lambda a: pt.policy_loss(lp, None, a, t, offsets=offsets), lambda a: pt.PolicyLoss(4)(torch.zeros(8, 4), (t, None, a), offsets),
+                 lambda a: pt.PolicyLoss(4).loss_and_grad(torch.zeros(8, 4), (t, None, a), offsets=offsets)):
+        for count in (2, 5):
+            with pytest.raises(ValueError, match=f"{count} values.*one per token.*repeat_interleave"):
+                call(torch.zeros(count))
+    with pytest.raises(ValueError, match="3 values.*8 tokens in 2 sequences"):
+        pt.policy_loss(lp.view(2, 4), None, torch.zeros(3), t.view(2, 4))
+    assert not seen
+    pt.policy_loss(lp, None, torch.zeros(8), t, offsets=offsets)                                      # per token
+    pt.policy_loss(lp.view(2, 4), None, torch.zeros(2), t.view(2, 4))                                 # per sequence, of one length
+    assert [d["advantage_per_sequence"] for d in seen] == [0, 1]
