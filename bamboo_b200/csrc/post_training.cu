@@ -981,6 +981,23 @@ template <typename T> __device__ __forceinline__ float sumsq_chunk(const uint4& 
   for (int i = 0; i < VEC; i += 2) sum = bb::fma2(make_float2(f[i], f[i + 1]), make_float2(f[i], f[i + 1]), sum);
   return sum.x + sum.y;
 }
+// A thread's share again with its squares in 64 bits, for values from 1.8e19 on (and infinities and NaN, which stay)
+template <typename T> __device__ __noinline__ double sumsq_share_wide(const T* x, int n) {
+  const Span<T> sp(x, n);
+  constexpr int VEC = Elem<T>::VEC;
+  const uint4* v = reinterpret_cast<const uint4*>(x + sp.lead);
+  double sum = 0.0;
+  for (int c = threadIdx.x; c < sp.nvec; c += NORM_THREADS) {
+    float f[VEC];
+    Elem<T>::unpack(v[c], f);
+    for (int i = 0; i < VEC; ++i) sum += (double)f[i] * (double)f[i];
+  }
+  for (int j = threadIdx.x; j < sp.lead + n - sp.tail; j += NORM_THREADS) {
+    const double f = (double)Elem<T>::get(x + (j < sp.lead ? j : sp.tail + j - sp.lead));
+    sum += f * f;
+  }
+  return sum;
+}
 // (a chunk's squares in 32 bits, everything above in 64)
 template <typename T> __device__ __forceinline__ double sumsq_piece(const T* x, int n) {
   constexpr int U = NORM_LOADS;
@@ -1000,7 +1017,7 @@ template <typename T> __device__ __forceinline__ double sumsq_piece(const T* x, 
     const float f = Elem<T>::get(x + (j < sp.lead ? j : sp.tail + j - sp.lead));
     sum += (double)(f * f);
   }
-  return sum;
+  return isfinite(sum) ? sum : sumsq_share_wide(x, n);
 }
 
 // What a squared norm means for the gradients: norm = pre_scale * sqrt(sum of squares), coefficient = min(1, max_norm / (norm + 1e-6)), NaN

@@ -403,7 +403,8 @@ int bb_rescale_grad(void* grad, int dtype, long long ld, long long rows, int col
  * over, e.g. other pipeline stages - or, with sumsq NULL, make it first from their own gradients: norm = grad_scale *
  * sqrt(sumsq), coefficient = min(1, max_norm / (norm + 1e-6)); the norm before clipping goes to `norm` (device).  bb_grad_clip
  * scales the tensors in place (not at all within the norm); bb_adam_step_clipped is an Adam step on coefficient * grad_scale
- * * grad.  A norm that is NaN makes everything NaN.  Squares are taken in 32 bits: values up to 1e19. */
+ * * grad.  A norm that is NaN makes everything NaN.  Squares are taken in 32 bits where that holds them: values below 1e-19 lose
+ * bits, and below 3e-23 they count as 0. */
 typedef struct bb_grad_tensor { void* data; long long numel; int dtype; } bb_grad_tensor;
 long long bb_grad_norm_workspace_bytes(void);
 int bb_grad_sumsq(const bb_grad_tensor* tensors, int count, void* workspace, long long workspace_bytes, void* stream);
