@@ -24,6 +24,7 @@ What is different underneath:
 """
 import collections
 import contextlib
+import itertools
 import json
 import os
 import signal
@@ -46,6 +47,7 @@ from .post_training import PolicyLoss
 
 should_stop = False
 _live_stores = []
+_engines = itertools.count()          # engines of this process in the order of their making, the same on every rank
 
 
 def sig_handler(signum, frame):
@@ -275,7 +277,11 @@ class PipelineEngine:
         if isinstance(self.loss_model, PolicyLoss):
             # it makes its gradient with its value: every micro-batch contributes loss / GAS
             self.loss_model.grad_scale = 1.0 / self.micro_batches
-        self._global_grad_norm, self._clip_epoch = None, 0
+        # what `gradient_clipping` publishes is known by engine, loaded checkpoints and step: engines of one job share a store, and their steps
+        # have the same numbers (an engine that is formed anew with its cluster keeps its place)
+        if not hasattr(self, "_engine_index"):
+            self._engine_index = next(_engines)
+        self._global_grad_norm, self._clip_epoch = None, self._engine_index * 1_000_000
         self._compute_loss = True
         self._losses: Dict[Tuple[int, int], torch.Tensor] = {}
         self.timers = collections.defaultdict(float)
