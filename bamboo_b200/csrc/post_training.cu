@@ -247,14 +247,12 @@ template <typename T> __device__ __forceinline__ void grad_chunk(uint4* d, const
   *d = Elem<T>::pack(f);
 }
 // What follows the chunks [0, whole): the target's entry (xt its logit, read before d, which may be x, was written; by the thread
-// that wrote its chunk), the chunk that the padding begins in, the padding, and the elements around the 16-byte boundaries.  The chunks here are
-// those of all columns: a vocabulary that ends before the first boundary has none, while the padding behind it goes on past it.
+// that wrote its chunk), the chunk that the padding begins in, the padding, and the elements around the 16-byte boundaries
 template <typename T, int THREADS>
-__device__ __forceinline__ void grad_rest(const T* x, float xt, T* d, int whole, int V, int cols, int t, float g, K2 k, float s, const GradRow& w) {
+__device__ __forceinline__ void grad_rest(const T* x, float xt, T* d, int lead, int whole, int V, int cols, int t, float g, K2 k, float s, const GradRow& w) {
   constexpr int VEC = Elem<T>::VEC;
-  const Span<T> sp(d, cols);
-  if (t >= sp.lead) {
-    const int tc = (t - sp.lead) / VEC;
+  if (t >= lead) {
+    const int tc = (t - lead) / VEC;
     if (tc < whole && tc % THREADS == row_thread<THREADS>()) Elem<T>::put(d + t, grad_target(g, xt, k, w.r, s));
   }
   auto one = [&](int j) {
@@ -262,12 +260,29 @@ __device__ __forceinline__ void grad_rest(const T* x, float xt, T* d, int whole,
     if (j < V) { const float f = Elem<T>::get(x + j); v = j == t ? grad_target(g, f, k, w.r, s) : grad_entry(w, f); }
     Elem<T>::put(d + j, v);
   };
-  for (int c = whole + row_thread<THREADS>(); c < sp.nvec; c += THREADS) {
-    const int j0 = sp.lead + c * VEC;
+  const int nvec = (cols - lead) / VEC, tail = lead + nvec * VEC;
+  for (int c = whole + row_thread<THREADS>(); c < nvec; c += THREADS) {
+    const int j0 = lead + c * VEC;
     if (j0 >= V) *reinterpret_cast<uint4*>(d + j0) = make_uint4(0, 0, 0, 0);
     else for (int i = 0; i < VEC; ++i) one(j0 + i);
   }
-  for (int j = row_thread<THREADS>(); j < sp.lead + cols - sp.tail; j += THREADS) one(j < sp.lead ? j : sp.tail + j - sp.lead);
+  for (int j = row_thread<THREADS>(); j < lead + cols - tail; j += THREADS) one(j < lead ? j : tail + j - lead);
+}
+
+// Rows element by element: those kept by differences, gradients of another alignment than the logits', and vocabularies of less than a vector, which
+// may end before the first boundary
+template <typename T, int THREADS>
+__device__ __noinline__ void grad_row_slow(const T* x, T* d, int V, int cols, int t, float g, K2 k, float r, float s) {
+  const GradRow w = grad_factors(g, k, s < 0.f ? 0.f : r, s);
+  for (int j = row_thread<THREADS>(); j < cols; j += THREADS) {
+    float v = 0.f;
+    if (j < V) {
+      const float f = Elem<T>::get(x + j);
+      if (s < 0.f) v = fmaf(g / s, ex2(bb::expo_gap(f - r, k)), j == t ? g : 0.f);
+      else v = j == t ? grad_target(g, f, k, r, s) : grad_entry(w, f);
+    }
+    Elem<T>::put(d + j, v);
+  }
 }
 
 // d[j] = g * ([j == t] - softmax_j) for j < V, 0 in [V, cols); zeros throughout when g == 0 (nothing is read then).  FAR: the row comes
@@ -284,19 +299,11 @@ __device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int 
     for (int j = tid; j < sp.lead + cols - sp.tail; j += THREADS) Elem<T>::put(d + (j < sp.lead ? j : sp.tail + j - sp.lead), 0.f);
     return;
   }
-  const GradRow w = grad_factors(g, k, s < 0.f ? 0.f : r, s);
-  if (s < 0.f || (((uintptr_t)x ^ (uintptr_t)d) & 15) != 0) {      // element by element
-    for (int j = tid; j < cols; j += THREADS) {
-      float v = 0.f;
-      if (j < V) {
-        const float f = Elem<T>::get(x + j);
-        if (s < 0.f) v = fmaf(g / s, ex2(bb::expo_gap(f - r, k)), j == t ? g : 0.f);
-        else v = j == t ? grad_target(g, f, k, r, s) : grad_entry(w, f);
-      }
-      Elem<T>::put(d + j, v);
-    }
+  if (s < 0.f || V < VEC || (((uintptr_t)x ^ (uintptr_t)d) & 15) != 0) {
+    grad_row_slow<T, THREADS>(x, d, V, cols, t, g, k, r, s);
     return;
   }
+  const GradRow w = grad_factors(g, k, r, s);
   const Span<T> sp(x, V);
   const uint4* xv = reinterpret_cast<const uint4*>(x + sp.lead);
   uint4* dv = reinterpret_cast<uint4*>(d + sp.lead);
@@ -319,7 +326,7 @@ __device__ __forceinline__ void grad_row(const T* x, T* d, int V, int cols, int 
   } else {
     for (; c < whole; c += THREADS) grad_chunk<T>(dv + c, xv[c], w);
   }
-  grad_rest<T, THREADS>(x, xt, d, whole, V, cols, t, g, k, s, w);
+  grad_rest<T, THREADS>(x, xt, d, sp.lead, whole, V, cols, t, g, k, s, w);
 }
 
 // ------------------------------------------------------------------ sums of a block
@@ -719,8 +726,10 @@ __device__ __forceinline__ void policy_row_finish(const PolicyParams& p, const P
 // One CTA per row of logits: log-probability, the token's loss and, because a row's gradient needs nothing of the other rows (the
 // weights follow from the targets), that gradient too.  For rows that are short, or too long for policy_ring_kernel: the second half reads
 // the row again, from L1 or L2.
+// Registers for 1536 threads of an SM where the compiler would take more (16384 bf16 rows of 8203: 118 us with 48, 116 with 40)
+template <typename T, int THREADS> constexpr int POLICY_BLOCKS = sizeof(T) == 2 && THREADS >= 64 && THREADS <= 256 ? 1536 / THREADS : 0;
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(BLOCK<THREADS>)
+__global__ void __launch_bounds__(BLOCK<THREADS>, POLICY_BLOCKS<T, THREADS>)
 policy_row_kernel(const T* logits, long long ld, const long long* targets, const PolicyParams p, K2 k, float gscale,
                   T* dlogits, long long ldd, int rows, int V, int cols, long long ignore_index, PolicyRow* row_sums, int* status) {
   __shared__ float2 smem[BLOCK<THREADS> / 32];
@@ -909,7 +918,7 @@ policy_ring_kernel(const T* logits, long long ld, const long long* targets, cons
       if (lane == 0) bb::mbar_arrive(&empty[j]);
     }
     if (plain) grad_row<T, THREADS, ROW_LOADS>(x, d, V, cols, t, g, k, r, s);
-    else grad_rest<T, THREADS>(x, xt, d, whole, V, cols, t, g, k, s, gw);
+    else grad_rest<T, THREADS>(x, xt, d, sp.lead, whole, V, cols, t, g, k, s, gw);
     turn_done();
     phase ^= 1;
   }
