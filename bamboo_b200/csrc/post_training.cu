@@ -582,6 +582,7 @@ struct PolicyParams {
   long long adv_div;
   float low, high, kl_coef;     // ratio bounds 1 - clip_low, 1 + clip_high
 };
+constexpr float LN2_HI = 0.693147181f, LN2_LO = -1.9046542e-9f;        // ln 2 in two floats
 struct PolicyInput { float old, adv, ref; };
 struct PolicyToken { float loss, kl, clipped, slope; };
 
@@ -618,13 +619,31 @@ __device__ __forceinline__ PolicyToken policy_token(const PolicyParams& p, const
   return o;
 }
 
-// What the row kernels wait for between their halves: row_logp with the logarithm of the sum's mantissa in 32 bits (6e-8; one in 64 bits takes a
-// thousand cycles), everything else in 64, since a ratio at 32 bits of a log-probability of -150 is 1e-5 off
-__device__ __forceinline__ double row_logp_quick(float xt, K2 k, float r, float s) {
-  if (!(s > 0.f)) return row_logp(xt, k, r, s);
-  const int bits = __float_as_int(s), e = (bits >> 23) - 127;
-  const double log2_s = (double)e + (double)log2f(__int_as_float((bits & 0x7FFFFF) | 0x3F800000));
-  return ((double)xt * ((double)k.hi + (double)k.lo) - ((double)r + log2_s)) * 0.69314718055994531;
+// What the row kernels wait for between their halves: the token's slope, and whether it is clipped, from the row's sums.  The gaps between the
+// log-probability and those of the other policies are differences of numbers of any size whose rounding to 32 bits would show (1e-5 at -150), so they
+// are kept in two floats each (k x - r - log2 s exactly but for the logarithm of the sum's mantissa, 6e-8): 64 bits cost 3 to 5 % of rows of 4 to 30 KB.
+struct PolicySlope { float slope; bool cut; };
+__device__ __forceinline__ PolicySlope policy_slope(const PolicyParams& p, const PolicyInput& in, float xt, K2 k, float r, float s) {
+  float to_old, to_ref;
+  const float a = __fmul_rn(xt, k.hi);                       // (a product that no sum below may take up)
+  if (s > 0.f && fabsf(a) < INFINITY) {
+    const int bits = __float_as_int(s);
+    const float log2_m = log2f(__int_as_float((bits & 0x7FFFFF) | 0x3F800000)), whole = r + (float)((bits >> 23) - 127);
+    const float b = a - whole, v = b - a, b_rest = (a - (b - v)) - (whole + v);      // (the sum's rounding, by Knuth)
+    const float rest = (b_rest - log2_m) + fmaf(xt, k.lo, fmaf(xt, k.hi, -a));
+    const float lp = __fmul_rn(b, LN2_HI), lp_rest = fmaf(rest, LN2_HI, fmaf(b, LN2_LO, fmaf(b, LN2_HI, -lp)));
+    to_old = (lp - in.old) + lp_rest;
+    to_ref = (in.ref - lp) - lp_rest;
+  } else {
+    const double lp = row_logp(xt, k, r, s);
+    to_old = (float)(lp - (double)in.old);
+    to_ref = (float)((double)in.ref - lp);
+  }
+  const float ratio = p.old_logp ? expf(to_old) : 1.f;
+  const float plain = in.adv == 0.f ? 0.f : ratio * in.adv, bounded = fminf(fmaxf(ratio, p.low), p.high) * in.adv;
+  PolicySlope o = {bounded < plain ? 0.f : -plain, bounded < plain};
+  if (p.ref) o.slope -= p.kl_coef * expm1f(to_ref);
+  return o;
 }
 
 // Counted tokens of each of `gridDim.x` pieces of the targets (sequences, or equal pieces when weight is NULL) and, per sequence,
@@ -718,9 +737,9 @@ policy_token_kernel(float* logp, const PolicyRow* row_sums, K2 k, const long lon
 // What thread 0 does between the two halves of a row; the token's loss follows in policy_token_kernel
 __device__ __forceinline__ void policy_row_finish(const PolicyParams& p, const PolicyInput& in, int row, float xt, K2 k, float r, float s, float weight, float gscale,
                                                   float* s_row, PolicyRow* row_sums) {
-  const PolicyToken o = policy_token(p, in, row_logp_quick(xt, k, r, s));
+  const PolicySlope o = policy_slope(p, in, xt, k, r, s);
   s_row[0] = r; s_row[1] = s; s_row[2] = o.slope * weight * gscale;
-  row_sums[row] = {r, s, xt, o.clipped != 0.f ? ROW_CLIPPED : ROW_COUNTS};
+  row_sums[row] = {r, s, xt, o.cut ? ROW_CLIPPED : ROW_COUNTS};
 }
 
 // One CTA per row of logits: log-probability, the token's loss and, because a row's gradient needs nothing of the other rows (the

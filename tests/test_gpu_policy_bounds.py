@@ -75,3 +75,30 @@ def test_kl_of_a_policy_near_its_reference(pt, gap):
     _, stats = pt.policy_loss(lp, None, torch.zeros(8, 40, device="cuda"), t, ref_logps=ref, kl_coef=1.0)
     g = ref.double() - lp.double()
     assert stats[0].item() == pytest.approx((torch.expm1(g) - g).mean().item(), rel=3e-6)
+
+
+@pytest.mark.parametrize("mask", ["-inf", "lowest", "-1e30", "-1e5"])
+@pytest.mark.parametrize("rows,vocab,dtype", ROWS)
+def test_tokens_that_the_policy_rules_out(pt, rows, vocab, dtype, mask):
+    """Targets that are masked: a ratio of 0, the clipped surrogate where the advantage is negative, and no gradient."""
+    gen = torch.Generator(device="cuda").manual_seed(64)
+    x = (torch.randn(rows, vocab, device="cuda", generator=gen) * 3).to(dtype)
+    t = torch.randint(0, vocab, (rows,), device="cuda", generator=gen)
+    masked = torch.rand(rows, device="cuda", generator=gen) < 0.5
+    masked[:2] = torch.tensor([True, False])
+    value = {"-inf": -math.inf, "lowest": torch.finfo(dtype).min}.get(mask) or float(mask)
+    x[masked, t[masked]] = value
+    lp, probs = torch.log_softmax(x.double(), 1).gather(1, t[:, None])[:, 0], torch.softmax(x.double(), 1)
+    old = torch.where(masked, torch.full_like(lp, -5.0), lp + 0.1).float()
+    adv = torch.randn(rows, device="cuda", generator=gen)
+    ratio, a = (lp - old.double()).exp(), adv.double()
+    want = -torch.minimum(ratio * a, ratio.clamp(0.8, 1.2) * a)
+    loss, stats, grad = pt.PolicyLoss(vocab).loss_and_grad(x, (t.view(1, -1), old, adv))
+    assert loss.item() == pytest.approx(want.mean().item(), rel=1e-5, abs=1e-6)
+    assert stats[1].item() == pytest.approx((masked & (adv < 0)).sum().item() / rows, rel=1e-6)
+    row = torch.where(masked, torch.zeros_like(a), -ratio * a / rows)[:, None]
+    d = -row * probs
+    d[torch.arange(rows, device="cuda"), t] += row[:, 0]
+    err = (grad.double() - d).abs()
+    assert (err <= (1.2e-5 if dtype == F32 else 2 ** -8) * d.abs() + 1e-6 * row.abs().max()).all()
+    assert torch.all(grad[masked] == 0)
