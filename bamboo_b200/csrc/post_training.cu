@@ -157,7 +157,8 @@ template <typename T, int THREADS> __device__ __forceinline__ void soft_edges(co
 // 2^(k x - r) is a float all the same, so the loop needs no maximum; a share whose sum reaches SHARE_MOST (above a first
 // chunk that is masked, for one) is taken (again) in the exact form.  That bound keeps what the merges make of the shares: 8 x 512 of them add up to less than 2^76, far from
 // overflow; a share that a difference of 127 between references flushes to zero was below 2^-63 of the sum; and 1 / s is no denormal
-// number.  U loads are in flight per thread.
+// number.  A share that is taken again comes from L2: 8192 bf16 rows of 50257 at temperatures of 1 and 0.2 125 us, at 0.1 and below 235 (randn x 2;
+// nearly every share).  U loads are in flight per thread.
 constexpr float SHARE_MOST = 0x1p64f;
 template <typename T, int THREADS, int U>
 __device__ __forceinline__ void soft_share(const uint4* v, int nvec, K2 k, float& r, float& s) {
@@ -789,8 +790,8 @@ constexpr int TURNS = 4;
 // follows into them.  Two CTAs per SM fill each other's turns: a row takes a CTA (V = 50257, bf16) about 1.7 us of ex2
 // for the sum and again for the gradient, most of one between them for the sum's barrier and the token's slope, and an SM's
 // share of the memory rate is a row in 4.5 us.  Rows that do not count cost a CTA a fraction of the others and come in
-// runs (prompts), so rows are drawn from a counter.  7777 tokens, 16 sequences: 241 us with the two small kernels around it, 5.9 TB/s
-// (a block per row, read twice, 349; ring with rows dealt out in advance 305; 512 threads 248, 256 threads 245-248).
+// runs (prompts), so rows are drawn from a counter.  7777 tokens, 16 sequences: 246-260 us from call to call with the two small kernels around it, 5.4-5.7 TB/s
+// (beside 241 us: a block per row, read twice, 349; ring with rows dealt out in advance 305; 512 threads 248, 256 threads 245-248).
 constexpr int RING_THREADS = 384, RING_CHUNKS = 4, RING_STAGE = RING_THREADS * RING_CHUNKS * 16, RING_STAGES = (int)(MAX_RING + RING_STAGE - 1) / RING_STAGE;
 template <typename T>
 __global__ void __launch_bounds__(RING_THREADS + 32, 2)

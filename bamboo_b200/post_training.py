@@ -13,7 +13,7 @@
 Formulas stand beside the kernels' declarations (``include/bamboo_b200.h``) and in ``csrc/post_training.cu``.  Tokens whose target is
 ``ignore_index`` (prompts, padding) count nowhere and get no gradient; what stands at their places in logits, log-probabilities and
 advantages may be anything, NaN and infinities included.  Everything runs on the current stream, nothing synchronises, and there is no
-fallback: CPU tensors are refused.
+fallback: CPU tensors are refused.  Gradients have no gradient of their own (it raises), and what is written over (``inplace``) is known to autograd.
 """
 import functools
 import itertools
