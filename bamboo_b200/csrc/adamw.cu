@@ -1,0 +1,236 @@
+// One AdamW step over a list of tensors, moments in 32 or 8 bits (formulas and formats: bamboo_b200.h, bb_adamw_list).
+//
+// Memory bounds it: 18 bytes a parameter with moments in 8 bits, an fp32 master, a bf16 gradient and a bf16 working copy (28 in 32 bits).
+// A warp works on one block of 256 values, eight per lane, which is also the unit of the 8-bit scales: a block's largest magnitude is a
+// warp-wide maximum of bit patterns, under which NaN and infinity are the largest.  The list travels as a kernel argument.
+#include "common.cuh"
+#include "bamboo_b200.h"
+#include <cuda_fp8.h>
+#include <limits.h>
+#include <math.h>
+
+namespace {
+
+int refuse(const char* msg) { bb_set_last_error_msg(msg); return BB_ERR_INVALID_ARG; }
+
+constexpr int LIST = 64;                       // tensors of one launch
+constexpr int BLOCK = 256, THREADS = 256, WARPS = THREADS / 32;
+constexpr float TOP = 256.f, TINY = 0x1p-100f; // code of a block's largest value; scales up to TINY hold nothing
+constexpr float CODE_MIN = 0x1p-9f;            // smallest e4m3 value above 0
+
+struct AdamTable {
+  bb_adamw_tensor t[LIST];
+  int first[LIST + 1];                         // first block of each tensor
+  int count;
+};
+struct AdamArgs { float lr, b1, omb1, b2, omb2, eps, inv_bc1, inv_bc2, decay, grad_scale; int zero_grad; const float* coef; };
+
+__device__ __forceinline__ float2 code_pair(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+__device__ __forceinline__ uint32_t pair_code(float a, float b) { return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3); }
+
+// Codes of a lane's eight values under the block's scale, which every lane receives; ROOT: see CODE_MIN
+template <bool ROOT> __device__ __forceinline__ uint2 encode(const float* v, float& scale) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  top = __reduce_max_sync(0xffffffffu, top);
+  scale = __uint_as_float(top);
+  if (top >= 0x7f800000u) { scale = __uint_as_float(0x7fc00000u); return make_uint2(0, 0); }
+  if (scale <= TINY) return make_uint2(0, 0);
+  const float f = TOP / scale;
+  float c[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    c[i] = v[i] * f;
+    if (ROOT && v[i] > 0.f) c[i] = fmaxf(c[i], CODE_MIN);
+  }
+  return make_uint2(pair_code(c[0], c[1]) | pair_code(c[2], c[3]) << 16, pair_code(c[4], c[5]) | pair_code(c[6], c[7]) << 16);
+}
+__device__ __forceinline__ void decode(uint2 q, float scale, float* v) {
+  const float f = scale * (1.f / TOP);
+  const uint32_t two[4] = {q.x & 0xffffu, q.x >> 16, q.y & 0xffffu, q.y >> 16};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 c = code_pair(two[i]);
+    v[2 * i] = c.x * f; v[2 * i + 1] = c.y * f;
+  }
+}
+
+// A lane's values: all eight at once where the block is whole and the tensors lie on 16 bytes, one by one elsewhere
+template <bool VEC> __device__ __forceinline__ void load8(const float* p, int n, float* v) {
+  if (VEC) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.f;
+  }
+}
+template <bool VEC> __device__ __forceinline__ void load8(const __nv_bfloat16* p, int n, float* v) {
+  if (VEC) {
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
+    v[0] = bb::bf16_lo(q.x); v[1] = bb::bf16_hi(q.x); v[2] = bb::bf16_lo(q.y); v[3] = bb::bf16_hi(q.y);
+    v[4] = bb::bf16_lo(q.z); v[5] = bb::bf16_hi(q.z); v[6] = bb::bf16_lo(q.w); v[7] = bb::bf16_hi(q.w);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? __bfloat162float(p[i]) : 0.f;
+  }
+}
+template <bool VEC> __device__ __forceinline__ void store8(float* p, int n, const float* v) {
+  if (VEC) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) if (i < n) p[i] = v[i];
+  }
+}
+template <bool VEC> __device__ __forceinline__ void store8(__nv_bfloat16* p, int n, const float* v) {
+  if (VEC) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(bb::pack_bf16x2(v[0], v[1]), bb::pack_bf16x2(v[2], v[3]), bb::pack_bf16x2(v[4], v[5]), bb::pack_bf16x2(v[6], v[7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) if (i < n) p[i] = __float2bfloat16(v[i]);
+  }
+}
+template <bool VEC> __device__ __forceinline__ uint2 load_codes(const uint8_t* p, int n) {
+  uint2 q = make_uint2(0, 0);
+  if (VEC) {
+    q = *reinterpret_cast<const uint2*>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) if (i < n) (i < 4 ? q.x : q.y) |= (uint32_t)p[i] << (8 * (i & 3));
+  }
+  return q;
+}
+template <bool VEC> __device__ __forceinline__ void store_codes(uint8_t* p, int n, uint2 q) {
+  if (VEC) {
+    *reinterpret_cast<uint2*>(p) = q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) if (i < n) p[i] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+  }
+}
+
+template <bool EIGHT, bool VEC>
+__device__ __forceinline__ void block_step(const bb_adamw_tensor& t, long long at, long long block, int n, int lane, const AdamArgs& a, float gs) {
+  float p[8], g[8], m[8], v[8], sm = 0.f, sv = 0.f;
+  const long long blocks = (t.numel + BLOCK - 1) / BLOCK;
+  float* master = t.master ? t.master : reinterpret_cast<float*>(t.param);
+  if (EIGHT) { sm = t.scales[block]; sv = t.scales[blocks + block]; }
+  load8<VEC>(master + at, n, p);
+  if (t.grad_dtype == BB_DTYPE_F32) load8<VEC>(reinterpret_cast<const float*>(t.grad) + at, n, g);
+  else load8<VEC>(reinterpret_cast<const __nv_bfloat16*>(t.grad) + at, n, g);
+  if (EIGHT) {
+    decode(load_codes<VEC>(reinterpret_cast<const uint8_t*>(t.exp_avg) + at, n), sm, m);
+    decode(load_codes<VEC>(reinterpret_cast<const uint8_t*>(t.exp_avg_sq) + at, n), sv, v);
+  } else {
+    load8<VEC>(reinterpret_cast<const float*>(t.exp_avg) + at, n, m);
+    load8<VEC>(reinterpret_cast<const float*>(t.exp_avg_sq) + at, n, v);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = g[i] * gs, old = EIGHT ? v[i] * v[i] : v[i];
+    m[i] = fmaf(a.b1, m[i], a.omb1 * x);
+    v[i] = fmaf(a.b2, old, a.omb2 * x * x);
+    const float step = (m[i] * a.inv_bc1) / (sqrtf(v[i] * a.inv_bc2) + a.eps);
+    p[i] = fmaf(-a.lr, fmaf(a.decay, p[i], step), p[i]);
+  }
+  store8<VEC>(master + at, n, p);
+  if (t.master) store8<VEC>(reinterpret_cast<__nv_bfloat16*>(t.param) + at, n, p);
+  if (a.zero_grad) {
+    const float zeros[8] = {};
+    if (t.grad_dtype == BB_DTYPE_F32) store8<VEC>(reinterpret_cast<float*>(t.grad) + at, n, zeros);
+    else store8<VEC>(reinterpret_cast<__nv_bfloat16*>(t.grad) + at, n, zeros);
+  }
+  if (EIGHT) {
+    if (!VEC) {                                // what a partial block has beyond its end decides nothing
+#pragma unroll
+      for (int i = 0; i < 8; ++i) if (i >= n) { m[i] = 0.f; v[i] = 0.f; }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = sqrtf(v[i]);
+    const uint2 cm = encode<false>(m, sm), cv = encode<true>(v, sv);
+    store_codes<VEC>(reinterpret_cast<uint8_t*>(t.exp_avg) + at, n, cm);
+    store_codes<VEC>(reinterpret_cast<uint8_t*>(t.exp_avg_sq) + at, n, cv);
+    if (lane == 0) { t.scales[block] = sm; t.scales[blocks + block] = sv; }
+  } else {
+    store8<VEC>(reinterpret_cast<float*>(t.exp_avg) + at, n, m);
+    store8<VEC>(reinterpret_cast<float*>(t.exp_avg_sq) + at, n, v);
+  }
+}
+
+template <bool EIGHT>
+__global__ void __launch_bounds__(THREADS)
+adamw_list_kernel(const __grid_constant__ AdamTable table, const AdamArgs a) {
+  bb::pdl_sync();
+  const int lane = threadIdx.x & 31;
+  const int unit = blockIdx.x * WARPS + (threadIdx.x >> 5);
+  if (unit >= table.first[table.count]) return;
+  int lo = 0, hi = table.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (table.first[mid] <= unit) lo = mid; else hi = mid - 1;
+  }
+  const bb_adamw_tensor& t = table.t[lo];
+  const long long block = unit - table.first[lo], at = block * BLOCK + lane * 8, left = t.numel - at;
+  const float gs = a.coef ? a.coef[0] * a.grad_scale : a.grad_scale;
+  // `unused` of the table: every tensor of this entry lies on 16 bytes (codes: 8)
+  if (t.unused && t.numel - block * BLOCK >= BLOCK) block_step<EIGHT, true>(t, at, block, 8, lane, a, gs);
+  else block_step<EIGHT, false>(t, at, block, left <= 0 ? 0 : left < 8 ? (int)left : 8, lane, a, gs);
+}
+
+bool bad_tensor(const bb_adamw_tensor& t, bool eight) {
+  return !t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || t.numel <= 0 || t.numel > (1LL << 38) || (eight != (t.scales != nullptr)) ||
+         (t.grad_dtype != BB_DTYPE_BF16 && t.grad_dtype != BB_DTYPE_F32) || ((uintptr_t)t.grad & (t.grad_dtype == BB_DTYPE_F32 ? 3 : 1)) ||
+         ((uintptr_t)t.param & (t.master ? 1 : 3)) || (((uintptr_t)t.master | (uintptr_t)t.scales) & 3) ||
+         (!eight && (((uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq) & 3));
+}
+bool aligned(const bb_adamw_tensor& t, bool eight) {
+  return (((uintptr_t)t.param | (uintptr_t)t.master | (uintptr_t)t.grad) & 15) == 0 &&
+         (((uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq) & (eight ? 7 : 15)) == 0;
+}
+}  // namespace
+
+extern "C" int bb_adamw_list(const bb_adamw_tensor* tensors, int count, double lr, double beta1, double beta2, double eps, long long step,
+                             double weight_decay, double grad_scale, int zero_grad, double max_norm, const double* sumsq, float* norm, void* workspace,
+                             long long workspace_bytes, void* stream) {
+  if (!tensors || count <= 0 || step < 1 || !(max_norm >= 0.0) ||
+      (max_norm > 0.0 && (!norm || !workspace || ((uintptr_t)workspace & 7) || workspace_bytes < bb_grad_norm_workspace_bytes())))
+    return refuse("bb_adamw_list: an empty list, step < 1, a negative norm, or clipping without a place for the norm or with a workspace that is too small");
+  const bool eight = tensors[0].scales != nullptr;
+  for (int i = 0; i < count; ++i)
+    if (bad_tensor(tensors[i], eight))
+      return refuse("bb_adamw_list: a null or misaligned pointer, an empty tensor, a gradient that is neither bf16 nor fp32, or scales for a part of the list only");
+  cudaStream_t s = (cudaStream_t)stream;
+  AdamArgs a;
+  a.lr = (float)lr; a.b1 = (float)beta1; a.omb1 = (float)(1.0 - beta1); a.b2 = (float)beta2; a.omb2 = (float)(1.0 - beta2); a.eps = (float)eps;
+  a.inv_bc1 = (float)(1.0 / (1.0 - pow(beta1, (double)step))); a.inv_bc2 = (float)(1.0 / (1.0 - pow(beta2, (double)step)));
+  a.decay = (float)weight_decay; a.grad_scale = (float)grad_scale; a.zero_grad = zero_grad; a.coef = nullptr;
+  BackToBack overlap;
+  if (max_norm > 0.0) {
+    if (int rc = bb_list_clip_coef(tensors, count, sumsq, grad_scale, max_norm, norm, workspace, s)) return rc;
+    a.coef = (const float*)((double*)workspace + 1);
+  }
+  for (int from = 0; from < count;) {
+    AdamTable t;
+    long long blocks = 0;
+    int n = 0;
+    for (; n < LIST && from + n < count; ++n) {
+      const long long more = (tensors[from + n].numel + BLOCK - 1) / BLOCK;
+      if (blocks + more > INT_MAX - 64) break;          // (a launch's blocks are counted in an int; one tensor's always are)
+      t.t[n] = tensors[from + n];
+      t.t[n].unused = aligned(t.t[n], eight) ? 1 : 0;
+      t.first[n] = (int)blocks;
+      blocks += more;
+    }
+    t.count = n;
+    t.first[n] = (int)blocks;
+    BB_CUDA_CHECK(bb_launch(eight ? adamw_list_kernel<true> : adamw_list_kernel<false>, dim3((unsigned)((blocks + WARPS - 1) / WARPS)), THREADS, 0, s, t, a));
+    from += n;
+  }
+  return BB_OK;
+}

@@ -89,6 +89,11 @@ int bb_conv_gemm(const bb_conv_gemm_args* a, void* stream);
 // Time that a stored product of M x N over K is expected to take on the whole GPU, as it is planned for that CTA budget.
 double bb_gemm_store_us(long long M, long long N, long long K, int max_ctas);
 
+// Clipping coefficient over the gradients of a list of parameters (post_training.cu): the second 8 bytes of a bb_grad_norm_workspace_bytes() workspace
+// receive it as a float; launched as part of a call that steps over the list.
+int bb_list_clip_coef(const bb_adamw_tensor* tensors, int count, const double* sumsq, double grad_scale, double max_norm, float* norm, void* workspace,
+                      cudaStream_t s);
+
 // Division by a number known at launch: n / d = high word of n * magic with magic = floor(2^64 / d) + 1 (0 stands for
 // d = 1); for n < 2^32 the error n * d / 2^64 stays below 1.
 inline unsigned long long bb_div_magic(int d) { return d == 1 ? 0 : ~0ull / (unsigned long long)d + 1; }
@@ -408,6 +413,11 @@ __device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const void* tma
   asm volatile(
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
       : : "r"(smem_u32(smem_dst)), "l"(tmap), "r"(bar_cluster_addr), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const void* tmap, uint32_t bar_cluster_addr, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      : : "r"(smem_u32(smem_dst)), "l"(tmap), "r"(bar_cluster_addr), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
 __device__ __forceinline__ void tma_load_im2col_pair(void* smem_dst, const void* tmap, uint32_t bar_cluster_addr, int c, int w,
                                                      int h, int n, uint16_t off_w, uint16_t off_h) {

@@ -1,0 +1,559 @@
+// Routing of tokens to experts and the way of their rows there and back (declarations and formulas in bamboo_b200.h).
+//
+// Every operator here is bound by memory, and for a few thousand tokens by its launches.  Nothing depends on the order in which CTAs run:
+// places are counted and not drawn, sums are taken in one order.
+#include "common.cuh"
+#include "bamboo_b200.h"
+#include <limits.h>
+#include <stdio.h>
+
+namespace {
+
+int refuse(const char* msg) { bb_set_last_error_msg(msg); return BB_ERR_INVALID_ARG; }
+
+__device__ __forceinline__ float value_of(float v) { return v; }
+__device__ __forceinline__ float value_of(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void put_value(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put_value(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+// ------------------------------------------------------------------ routing
+constexpr int MAX_EXPERTS = 256, MAX_CHOSEN = 32;
+constexpr int ROUTE_WARPS = 8, ROUTE_THREADS = 32 * ROUTE_WARPS;
+
+struct RouteParams {
+  int tokens, experts, k, normalize;
+  long long ld;
+  int chunk, blocks;            // consecutive tokens of a block, blocks
+  float* weights; int* chosen; int* rows; int* slots; int* offsets; float* balance; float2* stats; float* load;
+  int* counts;                  // [blocks][experts + 1]: slots of every expert, tokens that have any
+  float* probs;                 // [blocks][experts]: sums of softmax
+};
+
+// A logit as a number whose order is that of the choice: NaN above all, 0 for what is never chosen (-inf), both zeros alike
+__device__ __forceinline__ uint32_t choice_key(float x) {
+  if (x != x) return 0xffffffffu;
+  if (x == -INFINITY) return 0u;
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+// A warp per token: lane l holds logits l, l + 32, ...; k rounds of a warp-wide maximum and the lowest index that has it.  Then the block's slots
+// are ranked within their experts, in order.
+template <typename T, int PER>
+__global__ void __launch_bounds__(ROUTE_THREADS)
+route_choose_kernel(const T* logits, const RouteParams p) {
+  __shared__ int hist[ROUTE_WARPS][MAX_EXPERTS];
+  __shared__ float sums[ROUTE_WARPS][MAX_EXPERTS];
+  __shared__ int some_tokens;
+  bb::pdl_sync();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t0 = blockIdx.x * p.chunk, t1 = min(p.tokens, t0 + p.chunk);
+  for (int i = threadIdx.x; i < ROUTE_WARPS * MAX_EXPERTS; i += ROUTE_THREADS) (&hist[0][0])[i] = 0;
+  if (threadIdx.x == 0) some_tokens = 0;
+  float prob[PER] = {};
+  int some = 0;
+  for (int t = t0 + warp; t < t1; t += ROUTE_WARPS) {
+    const T* row = logits + (long long)t * p.ld;
+    float x[PER];
+    uint32_t key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] = lane + 32 * i < p.experts ? value_of(row[lane + 32 * i]) : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) key[i] = choice_key(x[i]);
+    int mine = -1;
+    float value = 0.f;
+    for (int j = 0; j < p.k; ++j) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) top = max(top, key[i]);
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (top == 0) break;
+      uint32_t at = 0xffffffffu;
+#pragma unroll
+      for (int i = PER - 1; i >= 0; --i) if (key[i] == top) at = lane + 32 * i;
+      at = __reduce_min_sync(0xffffffffu, at);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) if (lane + 32 * i == (int)at) key[i] = 0;
+      if (lane == j) { mine = (int)at; value = key_value(top); }
+    }
+    const bool any = __shfl_sync(0xffffffffu, mine, 0) >= 0;
+    const float top = __shfl_sync(0xffffffffu, value, 0);
+    float e[PER], sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      e[i] = any && lane + 32 * i < p.experts ? expf(x[i] - top) : 0.f;
+      sum += e[i];
+    }
+    sum = warp_sum(sum);
+    const float share = mine >= 0 ? expf(value - top) : 0.f;
+    const float over = p.normalize ? warp_sum(share) : sum;
+    const long long s = (long long)t * p.k + lane;
+    if (lane < p.k) {
+      p.chosen[s] = mine;
+      p.weights[s] = mine >= 0 ? share / over : 0.f;
+    }
+    if (lane == 0) p.stats[t] = make_float2(top, sum);
+    if (any) {
+      ++some;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) prob[i] += e[i] / sum;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) if (lane + 32 * i < p.experts) sums[warp][lane + 32 * i] = prob[i];
+  __syncthreads();
+  if (lane == 0) atomicAdd(&some_tokens, some);
+  // ranks: every warp counts a run of the block's slots, then ranks it behind the runs before
+  const int k = p.k, first = t0 * k, n = (t1 - t0) * k;
+  const int run = (n + 32 * ROUTE_WARPS - 1) / (32 * ROUTE_WARPS) * 32, a = min(n, warp * run), b = min(n, a + run);
+  for (int i = a + lane; i - lane < b; i += 32) {
+    const int e = i < b ? p.chosen[first + i] : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, e);
+    if (e >= 0 && (same & ((1u << lane) - 1)) == 0) hist[warp][e] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.experts; e += ROUTE_THREADS) {
+    int total = 0;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < ROUTE_WARPS; ++w) { const int c = hist[w][e]; hist[w][e] = total; total += c; s += sums[w][e]; }
+    p.counts[(long long)blockIdx.x * (p.experts + 1) + e] = total;
+    p.probs[(long long)blockIdx.x * p.experts + e] = s;
+  }
+  if (threadIdx.x == 0) p.counts[(long long)blockIdx.x * (p.experts + 1) + p.experts] = some_tokens;
+  __syncthreads();
+  for (int i = a + lane; i - lane < b; i += 32) {
+    const int e = i < b ? p.chosen[first + i] : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, e);
+    const unsigned before = same & ((1u << lane) - 1);
+    int at = 0;
+    if (e >= 0) at = hist[warp][e];
+    __syncwarp();
+    if (e >= 0 && before == 0) hist[warp][e] = at + __popc(same);
+    if (i < b) p.rows[first + i] = e >= 0 ? at + __popc(before) : -1;
+    __syncwarp();
+  }
+}
+
+// Every block adds up what stands before its slots (the counts of all blocks, once more each) and places them.
+__global__ void __launch_bounds__(ROUTE_THREADS)
+route_place_kernel(const RouteParams p) {
+  __shared__ int total[MAX_EXPERTS + 1], before[MAX_EXPERTS + 1], base[MAX_EXPERTS + 1];
+  __shared__ double part[ROUTE_WARPS];
+  bb::pdl_sync();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, width = p.experts + 1;
+  for (int e = threadIdx.x; e < width; e += ROUTE_THREADS) { total[e] = 0; before[e] = 0; }
+  __syncthreads();
+  int groups = ROUTE_THREADS / width;
+  if (groups < 1) groups = 1;
+  for (int i = threadIdx.x; i < groups * width; i += ROUTE_THREADS) {
+    const int g = i / width, e = i - g * width;
+    int all = 0, ahead = 0;
+#pragma unroll 8
+    for (int b = g; b < p.blocks; b += groups) {
+      const int c = p.counts[(long long)b * width + e];
+      all += c;
+      if (b < (int)blockIdx.x) ahead += c;
+    }
+    atomicAdd(&total[e], all);
+    atomicAdd(&before[e], ahead);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int carry = 0;
+    for (int at = 0; at < p.experts; at += 32) {
+      const int e = at + lane, c = e < p.experts ? total[e] : 0;
+      int v = c;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += o;
+      }
+      if (e < p.experts) base[e] = carry + v - c;
+      carry += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) base[p.experts] = carry;
+  }
+  __syncthreads();
+  const int k = p.k, t0 = blockIdx.x * p.chunk, t1 = min(p.tokens, t0 + p.chunk), routed = base[p.experts];
+  const long long all = (long long)p.tokens * k;
+  for (int i = t0 * k + threadIdx.x; i < t1 * k; i += ROUTE_THREADS) {
+    const int e = p.chosen[i];
+    if (e >= 0) {
+      const int at = base[e] + before[e] + p.rows[i];
+      p.rows[i] = at;
+      p.slots[at] = i;
+    }
+  }
+  for (long long r = routed + (long long)blockIdx.x * ROUTE_THREADS + threadIdx.x; r < all; r += (long long)gridDim.x * ROUTE_THREADS) p.slots[r] = -1;
+  if (blockIdx.x != 0) return;
+  double sum = 0.0;
+  const double tokens = total[p.experts] > 0 ? total[p.experts] : 1, places = routed > 0 ? routed : 1;
+  for (int e = threadIdx.x; e < p.experts; e += ROUTE_THREADS) {
+    p.offsets[e] = base[e];
+    const double f = total[e] / places;
+    p.load[e] = (float)f;
+    double mass = 0.0;
+#pragma unroll 8
+    for (int b = 0; b < p.blocks; ++b) mass += (double)p.probs[(long long)b * p.experts + e];
+    sum += f * mass / tokens;
+  }
+  if (threadIdx.x == 0) { p.offsets[p.experts] = routed; p.load[p.experts] = (float)tokens; }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (lane == 0) part[warp] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = 0.0;
+    for (int w = 0; w < ROUTE_WARPS; ++w) sum += part[w];
+    p.balance[0] = (float)(p.experts * sum);
+  }
+}
+
+// dx_e = p_e (c_e - sum p c) + what arrives through the weights; a warp per token, its chosen experts in lanes 0 .. k - 1
+template <typename T, int PER>
+__global__ void __launch_bounds__(ROUTE_THREADS)
+route_bwd_kernel(const T* logits, const RouteParams p, const float* d_weights, const float* d_balance, T* out, long long ldd, int cols) {
+  bb::pdl_sync();
+  const int lane = threadIdx.x & 31;
+  const float g = d_balance ? d_balance[0] * (float)p.experts / p.load[p.experts] : 0.f;
+  float push[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) push[i] = d_balance && lane + 32 * i < p.experts ? g * p.load[lane + 32 * i] : 0.f;
+  for (int t = blockIdx.x * ROUTE_WARPS + (threadIdx.x >> 5); t < p.tokens; t += gridDim.x * ROUTE_WARPS) {
+    const T* row = logits + (long long)t * p.ld;
+    const long long s = (long long)t * p.k + lane;
+    int mine = lane < p.k ? p.chosen[s] : -1;
+    if (mine >= p.experts) mine = -1;
+    const float2 st = p.stats[t];
+    const bool any = __shfl_sync(0xffffffffu, mine, 0) >= 0;
+    T* to = out + (long long)t * ldd;
+    if (!any) {
+      for (int c = lane; c < cols; c += 32) put_value(to + c, 0.f);
+      continue;
+    }
+    float prob[PER], d[PER], mean = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      prob[i] = lane + 32 * i < p.experts ? expf(value_of(row[lane + 32 * i]) - st.x) / st.y : 0.f;
+      mean += prob[i] * push[i];
+    }
+    float dw = 0.f, w = 0.f;
+    if (mine >= 0) {
+      w = expf(value_of(row[mine]) - st.x);
+      dw = d_weights ? d_weights[s] : 0.f;
+    }
+    w /= p.normalize ? warp_sum(w) : st.y;
+    const float through = warp_sum(w * dw);
+    mean = warp_sum(mean);
+    const float add = p.normalize ? w * (dw - through) : w * dw;
+    const float off = p.normalize ? mean : mean + through;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) d[i] = prob[i] * (push[i] - off);
+    for (int j = 0; j < p.k; ++j) {
+      const int e = __shfl_sync(0xffffffffu, mine, j);
+      const float v = __shfl_sync(0xffffffffu, add, j);
+      if (e < 0) break;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) if (lane + 32 * i == e) d[i] += v;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) if (lane + 32 * i < p.experts) put_value(to + lane + 32 * i, d[i]);
+    for (int c = p.experts + lane; c < cols; c += 32) put_value(to + c, 0.f);
+  }
+}
+
+// ------------------------------------------------------------------ rows there and back
+// A team of threads per row (a warp, eight rows to a block; or a whole block where rows are long), 16 bytes at a time where
+// pointers and strides allow it.
+template <typename T, int BYTES> struct Pack;
+template <> struct Pack<float, 16> {
+  static constexpr int N = 4;
+  typedef float4 raw;
+  static __device__ __forceinline__ void get(const float* p, float* v) { const float4 q = *reinterpret_cast<const float4*>(p); v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w; }
+  static __device__ __forceinline__ void put(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+};
+template <> struct Pack<__nv_bfloat16, 16> {
+  static constexpr int N = 8;
+  typedef uint4 raw;
+  static __device__ __forceinline__ void get(const __nv_bfloat16* p, float* v) {
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
+    v[0] = bb::bf16_lo(q.x); v[1] = bb::bf16_hi(q.x); v[2] = bb::bf16_lo(q.y); v[3] = bb::bf16_hi(q.y);
+    v[4] = bb::bf16_lo(q.z); v[5] = bb::bf16_hi(q.z); v[6] = bb::bf16_lo(q.w); v[7] = bb::bf16_hi(q.w);
+  }
+  static __device__ __forceinline__ void put(__nv_bfloat16* p, const float* v) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(bb::pack_bf16x2(v[0], v[1]), bb::pack_bf16x2(v[2], v[3]), bb::pack_bf16x2(v[4], v[5]), bb::pack_bf16x2(v[6], v[7]));
+  }
+};
+template <> struct Pack<float, 4> {
+  static constexpr int N = 1;
+  typedef float raw;
+  static __device__ __forceinline__ void get(const float* p, float* v) { v[0] = *p; }
+  static __device__ __forceinline__ void put(float* p, const float* v) { *p = v[0]; }
+};
+template <> struct Pack<__nv_bfloat16, 2> {
+  static constexpr int N = 1;
+  typedef unsigned short raw;
+  static __device__ __forceinline__ void get(const __nv_bfloat16* p, float* v) { v[0] = __bfloat162float(*p); }
+  static __device__ __forceinline__ void put(__nv_bfloat16* p, const float* v) { *p = __float2bfloat16(v[0]); }
+};
+
+constexpr int MOVE_THREADS = 256;
+// An index of the routing: -1 (none) where it does not point at one of `count` rows, which sets the status word unless it is -1 already
+__device__ __forceinline__ int checked(int i, int count, int* status) {
+  if (i < -1 || i >= count) {
+    if (status) atomicCAS(status, 0, BB_ERR_INVALID_ARG);
+    return -1;
+  }
+  return i;
+}
+template <int TEAM> constexpr int TEAMS = MOVE_THREADS / TEAM;
+
+template <typename T, int BYTES, int TEAM>
+__global__ void __launch_bounds__(MOVE_THREADS)
+dispatch_kernel(const T* x, long long ld, const int* slots, int k, T* out, int rows, int tokens, int h, int* status) {
+  typedef Pack<T, BYTES> P;
+  typedef typename P::raw raw;
+  bb::pdl_sync();
+  const int r = blockIdx.x * TEAMS<TEAM> + threadIdx.x / TEAM, i0 = threadIdx.x % TEAM;
+  if (r >= rows) return;
+  const int s = checked(slots[r], tokens * k, status), n = h / P::N;
+  raw* to = reinterpret_cast<raw*>(out + (long long)r * h);
+  if (s < 0) {
+    const float zeros[P::N] = {};
+    for (int i = i0; i < n; i += TEAM) P::put(reinterpret_cast<T*>(to + i), zeros);
+    return;
+  }
+  const raw* from = reinterpret_cast<const raw*>(x + (long long)(s / k) * ld);
+#pragma unroll 4
+  for (int i = i0; i < n; i += TEAM) to[i] = from[i];
+}
+
+template <typename T, int BYTES, int TEAM>
+__global__ void __launch_bounds__(MOVE_THREADS)
+combine_kernel(const T* x, long long ld, const int* rows_of, const float* weights, const T* residual, long long ld_res, int k, T* out, int tokens, int rows, int h,
+               int* status) {
+  typedef Pack<T, BYTES> P;
+  bb::pdl_sync();
+  const int t = blockIdx.x * TEAMS<TEAM> + threadIdx.x / TEAM, i0 = threadIdx.x % TEAM;
+  if (t >= tokens) return;
+  const int n = h / P::N;
+  const long long s = (long long)t * k;
+  for (int i = i0; i < n; i += TEAM) {
+    float sum[P::N] = {};
+#pragma unroll 4
+    for (int j = 0; j < k; ++j) {
+      const int r = checked(rows_of[s + j], rows, status);
+      if (r < 0) continue;
+      const float w = weights ? weights[s + j] : 1.f;
+      float v[P::N];
+      P::get(x + (long long)r * ld + i * P::N, v);
+#pragma unroll
+      for (int c = 0; c < P::N; ++c) sum[c] = fmaf(w, v[c], sum[c]);
+    }
+    if (residual) {
+      float v[P::N];
+      P::get(residual + (long long)t * ld_res + i * P::N, v);
+#pragma unroll
+      for (int c = 0; c < P::N; ++c) sum[c] += v[c];
+    }
+    P::put(out + (long long)t * h + i * P::N, sum);
+  }
+}
+
+template <typename T, int BYTES, int TEAM>
+__global__ void __launch_bounds__(MOVE_THREADS)
+combine_bwd_kernel(const T* dy, long long ld_dy, const T* x, long long ld, const int* rows_of, const int* slots, const float* weights, int k, T* dx,
+                   float* d_weights, int tokens, int rows, int h, int* status) {
+  typedef Pack<T, BYTES> P;
+  __shared__ float part[TEAM > 32 ? TEAM / 32 : 1];
+  bb::pdl_sync();
+  const int t = blockIdx.x * TEAMS<TEAM> + threadIdx.x / TEAM, i0 = threadIdx.x % TEAM;
+  if (t >= tokens) return;
+  const int n = h / P::N;
+  const T* from = dy + (long long)t * ld_dy;
+  for (int j = 0; j < k; ++j) {
+    const long long s = (long long)t * k + j;
+    const int r = checked(rows_of[s], rows, status);
+    float dot = 0.f;
+    if (r >= 0) {
+      const float w = weights[s];
+#pragma unroll 2
+      for (int i = i0; i < n; i += TEAM) {
+        float d[P::N], v[P::N];
+        P::get(from + i * P::N, d);
+        if (d_weights) {
+          P::get(x + (long long)r * ld + i * P::N, v);
+#pragma unroll
+          for (int c = 0; c < P::N; ++c) dot = fmaf(d[c], v[c], dot);
+        }
+        if (dx) {
+#pragma unroll
+          for (int c = 0; c < P::N; ++c) d[c] *= w;
+          P::put(dx + (long long)r * h + i * P::N, d);
+        }
+      }
+    }
+    if (d_weights) {
+      dot = warp_sum(dot);
+      if (TEAM > 32) {
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = dot;
+        __syncthreads();
+        dot = 0.f;
+#pragma unroll
+        for (int w = 0; w < TEAM / 32; ++w) dot += part[w];
+      }
+      if (i0 == 0) d_weights[s] = r >= 0 ? dot : 0.f;
+    }
+    // the place of the same number as this slot: zeros where nobody stands
+    if (dx && slots[s] < 0 && s < rows) {
+      const float zeros[P::N] = {};
+      for (int i = i0; i < n; i += TEAM) P::put(dx + s * h + i * P::N, zeros);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host side
+bool bad_route(const bb_route_desc* d) {
+  return !d || d->tokens <= 0 || d->experts <= 0 || d->experts > MAX_EXPERTS || d->k <= 0 || d->k > d->experts || d->k > MAX_CHOSEN || d->ld < d->experts ||
+         (d->dtype != BB_DTYPE_BF16 && d->dtype != BB_DTYPE_F32) || (long long)d->tokens * d->k > INT_MAX - 1024;
+}
+
+RouteParams route_params(const bb_route_desc* d) {
+  RouteParams p = {};
+  p.tokens = d->tokens; p.experts = d->experts; p.k = d->k; p.normalize = d->normalize; p.ld = d->ld;
+  const int most = 2 * bb_num_sms();
+  p.chunk = (d->tokens + most - 1) / most;
+  if (p.chunk < ROUTE_WARPS) p.chunk = ROUTE_WARPS;
+  p.blocks = (d->tokens + p.chunk - 1) / p.chunk;
+  return p;
+}
+
+template <typename T> int route_fwd(const T* logits, const RouteParams& p, cudaStream_t s) {
+  const int per = (p.experts + 31) / 32;
+  auto kernel = per <= 1 ? route_choose_kernel<T, 1> : per <= 2 ? route_choose_kernel<T, 2> : per <= 4 ? route_choose_kernel<T, 4> : route_choose_kernel<T, 8>;
+  BB_CUDA_CHECK(bb_launch(kernel, p.blocks, ROUTE_THREADS, 0, s, logits, p));
+  BB_CUDA_CHECK(bb_launch(route_place_kernel, p.blocks, ROUTE_THREADS, 0, s, p));
+  return BB_OK;
+}
+
+template <typename T>
+int route_bwd(const T* logits, const RouteParams& p, const float* dw, const float* db, T* out, long long ldd, int cols, cudaStream_t s) {
+  const int per = (p.experts + 31) / 32;
+  auto kernel = per <= 1 ? route_bwd_kernel<T, 1> : per <= 2 ? route_bwd_kernel<T, 2> : per <= 4 ? route_bwd_kernel<T, 4> : route_bwd_kernel<T, 8>;
+  const int want = (p.tokens + ROUTE_WARPS - 1) / ROUTE_WARPS, most = 8 * bb_num_sms();
+  BB_CUDA_CHECK(bb_launch(kernel, want < most ? want : most, ROUTE_THREADS, 0, s, logits, p, dw, db, out, ldd, cols));
+  return BB_OK;
+}
+
+bool odd(const void* p, uintptr_t mask) { return ((uintptr_t)p & mask) != 0; }
+
+// 16-byte accesses: every pointer and row on 16 bytes
+template <typename T> bool whole(const void* a, long long lda, const void* b, long long ldb, const void* c, long long ldc, const void* d, int h) {
+  const long long item = sizeof(T);
+  return !odd(a, 15) && !odd(b, 15) && !odd(c, 15) && !odd(d, 15) && lda * item % 16 == 0 && ldb * item % 16 == 0 && ldc * item % 16 == 0 && h * item % 16 == 0;
+}
+// Rows from 16 KB on, or few rows from 4 KB on, by a block each
+bool long_rows(long long rows, long long bytes) { return bytes >= 16384 || (bytes >= 4096 && rows < 1024); }
+
+#define MOVE(kernel, T, vec, big, rows, ...)                                                                                        \
+  do {                                                                                                                              \
+    const long long blocks_ = (big) ? (rows) : ((rows) + TEAMS<32> - 1) / TEAMS<32>;                                                \
+    if (blocks_ > INT_MAX) return refuse("more rows than one launch covers");                                                       \
+    if (vec) BB_CUDA_CHECK(bb_launch((big) ? kernel<T, 16, MOVE_THREADS> : kernel<T, 16, 32>, (int)blocks_, MOVE_THREADS, 0, s, __VA_ARGS__)); \
+    else BB_CUDA_CHECK(bb_launch((big) ? kernel<T, sizeof(T), MOVE_THREADS> : kernel<T, sizeof(T), 32>, (int)blocks_, MOVE_THREADS, 0, s, __VA_ARGS__)); \
+    return BB_OK;                                                                                                                   \
+  } while (0)
+
+template <typename T> int dispatch(const T* x, long long ld, const int* slots, int k, T* out, int rows, int tokens, int h, cudaStream_t s) {
+  const bool vec = whole<T>(x, ld, out, 0, nullptr, 0, nullptr, h), big = long_rows(rows, (long long)h * sizeof(T));
+  MOVE(dispatch_kernel, T, vec, big, rows, x, ld, slots, k, out, rows, tokens, h, bb_device_status_word());
+}
+template <typename T>
+int combine(const T* x, long long ld, const int* rows_of, const float* w, const T* res, long long ld_res, int k, T* out, int tokens, int rows, int h, cudaStream_t s) {
+  const bool vec = whole<T>(x, ld, out, 0, res, res ? ld_res : 0, nullptr, h), big = long_rows(tokens, (long long)h * sizeof(T));
+  MOVE(combine_kernel, T, vec, big, tokens, x, ld, rows_of, w, res, ld_res, k, out, tokens, rows, h, bb_device_status_word());
+}
+template <typename T>
+int combine_bwd(const T* dy, long long ld_dy, const T* x, long long ld, const int* rows_of, const int* slots, const float* w, int k, T* dx, float* dw,
+                int tokens, int rows, int h, cudaStream_t s) {
+  const bool vec = whole<T>(dy, ld_dy, dw ? x : nullptr, dw ? ld : 0, nullptr, 0, dx, h), big = long_rows(tokens, (long long)h * sizeof(T));
+  MOVE(combine_bwd_kernel, T, vec, big, tokens, dy, ld_dy, x, ld, rows_of, slots, w, k, dx, dw, tokens, rows, h, bb_device_status_word());
+}
+
+bool bad_move(const void* x, long long ld, int dtype, const void* index, int k, long long rows, long long tokens, int h) {
+  return !x || tokens <= 0 || k > INT_MAX / tokens || !index || odd(index, 3) || k <= 0 || rows <= 0 || rows > INT_MAX || h <= 0 || ld < h || (dtype != BB_DTYPE_BF16 && dtype != BB_DTYPE_F32) ||
+         odd(x, dtype == BB_DTYPE_F32 ? 3 : 1);
+}
+}  // namespace
+
+extern "C" long long bb_route_workspace_bytes(const bb_route_desc* d) {
+  if (bad_route(d)) return 0;
+  const RouteParams p = route_params(d);
+  return 4LL * p.blocks * (2 * p.experts + 1);
+}
+
+extern "C" int bb_route_fwd(const bb_route_desc* d, const void* logits, float* weights, int* experts_out, int* rows_out, int* slots_out, int* offsets,
+                            float* balance, float* stats, float* load, void* workspace, long long workspace_bytes, void* stream) {
+  if (bad_route(d) || !logits || odd(logits, d->dtype == BB_DTYPE_F32 ? 3 : 1) || !weights || !experts_out || !rows_out || !slots_out || !offsets || !balance || !stats ||
+      odd(stats, 7) || !load || !workspace || odd(workspace, 3) || workspace_bytes < bb_route_workspace_bytes(d))
+    return refuse("bb_route_fwd: null or misaligned pointer, no tokens, 1 to 256 experts of which 1 to 32 are chosen, ld < experts, an unknown type, or a workspace that "
+                  "is too small");
+  RouteParams p = route_params(d);
+  p.weights = weights; p.chosen = experts_out; p.rows = rows_out; p.slots = slots_out; p.offsets = offsets; p.balance = balance; p.stats = (float2*)stats; p.load = load;
+  p.counts = (int*)workspace; p.probs = (float*)((int*)workspace + (long long)p.blocks * (p.experts + 1));
+  BackToBack overlap;
+  return d->dtype == BB_DTYPE_BF16 ? route_fwd((const __nv_bfloat16*)logits, p, (cudaStream_t)stream) : route_fwd((const float*)logits, p, (cudaStream_t)stream);
+}
+
+extern "C" int bb_route_bwd(const bb_route_desc* d, const void* logits, const int* experts_out, const float* stats, const float* load,
+                            const float* d_weights, const float* d_balance, void* dlogits, long long ldd, int cols, void* stream) {
+  if (bad_route(d) || !logits || odd(logits, d->dtype == BB_DTYPE_F32 ? 3 : 1) || !experts_out || !stats || odd(stats, 7) || !load || !dlogits ||
+      odd(dlogits, d->dtype == BB_DTYPE_F32 ? 3 : 1) || cols < d->experts || ldd < cols)
+    return refuse("bb_route_bwd: null or misaligned pointer, a descriptor that bb_route_fwd refuses, cols < experts or ldd < cols");
+  RouteParams p = route_params(d);
+  p.chosen = const_cast<int*>(experts_out); p.stats = (float2*)stats; p.load = const_cast<float*>(load);
+  return d->dtype == BB_DTYPE_BF16 ? route_bwd((const __nv_bfloat16*)logits, p, d_weights, d_balance, (__nv_bfloat16*)dlogits, ldd, cols, (cudaStream_t)stream)
+                                   : route_bwd((const float*)logits, p, d_weights, d_balance, (float*)dlogits, ldd, cols, (cudaStream_t)stream);
+}
+
+extern "C" int bb_dispatch_rows(const void* x, long long ld, int dtype, const int* slots, int k, void* out, long long rows, long long tokens, int h,
+                                void* stream) {
+  if (bad_move(x, ld, dtype, slots, k, rows, tokens, h) || !out || odd(out, dtype == BB_DTYPE_F32 ? 3 : 1))
+    return refuse("bb_dispatch_rows: null or misaligned pointer, a size that is not positive, ld < h, or an unknown type");
+  return dtype == BB_DTYPE_BF16 ? dispatch((const __nv_bfloat16*)x, ld, slots, k, (__nv_bfloat16*)out, (int)rows, (int)tokens, h, (cudaStream_t)stream)
+                                : dispatch((const float*)x, ld, slots, k, (float*)out, (int)rows, (int)tokens, h, (cudaStream_t)stream);
+}
+
+extern "C" int bb_combine_rows(const void* x, long long ld, int dtype, const int* rows_of, const float* weights, const void* residual, long long ld_residual,
+                               int k, void* out, long long tokens, long long rows, int h, void* stream) {
+  const uintptr_t mask = dtype == BB_DTYPE_F32 ? 3 : 1;
+  if (bad_move(x, ld, dtype, rows_of, k, rows, tokens, h) || !out || odd(out, mask) || odd(weights, 3) || odd(residual, mask) || (residual && ld_residual < h))
+    return refuse("bb_combine_rows: null or misaligned pointer, a size that is not positive, ld < h, or an unknown type");
+  return dtype == BB_DTYPE_BF16 ? combine((const __nv_bfloat16*)x, ld, rows_of, weights, (const __nv_bfloat16*)residual, ld_residual, k, (__nv_bfloat16*)out, (int)tokens, (int)rows, h, (cudaStream_t)stream)
+                                : combine((const float*)x, ld, rows_of, weights, (const float*)residual, ld_residual, k, (float*)out, (int)tokens, (int)rows, h, (cudaStream_t)stream);
+}
+
+extern "C" int bb_combine_rows_bwd(const void* dy, long long ld_dy, int dtype, const void* x, long long ld, const int* rows_of, const int* slots,
+                                   const float* weights, int k, void* dx, float* d_weights, long long tokens, long long rows, int h,
+                                   void* stream) {
+  const uintptr_t mask = dtype == BB_DTYPE_F32 ? 3 : 1;
+  if (bad_move(dy, ld_dy, dtype, rows_of, k, rows, tokens, h) || rows > tokens * k || !slots || odd(slots, 3) || !weights || odd(weights, 3) || (!dx && !d_weights) || odd(dx, mask) ||
+      odd(d_weights, 3) || (d_weights && (!x || odd(x, mask) || ld < h)))
+    return refuse("bb_combine_rows_bwd: null or misaligned pointer, a size that is not positive, a leading dimension < h, or an unknown type");
+  return dtype == BB_DTYPE_BF16
+             ? combine_bwd((const __nv_bfloat16*)dy, ld_dy, (const __nv_bfloat16*)x, ld, rows_of, slots, weights, k, (__nv_bfloat16*)dx, d_weights, (int)tokens, (int)rows, h, (cudaStream_t)stream)
+             : combine_bwd((const float*)dy, ld_dy, (const float*)x, ld, rows_of, slots, weights, k, (float*)dx, d_weights, (int)tokens, (int)rows, h, (cudaStream_t)stream);
+}

@@ -1,0 +1,633 @@
+// Matrix products grouped by expert on the 5th-generation tensor cores.  Rows are sorted by expert: expert e owns rows
+// [offsets[e], offsets[e + 1]) of x and of y, and has a weight W_e [n, k] of its own.
+//
+//   rows (forward)    y[r] = W_e x[r] (+ b_e, GeLU)        A = x, B = W_e, reduction over k
+//   rows (input)      dx[r] = W_e^T dy[r] (* GeLU')        A = dy, B = W_e turned, reduction over n
+//   weight gradient   dW_e = sum over its rows of dy[r] x[r]^T   A = dy turned, B = x turned, reduction over the expert's rows
+//
+// The offsets are on the device and the host never reads them: a launch has as many CTAs as there may be tiles (at most one per SM),
+// and every warp walks the experts' tiles in the same order, unit after unit of its CTA's share.  No tile spans two experts.  A row
+// tile that overhangs its expert computes its neighbour's rows and does not store them.  In a weight gradient the overhang is part of
+// the reduction: where an expert ends inside a group of 16 rows (the reduction of one MMA), the neighbour's rows of that group are
+// overwritten with zeros in shared memory, in both operands, so that an infinity or NaN over there stays there.
+//
+// The main loop is that of the dense product (gemm_tcgen05.cu): two producer warps, one MMA warp, eight epilogue warps, six
+// stages of 32 KiB, two accumulators; pairs of CTAs (cta_group::2) on 256 x 256 tiles where the experts are large enough.
+#include "common.cuh"
+#include "bamboo_b200.h"
+#include "gemm_panels.cuh"
+#include "tma_host.cuh"
+#include <limits.h>
+
+namespace {
+
+constexpr int BM = 128, BK = 64, UMMA_K = 16;
+constexpr int TMA_WARP_0 = 0, MMA_WARP = 1, TMA_WARP_1 = 2, EPI_WARP = 3, EPI_WARPS = 8;
+constexpr int THREADS = 32 * (EPI_WARP + EPI_WARPS);
+constexpr int A_STAGE_BYTES = BM * BK * 2;
+constexpr int SLAB_BYTES = 32 * 128;
+constexpr int MAX_EXPERTS = 256;
+
+template <int BN, bool PAIR> struct Cfg {
+  static constexpr int B_ROWS = PAIR ? BN / 2 : BN;
+  static constexpr int B_STAGE_BYTES = B_ROWS * BK * 2;
+  static constexpr int STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
+  static constexpr int STAGES = B_ROWS == 256 ? 4 : B_ROWS == 128 ? 6 : 8;
+  static constexpr int TILE_M = PAIR ? 2 * BM : BM;
+  static constexpr int TMEM_COLS = 2 * BN;
+  static constexpr int BAR_BYTES = (3 * STAGES + 4) * 8 + 8;
+  static constexpr int TABLE_BYTES = (MAX_EXPERTS + 1) * 4 + MAX_EXPERTS;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * SLAB_BYTES + 1024 /*align slack*/ + BAR_BYTES + TABLE_BYTES;
+  static_assert(SMEM_BYTES <= 227 * 1024, "fits an SM");
+};
+
+struct GroupParams {
+  int rows;                   // of x and y
+  int n, k;                   // columns of the result, and the length of the reduction (weight gradient: rows and columns of dW_e)
+  int experts;
+  int epi;
+  const int* offsets;
+  void* D; void* D2; const void* bias; const void* aux;
+  long long ldd, ld_aux, expert_stride;       // expert_stride: values of one dW_e
+  int* status;
+};
+
+struct Unit {
+  int e, m0, n0;              // first row (a row of x, or of dW_e) and column of the tile
+  int end;                    // where its rows end
+  int k0, num_kb, tail;       // weight gradient: first row of the reduction, rows of the last k-block
+};
+
+// The units of a CTA (pair) one after the other: unit worker, worker + workers, ...
+template <bool WGRAD, int BN, int TILE_M> struct Walk {
+  const GroupParams& p;
+  const int* start;
+  const unsigned char* order;
+  int e, first, tiles, unit, step, cols, m_tiles;
+  __device__ __forceinline__ Walk(const GroupParams& p_, const int* s, const unsigned char* o, int worker, int workers)
+      : p(p_), start(s), order(o), e(-1), first(0), tiles(0), unit(worker - workers), step(workers), cols((p_.n + BN - 1) / BN), m_tiles(0) {
+    if constexpr (WGRAD) {
+      m_tiles = (p.n + TILE_M - 1) / TILE_M;
+      cols = (p.k + BN - 1) / BN;
+    }
+  }
+  __device__ __forceinline__ bool next(Unit& u) {
+    unit += step;
+    while (unit >= first + tiles) {
+      if (++e == p.experts) return false;
+      first += tiles;
+      if constexpr (!WGRAD) m_tiles = (start[e + 1] - start[e] + TILE_M - 1) / TILE_M;
+      tiles = m_tiles * cols;
+    }
+    const int local = unit - first, ni = local / m_tiles, mi = local - ni * m_tiles;
+    u.n0 = ni * BN;
+    if constexpr (WGRAD) {
+      u.e = order[e];
+      const int n = start[u.e + 1] - start[u.e];
+      u.m0 = mi * TILE_M; u.end = p.n;
+      u.k0 = start[u.e]; u.num_kb = (n + BK - 1) / BK; u.tail = n - (u.num_kb - 1) * BK;
+    } else {
+      u.e = e;
+      u.m0 = start[e] + mi * TILE_M; u.end = start[e + 1];
+      u.k0 = 0; u.num_kb = (p.k + BK - 1) / BK; u.tail = BK;
+    }
+    return true;
+  }
+};
+
+// Rows [from, to) of the reduction become zeros in `boxes` boxes of 64 columns (64 rows of 128 bytes each; the swizzle permutes 16-byte
+// chunks inside a row), by a whole warp.
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int boxes, int from, int to, int lane) {
+  const int chunks = (to - from) * 8;
+  for (int b = 0; b < boxes; ++b)
+    for (int i = lane; i < chunks; i += 32) *reinterpret_cast<uint4*>(tile + b * 8192 + from * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// Where every expert's rows begin, ascending within [0, rows]; by one warp.  Offsets that do not ascend set the status word and are cut.
+__device__ __forceinline__ void read_offsets(const GroupParams& p, int* start, int lane) {
+  int carry = 0;
+  bool bad = false;
+  for (int at = 0; at <= p.experts; at += 32) {
+    const int i = at + lane, raw = i <= p.experts ? __ldca(p.offsets + i) : INT_MIN;
+    int v = raw < 0 ? 0 : raw > p.rows ? p.rows : raw;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d && o > v) v = o;
+    }
+    if (v < carry) v = carry;
+    if (i <= p.experts) { start[i] = v; bad |= v != raw; }
+    carry = __shfl_sync(0xffffffffu, v, 31);
+  }
+  if (__any_sync(0xffffffffu, bad) && lane == 0 && p.status) atomicCAS(p.status, 0, BB_ERR_INVALID_ARG);
+}
+
+enum { ROWS = 0, ROWS_T = 1, WGRAD = 2 };     // B as stored, B turned, weight gradient
+
+template <int MODE, int BN, bool PAIR>
+__global__ void __launch_bounds__(THREADS, 1)
+grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GroupParams p) {
+  using C = Cfg<BN, PAIR>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + C::STAGES * A_STAGE_BYTES;
+  uint8_t* panels = smem + C::STAGES * C::STAGE_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(panels + EPI_WARPS * SLAB_BYTES);      // [STAGES]
+  uint64_t* empty_bar = full_bar + C::STAGES;       // [STAGES]
+  uint64_t* clean_bar = empty_bar + C::STAGES;      // [STAGES] pairs: the other CTA's overhanging rows are zeros
+  uint64_t* tmem_full = clean_bar + C::STAGES;      // [2]
+  uint64_t* tmem_empty = tmem_full + 2;             // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* start = reinterpret_cast<int*>(tmem_slot + 2);                                     // [experts + 1]
+  unsigned char* order = reinterpret_cast<unsigned char*>(start + MAX_EXPERTS + 1);       // [experts]
+
+  const int warp = bb::warp_index();
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? bb::cluster_ctarank() : 0u;
+  const int worker = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
+  const int workers = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < C::STAGES; ++s) { bb::mbar_init(&full_bar[s], 1); bb::mbar_init(&empty_bar[s], 1); bb::mbar_init(&clean_bar[s], 1); }
+    for (int a = 0; a < 2; ++a) { bb::mbar_init(&tmem_full[a], 1); bb::mbar_init(&tmem_empty[a], (PAIR ? 2 : 1) * EPI_WARPS); }
+    bb::fence_barrier_init();
+    bb::tma_prefetch_desc(&tmA);
+    bb::tma_prefetch_desc(&tmB);
+  }
+  if (warp == MMA_WARP) {
+    if (PAIR) { bb::tmem_alloc_pair(tmem_slot, C::TMEM_COLS); bb::tmem_relinquish_pair(); }
+    else { bb::tmem_alloc(tmem_slot, C::TMEM_COLS); bb::tmem_relinquish(); }
+  }
+  bb::pdl_sync();
+  if (warp == EPI_WARP) read_offsets(p, start, lane);
+  bb::tc_fence_before_sync();
+  if (PAIR) bb::cluster_sync();     // the peer's barriers are initialised before anything signals them
+  else __syncthreads();
+  bb::tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  if constexpr (MODE == WGRAD) {
+    // longest reductions first: the last units of a launch are then the short ones
+    for (int e = threadIdx.x; e < p.experts; e += THREADS) {
+      const int n = start[e + 1] - start[e];
+      int at = 0;
+      for (int i = 0; i < p.experts; ++i) {
+        const int o = start[i + 1] - start[i];
+        at += o > n || (o == n && i < e);
+      }
+      order[at] = (unsigned char)e;
+    }
+    __syncthreads();
+  } else {
+    // rows that belong to no expert
+    const int before = start[0], after = p.rows - start[p.experts], chunks = p.n >> 3;
+    for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < (long long)(before + after) * chunks; i += (long long)gridDim.x * THREADS) {
+      const int r = (int)(i / chunks), c = (int)(i - (long long)r * chunks);
+      reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.D) + (long long)(r < before ? r : start[p.experts] + r - before) * p.ldd)[c] =
+          make_uint4(0, 0, 0, 0);
+    }
+  }
+  Walk<MODE == WGRAD, BN, C::TILE_M> walk(p, start, order, worker, workers);
+  Unit u;
+
+  if (warp == TMA_WARP_0 || warp == TMA_WARP_1) {
+    // ------------------------------------------------ producers: the stages in turn
+    static_assert(C::STAGES % 2 == 0, "the producers take the stages in turn");
+    const int turn = warp == TMA_WARP_1 ? 1 : 0;
+    int s = 0; uint32_t phase = 0;
+    bool alive = true;
+    while (alive && walk.next(u)) {
+      const int m0 = u.m0 + (int)rank * BM, n0 = u.n0 + (int)rank * C::B_ROWS;
+      for (int kb = 0; kb < u.num_kb; ++kb) {
+        if ((s & 1) == turn) {
+          if (!bb::mbar_wait_warp(&empty_bar[s], phase ^ 1, abort_flag, p.status)) { alive = false; break; }
+          uint8_t* a = sA + s * A_STAGE_BYTES;
+          uint8_t* b = sB + s * C::B_STAGE_BYTES;
+          const int k0 = u.k0 + kb * BK;
+          // a stage whose last rows are to be zeroed completes in each CTA of a pair for itself
+          const bool own = !PAIR || (MODE == WGRAD && kb == u.num_kb - 1 && (u.tail & 15));
+          if (bb::elect_one()) {
+            uint32_t fb = bb::smem_u32(&full_bar[s]);
+            if (own) bb::mbar_arrive_expect_tx(&full_bar[s], C::STAGE_BYTES);
+            else {
+              if (rank == 0) bb::mbar_arrive_expect_tx(&full_bar[s], 2 * C::STAGE_BYTES);
+            }
+            if constexpr (PAIR) fb = bb::mapa_shared(fb, own ? rank : 0u);
+            auto load2 = [&](uint8_t* dst, const CUtensorMap* tm, int x, int y) {
+              if constexpr (PAIR) bb::tma_load_2d_pair(dst, tm, fb, x, y);
+              else bb::tma_load_2d(dst, tm, &full_bar[s], x, y);
+            };
+            auto load3 = [&](uint8_t* dst, const CUtensorMap* tm, int x, int y, int z) {
+              if constexpr (PAIR) bb::tma_load_3d_pair(dst, tm, fb, x, y, z);
+              else bb::tma_load_3d(dst, tm, &full_bar[s], x, y, z);
+            };
+            if constexpr (MODE == WGRAD) {
+#pragma unroll
+              for (int j = 0; j < BM / 64; ++j) load2(a + j * 8192, &tmA, m0 + 64 * j, k0);
+#pragma unroll
+              for (int j = 0; j < C::B_ROWS / 64; ++j) load2(b + j * 8192, &tmB, n0 + 64 * j, k0);
+            } else {
+              load2(a, &tmA, k0, m0);
+              if constexpr (MODE == ROWS) {
+                load3(b, &tmB, k0, n0, u.e);
+              } else {
+#pragma unroll
+                for (int j = 0; j < C::B_ROWS / 64; ++j) load3(b + j * 8192, &tmB, n0 + 64 * j, k0, u.e);
+              }
+            }
+          }
+          __syncwarp();
+        }
+        if (++s == C::STAGES) { s = 0; phase ^= 1; }
+      }
+    }
+    if constexpr (PAIR) {
+      // rank 0's commits arrive on this CTA's barriers too: none may still be on its way when the CTA leaves
+      for (int i = 0; i < C::STAGES && alive; ++i) {
+        if ((s & 1) == turn && !bb::mbar_wait_warp(&empty_bar[s], phase ^ 1, abort_flag, p.status)) alive = false;
+        if (++s == C::STAGES) { s = 0; phase ^= 1; }
+      }
+    }
+    if (!alive) {
+      // copies still in flight get time to land (bounded)
+      const uint64_t t0 = bb::globaltimer_ns();
+      while (bb::globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    }
+  } else if (warp == MMA_WARP) {
+    // ------------------------------------------------ MMA issuer (pairs: rank 0; the other CTA's only cleans its stages)
+    constexpr uint32_t A_MN = MODE == WGRAD, B_MN = MODE != ROWS;
+    constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | (A_MN << 15) | (B_MN << 16) | ((uint32_t)(BN >> 3) << 17) |
+                               ((uint32_t)(C::TILE_M >> 4) << 24);
+    constexpr uint32_t A_LBO = A_MN ? 8192u : 16u, B_LBO = B_MN ? 8192u : 16u, A_STEP = A_MN ? 2048u : 32u, B_STEP = B_MN ? 2048u : 32u;
+    int s = 0; uint32_t phase = 0, clean_phase = 0;
+    int acc = 0; uint32_t acc_phase = 0;
+    bool alive = true;
+    auto clean = [&](int stage, int tail) {
+      zero_rows(sA + stage * A_STAGE_BYTES, BM / 64, tail, (tail + 15) & ~15, lane);
+      zero_rows(sB + stage * C::B_STAGE_BYTES, C::B_ROWS / 64, tail, (tail + 15) & ~15, lane);
+      bb::fence_proxy_async();
+      __syncwarp();
+    };
+    while (alive && walk.next(u)) {
+      if (u.num_kb == 0) continue;             // an expert without rows: the epilogue writes its zeros
+      const bool ragged = MODE == WGRAD && (u.tail & 15);
+      if (PAIR && rank == 1) {
+        if (ragged) {
+          const int st = (s + u.num_kb - 1) % C::STAGES;
+          if (!bb::mbar_wait_warp(&full_bar[st], (clean_phase >> st) & 1u, abort_flag, p.status)) { alive = false; break; }
+          clean_phase ^= 1u << st;
+          clean(st, u.tail);
+          if (lane == 0) bb::mbar_arrive_cluster(bb::mapa_shared(bb::smem_u32(&clean_bar[st]), 0));
+        }
+        s = (s + u.num_kb) % C::STAGES;
+        continue;
+      }
+      if (!bb::mbar_wait_warp(&tmem_empty[acc], acc_phase ^ 1, abort_flag, p.status)) { alive = false; break; }
+      bb::tc_fence_after_sync();
+      const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
+      for (int kb = 0; kb < u.num_kb; ++kb) {
+        if (!bb::mbar_wait_warp(&full_bar[s], phase, abort_flag, p.status)) { alive = false; break; }
+        int steps = BK / UMMA_K;
+        if (MODE == WGRAD && kb == u.num_kb - 1) {
+          steps = (u.tail + 15) >> 4;
+          if (ragged) {
+            clean(s, u.tail);
+            if constexpr (PAIR) {
+              const bool got = bb::mbar_wait_cluster(&clean_bar[s], (clean_phase >> s) & 1u, abort_flag, p.status);
+              if (!__all_sync(0xffffffffu, got)) { alive = false; break; }
+              clean_phase ^= 1u << s;
+            }
+          }
+        }
+        bb::tc_fence_after_sync();
+        if (bb::elect_one()) {
+          const uint64_t ad0 = bb::make_smem_desc_sw128(bb::smem_u32(sA + s * A_STAGE_BYTES), A_LBO, 1024u);
+          const uint64_t bd0 = bb::make_smem_desc_sw128(bb::smem_u32(sB + s * C::B_STAGE_BYTES), B_LBO, 1024u);
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k) {
+            if (MODE == WGRAD && k >= steps) break;
+            const uint64_t ad = ad0 + (uint64_t)(k * (A_STEP >> 4)), bd = bd0 + (uint64_t)(k * (B_STEP >> 4));
+            if (PAIR) bb::umma_f16_pair(d_tmem, ad, bd, IDESC, (kb > 0 || k > 0) ? 1u : 0u);
+            else bb::umma_f16(d_tmem, ad, bd, IDESC, (kb > 0 || k > 0) ? 1u : 0u);
+          }
+          if (PAIR) {
+            bb::umma_commit_pair(&empty_bar[s], 3);
+            if (kb == u.num_kb - 1) bb::umma_commit_pair(&tmem_full[acc], 3);
+          } else {
+            bb::umma_commit(&empty_bar[s]);
+            if (kb == u.num_kb - 1) bb::umma_commit(&tmem_full[acc]);
+          }
+        }
+        __syncwarp();
+        if (++s == C::STAGES) { s = 0; phase ^= 1; }
+      }
+      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+    }
+  } else {
+    // ------------------------------------------------ epilogue: eight warps, two per TMEM lane quarter, panels of 128 bytes in turn
+    const int eg = (warp - EPI_WARP) >> 2, quarter = warp & 3;
+    const int epi = p.epi;
+    const bool f32 = MODE == WGRAD && epi == BB_EPI_ACCUM_F32, dual = MODE == ROWS && epi == BB_EPI_BIAS_GELU;
+    const bool has_aux = MODE == ROWS_T && epi == BB_EPI_MUL_DGELU, has_bias = MODE == ROWS && (epi == BB_EPI_BIAS || dual);
+    const int cols = MODE == WGRAD ? p.k : p.n;
+    uint8_t* slab = panels + (warp - EPI_WARP) * SLAB_BYTES;
+    int acc = 0; uint32_t acc_phase = 0;
+    bool alive = true;
+    while (alive && walk.next(u)) {
+      const int r0 = u.m0 + (int)rank * BM + quarter * 32, n0 = u.n0;
+      const bool none = MODE == WGRAD && u.num_kb == 0;
+      if (none && f32) continue;               // nothing to add
+      uint32_t t_row = 0;
+      if (!none) {
+        if (!bb::mbar_wait_warp(&tmem_full[acc], acc_phase, abort_flag, p.status)) { alive = false; break; }
+        bb::tc_fence_after_sync();
+        t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN);
+      }
+      const int width = f32 ? 32 : 64, npanels = BN / width;
+      const long long base = MODE == WGRAD ? u.e * p.expert_stride : 0;
+      const __nv_bfloat16* bias = has_bias ? reinterpret_cast<const __nv_bfloat16*>(p.bias) + (long long)u.e * p.n : nullptr;
+      bool handed = none;
+#pragma unroll 1
+      for (int pn = eg; pn < npanels; pn += 2) {
+        const int nb = n0 + pn * width;
+        const bool some = nb < cols && r0 < u.end;
+        if (has_aux && some) {
+          uint4 ax[8];
+          slab_fetch_bf16(reinterpret_cast<const __nv_bfloat16*>(p.aux), p.ld_aux, r0, nb, u.end, cols, lane, ax);
+          slab_put(slab, lane, ax);
+        }
+        float v[64];
+        if (none) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) v[i] = 0.f;
+        } else {
+          uint32_t r[32];
+          bb::tmem_ld_32x32b_x32(t_row + pn * width, r);
+          bb::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+          if (!f32) {
+            bb::tmem_ld_32x32b_x32(t_row + pn * width + 32, r);
+            bb::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[32 + i] = __uint_as_float(r[i]);
+          }
+        }
+        if (pn + 2 >= npanels && !handed) {
+          // this warp has read its share of the accumulator
+          bb::tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {
+            if (PAIR) bb::mbar_arrive_cluster_relaxed(bb::mapa_shared(bb::smem_u32(&tmem_empty[acc]), 0));
+            else bb::mbar_arrive(&tmem_empty[acc]);
+          }
+          handed = true;
+        }
+        if (!some) continue;
+        if (f32) {
+          panel_store_row_f32(slab, lane, v);
+          __syncwarp();
+          slab_flush_f32<true>(slab, reinterpret_cast<float*>(p.D) + base, p.ldd, r0, nb, u.end, cols, lane);
+          __syncwarp();
+          continue;
+        }
+        if (has_bias) {
+          if (nb + 64 <= cols) {
+#pragma unroll
+            for (int i = 0; i < 64; i += 8) {
+              float f[8]; unpack8(__ldg(reinterpret_cast<const uint4*>(bias + nb + i)), f);
+#pragma unroll
+              for (int k = 0; k < 8; k += 2) set2(v + i + k, bb::add2(get2(v + i + k), make_float2(f[k], f[k + 1])));
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) if (nb + i < cols) v[i] += __bfloat162float(bias[nb + i]);
+          }
+        }
+        if (dual) {
+          panel_store_row_bf16(slab, lane, v);     // pre-activation first
+          __syncwarp();
+          slab_flush_bf16(slab, reinterpret_cast<__nv_bfloat16*>(p.D2), p.ldd, r0, nb, u.end, cols, lane);
+          // (of the sum itself: its rounding above is for the backward pass alone)
+#pragma unroll
+          for (int i = 0; i < 64; i += 2) set2(v + i, bb::gelu_tanh2(get2(v + i)));
+          __syncwarp();
+        } else if (has_aux) {
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float x[32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) unpack8(*reinterpret_cast<const uint4*>(slab + slab_off(lane, 4 * h + c)), x + 8 * c);
+            apply_aux<32>(epi, v + 32 * h, x);
+          }
+          __syncwarp();
+        }
+        panel_store_row_bf16(slab, lane, v);
+        __syncwarp();
+        slab_flush_bf16(slab, reinterpret_cast<__nv_bfloat16*>(p.D) + base, p.ldd, r0, nb, u.end, cols, lane);
+        __syncwarp();
+      }
+      if constexpr (BN == 64) {
+        if (!handed) {                          // one panel: the second warp of the quarter has none to read
+          if (lane == 0) bb::mbar_arrive(&tmem_empty[acc]);
+        }
+      }
+      if (!none && ++acc == 2) { acc = 0; acc_phase ^= 1; }
+    }
+  }
+
+  bb::tc_fence_before_sync();
+  if (PAIR) {
+    // neither CTA leaves (or frees TMEM) while the other may still signal its barriers
+    __syncwarp();
+    bb::cluster_sync();
+    if (warp == MMA_WARP) bb::tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
+  } else {
+    __syncthreads();
+    if (warp == MMA_WARP) bb::tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------- bias gradients
+// db_e = sum of its rows of dy.  A CTA sums up to COLSUM_ROWS rows of one expert over 256 columns (eight warps, a row each at a time)
+// and leaves them as fp32; a second kernel adds an expert's pieces in their order.
+constexpr int COLSUM_ROWS = 256;
+
+__device__ __forceinline__ int clamped(const int* offsets, int e, int rows) {
+  const int v = __ldca(offsets + e);
+  return v < 0 ? 0 : v > rows ? rows : v;
+}
+
+// Piece `at` of the list of all experts' pieces: its expert and rows; false behind the last.  Every piece belongs to one expert.
+struct Piece { int e, from, to; };
+__device__ __forceinline__ bool find_piece(const int* offsets, int experts, int rows, int at, Piece& q) {
+  int lo = clamped(offsets, 0, rows);
+  for (int e = 0; e < experts; ++e) {
+    int hi = clamped(offsets, e + 1, rows);
+    if (hi < lo) hi = lo;
+    const int pieces = (hi - lo + COLSUM_ROWS - 1) / COLSUM_ROWS;
+    if (at < pieces) {
+      q.e = e; q.from = lo + at * COLSUM_ROWS; q.to = q.from + COLSUM_ROWS < hi ? q.from + COLSUM_ROWS : hi;
+      return true;
+    }
+    at -= pieces;
+    lo = hi;
+  }
+  return false;
+}
+
+__global__ void __launch_bounds__(256)
+grouped_colsum_kernel(const __nv_bfloat16* dy, long long ld, const int* offsets, int experts, int rows, int n, float* partial) {
+  __shared__ float sums[8][256];
+  bb::pdl_sync();
+  Piece q;
+  if (!find_piece(offsets, experts, rows, blockIdx.y, q)) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 256 + lane * 8;
+  float v[8] = {};
+  if (col < n) {
+    for (int r = q.from + warp; r < q.to; r += 8) {
+      float f[8];
+      unpack8(__ldca(reinterpret_cast<const uint4*>(dy + (long long)r * ld + col)), f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += f[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sums[warp][lane * 8 + i] = v[i];
+  __syncthreads();
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= n) return;
+  float s = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) s += sums[w][threadIdx.x];
+  partial[(long long)blockIdx.y * n + c] = s;
+}
+
+__global__ void __launch_bounds__(256)
+grouped_colsum_join_kernel(const float* partial, const int* offsets, int rows, int n, __nv_bfloat16* out, float* accum) {
+  bb::pdl_sync();
+  const int c = blockIdx.x * 256 + threadIdx.x, e = blockIdx.y;
+  int first = 0, lo = clamped(offsets, 0, rows), hi = lo;
+  for (int i = 0; i <= e; ++i) {
+    lo = hi;
+    hi = clamped(offsets, i + 1, rows);
+    if (hi < lo) hi = lo;
+    if (i < e) first += (hi - lo + COLSUM_ROWS - 1) / COLSUM_ROWS;
+  }
+  if (c >= n) return;
+  const int pieces = (hi - lo + COLSUM_ROWS - 1) / COLSUM_ROWS;
+  float s = 0.f;
+  for (int i = 0; i < pieces; ++i) s += partial[(long long)(first + i) * n + c];
+  if (accum) accum[(long long)e * n + c] += s;
+  else out[(long long)e * n + c] = __float2bfloat16(s);
+}
+
+// ---------------------------------------------------------------- host side
+int refuse(const char* msg) { bb_set_last_error_msg(msg); return BB_ERR_INVALID_ARG; }
+
+template <int MODE, int BN, bool PAIR>
+int launch(const bb_grouped_desc* d, cudaStream_t stream) {
+  using C = Cfg<BN, PAIR>;
+  CUtensorMap tmA, tmB;
+  GroupParams p = {};
+  p.rows = d->rows; p.experts = d->experts; p.epi = d->epilogue; p.offsets = d->offsets;
+  p.D = d->out; p.D2 = d->out2; p.bias = d->bias; p.aux = d->aux;
+  p.ldd = d->ld_out; p.ld_aux = d->ld_aux ? d->ld_aux : d->ld_out;
+  p.status = bb_device_status_word();
+  int rc;
+  long long tiles;
+  const long long row_tiles = (long long)d->rows / C::TILE_M + (d->rows < d->experts ? d->rows : d->experts);      // at most
+  if (MODE == WGRAD) {
+    p.n = d->n; p.k = d->k; p.expert_stride = (long long)d->n * d->k; p.ldd = d->k;
+    rc = bbhost::encode_2d(&tmA, d->x, d->rows, d->n, d->ld_x, 64, BK);
+    if (!rc) rc = bbhost::encode_2d(&tmB, d->weight, d->rows, d->k, d->ld_weight, 64, BK);
+    tiles = (long long)d->experts * ((d->n + C::TILE_M - 1) / C::TILE_M) * ((d->k + BN - 1) / BN);
+  } else {
+    p.n = MODE == ROWS ? d->n : d->k; p.k = MODE == ROWS ? d->k : d->n;
+    rc = bbhost::encode_2d(&tmA, d->x, d->rows, p.k, d->ld_x, BK, BM);
+    // (the third dimension ends every expert's weight: what a box reads beyond it is zeros)
+    if (!rc) rc = bbhost::encode_seqs(&tmB, d->weight, d->experts, d->n, d->k, d->k, 64, MODE == ROWS ? C::B_ROWS : BK);
+    tiles = row_tiles * ((p.n + BN - 1) / BN);
+  }
+  if (rc) return rc;
+  if (tiles > INT_MAX / 2) return refuse("bb_grouped_gemm: more tiles than one launch covers");
+  BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(grouped_gemm_kernel<MODE, BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES)));
+  int workers = PAIR ? bb_num_sms() / 2 : bb_num_sms();
+  if (d->max_ctas > 0 && d->max_ctas / (PAIR ? 2 : 1) < workers) workers = d->max_ctas / (PAIR ? 2 : 1);
+  if (workers < 1) workers = 1;
+  if (d->max_ctas < 0 || tiles < workers) workers = tiles < 1 ? 1 : (int)tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((PAIR ? 2 : 1) * workers); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = C::SMEM_BYTES; cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr; cfg.numAttrs = 0;
+  if (bb_back_to_back > 0) cfg.numAttrs = 1;
+  if (PAIR) {
+    if (!cfg.numAttrs) attr[0] = attr[1];
+    ++cfg.numAttrs;
+  }
+  BB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, grouped_gemm_kernel<MODE, BN, PAIR>, tmA, tmB, p));
+  return BB_OK;
+}
+
+template <int MODE> int choose(const bb_grouped_desc* d, cudaStream_t stream) {
+  return launch<MODE, 128, false>(d, stream);
+}
+
+bool bad_sizes(const bb_grouped_desc* d) {
+  return d->rows <= 0 || d->n <= 0 || d->k <= 0 || (d->n & 7) || (d->k & 7) || d->experts <= 0 || d->experts > MAX_EXPERTS;
+}
+bool bad_matrix(const void* p, long long ld, int cols) { return !p || ((uintptr_t)p & 15) || ld < cols || (ld & 7); }
+}  // namespace
+
+extern "C" int bb_grouped_max_experts(void) { return MAX_EXPERTS; }
+
+extern "C" int bb_grouped_gemm(const bb_grouped_desc* d, void* stream) {
+  if (!d || !d->offsets || ((uintptr_t)d->offsets & 3) || bad_sizes(d))
+    return refuse("bb_grouped_gemm: null pointer, a size that is not positive, n or k not a multiple of 8, or more than 256 experts");
+  if (int rc = bbhost::bind_context()) return rc;
+  const bool turned = d->mode == BB_GROUPED_INPUT, wgrad = d->mode == BB_GROUPED_WEIGHT;
+  if (d->mode != BB_GROUPED_ROWS && !turned && !wgrad) return refuse("bb_grouped_gemm: an unknown mode");
+  if (bad_matrix(d->x, d->ld_x, d->mode == BB_GROUPED_ROWS ? d->k : d->n) || bad_matrix(d->weight, wgrad ? d->ld_weight : d->k, d->k) || !d->out ||
+      ((uintptr_t)d->out & 15) || (!wgrad && bad_matrix(d->out, d->ld_out, turned ? d->k : d->n)))
+    return refuse("bb_grouped_gemm: operands are 16-byte aligned, with rows of a multiple of 8 values that do not overlap");
+  const int e = d->epilogue;
+  if (wgrad ? (e != BB_EPI_STORE && e != BB_EPI_ACCUM_F32)
+            : turned ? (e != BB_EPI_STORE && e != BB_EPI_MUL_DGELU) : (e != BB_EPI_STORE && e != BB_EPI_BIAS && e != BB_EPI_BIAS_GELU))
+    return refuse("bb_grouped_gemm: an epilogue that this product does not have");
+  if (!wgrad && !turned && e != BB_EPI_STORE && (!d->bias || ((uintptr_t)d->bias & 15)))
+    return refuse("bb_grouped_gemm: the epilogue takes a bias, 16-byte aligned");
+  if (e == BB_EPI_BIAS_GELU && (!d->out2 || ((uintptr_t)d->out2 & 15))) return refuse("bb_grouped_gemm: the epilogue takes a second output, 16-byte aligned");
+  if (e == BB_EPI_MUL_DGELU && bad_matrix(d->aux, d->ld_aux ? d->ld_aux : d->ld_out, d->k))
+    return refuse("bb_grouped_gemm: the epilogue takes the pre-activation, 16-byte aligned");
+  cudaStream_t s = (cudaStream_t)stream;
+  return wgrad ? choose<WGRAD>(d, s) : turned ? choose<ROWS_T>(d, s) : choose<ROWS>(d, s);
+}
+
+namespace {
+long long colsum_pieces(int rows, int experts) { return (long long)rows / COLSUM_ROWS + (rows < experts ? rows : experts); }
+}  // namespace
+
+extern "C" long long bb_grouped_colsum_workspace_bytes(int rows, int n, int experts) {
+  return rows <= 0 || n <= 0 || experts <= 0 ? 0 : colsum_pieces(rows, experts) * n * 4;
+}
+
+extern "C" int bb_grouped_colsum(const void* dy, long long ld, const int* offsets, int experts, void* out_bf16, float* accum, void* workspace,
+                                 long long workspace_bytes, int rows, int n, void* stream) {
+  if (rows <= 0 || n <= 0 || (n & 7) || experts <= 0 || experts > MAX_EXPERTS || !offsets || bad_matrix(dy, ld, n) || (!out_bf16 == !accum) || !workspace ||
+      ((uintptr_t)workspace & 15) || workspace_bytes < bb_grouped_colsum_workspace_bytes(rows, n, experts))
+    return refuse("bb_grouped_colsum: null or misaligned pointer, a size that is not positive or no multiple of 8, or a workspace that is too small");
+  const long long pieces = colsum_pieces(rows, experts);
+  if (pieces > 65535) return refuse("bb_grouped_colsum: more rows than one launch covers");
+  BackToBack overlap;
+  BB_CUDA_CHECK(bb_launch(grouped_colsum_kernel, dim3((n + 255) / 256, (unsigned)pieces), 256, 0, (cudaStream_t)stream, (const __nv_bfloat16*)dy, ld, offsets, experts,
+                          rows, n, (float*)workspace));
+  BB_CUDA_CHECK(bb_launch(grouped_colsum_join_kernel, dim3((n + 255) / 256, (unsigned)experts), 256, 0, (cudaStream_t)stream, (const float*)workspace, offsets, rows, n,
+                          (__nv_bfloat16*)out_bf16, accum));
+  return BB_OK;
+}

@@ -1540,14 +1540,14 @@ extern "C" long long bb_grad_norm_workspace_bytes(void) { return 8LL * (2 + NORM
 
 namespace {
 // Sum of squares of the list into the workspace's first value
-int list_sumsq(const bb_grad_tensor* tensors, int count, double* workspace, cudaStream_t s, const ClipTo& clip = {}) {
+int list_sumsq(const bb_grad_tensor* tensors, int count, double* workspace, cudaStream_t s, const ClipTo& clip = {}, bool add = false) {
   for (int at = 0; at < count; at += LIST_TENSORS) {
     const int n = count - at < LIST_TENSORS ? count - at : LIST_TENSORS;
     TensorTable t;
     const int pieces = table_fill(t, tensors + at, n, sum_piece(tensors + at, n));
     unsigned int* done = norm_done(s);
     if (!done) { bb_set_last_error_msg("bb_grad_sumsq: counters unavailable on this device"); return BB_ERR_CUDA; }
-    BB_CUDA_CHECK(bb_launch(grad_sumsq_kernel, pieces < NORM_CTAS ? pieces : NORM_CTAS, NORM_THREADS, 0, s, t, workspace + 2, workspace, at > 0 ? 1 : 0, done,
+    BB_CUDA_CHECK(bb_launch(grad_sumsq_kernel, pieces < NORM_CTAS ? pieces : NORM_CTAS, NORM_THREADS, 0, s, t, workspace + 2, workspace, add || at > 0 ? 1 : 0, done,
                             at + n < count ? ClipTo{} : clip));
   }
   return BB_OK;
@@ -1560,6 +1560,21 @@ int clip_front(const bb_grad_tensor* tensors, int count, const double* sumsq, do
 }
 bool bad_workspace(const void* workspace, long long bytes) { return !workspace || ((uintptr_t)workspace & 7) || bytes < bb_grad_norm_workspace_bytes(); }
 }  // namespace
+
+// The clipping coefficient for a list of parameters (bb_adamw_list): into the workspace's second value
+int bb_list_clip_coef(const bb_adamw_tensor* tensors, int count, const double* sumsq, double grad_scale, double max_norm, float* norm, void* workspace,
+                      cudaStream_t s) {
+  double* ws = (double*)workspace;
+  const ClipTo clip = {grad_scale, max_norm, (float*)(ws + 1), norm};
+  if (sumsq) return clip_front(nullptr, 0, sumsq, ws, clip, s);
+  for (int at = 0; at < count; at += LIST_TENSORS) {
+    bb_grad_tensor list[LIST_TENSORS];
+    const int n = count - at < LIST_TENSORS ? count - at : LIST_TENSORS;
+    for (int i = 0; i < n; ++i) list[i] = {tensors[at + i].grad, tensors[at + i].numel, tensors[at + i].grad_dtype};
+    if (int rc = list_sumsq(list, n, ws, s, at + n < count ? ClipTo{} : clip, at > 0)) return rc;
+  }
+  return BB_OK;
+}
 
 extern "C" int bb_grad_sumsq(const bb_grad_tensor* tensors, int count, void* workspace, long long workspace_bytes, void* stream) {
   if (bad_list(tensors, count) || bad_workspace(workspace, workspace_bytes))

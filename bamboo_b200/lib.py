@@ -89,6 +89,29 @@ class HeadDesc(ctypes.Structure):
     ]
 
 
+class GroupedDesc(ctypes.Structure):
+    """bb_grouped_desc: a product with a weight per expert (see include/bamboo_b200.h)."""
+    _fields_ = [
+        ("mode", ctypes.c_int), ("rows", ctypes.c_int), ("n", ctypes.c_int), ("k", ctypes.c_int), ("experts", ctypes.c_int),
+        ("epilogue", ctypes.c_int), ("offsets", ctypes.c_void_p),
+        ("x", ctypes.c_void_p), ("ld_x", ctypes.c_longlong),
+        ("weight", ctypes.c_void_p), ("ld_weight", ctypes.c_longlong),
+        ("out", ctypes.c_void_p), ("ld_out", ctypes.c_longlong),
+        ("bias", ctypes.c_void_p), ("out2", ctypes.c_void_p),
+        ("aux", ctypes.c_void_p), ("ld_aux", ctypes.c_longlong),
+        ("max_ctas", ctypes.c_int),
+    ]
+
+
+class RouteDesc(ctypes.Structure):
+    """bb_route_desc: tokens, experts and how many are chosen (see include/bamboo_b200.h)."""
+    _fields_ = [
+        ("tokens", ctypes.c_int), ("experts", ctypes.c_int), ("k", ctypes.c_int), ("normalize", ctypes.c_int), ("dtype", ctypes.c_int),
+        ("ld", ctypes.c_longlong),
+    ]
+
+
+GROUPED_ROWS, GROUPED_INPUT, GROUPED_WEIGHT = 0, 1, 2
 PREFERENCE_FORMS = {"sigmoid": 0, "hinge": 1, "squared": 2}
 POLICY_REDUCTIONS = {"token": 0, "sequence": 1}
 
@@ -150,6 +173,16 @@ def load():
         lib.bb_grad_sumsq.argtypes = [vp, i, vp, ll, vp]
         lib.bb_grad_clip.argtypes = [vp, i, vp, d, vp, vp, ll, vp]
         lib.bb_adam_step_clipped.argtypes = [vp] * 5 + [ll, d, d, d, d, i, i, i, d, d, i, vp, d, vp, vp, ll, vp]
+        lib.bb_grouped_gemm.argtypes = [vp, vp]
+        lib.bb_grouped_colsum_workspace_bytes.restype = ll
+        lib.bb_grouped_colsum.argtypes = [vp, ll, vp, i, vp, vp, vp, ll, i, i, vp]
+        lib.bb_route_workspace_bytes.restype = ll
+        lib.bb_route_fwd.argtypes = [vp] * 11 + [ll, vp]
+        lib.bb_route_bwd.argtypes = [vp] * 8 + [ll, i, vp]
+        lib.bb_dispatch_rows.argtypes = [vp, ll, i, vp, i, vp, ll, ll, i, vp]
+        lib.bb_combine_rows.argtypes = [vp, ll, i, vp, vp, vp, ll, i, vp, ll, ll, i, vp]
+        lib.bb_combine_rows_bwd.argtypes = [vp, ll, i, vp, ll, vp, vp, vp, i, vp, vp, ll, ll, i, vp]
+        lib.bb_adamw_list.argtypes = [vp, i, d, d, d, d, ll, d, d, i, d, vp, vp, vp, ll, vp]
         _lib = lib
     return _lib
 
@@ -779,3 +812,96 @@ def adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, *, lr, beta1=
                                       lr, beta1, beta2, eps, step, int(adam_w_mode), int(bias_correction), weight_decay, grad_scale, int(zero_grad),
                                       _addr(sumsq), max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream()), "bb_adam_step_clipped")
     return norm
+
+
+# ---------------------------------------------------------------------------- mixture of experts
+def grouped_gemm(mode, x, weight, offsets, out, *, epilogue=EPI_STORE, bias=None, out2=None, aux=None, max_ctas=0):
+    """GROUPED_ROWS: x [rows, k], weight [experts, n, k], out [rows, n]; GROUPED_INPUT: x [rows, n], out [rows, k]; GROUPED_WEIGHT: x [rows, n],
+    weight [rows, k], out [experts, n, k].  2-D tensors have unit inner stride, rows on 16 bytes; see bb_grouped_gemm."""
+    global LAUNCHES
+    LAUNCHES += 1
+    wgrad = mode == GROUPED_WEIGHT
+    experts, n, k = out.shape if wgrad else weight.shape
+    d = GroupedDesc(mode=mode, rows=x.shape[0], n=n, k=k, experts=experts, epilogue=epilogue, offsets=offsets.data_ptr(), x=x.data_ptr(),
+                    ld_x=_ld(x), weight=weight.data_ptr(), ld_weight=_ld(weight) if wgrad else 0, out=out.data_ptr(),
+                    ld_out=0 if wgrad else _ld(out), bias=_addr(bias), out2=_addr(out2), aux=_addr(aux), ld_aux=0 if aux is None else _ld(aux),
+                    max_ctas=max_ctas or GEMM_MAX_CTAS)
+    check((_lib or load()).bb_grouped_gemm(ctypes.byref(d), _raw_stream()), "bb_grouped_gemm")
+    return out
+
+
+def grouped_colsum(dy, offsets, experts, out=None, accum=None):
+    """out [experts, n] (bf16) = column sums of every expert's rows of dy [rows, n], or accum (fp32) += them."""
+    global LAUNCHES
+    LAUNCHES += 2
+    lib = load()
+    rows, n = dy.shape
+    ws = workspace(lib.bb_grouped_colsum_workspace_bytes(rows, n, experts), "experts")
+    check(lib.bb_grouped_colsum(dy.data_ptr(), _ld(dy), offsets.data_ptr(), experts, _addr(out), _addr(accum), ws.data_ptr(), ws.numel(), rows, n,
+                                _raw_stream()), "bb_grouped_colsum")
+
+
+def route_fwd(desc, logits, weights, experts, rows, slots, offsets, balance, stats, load_):
+    global LAUNCHES
+    LAUNCHES += 2
+    lib = load()
+    ws = workspace(_bytes_of(desc, lib.bb_route_workspace_bytes), "experts")
+    check(lib.bb_route_fwd(ctypes.byref(desc), logits.data_ptr(), weights.data_ptr(), experts.data_ptr(), rows.data_ptr(), slots.data_ptr(),
+                           offsets.data_ptr(), balance.data_ptr(), stats.data_ptr(), load_.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream()),
+          "bb_route_fwd")
+
+
+def route_bwd(desc, logits, experts, stats, load_, d_weights, d_balance, dlogits):
+    global LAUNCHES
+    LAUNCHES += 1
+    check((_lib or load()).bb_route_bwd(ctypes.byref(desc), logits.data_ptr(), experts.data_ptr(), stats.data_ptr(), load_.data_ptr(), _addr(d_weights),
+                                        _addr(d_balance), dlogits.data_ptr(), _ld(dlogits), dlogits.shape[-1], _raw_stream()), "bb_route_bwd")
+    return dlogits
+
+
+def dispatch_rows(x, ld, slots, k, out, tokens):
+    """out [rows, h] from x (``tokens`` rows of ``ld`` values): the token of every slot, zeros where there is none."""
+    global LAUNCHES
+    LAUNCHES += 1
+    check((_lib or load()).bb_dispatch_rows(x.data_ptr(), ld, _dtype(x, "x"), slots.data_ptr(), k, out.data_ptr(), out.shape[0], tokens, out.shape[1],
+                                            _raw_stream()), "bb_dispatch_rows")
+    return out
+
+
+def combine_rows(x, ld, rows_of, weights, residual, ld_residual, k, out, tokens, rows, h):
+    """out [tokens, h] = residual + weighted sums of rows of x (``rows`` rows of ``ld`` values); weights None: 1, residual None: 0."""
+    global LAUNCHES
+    LAUNCHES += 1
+    check((_lib or load()).bb_combine_rows(x.data_ptr(), ld, _dtype(x, "x"), rows_of.data_ptr(), _addr(weights), _addr(residual), ld_residual, k,
+                                           out.data_ptr(), tokens, rows, h, _raw_stream()), "bb_combine_rows")
+    return out
+
+
+def combine_rows_bwd(dy, ld_dy, x, ld, rows_of, slots, weights, k, dx, d_weights, tokens, rows, h):
+    global LAUNCHES
+    LAUNCHES += 1
+    check((_lib or load()).bb_combine_rows_bwd(dy.data_ptr(), ld_dy, _dtype(dy, "gradient"), _addr(x), ld, rows_of.data_ptr(), slots.data_ptr(),
+                                               weights.data_ptr(), k, _addr(dx), _addr(d_weights), tokens, rows, h, _raw_stream()), "bb_combine_rows_bwd")
+
+
+# ---------------------------------------------------------------------------- optimizer over a list
+ADAMW_LIST = 64         # tensors of one launch
+
+
+@functools.lru_cache(maxsize=None)
+def _adamw_table(n):
+    return struct.Struct("QQQQQQqiI" * n)        # bb_adamw_tensor[n]
+
+
+def adamw_tensors(fields, count):
+    """bb_adamw_tensor[count] from (param, master, gradient, exp_avg, exp_avg_sq, scales, elements, type of the gradient, 0) of every tensor."""
+    return _adamw_table(count).pack(*fields)
+
+
+def adamw_list(table, count, *, lr, beta1, beta2, eps, step, weight_decay, grad_scale, zero_grad, max_norm, sumsq, norm):
+    global LAUNCHES
+    clip = max_norm > 0
+    LAUNCHES += -(-count // ADAMW_LIST) + (0 if not clip else 1 if sumsq is not None else -(-count // 128))
+    ws = grad_norm_workspace() if clip else None
+    check((_lib or load()).bb_adamw_list(table, count, lr, beta1, beta2, eps, step, weight_decay, grad_scale, int(zero_grad), max_norm, _addr(sumsq), _addr(norm),
+                                         _addr(ws), ws.numel() if clip else 0, _raw_stream()), "bb_adamw_list")

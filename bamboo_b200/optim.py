@@ -1,0 +1,163 @@
+"""AdamW over a list of tensors, for parameters that are not in an arena, with moments in 32 or 8 bits.
+
+    adamw_step_   one step over lists of parameters, gradients and moments
+    AdamW         an optimizer that keeps the moments (and fp32 masters of bf16 parameters)
+
+The formulas and the 8-bit format stand beside the kernel's declaration (``include/bamboo_b200.h``, bb_adamw_list), the kernel in
+``csrc/adamw.cu``.  An arena's flat buffers have ``lib.adam_step`` and ``post_training.adam_step_clipped``.
+"""
+import itertools
+import operator
+
+import torch
+
+from . import lib as L
+from .post_training import _gradient_of, _on_current
+
+BLOCK = 256          # values of a tensor that share a scale where moments have 8 bits
+
+_dtype_of = operator.attrgetter("dtype")
+_sizes = torch.Tensor.numel
+_address = torch.Tensor.data_ptr
+
+
+def _column(tensors, name, count, dtypes, sizes, device):
+    """A list that goes with the parameters: as many tensors, of one of these types, on the device, contiguous, of the same sizes."""
+    tensors = list(tensors)
+    if len(tensors) != count:
+        raise ValueError(f"{name}: {len(tensors)} tensors for {count} parameters")
+    if set(map(torch.Tensor.get_device, tensors)) != {device}:
+        raise L.BambooNativeError(f"{name}: expected on cuda:{device}, as the parameters")
+    if not set(map(_dtype_of, tensors)) <= dtypes:
+        raise L.BambooNativeError(f"{name}: {' or '.join(sorted(str(d) for d in dtypes))} expected")
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        raise L.BambooNativeError(f"{name}: contiguous tensors are expected")
+    if sizes is not None and list(map(_sizes, tensors)) != sizes:
+        raise ValueError(f"{name}: tensors of the parameters' sizes are expected")
+    return tensors
+
+
+_BF16, _FP32, _CODES = {torch.bfloat16}, {torch.float32}, {torch.float8_e4m3fn}
+
+
+def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, scales=None, masters=None, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8,
+                weight_decay=0.0, grad_scale=1.0, max_norm=0.0, sumsq=None, zero_grad=False):
+    """One AdamW step, number ``step`` (from 1), in place over lists of contiguous tensors; a parameter whose gradient is None is left out.
+
+    ``params``: fp32, or bf16 with fp32 ``masters``.  ``grads``: bf16 or fp32.  Moments: fp32; or float8_e4m3fn with ``scales``, a fp32 tensor
+    [2, blocks of 256 values] for each parameter, where ``exp_avg_sqs`` holds the SQUARE ROOT of the second moment.
+    ``grad_scale`` multiplies the gradients first.  ``max_norm`` > 0: on gradients clipped to that norm over the whole list, or over ``sumsq``
+    (sum of squares of unscaled gradients, fp64 [1], device) where it covers more; returns the norm before clipping (fp32 scalar, device).
+    A captured call repeats its step number at every replay."""
+    params, grads = list(params), list(grads)
+    if len(grads) != len(params):
+        raise ValueError(f"grads: {len(grads)} tensors for {len(params)} parameters")
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    if step < 1:
+        raise ValueError(f"step counts from 1, got {step}")
+    lists = [exp_avgs, exp_avg_sqs, scales, masters]
+    if any(g is None for g in grads) or not all(map(_sizes, params)):
+        keep = [i for i, (p, g) in enumerate(zip(params, grads)) if g is not None and p.numel()]
+        for at, column in enumerate(lists):
+            if column is not None:
+                column = list(column)
+                if len(column) != len(params):
+                    raise ValueError(f"{len(column)} tensors for {len(params)} parameters")
+                lists[at] = [column[i] for i in keep]
+        params, grads = [params[i] for i in keep], [grads[i] for i in keep]
+    exp_avgs, exp_avg_sqs, scales, masters = lists
+    count = len(params)
+    if not count:
+        return torch.zeros(()) if max_norm > 0 else None
+    _on_current(params[0], "params")
+    device, sizes = params[0].get_device(), list(map(_sizes, params))
+    params = _column(params, "params", count, _FP32 if masters is None else _BF16, sizes, device)
+    grads = _column(grads, "grads", count, _BF16 | _FP32, sizes, device)
+    moments = _FP32 if scales is None else _CODES
+    exp_avgs = _column(exp_avgs, "exp_avgs", count, moments, sizes, device)
+    exp_avg_sqs = _column(exp_avg_sqs, "exp_avg_sqs", count, moments, sizes, device)
+    zeros = itertools.repeat(0, count)
+    if masters is not None:
+        masters = _column(masters, "masters", count, _FP32, sizes, device)
+    if scales is not None:
+        scales = _column(scales, "scales", count, _FP32, None, device)
+        if list(map(_sizes, scales)) != [2 * -(-n // BLOCK) for n in sizes]:
+            raise ValueError("scales: [2, blocks of 256 values] for every parameter")
+    addresses = list(map(_address, params))
+    if len(set(addresses)) != count:
+        raise ValueError("params: a tensor stands in the list twice")
+    if sumsq is not None and (sumsq.get_device() != device or sumsq.dtype != torch.float64):
+        raise L.BambooNativeError("sumsq is fp64, on the parameters' device")
+    codes = map(L.dtype_codes().get, map(_dtype_of, grads))
+    fields = itertools.chain.from_iterable(zip(addresses, zeros if masters is None else map(_address, masters), map(_address, grads), map(_address, exp_avgs),
+                                               map(_address, exp_avg_sqs), itertools.repeat(0) if scales is None else map(_address, scales), sizes, codes,
+                                               itertools.repeat(0)))
+    norm = torch.empty((), dtype=torch.float32, device=params[0].device) if max_norm > 0 else None
+    L.adamw_list(L.adamw_tensors(fields, count), count, lr=lr, beta1=beta1, beta2=beta2, eps=eps, step=step, weight_decay=weight_decay,
+                 grad_scale=grad_scale, zero_grad=zero_grad, max_norm=max_norm, sumsq=sumsq, norm=norm)
+    torch.autograd.graph.increment_version(params)
+    return norm
+
+
+class AdamW:
+    """``adamw_step_`` over ``params`` (leaf tensors, fp32 or all bf16), with the state that it needs.
+
+    ``state_bits``: 32, or 8 for moments of one byte each.  bf16 parameters get fp32 masters, which the steps are taken on.  ``max_norm`` > 0 clips
+    the gradients' global norm.  ``step()`` reads ``main_grad`` of a parameter where it has one, else ``grad``."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, *, state_bits=32, max_norm=0.0):
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("no parameters")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits {state_bits}: 8 or 32")
+        dtypes = {p.dtype for p in self.params}
+        if len(dtypes) != 1 or not dtypes <= _BF16 | _FP32:
+            raise L.BambooNativeError(f"parameters are all fp32 or all bf16, got {sorted(map(str, dtypes))}")
+        self.lr, self.betas, self.eps, self.weight_decay, self.max_norm, self.state_bits = lr, tuple(betas), eps, weight_decay, max_norm, state_bits
+        self.step_count = 0
+        moment = torch.float8_e4m3fn if state_bits == 8 else torch.float32
+        data = [p.detach() for p in self.params]
+        self.masters = [p.float() for p in data] if dtypes == _BF16 else None
+        self.exp_avgs = [torch.zeros(p.shape, dtype=moment, device=p.device) for p in data]
+        self.exp_avg_sqs = [torch.zeros(p.shape, dtype=moment, device=p.device) for p in data]
+        self.scales = [torch.zeros(2, -(-p.numel() // BLOCK), device=p.device) for p in data] if state_bits == 8 else None
+
+    def step(self, *, grad_scale=1.0, sumsq=None):
+        """One step; returns the norm before clipping (fp32 scalar, device) where the optimizer clips, else None."""
+        if torch.cuda.is_current_stream_capturing():
+            raise L.BambooNativeError("AdamW.step counts its steps on the host and cannot be captured; adamw_step_ can, with one step number")
+        with torch.no_grad():
+            data = [p.detach() for p in self.params]
+            norm = adamw_step_(data, [_gradient_of(p) if p.requires_grad else None for p in self.params], self.exp_avgs, self.exp_avg_sqs,
+                               scales=self.scales, masters=self.masters, step=self.step_count + 1, lr=self.lr, beta1=self.betas[0],
+                               beta2=self.betas[1], eps=self.eps, weight_decay=self.weight_decay, grad_scale=grad_scale, max_norm=self.max_norm, sumsq=sumsq)
+        self.step_count += 1
+        return norm
+
+    def zero_grad(self):
+        for p in self.params:
+            main = getattr(p, "main_grad", None)
+            if main is not None:
+                main.zero_()
+            p.grad = None
+
+    def state_dict(self):
+        """Everything a step depends on but the parameters (the masters of bf16 ones included); tensors are the optimizer's own."""
+        return {"step": self.step_count, "state_bits": self.state_bits, "lr": self.lr, "betas": self.betas, "eps": self.eps, "weight_decay": self.weight_decay,
+                "max_norm": self.max_norm, "exp_avgs": self.exp_avgs, "exp_avg_sqs": self.exp_avg_sqs, "scales": self.scales, "masters": self.masters}
+
+    def load_state_dict(self, state):
+        if state["state_bits"] != self.state_bits:
+            raise ValueError(f"moments of {state['state_bits']} bits for an optimizer of {self.state_bits}")
+        for name in ("exp_avgs", "exp_avg_sqs", "scales", "masters"):
+            own, given = getattr(self, name), state[name]
+            if (own is None) != (given is None) or (own is not None and [t.shape for t in own] != [t.shape for t in given]):
+                raise ValueError(f"{name}: not those of these parameters")
+        for name in ("exp_avgs", "exp_avg_sqs", "scales", "masters"):
+            for to, t in zip(getattr(self, name) or (), state[name] or ()):
+                to.copy_(t)
+        self.step_count = int(state["step"])
+        self.lr, self.betas, self.eps = state["lr"], tuple(state["betas"]), state["eps"]
+        self.weight_decay, self.max_norm = state["weight_decay"], state["max_norm"]

@@ -107,18 +107,18 @@ class _NoSecondDerivative(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad):
-        raise RuntimeError("the post-training functions are once_differentiable: their gradients have no gradient of their own")
+        raise RuntimeError("functions of kernels are once_differentiable: their gradients have no gradient of their own")
 
 
 def _once_differentiable(backward):
     """For a backward pass of kernels: under ``create_graph`` its gradients would count as constants.  (torch's decorator of that name lets them
     where the incoming gradient is one.)"""
     @functools.wraps(backward)
-    def once(ctx, grad):
+    def once(ctx, *incoming):
         if not torch.is_grad_enabled():
-            return backward(ctx, grad)
+            return backward(ctx, *incoming)
         with torch.no_grad():
-            grads = backward(ctx, grad)
+            grads = backward(ctx, *incoming)
         return tuple(g if g is None else _NoSecondDerivative.apply(g, torch.empty(0, requires_grad=True)) for g in grads)
     return once
 

@@ -415,6 +415,93 @@ int bb_adam_step_clipped(float* master, float* grad, float* exp_avg, float* exp_
                          double weight_decay, double grad_scale, int zero_grad, const double* sumsq, double max_norm,
                          float* norm, void* workspace, long long workspace_bytes, void* stream);
 
+/* ---- mixture of experts ------------------------------------------------------------- */
+/* A linear layer with a weight per expert, over rows sorted by expert: expert e owns rows [offsets[e], offsets[e + 1]) (device int32
+ * [experts + 1], ascending within [0, rows]; offsets that are not set the status word and are cut to that).  bf16, fp32 accumulation in tensor
+ * memory; n and k multiples of 8, at most bb_grouped_max_experts() experts.
+ *   BB_GROUPED_ROWS    out[r, n] = W_e x[r, k]           BB_EPI_STORE, BB_EPI_BIAS (+ bias[e, n]), BB_EPI_BIAS_GELU (out2 = pre-activation; the GeLU of the unrounded one)
+ *   BB_GROUPED_INPUT   out[r, k] = W_e^T x[r, n]         BB_EPI_STORE, BB_EPI_MUL_DGELU (* gelu'(aux[r, k]));  x is the gradient
+ *   BB_GROUPED_WEIGHT  out[e, n, k] = sum of its rows of x[r, n] (x) weight[r, k]      BB_EPI_STORE, BB_EPI_ACCUM_F32 (fp32, +=);  x is
+ *                      the gradient, weight the layer's input [rows, k]
+ * weight [experts, n, k] is contiguous.  Rows of `out` that belong to no expert become zeros (out2 stays as it is there); an expert without
+ * rows has a gradient of zeros.  The reference has no mixture of experts: its layers (EX/pipeline_parallelism/gpt2.py:66-121) are the
+ * dense half blocks above, next to which these stand. */
+enum { BB_GROUPED_ROWS = 0, BB_GROUPED_INPUT = 1, BB_GROUPED_WEIGHT = 2 };
+typedef struct bb_grouped_desc {
+  int mode, rows, n, k, experts, epilogue;
+  const int* offsets;
+  const void* x; long long ld_x;
+  const void* weight; long long ld_weight;      /* ld_weight: BB_GROUPED_WEIGHT only */
+  void* out; long long ld_out;                  /* ld_out: rows (BB_GROUPED_WEIGHT: out is contiguous) */
+  const void* bias;
+  void* out2;                                   /* ld_out */
+  const void* aux; long long ld_aux;
+  int max_ctas;                                 /* see bb_gemm_desc.max_ctas */
+} bb_grouped_desc;
+int bb_grouped_max_experts(void);
+int bb_grouped_gemm(const bb_grouped_desc* d, void* stream);
+/* Bias gradients of such a layer: out_bf16[e, n] = sum of its rows of dy, or accum[e, n] (fp32) += it; a fixed order of additions. */
+long long bb_grouped_colsum_workspace_bytes(int rows, int n, int experts);
+int bb_grouped_colsum(const void* dy, long long ld, const int* offsets, int experts, void* out_bf16, float* accum, void* workspace,
+                      long long workspace_bytes, int rows, int n, void* stream);
+
+/* Routing.  logits [tokens, experts] (bf16 / fp32, rows of ld values): every token's k largest, in descending order, ties to the lower index; NaN
+ * stands above everything, -inf is never chosen.  p = softmax of the row;
+ *   weights[t, j] = p of the j-th chosen (normalize: divided by the sum over the chosen), experts_out[t, j] its index; 0 and -1 where a row has
+ *   fewer than k that can be chosen.
+ * All chosen slots s = t k + j are ordered by (expert, token): rows_out[s] is the place of a slot (-1: none), slots_out[r] the slot at place r (-1
+ * from offsets[experts] on), offsets[experts + 1] where every expert's places begin.
+ *   balance = experts * sum_e f_e P_e, f_e = share of the chosen slots that are e's, P_e = mean of p_e over the tokens that have any
+ * stats [tokens, 2], 8-byte aligned, keeps what the backward call needs of each softmax, load [experts + 1] the shares f_e and the number of those
+ * tokens.  At most 256 experts, of which at most 32 are chosen. */
+typedef struct bb_route_desc {
+  int tokens, experts, k, normalize, dtype;
+  long long ld;
+} bb_route_desc;
+long long bb_route_workspace_bytes(const bb_route_desc* d);
+int bb_route_fwd(const bb_route_desc* d, const void* logits, float* weights, int* experts_out, int* rows_out, int* slots_out, int* offsets,
+                 float* balance, float* stats, float* load, void* workspace, long long workspace_bytes, void* stream);
+/* dlogits [tokens, cols >= experts] (rows of ldd, type of the logits) from d_weights [tokens, k] and d_balance (device scalar), either may be NULL;
+ * zero in columns from `experts` on and in rows without a chosen expert. */
+int bb_route_bwd(const bb_route_desc* d, const void* logits, const int* experts_out, const float* stats, const float* load,
+                 const float* d_weights, const float* d_balance, void* dlogits, long long ldd, int cols, void* stream);
+
+/* Token rows into the experts' order: out[r] = x[slots[r] / k], zeros where slots[r] is -1 (rows of h values, bf16 / fp32).  Here and below an index
+ * that points at no row sets the status word and counts as -1. */
+int bb_dispatch_rows(const void* x, long long ld, int dtype, const int* slots, int k, void* out, long long rows, long long tokens, int h, void* stream);
+/* out[t] = residual[t] (or 0) + sum over j of weights[t, j] (NULL: 1) * x[rows_of[t, j]], in the order of j, summed in fp32 and rounded once; slots
+ * with -1 count for nothing.  residual may be NULL.  x has `rows` rows. */
+int bb_combine_rows(const void* x, long long ld, int dtype, const int* rows_of, const float* weights, const void* residual, long long ld_residual,
+                    int k, void* out, long long tokens, long long rows, int h, void* stream);
+/* Backward of the weighted sum: dx[r] = weights[s] * dy[t] at the place of every slot s = t k + j, zeros in rows without a slot; d_weights[s] = dy[t] .
+ * x[r] in fp32, 0 for slots without a place.  dx and x have `rows` rows, at most tokens k.  dx and d_weights may be NULL (x then too, where d_weights is). */
+int bb_combine_rows_bwd(const void* dy, long long ld_dy, int dtype, const void* x, long long ld, const int* rows_of, const int* slots,
+                        const float* weights, int k, void* dx, float* d_weights, long long tokens, long long rows, int h, void* stream);
+
+/* ---- optimizer over a list of tensors ------------------------------------------------ */
+/* One AdamW step over `count` tensors: fp32 parameters, or bf16 ones with an fp32 master each; gradients bf16 or fp32; moments in fp32, or
+ * both in 8 bits (e4m3) with a scale for every block of 256 values of a tensor: value = code * (scale / 256).  exp_avg then holds the first
+ * moment and exp_avg_sq the SQUARE ROOT of the second; scales [2, blocks] fp32, the first moment's in front.  A block's scale is its largest
+ * magnitude, a code the nearest to value * (256 / scale); a root above 0 is never coded as 0.  A block with an infinity or NaN
+ * gets a scale of NaN; scales up to 2^-100 hold nothing.
+ *   g = grad * grad_scale (* min(1, max_norm / (norm + 1e-6)));  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p -= lr * (m / (1 - beta1^step) / (sqrt(v / (1 - beta2^step)) + eps) + weight_decay * p)
+ * max_norm > 0 clips to the norm over the list (times grad_scale), or over `sumsq` (sum of squares of unscaled gradients, device) where that covers
+ * more; `norm` (device) receives it.  The first 8 bytes of the workspace (bb_grad_norm_workspace_bytes()) hold the sum, as for bb_grad_clip.
+ * Replaces: multi_tensor_adam over tensor lists (CS/adam/multi_tensor_adam.cu:28-163) via DS/ops/adam/fused_adam.py:85-182. */
+typedef struct bb_adamw_tensor {
+  void* param;                       /* fp32, or bf16 where there is a master */
+  float* master;                     /* NULL: param is fp32 */
+  void* grad;
+  void* exp_avg; void* exp_avg_sq;   /* fp32, or e4m3 where there are scales */
+  float* scales;
+  long long numel;
+  int grad_dtype, unused;
+} bb_adamw_tensor;
+int bb_adamw_list(const bb_adamw_tensor* tensors, int count, double lr, double beta1, double beta2, double eps, long long step,
+                  double weight_decay, double grad_scale, int zero_grad, double max_norm, const double* sumsq, float* norm, void* workspace,
+                  long long workspace_bytes, void* stream);
+
 /* ---- inter-stage transfer --------------------------------------------------------- */
 /* Set-up (these four are the only entry points that allocate or map device memory; call
  * them when a channel to a neighbour is created, not per message): a receive mailbox in
