@@ -24,16 +24,46 @@ __device__ __forceinline__ float warp_sum(float v) {
 
 // ------------------------------------------------------------------ routing
 constexpr int MAX_EXPERTS = 256, MAX_CHOSEN = 32;
-constexpr int ROUTE_WARPS = 8, ROUTE_THREADS = 32 * ROUTE_WARPS;
+constexpr int ROUTE_WARPS = 32, ROUTE_THREADS = 32 * ROUTE_WARPS;
+constexpr int BWD_WARPS = 8;
 
 struct RouteParams {
   int tokens, experts, k, normalize;
   long long ld;
+  int vec;                      // rows can be read in runs of a lane's logits
   int chunk, blocks;            // consecutive tokens of a block, blocks
   float* weights; int* chosen; int* rows; int* slots; int* offsets; float* balance; float2* stats; float* load;
   int* counts;                  // [blocks][experts + 1]: slots of every expert, tokens that have any
   float* probs;                 // [blocks][experts]: sums of softmax
 };
+
+// A lane's PER consecutive logits (-inf behind the last)
+template <typename T, int PER> __device__ __forceinline__ void load_run(const T* row, int first, int n, int vec, float* x) {
+  if (vec) {
+    if (first < n) {
+      constexpr int BYTES = PER * sizeof(T);
+      alignas(16) T v[PER];
+      if constexpr (BYTES >= 16) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(row + first)[i];
+      } else if constexpr (BYTES == 8) {
+        *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(row + first);
+      } else if constexpr (BYTES == 4) {
+        *reinterpret_cast<uint32_t*>(v) = *reinterpret_cast<const uint32_t*>(row + first);
+      } else {
+        v[0] = row[first];
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] = value_of(v[i]);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] = -INFINITY;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) x[i] = first + i < n ? value_of(row[first + i]) : -INFINITY;
+}
 
 // A logit as a number whose order is that of the choice: NaN above all, 0 for what is never chosen (-inf), both zeros alike
 __device__ __forceinline__ uint32_t choice_key(float x) {
@@ -47,55 +77,61 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// A warp per token: lane l holds logits l, l + 32, ...; k rounds of a warp-wide maximum and the lowest index that has it.  Then the block's slots
-// are ranked within their experts, in order.
+// A warp per token, PER consecutive logits a lane; k rounds of a warp-wide maximum, which goes to the first lane and there the first logit that has it.
+// Then the block's slots are ranked within their experts, in order: every warp counts a run of them, and ranks it behind the runs before.
+// A block per SM with all its warps: few blocks, because each adds up the counts of all others in the next kernel.
 template <typename T, int PER>
 __global__ void __launch_bounds__(ROUTE_THREADS)
 route_choose_kernel(const T* logits, const RouteParams p) {
-  __shared__ int hist[ROUTE_WARPS][MAX_EXPERTS];
-  __shared__ float sums[ROUTE_WARPS][MAX_EXPERTS];
+  extern __shared__ int shared[];
+  int* hist = shared;                                                        // [ROUTE_WARPS][experts]
+  float* sums = reinterpret_cast<float*>(shared + ROUTE_WARPS * p.experts);  // [ROUTE_WARPS][experts]
   __shared__ int some_tokens;
   bb::pdl_sync();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = p.experts, first = lane * PER;
   const int t0 = blockIdx.x * p.chunk, t1 = min(p.tokens, t0 + p.chunk);
-  for (int i = threadIdx.x; i < ROUTE_WARPS * MAX_EXPERTS; i += ROUTE_THREADS) (&hist[0][0])[i] = 0;
+  for (int i = threadIdx.x; i < ROUTE_WARPS * n; i += ROUTE_THREADS) hist[i] = 0;
   if (threadIdx.x == 0) some_tokens = 0;
   float prob[PER] = {};
   int some = 0;
-  for (int t = t0 + warp; t < t1; t += ROUTE_WARPS) {
-    const T* row = logits + (long long)t * p.ld;
-    float x[PER];
+  float x[PER];
+  int t = t0 + warp;
+  if (t < t1) load_run<T, PER>(logits + (long long)t * p.ld, first, n, p.vec, x);
+  for (; t < t1; t += ROUTE_WARPS) {
     uint32_t key[PER];
+    float own[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) x[i] = lane + 32 * i < p.experts ? value_of(row[lane + 32 * i]) : -INFINITY;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) key[i] = choice_key(x[i]);
+    for (int i = 0; i < PER; ++i) { key[i] = choice_key(x[i]); own[i] = x[i]; }
+    if (t + ROUTE_WARPS < t1) load_run<T, PER>(logits + (long long)(t + ROUTE_WARPS) * p.ld, first, n, p.vec, x);       // the next token's
     int mine = -1;
-    float value = 0.f;
+    uint32_t value = 0;
     for (int j = 0; j < p.k; ++j) {
-      uint32_t top = 0;
+      uint32_t best = key[0];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) top = max(top, key[i]);
-      top = __reduce_max_sync(0xffffffffu, top);
+      for (int i = 1; i < PER; ++i) best = max(best, key[i]);
+      const uint32_t top = __reduce_max_sync(0xffffffffu, best);
       if (top == 0) break;
-      uint32_t at = 0xffffffffu;
+      const int from = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
+      int at = 0;
 #pragma unroll
-      for (int i = PER - 1; i >= 0; --i) if (key[i] == top) at = lane + 32 * i;
-      at = __reduce_min_sync(0xffffffffu, at);
+      for (int i = PER - 1; i >= 0; --i) if (key[i] == top) at = i;
+      if (lane == from) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) if (lane + 32 * i == (int)at) key[i] = 0;
-      if (lane == j) { mine = (int)at; value = key_value(top); }
+        for (int i = 0; i < PER; ++i) if (i == at) key[i] = 0;
+      }
+      at = __shfl_sync(0xffffffffu, at, from);
+      if (lane == j) { mine = from * PER + at; value = top; }
     }
     const bool any = __shfl_sync(0xffffffffu, mine, 0) >= 0;
-    const float top = __shfl_sync(0xffffffffu, value, 0);
+    const float top = any ? key_value(__shfl_sync(0xffffffffu, value, 0)) : 0.f;
     float e[PER], sum = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      e[i] = any && lane + 32 * i < p.experts ? expf(x[i] - top) : 0.f;
+      e[i] = any && first + i < n ? expf(own[i] - top) : 0.f;
       sum += e[i];
     }
     sum = warp_sum(sum);
-    const float share = mine >= 0 ? expf(value - top) : 0.f;
+    const float share = mine >= 0 ? expf(key_value(value) - top) : 0.f;
     const float over = p.normalize ? warp_sum(share) : sum;
     const long long s = (long long)t * p.k + lane;
     if (lane < p.k) {
@@ -105,89 +141,90 @@ route_choose_kernel(const T* logits, const RouteParams p) {
     if (lane == 0) p.stats[t] = make_float2(top, sum);
     if (any) {
       ++some;
+      const float each = 1.f / sum;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) prob[i] += e[i] / sum;
+      for (int i = 0; i < PER; ++i) prob[i] = fmaf(e[i], each, prob[i]);
     }
   }
 #pragma unroll
-  for (int i = 0; i < PER; ++i) if (lane + 32 * i < p.experts) sums[warp][lane + 32 * i] = prob[i];
+  for (int i = 0; i < PER; ++i) if (first + i < n) sums[warp * n + first + i] = prob[i];
   __syncthreads();
-  if (lane == 0) atomicAdd(&some_tokens, some);
-  // ranks: every warp counts a run of the block's slots, then ranks it behind the runs before
-  const int k = p.k, first = t0 * k, n = (t1 - t0) * k;
-  const int run = (n + 32 * ROUTE_WARPS - 1) / (32 * ROUTE_WARPS) * 32, a = min(n, warp * run), b = min(n, a + run);
+  if (lane == 0 && some) atomicAdd(&some_tokens, some);
+  const int k = p.k, slot0 = t0 * k, count = (t1 - t0) * k;
+  const int run = (count + 32 * ROUTE_WARPS - 1) / (32 * ROUTE_WARPS) * 32, a = min(count, warp * run), b = min(count, a + run);
+  int* mine = hist + warp * n;
   for (int i = a + lane; i - lane < b; i += 32) {
-    const int e = i < b ? p.chosen[first + i] : -1;
+    const int e = i < b ? p.chosen[slot0 + i] : -1;
     const unsigned same = __match_any_sync(0xffffffffu, e);
-    if (e >= 0 && (same & ((1u << lane) - 1)) == 0) hist[warp][e] += __popc(same);
+    if (e >= 0 && (same & ((1u << lane) - 1)) == 0) mine[e] += __popc(same);
     __syncwarp();
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < p.experts; e += ROUTE_THREADS) {
+  for (int e = threadIdx.x; e < n; e += ROUTE_THREADS) {
     int total = 0;
     float s = 0.f;
-#pragma unroll
-    for (int w = 0; w < ROUTE_WARPS; ++w) { const int c = hist[w][e]; hist[w][e] = total; total += c; s += sums[w][e]; }
-    p.counts[(long long)blockIdx.x * (p.experts + 1) + e] = total;
-    p.probs[(long long)blockIdx.x * p.experts + e] = s;
+#pragma unroll 8
+    for (int w = 0; w < ROUTE_WARPS; ++w) { const int c = hist[w * n + e]; hist[w * n + e] = total; total += c; s += sums[w * n + e]; }
+    p.counts[(long long)blockIdx.x * (n + 1) + e] = total;
+    p.probs[(long long)blockIdx.x * n + e] = s;
   }
-  if (threadIdx.x == 0) p.counts[(long long)blockIdx.x * (p.experts + 1) + p.experts] = some_tokens;
+  if (threadIdx.x == 0) p.counts[(long long)blockIdx.x * (n + 1) + n] = some_tokens;
   __syncthreads();
   for (int i = a + lane; i - lane < b; i += 32) {
-    const int e = i < b ? p.chosen[first + i] : -1;
+    const int e = i < b ? p.chosen[slot0 + i] : -1;
     const unsigned same = __match_any_sync(0xffffffffu, e);
     const unsigned before = same & ((1u << lane) - 1);
     int at = 0;
-    if (e >= 0) at = hist[warp][e];
+    if (e >= 0) at = mine[e];
     __syncwarp();
-    if (e >= 0 && before == 0) hist[warp][e] = at + __popc(same);
-    if (i < b) p.rows[first + i] = e >= 0 ? at + __popc(before) : -1;
+    if (e >= 0 && before == 0) mine[e] = at + __popc(same);
+    if (i < b) p.rows[slot0 + i] = e >= 0 ? at + __popc(before) : -1;
     __syncwarp();
   }
 }
 
-// Every block adds up what stands before its slots (the counts of all blocks, once more each) and places them.
+// Every block adds up what stands before its slots (the counts of all blocks, once more each) and places them; the first also makes what
+// there is one of.
 __global__ void __launch_bounds__(ROUTE_THREADS)
 route_place_kernel(const RouteParams p) {
   __shared__ int total[MAX_EXPERTS + 1], before[MAX_EXPERTS + 1], base[MAX_EXPERTS + 1];
-  __shared__ double part[ROUTE_WARPS];
+  __shared__ float mass[ROUTE_THREADS];
+  __shared__ double part[MAX_EXPERTS];
   bb::pdl_sync();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, width = p.experts + 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = p.experts, width = n + 1;
   for (int e = threadIdx.x; e < width; e += ROUTE_THREADS) { total[e] = 0; before[e] = 0; }
   __syncthreads();
-  int groups = ROUTE_THREADS / width;
-  if (groups < 1) groups = 1;
-  for (int i = threadIdx.x; i < groups * width; i += ROUTE_THREADS) {
-    const int g = i / width, e = i - g * width;
+  const int groups = ROUTE_THREADS / width, g = threadIdx.x / width, e0 = threadIdx.x - g * width;
+  if (g < groups) {
     int all = 0, ahead = 0;
 #pragma unroll 8
     for (int b = g; b < p.blocks; b += groups) {
-      const int c = p.counts[(long long)b * width + e];
+      const int c = p.counts[(long long)b * width + e0];
       all += c;
       if (b < (int)blockIdx.x) ahead += c;
     }
-    atomicAdd(&total[e], all);
-    atomicAdd(&before[e], ahead);
+    atomicAdd(&total[e0], all);
+    atomicAdd(&before[e0], ahead);
   }
   __syncthreads();
   if (warp == 0) {
     int carry = 0;
-    for (int at = 0; at < p.experts; at += 32) {
-      const int e = at + lane, c = e < p.experts ? total[e] : 0;
+    for (int at = 0; at < n; at += 32) {
+      const int e = at + lane, c = e < n ? total[e] : 0;
       int v = c;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int o = __shfl_up_sync(0xffffffffu, v, d);
         if (lane >= d) v += o;
       }
-      if (e < p.experts) base[e] = carry + v - c;
+      if (e < n) base[e] = carry + v - c;
       carry += __shfl_sync(0xffffffffu, v, 31);
     }
-    if (lane == 0) base[p.experts] = carry;
+    if (lane == 0) base[n] = carry;
   }
   __syncthreads();
-  const int k = p.k, t0 = blockIdx.x * p.chunk, t1 = min(p.tokens, t0 + p.chunk), routed = base[p.experts];
-  const long long all = (long long)p.tokens * k;
+  const int k = p.k, t0 = blockIdx.x * p.chunk, t1 = min(p.tokens, t0 + p.chunk), routed = base[n];
+  const int all = p.tokens * k;
   for (int i = t0 * k + threadIdx.x; i < t1 * k; i += ROUTE_THREADS) {
     const int e = p.chosen[i];
     if (e >= 0) {
@@ -196,82 +233,109 @@ route_place_kernel(const RouteParams p) {
       p.slots[at] = i;
     }
   }
-  for (long long r = routed + (long long)blockIdx.x * ROUTE_THREADS + threadIdx.x; r < all; r += (long long)gridDim.x * ROUTE_THREADS) p.slots[r] = -1;
-  if (blockIdx.x != 0) return;
-  double sum = 0.0;
-  const double tokens = total[p.experts] > 0 ? total[p.experts] : 1, places = routed > 0 ? routed : 1;
-  for (int e = threadIdx.x; e < p.experts; e += ROUTE_THREADS) {
-    p.offsets[e] = base[e];
-    const double f = total[e] / places;
-    p.load[e] = (float)f;
-    double mass = 0.0;
+  for (long long r = (long long)routed + blockIdx.x * ROUTE_THREADS + threadIdx.x; r < all; r += (long long)gridDim.x * ROUTE_THREADS) p.slots[r] = -1;
+  if (blockIdx.x != gridDim.x - 1) return;
+  // sums of softmax: blocks b = g, g + groups, ... by one thread, then the threads of an expert in their order
+  const int teams = ROUTE_THREADS / n, team = threadIdx.x / n, e = threadIdx.x - team * n;
+  float m = 0.f;
+  if (team < teams) {
 #pragma unroll 8
-    for (int b = 0; b < p.blocks; ++b) mass += (double)p.probs[(long long)b * p.experts + e];
-    sum += f * mass / tokens;
+    for (int b = team; b < p.blocks; b += teams) m += p.probs[(long long)b * n + e];
   }
-  if (threadIdx.x == 0) { p.offsets[p.experts] = routed; p.load[p.experts] = (float)tokens; }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  if (lane == 0) part[warp] = sum;
+  mass[threadIdx.x] = m;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    sum = 0.0;
-    for (int w = 0; w < ROUTE_WARPS; ++w) sum += part[w];
-    p.balance[0] = (float)(p.experts * sum);
+  const double tokens = total[n] > 0 ? total[n] : 1, places = routed > 0 ? routed : 1;
+  if (threadIdx.x < n) {
+    double sum = 0.0;
+    for (int i = 0; i < teams; ++i) sum += (double)mass[i * n + threadIdx.x];
+    const double f = total[threadIdx.x] / places;
+    p.offsets[threadIdx.x] = base[threadIdx.x];
+    p.load[threadIdx.x] = (float)f;
+    part[threadIdx.x] = f * sum / tokens;
+  }
+  if (threadIdx.x == 0) { p.offsets[n] = routed; p.load[n] = (float)tokens; }
+  __syncthreads();
+  if (warp == 0) {
+    double sum = 0.0;
+    for (int i = lane; i < n; i += 32) sum += part[i];
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) p.balance[0] = (float)(n * sum);
   }
 }
 
-// dx_e = p_e (c_e - sum p c) + what arrives through the weights; a warp per token, its chosen experts in lanes 0 .. k - 1
+// dx_e = p_e (c_e - sum p c) + what arrives through the weights; a warp per token, its chosen experts in lanes 0 .. k - 1.  What arrives goes to the
+// lanes that own the experts through shared memory.
 template <typename T, int PER>
-__global__ void __launch_bounds__(ROUTE_THREADS)
-route_bwd_kernel(const T* logits, const RouteParams p, const float* d_weights, const float* d_balance, T* out, long long ldd, int cols) {
+__global__ void __launch_bounds__(32 * BWD_WARPS)
+route_bwd_kernel(const T* logits, const RouteParams p, const float* d_weights, const float* d_balance, T* out, long long ldd, int cols, int vec_out) {
+  __shared__ alignas(16) float arrived[BWD_WARPS][32 * PER];
   bb::pdl_sync();
-  const int lane = threadIdx.x & 31;
-  const float g = d_balance ? d_balance[0] * (float)p.experts / p.load[p.experts] : 0.f;
-  float push[PER];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = p.experts, first = lane * PER;
+  const int t = blockIdx.x * BWD_WARPS + warp;
+  if (t >= p.tokens) return;
+  const T* row = logits + (long long)t * p.ld;
+  const long long s = (long long)t * p.k + lane;
+  int mine = lane < p.k ? p.chosen[s] : -1;
+  if (mine >= n) mine = -1;
+  const float2 st = p.stats[t];
+  float x[PER], d[PER];
+  load_run<T, PER>(row, first, n, p.vec, x);
+  float dw = 0.f, w = 0.f;
+  if (mine >= 0) {
+    w = value_of(row[mine]);
+    dw = d_weights ? d_weights[s] : 0.f;
+  }
+  const float g = d_balance ? d_balance[0] * (float)n / p.load[n] : 0.f;
+  T* to = out + (long long)t * ldd;
+  if (__shfl_sync(0xffffffffu, mine, 0) >= 0) {
+    float* mail = arrived[warp];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) push[i] = d_balance && lane + 32 * i < p.experts ? g * p.load[lane + 32 * i] : 0.f;
-  for (int t = blockIdx.x * ROUTE_WARPS + (threadIdx.x >> 5); t < p.tokens; t += gridDim.x * ROUTE_WARPS) {
-    const T* row = logits + (long long)t * p.ld;
-    const long long s = (long long)t * p.k + lane;
-    int mine = lane < p.k ? p.chosen[s] : -1;
-    if (mine >= p.experts) mine = -1;
-    const float2 st = p.stats[t];
-    const bool any = __shfl_sync(0xffffffffu, mine, 0) >= 0;
-    T* to = out + (long long)t * ldd;
-    if (!any) {
-      for (int c = lane; c < cols; c += 32) put_value(to + c, 0.f);
-      continue;
-    }
-    float prob[PER], d[PER], mean = 0.f;
+    for (int i = 0; i < PER; ++i) mail[first + i] = 0.f;
+    const float over = 1.f / st.y;
+    float prob[PER], push[PER], mean = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      prob[i] = lane + 32 * i < p.experts ? expf(value_of(row[lane + 32 * i]) - st.x) / st.y : 0.f;
-      mean += prob[i] * push[i];
+      prob[i] = first + i < n ? expf(x[i] - st.x) * over : 0.f;
+      push[i] = d_balance && first + i < n ? g * p.load[first + i] : 0.f;
+      mean = fmaf(prob[i], push[i], mean);
     }
-    float dw = 0.f, w = 0.f;
-    if (mine >= 0) {
-      w = expf(value_of(row[mine]) - st.x);
-      dw = d_weights ? d_weights[s] : 0.f;
-    }
-    w /= p.normalize ? warp_sum(w) : st.y;
+    if (mine >= 0) w = expf(w - st.x);
+    w = p.normalize ? w / warp_sum(w) : w * over;
     const float through = warp_sum(w * dw);
     mean = warp_sum(mean);
-    const float add = p.normalize ? w * (dw - through) : w * dw;
+    __syncwarp();
+    if (mine >= 0) mail[mine] = p.normalize ? w * (dw - through) : w * dw;
+    __syncwarp();
     const float off = p.normalize ? mean : mean + through;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) d[i] = prob[i] * (push[i] - off);
-    for (int j = 0; j < p.k; ++j) {
-      const int e = __shfl_sync(0xffffffffu, mine, j);
-      const float v = __shfl_sync(0xffffffffu, add, j);
-      if (e < 0) break;
+    for (int i = 0; i < PER; ++i) d[i] = fmaf(prob[i], push[i] - off, mail[first + i]);
+  } else {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) if (lane + 32 * i == e) d[i] += v;
-    }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) if (lane + 32 * i < p.experts) put_value(to + lane + 32 * i, d[i]);
-    for (int c = p.experts + lane; c < cols; c += 32) put_value(to + c, 0.f);
+    for (int i = 0; i < PER; ++i) d[i] = 0.f;
   }
+  if (vec_out) {
+    if (first < n) {
+      alignas(16) T v[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) put_value(&v[i], d[i]);
+      constexpr int BYTES = PER * sizeof(T);
+      if constexpr (BYTES >= 16) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(to + first)[i] = reinterpret_cast<uint4*>(v)[i];
+      } else if constexpr (BYTES == 8) {
+        *reinterpret_cast<uint2*>(to + first) = *reinterpret_cast<uint2*>(v);
+      } else if constexpr (BYTES == 4) {
+        *reinterpret_cast<uint32_t*>(to + first) = *reinterpret_cast<uint32_t*>(v);
+      } else {
+        to[first] = v[0];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) if (first + i < n) put_value(to + first + i, d[i]);
+  }
+  for (int c = n + lane; c < cols; c += 32) put_value(to + c, 0.f);
 }
 
 // ------------------------------------------------------------------ rows there and back
@@ -431,34 +495,48 @@ bool bad_route(const bb_route_desc* d) {
          (d->dtype != BB_DTYPE_BF16 && d->dtype != BB_DTYPE_F32) || (long long)d->tokens * d->k > INT_MAX - 1024;
 }
 
+int per_lane(int experts) { return experts <= 32 ? 1 : experts <= 64 ? 2 : experts <= 128 ? 4 : 8; }
+bool odd(const void* p, uintptr_t mask) { return ((uintptr_t)p & mask) != 0; }
+// Rows in runs of a lane's values: runs end with the row, and begin on their size (16 bytes at most)
+template <typename T> bool in_runs(const T* p, long long ld, int experts) {
+  const int per = per_lane(experts), bytes = per * (int)sizeof(T) < 16 ? per * (int)sizeof(T) : 16;
+  return experts % per == 0 && ld * (long long)sizeof(T) % bytes == 0 && !odd(p, bytes - 1);
+}
+
 RouteParams route_params(const bb_route_desc* d) {
   RouteParams p = {};
   p.tokens = d->tokens; p.experts = d->experts; p.k = d->k; p.normalize = d->normalize; p.ld = d->ld;
-  const int most = 2 * bb_num_sms();
+  const int most = bb_num_sms();
   p.chunk = (d->tokens + most - 1) / most;
   if (p.chunk < ROUTE_WARPS) p.chunk = ROUTE_WARPS;
   p.blocks = (d->tokens + p.chunk - 1) / p.chunk;
   return p;
 }
 
-template <typename T> int route_fwd(const T* logits, const RouteParams& p, cudaStream_t s) {
-  const int per = (p.experts + 31) / 32;
-  auto kernel = per <= 1 ? route_choose_kernel<T, 1> : per <= 2 ? route_choose_kernel<T, 2> : per <= 4 ? route_choose_kernel<T, 4> : route_choose_kernel<T, 8>;
-  BB_CUDA_CHECK(bb_launch(kernel, p.blocks, ROUTE_THREADS, 0, s, logits, p));
+template <typename T, int PER> int choose_launch(const T* logits, const RouteParams& p, cudaStream_t s) {
+  BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(route_choose_kernel<T, PER>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * ROUTE_WARPS * 32 * PER * 4)));
+  BB_CUDA_CHECK(bb_launch(route_choose_kernel<T, PER>, p.blocks, ROUTE_THREADS, 2 * ROUTE_WARPS * p.experts * 4, s, logits, p));
+  return BB_OK;
+}
+
+template <typename T> int route_fwd(const T* logits, RouteParams p, cudaStream_t s) {
+  const int per = per_lane(p.experts);
+  p.vec = in_runs(logits, p.ld, p.experts);
+  if (int rc = per == 1 ? choose_launch<T, 1>(logits, p, s) : per == 2 ? choose_launch<T, 2>(logits, p, s) : per == 4 ? choose_launch<T, 4>(logits, p, s)
+                                                                                                            : choose_launch<T, 8>(logits, p, s))
+    return rc;
   BB_CUDA_CHECK(bb_launch(route_place_kernel, p.blocks, ROUTE_THREADS, 0, s, p));
   return BB_OK;
 }
 
 template <typename T>
-int route_bwd(const T* logits, const RouteParams& p, const float* dw, const float* db, T* out, long long ldd, int cols, cudaStream_t s) {
-  const int per = (p.experts + 31) / 32;
-  auto kernel = per <= 1 ? route_bwd_kernel<T, 1> : per <= 2 ? route_bwd_kernel<T, 2> : per <= 4 ? route_bwd_kernel<T, 4> : route_bwd_kernel<T, 8>;
-  const int want = (p.tokens + ROUTE_WARPS - 1) / ROUTE_WARPS, most = 8 * bb_num_sms();
-  BB_CUDA_CHECK(bb_launch(kernel, want < most ? want : most, ROUTE_THREADS, 0, s, logits, p, dw, db, out, ldd, cols));
+int route_bwd(const T* logits, RouteParams p, const float* dw, const float* db, T* out, long long ldd, int cols, cudaStream_t s) {
+  const int per = per_lane(p.experts);
+  p.vec = in_runs(logits, p.ld, p.experts);
+  auto kernel = per == 1 ? route_bwd_kernel<T, 1> : per == 2 ? route_bwd_kernel<T, 2> : per == 4 ? route_bwd_kernel<T, 4> : route_bwd_kernel<T, 8>;
+  BB_CUDA_CHECK(bb_launch(kernel, (p.tokens + BWD_WARPS - 1) / BWD_WARPS, 32 * BWD_WARPS, 0, s, logits, p, dw, db, out, ldd, cols, (int)in_runs(out, ldd, p.experts)));
   return BB_OK;
 }
-
-bool odd(const void* p, uintptr_t mask) { return ((uintptr_t)p & mask) != 0; }
 
 // 16-byte accesses: every pointer and row on 16 bytes
 template <typename T> bool whole(const void* a, long long lda, const void* b, long long ldb, const void* c, long long ldc, const void* d, int h) {

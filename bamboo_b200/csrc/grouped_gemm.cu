@@ -18,6 +18,7 @@
 #include "gemm_panels.cuh"
 #include "tma_host.cuh"
 #include <limits.h>
+#include <math.h>
 
 namespace {
 
@@ -32,7 +33,7 @@ template <int BN, bool PAIR> struct Cfg {
   static constexpr int B_ROWS = PAIR ? BN / 2 : BN;
   static constexpr int B_STAGE_BYTES = B_ROWS * BK * 2;
   static constexpr int STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
-  static constexpr int STAGES = B_ROWS == 256 ? 4 : B_ROWS == 128 ? 6 : 8;
+  static constexpr int STAGES = B_ROWS == 256 ? 4 : 6;
   static constexpr int TILE_M = PAIR ? 2 * BM : BM;
   static constexpr int TMEM_COLS = 2 * BN;
   static constexpr int BAR_BYTES = (3 * STAGES + 4) * 8 + 8;
@@ -348,7 +349,6 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       const int width = f32 ? 32 : 64, npanels = BN / width;
       const long long base = MODE == WGRAD ? u.e * p.expert_stride : 0;
       const __nv_bfloat16* bias = has_bias ? reinterpret_cast<const __nv_bfloat16*>(p.bias) + (long long)u.e * p.n : nullptr;
-      bool handed = none;
 #pragma unroll 1
       for (int pn = eg; pn < npanels; pn += 2) {
         const int nb = n0 + pn * width;
@@ -375,7 +375,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             for (int i = 0; i < 32; ++i) v[32 + i] = __uint_as_float(r[i]);
           }
         }
-        if (pn + 2 >= npanels && !handed) {
+        if (pn + 2 >= npanels && !none) {
           // this warp has read its share of the accumulator
           bb::tc_fence_before_sync();
           __syncwarp();
@@ -383,7 +383,6 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             if (PAIR) bb::mbar_arrive_cluster_relaxed(bb::mapa_shared(bb::smem_u32(&tmem_empty[acc]), 0));
             else bb::mbar_arrive(&tmem_empty[acc]);
           }
-          handed = true;
         }
         if (!some) continue;
         if (f32) {
@@ -430,11 +429,6 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         slab_flush_bf16(slab, reinterpret_cast<__nv_bfloat16*>(p.D) + base, p.ldd, r0, nb, u.end, cols, lane);
         __syncwarp();
       }
-      if constexpr (BN == 64) {
-        if (!handed) {                          // one panel: the second warp of the quarter has none to read
-          if (lane == 0) bb::mbar_arrive(&tmem_empty[acc]);
-        }
-      }
       if (!none && ++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
   }
@@ -452,43 +446,48 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 }
 
 // ---------------------------------------------------------------- bias gradients
-// db_e = sum of its rows of dy.  A CTA sums up to COLSUM_ROWS rows of one expert over 256 columns (eight warps, a row each at a time)
-// and leaves them as fp32; a second kernel adds an expert's pieces in their order.
-constexpr int COLSUM_ROWS = 256;
+// db_e = sum of its rows of dy.  A cluster of CTAs shares an expert's rows for 128 columns: every CTA sums a run of them (16 rows of 256 bytes at a
+// time, four such steps in flight), the first adds the CTAs' sums in their order through distributed shared memory.  Bound by memory: 16384 rows of
+// 4096, 8 experts COLSUM_US.
+constexpr int COLSUM_COLS = 128, COLSUM_MOST = 8, COLSUM_U = 4;
 
 __device__ __forceinline__ int clamped(const int* offsets, int e, int rows) {
   const int v = __ldca(offsets + e);
   return v < 0 ? 0 : v > rows ? rows : v;
 }
 
-// Piece `at` of the list of all experts' pieces: its expert and rows; false behind the last.  Every piece belongs to one expert.
-struct Piece { int e, from, to; };
-__device__ __forceinline__ bool find_piece(const int* offsets, int experts, int rows, int at, Piece& q) {
-  int lo = clamped(offsets, 0, rows);
-  for (int e = 0; e < experts; ++e) {
-    int hi = clamped(offsets, e + 1, rows);
-    if (hi < lo) hi = lo;
-    const int pieces = (hi - lo + COLSUM_ROWS - 1) / COLSUM_ROWS;
-    if (at < pieces) {
-      q.e = e; q.from = lo + at * COLSUM_ROWS; q.to = q.from + COLSUM_ROWS < hi ? q.from + COLSUM_ROWS : hi;
-      return true;
-    }
-    at -= pieces;
-    lo = hi;
-  }
-  return false;
-}
-
 __global__ void __launch_bounds__(256)
-grouped_colsum_kernel(const __nv_bfloat16* dy, long long ld, const int* offsets, int experts, int rows, int n, float* partial) {
-  __shared__ float sums[8][256];
+grouped_colsum_kernel(const __nv_bfloat16* dy, long long ld, const int* offsets, int rows, int n, __nv_bfloat16* out, float* accum) {
+  __shared__ float part[16][COLSUM_COLS], mine[COLSUM_COLS];
+  __shared__ int range[2];
   bb::pdl_sync();
-  Piece q;
-  if (!find_piece(offsets, experts, rows, blockIdx.y, q)) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 256 + lane * 8;
+  const int rank = (int)bb::cluster_ctarank(), parts = (int)bb::cluster_nctarank(), e = blockIdx.z;
+  const int lane16 = threadIdx.x & 15, line = threadIdx.x >> 4, col = blockIdx.y * COLSUM_COLS + lane16 * 8;
+  if (threadIdx.x < 32) {
+    // the expert's rows: offsets that do not ascend are cut as the products cut them
+    int lo = 0;
+    for (int i = threadIdx.x; i <= e; i += 32) lo = max(lo, clamped(offsets, i, rows));
+    lo = __reduce_max_sync(0xffffffffu, lo);
+    if (threadIdx.x == 0) { range[0] = lo; range[1] = max(lo, clamped(offsets, e + 1, rows)); }
+  }
+  __syncthreads();
+  const int each = (range[1] - range[0] + parts - 1) / parts, from = min(range[1], range[0] + rank * each), to = min(range[1], from + each);
   float v[8] = {};
   if (col < n) {
-    for (int r = q.from + warp; r < q.to; r += 8) {
+    int r = from + line;
+    for (; r + (COLSUM_U - 1) * 16 < to; r += COLSUM_U * 16) {
+      uint4 q[COLSUM_U];
+#pragma unroll
+      for (int u = 0; u < COLSUM_U; ++u) q[u] = __ldca(reinterpret_cast<const uint4*>(dy + (long long)(r + u * 16) * ld + col));
+#pragma unroll
+      for (int u = 0; u < COLSUM_U; ++u) {
+        float f[8];
+        unpack8(q[u], f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += f[i];
+      }
+    }
+    for (; r < to; r += 16) {
       float f[8];
       unpack8(__ldca(reinterpret_cast<const uint4*>(dy + (long long)r * ld + col)), f);
 #pragma unroll
@@ -496,33 +495,27 @@ grouped_colsum_kernel(const __nv_bfloat16* dy, long long ld, const int* offsets,
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sums[warp][lane * 8 + i] = v[i];
+  for (int i = 0; i < 8; ++i) part[line][lane16 * 8 + i] = v[i];
   __syncthreads();
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= n) return;
-  float s = 0.f;
+  if (threadIdx.x < COLSUM_COLS) {
+    float s = 0.f;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) s += sums[w][threadIdx.x];
-  partial[(long long)blockIdx.y * n + c] = s;
-}
-
-__global__ void __launch_bounds__(256)
-grouped_colsum_join_kernel(const float* partial, const int* offsets, int rows, int n, __nv_bfloat16* out, float* accum) {
-  bb::pdl_sync();
-  const int c = blockIdx.x * 256 + threadIdx.x, e = blockIdx.y;
-  int first = 0, lo = clamped(offsets, 0, rows), hi = lo;
-  for (int i = 0; i <= e; ++i) {
-    lo = hi;
-    hi = clamped(offsets, i + 1, rows);
-    if (hi < lo) hi = lo;
-    if (i < e) first += (hi - lo + COLSUM_ROWS - 1) / COLSUM_ROWS;
+    for (int l = 0; l < 16; ++l) s += part[l][threadIdx.x];
+    mine[threadIdx.x] = s;
   }
-  if (c >= n) return;
-  const int pieces = (hi - lo + COLSUM_ROWS - 1) / COLSUM_ROWS;
-  float s = 0.f;
-  for (int i = 0; i < pieces; ++i) s += partial[(long long)(first + i) * n + c];
-  if (accum) accum[(long long)e * n + c] += s;
-  else out[(long long)e * n + c] = __float2bfloat16(s);
+  bb::cluster_sync();
+  const int c = blockIdx.y * COLSUM_COLS + threadIdx.x;
+  if (rank == 0 && threadIdx.x < COLSUM_COLS && c < n) {
+    float s = 0.f;
+    for (int p = 0; p < parts; ++p) {
+      float o;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(bb::mapa_shared(bb::smem_u32(&mine[threadIdx.x]), p)) : "memory");
+      s += o;
+    }
+    if (accum) accum[(long long)e * n + c] += s;
+    else out[(long long)e * n + c] = __float2bfloat16(s);
+  }
+  bb::cluster_sync();               // no CTA leaves before its sums were read
 }
 
 // ---------------------------------------------------------------- host side
@@ -575,8 +568,37 @@ int launch(const bb_grouped_desc* d, cudaStream_t stream) {
   return BB_OK;
 }
 
+// The tile by the time that it is expected to take, as for stored products (gemm_tcgen05.cu), with the number of row tiles that evenly spread rows
+// would make: the host does not know the offsets.  Every expert adds half a tile of overhang.  us, pairs | 128 x 256 | 128 x 128, without
+// an epilogue: 16384 rows of 8 experts, 4096 x 1024, 103 | 116 | 144 (1.33 PFLOP/s); 16384 of 64, 1024 x 1024, 44 | 49 | 54; 4096 of 64,
+// 2048 x 512, 33 | 31 | 31; 2000 of 16, 1416 x 776, 19 | 15 | 16; 1024 of 8, 1024 x 256, 9.2 | 8.3 | 6.8; 14 of 8, 4096 x 1024, 19 | 15 | 20.  Tiles of 64
+// columns were never quicker (248 | 7.4 | 26 us).
 template <int MODE> int choose(const bb_grouped_desc* d, cudaStream_t stream) {
-  return launch<MODE, 128, false>(d, stream);
+  static const struct { int bn; bool pair; double kblock, wave, once; } kinds[3] = {
+      {256, true, 0.32, 1.9, 5.0}, {256, false, 0.375, 1.8, 3.7}, {128, false, 0.283, 1.0, 3.7}};
+  const double used = d->rows < d->experts ? d->rows : d->experts, each = d->rows / used;
+  int best = 0;
+  double best_us = -1;
+  for (int i = 0; i < 3; ++i) {
+    const auto& k = kinds[i];
+    if ((d->tile_n && d->tile_n != k.bn) || (d->cta_pair && (d->cta_pair > 0) != k.pair)) continue;
+    const int tm = k.pair ? 2 * BM : BM, n = MODE == ROWS ? d->n : d->k;
+    double row_tiles, kb;
+    if (MODE == WGRAD) {
+      row_tiles = (double)d->experts * ((d->n + tm - 1) / tm);
+      kb = each / BK + 0.5;
+    } else {
+      const double per = each / tm + 0.5;
+      row_tiles = used * (per > 1 ? per : 1);
+      kb = ((MODE == ROWS ? d->k : d->n) + BK - 1) / BK;
+    }
+    int workers = bb_num_sms();
+    if (d->max_ctas > 0 && d->max_ctas < workers) workers = d->max_ctas;
+    if (k.pair) workers = workers > 1 ? workers / 2 : 1;
+    const double us = ceil(row_tiles * ((n + k.bn - 1) / k.bn) / workers) * (kb * k.kblock + k.wave) + k.once;
+    if (best_us < 0 || us < best_us) { best_us = us; best = i; }
+  }
+  return best == 0 ? launch<MODE, 256, true>(d, stream) : best == 1 ? launch<MODE, 256, false>(d, stream) : launch<MODE, 128, false>(d, stream);
 }
 
 bool bad_sizes(const bb_grouped_desc* d) {
@@ -596,6 +618,8 @@ extern "C" int bb_grouped_gemm(const bb_grouped_desc* d, void* stream) {
   if (bad_matrix(d->x, d->ld_x, d->mode == BB_GROUPED_ROWS ? d->k : d->n) || bad_matrix(d->weight, wgrad ? d->ld_weight : d->k, d->k) || !d->out ||
       ((uintptr_t)d->out & 15) || (!wgrad && bad_matrix(d->out, d->ld_out, turned ? d->k : d->n)))
     return refuse("bb_grouped_gemm: operands are 16-byte aligned, with rows of a multiple of 8 values that do not overlap");
+  if ((d->tile_n != 0 && d->tile_n != 128 && d->tile_n != 256) || (d->cta_pair > 0 && d->tile_n == 128))
+    return refuse("bb_grouped_gemm: tile_n is 128 or 256, of a CTA pair 256");
   const int e = d->epilogue;
   if (wgrad ? (e != BB_EPI_STORE && e != BB_EPI_ACCUM_F32)
             : turned ? (e != BB_EPI_STORE && e != BB_EPI_MUL_DGELU) : (e != BB_EPI_STORE && e != BB_EPI_BIAS && e != BB_EPI_BIAS_GELU))
@@ -609,25 +633,72 @@ extern "C" int bb_grouped_gemm(const bb_grouped_desc* d, void* stream) {
   return wgrad ? choose<WGRAD>(d, s) : turned ? choose<ROWS_T>(d, s) : choose<ROWS>(d, s);
 }
 
-namespace {
-long long colsum_pieces(int rows, int experts) { return (long long)rows / COLSUM_ROWS + (rows < experts ? rows : experts); }
-}  // namespace
-
-extern "C" long long bb_grouped_colsum_workspace_bytes(int rows, int n, int experts) {
-  return rows <= 0 || n <= 0 || experts <= 0 ? 0 : colsum_pieces(rows, experts) * n * 4;
+extern "C" int bb_grouped_colsum(const void* dy, long long ld, const int* offsets, int experts, void* out_bf16, float* accum, int rows, int n, void* stream) {
+  if (rows <= 0 || n <= 0 || (n & 7) || experts <= 0 || experts > MAX_EXPERTS || !offsets || ((uintptr_t)offsets & 3) || bad_matrix(dy, ld, n) || (!out_bf16 == !accum) ||
+      ((uintptr_t)out_bf16 & 1) || ((uintptr_t)accum & 3))
+    return refuse("bb_grouped_colsum: null or misaligned pointer, a size that is not positive, n no multiple of 8, more than 256 experts, or not one output");
+  if ((n + COLSUM_COLS - 1) / COLSUM_COLS > 65535) return refuse("bb_grouped_colsum: more columns than one launch covers");
+  int parts = 1;
+  while (parts < COLSUM_MOST && rows / experts >= 64 * parts) parts *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(parts, (n + COLSUM_COLS - 1) / COLSUM_COLS, experts); cfg.blockDim = dim3(256); cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = bb_back_to_back > 0 ? 2 : 1;
+  BB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, grouped_colsum_kernel, (const __nv_bfloat16*)dy, ld, offsets, rows, n, (__nv_bfloat16*)out_bf16, accum));
+  return BB_OK;
 }
 
-extern "C" int bb_grouped_colsum(const void* dy, long long ld, const int* offsets, int experts, void* out_bf16, float* accum, void* workspace,
-                                 long long workspace_bytes, int rows, int n, void* stream) {
-  if (rows <= 0 || n <= 0 || (n & 7) || experts <= 0 || experts > MAX_EXPERTS || !offsets || bad_matrix(dy, ld, n) || (!out_bf16 == !accum) || !workspace ||
-      ((uintptr_t)workspace & 15) || workspace_bytes < bb_grouped_colsum_workspace_bytes(rows, n, experts))
-    return refuse("bb_grouped_colsum: null or misaligned pointer, a size that is not positive or no multiple of 8, or a workspace that is too small");
-  const long long pieces = colsum_pieces(rows, experts);
-  if (pieces > 65535) return refuse("bb_grouped_colsum: more rows than one launch covers");
-  BackToBack overlap;
-  BB_CUDA_CHECK(bb_launch(grouped_colsum_kernel, dim3((n + 255) / 256, (unsigned)pieces), 256, 0, (cudaStream_t)stream, (const __nv_bfloat16*)dy, ld, offsets, experts,
-                          rows, n, (float*)workspace));
-  BB_CUDA_CHECK(bb_launch(grouped_colsum_join_kernel, dim3((n + 255) / 256, (unsigned)experts), 256, 0, (cudaStream_t)stream, (const float*)workspace, offsets, rows, n,
-                          (__nv_bfloat16*)out_bf16, accum));
+// ---------------------------------------------------------------- two layers per expert
+namespace {
+bb_grouped_desc part_of(const bb_expert_mlp_desc* m, int mode, int n, int k, int epilogue) {
+  bb_grouped_desc d = {};
+  d.mode = mode; d.rows = m->rows; d.n = n; d.k = k; d.experts = m->experts; d.epilogue = epilogue; d.offsets = m->offsets; d.max_ctas = m->max_ctas;
+  return d;
+}
+bool bad_mlp(const bb_expert_mlp_desc* m) { return !m || m->rows <= 0 || m->in <= 0 || m->inner <= 0 || m->out <= 0 || !m->offsets; }
+// the weight's and the bias's gradient of one layer, each where it is asked for
+int weight_and_bias(const bb_expert_mlp_desc* m, const void* dy, long long ld_dy, int n, const void* x, long long ld_x, int k, void* dw, float* g_w, void* db, float* g_b,
+                    void* stream) {
+  if (dw || g_w) {
+    bb_grouped_desc d = part_of(m, BB_GROUPED_WEIGHT, n, k, g_w ? BB_EPI_ACCUM_F32 : BB_EPI_STORE);
+    d.x = dy; d.ld_x = ld_dy; d.weight = x; d.ld_weight = ld_x; d.out = g_w ? (void*)g_w : dw;
+    if (int rc = bb_grouped_gemm(&d, stream)) return rc;
+  }
+  if (db || g_b) return bb_grouped_colsum(dy, ld_dy, m->offsets, m->experts, g_b ? nullptr : db, g_b, m->rows, n, stream);
   return BB_OK;
+}
+}  // namespace
+
+extern "C" int bb_expert_mlp_fwd(const bb_expert_mlp_desc* m, const void* x, long long ld_x, void* pre, void* act, void* y, void* stream) {
+  if (bad_mlp(m)) return refuse("bb_expert_mlp_fwd: null pointer or a size that is not positive");
+  BackToBack overlap(m->max_ctas == 0);
+  bb_grouped_desc d = part_of(m, BB_GROUPED_ROWS, m->inner, m->in, BB_EPI_BIAS_GELU);
+  d.x = x; d.ld_x = ld_x; d.weight = m->w1; d.bias = m->b1; d.out = act; d.ld_out = m->inner; d.out2 = pre;
+  if (int rc = bb_grouped_gemm(&d, stream)) return rc;
+  d = part_of(m, BB_GROUPED_ROWS, m->out, m->inner, BB_EPI_BIAS);
+  d.x = act; d.ld_x = m->inner; d.weight = m->w2; d.bias = m->b2; d.out = y; d.ld_out = m->out;
+  return bb_grouped_gemm(&d, stream);
+}
+
+extern "C" int bb_expert_mlp_bwd(const bb_expert_mlp_desc* m, const void* x, long long ld_x, const void* pre, const void* act, const void* dy, long long ld_dy, void* dpre,
+                                 void* dx, void* stream) {
+  if (bad_mlp(m)) return refuse("bb_expert_mlp_bwd: null pointer or a size that is not positive");
+  BackToBack overlap(m->max_ctas == 0);
+  if (dpre) {
+    bb_grouped_desc d = part_of(m, BB_GROUPED_INPUT, m->out, m->inner, BB_EPI_MUL_DGELU);
+    d.x = dy; d.ld_x = ld_dy; d.weight = m->w2; d.out = dpre; d.ld_out = m->inner; d.aux = pre; d.ld_aux = m->inner;
+    if (int rc = bb_grouped_gemm(&d, stream)) return rc;
+  } else if (dx || m->dw1 || m->g_w1 || m->db1 || m->g_b1) {
+    return refuse("bb_expert_mlp_bwd: gradients of the first layer go through dpre");
+  }
+  if (dx) {
+    bb_grouped_desc d = part_of(m, BB_GROUPED_INPUT, m->inner, m->in, BB_EPI_STORE);
+    d.x = dpre; d.ld_x = m->inner; d.weight = m->w1; d.out = dx; d.ld_out = m->in;
+    if (int rc = bb_grouped_gemm(&d, stream)) return rc;
+  }
+  if (int rc = weight_and_bias(m, dpre, m->inner, m->inner, x, ld_x, m->in, m->dw1, m->g_w1, m->db1, m->g_b1, stream)) return rc;
+  return weight_and_bias(m, dy, ld_dy, m->out, act, m->inner, m->inner, m->dw2, m->g_w2, m->db2, m->g_b2, stream);
 }

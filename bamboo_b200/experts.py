@@ -329,36 +329,52 @@ def _mlp_operands(x, w1, b1, w2, b2):
     return (_grouped_rows(x), _weight(w1, "w1", x.shape[-1]), _bias(b1, "b1", w1), _weight(w2, "w2", w1.shape[1]), _bias(b2, "b2", w2))
 
 
+def _mlp_desc(x, w1, b1, w2, b2, offsets):
+    return L.ExpertMLPDesc(rows=x.shape[0], inputs=x.shape[1], inner=w1.shape[1], outputs=w2.shape[1], experts=w1.shape[0], max_ctas=L.GEMM_MAX_CTAS,
+                           offsets=offsets.data_ptr(), w1=w1.data_ptr(), b1=b1.data_ptr(), w2=w2.data_ptr(), b2=b2.data_ptr())
+
+
 def _mlp_forward(x, w1, b1, w2, b2, offsets):
-    pre = torch.empty(x.shape[0], w1.shape[1], dtype=torch.bfloat16, device=x.device)
-    act = _product(L.GROUPED_ROWS, x, w1, offsets, w1.shape[1], epilogue=L.EPI_BIAS_GELU, bias=b1, out2=pre)
-    return pre, act, _product(L.GROUPED_ROWS, act, w2, offsets, w2.shape[1], epilogue=L.EPI_BIAS, bias=b2)
+    """(what the backward pass needs, result): pre-activation and activation stand behind one another in one tensor"""
+    rows, inner = x.shape[0], w1.shape[1]
+    kept = torch.empty(2, rows, inner, dtype=torch.bfloat16, device=x.device)
+    y = torch.empty(rows, w2.shape[1], dtype=torch.bfloat16, device=x.device)
+    if rows:
+        L.expert_mlp_fwd(_mlp_desc(x, w1, b1, w2, b2, offsets), x, kept[0], kept[1], y)
+    return kept, y
 
 
 class _ExpertMLPFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w1, b1, w2, b2, offsets):
-        xm, v1, c1, v2, c2 = _mlp_operands(x, w1, b1, w2, b2)
-        pre, act, y = _mlp_forward(xm, v1, c1, v2, c2, offsets)
+        operands = _mlp_operands(x, w1, b1, w2, b2)
+        kept, y = _mlp_forward(*operands, offsets)
         ctx.parameters = w1, b1, w2, b2
-        ctx.save_for_backward(xm, v1, v2, offsets, pre, act)
+        ctx.save_for_backward(*operands, offsets, kept)
         return y
 
     @staticmethod
     @_once_differentiable
     def backward(ctx, dy):
-        x, w1, w2, offsets, pre, act = ctx.saved_tensors
-        need_x, need_w1, need_b1, need_w2, need_b2 = ctx.needs_input_grad[:5]
-        p1, c1, p2, c2 = ctx.parameters
+        x, w1, b1, w2, b2, offsets, kept = ctx.saved_tensors
+        need = ctx.needs_input_grad
         dy = _grouped_rows(dy, "gradient")
-        dw2, db2 = _weight_gradients(dy, act, offsets, p2, c2, need_w2, need_b2)
-        dx = dw1 = db1 = None
-        if need_x or need_w1 or need_b1:
-            dpre = _product(L.GROUPED_INPUT, dy, w2, offsets, w2.shape[2], epilogue=L.EPI_MUL_DGELU, aux=pre)
-            dw1, db1 = _weight_gradients(dpre, x, offsets, p1, c1, need_w1, need_b1)
-            if need_x:
-                dx = _product(L.GROUPED_INPUT, dpre, w1, offsets, w1.shape[2])
-        return dx, dw1, db1, dw2, db2, None
+        rows, dev = x.shape[0], x.device
+        desc = _mlp_desc(x, w1, b1, w2, b2, offsets)
+        grads = []
+        for name, p, wanted in zip(("w1", "b1", "w2", "b2"), ctx.parameters, need[1:5]):
+            main = getattr(p, "main_grad", None) if wanted else None
+            g = (torch.empty if rows else torch.zeros)(p.shape, dtype=torch.bfloat16, device=dev) if wanted and main is None else None
+            if g is not None:
+                setattr(desc, "d" + name, g.data_ptr())
+            elif wanted:
+                setattr(desc, "g_" + name, main.data_ptr())
+            grads.append(g)
+        dx = torch.empty(rows, x.shape[1], dtype=torch.bfloat16, device=dev) if need[0] else None
+        if rows:
+            dpre = torch.empty(rows, w1.shape[1], dtype=torch.bfloat16, device=dev) if any(need[:3]) else None
+            L.expert_mlp_bwd(desc, x, kept[0], kept[1], dy, dpre, dx)
+        return dx, *grads, None
 
 
 def expert_mlp(x, offsets, w1, b1, w2, b2):
@@ -374,4 +390,4 @@ def expert_mlp(x, offsets, w1, b1, w2, b2):
     offsets = _offsets(offsets, w1)
     if any(_wants_grad(t) for t in (x, w1, b1, w2, b2)):
         return _ExpertMLPFn.apply(x, w1, b1, w2, b2, offsets)
-    return _mlp_forward(*_mlp_operands(x, w1, b1, w2, b2), offsets)[2]
+    return _mlp_forward(*_mlp_operands(x, w1, b1, w2, b2), offsets)[1]

@@ -99,7 +99,18 @@ class GroupedDesc(ctypes.Structure):
         ("out", ctypes.c_void_p), ("ld_out", ctypes.c_longlong),
         ("bias", ctypes.c_void_p), ("out2", ctypes.c_void_p),
         ("aux", ctypes.c_void_p), ("ld_aux", ctypes.c_longlong),
-        ("max_ctas", ctypes.c_int),
+        ("max_ctas", ctypes.c_int), ("tile_n", ctypes.c_int), ("cta_pair", ctypes.c_int),
+    ]
+
+
+class ExpertMLPDesc(ctypes.Structure):
+    """bb_expert_mlp_desc: two layers per expert, their parameters and where gradients go (see include/bamboo_b200.h)."""
+    _fields_ = [
+        ("rows", ctypes.c_int), ("inputs", ctypes.c_int), ("inner", ctypes.c_int), ("outputs", ctypes.c_int), ("experts", ctypes.c_int),
+        ("max_ctas", ctypes.c_int), ("offsets", ctypes.c_void_p),
+        ("w1", ctypes.c_void_p), ("b1", ctypes.c_void_p), ("w2", ctypes.c_void_p), ("b2", ctypes.c_void_p),
+        ("dw1", ctypes.c_void_p), ("db1", ctypes.c_void_p), ("dw2", ctypes.c_void_p), ("db2", ctypes.c_void_p),
+        ("g_w1", ctypes.c_void_p), ("g_b1", ctypes.c_void_p), ("g_w2", ctypes.c_void_p), ("g_b2", ctypes.c_void_p),
     ]
 
 
@@ -174,8 +185,9 @@ def load():
         lib.bb_grad_clip.argtypes = [vp, i, vp, d, vp, vp, ll, vp]
         lib.bb_adam_step_clipped.argtypes = [vp] * 5 + [ll, d, d, d, d, i, i, i, d, d, i, vp, d, vp, vp, ll, vp]
         lib.bb_grouped_gemm.argtypes = [vp, vp]
-        lib.bb_grouped_colsum_workspace_bytes.restype = ll
-        lib.bb_grouped_colsum.argtypes = [vp, ll, vp, i, vp, vp, vp, ll, i, i, vp]
+        lib.bb_grouped_colsum.argtypes = [vp, ll, vp, i, vp, vp, i, i, vp]
+        lib.bb_expert_mlp_fwd.argtypes = [vp, vp, ll, vp, vp, vp, vp]
+        lib.bb_expert_mlp_bwd.argtypes = [vp, vp, ll, vp, vp, vp, ll, vp, vp, vp]
         lib.bb_route_workspace_bytes.restype = ll
         lib.bb_route_fwd.argtypes = [vp] * 11 + [ll, vp]
         lib.bb_route_bwd.argtypes = [vp] * 8 + [ll, i, vp]
@@ -815,7 +827,7 @@ def adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, *, lr, beta1=
 
 
 # ---------------------------------------------------------------------------- mixture of experts
-def grouped_gemm(mode, x, weight, offsets, out, *, epilogue=EPI_STORE, bias=None, out2=None, aux=None, max_ctas=0):
+def grouped_gemm(mode, x, weight, offsets, out, *, epilogue=EPI_STORE, bias=None, out2=None, aux=None, max_ctas=0, tile_n=0, cta_pair=0):
     """GROUPED_ROWS: x [rows, k], weight [experts, n, k], out [rows, n]; GROUPED_INPUT: x [rows, n], out [rows, k]; GROUPED_WEIGHT: x [rows, n],
     weight [rows, k], out [experts, n, k].  2-D tensors have unit inner stride, rows on 16 bytes; see bb_grouped_gemm."""
     global LAUNCHES
@@ -825,7 +837,7 @@ def grouped_gemm(mode, x, weight, offsets, out, *, epilogue=EPI_STORE, bias=None
     d = GroupedDesc(mode=mode, rows=x.shape[0], n=n, k=k, experts=experts, epilogue=epilogue, offsets=offsets.data_ptr(), x=x.data_ptr(),
                     ld_x=_ld(x), weight=weight.data_ptr(), ld_weight=_ld(weight) if wgrad else 0, out=out.data_ptr(),
                     ld_out=0 if wgrad else _ld(out), bias=_addr(bias), out2=_addr(out2), aux=_addr(aux), ld_aux=0 if aux is None else _ld(aux),
-                    max_ctas=max_ctas or GEMM_MAX_CTAS)
+                    max_ctas=max_ctas or GEMM_MAX_CTAS, tile_n=tile_n, cta_pair=cta_pair)
     check((_lib or load()).bb_grouped_gemm(ctypes.byref(d), _raw_stream()), "bb_grouped_gemm")
     return out
 
@@ -833,12 +845,27 @@ def grouped_gemm(mode, x, weight, offsets, out, *, epilogue=EPI_STORE, bias=None
 def grouped_colsum(dy, offsets, experts, out=None, accum=None):
     """out [experts, n] (bf16) = column sums of every expert's rows of dy [rows, n], or accum (fp32) += them."""
     global LAUNCHES
-    LAUNCHES += 2
-    lib = load()
+    LAUNCHES += 1
     rows, n = dy.shape
-    ws = workspace(lib.bb_grouped_colsum_workspace_bytes(rows, n, experts), "experts")
-    check(lib.bb_grouped_colsum(dy.data_ptr(), _ld(dy), offsets.data_ptr(), experts, _addr(out), _addr(accum), ws.data_ptr(), ws.numel(), rows, n,
-                                _raw_stream()), "bb_grouped_colsum")
+    check((_lib or load()).bb_grouped_colsum(dy.data_ptr(), _ld(dy), offsets.data_ptr(), experts, _addr(out), _addr(accum), rows, n, _raw_stream()),
+          "bb_grouped_colsum")
+
+
+def expert_mlp_fwd(desc, x, pre, act, y):
+    global LAUNCHES
+    LAUNCHES += 2
+    check((_lib or load()).bb_expert_mlp_fwd(ctypes.byref(desc), x.data_ptr(), _ld(x), pre.data_ptr(), act.data_ptr(), y.data_ptr(), _raw_stream()),
+          "bb_expert_mlp_fwd")
+    return y
+
+
+def expert_mlp_bwd(desc, x, pre, act, dy, dpre, dx):
+    """Gradients as the descriptor asks for them; dpre and dx may be None (see bb_expert_mlp_bwd)."""
+    global LAUNCHES
+    LAUNCHES += (dpre is not None) + (dx is not None) + sum(bool(getattr(desc, a) or getattr(desc, b)) for a, b in
+                                                          (("dw1", "g_w1"), ("db1", "g_b1"), ("dw2", "g_w2"), ("db2", "g_b2")))
+    check((_lib or load()).bb_expert_mlp_bwd(ctypes.byref(desc), x.data_ptr(), _ld(x), pre.data_ptr(), act.data_ptr(), dy.data_ptr(), _ld(dy), _addr(dpre),
+                                             _addr(dx), _raw_stream()), "bb_expert_mlp_bwd")
 
 
 def route_fwd(desc, logits, weights, experts, rows, slots, offsets, balance, stats, load_):

@@ -437,13 +437,28 @@ typedef struct bb_grouped_desc {
   void* out2;                                   /* ld_out */
   const void* aux; long long ld_aux;
   int max_ctas;                                 /* see bb_gemm_desc.max_ctas */
+  int tile_n;                                   /* 0 = choose, else 128 or 256 columns */
+  int cta_pair;                                 /* 0 = choose, 1 = CTA pairs (256 x 256 tiles), -1 = single CTAs */
 } bb_grouped_desc;
 int bb_grouped_max_experts(void);
 int bb_grouped_gemm(const bb_grouped_desc* d, void* stream);
 /* Bias gradients of such a layer: out_bf16[e, n] = sum of its rows of dy, or accum[e, n] (fp32) += it; a fixed order of additions. */
-long long bb_grouped_colsum_workspace_bytes(int rows, int n, int experts);
-int bb_grouped_colsum(const void* dy, long long ld, const int* offsets, int experts, void* out_bf16, float* accum, void* workspace,
-                      long long workspace_bytes, int rows, int n, void* stream);
+int bb_grouped_colsum(const void* dy, long long ld, const int* offsets, int experts, void* out_bf16, float* accum, int rows, int n, void* stream);
+
+/* Two such layers with a tanh GeLU between, one call each way: y = W2 gelu(W1 x + b1) + b2 per expert.  w1 [experts, inner, in], b1 [experts, inner],
+ * w2 [experts, out, inner], b2 [experts, out].  pre and act [rows, inner] are kept for the backward pass, which writes each gradient that has a place: d* in
+ * bf16, or g_* in fp32 (+=); dpre [rows, inner] is scratch, NULL where only the second layer's gradients are wanted.  pre, act, y, dpre, dx are contiguous. */
+typedef struct bb_expert_mlp_desc {
+  int rows, in, inner, out, experts;
+  int max_ctas;                                 /* forwarded to every product */
+  const int* offsets;
+  const void *w1, *b1, *w2, *b2;
+  void *dw1, *db1, *dw2, *db2;
+  float *g_w1, *g_b1, *g_w2, *g_b2;
+} bb_expert_mlp_desc;
+int bb_expert_mlp_fwd(const bb_expert_mlp_desc* m, const void* x, long long ld_x, void* pre, void* act, void* y, void* stream);
+int bb_expert_mlp_bwd(const bb_expert_mlp_desc* m, const void* x, long long ld_x, const void* pre, const void* act, const void* dy, long long ld_dy, void* dpre,
+                      void* dx, void* stream);
 
 /* Routing.  logits [tokens, experts] (bf16 / fp32, rows of ld values): every token's k largest, in descending order, ties to the lower index; NaN
  * stands above everything, -inf is never chosen.  p = softmax of the row;

@@ -381,7 +381,27 @@ def test_grouped_linear(ex, lengths, before, after, n, k, bias):
     assert torch.all(y[~own] == 0) and torch.all(grads[0][~own] == 0)
 
 
-def test_an_experts_gradient_does_not_see_its_neighbours_values(ex):
+TILES = [(256, 1), (256, -1), (128, -1)]
+
+
+@pytest.fixture
+def tile(request, ex, monkeypatch):
+    """Every product on tiles of one kind."""
+    import functools
+
+    from bamboo_b200 import lib
+    monkeypatch.setattr(lib, "grouped_gemm", functools.partial(lib.grouped_gemm, tile_n=request.param[0], cta_pair=request.param[1]))
+
+
+@pytest.mark.parametrize("tile", TILES, indirect=True)
+@pytest.mark.parametrize("lengths,before,after", GROUPS, ids=[f"{len(g[0])}experts{sum(g[0])}rows" for g in GROUPS])
+@pytest.mark.parametrize("n,k", [(64, 64), (136, 72), (520, 1000)])
+def test_grouped_linear_on_every_kind_of_tile(ex, tile, lengths, before, after, n, k):
+    test_grouped_linear(ex, lengths, before, after, n, k, True)
+
+
+@pytest.mark.parametrize("tile", TILES, indirect=True)
+def test_an_experts_gradient_does_not_see_its_neighbours_values(ex, tile):
     """Infinities and NaN in one expert's rows stay in its results: in the reduction over rows too, where tiles overhang."""
     lengths, n, k = [37, 50, 21, 1, 130], 136, 72
     x, w, b, dy = product_inputs(lengths, 0, 0, n, k)
@@ -463,6 +483,13 @@ def gelu(x):
 def gelu_bound(pre):
     """GeLU of a bound: slope at most 1.13; tanh.approx is off by 2^-10.9 of 1, times half the argument."""
     return Bound(gelu(pre.value), 1.13 * pre.err + 2 ** -11 * (pre.value.abs() + pre.err))
+
+
+@pytest.mark.parametrize("tile", TILES, indirect=True)
+def test_many_tiles_a_cta_on_every_kind(ex, tile):
+    """More tiles than CTAs: stages, accumulators and the hand-over of cleaned stages go round many times."""
+    test_grouped_linear(ex, [700, 3, 0, 1201, 15, 16, 17, 333, 2, 64, 900, 1], 5, 7, 1544, 776, True)
+    test_grouped_linear(ex, [5] * 200, 0, 0, 264, 520, True)
 
 
 @pytest.mark.parametrize("lengths,before,after", [([3], 0, 0), ([40, 0, 130, 7], 0, 5), ([300, 200], 1, 0), ([16] * 12, 0, 0)])
