@@ -23,7 +23,20 @@ struct AdamTable {
   int first[LIST + 1];                         // first block of each tensor
   int count;
 };
-struct AdamArgs { float lr, b1, omb1, b2, omb2, eps, inv_bc1, inv_bc2, decay, grad_scale; int zero_grad; const float* coef; };
+// (lr is folded into the rest: p -= rate m / (root sqrt(v) + eps) + shrink p, rate = lr / (1 - beta1^step), root = 1 / sqrt(1 - beta2^step))
+struct AdamArgs { float b1, omb1, b2, omb2, eps, rate, root, shrink, grad_scale; int zero_grad; const float* coef; };
+
+// One instruction each, within 2^-22 of the value; subnormal arguments count.  The update that they make is of the order of lr.
+__device__ __forceinline__ float root_of(float v) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float over(float v) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 
 __device__ __forceinline__ float2 code_pair(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
@@ -131,13 +144,19 @@ __device__ __forceinline__ void block_step(const bb_adamw_tensor& t, long long a
     load8<VEC>(reinterpret_cast<const float*>(t.exp_avg) + at, n, m);
     load8<VEC>(reinterpret_cast<const float*>(t.exp_avg_sq) + at, n, v);
   }
+  const float2 b1 = make_float2(a.b1, a.b1), b2 = make_float2(a.b2, a.b2), gs1 = make_float2(gs * a.omb1, gs * a.omb1), gs2 = make_float2(gs, gs);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x = g[i] * gs, old = EIGHT ? v[i] * v[i] : v[i];
-    m[i] = fmaf(a.b1, m[i], a.omb1 * x);
-    v[i] = fmaf(a.b2, old, a.omb2 * x * x);
-    const float step = (m[i] * a.inv_bc1) / (sqrtf(v[i] * a.inv_bc2) + a.eps);
-    p[i] = fmaf(-a.lr, fmaf(a.decay, p[i], step), p[i]);
+  for (int i = 0; i < 8; i += 2) {
+    const float2 x = make_float2(g[i], g[i + 1]), y = bb::mul2(x, gs2), old = make_float2(v[i], v[i + 1]);
+    const float2 m2 = bb::fma2(b1, make_float2(m[i], m[i + 1]), bb::mul2(x, gs1));
+    const float2 v2 = bb::fma2(b2, EIGHT ? bb::mul2(old, old) : old, bb::mul2(bb::mul2(y, y), make_float2(a.omb2, a.omb2)));
+    const float2 r = make_float2(root_of(v2.x), root_of(v2.y));
+    const float2 d = bb::fma2(r, make_float2(a.root, a.root), make_float2(a.eps, a.eps));
+    const float2 u = bb::mul2(bb::mul2(m2, make_float2(-a.rate, -a.rate)), make_float2(over(d.x), over(d.y)));
+    const float2 w = make_float2(p[i], p[i + 1]), q = bb::add2(w, bb::fma2(w, make_float2(-a.shrink, -a.shrink), u));
+    m[i] = m2.x; m[i + 1] = m2.y;
+    v[i] = EIGHT ? r.x : v2.x; v[i + 1] = EIGHT ? r.y : v2.y;
+    p[i] = q.x; p[i + 1] = q.y;
   }
   store8<VEC>(master + at, n, p);
   if (t.master) store8<VEC>(reinterpret_cast<__nv_bfloat16*>(t.param) + at, n, p);
@@ -151,8 +170,6 @@ __device__ __forceinline__ void block_step(const bb_adamw_tensor& t, long long a
 #pragma unroll
       for (int i = 0; i < 8; ++i) if (i >= n) { m[i] = 0.f; v[i] = 0.f; }
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = sqrtf(v[i]);
     const uint2 cm = encode<false>(m, sm), cv = encode<true>(v, sv);
     store_codes<VEC>(reinterpret_cast<uint8_t*>(t.exp_avg) + at, n, cm);
     store_codes<VEC>(reinterpret_cast<uint8_t*>(t.exp_avg_sq) + at, n, cv);
@@ -164,17 +181,14 @@ __device__ __forceinline__ void block_step(const bb_adamw_tensor& t, long long a
 }
 
 template <bool EIGHT>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 4)
 adamw_list_kernel(const __grid_constant__ AdamTable table, const AdamArgs a) {
   bb::pdl_sync();
   const int lane = threadIdx.x & 31;
   const int unit = blockIdx.x * WARPS + (threadIdx.x >> 5);
   if (unit >= table.first[table.count]) return;
-  int lo = 0, hi = table.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (table.first[mid] <= unit) lo = mid; else hi = mid - 1;
-  }
+  static_assert(LIST == 64, "two comparisons a lane find the tensor");
+  const int lo = __popc(__ballot_sync(0xffffffffu, table.first[lane] <= unit)) + __popc(__ballot_sync(0xffffffffu, table.first[lane + 32] <= unit)) - 1;
   const bb_adamw_tensor& t = table.t[lo];
   const long long block = unit - table.first[lo], at = block * BLOCK + lane * 8, left = t.numel - at;
   const float gs = a.coef ? a.coef[0] * a.grad_scale : a.grad_scale;
@@ -207,9 +221,9 @@ extern "C" int bb_adamw_list(const bb_adamw_tensor* tensors, int count, double l
       return refuse("bb_adamw_list: a null or misaligned pointer, an empty tensor, a gradient that is neither bf16 nor fp32, or scales for a part of the list only");
   cudaStream_t s = (cudaStream_t)stream;
   AdamArgs a;
-  a.lr = (float)lr; a.b1 = (float)beta1; a.omb1 = (float)(1.0 - beta1); a.b2 = (float)beta2; a.omb2 = (float)(1.0 - beta2); a.eps = (float)eps;
-  a.inv_bc1 = (float)(1.0 / (1.0 - pow(beta1, (double)step))); a.inv_bc2 = (float)(1.0 / (1.0 - pow(beta2, (double)step)));
-  a.decay = (float)weight_decay; a.grad_scale = (float)grad_scale; a.zero_grad = zero_grad; a.coef = nullptr;
+  a.b1 = (float)beta1; a.omb1 = (float)(1.0 - beta1); a.b2 = (float)beta2; a.omb2 = (float)(1.0 - beta2); a.eps = (float)eps;
+  a.rate = (float)(lr / (1.0 - pow(beta1, (double)step))); a.root = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
+  a.shrink = (float)(lr * weight_decay); a.grad_scale = (float)grad_scale; a.zero_grad = zero_grad; a.coef = nullptr;
   BackToBack overlap;
   if (max_norm > 0.0) {
     if (int rc = bb_list_clip_coef(tensors, count, sumsq, grad_scale, max_norm, norm, workspace, s)) return rc;
@@ -229,6 +243,7 @@ extern "C" int bb_adamw_list(const bb_adamw_tensor* tensors, int count, double l
     }
     t.count = n;
     t.first[n] = (int)blocks;
+    for (int i = n + 1; i <= LIST; ++i) t.first[i] = INT_MAX;
     BB_CUDA_CHECK(bb_launch(eight ? adamw_list_kernel<true> : adamw_list_kernel<false>, dim3((unsigned)((blocks + WARPS - 1) / WARPS)), THREADS, 0, s, t, a));
     from += n;
   }

@@ -404,88 +404,140 @@ dispatch_kernel(const T* x, long long ld, const int* slots, int k, T* out, int r
   for (int i = i0; i < n; i += TEAM) to[i] = from[i];
 }
 
+// A team goes through its token's row in runs of TEAM x U pieces: their loads are in flight together, of every row that the token has.  Row numbers and
+// weights wait in the lanes of each warp.
 template <typename T, int BYTES, int TEAM>
 __global__ void __launch_bounds__(MOVE_THREADS)
 combine_kernel(const T* x, long long ld, const int* rows_of, const float* weights, const T* residual, long long ld_res, int k, T* out, int tokens, int rows, int h,
                int* status) {
   typedef Pack<T, BYTES> P;
+  constexpr int U = BYTES == 16 ? 16 / P::N : 4;
   bb::pdl_sync();
-  const int t = blockIdx.x * TEAMS<TEAM> + threadIdx.x / TEAM, i0 = threadIdx.x % TEAM;
+  const int t = blockIdx.x * TEAMS<TEAM> + threadIdx.x / TEAM, i0 = threadIdx.x % TEAM, lane = threadIdx.x & 31;
   if (t >= tokens) return;
   const int n = h / P::N;
   const long long s = (long long)t * k;
-  for (int i = i0; i < n; i += TEAM) {
-    float sum[P::N] = {};
-#pragma unroll 4
+  const int my_row = lane < k ? checked(rows_of[s + lane], rows, status) : -1;
+  const float my_weight = weights && lane < k ? weights[s + lane] : 1.f;
+  for (int run = 0; run < n; run += TEAM * U) {
+    const int i = run + i0;
+    float sum[U][P::N] = {};
+#pragma unroll 2
     for (int j = 0; j < k; ++j) {
-      const int r = checked(rows_of[s + j], rows, status);
+      const int r = __shfl_sync(0xffffffffu, my_row, j);
+      const float w = __shfl_sync(0xffffffffu, my_weight, j);
       if (r < 0) continue;
-      const float w = weights ? weights[s + j] : 1.f;
-      float v[P::N];
-      P::get(x + (long long)r * ld + i * P::N, v);
+      const T* from = x + (long long)r * ld;
+      float v[U][P::N];
 #pragma unroll
-      for (int c = 0; c < P::N; ++c) sum[c] = fmaf(w, v[c], sum[c]);
-    }
-    if (residual) {
-      float v[P::N];
-      P::get(residual + (long long)t * ld_res + i * P::N, v);
+      for (int u = 0; u < U; ++u) {
+        if (i + u * TEAM < n) {
+          P::get(from + (i + u * TEAM) * P::N, v[u]);
+        } else {
 #pragma unroll
-      for (int c = 0; c < P::N; ++c) sum[c] += v[c];
+          for (int c = 0; c < P::N; ++c) v[u][c] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int c = 0; c < P::N; ++c) sum[u][c] = fmaf(w, v[u][c], sum[u][c]);
     }
-    P::put(out + (long long)t * h + i * P::N, sum);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u * TEAM >= n) break;
+      if (residual) {
+        float v[P::N];
+        P::get(residual + (long long)t * ld_res + (i + u * TEAM) * P::N, v);
+#pragma unroll
+        for (int c = 0; c < P::N; ++c) sum[u][c] += v[c];
+      }
+      P::put(out + (long long)t * h + (i + u * TEAM) * P::N, sum[u]);
+    }
   }
 }
 
+// The gradient of the sum is read once per run and token; a warp's share of the j-th product gathers in its lane j.
 template <typename T, int BYTES, int TEAM>
 __global__ void __launch_bounds__(MOVE_THREADS)
 combine_bwd_kernel(const T* dy, long long ld_dy, const T* x, long long ld, const int* rows_of, const int* slots, const float* weights, int k, T* dx,
                    float* d_weights, int tokens, int rows, int h, int* status) {
   typedef Pack<T, BYTES> P;
-  __shared__ float part[TEAM > 32 ? TEAM / 32 : 1];
+  constexpr int U = BYTES == 16 ? 32 / P::N : 4;
+  __shared__ float part[TEAM > 32 ? TEAM / 32 : 1][32];
   bb::pdl_sync();
-  const int t = blockIdx.x * TEAMS<TEAM> + threadIdx.x / TEAM, i0 = threadIdx.x % TEAM;
+  const int t = blockIdx.x * TEAMS<TEAM> + threadIdx.x / TEAM, i0 = threadIdx.x % TEAM, lane = threadIdx.x & 31;
   if (t >= tokens) return;
   const int n = h / P::N;
+  const long long s = (long long)t * k;
   const T* from = dy + (long long)t * ld_dy;
-  for (int j = 0; j < k; ++j) {
-    const long long s = (long long)t * k + j;
-    const int r = checked(rows_of[s], rows, status);
-    float dot = 0.f;
-    if (r >= 0) {
-      const float w = weights[s];
-#pragma unroll 2
-      for (int i = i0; i < n; i += TEAM) {
-        float d[P::N], v[P::N];
-        P::get(from + i * P::N, d);
-        if (d_weights) {
-          P::get(x + (long long)r * ld + i * P::N, v);
+  const int my_row = lane < k ? checked(rows_of[s + lane], rows, status) : -1, my_slot = lane < k && s + lane < rows ? slots[s + lane] : 0;
+  const float my_weight = lane < k ? weights[s + lane] : 0.f;
+  float dot = 0.f;
+  for (int run = 0; run < n; run += TEAM * U) {
+    const int i = run + i0;
+    float d[U][P::N];
 #pragma unroll
-          for (int c = 0; c < P::N; ++c) dot = fmaf(d[c], v[c], dot);
+    for (int u = 0; u < U; ++u) {
+      if (i + u * TEAM < n) {
+        P::get(from + (i + u * TEAM) * P::N, d[u]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < P::N; ++c) d[u][c] = 0.f;
+      }
+    }
+    for (int j = 0; j < k; ++j) {
+      const int r = __shfl_sync(0xffffffffu, my_row, j);
+      const float w = __shfl_sync(0xffffffffu, my_weight, j);
+      if (r >= 0) {
+        if (d_weights) {
+          float v[U][P::N], sum = 0.f;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            if (i + u * TEAM < n) {
+              P::get(x + (long long)r * ld + (i + u * TEAM) * P::N, v[u]);
+            } else {
+#pragma unroll
+              for (int c = 0; c < P::N; ++c) v[u][c] = 0.f;
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int c = 0; c < P::N; ++c) sum = fmaf(d[u][c], v[u][c], sum);
+          sum = warp_sum(sum);
+          if (lane == j) dot += sum;
         }
         if (dx) {
 #pragma unroll
-          for (int c = 0; c < P::N; ++c) d[c] *= w;
-          P::put(dx + (long long)r * h + i * P::N, d);
+          for (int u = 0; u < U; ++u) {
+            if (i + u * TEAM >= n) break;
+            float v[P::N];
+#pragma unroll
+            for (int c = 0; c < P::N; ++c) v[c] = w * d[u][c];
+            P::put(dx + (long long)r * h + (i + u * TEAM) * P::N, v);
+          }
         }
       }
-    }
-    if (d_weights) {
-      dot = warp_sum(dot);
-      if (TEAM > 32) {
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = dot;
-        __syncthreads();
-        dot = 0.f;
+      // the place of the same number as this slot: zeros where nobody stands
+      if (dx && __shfl_sync(0xffffffffu, my_slot, j) < 0) {
+        const float zeros[P::N] = {};
 #pragma unroll
-        for (int w = 0; w < TEAM / 32; ++w) dot += part[w];
+        for (int u = 0; u < U; ++u) if (i + u * TEAM < n) P::put(dx + (s + j) * h + (i + u * TEAM) * P::N, zeros);
       }
-      if (i0 == 0) d_weights[s] = r >= 0 ? dot : 0.f;
     }
-    // the place of the same number as this slot: zeros where nobody stands
-    if (dx && slots[s] < 0 && s < rows) {
-      const float zeros[P::N] = {};
-      for (int i = i0; i < n; i += TEAM) P::put(dx + s * h + i * P::N, zeros);
-    }
+  }
+  if (!d_weights) return;
+  if (TEAM > 32) {
+    part[threadIdx.x / 32 % (TEAM / 32)][lane] = dot;
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    dot = 0.f;
+#pragma unroll
+    for (int w = 0; w < TEAM / 32; ++w) dot += part[w][lane];
+    if (lane < k) d_weights[s + lane] = dot;
+  } else if (lane < k) {
+    d_weights[s + lane] = dot;
   }
 }
 
@@ -572,7 +624,7 @@ int combine_bwd(const T* dy, long long ld_dy, const T* x, long long ld, const in
 }
 
 bool bad_move(const void* x, long long ld, int dtype, const void* index, int k, long long rows, long long tokens, int h) {
-  return !x || tokens <= 0 || k > INT_MAX / tokens || !index || odd(index, 3) || k <= 0 || rows <= 0 || rows > INT_MAX || h <= 0 || ld < h || (dtype != BB_DTYPE_BF16 && dtype != BB_DTYPE_F32) ||
+  return k > MAX_CHOSEN || !x || tokens <= 0 || k > INT_MAX / tokens || !index || odd(index, 3) || k <= 0 || rows <= 0 || rows > INT_MAX || h <= 0 || ld < h || (dtype != BB_DTYPE_BF16 && dtype != BB_DTYPE_F32) ||
          odd(x, dtype == BB_DTYPE_F32 ? 3 : 1);
 }
 }  // namespace

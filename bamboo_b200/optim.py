@@ -19,25 +19,26 @@ BLOCK = 256          # values of a tensor that share a scale where moments have 
 _dtype_of = operator.attrgetter("dtype")
 _sizes = torch.Tensor.numel
 _address = torch.Tensor.data_ptr
+_device_of = torch.Tensor.get_device
+_contiguous = torch.Tensor.is_contiguous
 
 
 def _column(tensors, name, count, dtypes, sizes, device):
     """A list that goes with the parameters: as many tensors, of one of these types, on the device, contiguous, of the same sizes."""
-    tensors = list(tensors)
     if len(tensors) != count:
         raise ValueError(f"{name}: {len(tensors)} tensors for {count} parameters")
-    if set(map(torch.Tensor.get_device, tensors)) != {device}:
+    if set(map(_device_of, tensors)) != {device}:
         raise L.BambooNativeError(f"{name}: expected on cuda:{device}, as the parameters")
     if not set(map(_dtype_of, tensors)) <= dtypes:
         raise L.BambooNativeError(f"{name}: {' or '.join(sorted(str(d) for d in dtypes))} expected")
-    if not all(map(torch.Tensor.is_contiguous, tensors)):
+    if not all(map(_contiguous, tensors)):
         raise L.BambooNativeError(f"{name}: contiguous tensors are expected")
     if sizes is not None and list(map(_sizes, tensors)) != sizes:
         raise ValueError(f"{name}: tensors of the parameters' sizes are expected")
-    return tensors
+    return map(_address, tensors)
 
 
-_BF16, _FP32, _CODES = {torch.bfloat16}, {torch.float32}, {torch.float8_e4m3fn}
+_BF16, _FP32, _EITHER, _CODES = {torch.bfloat16}, {torch.float32}, {torch.bfloat16, torch.float32}, {torch.float8_e4m3fn}
 
 
 def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, scales=None, masters=None, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8,
@@ -50,49 +51,38 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, scales=None, masters=No
     (sum of squares of unscaled gradients, fp64 [1], device) where it covers more; returns the norm before clipping (fp32 scalar, device).
     A captured call repeats its step number at every replay."""
     params, grads = list(params), list(grads)
-    if len(grads) != len(params):
-        raise ValueError(f"grads: {len(grads)} tensors for {len(params)} parameters")
     if not max_norm >= 0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if step < 1:
         raise ValueError(f"step counts from 1, got {step}")
-    lists = [exp_avgs, exp_avg_sqs, scales, masters]
-    if any(g is None for g in grads) or not all(map(_sizes, params)):
-        keep = [i for i, (p, g) in enumerate(zip(params, grads)) if g is not None and p.numel()]
-        for at, column in enumerate(lists):
-            if column is not None:
-                column = list(column)
-                if len(column) != len(params):
-                    raise ValueError(f"{len(column)} tensors for {len(params)} parameters")
-                lists[at] = [column[i] for i in keep]
-        params, grads = [params[i] for i in keep], [grads[i] for i in keep]
-    exp_avgs, exp_avg_sqs, scales, masters = lists
+    lists = [grads, *(None if column is None else list(column) for column in (exp_avgs, exp_avg_sqs, scales, masters))]
+    for name, column in zip(("grads", "exp_avgs", "exp_avg_sqs", "scales", "masters"), lists):
+        if column is not None and len(column) != len(params):
+            raise ValueError(f"{name}: {len(column)} tensors for {len(params)} parameters")
+    sizes = list(map(_sizes, params))
+    if not all(sizes) or type(None) in set(map(type, grads)):
+        keep = [i for i, g in enumerate(grads) if g is not None and sizes[i]]
+        params, sizes = [params[i] for i in keep], [sizes[i] for i in keep]
+        lists = [None if column is None else [column[i] for i in keep] for column in lists]
+    grads, exp_avgs, exp_avg_sqs, scales, masters = lists
     count = len(params)
     if not count:
         return torch.zeros(()) if max_norm > 0 else None
     _on_current(params[0], "params")
-    device, sizes = params[0].get_device(), list(map(_sizes, params))
-    params = _column(params, "params", count, _FP32 if masters is None else _BF16, sizes, device)
-    grads = _column(grads, "grads", count, _BF16 | _FP32, sizes, device)
+    device = params[0].get_device()
     moments = _FP32 if scales is None else _CODES
-    exp_avgs = _column(exp_avgs, "exp_avgs", count, moments, sizes, device)
-    exp_avg_sqs = _column(exp_avg_sqs, "exp_avg_sqs", count, moments, sizes, device)
-    zeros = itertools.repeat(0, count)
-    if masters is not None:
-        masters = _column(masters, "masters", count, _FP32, sizes, device)
-    if scales is not None:
-        scales = _column(scales, "scales", count, _FP32, None, device)
-        if list(map(_sizes, scales)) != [2 * -(-n // BLOCK) for n in sizes]:
-            raise ValueError("scales: [2, blocks of 256 values] for every parameter")
-    addresses = list(map(_address, params))
+    addresses = list(_column(params, "params", count, _FP32 if masters is None else _BF16, None, device))
     if len(set(addresses)) != count:
         raise ValueError("params: a tensor stands in the list twice")
+    if scales is not None and list(map(_sizes, scales)) != [2 * -(-n // BLOCK) for n in sizes]:
+        raise ValueError("scales: [2, blocks of 256 values] for every parameter")
     if sumsq is not None and (sumsq.get_device() != device or sumsq.dtype != torch.float64):
         raise L.BambooNativeError("sumsq is fp64, on the parameters' device")
-    codes = map(L.dtype_codes().get, map(_dtype_of, grads))
-    fields = itertools.chain.from_iterable(zip(addresses, zeros if masters is None else map(_address, masters), map(_address, grads), map(_address, exp_avgs),
-                                               map(_address, exp_avg_sqs), itertools.repeat(0) if scales is None else map(_address, scales), sizes, codes,
-                                               itertools.repeat(0)))
+    nothing = itertools.repeat(0)
+    fields = itertools.chain.from_iterable(zip(
+        addresses, nothing if masters is None else _column(masters, "masters", count, _FP32, sizes, device), _column(grads, "grads", count, _EITHER, sizes, device),
+        _column(exp_avgs, "exp_avgs", count, moments, sizes, device), _column(exp_avg_sqs, "exp_avg_sqs", count, moments, sizes, device),
+        nothing if scales is None else _column(scales, "scales", count, _FP32, None, device), sizes, map(L.dtype_codes().get, map(_dtype_of, grads)), nothing))
     norm = torch.empty((), dtype=torch.float32, device=params[0].device) if max_norm > 0 else None
     L.adamw_list(L.adamw_tensors(fields, count), count, lr=lr, beta1=beta1, beta2=beta2, eps=eps, step=step, weight_decay=weight_decay,
                  grad_scale=grad_scale, zero_grad=zero_grad, max_norm=max_norm, sumsq=sumsq, norm=norm)
@@ -113,7 +103,7 @@ class AdamW:
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits {state_bits}: 8 or 32")
         dtypes = {p.dtype for p in self.params}
-        if len(dtypes) != 1 or not dtypes <= _BF16 | _FP32:
+        if len(dtypes) != 1 or not dtypes <= _EITHER:
             raise L.BambooNativeError(f"parameters are all fp32 or all bf16, got {sorted(map(str, dtypes))}")
         self.lr, self.betas, self.eps, self.weight_decay, self.max_norm, self.state_bits = lr, tuple(betas), eps, weight_decay, max_norm, state_bits
         self.step_count = 0

@@ -237,7 +237,7 @@ def test_dispatch_and_combine(ex, tokens, hidden, experts, k, dtype):
         dxs = torch.where((slots >= 0)[:, None], r.weights.double().reshape(-1)[at][:, None] * dy.double()[at // k], 0.0)
         near(grads[0], dxs, HALF_STEP[dtype] + 2 ** -24)
         products = each * dy.double()[:, None]
-        # a thread adds up to hidden / 32 products, then five or thirteen sums: at most hidden / 16 + 16 roundings
+        # a thread adds at most hidden / 32 + 16 products one after the other, then come five sums a run and the runs: below hidden / 16 + 16 roundings
         near(grads[1], products.sum(2), 2 ** -24, (hidden / 16 + 16) * 2 ** -24 * products.abs().sum(2))
         if c is not None:
             assert torch.equal(grads[2], dy)
