@@ -14,7 +14,11 @@ namespace {
 int refuse(const char* msg) { bb_set_last_error_msg(msg); return BB_ERR_INVALID_ARG; }
 
 constexpr int LIST = 64;                       // tensors of one launch
-constexpr int BLOCK = 256, THREADS = 256, WARPS = THREADS / 32;
+// Ten CTAs of four warps per SM: with moments in 8 bits a warp spends longer between its loads and its stores than in 32, and 48 registers let 40 of
+// them cover that.  150 M parameters, bf16 gradients and working copies, us: 8 bits 354 (6.8 TB/s); eight CTAs 385, twelve (which spill) 400; 32 bits 613
+// whatever the number.  Before, lanes with eight neighbouring values each, exact quotients and a tensor found by comparisons in all lanes (constant
+// memory gives one address at a time): 498.
+constexpr int BLOCK = 256, THREADS = 128, WARPS = THREADS / 32, CTAS = 10;
 constexpr float TOP = 256.f, TINY = 0x1p-100f; // code of a block's largest value; scales up to TINY hold nothing
 constexpr float CODE_MIN = 0x1p-9f;            // smallest e4m3 value above 0
 
@@ -53,7 +57,7 @@ template <bool ROOT> __device__ __forceinline__ uint2 encode(const float* v, flo
   scale = __uint_as_float(top);
   if (top >= 0x7f800000u) { scale = __uint_as_float(0x7fc00000u); return make_uint2(0, 0); }
   if (scale <= TINY) return make_uint2(0, 0);
-  const float f = TOP / scale;
+  const float f = TOP * over(scale);
   float c[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -63,68 +67,74 @@ template <bool ROOT> __device__ __forceinline__ uint2 encode(const float* v, flo
   return make_uint2(pair_code(c[0], c[1]) | pair_code(c[2], c[3]) << 16, pair_code(c[4], c[5]) | pair_code(c[6], c[7]) << 16);
 }
 __device__ __forceinline__ void decode(uint2 q, float scale, float* v) {
-  const float f = scale * (1.f / TOP);
+  const float2 f = make_float2(scale * (1.f / TOP), scale * (1.f / TOP));
   const uint32_t two[4] = {q.x & 0xffffu, q.x >> 16, q.y & 0xffffu, q.y >> 16};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 c = code_pair(two[i]);
-    v[2 * i] = c.x * f; v[2 * i + 1] = c.y * f;
+    const float2 c = bb::mul2(code_pair(two[i]), f);
+    v[2 * i] = c.x; v[2 * i + 1] = c.y;
   }
 }
 
-// A lane's values: all eight at once where the block is whole and the tensors lie on 16 bytes, one by one elsewhere
-template <bool VEC> __device__ __forceinline__ void load8(const float* p, int n, float* v) {
+// A lane's values: four in each half of the block, so that a warp's access is one run of memory; at once where the block is whole and the tensors lie
+// on 16 bytes, one by one elsewhere (value i is the block's (i / 4) 128 + 4 lane + i % 4, of which n are there)
+constexpr int HALF = BLOCK / 2;
+__device__ __forceinline__ int place(int lane, int i) { return (i >> 2) * HALF + 4 * lane + (i & 3); }
+
+template <bool VEC> __device__ __forceinline__ void load8(const float* p, int lane, int n, float* v) {
   if (VEC) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    const float4 a = reinterpret_cast<const float4*>(p)[lane], b = reinterpret_cast<const float4*>(p + HALF)[lane];
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = place(lane, i) < n ? p[place(lane, i)] : 0.f;
   }
 }
-template <bool VEC> __device__ __forceinline__ void load8(const __nv_bfloat16* p, int n, float* v) {
+template <bool VEC> __device__ __forceinline__ void load8(const __nv_bfloat16* p, int lane, int n, float* v) {
   if (VEC) {
-    const uint4 q = *reinterpret_cast<const uint4*>(p);
-    v[0] = bb::bf16_lo(q.x); v[1] = bb::bf16_hi(q.x); v[2] = bb::bf16_lo(q.y); v[3] = bb::bf16_hi(q.y);
-    v[4] = bb::bf16_lo(q.z); v[5] = bb::bf16_hi(q.z); v[6] = bb::bf16_lo(q.w); v[7] = bb::bf16_hi(q.w);
+    const uint2 a = reinterpret_cast<const uint2*>(p)[lane], b = reinterpret_cast<const uint2*>(p + HALF)[lane];
+    v[0] = bb::bf16_lo(a.x); v[1] = bb::bf16_hi(a.x); v[2] = bb::bf16_lo(a.y); v[3] = bb::bf16_hi(a.y);
+    v[4] = bb::bf16_lo(b.x); v[5] = bb::bf16_hi(b.x); v[6] = bb::bf16_lo(b.y); v[7] = bb::bf16_hi(b.y);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? __bfloat162float(p[i]) : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = place(lane, i) < n ? __bfloat162float(p[place(lane, i)]) : 0.f;
   }
 }
-template <bool VEC> __device__ __forceinline__ void store8(float* p, int n, const float* v) {
+template <bool VEC> __device__ __forceinline__ void store8(float* p, int lane, int n, const float* v) {
   if (VEC) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    reinterpret_cast<float4*>(p)[lane] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p + HALF)[lane] = make_float4(v[4], v[5], v[6], v[7]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) if (i < n) p[i] = v[i];
+    for (int i = 0; i < 8; ++i) if (place(lane, i) < n) p[place(lane, i)] = v[i];
   }
 }
-template <bool VEC> __device__ __forceinline__ void store8(__nv_bfloat16* p, int n, const float* v) {
+template <bool VEC> __device__ __forceinline__ void store8(__nv_bfloat16* p, int lane, int n, const float* v) {
   if (VEC) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(bb::pack_bf16x2(v[0], v[1]), bb::pack_bf16x2(v[2], v[3]), bb::pack_bf16x2(v[4], v[5]), bb::pack_bf16x2(v[6], v[7]));
+    reinterpret_cast<uint2*>(p)[lane] = make_uint2(bb::pack_bf16x2(v[0], v[1]), bb::pack_bf16x2(v[2], v[3]));
+    reinterpret_cast<uint2*>(p + HALF)[lane] = make_uint2(bb::pack_bf16x2(v[4], v[5]), bb::pack_bf16x2(v[6], v[7]));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) if (i < n) p[i] = __float2bfloat16(v[i]);
+    for (int i = 0; i < 8; ++i) if (place(lane, i) < n) p[place(lane, i)] = __float2bfloat16(v[i]);
   }
 }
-template <bool VEC> __device__ __forceinline__ uint2 load_codes(const uint8_t* p, int n) {
+template <bool VEC> __device__ __forceinline__ uint2 load_codes(const uint8_t* p, int lane, int n) {
   uint2 q = make_uint2(0, 0);
   if (VEC) {
-    q = *reinterpret_cast<const uint2*>(p);
+    q = make_uint2(reinterpret_cast<const uint32_t*>(p)[lane], reinterpret_cast<const uint32_t*>(p + HALF)[lane]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) if (i < n) (i < 4 ? q.x : q.y) |= (uint32_t)p[i] << (8 * (i & 3));
+    for (int i = 0; i < 8; ++i) if (place(lane, i) < n) (i < 4 ? q.x : q.y) |= (uint32_t)p[place(lane, i)] << (8 * (i & 3));
   }
   return q;
 }
-template <bool VEC> __device__ __forceinline__ void store_codes(uint8_t* p, int n, uint2 q) {
+template <bool VEC> __device__ __forceinline__ void store_codes(uint8_t* p, int lane, int n, uint2 q) {
   if (VEC) {
-    *reinterpret_cast<uint2*>(p) = q;
+    reinterpret_cast<uint32_t*>(p)[lane] = q.x;
+    reinterpret_cast<uint32_t*>(p + HALF)[lane] = q.y;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) if (i < n) p[i] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+    for (int i = 0; i < 8; ++i) if (place(lane, i) < n) p[place(lane, i)] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
   }
 }
 
@@ -134,15 +144,15 @@ __device__ __forceinline__ void block_step(const bb_adamw_tensor& t, long long a
   const long long blocks = (t.numel + BLOCK - 1) / BLOCK;
   float* master = t.master ? t.master : reinterpret_cast<float*>(t.param);
   if (EIGHT) { sm = t.scales[block]; sv = t.scales[blocks + block]; }
-  load8<VEC>(master + at, n, p);
-  if (t.grad_dtype == BB_DTYPE_F32) load8<VEC>(reinterpret_cast<const float*>(t.grad) + at, n, g);
-  else load8<VEC>(reinterpret_cast<const __nv_bfloat16*>(t.grad) + at, n, g);
+  load8<VEC>(master + at, lane, n, p);
+  if (t.grad_dtype == BB_DTYPE_F32) load8<VEC>(reinterpret_cast<const float*>(t.grad) + at, lane, n, g);
+  else load8<VEC>(reinterpret_cast<const __nv_bfloat16*>(t.grad) + at, lane, n, g);
   if (EIGHT) {
-    decode(load_codes<VEC>(reinterpret_cast<const uint8_t*>(t.exp_avg) + at, n), sm, m);
-    decode(load_codes<VEC>(reinterpret_cast<const uint8_t*>(t.exp_avg_sq) + at, n), sv, v);
+    decode(load_codes<VEC>(reinterpret_cast<const uint8_t*>(t.exp_avg) + at, lane, n), sm, m);
+    decode(load_codes<VEC>(reinterpret_cast<const uint8_t*>(t.exp_avg_sq) + at, lane, n), sv, v);
   } else {
-    load8<VEC>(reinterpret_cast<const float*>(t.exp_avg) + at, n, m);
-    load8<VEC>(reinterpret_cast<const float*>(t.exp_avg_sq) + at, n, v);
+    load8<VEC>(reinterpret_cast<const float*>(t.exp_avg) + at, lane, n, m);
+    load8<VEC>(reinterpret_cast<const float*>(t.exp_avg_sq) + at, lane, n, v);
   }
   const float2 b1 = make_float2(a.b1, a.b1), b2 = make_float2(a.b2, a.b2), gs1 = make_float2(gs * a.omb1, gs * a.omb1), gs2 = make_float2(gs, gs);
 #pragma unroll
@@ -158,43 +168,44 @@ __device__ __forceinline__ void block_step(const bb_adamw_tensor& t, long long a
     v[i] = EIGHT ? r.x : v2.x; v[i + 1] = EIGHT ? r.y : v2.y;
     p[i] = q.x; p[i + 1] = q.y;
   }
-  store8<VEC>(master + at, n, p);
-  if (t.master) store8<VEC>(reinterpret_cast<__nv_bfloat16*>(t.param) + at, n, p);
+  store8<VEC>(master + at, lane, n, p);
+  if (t.master) store8<VEC>(reinterpret_cast<__nv_bfloat16*>(t.param) + at, lane, n, p);
   if (a.zero_grad) {
     const float zeros[8] = {};
-    if (t.grad_dtype == BB_DTYPE_F32) store8<VEC>(reinterpret_cast<float*>(t.grad) + at, n, zeros);
-    else store8<VEC>(reinterpret_cast<__nv_bfloat16*>(t.grad) + at, n, zeros);
+    if (t.grad_dtype == BB_DTYPE_F32) store8<VEC>(reinterpret_cast<float*>(t.grad) + at, lane, n, zeros);
+    else store8<VEC>(reinterpret_cast<__nv_bfloat16*>(t.grad) + at, lane, n, zeros);
   }
   if (EIGHT) {
     if (!VEC) {                                // what a partial block has beyond its end decides nothing
 #pragma unroll
-      for (int i = 0; i < 8; ++i) if (i >= n) { m[i] = 0.f; v[i] = 0.f; }
+      for (int i = 0; i < 8; ++i) if (place(lane, i) >= n) { m[i] = 0.f; v[i] = 0.f; }
     }
     const uint2 cm = encode<false>(m, sm), cv = encode<true>(v, sv);
-    store_codes<VEC>(reinterpret_cast<uint8_t*>(t.exp_avg) + at, n, cm);
-    store_codes<VEC>(reinterpret_cast<uint8_t*>(t.exp_avg_sq) + at, n, cv);
+    store_codes<VEC>(reinterpret_cast<uint8_t*>(t.exp_avg) + at, lane, n, cm);
+    store_codes<VEC>(reinterpret_cast<uint8_t*>(t.exp_avg_sq) + at, lane, n, cv);
     if (lane == 0) { t.scales[block] = sm; t.scales[blocks + block] = sv; }
   } else {
-    store8<VEC>(reinterpret_cast<float*>(t.exp_avg) + at, n, m);
-    store8<VEC>(reinterpret_cast<float*>(t.exp_avg_sq) + at, n, v);
+    store8<VEC>(reinterpret_cast<float*>(t.exp_avg) + at, lane, n, m);
+    store8<VEC>(reinterpret_cast<float*>(t.exp_avg_sq) + at, lane, n, v);
   }
 }
 
 template <bool EIGHT>
-__global__ void __launch_bounds__(THREADS, 4)
+__global__ void __launch_bounds__(THREADS, CTAS)
 adamw_list_kernel(const __grid_constant__ AdamTable table, const AdamArgs a) {
   bb::pdl_sync();
   const int lane = threadIdx.x & 31;
-  const int unit = blockIdx.x * WARPS + (threadIdx.x >> 5);
+  const int unit = (gridDim.x - 1 - blockIdx.x) * WARPS + bb::warp_index();         // last ones first: the norm read them last
   if (unit >= table.first[table.count]) return;
-  static_assert(LIST == 64, "two comparisons a lane find the tensor");
-  const int lo = __popc(__ballot_sync(0xffffffffu, table.first[lane] <= unit)) + __popc(__ballot_sync(0xffffffffu, table.first[lane + 32] <= unit)) - 1;
+  int lo = 0;
+#pragma unroll
+  for (int step = LIST / 2; step; step >>= 1) if (table.first[lo + step] <= unit) lo += step;
   const bb_adamw_tensor& t = table.t[lo];
-  const long long block = unit - table.first[lo], at = block * BLOCK + lane * 8, left = t.numel - at;
+  const long long block = unit - table.first[lo], at = block * BLOCK, left = t.numel - at;
   const float gs = a.coef ? a.coef[0] * a.grad_scale : a.grad_scale;
   // `unused` of the table: every tensor of this entry lies on 16 bytes (codes: 8)
-  if (t.unused && t.numel - block * BLOCK >= BLOCK) block_step<EIGHT, true>(t, at, block, 8, lane, a, gs);
-  else block_step<EIGHT, false>(t, at, block, left <= 0 ? 0 : left < 8 ? (int)left : 8, lane, a, gs);
+  if (t.unused && left >= BLOCK) block_step<EIGHT, true>(t, at, block, BLOCK, lane, a, gs);
+  else block_step<EIGHT, false>(t, at, block, left < BLOCK ? (int)left : BLOCK, lane, a, gs);
 }
 
 bool bad_tensor(const bb_adamw_tensor& t, bool eight) {
