@@ -612,7 +612,6 @@ extern "C" int bb_grouped_max_experts(void) { return MAX_EXPERTS; }
 extern "C" int bb_grouped_gemm(const bb_grouped_desc* d, void* stream) {
   if (!d || !d->offsets || ((uintptr_t)d->offsets & 3) || bad_sizes(d))
     return refuse("bb_grouped_gemm: null pointer, a size that is not positive, n or k not a multiple of 8, or more than 256 experts");
-  if (int rc = bbhost::bind_context()) return rc;
   const bool turned = d->mode == BB_GROUPED_INPUT, wgrad = d->mode == BB_GROUPED_WEIGHT;
   if (d->mode != BB_GROUPED_ROWS && !turned && !wgrad) return refuse("bb_grouped_gemm: an unknown mode");
   if (bad_matrix(d->x, d->ld_x, d->mode == BB_GROUPED_ROWS ? d->k : d->n) || bad_matrix(d->weight, wgrad ? d->ld_weight : d->k, d->k) || !d->out ||
@@ -629,6 +628,7 @@ extern "C" int bb_grouped_gemm(const bb_grouped_desc* d, void* stream) {
   if (e == BB_EPI_BIAS_GELU && (!d->out2 || ((uintptr_t)d->out2 & 15))) return refuse("bb_grouped_gemm: the epilogue takes a second output, 16-byte aligned");
   if (e == BB_EPI_MUL_DGELU && bad_matrix(d->aux, d->ld_aux ? d->ld_aux : d->ld_out, d->k))
     return refuse("bb_grouped_gemm: the epilogue takes the pre-activation, 16-byte aligned");
+  if (int rc = bbhost::bind_context()) return rc;
   cudaStream_t s = (cudaStream_t)stream;
   return wgrad ? choose<WGRAD>(d, s) : turned ? choose<ROWS_T>(d, s) : choose<ROWS>(d, s);
 }

@@ -277,6 +277,7 @@ class PipelineEngine:
         if isinstance(self.loss_model, PolicyLoss):
             # it makes its gradient with its value: every micro-batch contributes loss / GAS
             self.loss_model.grad_scale = 1.0 / self.micro_batches
+        self.module.scale_layer_gradients(1.0 / self.micro_batches)
         # what `gradient_clipping` publishes is known by engine, loaded checkpoints and step: engines of one job share a store, and their steps
         # have the same numbers (an engine that is formed anew with its cluster keeps its place)
         if not hasattr(self, "_engine_index"):

@@ -21,6 +21,7 @@ from typing import Iterable, List, Optional
 import torch
 from torch import nn
 
+from . import experts as E
 from . import lib as L
 from .arena import ParamArena  # noqa: F401  (re-exported)
 
@@ -557,6 +558,43 @@ class _CrossEntropyFn(torch.autograd.Function):
         return lg.view(ctx.shape), None, None, None
 
 
+class _RouterFn(torch.autograd.Function):
+    """fp32 logits x W^T of a router: the choice of experts and its weights are not rounded to bf16."""
+
+    @staticmethod
+    def forward(ctx, x, mod, w):
+        _require_cuda(x, "router")
+        x2 = x.reshape(-1, x.shape[-1])
+        if not x2.is_contiguous():
+            x2 = x2.contiguous()
+        y = torch.empty(x2.shape[0], w.shape[0], dtype=torch.float32, device=x.device)
+        L.gemm(x2, w, y, epilogue=L.EPI_STORE_F32)
+        ctx.mod, ctx.shape = mod, x.shape
+        ctx.save_for_backward(x2)
+        return y.view(*x.shape[:-1], w.shape[0])
+
+    @staticmethod
+    def backward(ctx, dy):
+        (x2,) = ctx.saved_tensors
+        d2 = dy.reshape(-1, dy.shape[-1]).to(torch.bfloat16).contiguous()       # (operands of the two products are bf16)
+        return _linear_backward(d2, x2, ctx.mod.gate, None).view(ctx.shape), None, None
+
+
+class _WithTermFn(torch.autograd.Function):
+    """``x`` as it is; in the backward pass ``term`` receives ``weight``, as if weight * term were part of the loss."""
+
+    @staticmethod
+    def forward(ctx, x, term, weight):
+        ctx.weight = weight
+        ctx.save_for_backward(term)
+        return x.view_as(x)
+
+    @staticmethod
+    def backward(ctx, dx):
+        (term,) = ctx.saved_tensors
+        return dx, torch.full_like(term, ctx.weight), None
+
+
 # ----------------------------------------------------------------------------------- modules
 def _normal(shape, gen, std=0.02):
     return torch.randn(shape, generator=gen, dtype=torch.float32) * std
@@ -633,6 +671,38 @@ class MLPHalf(nn.Module):
         if _use_native_blocks():
             return _half(x, self, L.HALF_MLP)
         return _MLPHalfFn.apply(x, self, self.ln2_w, self.ln2_b, self.fc1_w, self.fc1_b, self.fc2_w, self.fc2_b)
+
+
+class ExpertMLPHalf(nn.Module):
+    """The MLP half of a block as a mixture of experts: x + sum over a token's ``k`` best experts of weight * fc2_e(gelu(fc1_e(LN(x)))); after an
+    ``AttentionHalf`` it takes the place of an ``MLPHalf``.
+
+    The router's softmax is over all experts, ``normalize``: over the chosen ones.  ``balance_coef`` times the balance term (``experts.route``) counts as
+    part of the loss: its gradient enters here, times ``balance_grad_scale``, which the pipeline engine sets to 1 / micro-batches; the loss that is reported
+    does not hold it.  ``balance`` keeps the last call's term (device).  ``experts`` is at most 256."""
+
+    def __init__(self, hidden, experts, ffn, k=2, eps=1e-5, seed=0, balance_coef=0.01, normalize=True):
+        super().__init__()
+        if not 0 < k <= min(experts, 32):
+            raise ValueError(f"{k} of {experts} experts")
+        g = torch.Generator().manual_seed(seed)
+        _normal((3 * hidden, hidden), g); _normal((hidden, hidden), g)      # the attention half's draws
+        self.experts, self.k, self.balance_coef, self.normalize, self.balance_grad_scale, self.balance = experts, k, balance_coef, normalize, 1.0, None
+        self.ln = LayerNorm(hidden, eps)
+        gate = torch.zeros((experts + 7) // 8 * 8, hidden)                  # (the kernels' 8-element leading-dimension rule; the rows beyond stay zero)
+        gate[:experts] = _normal((experts, hidden), g)
+        self.gate = nn.Parameter(gate)
+        self.fc1_w = nn.Parameter(_normal((experts, ffn, hidden), g)); self.fc1_b = nn.Parameter(torch.zeros(experts, ffn))
+        self.fc2_w = nn.Parameter(_normal((experts, hidden, ffn), g)); self.fc2_b = nn.Parameter(torch.zeros(experts, hidden))
+
+    def forward(self, x):
+        h = self.ln(x)
+        r = E.route(_RouterFn.apply(h, self, self.gate), self.k, self.experts, normalize=self.normalize)
+        y = E.combine(E.expert_mlp(E.dispatch(h, r), r.offsets, self.fc1_w, self.fc1_b, self.fc2_w, self.fc2_b), r, residual=x)
+        self.balance = r.balance.detach()
+        if self.balance_coef and r.balance.requires_grad:
+            y = _WithTermFn.apply(y, r.balance, self.balance_coef * self.balance_grad_scale)
+        return y
 
 
 class LayerNorm(nn.Module):

@@ -21,7 +21,7 @@ from dataclasses import dataclass
 
 import torch
 
-from .layers import (AttentionHalf, CrossEntropyLoss, LayerNorm, Linear, MLMTransform, MLPHalf, TokenEmbedding,
+from .layers import (AttentionHalf, CrossEntropyLoss, ExpertMLPHalf, LayerNorm, Linear, MLMTransform, MLPHalf, TokenEmbedding,
                      TransformerBlock)
 from .module import LayerSpec
 
@@ -37,6 +37,9 @@ class TransformerConfig:
     causal: bool = True
     vocab_pad: int = 128
     mlm: bool = False
+    experts: int = 0                # > 0: the MLP half of every block is a mixture of that many
+    experts_per_token: int = 2
+    balance_coef: float = 0.01
 
     @property
     def padded_vocab(self):
@@ -44,9 +47,12 @@ class TransformerConfig:
 
     def flops_per_token(self):
         """Training FLOPs per token, dense attention count: 3 * (L*(24h^2 + 4sh) + 2hV), plus
-        2h^2 forward for the masked-LM transform (logits are computed at every position)."""
+        2h^2 forward for the masked-LM transform (logits are computed at every position); with experts, those that a token takes and the router."""
         h = self.hidden
         head = 2 * h * self.vocab + (2 * h * h if self.mlm else 0)
+        if self.experts:            # of 24 h^2, 16 h^2 are the MLP's
+            mlp = 4 * h * self.ffn * self.experts_per_token + 2 * h * self.experts
+            return 3 * (self.layers * (8 * h * h + mlp + 4 * self.seq * h) + head)
         return 3 * (self.layers * (24 * h * h + 4 * self.seq * h) + head)
 
 
@@ -59,11 +65,15 @@ GPT_6_7B = TransformerConfig(layers=32, hidden=4096, heads=32, ffn=16384, seq=20
 
 def transformer_layer_specs(cfg: TransformerConfig, seed: int = 0, split_blocks: bool = False):
     """``split_blocks``: every block becomes two pipeline layers (attention half, MLP half) with
-    the same weights and arithmetic, so that stage boundaries can fall inside a block."""
+    the same weights and arithmetic, so that stage boundaries can fall inside a block (those of a model with experts always are two)."""
     base = seed * 1000
     specs = [LayerSpec(TokenEmbedding, cfg.vocab, cfg.hidden, cfg.seq, seed=base)]
     for i in range(cfg.layers):
-        if split_blocks:
+        if cfg.experts:
+            specs.append(LayerSpec(AttentionHalf, cfg.hidden, cfg.heads, cfg.ffn, causal=cfg.causal, seed=base + 1 + i))
+            specs.append(LayerSpec(ExpertMLPHalf, cfg.hidden, cfg.experts, cfg.ffn, k=cfg.experts_per_token, seed=base + 1 + i,
+                                   balance_coef=cfg.balance_coef))
+        elif split_blocks:
             specs.append(LayerSpec(AttentionHalf, cfg.hidden, cfg.heads, cfg.ffn, causal=cfg.causal, seed=base + 1 + i))
             specs.append(LayerSpec(MLPHalf, cfg.hidden, cfg.heads, cfg.ffn, causal=cfg.causal, seed=base + 1 + i))
         else:

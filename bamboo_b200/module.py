@@ -169,6 +169,17 @@ class PipelineModule(nn.Module):
         return self._compute_parts(self.partition_method, new_num_stages)
 
     # ------------------------------------------------------------------ building stages
+    # factor of the loss terms that layers add in their own backward pass (layers with a ``balance_grad_scale``)
+    layer_grad_scale = 1.0
+
+    def scale_layer_gradients(self, scale):
+        """Set that factor, for the layers that are built and those that will be."""
+        self.layer_grad_scale = scale
+        for stage in self.stages.values():
+            for mod in stage.modules.values():
+                if hasattr(mod, "balance_grad_scale"):
+                    mod.balance_grad_scale = scale
+
     def build_layers(self, stage_id, buffer=None):
         """Instantiate the layers of ``stage_id`` on this rank's device.  ``buffer`` maps
         parameter names to tensors that overwrite the freshly built parameters (promotion
@@ -192,6 +203,8 @@ class PipelineModule(nn.Module):
             elif isinstance(layer, (LayerSpec, nn.Module)):
                 mod = layer.build() if isinstance(layer, LayerSpec) else layer
                 mod = mod.to(self.device)
+                if hasattr(mod, "balance_grad_scale"):
+                    mod.balance_grad_scale = self.layer_grad_scale
                 stage.funcs.append(mod)
                 stage.modules[name] = mod
                 if name not in self._modules:

@@ -1,0 +1,260 @@
+"""What the mixture-of-experts and list-optimizer entry points refuse, and what reaches the native calls, as far as that needs no GPU."""
+import ctypes
+
+import pytest
+import torch
+
+BF16 = torch.bfloat16
+
+
+@pytest.fixture
+def recorded(monkeypatch):
+    """experts and optim with CPU tensors let through; native calls are recorded instead of made."""
+    from bamboo_b200 import experts, lib, optim
+    seen = []
+    for name in ("grouped_gemm", "grouped_colsum", "expert_mlp_fwd", "expert_mlp_bwd", "route_fwd", "route_bwd", "dispatch_rows", "combine_rows", "combine_rows_bwd",
+                 "adamw_list"):
+        monkeypatch.setattr(lib, name, lambda *a, _name=name, **kw: seen.append((_name, a, kw)))
+    for module in (experts, optim):
+        monkeypatch.setattr(module, "_on_current", lambda t, name: None)
+    from bamboo_b200 import post_training
+    monkeypatch.setattr(post_training, "_on_current", lambda t, name: None)
+    return experts, optim, seen
+
+
+def test_cpu_tensors_are_refused():
+    from bamboo_b200 import experts as ex
+    from bamboo_b200 import lib, optim
+    x, w = torch.zeros(4, 8, dtype=BF16), torch.zeros(2, 8, 8, dtype=BF16)
+    offsets, ints = torch.tensor([0, 2, 4]), torch.zeros(4, 1, dtype=torch.int32)
+    r = ex.Routing(torch.zeros(4, 1), ints, ints, ints.view(-1), offsets)
+    for call in (lambda: ex.route(x, 1), lambda: ex.dispatch(x, r), lambda: ex.combine(x, r), lambda: ex.grouped_linear(x, w, offsets),
+                 lambda: ex.expert_mlp(x, offsets, w, w[:, 0], w, w[:, 0]),
+                 lambda: optim.adamw_step_([torch.zeros(4)], [torch.zeros(4)], [torch.zeros(4)], [torch.zeros(4)], step=1)):
+        with pytest.raises(lib.BambooNativeError, match="no CPU fallback"):
+            call()
+
+
+def test_route_refuses(recorded):
+    ex, _, seen = recorded
+    from bamboo_b200 import lib
+    x = torch.zeros(4, 8)
+    for k in (0, 9, -1):
+        with pytest.raises(ValueError, match="k"):
+            ex.route(x, k)
+    with pytest.raises(ValueError, match="k 33"):
+        ex.route(torch.zeros(4, 64), 33)
+    with pytest.raises(ValueError, match="at most 256"):
+        ex.route(torch.zeros(4, 257), 2)
+    with pytest.raises(ValueError, match="does not fit"):
+        ex.route(x, 2, 9)
+    with pytest.raises(lib.BambooNativeError, match="bf16 or fp32"):
+        ex.route(x.half(), 2)
+    assert not seen
+    r = ex.route(x.view(2, 2, 8), 2, 5)
+    assert r.weights.shape == (2, 2, 2) and r.offsets.shape == (6,) and r.slots.shape == (8,)
+    desc = seen[0][1][0]
+    assert (desc.tokens, desc.experts, desc.k, desc.normalize, desc.dtype, desc.ld) == (4, 5, 2, 1, 1, 8)
+
+
+def test_moves_refuse(recorded):
+    ex, _, seen = recorded
+    from bamboo_b200 import lib
+    rows, slots = torch.zeros(4, 2, dtype=torch.int32), torch.zeros(8, dtype=torch.int32)
+    r = ex.Routing(torch.zeros(4, 2), rows, rows, slots, None)
+    for bad in (torch.zeros(5, 8), torch.zeros(3, 8)):
+        with pytest.raises(ValueError, match="4 tokens"):
+            ex.dispatch(bad, r)
+    with pytest.raises(lib.BambooNativeError, match="bf16 or fp32"):
+        ex.dispatch(torch.zeros(4, 8).half(), r)
+    with pytest.raises(ValueError, match="slots"):
+        ex.dispatch(torch.zeros(4, 8), r._replace(slots=slots[:7]))
+    with pytest.raises(TypeError, match="integers"):
+        ex.dispatch(torch.zeros(4, 8), r._replace(rows=rows.float()))
+    for bad in (torch.zeros(7, 8), torch.zeros(4, 2, 8)):
+        with pytest.raises(ValueError, match="8 places"):
+            ex.combine(bad, r)
+    with pytest.raises(ValueError, match="weights"):
+        ex.combine(torch.zeros(8, 8), r._replace(weights=torch.zeros(4, 3)))
+    for bad in (torch.zeros(4, 9), torch.zeros(3, 8), torch.zeros(4, 8, dtype=BF16)):
+        with pytest.raises(ValueError, match="residual"):
+            ex.combine(torch.zeros(8, 8), r, residual=bad)
+    assert not seen
+
+
+def test_products_refuse(recorded):
+    ex, _, seen = recorded
+    from bamboo_b200 import lib
+    x, w, b, offsets = torch.zeros(6, 16, dtype=BF16), torch.zeros(3, 8, 16, dtype=BF16), torch.zeros(3, 8, dtype=BF16), torch.zeros(4, dtype=torch.int32)
+    for bad in (torch.zeros(3, dtype=torch.int32), torch.zeros(5, dtype=torch.int32), torch.zeros(2, 2, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="one more than there are experts"):
+            ex.grouped_linear(x, w, bad, b)
+    with pytest.raises(TypeError, match="integers"):
+        ex.grouped_linear(x, w, offsets.float(), b)
+    for bad in (x.float(), x.half()):
+        with pytest.raises(lib.BambooNativeError, match="bf16"):
+            ex.grouped_linear(bad, w, offsets, b)
+    with pytest.raises(ValueError, match="rows of 16"):
+        ex.grouped_linear(x, torch.zeros(3, 8, 24, dtype=BF16), offsets)
+    with pytest.raises(ValueError, match="multiples of 8"):
+        ex.grouped_linear(x[:, :12], torch.zeros(3, 8, 12, dtype=BF16), offsets)
+    with pytest.raises(ValueError, match="multiples of 8"):
+        ex.grouped_linear(x, torch.zeros(3, 9, 16, dtype=BF16), offsets)
+    with pytest.raises(ValueError, match="1 to 256"):
+        ex.grouped_linear(x, torch.zeros(257, 8, 16, dtype=BF16), torch.zeros(258, dtype=torch.int32))
+    with pytest.raises(ValueError, match="bias"):
+        ex.grouped_linear(x, w, offsets, b[:, :4])
+    with pytest.raises(ValueError, match=r"\[rows, values\]"):
+        ex.grouped_linear(x.view(2, 3, 16), w, offsets)
+    with pytest.raises(ValueError, match=r"\[experts, out, in\]"):
+        ex.grouped_linear(x, w[0], offsets)
+    with pytest.raises(ValueError, match="both biases"):
+        ex.expert_mlp(x, offsets, w, None, torch.zeros(3, 16, 8, dtype=BF16), None)
+    with pytest.raises(ValueError, match="one number of experts"):
+        ex.expert_mlp(x, offsets, w, b, torch.zeros(2, 16, 8, dtype=BF16), b)
+    assert not seen
+    ex.grouped_linear(x, w, offsets.long(), b)
+    assert seen[0][0] == "grouped_gemm" and seen[0][1][3].dtype == torch.int32
+
+
+def test_native_calls_refuse_what_python_would_not_send():
+    from bamboo_b200 import lib
+    handle, at = lib.load(), 1 << 20
+    good = dict(mode=0, rows=64, n=64, k=64, experts=4, epilogue=0, offsets=at, x=at, ld_x=64, weight=at, out=at, ld_out=64)
+    for change in (dict(rows=0), dict(n=60), dict(k=0), dict(experts=257), dict(offsets=None), dict(offsets=at + 2), dict(mode=3), dict(x=at + 8), dict(ld_x=56), dict(ld_x=68),
+                   dict(weight=None), dict(out=None), dict(ld_out=60), dict(epilogue=lib.EPI_BIAS), dict(epilogue=lib.EPI_MUL_DGELU), dict(epilogue=lib.EPI_ACCUM_F32),
+                   dict(epilogue=lib.EPI_BIAS_GELU, bias=at), dict(mode=1, epilogue=lib.EPI_BIAS, bias=at), dict(mode=1, epilogue=lib.EPI_MUL_DGELU),
+                   dict(mode=2, ld_weight=32), dict(mode=2, ld_weight=64, epilogue=lib.EPI_BIAS, bias=at), dict(tile_n=64), dict(tile_n=96), dict(tile_n=128, cta_pair=1)):
+        d = lib.GroupedDesc(**{**good, **change})
+        assert handle.bb_grouped_gemm(ctypes.byref(d), None) == -1 and b"bb_grouped_gemm" in handle.bb_last_error(), change
+    assert handle.bb_grouped_gemm(None, None) == -1 and b"bb_grouped_gemm" in handle.bb_last_error()
+    for args in ((None, 64, at, 4, at, None, 8, 64), (at, 64, at, 4, None, None, 8, 64), (at, 64, at, 4, at, at, 8, 64), (at, 64, at, 0, at, None, 8, 64),
+                 (at, 64, at, 257, at, None, 8, 64), (at, 64, at, 4, at, None, 0, 64), (at, 64, at, 4, at, None, 8, 60), (at, 32, at, 4, at, None, 8, 64)):
+        assert handle.bb_grouped_colsum(*args, None) == -1 and b"bb_grouped_colsum" in handle.bb_last_error(), args
+    route = dict(tokens=16, experts=8, k=2, normalize=1, dtype=0, ld=8)
+    for change in (dict(tokens=0), dict(experts=0), dict(experts=257), dict(k=0), dict(k=9), dict(experts=64, ld=64, k=33), dict(ld=7), dict(dtype=2), dict(tokens=1 << 30, k=4)):
+        d = lib.RouteDesc(**{**route, **change})
+        assert handle.bb_route_workspace_bytes(ctypes.byref(d)) == 0
+        assert handle.bb_route_fwd(ctypes.byref(d), *[at] * 10, 1 << 40, None) == -1, change
+        assert handle.bb_route_bwd(ctypes.byref(d), *[at] * 7, 512, 256, None) == -1, change
+    d = lib.RouteDesc(**route)
+    assert handle.bb_route_fwd(ctypes.byref(d), *[at] * 10, 8, None) == -1 and b"workspace" in handle.bb_last_error()
+    assert handle.bb_route_bwd(ctypes.byref(d), *[at] * 7, 8, 4, None) == -1
+    for args in ((None, 8, 0, at, 2, at, 8, 4, 8), (at, 4, 0, at, 2, at, 8, 4, 8), (at, 8, 2, at, 2, at, 8, 4, 8), (at, 8, 0, at, 0, at, 8, 4, 8), (at, 8, 0, at, 33, at, 8, 4, 8),
+                 (at, 8, 0, at, 2, at, 0, 4, 8), (at, 8, 0, at, 2, at, 8, 0, 8), (at + 1, 8, 0, at, 2, at, 8, 4, 8), (at, 8, 0, at, 2, None, 8, 4, 8)):
+        assert handle.bb_dispatch_rows(*args, None) == -1 and b"bb_dispatch_rows" in handle.bb_last_error(), args
+    assert handle.bb_combine_rows(at, 8, 0, at, at, at, 4, 2, at, 4, 8, 8, None) == -1             # residual rows that overlap
+    assert handle.bb_combine_rows_bwd(at, 8, 0, at, 8, at, at, at, 2, None, None, 4, 8, 8, None) == -1       # nothing asked for
+    assert handle.bb_combine_rows_bwd(at, 8, 0, at, 8, at, at, at, 2, at, at, 4, 9, 8, None) == -1           # more rows than slots
+
+
+def lists(n=3, size=300, bits=32, dtype=torch.float32):
+    moment = torch.float32 if bits == 32 else torch.float8_e4m3fn
+    make = lambda d: [torch.zeros(size, dtype=d) for _ in range(n)]  # noqa: E731
+    return dict(params=make(dtype), grads=make(dtype), exp_avgs=make(moment), exp_avg_sqs=make(moment), scales=None if bits == 32 else
+                [torch.zeros(2, 2) for _ in range(n)], masters=None if dtype == torch.float32 else make(torch.float32))
+
+
+def run(optim, args, **kw):
+    a = dict(args)
+    return optim.adamw_step_(a.pop("params"), a.pop("grads"), a.pop("exp_avgs"), a.pop("exp_avg_sqs"), **{**a, "step": 1, **kw})
+
+
+def test_adamw_refuses(recorded):
+    _, optim, seen = recorded
+    from bamboo_b200 import lib
+    for name in ("grads", "exp_avgs", "exp_avg_sqs", "masters"):
+        args = lists(dtype=BF16)
+        args[name] = args[name][:2]
+        with pytest.raises(ValueError, match=name):
+            run(optim, args)
+        args = lists(dtype=BF16)
+        args[name][1] = args[name][1][:299]
+        with pytest.raises(ValueError, match=name):
+            run(optim, args)
+        args = lists(dtype=BF16)
+        args[name][1] = args[name][1].half()
+        with pytest.raises(lib.BambooNativeError, match=name):
+            run(optim, args)
+        args = lists(dtype=BF16)
+        args[name][1] = torch.zeros(600, dtype=args[name][1].dtype)[::2]
+        with pytest.raises(lib.BambooNativeError, match="contiguous"):
+            run(optim, args)
+    with pytest.raises(lib.BambooNativeError, match="params"):
+        run(optim, {**lists(dtype=BF16), "masters": None})             # bf16 parameters without masters
+    with pytest.raises(lib.BambooNativeError, match="params"):
+        run(optim, {**lists(), "masters": lists()["params"]})
+    with pytest.raises(lib.BambooNativeError, match="exp_avgs"):
+        run(optim, {**lists(), "scales": lists(bits=8)["scales"]})
+    with pytest.raises(ValueError, match="scales"):
+        run(optim, {**lists(bits=8), "scales": [torch.zeros(2, 1)] * 3})
+    twice = lists()
+    twice["params"][2] = twice["params"][0]
+    with pytest.raises(ValueError, match="twice"):
+        run(optim, twice)
+    for kw, what in ((dict(step=0), "step"), (dict(max_norm=-1.0), "max_norm"), (dict(max_norm=float("nan")), "max_norm")):
+        with pytest.raises(ValueError, match=what):
+            run(optim, lists(), **kw)
+    with pytest.raises(lib.BambooNativeError, match="sumsq"):
+        run(optim, lists(), max_norm=1.0, sumsq=torch.zeros(1))
+    assert not seen
+
+
+def test_adamw_leaves_out_what_has_no_gradient(recorded):
+    _, optim, seen = recorded
+    args = lists(4, bits=8)
+    args["grads"][1] = None
+    for name in ("params", "grads", "exp_avgs", "exp_avg_sqs"):
+        args[name][3] = args[name][3][:0]
+    args["scales"][3] = args["scales"][3][:, :0]
+    run(optim, args)
+    (_, (table, count), _), = seen
+    import struct
+    fields = struct.unpack("QQQQQQqiI" * count, table)
+    assert count == 2 and [fields[0], fields[9]] == [args["params"][0].data_ptr(), args["params"][2].data_ptr()]
+    assert [fields[6], fields[15]] == [300, 300] and fields[1] == 0 and fields[5] == args["scales"][0].data_ptr()
+    seen.clear()
+    args["grads"] = [None] * 4
+    assert run(optim, args) is None and run(optim, args, max_norm=1.0) == 0.0 and not seen
+
+
+def test_optimizer_object_refuses(recorded):
+    _, optim, _ = recorded
+    from bamboo_b200 import lib
+    with pytest.raises(ValueError, match="no parameters"):
+        optim.AdamW([])
+    with pytest.raises(ValueError, match="state_bits"):
+        optim.AdamW([torch.zeros(4)], state_bits=16)
+    with pytest.raises(lib.BambooNativeError, match="all fp32 or all bf16"):
+        optim.AdamW([torch.zeros(4), torch.zeros(4, dtype=BF16)])
+    with pytest.raises(ValueError, match="bits"):
+        optim.AdamW([torch.zeros(4)]).load_state_dict(optim.AdamW([torch.zeros(4)], state_bits=8).state_dict())
+    with pytest.raises(ValueError, match="not those of these parameters"):
+        optim.AdamW([torch.zeros(4)]).load_state_dict(optim.AdamW([torch.zeros(5)]).state_dict())
+
+
+def test_models_with_experts():
+    from bamboo_b200 import layers, models
+    cfg = models.TransformerConfig(layers=2, hidden=64, heads=2, ffn=256, seq=32, vocab=100, experts=5, experts_per_token=3)
+    names = [s.typename for s in models.transformer_layer_specs(cfg)]
+    assert names == [layers.TokenEmbedding, layers.AttentionHalf, layers.ExpertMLPHalf, layers.AttentionHalf, layers.ExpertMLPHalf, layers.LayerNorm, layers.Linear]
+    dense = models.TransformerConfig(layers=2, hidden=64, heads=2, ffn=256, seq=32, vocab=100)
+    one = models.TransformerConfig(layers=2, hidden=64, heads=2, ffn=256, seq=32, vocab=100, experts=1, experts_per_token=1)
+    assert one.flops_per_token() - dense.flops_per_token() == 3 * 2 * 2 * 64
+    a, b = (layers.ExpertMLPHalf(64, 5, 256, seed=4) for _ in range(2))
+    assert all(torch.equal(p, q) for p, q in zip(a.parameters(), b.parameters()))
+    assert a.gate.shape == (8, 64) and torch.all(a.gate[5:] == 0)
+    with pytest.raises(ValueError, match="3 of 2"):
+        layers.ExpertMLPHalf(64, 2, 256, k=3)
+
+
+def test_layers_learn_the_engines_factor():
+    from bamboo_b200 import layers
+    from bamboo_b200.module import LayerSpec, PipelineModule
+    m = PipelineModule([LayerSpec(layers.ExpertMLPHalf, 16, 2, 32), LayerSpec(torch.nn.Linear, 4, 4)], num_stages=1, loss_fn=None, partition_method="uniform")
+    layer = next(iter(m.stages[0].modules.values()))
+    assert layer.balance_grad_scale == 1.0
+    m.scale_layer_gradients(0.25)
+    assert layer.balance_grad_scale == 0.25
+    m.build_layers(0)
+    assert next(iter(m.stages[0].modules.values())).balance_grad_scale == 0.25
