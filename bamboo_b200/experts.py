@@ -32,7 +32,12 @@ class Routing(NamedTuple):
 
 
 # ----------------------------------------------------------------------------------- arguments
+_device = torch._C._cuda_getDevice
+
+
 def _int32(t, name, numel=None):
+    if t.dtype is torch.int32 and t.is_cuda and t.get_device() == _device() and t.is_contiguous() and (numel is None or t.numel() == numel):
+        return t
     _on_current(t, name)
     if t.is_floating_point():
         raise TypeError(f"{name}: integers expected, got {t.dtype}")
@@ -45,10 +50,12 @@ def _int32(t, name, numel=None):
 
 def _row_matrix(t, name):
     """(tensor, rows, row width, stride between rows) of [..., h]: as it is where rows have unit stride and one distance, else a copy."""
+    h = t.shape[-1]
+    if h and t.is_contiguous() and t.is_cuda and t.get_device() == _device() and t.dtype in L.dtype_codes():
+        return t, t.numel() // h, h, h
     _on_current(t, name)
     if t.dtype not in L.dtype_codes():
         raise L.BambooNativeError(f"{name}: bf16 or fp32 expected, got {t.dtype}")
-    h = t.shape[-1]
     if h == 0:
         raise ValueError(f"{name}: rows without values")
     if t.is_contiguous():
@@ -61,12 +68,12 @@ def _row_matrix(t, name):
 
 def _plan(routing, tokens=None):
     """(rows, slots, k, tokens) of a routing, checked against each other."""
-    k = routing.rows.shape[-1]
     rows = _int32(routing.rows, "rows")
-    slots = _int32(routing.slots, "slots", rows.numel())
-    if tokens is not None and rows.numel() != tokens * k:
-        raise ValueError(f"a routing of {rows.numel() // k} tokens for {tokens}")
-    return rows, slots, k, rows.numel() // k
+    k, count = rows.shape[-1], rows.numel()
+    slots = _int32(routing.slots, "slots", count)
+    if tokens is not None and count != tokens * k:
+        raise ValueError(f"a routing of {count // k} tokens for {tokens}")
+    return rows, slots, k, count // k
 
 
 # ----------------------------------------------------------------------------------- routing
@@ -91,18 +98,18 @@ def _route(logits, k, experts, normalize):
     slots = torch.empty(tokens * k, dtype=torch.int32, device=dev)
     make = torch.empty if tokens else torch.zeros
     offsets, balance = make(n + 1, dtype=torch.int32, device=dev), make((), dtype=torch.float32, device=dev)
-    stats, load = torch.empty(tokens, 2, dtype=torch.float32, device=dev), torch.empty(n + 1, dtype=torch.float32, device=dev)
+    kept = torch.empty(2 * tokens + n + 1, dtype=torch.float32, device=dev)        # what the backward pass needs of each softmax, then the shares
     desc = _route_desc(tokens, n, k, int(bool(normalize)), L.dtype_codes()[lg.dtype], L._ld(lg) if tokens else lg.shape[-1])
     if tokens:
-        L.route_fwd(desc, lg, weights, experts_out, rows, slots, offsets, balance, stats, load)
-    return lg, desc, weights, balance, experts_out, rows, slots, offsets, stats, load
+        L.route_fwd(desc, lg, weights, experts_out, rows, slots, offsets, balance, kept)
+    return lg, desc, weights, balance, experts_out, rows, slots, offsets, kept
 
 
 class _RouteFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, k, experts, normalize):
-        lg, desc, weights, balance, chosen, rows, slots, offsets, stats, load = _route(logits, k, experts, normalize)
-        ctx.args = desc, stats, load, None if lg is logits else logits.shape
+        lg, desc, weights, balance, chosen, rows, slots, offsets, kept = _route(logits, k, experts, normalize)
+        ctx.args = desc, kept, None if lg is logits else logits.shape
         ctx.save_for_backward(lg, chosen)
         ctx.mark_non_differentiable(chosen, rows, slots, offsets)
         ctx.set_materialize_grads(False)
@@ -112,13 +119,14 @@ class _RouteFn(torch.autograd.Function):
     @_once_differentiable
     def backward(ctx, d_weights, d_balance, *_):
         lg, chosen = ctx.saved_tensors
-        desc, stats, load, shape = ctx.args
+        desc, kept, shape = ctx.args
         if d_weights is None and d_balance is None:
             return None, None, None, None
         out = torch.empty(lg.shape, dtype=lg.dtype, device=lg.device)
         if desc.tokens:
-            d_weights, d_balance = (None if g is None else g.to(torch.float32).contiguous() for g in (d_weights, d_balance))
-            L.route_bwd(desc, lg, chosen, stats, load, d_weights, d_balance, out)
+            if d_weights is not None and not d_weights.is_contiguous():
+                d_weights = d_weights.contiguous()
+            L.route_bwd(desc, lg, chosen, kept, d_weights, d_balance, out)
         return out if shape is None else out.view(shape), None, None, None
 
 

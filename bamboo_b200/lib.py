@@ -868,20 +868,23 @@ def expert_mlp_bwd(desc, x, pre, act, dy, dpre, dx):
                                              _addr(dx), _raw_stream()), "bb_expert_mlp_bwd")
 
 
-def route_fwd(desc, logits, weights, experts, rows, slots, offsets, balance, stats, load_):
+def route_fwd(desc, logits, weights, experts, rows, slots, offsets, balance, kept):
+    """``kept`` [2 tokens + experts + 1] fp32: what route_bwd needs, the softmax statistics and behind them the experts' shares."""
     global LAUNCHES
     LAUNCHES += 2
-    lib = load()
+    lib = _lib or load()
+    at = kept.data_ptr()
     ws = workspace(_bytes_of(desc, lib.bb_route_workspace_bytes), "experts")
     check(lib.bb_route_fwd(ctypes.byref(desc), logits.data_ptr(), weights.data_ptr(), experts.data_ptr(), rows.data_ptr(), slots.data_ptr(),
-                           offsets.data_ptr(), balance.data_ptr(), stats.data_ptr(), load_.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream()),
+                           offsets.data_ptr(), balance.data_ptr(), at, at + 8 * desc.tokens, ws.data_ptr(), ws.numel(), _raw_stream()),
           "bb_route_fwd")
 
 
-def route_bwd(desc, logits, experts, stats, load_, d_weights, d_balance, dlogits):
+def route_bwd(desc, logits, experts, kept, d_weights, d_balance, dlogits):
     global LAUNCHES
     LAUNCHES += 1
-    check((_lib or load()).bb_route_bwd(ctypes.byref(desc), logits.data_ptr(), experts.data_ptr(), stats.data_ptr(), load_.data_ptr(), _addr(d_weights),
+    at = kept.data_ptr()
+    check((_lib or load()).bb_route_bwd(ctypes.byref(desc), logits.data_ptr(), experts.data_ptr(), at, at + 8 * desc.tokens, _addr(d_weights),
                                         _addr(d_balance), dlogits.data_ptr(), _ld(dlogits), dlogits.shape[-1], _raw_stream()), "bb_route_bwd")
     return dlogits
 
