@@ -24,7 +24,8 @@ namespace {
 
 constexpr int BM = 128, BK = 64, UMMA_K = 16;
 constexpr int TMA_WARP_0 = 0, MMA_WARP = 1, TMA_WARP_1 = 2, EPI_WARP = 3, EPI_WARPS = 8;
-constexpr int THREADS = 32 * (EPI_WARP + EPI_WARPS);
+constexpr int SUM_WARP = EPI_WARP + EPI_WARPS;        // weight gradients only
+template <bool WEIGHT> constexpr int THREADS = 32 * (SUM_WARP + (WEIGHT ? 1 : 0));
 constexpr int A_STAGE_BYTES = BM * BK * 2;
 constexpr int SLAB_BYTES = 32 * 128;
 constexpr int MAX_EXPERTS = 256;
@@ -36,7 +37,7 @@ template <int BN, bool PAIR> struct Cfg {
   static constexpr int STAGES = B_ROWS == 256 ? 4 : 6;
   static constexpr int TILE_M = PAIR ? 2 * BM : BM;
   static constexpr int TMEM_COLS = 2 * BN;
-  static constexpr int BAR_BYTES = (3 * STAGES + 4) * 8 + 8;
+  static constexpr int BAR_BYTES = (5 * STAGES + 4) * 8 + 8;
   static constexpr int TABLE_BYTES = (MAX_EXPERTS + 1) * 4 + MAX_EXPERTS;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * SLAB_BYTES + 1024 /*align slack*/ + BAR_BYTES + TABLE_BYTES;
   static_assert(SMEM_BYTES <= 227 * 1024, "fits an SM");
@@ -49,12 +50,14 @@ struct GroupParams {
   int epi;
   const int* offsets;
   void* D; void* D2; const void* bias; const void* aux;
+  __nv_bfloat16* bias_grad; float* bias_accum;            // weight gradient: where db_e goes (one of them, or none) ...
+  float* bias_parts;          // ... by way of [column tiles][experts][n], where there is more than one column of tiles
   long long ldd, ld_aux, expert_stride;       // expert_stride: values of one dW_e
   int* status;
 };
 
 struct Unit {
-  int e, m0, n0;              // first row (a row of x, or of dW_e) and column of the tile
+  int e, ni, m0, n0;          // first row (a row of x, or of dW_e) and column of the tile
   int end;                    // where its rows end
   int k0, num_kb, tail;       // weight gradient: first row of the reduction, rows of the last k-block
 };
@@ -81,7 +84,7 @@ template <bool WGRAD, int BN, int TILE_M> struct Walk {
       tiles = m_tiles * cols;
     }
     const int local = unit - first, ni = local / m_tiles, mi = local - ni * m_tiles;
-    u.n0 = ni * BN;
+    u.ni = ni; u.n0 = ni * BN;
     if constexpr (WGRAD) {
       u.e = order[e];
       const int n = start[u.e + 1] - start[u.e];
@@ -125,8 +128,54 @@ __device__ __forceinline__ void read_offsets(const GroupParams& p, int* start, i
 
 enum { ROWS = 0, ROWS_T = 1, WGRAD = 2 };     // B as stored, B turned, weight gradient
 
+// db_e along with dW_e: one warp adds up rows of dy that stand in shared memory anyway, behind the MMAs that read them (`read_bar`) and in front of the
+// copies that replace them (`summed_bar`).  It takes 1000 cycles for a k-block whose MMAs take 512, so the column tiles that share the rows take
+// their k-blocks in turn - tile i the k-blocks i, i + tiles, ... - and a second kernel adds the tiles' sums in their order (16384 rows of 8 experts,
+// 4096 x 1024, us: 122, of which 108 are the weight gradient's; by the tiles of the first columns alone 169, with a pass of its own 108 + 33).  A lane keeps eight columns of each box and every fourth row.
+struct ColumnSums {
+  float2 v[BM / 64][4];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int b = 0; b < BM / 64; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[b][i] = make_float2(0.f, 0.f);
+  }
+  __device__ __forceinline__ void add(const uint8_t* tile, int rows, int lane) {
+#pragma unroll
+    for (int b = 0; b < BM / 64; ++b)
+#pragma unroll 4
+      for (int r = lane >> 3; r < rows; r += 4) {
+        const uint4 q = *reinterpret_cast<const uint4*>(tile + b * 8192 + slab_off(r, lane & 7));
+        v[b][0] = bb::add2(v[b][0], make_float2(bb::bf16_lo(q.x), bb::bf16_hi(q.x)));
+        v[b][1] = bb::add2(v[b][1], make_float2(bb::bf16_lo(q.y), bb::bf16_hi(q.y)));
+        v[b][2] = bb::add2(v[b][2], make_float2(bb::bf16_lo(q.z), bb::bf16_hi(q.z)));
+        v[b][3] = bb::add2(v[b][3], make_float2(bb::bf16_lo(q.w), bb::bf16_hi(q.w)));
+      }
+  }
+  __device__ __forceinline__ void write(const GroupParams& p, int e, int ni, int m0, int lane) {
+#pragma unroll
+    for (int b = 0; b < BM / 64; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float2 s = v[b][i];
+#pragma unroll
+        for (int d = 8; d < 32; d <<= 1) {
+          s.x += __shfl_xor_sync(0xffffffffu, s.x, d);
+          s.y += __shfl_xor_sync(0xffffffffu, s.y, d);
+        }
+        const int c = m0 + b * 64 + (lane & 7) * 8 + i * 2;
+        if (lane < 8 && c < p.n) {             // (n is even)
+          const long long at = (long long)e * p.n + c;
+          if (p.bias_parts) *reinterpret_cast<float2*>(p.bias_parts + (long long)ni * p.experts * p.n + at) = s;
+          else if (p.bias_accum) { p.bias_accum[at] += s.x; p.bias_accum[at + 1] += s.y; }
+          else { p.bias_grad[at] = __float2bfloat16(s.x); p.bias_grad[at + 1] = __float2bfloat16(s.y); }
+        }
+      }
+  }
+};
+
 template <int MODE, int BN, bool PAIR>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(THREADS<MODE == WGRAD>, 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GroupParams p) {
   using C = Cfg<BN, PAIR>;
   extern __shared__ uint8_t smem_raw[];
@@ -137,7 +186,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(panels + EPI_WARPS * SLAB_BYTES);      // [STAGES]
   uint64_t* empty_bar = full_bar + C::STAGES;       // [STAGES]
   uint64_t* clean_bar = empty_bar + C::STAGES;      // [STAGES] pairs: the other CTA's overhanging rows are zeros
-  uint64_t* tmem_full = clean_bar + C::STAGES;      // [2]
+  uint64_t* read_bar = clean_bar + C::STAGES;       // [STAGES] weight gradient: the MMAs have read a stage that is to be summed
+  uint64_t* summed_bar = read_bar + C::STAGES;      // [STAGES] ... and its rows are added up
+  uint64_t* tmem_full = summed_bar + C::STAGES;     // [2]
   uint64_t* tmem_empty = tmem_full + 2;             // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -152,7 +203,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int s = 0; s < C::STAGES; ++s) { bb::mbar_init(&full_bar[s], 1); bb::mbar_init(&empty_bar[s], 1); bb::mbar_init(&clean_bar[s], 1); }
+    for (int s = 0; s < C::STAGES; ++s) { bb::mbar_init(&full_bar[s], 1); bb::mbar_init(&empty_bar[s], 1); bb::mbar_init(&clean_bar[s], 1); bb::mbar_init(&read_bar[s], 1); bb::mbar_init(&summed_bar[s], 1); }
     for (int a = 0; a < 2; ++a) { bb::mbar_init(&tmem_full[a], 1); bb::mbar_init(&tmem_empty[a], (PAIR ? 2 : 1) * EPI_WARPS); }
     bb::fence_barrier_init();
     bb::tma_prefetch_desc(&tmA);
@@ -171,7 +222,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const uint32_t tmem_base = *tmem_slot;
   if constexpr (MODE == WGRAD) {
     // longest reductions first: the last units of a launch are then the short ones
-    for (int e = threadIdx.x; e < p.experts; e += THREADS) {
+    for (int e = threadIdx.x; e < p.experts; e += THREADS<true>) {
       const int n = start[e + 1] - start[e];
       int at = 0;
       for (int i = 0; i < p.experts; ++i) {
@@ -184,7 +235,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   } else {
     // rows that belong to no expert
     const int before = start[0], after = p.rows - start[p.experts], chunks = p.n >> 3;
-    for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < (long long)(before + after) * chunks; i += (long long)gridDim.x * THREADS) {
+    for (long long i = (long long)blockIdx.x * THREADS<false> + threadIdx.x; i < (long long)(before + after) * chunks; i += (long long)gridDim.x * THREADS<false>) {
       const int r = (int)(i / chunks), c = (int)(i - (long long)r * chunks);
       reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.D) + (long long)(r < before ? r : start[p.experts] + r - before) * p.ldd)[c] =
           make_uint4(0, 0, 0, 0);
@@ -192,18 +243,30 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
   Walk<MODE == WGRAD, BN, C::TILE_M> walk(p, start, order, worker, workers);
   Unit u;
+  const bool with_bias = MODE == WGRAD && (p.bias_grad || p.bias_accum);
 
   if (warp == TMA_WARP_0 || warp == TMA_WARP_1) {
     // ------------------------------------------------ producers: the stages in turn
     static_assert(C::STAGES % 2 == 0, "the producers take the stages in turn");
     const int turn = warp == TMA_WARP_1 ? 1 : 0;
-    int s = 0; uint32_t phase = 0;
+    int s = 0; uint32_t phase = 0, summing = 0, summed_phase = 0;       // summing: stages whose last rows are (or were) added up
     bool alive = true;
+    auto wait_summed = [&]() {
+      if (!(MODE == WGRAD && ((summing >> s) & 1u))) return true;
+      const bool got = bb::mbar_wait_warp(&summed_bar[s], (summed_phase >> s) & 1u, abort_flag, p.status);
+      summed_phase ^= 1u << s;
+      summing &= ~(1u << s);
+      return got;
+    };
     while (alive && walk.next(u)) {
       const int m0 = u.m0 + (int)rank * BM, n0 = u.n0 + (int)rank * C::B_ROWS;
+      int next_sum = with_bias ? u.ni : -1;
       for (int kb = 0; kb < u.num_kb; ++kb) {
+        const bool sums = MODE == WGRAD && kb == next_sum;
+        if (sums) next_sum += walk.cols;
         if ((s & 1) == turn) {
-          if (!bb::mbar_wait_warp(&empty_bar[s], phase ^ 1, abort_flag, p.status)) { alive = false; break; }
+          if (!bb::mbar_wait_warp(&empty_bar[s], phase ^ 1, abort_flag, p.status) || !wait_summed()) { alive = false; break; }
+          if (sums) summing |= 1u << s;
           uint8_t* a = sA + s * A_STAGE_BYTES;
           uint8_t* b = sB + s * C::B_STAGE_BYTES;
           const int k0 = u.k0 + kb * BK;
@@ -247,7 +310,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     if constexpr (PAIR) {
       // rank 0's commits arrive on this CTA's barriers too: none may still be on its way when the CTA leaves
       for (int i = 0; i < C::STAGES && alive; ++i) {
-        if ((s & 1) == turn && !bb::mbar_wait_warp(&empty_bar[s], phase ^ 1, abort_flag, p.status)) alive = false;
+        if ((s & 1) == turn && (!bb::mbar_wait_warp(&empty_bar[s], phase ^ 1, abort_flag, p.status) || !wait_summed())) alive = false;
         if (++s == C::STAGES) { s = 0; phase ^= 1; }
       }
     }
@@ -288,7 +351,10 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       if (!bb::mbar_wait_warp(&tmem_empty[acc], acc_phase ^ 1, abort_flag, p.status)) { alive = false; break; }
       bb::tc_fence_after_sync();
       const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
+      int next_sum = with_bias ? u.ni : -1;
       for (int kb = 0; kb < u.num_kb; ++kb) {
+        const bool sums = MODE == WGRAD && kb == next_sum;
+        if (sums) next_sum += walk.cols;
         if (!bb::mbar_wait_warp(&full_bar[s], phase, abort_flag, p.status)) { alive = false; break; }
         int steps = BK / UMMA_K;
         if (MODE == WGRAD && kb == u.num_kb - 1) {
@@ -313,6 +379,10 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             if (PAIR) bb::umma_f16_pair(d_tmem, ad, bd, IDESC, (kb > 0 || k > 0) ? 1u : 0u);
             else bb::umma_f16(d_tmem, ad, bd, IDESC, (kb > 0 || k > 0) ? 1u : 0u);
           }
+          if (sums) {
+            if (PAIR) bb::umma_commit_pair(&read_bar[s], 3);
+            else bb::umma_commit(&read_bar[s]);
+          }
           if (PAIR) {
             bb::umma_commit_pair(&empty_bar[s], 3);
             if (kb == u.num_kb - 1) bb::umma_commit_pair(&tmem_full[acc], 3);
@@ -325,6 +395,24 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         if (++s == C::STAGES) { s = 0; phase ^= 1; }
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+    }
+  } else if (MODE == WGRAD && warp == SUM_WARP) {
+    // ------------------------------------------------ bias gradient
+    int s = 0; uint32_t read_phase = 0;
+    bool alive = with_bias;
+    while (alive && walk.next(u)) {
+      ColumnSums sums;
+      sums.clear();
+      for (int kb = u.ni; kb < u.num_kb; kb += walk.cols) {
+        const int st = (s + kb) % C::STAGES;
+        if (!bb::mbar_wait_warp(&read_bar[st], (read_phase >> st) & 1u, abort_flag, p.status)) { alive = false; break; }
+        read_phase ^= 1u << st;
+        sums.add(sA + st * A_STAGE_BYTES, kb == u.num_kb - 1 ? u.tail : BK, lane);
+        __syncwarp();
+        if (lane == 0) bb::mbar_arrive(&summed_bar[st]);
+      }
+      s = (s + u.num_kb) % C::STAGES;
+      if (alive) sums.write(p, u.e, u.ni, u.m0 + (int)rank * BM, lane);
     }
   } else {
     // ------------------------------------------------ epilogue: eight warps, two per TMEM lane quarter, panels of 128 bytes in turn
@@ -445,10 +533,23 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
 }
 
+// The column tiles' sums (see ColumnSums), in their order
+__global__ void __launch_bounds__(256)
+grouped_bias_join_kernel(const float* parts, int tiles, long long values, __nv_bfloat16* out, float* accum) {
+  bb::pdl_sync();
+  const long long i = blockIdx.x * 256LL + threadIdx.x;
+  if (i >= values) return;
+  float s = 0.f;
+#pragma unroll 4
+  for (int t = 0; t < tiles; ++t) s += parts[t * values + i];
+  if (accum) accum[i] += s;
+  else out[i] = __float2bfloat16(s);
+}
+
 // ---------------------------------------------------------------- bias gradients
-// db_e = sum of its rows of dy.  A cluster of CTAs shares an expert's rows for 128 columns: every CTA sums a run of them (16 rows of 256 bytes at a
-// time, four such steps in flight), the first adds the CTAs' sums in their order through distributed shared memory.  Bound by memory: 16384 rows of
-// 4096, 8 experts COLSUM_US.
+// db_e = sum of its rows of dy, where no weight gradient carries it along.  A cluster of CTAs shares an expert's rows for 128 columns: every CTA sums a run of them (16 rows of 256 bytes at a
+// time, four such steps in flight), the first adds the CTAs' sums in their order through distributed shared memory.  16384 rows of 4096, 8 experts, 30 us
+// (4.4 TB/s): a CTA's start and the two cluster barriers weigh on runs of 256 rows; longer ones leave SMs idle (four CTAs an expert 31, two 42).
 constexpr int COLSUM_COLS = 128, COLSUM_MOST = 8, COLSUM_U = 4;
 
 __device__ __forceinline__ int clamped(const int* offsets, int e, int rows) {
@@ -529,6 +630,8 @@ int launch(const bb_grouped_desc* d, cudaStream_t stream) {
   p.rows = d->rows; p.experts = d->experts; p.epi = d->epilogue; p.offsets = d->offsets;
   p.D = d->out; p.D2 = d->out2; p.bias = d->bias; p.aux = d->aux;
   p.ldd = d->ld_out; p.ld_aux = d->ld_aux ? d->ld_aux : d->ld_out;
+  const int bias_tiles = d->bias_grad || d->bias_accum ? (d->k + BN - 1) / BN : 0;
+  p.bias_grad = (__nv_bfloat16*)d->bias_grad; p.bias_accum = d->bias_accum; p.bias_parts = bias_tiles > 1 ? d->bias_parts : nullptr;
   p.status = bb_device_status_word();
   int rc;
   long long tiles;
@@ -553,7 +656,7 @@ int launch(const bb_grouped_desc* d, cudaStream_t stream) {
   if (workers < 1) workers = 1;
   if (d->max_ctas < 0 || tiles < workers) workers = tiles < 1 ? 1 : (int)tiles;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((PAIR ? 2 : 1) * workers); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = C::SMEM_BYTES; cfg.stream = stream;
+  cfg.gridDim = dim3((PAIR ? 2 : 1) * workers); cfg.blockDim = dim3(THREADS<MODE == WGRAD>); cfg.dynamicSmemBytes = C::SMEM_BYTES; cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
@@ -564,7 +667,13 @@ int launch(const bb_grouped_desc* d, cudaStream_t stream) {
     if (!cfg.numAttrs) attr[0] = attr[1];
     ++cfg.numAttrs;
   }
+  BackToBack overlap(bias_tiles > 1 && d->max_ctas == 0);
   BB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, grouped_gemm_kernel<MODE, BN, PAIR>, tmA, tmB, p));
+  if (bias_tiles > 1) {
+    const long long values = (long long)d->experts * d->n;
+    BB_CUDA_CHECK(bb_launch(grouped_bias_join_kernel, (unsigned)((values + 255) / 256), 256, 0, stream, (const float*)p.bias_parts, bias_tiles, values, p.bias_grad,
+                            p.bias_accum));
+  }
   return BB_OK;
 }
 
@@ -609,6 +718,10 @@ bool bad_matrix(const void* p, long long ld, int cols) { return !p || ((uintptr_
 
 extern "C" int bb_grouped_max_experts(void) { return MAX_EXPERTS; }
 
+extern "C" long long bb_grouped_bias_bytes(int n, int k, int experts) {
+  return n <= 0 || k <= 0 || experts <= 0 ? 0 : 4LL * ((k + 127) / 128) * experts * n;
+}
+
 extern "C" int bb_grouped_gemm(const bb_grouped_desc* d, void* stream) {
   if (!d || !d->offsets || ((uintptr_t)d->offsets & 3) || bad_sizes(d))
     return refuse("bb_grouped_gemm: null pointer, a size that is not positive, n or k not a multiple of 8, or more than 256 experts");
@@ -619,6 +732,10 @@ extern "C" int bb_grouped_gemm(const bb_grouped_desc* d, void* stream) {
     return refuse("bb_grouped_gemm: operands are 16-byte aligned, with rows of a multiple of 8 values that do not overlap");
   if ((d->tile_n != 0 && d->tile_n != 128 && d->tile_n != 256) || (d->cta_pair > 0 && d->tile_n == 128))
     return refuse("bb_grouped_gemm: tile_n is 128 or 256, of a CTA pair 256");
+  if ((d->bias_grad || d->bias_accum) && (!wgrad || (d->bias_grad && d->bias_accum) || ((uintptr_t)d->bias_grad & 1) || ((uintptr_t)d->bias_accum & 3)))
+    return refuse("bb_grouped_gemm: a bias gradient goes with a weight gradient, to one place");
+  if ((d->bias_grad || d->bias_accum) && (!d->bias_parts || ((uintptr_t)d->bias_parts & 15) || d->bias_parts_bytes < bb_grouped_bias_bytes(d->n, d->k, d->experts)))
+    return refuse("bb_grouped_gemm: a bias gradient takes bb_grouped_bias_bytes() of scratch");
   const int e = d->epilogue;
   if (wgrad ? (e != BB_EPI_STORE && e != BB_EPI_ACCUM_F32)
             : turned ? (e != BB_EPI_STORE && e != BB_EPI_MUL_DGELU) : (e != BB_EPI_STORE && e != BB_EPI_BIAS && e != BB_EPI_BIAS_GELU))
@@ -665,7 +782,8 @@ int weight_and_bias(const bb_expert_mlp_desc* m, const void* dy, long long ld_dy
   if (dw || g_w) {
     bb_grouped_desc d = part_of(m, BB_GROUPED_WEIGHT, n, k, g_w ? BB_EPI_ACCUM_F32 : BB_EPI_STORE);
     d.x = dy; d.ld_x = ld_dy; d.weight = x; d.ld_weight = ld_x; d.out = g_w ? (void*)g_w : dw;
-    if (int rc = bb_grouped_gemm(&d, stream)) return rc;
+    d.bias_accum = g_b; d.bias_grad = g_b ? nullptr : db; d.bias_parts = m->scratch; d.bias_parts_bytes = m->scratch_bytes;
+    return bb_grouped_gemm(&d, stream);
   }
   if (db || g_b) return bb_grouped_colsum(dy, ld_dy, m->offsets, m->experts, g_b ? nullptr : db, g_b, m->rows, n, stream);
   return BB_OK;

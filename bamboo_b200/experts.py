@@ -276,21 +276,19 @@ def _product(mode, x, w, offsets, width, **kw):
 
 def _weight_gradients(dy, x, offsets, weight, bias, need_w, need_b):
     """(gradient of the weight, of the bias) for autograd; where a parameter belongs to an arena, its fp32 ``main_grad`` is added to instead (None)."""
-    dw = db = None
-    empty = dy.shape[0] == 0
-    if need_w:
-        main = getattr(weight, "main_grad", None)
-        if main is None:
-            dw = (torch.zeros if empty else torch.empty)(weight.shape, dtype=torch.bfloat16, device=dy.device)
-        if not empty:
-            L.grouped_gemm(L.GROUPED_WEIGHT, dy, x, offsets, dw if main is None else main, epilogue=L.EPI_STORE if main is None else L.EPI_ACCUM_F32)
-    if need_b:
-        main = getattr(bias, "main_grad", None)
-        if main is None:
-            db = (torch.zeros if empty else torch.empty)(bias.shape, dtype=torch.bfloat16, device=dy.device)
-        if not empty:
-            L.grouped_colsum(dy, offsets, bias.shape[0], out=db, accum=main)
-    return dw, db
+    grads, empty = {}, dy.shape[0] == 0
+    places = {}
+    for name, p, wanted in (("weight", weight, need_w), ("bias", bias, need_b)):
+        main = getattr(p, "main_grad", None) if wanted else None
+        grads[name] = (torch.zeros if empty else torch.empty)(p.shape, dtype=torch.bfloat16, device=dy.device) if wanted and main is None else None
+        places[name] = main
+    if need_w and not empty:
+        main = places["weight"]
+        L.grouped_gemm(L.GROUPED_WEIGHT, dy, x, offsets, grads["weight"] if main is None else main, epilogue=L.EPI_STORE if main is None else L.EPI_ACCUM_F32,
+                       bias_grad=grads["bias"], bias_accum=places["bias"])
+    elif need_b and not empty:
+        L.grouped_colsum(dy, offsets, bias.shape[0], out=grads["bias"], accum=places["bias"])
+    return grads["weight"], grads["bias"]
 
 
 class _GroupedLinearFn(torch.autograd.Function):
@@ -337,9 +335,9 @@ def _mlp_operands(x, w1, b1, w2, b2):
     return (_grouped_rows(x), _weight(w1, "w1", x.shape[-1]), _bias(b1, "b1", w1), _weight(w2, "w2", w1.shape[1]), _bias(b2, "b2", w2))
 
 
-def _mlp_desc(x, w1, b1, w2, b2, offsets):
-    return L.ExpertMLPDesc(rows=x.shape[0], inputs=x.shape[1], inner=w1.shape[1], outputs=w2.shape[1], experts=w1.shape[0], max_ctas=L.GEMM_MAX_CTAS,
-                           offsets=offsets.data_ptr(), w1=w1.data_ptr(), b1=b1.data_ptr(), w2=w2.data_ptr(), b2=b2.data_ptr())
+def _mlp_desc(x, w1, b1, w2, b2, offsets, *gradients):
+    return L.ExpertMLPDesc(*x.shape, w1.shape[1], w2.shape[1], w1.shape[0], L.GEMM_MAX_CTAS, offsets.data_ptr(), w1.data_ptr(), b1.data_ptr(), w2.data_ptr(),
+                           b2.data_ptr(), *gradients)
 
 
 def _mlp_forward(x, w1, b1, w2, b2, offsets):
@@ -348,7 +346,7 @@ def _mlp_forward(x, w1, b1, w2, b2, offsets):
     kept = torch.empty(2, rows, inner, dtype=torch.bfloat16, device=x.device)
     y = torch.empty(rows, w2.shape[1], dtype=torch.bfloat16, device=x.device)
     if rows:
-        L.expert_mlp_fwd(_mlp_desc(x, w1, b1, w2, b2, offsets), x, kept[0], kept[1], y)
+        L.expert_mlp_fwd(_mlp_desc(x, w1, b1, w2, b2, offsets), x, kept, y)
     return kept, y
 
 
@@ -368,20 +366,25 @@ class _ExpertMLPFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         dy = _grouped_rows(dy, "gradient")
         rows, dev = x.shape[0], x.device
-        desc = _mlp_desc(x, w1, b1, w2, b2, offsets)
-        grads = []
-        for name, p, wanted in zip(("w1", "b1", "w2", "b2"), ctx.parameters, need[1:5]):
-            main = getattr(p, "main_grad", None) if wanted else None
-            g = (torch.empty if rows else torch.zeros)(p.shape, dtype=torch.bfloat16, device=dev) if wanted and main is None else None
-            if g is not None:
-                setattr(desc, "d" + name, g.data_ptr())
-            elif wanted:
-                setattr(desc, "g_" + name, main.data_ptr())
+        grads, to, added = [], [None] * 4, [None] * 4                # gradients for autograd, and addresses: of those, or of arena gradients
+        for at, p in enumerate(ctx.parameters):
+            g = None
+            if need[1 + at]:
+                main = getattr(p, "main_grad", None)
+                if main is None:
+                    g = (torch.empty if rows else torch.zeros)(p.shape, dtype=torch.bfloat16, device=dev)
+                    to[at] = g.data_ptr()
+                else:
+                    added[at] = main.data_ptr()
             grads.append(g)
         dx = torch.empty(rows, x.shape[1], dtype=torch.bfloat16, device=dev) if need[0] else None
         if rows:
-            dpre = torch.empty(rows, w1.shape[1], dtype=torch.bfloat16, device=dev) if any(need[:3]) else None
-            L.expert_mlp_bwd(desc, x, kept[0], kept[1], dy, dpre, dx)
+            inner = w1.shape[1]
+            first = need[0] or need[1] or need[2]
+            behind = (2 * rows * inner + 255) & ~255 if first else 0         # the gradient of the pre-activation, then scratch of the bias gradients
+            size = L.expert_mlp_scratch(x.shape[1], inner, w2.shape[1], w1.shape[0])
+            work = torch.empty(behind + size, dtype=torch.uint8, device=dev)
+            L.expert_mlp_bwd(_mlp_desc(x, w1, b1, w2, b2, offsets, *to, *added, work.data_ptr() + behind, size), x, kept, dy, work.data_ptr() if first else None, dx)
         return dx, *grads, None
 
 

@@ -100,6 +100,7 @@ class GroupedDesc(ctypes.Structure):
         ("bias", ctypes.c_void_p), ("out2", ctypes.c_void_p),
         ("aux", ctypes.c_void_p), ("ld_aux", ctypes.c_longlong),
         ("max_ctas", ctypes.c_int), ("tile_n", ctypes.c_int), ("cta_pair", ctypes.c_int),
+        ("bias_grad", ctypes.c_void_p), ("bias_accum", ctypes.c_void_p), ("bias_parts", ctypes.c_void_p), ("bias_parts_bytes", ctypes.c_longlong),
     ]
 
 
@@ -111,6 +112,7 @@ class ExpertMLPDesc(ctypes.Structure):
         ("w1", ctypes.c_void_p), ("b1", ctypes.c_void_p), ("w2", ctypes.c_void_p), ("b2", ctypes.c_void_p),
         ("dw1", ctypes.c_void_p), ("db1", ctypes.c_void_p), ("dw2", ctypes.c_void_p), ("db2", ctypes.c_void_p),
         ("g_w1", ctypes.c_void_p), ("g_b1", ctypes.c_void_p), ("g_w2", ctypes.c_void_p), ("g_b2", ctypes.c_void_p),
+        ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_longlong),
     ]
 
 
@@ -185,6 +187,7 @@ def load():
         lib.bb_grad_clip.argtypes = [vp, i, vp, d, vp, vp, ll, vp]
         lib.bb_adam_step_clipped.argtypes = [vp] * 5 + [ll, d, d, d, d, i, i, i, d, d, i, vp, d, vp, vp, ll, vp]
         lib.bb_grouped_gemm.argtypes = [vp, vp]
+        lib.bb_grouped_bias_bytes.argtypes, lib.bb_grouped_bias_bytes.restype = [i, i, i], ll
         lib.bb_grouped_colsum.argtypes = [vp, ll, vp, i, vp, vp, i, i, vp]
         lib.bb_expert_mlp_fwd.argtypes = [vp, vp, ll, vp, vp, vp, vp]
         lib.bb_expert_mlp_bwd.argtypes = [vp, vp, ll, vp, vp, vp, ll, vp, vp, vp]
@@ -827,17 +830,29 @@ def adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, *, lr, beta1=
 
 
 # ---------------------------------------------------------------------------- mixture of experts
-def grouped_gemm(mode, x, weight, offsets, out, *, epilogue=EPI_STORE, bias=None, out2=None, aux=None, max_ctas=0, tile_n=0, cta_pair=0):
+def grouped_bias_scratch(n, k, experts):
+    """What a bias gradient that comes with a weight gradient [experts, n, k] needs."""
+    return workspace((_lib or load()).bb_grouped_bias_bytes(n, k, experts), "experts")
+
+
+def grouped_gemm(mode, x, weight, offsets, out, *, epilogue=EPI_STORE, bias=None, out2=None, aux=None, max_ctas=0, tile_n=0, cta_pair=0, bias_grad=None,
+                 bias_accum=None):
     """GROUPED_ROWS: x [rows, k], weight [experts, n, k], out [rows, n]; GROUPED_INPUT: x [rows, n], out [rows, k]; GROUPED_WEIGHT: x [rows, n],
     weight [rows, k], out [experts, n, k].  2-D tensors have unit inner stride, rows on 16 bytes; see bb_grouped_gemm."""
     global LAUNCHES
     LAUNCHES += 1
     wgrad = mode == GROUPED_WEIGHT
     experts, n, k = out.shape if wgrad else weight.shape
+    parts = parts_bytes = 0
+    if bias_grad is not None or bias_accum is not None:
+        LAUNCHES += 1
+        ws = grouped_bias_scratch(n, k, experts)
+        parts, parts_bytes = ws.data_ptr(), ws.numel()
     d = GroupedDesc(mode=mode, rows=x.shape[0], n=n, k=k, experts=experts, epilogue=epilogue, offsets=offsets.data_ptr(), x=x.data_ptr(),
                     ld_x=_ld(x), weight=weight.data_ptr(), ld_weight=_ld(weight) if wgrad else 0, out=out.data_ptr(),
                     ld_out=0 if wgrad else _ld(out), bias=_addr(bias), out2=_addr(out2), aux=_addr(aux), ld_aux=0 if aux is None else _ld(aux),
-                    max_ctas=max_ctas or GEMM_MAX_CTAS, tile_n=tile_n, cta_pair=cta_pair)
+                    max_ctas=max_ctas or GEMM_MAX_CTAS, tile_n=tile_n, cta_pair=cta_pair, bias_grad=_addr(bias_grad), bias_accum=_addr(bias_accum),
+                    bias_parts=parts, bias_parts_bytes=parts_bytes)
     check((_lib or load()).bb_grouped_gemm(ctypes.byref(d), _raw_stream()), "bb_grouped_gemm")
     return out
 
@@ -851,20 +866,30 @@ def grouped_colsum(dy, offsets, experts, out=None, accum=None):
           "bb_grouped_colsum")
 
 
-def expert_mlp_fwd(desc, x, pre, act, y):
+def expert_mlp_fwd(desc, x, kept, y):
+    """``kept`` [2, rows, inner]: pre-activation and activation, for the backward pass."""
     global LAUNCHES
     LAUNCHES += 2
-    check((_lib or load()).bb_expert_mlp_fwd(ctypes.byref(desc), x.data_ptr(), _ld(x), pre.data_ptr(), act.data_ptr(), y.data_ptr(), _raw_stream()),
+    at = kept.data_ptr()
+    check((_lib or load()).bb_expert_mlp_fwd(ctypes.byref(desc), x.data_ptr(), _ld(x), at, at + 2 * desc.rows * desc.inner, y.data_ptr(), _raw_stream()),
           "bb_expert_mlp_fwd")
     return y
 
 
-def expert_mlp_bwd(desc, x, pre, act, dy, dpre, dx):
-    """Gradients as the descriptor asks for them; dpre and dx may be None (see bb_expert_mlp_bwd)."""
+@functools.lru_cache(maxsize=256)
+def expert_mlp_scratch(inputs, inner, outputs, experts):
+    """Bytes of scratch for the bias gradients that come with weight gradients."""
+    ask = load().bb_grouped_bias_bytes
+    return max(ask(inner, inputs, experts), ask(outputs, inner, experts))
+
+
+def expert_mlp_bwd(desc, x, kept, dy, dpre, dx):
+    """Gradients as the descriptor asks for them; dpre (an address) and dx may be None (see bb_expert_mlp_bwd)."""
     global LAUNCHES
     LAUNCHES += (dpre is not None) + (dx is not None) + sum(bool(getattr(desc, a) or getattr(desc, b)) for a, b in
                                                           (("dw1", "g_w1"), ("db1", "g_b1"), ("dw2", "g_w2"), ("db2", "g_b2")))
-    check((_lib or load()).bb_expert_mlp_bwd(ctypes.byref(desc), x.data_ptr(), _ld(x), pre.data_ptr(), act.data_ptr(), dy.data_ptr(), _ld(dy), _addr(dpre),
+    at = kept.data_ptr()
+    check((_lib or load()).bb_expert_mlp_bwd(ctypes.byref(desc), x.data_ptr(), _ld(x), at, at + 2 * desc.rows * desc.inner, dy.data_ptr(), _ld(dy), dpre,
                                              _addr(dx), _raw_stream()), "bb_expert_mlp_bwd")
 
 

@@ -439,10 +439,14 @@ typedef struct bb_grouped_desc {
   int max_ctas;                                 /* see bb_gemm_desc.max_ctas */
   int tile_n;                                   /* 0 = choose, else 128 or 256 columns */
   int cta_pair;                                 /* 0 = choose, 1 = CTA pairs (256 x 256 tiles), -1 = single CTAs */
+  void* bias_grad; float* bias_accum;           /* BB_GROUPED_WEIGHT: also the sum of every expert's rows of x, to one of them: bf16 [experts, n], or
+                                                   fp32 [experts, n] (+=); NULL: not wanted */
+  float* bias_parts; long long bias_parts_bytes;/* scratch for it, bb_grouped_bias_bytes() */
 } bb_grouped_desc;
+long long bb_grouped_bias_bytes(int n, int k, int experts);
 int bb_grouped_max_experts(void);
 int bb_grouped_gemm(const bb_grouped_desc* d, void* stream);
-/* Bias gradients of such a layer: out_bf16[e, n] = sum of its rows of dy, or accum[e, n] (fp32) += it; a fixed order of additions. */
+/* Bias gradients of such a layer without its weight gradients: out_bf16[e, n] = sum of its rows of dy, or accum[e, n] (fp32) += it; a fixed order of additions. */
 int bb_grouped_colsum(const void* dy, long long ld, const int* offsets, int experts, void* out_bf16, float* accum, int rows, int n, void* stream);
 
 /* Two such layers with a tanh GeLU between, one call each way: y = W2 gelu(W1 x + b1) + b2 per expert.  w1 [experts, inner, in], b1 [experts, inner],
@@ -455,6 +459,7 @@ typedef struct bb_expert_mlp_desc {
   const void *w1, *b1, *w2, *b2;
   void *dw1, *db1, *dw2, *db2;
   float *g_w1, *g_b1, *g_w2, *g_b2;
+  float* scratch; long long scratch_bytes;      /* where bias gradients come with weight gradients: the larger bb_grouped_bias_bytes() of the two layers */
 } bb_expert_mlp_desc;
 int bb_expert_mlp_fwd(const bb_expert_mlp_desc* m, const void* x, long long ld_x, void* pre, void* act, void* y, void* stream);
 int bb_expert_mlp_bwd(const bb_expert_mlp_desc* m, const void* x, long long ld_x, const void* pre, const void* act, const void* dy, long long ld_dy, void* dpre,

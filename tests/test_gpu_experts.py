@@ -400,6 +400,26 @@ def test_grouped_linear_on_every_kind_of_tile(ex, tile, lengths, before, after, 
     test_grouped_linear(ex, lengths, before, after, n, k, True)
 
 
+@pytest.mark.parametrize("rows,experts,n", [(1, 1, 8), (700, 3, 136), (5000, 1, 264), (3000, 40, 1032), (9, 4, 4096)])
+def test_a_bias_that_is_trained_alone(ex, rows, experts, n):
+    cuts = sorted(torch.randint(0, rows + 1, (experts - 1,), generator=torch.Generator().manual_seed(rows)).tolist())
+    at = [0] + cuts + [rows]
+    offsets = torch.tensor(at, dtype=torch.int32, device="cuda")
+    x, w = randn(rows, 64, seed=1, dtype=BF16), randn(experts, n, 64, seed=2, dtype=BF16)
+    bias, dy = randn(experts, n, seed=3, dtype=BF16).requires_grad_(True), randn(rows, n, seed=4, dtype=BF16)
+    y = ex.grouped_linear(x, w, offsets, bias)
+    (got,) = torch.autograd.grad(y, bias, dy, retain_graph=True)
+    arena = torch.nn.Parameter(bias.detach())
+    arena.main_grad = randn(experts, n, seed=5)
+    before = arena.main_grad.clone()
+    ex.grouped_linear(x, w, offsets, arena).backward(dy)
+    for e, (a, b) in enumerate(zip(at, at[1:])):
+        d = dy[a:b].double()
+        want = Bound(d.sum(0), (b - a + 24) * 2 ** -24 * d.abs().sum(0))
+        want.rounded().check(got[e])
+        Bound(want.value + before[e].double(), want.err + 2 ** -23 * (want.value.abs() + before[e].double().abs())).check(arena.main_grad[e])
+
+
 @pytest.mark.parametrize("tile", TILES, indirect=True)
 def test_an_experts_gradient_does_not_see_its_neighbours_values(ex, tile):
     """Infinities and NaN in one expert's rows stay in its results: in the reduction over rows too, where tiles overhang."""
