@@ -223,9 +223,9 @@ bool aligned(const bb_adamw_tensor& t, bool eight) {
 extern "C" int bb_adamw_list(const bb_adamw_tensor* tensors, int count, double lr, double beta1, double beta2, double eps, long long step,
                              double weight_decay, double grad_scale, int zero_grad, double max_norm, const double* sumsq, float* norm, void* workspace,
                              long long workspace_bytes, void* stream) {
-  if (!tensors || count <= 0 || step < 1 || !(max_norm >= 0.0) ||
+  if (!tensors || count <= 0 || step < 1 || !(max_norm >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0) ||
       (max_norm > 0.0 && (!norm || !workspace || ((uintptr_t)workspace & 7) || workspace_bytes < bb_grad_norm_workspace_bytes())))
-    return refuse("bb_adamw_list: an empty list, step < 1, a negative norm, or clipping without a place for the norm or with a workspace that is too small");
+    return refuse("bb_adamw_list: an empty list, step < 1, a beta outside [0, 1), a negative norm, or clipping without a place for the norm or with a workspace that is too small");
   const bool eight = tensors[0].scales != nullptr;
   for (int i = 0; i < count; ++i)
     if (bad_tensor(tensors[i], eight))

@@ -711,7 +711,7 @@ template <int MODE> int choose(const bb_grouped_desc* d, cudaStream_t stream) {
 }
 
 bool bad_sizes(const bb_grouped_desc* d) {
-  return d->rows <= 0 || d->n <= 0 || d->k <= 0 || (d->n & 7) || (d->k & 7) || d->experts <= 0 || d->experts > MAX_EXPERTS;
+  return d->rows <= 0 || d->rows > INT_MAX - 1024 || d->n <= 0 || d->k <= 0 || (d->n & 7) || (d->k & 7) || d->experts <= 0 || d->experts > MAX_EXPERTS;
 }
 bool bad_matrix(const void* p, long long ld, int cols) { return !p || ((uintptr_t)p & 15) || ld < cols || (ld & 7); }
 }  // namespace

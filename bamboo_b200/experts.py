@@ -32,6 +32,7 @@ class Routing(NamedTuple):
 
 
 # ----------------------------------------------------------------------------------- arguments
+_MOST = 2 ** 31 - 1025          # rows and places are counted in 32 bits
 _device = torch._C._cuda_getDevice
 
 
@@ -98,8 +99,11 @@ def _route(logits, k, experts, normalize):
     slots = torch.empty(tokens * k, dtype=torch.int32, device=dev)
     make = torch.empty if tokens else torch.zeros
     offsets, balance = make(n + 1, dtype=torch.int32, device=dev), make((), dtype=torch.float32, device=dev)
-    kept = torch.empty(2 * tokens + n + 1, dtype=torch.float32, device=dev)        # what the backward pass needs of each softmax, then the shares
+    if tokens * k > _MOST:
+        raise ValueError(f"{tokens} tokens with {k} experts each: at most {_MOST} rows")
     desc = _route_desc(tokens, n, k, int(bool(normalize)), L.dtype_codes()[lg.dtype], L._ld(lg) if tokens else lg.shape[-1])
+    # what the backward pass needs of each softmax, then the shares, then scratch of this call (no buffer that calls share: a captured one keeps its own)
+    kept = torch.empty(2 * tokens + n + 1 + L.route_scratch(desc) // 4, dtype=torch.float32, device=dev)
     if tokens:
         L.route_fwd(desc, lg, weights, experts_out, rows, slots, offsets, balance, kept)
     return lg, desc, weights, balance, experts_out, rows, slots, offsets, kept
@@ -264,6 +268,8 @@ def _grouped_rows(x, name="x"):
         raise L.BambooNativeError(f"{name}: bf16 expected, got {x.dtype}")
     if x.dim() != 2:
         raise ValueError(f"{name} {tuple(x.shape)}: [rows, values] is expected")
+    if x.shape[0] > _MOST:
+        raise ValueError(f"{name}: {x.shape[0]} rows, at most {_MOST}")
     return _aligned_rows(x, x.shape[1])[0]
 
 
@@ -274,18 +280,28 @@ def _product(mode, x, w, offsets, width, **kw):
     return out
 
 
+def _arena_gradient(p):
+    """``main_grad`` of a parameter, None where it has none; what the kernels add to is contiguous fp32 of the parameter's shape on 16 bytes."""
+    main = getattr(p, "main_grad", None)
+    if main is not None and (main.dtype != torch.float32 or main.shape != p.shape or main.get_device() != p.get_device() or not main.is_contiguous() or
+                             main.data_ptr() % 16):
+        raise L.BambooNativeError(f"main_grad {tuple(main.shape)} {main.dtype}: contiguous fp32 like the parameter {tuple(p.shape)} is expected, on 16 bytes")
+    return main
+
+
 def _weight_gradients(dy, x, offsets, weight, bias, need_w, need_b):
     """(gradient of the weight, of the bias) for autograd; where a parameter belongs to an arena, its fp32 ``main_grad`` is added to instead (None)."""
     grads, empty = {}, dy.shape[0] == 0
     places = {}
     for name, p, wanted in (("weight", weight, need_w), ("bias", bias, need_b)):
-        main = getattr(p, "main_grad", None) if wanted else None
+        main = _arena_gradient(p) if wanted else None
         grads[name] = (torch.zeros if empty else torch.empty)(p.shape, dtype=torch.bfloat16, device=dy.device) if wanted and main is None else None
         places[name] = main
     if need_w and not empty:
         main = places["weight"]
+        scratch = torch.empty(L.grouped_bias_scratch(*weight.shape), dtype=torch.uint8, device=dy.device) if need_b else None
         L.grouped_gemm(L.GROUPED_WEIGHT, dy, x, offsets, grads["weight"] if main is None else main, epilogue=L.EPI_STORE if main is None else L.EPI_ACCUM_F32,
-                       bias_grad=grads["bias"], bias_accum=places["bias"])
+                       bias_grad=grads["bias"], bias_accum=places["bias"], bias_parts=scratch)
     elif need_b and not empty:
         L.grouped_colsum(dy, offsets, bias.shape[0], out=grads["bias"], accum=places["bias"])
     return grads["weight"], grads["bias"]
@@ -370,7 +386,7 @@ class _ExpertMLPFn(torch.autograd.Function):
         for at, p in enumerate(ctx.parameters):
             g = None
             if need[1 + at]:
-                main = getattr(p, "main_grad", None)
+                main = _arena_gradient(p)
                 if main is None:
                     g = (torch.empty if rows else torch.zeros)(p.shape, dtype=torch.bfloat16, device=dev)
                     to[at] = g.data_ptr()

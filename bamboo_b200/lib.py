@@ -791,11 +791,15 @@ def grad_tensors(fields, count):
 _norm_bytes = None
 
 
-def grad_norm_workspace():
+def grad_norm_bytes():
     global _norm_bytes
     if _norm_bytes is None:
         _norm_bytes = load().bb_grad_norm_workspace_bytes()
-    return workspace(_norm_bytes, "grad_norm")
+    return _norm_bytes
+
+
+def grad_norm_workspace():
+    return workspace(grad_norm_bytes(), "grad_norm")
 
 
 def grad_sumsq(table, count):
@@ -830,29 +834,26 @@ def adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, *, lr, beta1=
 
 
 # ---------------------------------------------------------------------------- mixture of experts
-def grouped_bias_scratch(n, k, experts):
-    """What a bias gradient that comes with a weight gradient [experts, n, k] needs."""
-    return workspace((_lib or load()).bb_grouped_bias_bytes(n, k, experts), "experts")
+@functools.lru_cache(maxsize=256)
+def grouped_bias_scratch(experts, n, k):
+    """Bytes of scratch for a bias gradient that comes with a weight gradient [experts, n, k]."""
+    return load().bb_grouped_bias_bytes(n, k, experts)
 
 
 def grouped_gemm(mode, x, weight, offsets, out, *, epilogue=EPI_STORE, bias=None, out2=None, aux=None, max_ctas=0, tile_n=0, cta_pair=0, bias_grad=None,
-                 bias_accum=None):
+                 bias_accum=None, bias_parts=None):
     """GROUPED_ROWS: x [rows, k], weight [experts, n, k], out [rows, n]; GROUPED_INPUT: x [rows, n], out [rows, k]; GROUPED_WEIGHT: x [rows, n],
     weight [rows, k], out [experts, n, k].  2-D tensors have unit inner stride, rows on 16 bytes; see bb_grouped_gemm."""
     global LAUNCHES
     LAUNCHES += 1
     wgrad = mode == GROUPED_WEIGHT
     experts, n, k = out.shape if wgrad else weight.shape
-    parts = parts_bytes = 0
-    if bias_grad is not None or bias_accum is not None:
-        LAUNCHES += 1
-        ws = grouped_bias_scratch(n, k, experts)
-        parts, parts_bytes = ws.data_ptr(), ws.numel()
+    LAUNCHES += bias_parts is not None
     d = GroupedDesc(mode=mode, rows=x.shape[0], n=n, k=k, experts=experts, epilogue=epilogue, offsets=offsets.data_ptr(), x=x.data_ptr(),
                     ld_x=_ld(x), weight=weight.data_ptr(), ld_weight=_ld(weight) if wgrad else 0, out=out.data_ptr(),
                     ld_out=0 if wgrad else _ld(out), bias=_addr(bias), out2=_addr(out2), aux=_addr(aux), ld_aux=0 if aux is None else _ld(aux),
                     max_ctas=max_ctas or GEMM_MAX_CTAS, tile_n=tile_n, cta_pair=cta_pair, bias_grad=_addr(bias_grad), bias_accum=_addr(bias_accum),
-                    bias_parts=parts, bias_parts_bytes=parts_bytes)
+                    bias_parts=_addr(bias_parts), bias_parts_bytes=0 if bias_parts is None else bias_parts.numel())
     check((_lib or load()).bb_grouped_gemm(ctypes.byref(d), _raw_stream()), "bb_grouped_gemm")
     return out
 
@@ -879,8 +880,7 @@ def expert_mlp_fwd(desc, x, kept, y):
 @functools.lru_cache(maxsize=256)
 def expert_mlp_scratch(inputs, inner, outputs, experts):
     """Bytes of scratch for the bias gradients that come with weight gradients."""
-    ask = load().bb_grouped_bias_bytes
-    return max(ask(inner, inputs, experts), ask(outputs, inner, experts))
+    return max(grouped_bias_scratch(experts, inner, inputs), grouped_bias_scratch(experts, outputs, inner))
 
 
 def expert_mlp_bwd(desc, x, kept, dy, dpre, dx):
@@ -893,15 +893,20 @@ def expert_mlp_bwd(desc, x, kept, dy, dpre, dx):
                                              _addr(dx), _raw_stream()), "bb_expert_mlp_bwd")
 
 
+def route_scratch(desc):
+    """Bytes of scratch for route_fwd."""
+    return _bytes_of(desc, (_lib or load()).bb_route_workspace_bytes)
+
+
 def route_fwd(desc, logits, weights, experts, rows, slots, offsets, balance, kept):
-    """``kept`` [2 tokens + experts + 1] fp32: what route_bwd needs, the softmax statistics and behind them the experts' shares."""
+    """``kept``: 2 tokens + experts + 1 fp32 values that route_bwd needs, the softmax statistics and behind them the experts' shares, then scratch."""
     global LAUNCHES
     LAUNCHES += 2
     lib = _lib or load()
     at = kept.data_ptr()
-    ws = workspace(_bytes_of(desc, lib.bb_route_workspace_bytes), "experts")
+    scratch = at + 4 * (2 * desc.tokens + desc.experts + 1)
     check(lib.bb_route_fwd(ctypes.byref(desc), logits.data_ptr(), weights.data_ptr(), experts.data_ptr(), rows.data_ptr(), slots.data_ptr(),
-                           offsets.data_ptr(), balance.data_ptr(), at, at + 8 * desc.tokens, ws.data_ptr(), ws.numel(), _raw_stream()),
+                           offsets.data_ptr(), balance.data_ptr(), at, at + 8 * desc.tokens, scratch, route_scratch(desc), _raw_stream()),
           "bb_route_fwd")
 
 
@@ -953,10 +958,10 @@ def adamw_tensors(fields, count):
     return _adamw_table(count).pack(*fields)
 
 
-def adamw_list(table, count, *, lr, beta1, beta2, eps, step, weight_decay, grad_scale, zero_grad, max_norm, sumsq, norm):
+def adamw_list(table, count, *, lr, beta1, beta2, eps, step, weight_decay, grad_scale, zero_grad, max_norm, sumsq, norm, scratch):
+    """``norm`` and ``scratch`` (grad_norm_bytes()): where it clips."""
     global LAUNCHES
     clip = max_norm > 0
     LAUNCHES += -(-count // ADAMW_LIST) + (0 if not clip else 1 if sumsq is not None else -(-count // 128))
-    ws = grad_norm_workspace() if clip else None
     check((_lib or load()).bb_adamw_list(table, count, lr, beta1, beta2, eps, step, weight_decay, grad_scale, int(zero_grad), max_norm, _addr(sumsq), _addr(norm),
-                                         _addr(ws), ws.numel() if clip else 0, _raw_stream()), "bb_adamw_list")
+                                         _addr(scratch), 0 if scratch is None else scratch.numel(), _raw_stream()), "bb_adamw_list")

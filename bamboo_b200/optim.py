@@ -55,6 +55,8 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, scales=None, masters=No
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if step < 1:
         raise ValueError(f"step counts from 1, got {step}")
+    if not (0 <= beta1 < 1 and 0 <= beta2 < 1):
+        raise ValueError(f"beta1 {beta1}, beta2 {beta2}: from 0 to below 1")
     lists = [grads, *(None if column is None else list(column) for column in (exp_avgs, exp_avg_sqs, scales, masters))]
     for name, column in zip(("grads", "exp_avgs", "exp_avg_sqs", "scales", "masters"), lists):
         if column is not None and len(column) != len(params):
@@ -83,10 +85,14 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, scales=None, masters=No
         addresses, nothing if masters is None else _column(masters, "masters", count, _FP32, sizes, device), _column(grads, "grads", count, _EITHER, sizes, device),
         _column(exp_avgs, "exp_avgs", count, moments, sizes, device), _column(exp_avg_sqs, "exp_avg_sqs", count, moments, sizes, device),
         nothing if scales is None else _column(scales, "scales", count, _FP32, None, device), sizes, map(L.dtype_codes().get, map(_dtype_of, grads)), nothing))
-    norm = torch.empty((), dtype=torch.float32, device=params[0].device) if max_norm > 0 else None
-    L.adamw_list(L.adamw_tensors(fields, count), count, lr=lr, beta1=beta1, beta2=beta2, eps=eps, step=step, weight_decay=weight_decay,
-                 grad_scale=grad_scale, zero_grad=zero_grad, max_norm=max_norm, sumsq=sumsq, norm=norm)
-    torch.autograd.graph.increment_version(params)
+    norm = scratch = None
+    if max_norm > 0:            # (no buffer that calls share: a captured one keeps its own)
+        norm = torch.empty((), dtype=torch.float32, device=params[0].device)
+        scratch = torch.empty(L.grad_norm_bytes(), dtype=torch.uint8, device=params[0].device)
+    L.adamw_list(L.adamw_tensors(fields, count), count, lr=float(lr), beta1=float(beta1), beta2=float(beta2), eps=float(eps), step=int(step),
+                 weight_decay=float(weight_decay), grad_scale=float(grad_scale), zero_grad=zero_grad, max_norm=float(max_norm), sumsq=sumsq, norm=norm,
+                 scratch=scratch)
+    torch.autograd.graph.increment_version(params + grads if zero_grad else params)
     return norm
 
 

@@ -124,7 +124,9 @@ def test_native_calls_refuse_what_python_would_not_send():
     for change in (dict(rows=0), dict(n=60), dict(k=0), dict(experts=257), dict(offsets=None), dict(offsets=at + 2), dict(mode=3), dict(x=at + 8), dict(ld_x=56), dict(ld_x=68),
                    dict(weight=None), dict(out=None), dict(ld_out=60), dict(epilogue=lib.EPI_BIAS), dict(epilogue=lib.EPI_MUL_DGELU), dict(epilogue=lib.EPI_ACCUM_F32),
                    dict(epilogue=lib.EPI_BIAS_GELU, bias=at), dict(mode=1, epilogue=lib.EPI_BIAS, bias=at), dict(mode=1, epilogue=lib.EPI_MUL_DGELU),
-                   dict(mode=2, ld_weight=32), dict(mode=2, ld_weight=64, epilogue=lib.EPI_BIAS, bias=at), dict(tile_n=64), dict(tile_n=96), dict(tile_n=128, cta_pair=1)):
+                   dict(mode=2, ld_weight=32), dict(mode=2, ld_weight=64, epilogue=lib.EPI_BIAS, bias=at), dict(tile_n=64), dict(tile_n=96), dict(tile_n=128, cta_pair=1), dict(rows=2 ** 31 - 1), dict(bias_grad=at),
+                   dict(mode=2, ld_weight=64, bias_grad=at), dict(mode=2, ld_weight=64, bias_grad=at, bias_parts=at, bias_parts_bytes=64),
+                   dict(mode=2, ld_weight=64, bias_grad=at, bias_accum=at, bias_parts=at, bias_parts_bytes=1 << 30)):
         d = lib.GroupedDesc(**{**good, **change})
         assert handle.bb_grouped_gemm(ctypes.byref(d), None) == -1 and b"bb_grouped_gemm" in handle.bb_last_error(), change
     assert handle.bb_grouped_gemm(None, None) == -1 and b"bb_grouped_gemm" in handle.bb_last_error()
@@ -192,7 +194,8 @@ def test_adamw_refuses(recorded):
     twice["params"][2] = twice["params"][0]
     with pytest.raises(ValueError, match="twice"):
         run(optim, twice)
-    for kw, what in ((dict(step=0), "step"), (dict(max_norm=-1.0), "max_norm"), (dict(max_norm=float("nan")), "max_norm")):
+    for kw, what in ((dict(step=0), "step"), (dict(max_norm=-1.0), "max_norm"), (dict(max_norm=float("nan")), "max_norm"), (dict(beta1=1.0), "beta1"),
+                     (dict(beta2=-0.1), "beta2")):
         with pytest.raises(ValueError, match=what):
             run(optim, lists(), **kw)
     with pytest.raises(lib.BambooNativeError, match="sumsq"):
@@ -258,3 +261,24 @@ def test_layers_learn_the_engines_factor():
     assert layer.balance_grad_scale == 0.25
     m.build_layers(0)
     assert next(iter(m.stages[0].modules.values())).balance_grad_scale == 0.25
+
+
+def test_arena_gradients_that_kernels_could_not_add_to(recorded):
+    ex, _, _ = recorded
+    from bamboo_b200 import lib
+    for bad in (torch.zeros(2, 8, 8, dtype=BF16), torch.zeros(2, 8, 9), torch.zeros(2, 8, 16)[..., ::2], torch.zeros(129)[1:].view(2, 8, 8)):
+        p = torch.nn.Parameter(torch.zeros(2, 8, 8, dtype=BF16))
+        p.main_grad = bad
+        with pytest.raises(lib.BambooNativeError, match="main_grad"):
+            ex._arena_gradient(p)
+    p.main_grad = torch.zeros(2, 8, 8)
+    assert ex._arena_gradient(p) is p.main_grad
+
+
+def test_constants_given_as_tensors(recorded):
+    _, optim, seen = recorded
+    value = torch.tensor(0.25)
+    for want in (0.25, 0.5):
+        value.fill_(want)
+        run(optim, lists(), lr=value, weight_decay=value, beta1=value, grad_scale=value)
+        assert [seen[-1][2][n] for n in ("lr", "weight_decay", "beta1", "grad_scale")] == [want] * 4

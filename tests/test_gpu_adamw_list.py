@@ -274,3 +274,38 @@ def test_a_captured_step_replays(optim):
         p.grad = torch.ones(8, device="cuda")
         with torch.cuda.graph(other):
             opt.step()
+
+
+def test_a_tensor_of_more_than_32_bits(optim):
+    n = 2 ** 31 + 1000
+    p, g = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda", dtype=BF16)
+    m, v = (torch.zeros(n, device="cuda", dtype=E4M3) for _ in range(2))
+    s = torch.zeros(2, -(-n // BLOCK), device="cuda")
+    ends = torch.tensor([0, 255, 2 ** 31 - 1, 2 ** 31, n - 1], device="cuda")
+    g[ends] = 1.0
+    optim.adamw_step_([p], [g], [m], [v], scales=[s], step=1, lr=0.5)
+    near(p[ends], torch.full((5,), -0.5, device="cuda", dtype=torch.float64), 2 ** -19)
+    assert torch.all(m[ends].float() == 256) and torch.all(v[ends].float() == 256)
+    assert torch.count_nonzero(p) == 5 and torch.count_nonzero(s) == 2 * 4
+
+
+def test_two_captured_clipped_steps_at_once(optim):
+    sets = [Lists([300_000, 17, 5000], BF16, [BF16] * 3, 8, seed=s) for s in (21, 22)]
+    eager = [Lists([300_000, 17, 5000], BF16, [BF16] * 3, 8, seed=s) for s in (21, 22)]
+    graphs = []
+    for l in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            norm = l.step(optim, step=5, max_norm=0.5)
+        graphs.append((graph, norm, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for graph, _, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for (_, norm, _), l, e in zip(graphs, sets, eager):
+        for _ in range(4):
+            want = e.step(optim, step=5, max_norm=0.5)
+        assert norm.item() == want.item()
+        assert all(torch.equal(a, b) for a, b in zip(l.masters, e.masters))

@@ -664,3 +664,77 @@ def test_second_derivatives_and_overwritten_inputs_are_refused(ex):
     x.zero_()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_two_captured_graphs_at_once(ex):
+    """Nothing is shared between captured calls: replays on two streams beside each other, and beside eager calls that need larger scratch."""
+    up = torch.tensor(0.5, device="cuda")
+    graphs = []
+    for seed in (131, 141):
+        leaves = [t.requires_grad_(True) for t in mixture_inputs(600, 128, 256, 7, seed=seed)]
+        dy = randn(600, 128, seed=seed + 9, dtype=BF16)
+
+        def step(leaves=leaves, dy=dy):
+            y, r = mixture(ex, *leaves, 2)
+            return [y.detach(), *torch.autograd.grad((y, r.balance), leaves, (dy, up))]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = [t.clone() for t in step()]
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        graphs.append((graph, want, got, torch.cuda.Stream()))
+    big = [t.requires_grad_(True) for t in mixture_inputs(3000, 256, 512, 9, seed=151)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, _, _, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        y, r = mixture(ex, *big, 3)
+        torch.autograd.grad(y, big[2], torch.ones_like(y))
+    torch.cuda.synchronize()
+    for _, want, got, _ in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_offsets_beyond_32_bits(ex):
+    """More than 2^31 values in what is read and written."""
+    tokens, k, h = 70_000, 8, 4096
+    r = ex.route(randn(tokens, 16, seed=161), k)
+    x = randn(tokens, h, seed=162, dtype=BF16)
+    xs = ex.dispatch(x, r)
+    assert xs.numel() > 2 ** 31
+    at = torch.tensor([0, 1, tokens * k // 2, tokens * k - 2, tokens * k - 1], device="cuda")
+    assert torch.equal(xs[at], x[r.slots[at].long() // k])
+    y = ex.combine(xs, r._replace(weights=torch.full_like(r.weights, 1 / 8)))
+    assert torch.equal(y, x)                                             # (eight times an eighth of the same row)
+    weights = torch.full_like(r.weights, 0.5).requires_grad_(True)
+    leaf = xs.requires_grad_(True)
+    dxs, dw = torch.autograd.grad(ex.combine(leaf, r._replace(weights=weights)), (leaf, weights), x)
+    assert torch.equal(dxs[at], x[r.slots[at].long() // k] * 0.5)
+    near(dw[-1], x[-1].double().square().sum().expand(k), 2 ** -24, (h / 16 + 16) * 2 ** -24 * x[-1].double().square().sum())
+    del xs, leaf, dxs, y
+    rows, n, kk = 140_000, 16384, 64
+    cuts = torch.tensor([0, 60_001, 60_001, 139_990], dtype=torch.int32, device="cuda")
+    x, w = randn(rows, kk, seed=163, dtype=BF16), randn(3, n, kk, seed=164, dtype=BF16)
+    y = ex.grouped_linear(x, w, cuts)
+    for a, e in ((0, 0), (60_000, 0), (60_001, 2), (139_989, 2)):
+        matmul(Bound(x[a:a + 1].double()), Bound(w[e].double().t())).rounded().check(y[a:a + 1])
+    assert torch.all(y[139_990:] == 0)
+    dx, dw, = torch.autograd.grad(ex.grouped_linear(a := x.clone().requires_grad_(True), b := w.clone().requires_grad_(True), cuts), (a, b), y)
+    matmul(Bound(y[139_989:139_990].double()), Bound(w[2].double())).rounded().check(dx[139_989:139_990])
+    matmul(Bound(y[60_001:139_990, -8:].double().t()), Bound(x[60_001:139_990].double())).rounded().check(dw[2, -8:])
+    del y, dx, dw, x, w
+    e, n, kk = 256, 4096, 2064                                           # the weights
+    cuts = torch.arange(0, 2 * e + 1, 2, dtype=torch.int32, device="cuda")
+    x, dy = randn(2 * e, kk, seed=165, dtype=BF16), randn(2 * e, n, seed=166, dtype=BF16)
+    w = torch.zeros(e, n, kk, dtype=BF16, device="cuda")
+    w[-1] = randn(n, kk, seed=167)
+    w.requires_grad_(True)
+    assert w.numel() > 2 ** 31
+    y = ex.grouped_linear(x, w, cuts)
+    matmul(Bound(x[-2:].double()), Bound(w[-1].detach().double().t())).rounded().check(y[-2:].detach())
+    (dw,) = torch.autograd.grad(y, w, dy)
+    matmul(Bound(dy[-2:].double().t()), Bound(x[-2:].double())).rounded().check(dw[-1])
