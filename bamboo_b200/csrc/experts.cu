@@ -54,7 +54,7 @@ template <typename T, int PER> __device__ __forceinline__ void load_run(const T*
         v[0] = row[first];
       }
 #pragma unroll
-      for (int i = 0; i < PER; ++i) x[i] = value_of(v[i]);
+      for (int i = 0; i < PER; ++i) x[i] = first + i < n ? value_of(v[i]) : -INFINITY;         // (a run may go on into the padding)
       return;
     }
 #pragma unroll
@@ -77,77 +77,139 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// A warp per token, PER consecutive logits a lane; k rounds of a warp-wide maximum, which goes to the first lane and there the first logit that has it.
-// Then the block's slots are ranked within their experts, in order: every warp counts a run of them, and ranks it behind the runs before.
+// One instruction each besides a product: arguments are at most 0 where it matters (a probability of e^-30 is off by 2e-6 of itself), and quotients within
+// 2^-22.  The instructions of these kernels are what bounds them.
+__device__ __forceinline__ float exp_fast(float x) { return __expf(x); }
+__device__ __forceinline__ float over(float v) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// A lane's logits in the order of the choice, the first in front, their numbers (0 .. PER - 1) in the bytes of `which`
+template <int PER> __device__ __forceinline__ void sort_keys(uint32_t* key, uint64_t& which) {
+  uint32_t at[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) at[i] = i;
+  // (a key moves in front of another only where it is larger: equal ones keep their order)
+#pragma unroll
+  for (int i = 1; i < PER; ++i)
+#pragma unroll
+    for (int j = i; j > 0; --j) {
+      const bool swap = key[j] > key[j - 1];
+      const uint32_t a = key[j], b = at[j];
+      key[j] = swap ? key[j - 1] : a; at[j] = swap ? at[j - 1] : b;
+      key[j - 1] = swap ? a : key[j - 1]; at[j - 1] = swap ? b : at[j - 1];
+    }
+  which = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) which |= (uint64_t)at[i] << (8 * i);
+}
+
+// Over the G lanes that share a token
+template <int G> __device__ __forceinline__ float team_sum(float v) {
+#pragma unroll
+  for (int d = G / 2; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+template <int G> __device__ __forceinline__ uint32_t team_max(uint32_t v) {
+  if constexpr (G == 32) {
+    v = __reduce_max_sync(0xffffffffu, v);
+  } else {
+#pragma unroll
+    for (int d = G / 2; d; d >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
+  }
+  return v;
+}
+
+// A team of G lanes per token (8, 16 or the warp, 32 / G tokens at a time), PER consecutive logits a lane, sorted; k rounds of a team-wide maximum, which goes
+// to the first lane that has it in front, the j-th choice to lane j.  Then the block's slots are ranked within their experts, in order: every warp counts a run of
+// them, and ranks it behind the runs before.  Instructions bound it: both kernels, us, 65536 tokens, 2 of 8 experts 17 (a warp per token 36), 6 of 64 34 (64);
+// 32768, 8 of 128 33 (with two tokens a warp and 8 logits a lane 32: sorting them costs what the rounds save).
 // A block per SM with all its warps: few blocks, because each adds up the counts of all others in the next kernel.
-template <typename T, int PER>
+template <typename T, int PER, int G>
 __global__ void __launch_bounds__(ROUTE_THREADS)
 route_choose_kernel(const T* logits, const RouteParams p) {
+  constexpr int S = 32 / G;
   extern __shared__ int shared[];
   int* hist = shared;                                                        // [ROUTE_WARPS][experts]
   float* sums = reinterpret_cast<float*>(shared + ROUTE_WARPS * p.experts);  // [ROUTE_WARPS][experts]
   __shared__ int some_tokens;
   bb::pdl_sync();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = p.experts, first = lane * PER;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = p.experts, seat = lane & (G - 1), first = seat * PER;
+  const unsigned team = G == 32 ? 0xffffffffu : ((1u << (G & 31)) - 1) << (lane & ~(G - 1));
   const int t0 = blockIdx.x * p.chunk, t1 = min(p.tokens, t0 + p.chunk);
   for (int i = threadIdx.x; i < ROUTE_WARPS * n; i += ROUTE_THREADS) hist[i] = 0;
   if (threadIdx.x == 0) some_tokens = 0;
   float prob[PER] = {};
   int some = 0;
   float x[PER];
-  int t = t0 + warp;
-  if (t < t1) load_run<T, PER>(logits + (long long)t * p.ld, first, n, p.vec, x);
-  for (; t < t1; t += ROUTE_WARPS) {
+  auto load = [&](int t) {
+    if (t < t1) {
+      load_run<T, PER>(logits + (long long)t * p.ld, first, n, p.vec, x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] = -INFINITY;
+    }
+  };
+  int t = t0 + warp * S + lane / G;
+  load(t);
+  for (; t - lane / G < t1; t += ROUTE_WARPS * S) {
     uint32_t key[PER];
     float own[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) { key[i] = choice_key(x[i]); own[i] = x[i]; }
-    if (t + ROUTE_WARPS < t1) load_run<T, PER>(logits + (long long)(t + ROUTE_WARPS) * p.ld, first, n, p.vec, x);       // the next token's
+    load(t + ROUTE_WARPS * S);           // the next token's
     int mine = -1;
     uint32_t value = 0;
+    uint64_t which;
+    sort_keys<PER>(key, which);
     for (int j = 0; j < p.k; ++j) {
-      uint32_t best = key[0];
-#pragma unroll
-      for (int i = 1; i < PER; ++i) best = max(best, key[i]);
-      const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-      if (top == 0) break;
-      const int from = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
-      int at = 0;
-#pragma unroll
-      for (int i = PER - 1; i >= 0; --i) if (key[i] == top) at = i;
+      const uint32_t top = team_max<G>(key[0]);
+      const int from = __ffs(__ballot_sync(0xffffffffu, key[0] == top) & team) - 1;
+      const int at = __shfl_sync(0xffffffffu, first + (int)(which & 0xff), from);
+      if (seat == j && top != 0) { mine = at; value = top; }
       if (lane == from) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) if (i == at) key[i] = 0;
+        for (int i = 0; i + 1 < PER; ++i) key[i] = key[i + 1];
+        key[PER - 1] = 0;
+        which >>= 8;
       }
-      at = __shfl_sync(0xffffffffu, at, from);
-      if (lane == j) { mine = from * PER + at; value = top; }
     }
-    const bool any = __shfl_sync(0xffffffffu, mine, 0) >= 0;
-    const float top = any ? key_value(__shfl_sync(0xffffffffu, value, 0)) : 0.f;
+    const uint32_t best = __shfl_sync(0xffffffffu, value, lane & ~(G - 1));          // 0: nothing to choose
+    const bool any = best != 0;
+    const float top = any ? key_value(best) : 0.f;
     float e[PER], sum = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      e[i] = any && first + i < n ? expf(own[i] - top) : 0.f;
+      e[i] = any && first + i < n ? exp_fast(own[i] - top) : 0.f;
       sum += e[i];
     }
-    sum = warp_sum(sum);
-    const float share = mine >= 0 ? expf(key_value(value) - top) : 0.f;
-    const float over = p.normalize ? warp_sum(share) : sum;
-    const long long s = (long long)t * p.k + lane;
-    if (lane < p.k) {
+    sum = team_sum<G>(sum);
+    const float share = mine >= 0 ? exp_fast(key_value(value) - top) : 0.f, each = over(sum);
+    const float scale = p.normalize ? over(team_sum<G>(share)) : each;
+    if (t >= t1) continue;               // (a whole team; nothing below is done together)
+    const long long s = (long long)t * p.k + seat;
+    if (seat < p.k) {
       p.chosen[s] = mine;
-      p.weights[s] = mine >= 0 ? share / over : 0.f;
+      p.weights[s] = mine >= 0 ? share * scale : 0.f;
     }
-    if (lane == 0) p.stats[t] = make_float2(top, sum);
+    if (seat == 0) p.stats[t] = make_float2(top, sum);
     if (any) {
       ++some;
-      const float each = 1.f / sum;
 #pragma unroll
       for (int i = 0; i < PER; ++i) prob[i] = fmaf(e[i], each, prob[i]);
     }
   }
+  __syncwarp();
 #pragma unroll
-  for (int i = 0; i < PER; ++i) if (first + i < n) sums[warp * n + first + i] = prob[i];
+  for (int d = G; d < 32; d <<= 1) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) prob[i] += __shfl_xor_sync(0xffffffffu, prob[i], d);
+    some += __shfl_xor_sync(0xffffffffu, some, d);
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) if (lane < G && first + i < n) sums[warp * n + first + i] = prob[i];
   __syncthreads();
   if (lane == 0 && some) atomicAdd(&some_tokens, some);
   const int k = p.k, slot0 = t0 * k, count = (t1 - t0) * k;
@@ -183,13 +245,13 @@ route_choose_kernel(const T* logits, const RouteParams p) {
   }
 }
 
-// Every block adds up what stands before its slots (the counts of all blocks, once more each) and places them; the first also makes what
-// there is one of.
+// Every block adds up what stands before its slots (the counts of all blocks, once more each) and places them; one more block makes what there is one of.
 __global__ void __launch_bounds__(ROUTE_THREADS)
 route_place_kernel(const RouteParams p) {
   __shared__ int total[MAX_EXPERTS + 1], before[MAX_EXPERTS + 1], base[MAX_EXPERTS + 1];
   __shared__ float mass[ROUTE_THREADS];
   __shared__ double part[MAX_EXPERTS];
+  const bool extra = (int)blockIdx.x == p.blocks;
   bb::pdl_sync();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = p.experts, width = n + 1;
   for (int e = threadIdx.x; e < width; e += ROUTE_THREADS) { total[e] = 0; before[e] = 0; }
@@ -223,18 +285,20 @@ route_place_kernel(const RouteParams p) {
     if (lane == 0) base[n] = carry;
   }
   __syncthreads();
-  const int k = p.k, t0 = blockIdx.x * p.chunk, t1 = min(p.tokens, t0 + p.chunk), routed = base[n];
-  const int all = p.tokens * k;
-  for (int i = t0 * k + threadIdx.x; i < t1 * k; i += ROUTE_THREADS) {
-    const int e = p.chosen[i];
-    if (e >= 0) {
-      const int at = base[e] + before[e] + p.rows[i];
-      p.rows[i] = at;
-      p.slots[at] = i;
+  const int routed = base[n];
+  if (!extra) {
+    const int k = p.k, t0 = blockIdx.x * p.chunk, t1 = min(p.tokens, t0 + p.chunk), all = p.tokens * k;
+    for (int i = t0 * k + threadIdx.x; i < t1 * k; i += ROUTE_THREADS) {
+      const int e = p.chosen[i];
+      if (e >= 0) {
+        const int at = base[e] + before[e] + p.rows[i];
+        p.rows[i] = at;
+        p.slots[at] = i;
+      }
     }
+    for (long long r = (long long)routed + blockIdx.x * ROUTE_THREADS + threadIdx.x; r < all; r += (long long)p.blocks * ROUTE_THREADS) p.slots[r] = -1;
+    return;
   }
-  for (long long r = (long long)routed + blockIdx.x * ROUTE_THREADS + threadIdx.x; r < all; r += (long long)gridDim.x * ROUTE_THREADS) p.slots[r] = -1;
-  if (blockIdx.x != gridDim.x - 1) return;
   // sums of softmax: blocks b = g, g + groups, ... by one thread, then the threads of an expert in their order
   const int teams = ROUTE_THREADS / n, team = threadIdx.x / n, e = threadIdx.x - team * n;
   float m = 0.f;
@@ -244,14 +308,13 @@ route_place_kernel(const RouteParams p) {
   }
   mass[threadIdx.x] = m;
   __syncthreads();
-  const double tokens = total[n] > 0 ? total[n] : 1, places = routed > 0 ? routed : 1;
+  const int tokens = max(total[n], 1), places = max(routed, 1);
   if (threadIdx.x < n) {
     double sum = 0.0;
     for (int i = 0; i < teams; ++i) sum += (double)mass[i * n + threadIdx.x];
-    const double f = total[threadIdx.x] / places;
     p.offsets[threadIdx.x] = base[threadIdx.x];
-    p.load[threadIdx.x] = (float)f;
-    part[threadIdx.x] = f * sum / tokens;
+    p.load[threadIdx.x] = (float)total[threadIdx.x] / (float)places;
+    part[threadIdx.x] = (double)total[threadIdx.x] * sum;
   }
   if (threadIdx.x == 0) { p.offsets[n] = routed; p.load[n] = (float)tokens; }
   __syncthreads();
@@ -260,60 +323,87 @@ route_place_kernel(const RouteParams p) {
     for (int i = lane; i < n; i += 32) sum += part[i];
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) p.balance[0] = (float)(n * sum);
+    if (lane == 0) p.balance[0] = (float)(n * sum / ((double)places * (double)tokens));
   }
 }
 
-// dx_e = p_e (c_e - sum p c) + what arrives through the weights; a warp per token, its chosen experts in lanes 0 .. k - 1.  What arrives goes to the
-// lanes that own the experts through shared memory.
-template <typename T, int PER>
+// A lane's run in shared memory (on its size, 16 bytes at most)
+template <int PER> __device__ __forceinline__ void put_run(float* to, const float* v) {
+  if constexpr (PER >= 4) {
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) *reinterpret_cast<float4*>(to + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+  } else if constexpr (PER == 2) {
+    *reinterpret_cast<float2*>(to) = make_float2(v[0], v[1]);
+  } else {
+    to[0] = v[0];
+  }
+}
+template <int PER> __device__ __forceinline__ void get_run(const float* from, float* v) {
+  if constexpr (PER >= 4) {
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) { const float4 q = *reinterpret_cast<const float4*>(from + i); v[i] = q.x; v[i + 1] = q.y; v[i + 2] = q.z; v[i + 3] = q.w; }
+  } else if constexpr (PER == 2) {
+    const float2 q = *reinterpret_cast<const float2*>(from);
+    v[0] = q.x; v[1] = q.y;
+  } else {
+    v[0] = from[0];
+  }
+}
+
+// dx_e = p_e (c_e - sum p c) + what arrives through the weights; a team of lanes per token as above.  What arrives goes to the lanes that own the experts
+// through shared memory.
+template <typename T, int PER, int G>
 __global__ void __launch_bounds__(32 * BWD_WARPS)
 route_bwd_kernel(const T* logits, const RouteParams p, const float* d_weights, const float* d_balance, T* out, long long ldd, int cols, int vec_out) {
   __shared__ alignas(16) float arrived[BWD_WARPS][32 * PER];
   bb::pdl_sync();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = p.experts, first = lane * PER;
-  const int t = blockIdx.x * BWD_WARPS + warp;
-  if (t >= p.tokens) return;
-  const T* row = logits + (long long)t * p.ld;
-  const long long s = (long long)t * p.k + lane;
-  int mine = lane < p.k ? p.chosen[s] : -1;
-  if (mine >= n) mine = -1;
-  const float2 st = p.stats[t];
-  float x[PER], d[PER];
-  load_run<T, PER>(row, first, n, p.vec, x);
-  float dw = 0.f, w = 0.f;
-  if (mine >= 0) {
-    w = value_of(row[mine]);
-    dw = d_weights ? d_weights[s] : 0.f;
-  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = p.experts, seat = lane & (G - 1), first = seat * PER;
+  const int t = blockIdx.x * (BWD_WARPS * (32 / G)) + threadIdx.x / G;
+  const bool there = t < p.tokens;
+  float* mail = arrived[warp] + lane / G * (G * PER);
   const float g = d_balance ? d_balance[0] * (float)n / p.load[n] : 0.f;
-  T* to = out + (long long)t * ldd;
-  if (__shfl_sync(0xffffffffu, mine, 0) >= 0) {
-    float* mail = arrived[warp];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) mail[first + i] = 0.f;
-    const float over = 1.f / st.y;
-    float prob[PER], push[PER], mean = 0.f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      prob[i] = first + i < n ? expf(x[i] - st.x) * over : 0.f;
-      push[i] = d_balance && first + i < n ? g * p.load[first + i] : 0.f;
-      mean = fmaf(prob[i], push[i], mean);
-    }
-    if (mine >= 0) w = expf(w - st.x);
-    w = p.normalize ? w / warp_sum(w) : w * over;
-    const float through = warp_sum(w * dw);
-    mean = warp_sum(mean);
-    __syncwarp();
-    if (mine >= 0) mail[mine] = p.normalize ? w * (dw - through) : w * dw;
-    __syncwarp();
-    const float off = p.normalize ? mean : mean + through;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) d[i] = fmaf(prob[i], push[i] - off, mail[first + i]);
+  const long long s = (long long)t * p.k + seat;
+  int mine = there && seat < p.k ? p.chosen[s] : -1;
+  if (mine >= n) mine = -1;
+  const float2 st = there ? p.stats[t] : make_float2(0.f, 1.f);
+  float x[PER], push[PER], d[PER];
+  if (there) {
+    load_run<T, PER>(logits + (long long)t * p.ld, first, n, p.vec, x);
   } else {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) d[i] = 0.f;
+    for (int i = 0; i < PER; ++i) x[i] = 0.f;
   }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) push[i] = d_balance && first + i < n ? g * p.load[first + i] : 0.f;
+  const float dw = mine >= 0 && d_weights ? d_weights[s] : 0.f;
+  const bool any = __shfl_sync(0xffffffffu, mine, lane & ~(G - 1)) >= 0;
+  const float scale = over(st.y);
+  float prob[PER], mean = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    x[i] = first + i < n ? exp_fast(x[i] - st.x) : 0.f;
+    prob[i] = x[i] * scale;
+    mean = fmaf(prob[i], push[i], mean);
+    d[i] = 0.f;
+  }
+  put_run<PER>(mail + first, x);
+  __syncwarp();
+  float w = mine >= 0 ? mail[mine] : 0.f;          // the chosen ones' exponentials come back the way their gradients go
+  w *= p.normalize ? over(team_sum<G>(w)) : scale;
+  if (mine < 0) w = 0.f;
+  const float through = team_sum<G>(w * dw);
+  if (d_balance) mean = team_sum<G>(mean);
+  __syncwarp();
+  put_run<PER>(mail + first, d);
+  __syncwarp();
+  if (mine >= 0) mail[mine] = p.normalize ? w * (dw - through) : w * dw;
+  __syncwarp();
+  if (!there) return;
+  const float off = p.normalize ? mean : mean + through;
+  get_run<PER>(mail + first, d);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) d[i] = any ? fmaf(prob[i], push[i] - off, d[i]) : 0.f;
+  T* to = out + (long long)t * ldd;
   if (vec_out) {
     if (first < n) {
       alignas(16) T v[PER];
@@ -335,7 +425,7 @@ route_bwd_kernel(const T* logits, const RouteParams p, const float* d_weights, c
 #pragma unroll
     for (int i = 0; i < PER; ++i) if (first + i < n) put_value(to + first + i, d[i]);
   }
-  for (int c = n + lane; c < cols; c += 32) put_value(to + c, 0.f);
+  for (int c = n + seat; c < cols; c += G) put_value(to + c, 0.f);
 }
 
 // ------------------------------------------------------------------ rows there and back
@@ -543,16 +633,22 @@ combine_bwd_kernel(const T* dy, long long ld_dy, const T* x, long long ld, const
 
 // ------------------------------------------------------------------ host side
 bool bad_route(const bb_route_desc* d) {
-  return !d || d->tokens <= 0 || d->experts <= 0 || d->experts > MAX_EXPERTS || d->k <= 0 || d->k > d->experts || d->k > MAX_CHOSEN || d->ld < d->experts ||
+  return !d || d->tokens <= 0 || d->experts <= 0 || d->experts > MAX_EXPERTS || d->k <= 0 || d->k > d->experts || d->k > MAX_CHOSEN || d->cols < d->experts || d->ld < d->cols ||
          (d->dtype != BB_DTYPE_BF16 && d->dtype != BB_DTYPE_F32) || (long long)d->tokens * d->k > INT_MAX - 1024;
 }
 
-int per_lane(int experts) { return experts <= 32 ? 1 : experts <= 64 ? 2 : experts <= 128 ? 4 : 8; }
+// Lanes of a token's team, as many as its choices at least, and logits a lane
+struct Team { int lanes, per; };
+Team team_of(int experts, int k) {
+  if (experts <= 32 && k <= 8) return {8, experts <= 8 ? 1 : experts <= 16 ? 2 : 4};
+  if (experts <= 64 && k <= 16) return {16, 4};
+  return {32, experts <= 32 ? 1 : experts <= 64 ? 2 : experts <= 128 ? 4 : 8};
+}
 bool odd(const void* p, uintptr_t mask) { return ((uintptr_t)p & mask) != 0; }
-// Rows in runs of a lane's values: runs end with the row, and begin on their size (16 bytes at most)
-template <typename T> bool in_runs(const T* p, long long ld, int experts) {
-  const int per = per_lane(experts), bytes = per * (int)sizeof(T) < 16 ? per * (int)sizeof(T) : 16;
-  return experts % per == 0 && ld * (long long)sizeof(T) % bytes == 0 && !odd(p, bytes - 1);
+// Rows in runs of a lane's values, that end inside the row's `cols` and begin on their size (16 bytes at most)
+template <typename T> bool in_runs(const T* p, long long ld, int experts, int cols, int per) {
+  const int bytes = per * (int)sizeof(T) < 16 ? per * (int)sizeof(T) : 16;
+  return (experts + per - 1) / per * per <= cols && ld * (long long)sizeof(T) % bytes == 0 && !odd(p, bytes - 1);
 }
 
 RouteParams route_params(const bb_route_desc* d) {
@@ -565,29 +661,31 @@ RouteParams route_params(const bb_route_desc* d) {
   return p;
 }
 
-template <typename T, int PER> int choose_launch(const T* logits, const RouteParams& p, cudaStream_t s) {
-  BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(route_choose_kernel<T, PER>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * ROUTE_WARPS * 32 * PER * 4)));
-  BB_CUDA_CHECK(bb_launch(route_choose_kernel<T, PER>, p.blocks, ROUTE_THREADS, 2 * ROUTE_WARPS * p.experts * 4, s, logits, p));
+template <typename T> struct RouteCall {
+  const T* logits; RouteParams p; cudaStream_t s;
+  const float *dw, *db; T* out; long long ldd; int cols, vec_out;
+};
+template <typename T, int PER, int G> int route_fwd_as(const RouteCall<T>& c) {
+  BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(route_choose_kernel<T, PER, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * ROUTE_WARPS * G * PER * 4)));
+  BB_CUDA_CHECK(bb_launch(route_choose_kernel<T, PER, G>, c.p.blocks, ROUTE_THREADS, 2 * ROUTE_WARPS * c.p.experts * 4, c.s, c.logits, c.p));
+  BB_CUDA_CHECK(bb_launch(route_place_kernel, c.p.blocks + 1, ROUTE_THREADS, 0, c.s, c.p));
   return BB_OK;
 }
-
-template <typename T> int route_fwd(const T* logits, RouteParams p, cudaStream_t s) {
-  const int per = per_lane(p.experts);
-  p.vec = in_runs(logits, p.ld, p.experts);
-  if (int rc = per == 1 ? choose_launch<T, 1>(logits, p, s) : per == 2 ? choose_launch<T, 2>(logits, p, s) : per == 4 ? choose_launch<T, 4>(logits, p, s)
-                                                                                                            : choose_launch<T, 8>(logits, p, s))
-    return rc;
-  BB_CUDA_CHECK(bb_launch(route_place_kernel, p.blocks, ROUTE_THREADS, 0, s, p));
+template <typename T, int PER, int G> int route_bwd_as(const RouteCall<T>& c) {
+  constexpr int TOKENS = BWD_WARPS * (32 / G);
+  BB_CUDA_CHECK(bb_launch(route_bwd_kernel<T, PER, G>, (c.p.tokens + TOKENS - 1) / TOKENS, 32 * BWD_WARPS, 0, c.s, c.logits, c.p, c.dw, c.db, c.out, c.ldd, c.cols,
+                          c.vec_out));
   return BB_OK;
 }
-
-template <typename T>
-int route_bwd(const T* logits, RouteParams p, const float* dw, const float* db, T* out, long long ldd, int cols, cudaStream_t s) {
-  const int per = per_lane(p.experts);
-  p.vec = in_runs(logits, p.ld, p.experts);
-  auto kernel = per == 1 ? route_bwd_kernel<T, 1> : per == 2 ? route_bwd_kernel<T, 2> : per == 4 ? route_bwd_kernel<T, 4> : route_bwd_kernel<T, 8>;
-  BB_CUDA_CHECK(bb_launch(kernel, (p.tokens + BWD_WARPS - 1) / BWD_WARPS, 32 * BWD_WARPS, 0, s, logits, p, dw, db, out, ldd, cols, (int)in_runs(out, ldd, p.experts)));
-  return BB_OK;
+template <typename T> int route(RouteCall<T> c, int logits_cols, bool backward) {
+  const Team t = team_of(c.p.experts, c.p.k);
+  c.p.vec = in_runs(c.logits, c.p.ld, c.p.experts, logits_cols, t.per);
+  if (backward) c.vec_out = c.p.experts % t.per == 0 && in_runs(c.out, c.ldd, c.p.experts, c.cols, t.per);
+#define ROUTE_AS(per, lanes) (backward ? route_bwd_as<T, per, lanes>(c) : route_fwd_as<T, per, lanes>(c))
+  if (t.lanes == 8) return t.per == 1 ? ROUTE_AS(1, 8) : t.per == 2 ? ROUTE_AS(2, 8) : ROUTE_AS(4, 8);
+  if (t.lanes == 16) return ROUTE_AS(4, 16);
+  return t.per == 1 ? ROUTE_AS(1, 32) : t.per == 2 ? ROUTE_AS(2, 32) : t.per == 4 ? ROUTE_AS(4, 32) : ROUTE_AS(8, 32);
+#undef ROUTE_AS
 }
 
 // 16-byte accesses: every pointer and row on 16 bytes
@@ -639,13 +737,14 @@ extern "C" int bb_route_fwd(const bb_route_desc* d, const void* logits, float* w
                             float* balance, float* stats, float* load, void* workspace, long long workspace_bytes, void* stream) {
   if (bad_route(d) || !logits || odd(logits, d->dtype == BB_DTYPE_F32 ? 3 : 1) || !weights || !experts_out || !rows_out || !slots_out || !offsets || !balance || !stats ||
       odd(stats, 7) || !load || !workspace || odd(workspace, 3) || workspace_bytes < bb_route_workspace_bytes(d))
-    return refuse("bb_route_fwd: null or misaligned pointer, no tokens, 1 to 256 experts of which 1 to 32 are chosen, ld < experts, an unknown type, or a workspace that "
+    return refuse("bb_route_fwd: null or misaligned pointer, no tokens, 1 to 256 experts of which 1 to 32 are chosen, cols < experts, ld < cols, an unknown type, or a workspace that "
                   "is too small");
   RouteParams p = route_params(d);
   p.weights = weights; p.chosen = experts_out; p.rows = rows_out; p.slots = slots_out; p.offsets = offsets; p.balance = balance; p.stats = (float2*)stats; p.load = load;
   p.counts = (int*)workspace; p.probs = (float*)((int*)workspace + (long long)p.blocks * (p.experts + 1));
   BackToBack overlap;
-  return d->dtype == BB_DTYPE_BF16 ? route_fwd((const __nv_bfloat16*)logits, p, (cudaStream_t)stream) : route_fwd((const float*)logits, p, (cudaStream_t)stream);
+  return d->dtype == BB_DTYPE_BF16 ? route(RouteCall<__nv_bfloat16>{(const __nv_bfloat16*)logits, p, (cudaStream_t)stream}, d->cols, false)
+                                   : route(RouteCall<float>{(const float*)logits, p, (cudaStream_t)stream}, d->cols, false);
 }
 
 extern "C" int bb_route_bwd(const bb_route_desc* d, const void* logits, const int* experts_out, const float* stats, const float* load,
@@ -655,8 +754,9 @@ extern "C" int bb_route_bwd(const bb_route_desc* d, const void* logits, const in
     return refuse("bb_route_bwd: null or misaligned pointer, a descriptor that bb_route_fwd refuses, cols < experts or ldd < cols");
   RouteParams p = route_params(d);
   p.chosen = const_cast<int*>(experts_out); p.stats = (float2*)stats; p.load = const_cast<float*>(load);
-  return d->dtype == BB_DTYPE_BF16 ? route_bwd((const __nv_bfloat16*)logits, p, d_weights, d_balance, (__nv_bfloat16*)dlogits, ldd, cols, (cudaStream_t)stream)
-                                   : route_bwd((const float*)logits, p, d_weights, d_balance, (float*)dlogits, ldd, cols, (cudaStream_t)stream);
+  return d->dtype == BB_DTYPE_BF16
+             ? route(RouteCall<__nv_bfloat16>{(const __nv_bfloat16*)logits, p, (cudaStream_t)stream, d_weights, d_balance, (__nv_bfloat16*)dlogits, ldd, cols}, d->cols, true)
+             : route(RouteCall<float>{(const float*)logits, p, (cudaStream_t)stream, d_weights, d_balance, (float*)dlogits, ldd, cols}, d->cols, true);
 }
 
 extern "C" int bb_dispatch_rows(const void* x, long long ld, int dtype, const int* slots, int k, void* out, long long rows, long long tokens, int h,

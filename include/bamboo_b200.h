@@ -476,6 +476,7 @@ int bb_expert_mlp_bwd(const bb_expert_mlp_desc* m, const void* x, long long ld_x
  * tokens.  At most 256 experts, of which at most 32 are chosen. */
 typedef struct bb_route_desc {
   int tokens, experts, k, normalize, dtype;
+  int cols;                                     /* of a row of logits, >= experts: those behind may be read, and count for nothing */
   long long ld;
 } bb_route_desc;
 long long bb_route_workspace_bytes(const bb_route_desc* d);

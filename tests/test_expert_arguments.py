@@ -133,8 +133,8 @@ def test_native_calls_refuse_what_python_would_not_send():
     for args in ((None, 64, at, 4, at, None, 8, 64), (at, 64, at, 4, None, None, 8, 64), (at, 64, at, 4, at, at, 8, 64), (at, 64, at, 0, at, None, 8, 64),
                  (at, 64, at, 257, at, None, 8, 64), (at, 64, at, 4, at, None, 0, 64), (at, 64, at, 4, at, None, 8, 60), (at, 32, at, 4, at, None, 8, 64)):
         assert handle.bb_grouped_colsum(*args, None) == -1 and b"bb_grouped_colsum" in handle.bb_last_error(), args
-    route = dict(tokens=16, experts=8, k=2, normalize=1, dtype=0, ld=8)
-    for change in (dict(tokens=0), dict(experts=0), dict(experts=257), dict(k=0), dict(k=9), dict(experts=64, ld=64, k=33), dict(ld=7), dict(dtype=2), dict(tokens=1 << 30, k=4)):
+    route = dict(tokens=16, experts=8, k=2, normalize=1, dtype=0, cols=8, ld=8)
+    for change in (dict(tokens=0), dict(experts=0), dict(experts=257), dict(k=0), dict(k=9), dict(experts=64, cols=64, ld=64, k=33), dict(ld=7), dict(cols=7), dict(dtype=2), dict(tokens=1 << 30, k=4)):
         d = lib.RouteDesc(**{**route, **change})
         assert handle.bb_route_workspace_bytes(ctypes.byref(d)) == 0
         assert handle.bb_route_fwd(ctypes.byref(d), *[at] * 10, 1 << 40, None) == -1, change
