@@ -3,6 +3,7 @@
     python -m bamboo_b200.kernel_bench attention     # tcgen05 attention forward / backward
     python -m bamboo_b200.kernel_bench rowwise       # LayerNorm backward, bias-gradient column sums
     python -m bamboo_b200.kernel_bench gemm          # the GEMM shapes of a GPT-2-medium step, beside torch.matmul
+    python -m bamboo_b200.kernel_bench experts       # routing, moved rows and grouped products of a mixture of experts, the optimizer step over a list
 
 Every measurement rotates over operand sets larger than the 126 MB L2.  The row-wise kernels are
 short enough for the host to be the bottleneck of a launch loop, so their calls are captured into
@@ -137,6 +138,50 @@ def gemm():
     print("device status", L.read_status())
 
 
+def experts():
+    from . import experts as E
+    from . import optim
+    for tokens, n, k in [(8192, 8, 2), (32768, 128, 8), (512, 8, 2)]:
+        x = [torch.randn(tokens, n, device="cuda") for _ in range(4)]
+        t = _graph_us(lambda i: E.route(x[i], k), 4)
+        print(f"route {tokens} tokens, {k} of {n}: {t:.1f} us", flush=True)
+    for tokens, h, n, k in [(8192, 1024, 8, 2), (8192, 1024, 64, 4)]:
+        r = E.route(torch.randn(tokens, n, device="cuda"), k)
+        x = [torch.randn(tokens, h, device="cuda").bfloat16() for _ in range(6)]
+        rows = [E.dispatch(t, r) for t in x]
+        out = _graph_us(lambda i: E.dispatch(x[i], r), 6)
+        back = _graph_us(lambda i: E.combine(rows[i], r, residual=x[i]), 6)
+        print(f"dispatch {tokens} x {h}, {k} of {n}: {out:.1f} us ({2 * (k + 1) * tokens * h / out / 1e6:.2f} TB/s), combine {back:.1f} us "
+              f"({2 * (k + 2) * tokens * h / back / 1e6:.2f} TB/s)", flush=True)
+        del x, rows
+    for rows, n, out, inner in [(16384, 8, 4096, 1024), (16384, 8, 1024, 4096), (8192, 8, 16384, 4096), (14, 8, 4096, 1024)]:
+        sets = max(2, min(6, int(5e8 / (2 * (rows * (out + inner) + n * out * inner)))))
+        offsets = torch.tensor([rows * e // n for e in range(n + 1)], dtype=torch.int32, device="cuda")
+        x = [torch.randn(rows, inner, device="cuda").bfloat16() for _ in range(sets)]
+        dy = [torch.randn(rows, out, device="cuda").bfloat16() for _ in range(sets)]
+        w = [torch.randn(n, out, inner, device="cuda").bfloat16() for _ in range(sets)]
+        bias = torch.zeros(n, out, device="cuda").bfloat16()
+        y, dx, dw, db = torch.empty_like(dy[0]), torch.empty_like(x[0]), torch.empty_like(w[0]), torch.empty_like(bias)
+        parts = torch.empty(L.grouped_bias_scratch(n, out, inner), dtype=torch.uint8, device="cuda")
+        times = [_graph_us(f, sets) for f in (
+            lambda i: L.grouped_gemm(L.GROUPED_ROWS, x[i], w[i], offsets, y, epilogue=L.EPI_BIAS, bias=bias),
+            lambda i: L.grouped_gemm(L.GROUPED_INPUT, dy[i], w[i], offsets, dx),
+            lambda i: L.grouped_gemm(L.GROUPED_WEIGHT, dy[i], x[i], offsets, dw, bias_grad=db, bias_parts=parts))]
+        print(f"grouped products {rows} rows, {n} experts {out} x {inner}: " + ", ".join(
+            f"{name} {t:.1f} us {2 * rows * out * inner / t / 1e6:.0f} TFLOP/s" for name, t in zip(("rows", "input gradient", "weight and bias gradient"), times)),
+            flush=True)
+        del x, dy, w, y, dx, dw
+    for bits in (8, 32):
+        size, count = 4_000_000, 24
+        params = [torch.randn(size, device="cuda").bfloat16() for _ in range(count)]
+        opt = optim.AdamW(params, state_bits=bits)
+        grads = [torch.randn(size, device="cuda").bfloat16() for _ in range(count)]
+        t = _graph_us(lambda i: optim.adamw_step_(opt.params, grads, opt.exp_avgs, opt.exp_avg_sqs, scales=opt.scales, masters=opt.masters, step=1), 1)
+        print(f"AdamW over {count} tensors of {size}, moments in {bits} bits: {t:.1f} us ({(12 + bits // 2) * size * count / t / 1e6:.2f} TB/s)", flush=True)
+        del opt, params, grads
+    print("device status", L.read_status())
+
+
 if __name__ == "__main__":
     L.load()
     which = sys.argv[1] if len(sys.argv) > 1 else "all"
@@ -146,3 +191,5 @@ if __name__ == "__main__":
         rowwise()
     if which in ("gemm", "all"):
         gemm()
+    if which in ("experts", "all"):
+        experts()
