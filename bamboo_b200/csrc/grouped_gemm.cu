@@ -130,9 +130,10 @@ __device__ __forceinline__ void read_offsets(const GroupParams& p, int* start, i
 enum { ROWS = 0, ROWS_T = 1, WGRAD = 2 };     // B as stored, B turned, weight gradient
 
 // db_e along with dW_e: one warp adds up rows of dy that stand in shared memory anyway, behind the MMAs that read them (`read_bar`) and in front of the
-// copies that replace them (`summed_bar`).  It takes 1000 cycles for a k-block whose MMAs take 512, so the column tiles that share the rows take
+// copies that replace them (`summed_bar`).  (Beside the MMAs, told by the warp that issues them when a stage has landed: pairs took 85 us for 52 even
+// without a bias.)  It takes longer for a k-block than its MMAs (512 cycles), so the column tiles that share the rows take
 // their k-blocks in turn - tile i the k-blocks i, i + tiles, ... - and a second kernel adds the tiles' sums in their order (16384 rows of 8 experts,
-// 4096 x 1024, us: 122, of which 108 are the weight gradient's; by the tiles of the first columns alone 169, with a pass of its own 108 + 33).  A lane keeps eight columns of each box and every fourth row.
+// 4096 x 1024, us: 116, of which 108 are the weight gradient's; by the tiles of the first columns alone 169, with a pass of its own 108 + 33).  A lane keeps eight columns of each box and every fourth row.
 struct ColumnSums {
   float2 v[BM / 64][4];
   __device__ __forceinline__ void clear() {
@@ -141,17 +142,26 @@ struct ColumnSums {
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[b][i] = make_float2(0.f, 0.f);
   }
+  __device__ __forceinline__ void add(int b, const uint4& q) {
+    v[b][0] = bb::add2(v[b][0], make_float2(bb::bf16_lo(q.x), bb::bf16_hi(q.x)));
+    v[b][1] = bb::add2(v[b][1], make_float2(bb::bf16_lo(q.y), bb::bf16_hi(q.y)));
+    v[b][2] = bb::add2(v[b][2], make_float2(bb::bf16_lo(q.z), bb::bf16_hi(q.z)));
+    v[b][3] = bb::add2(v[b][3], make_float2(bb::bf16_lo(q.w), bb::bf16_hi(q.w)));
+  }
   __device__ __forceinline__ void add(const uint8_t* tile, int rows, int lane) {
 #pragma unroll
-    for (int b = 0; b < BM / 64; ++b)
-#pragma unroll 4
-      for (int r = lane >> 3; r < rows; r += 4) {
-        const uint4 q = *reinterpret_cast<const uint4*>(tile + b * 8192 + slab_off(r, lane & 7));
-        v[b][0] = bb::add2(v[b][0], make_float2(bb::bf16_lo(q.x), bb::bf16_hi(q.x)));
-        v[b][1] = bb::add2(v[b][1], make_float2(bb::bf16_lo(q.y), bb::bf16_hi(q.y)));
-        v[b][2] = bb::add2(v[b][2], make_float2(bb::bf16_lo(q.z), bb::bf16_hi(q.z)));
-        v[b][3] = bb::add2(v[b][3], make_float2(bb::bf16_lo(q.w), bb::bf16_hi(q.w)));
+    for (int b = 0; b < BM / 64; ++b) {
+      const uint8_t* box = tile + b * 8192;
+      if (rows == BK) {
+        uint4 q[BK / 4];
+#pragma unroll
+        for (int i = 0; i < BK / 4; ++i) q[i] = *reinterpret_cast<const uint4*>(box + slab_off((lane >> 3) + 4 * i, lane & 7));
+#pragma unroll
+        for (int i = 0; i < BK / 4; ++i) add(b, q[i]);
+      } else {
+        for (int r = lane >> 3; r < rows; r += 4) add(b, *reinterpret_cast<const uint4*>(box + slab_off(r, lane & 7)));
       }
+    }
   }
   __device__ __forceinline__ void write(const GroupParams& p, int e, int ni, int m0, int lane) {
 #pragma unroll
@@ -187,7 +197,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(panels + EPI_WARPS * SLAB_BYTES);      // [STAGES]
   uint64_t* empty_bar = full_bar + C::STAGES;       // [STAGES]
   uint64_t* clean_bar = empty_bar + C::STAGES;      // [STAGES] pairs: the other CTA's overhanging rows are zeros
-  uint64_t* read_bar = clean_bar + C::STAGES;       // [STAGES] weight gradient: the MMAs have read a stage that is to be summed
+  uint64_t* read_bar = clean_bar + C::STAGES;     // [STAGES] weight gradient: the MMAs have read a stage that is to be summed
   uint64_t* summed_bar = read_bar + C::STAGES;      // [STAGES] ... and its rows are added up
   uint64_t* tmem_full = summed_bar + C::STAGES;     // [2]
   uint64_t* tmem_empty = tmem_full + 2;             // [2]
