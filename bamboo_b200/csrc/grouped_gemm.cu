@@ -302,7 +302,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 #pragma unroll
               for (int j = 0; j < C::B_ROWS / 64; ++j) load2(b + j * 8192, &tmB, n0 + 64 * j, k0);
             } else {
-              load2(a, &tmA, k0, m0);
+              // (a CTA of a pair without rows of this expert multiplies zeros, which behind the last row come from nowhere)
+              load2(a, &tmA, k0, PAIR && m0 >= u.end ? p.rows : m0);
               if constexpr (MODE == ROWS) {
                 load3(b, &tmB, k0, n0, u.e);
               } else {
