@@ -424,7 +424,7 @@ int bb_adam_step_clipped(float* master, float* grad, float* exp_avg, float* exp_
  *   BB_GROUPED_WEIGHT  out[e, n, k] = sum of its rows of x[r, n] (x) weight[r, k]      BB_EPI_STORE, BB_EPI_ACCUM_F32 (fp32, +=);  x is
  *                      the gradient, weight the layer's input [rows, k]
  * weight [experts, n, k] is contiguous.  Rows of `out` that belong to no expert become zeros (out2 stays as it is there); an expert without
- * rows has a gradient of zeros.  The reference has no mixture of experts: its layers (EX/pipeline_parallelism/gpt2.py:66-121) are the
+ * rows has a gradient of zeros; a weight gradient covers at most 2^27 rows.  The reference has no mixture of experts: its layers (EX/pipeline_parallelism/gpt2.py:66-121) are the
  * dense half blocks above, next to which these stand. */
 enum { BB_GROUPED_ROWS = 0, BB_GROUPED_INPUT = 1, BB_GROUPED_WEIGHT = 2 };
 typedef struct bb_grouped_desc {

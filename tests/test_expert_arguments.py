@@ -129,6 +129,8 @@ def test_native_calls_refuse_what_python_would_not_send():
                    dict(mode=2, ld_weight=64, bias_grad=at, bias_accum=at, bias_parts=at, bias_parts_bytes=1 << 30)):
         d = lib.GroupedDesc(**{**good, **change})
         assert handle.bb_grouped_gemm(ctypes.byref(d), None) == -1 and b"bb_grouped_gemm" in handle.bb_last_error(), change
+    d = lib.GroupedDesc(**{**good, "mode": 2, "ld_weight": 64, "rows": 2 ** 27 + 1})
+    assert handle.bb_grouped_gemm(ctypes.byref(d), None) == -4 and b"2^27" in handle.bb_last_error()
     assert handle.bb_grouped_gemm(None, None) == -1 and b"bb_grouped_gemm" in handle.bb_last_error()
     for args in ((None, 64, at, 4, at, None, 8, 64), (at, 64, at, 4, None, None, 8, 64), (at, 64, at, 4, at, at, 8, 64), (at, 64, at, 0, at, None, 8, 64),
                  (at, 64, at, 257, at, None, 8, 64), (at, 64, at, 4, at, None, 0, 64), (at, 64, at, 4, at, None, 8, 60), (at, 32, at, 4, at, None, 8, 64)):
