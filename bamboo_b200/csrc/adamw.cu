@@ -25,6 +25,7 @@ constexpr float CODE_MIN = 0x1p-9f;            // smallest e4m3 value above 0
 struct AdamTable {
   bb_adamw_tensor t[LIST];
   int first[LIST + 1];                         // first block of each tensor
+  unsigned char vec[LIST];                     // whether it lies on 16 bytes (codes: 8) everywhere
   int count;
 };
 // (lr is folded into the rest: p -= rate m / (root sqrt(v) + eps) + shrink p, rate = lr / (1 - beta1^step), root = 1 / sqrt(1 - beta2^step))
@@ -159,7 +160,7 @@ __device__ __forceinline__ void block_step(const bb_adamw_tensor& t, long long a
   for (int i = 0; i < 8; i += 2) {
     const float2 x = make_float2(g[i], g[i + 1]), y = bb::mul2(x, gs2), old = make_float2(v[i], v[i + 1]);
     const float2 m2 = bb::fma2(b1, make_float2(m[i], m[i + 1]), bb::mul2(x, gs1));
-    const float2 v2 = bb::fma2(b2, EIGHT ? bb::mul2(old, old) : old, bb::mul2(bb::mul2(y, y), make_float2(a.omb2, a.omb2)));
+    const float2 v2 = bb::fma2(b2, EIGHT ? bb::mul2(old, old) : old, bb::mul2(bb::mul2(y, make_float2(a.omb2, a.omb2)), y));
     const float2 r = make_float2(root_of(v2.x), root_of(v2.y));
     const float2 d = bb::fma2(r, make_float2(a.root, a.root), make_float2(a.eps, a.eps));
     const float2 u = bb::mul2(bb::mul2(m2, make_float2(-a.rate, -a.rate)), make_float2(over(d.x), over(d.y)));
@@ -203,8 +204,7 @@ adamw_list_kernel(const __grid_constant__ AdamTable table, const AdamArgs a) {
   const bb_adamw_tensor& t = table.t[lo];
   const long long block = unit - table.first[lo], at = block * BLOCK, left = t.numel - at;
   const float gs = a.coef ? a.coef[0] * a.grad_scale : a.grad_scale;
-  // `unused` of the table: every tensor of this entry lies on 16 bytes (codes: 8)
-  if (t.unused && left >= BLOCK) block_step<EIGHT, true>(t, at, block, BLOCK, lane, a, gs);
+  if (table.vec[lo] && left >= BLOCK) block_step<EIGHT, true>(t, at, block, BLOCK, lane, a, gs);
   else block_step<EIGHT, false>(t, at, block, left < BLOCK ? (int)left : BLOCK, lane, a, gs);
 }
 
@@ -248,7 +248,7 @@ extern "C" int bb_adamw_list(const bb_adamw_tensor* tensors, int count, double l
       const long long more = (tensors[from + n].numel + BLOCK - 1) / BLOCK;
       if (blocks + more > INT_MAX - 64) break;          // (a launch's blocks are counted in an int; one tensor's always are)
       t.t[n] = tensors[from + n];
-      t.t[n].unused = aligned(t.t[n], eight) ? 1 : 0;
+      t.vec[n] = aligned(t.t[n], eight) ? 1 : 0;
       t.first[n] = (int)blocks;
       blocks += more;
     }

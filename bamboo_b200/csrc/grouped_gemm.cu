@@ -801,7 +801,14 @@ bb_grouped_desc part_of(const bb_expert_mlp_desc* m, int mode, int n, int k, int
   d.mode = mode; d.rows = m->rows; d.n = n; d.k = k; d.experts = m->experts; d.epilogue = epilogue; d.offsets = m->offsets; d.max_ctas = m->max_ctas;
   return d;
 }
-bool bad_mlp(const bb_expert_mlp_desc* m) { return !m || m->rows <= 0 || m->in <= 0 || m->inner <= 0 || m->out <= 0 || !m->offsets; }
+// (all that the later products of a call could refuse, before the first is launched)
+bool bad_mlp(const bb_expert_mlp_desc* m) {
+  return !m || m->rows <= 0 || m->rows > INT_MAX - 1024 || m->in <= 0 || m->inner <= 0 || m->out <= 0 || ((m->in | m->inner | m->out) & 7) || m->experts <= 0 ||
+         m->experts > MAX_EXPERTS || !m->offsets || ((uintptr_t)m->offsets & 3) || !m->w1 || !m->w2 || (((uintptr_t)m->w1 | (uintptr_t)m->w2) & 15);
+}
+bool bad_scratch(const bb_expert_mlp_desc* m, bool wanted, int n, int k) {
+  return wanted && (!m->scratch || ((uintptr_t)m->scratch & 15) || m->scratch_bytes < bb_grouped_bias_bytes(n, k, m->experts));
+}
 // the weight's and the bias's gradient of one layer, each where it is asked for
 int weight_and_bias(const bb_expert_mlp_desc* m, const void* dy, long long ld_dy, int n, const void* x, long long ld_x, int k, void* dw, float* g_w, void* db, float* g_b,
                     void* stream) {
@@ -817,7 +824,9 @@ int weight_and_bias(const bb_expert_mlp_desc* m, const void* dy, long long ld_dy
 }  // namespace
 
 extern "C" int bb_expert_mlp_fwd(const bb_expert_mlp_desc* m, const void* x, long long ld_x, void* pre, void* act, void* y, void* stream) {
-  if (bad_mlp(m)) return refuse("bb_expert_mlp_fwd: null pointer or a size that is not positive");
+  if (bad_mlp(m) || bad_matrix(x, ld_x, m->in) || !m->b1 || !m->b2 || (((uintptr_t)m->b1 | (uintptr_t)m->b2) & 15) || !pre || !act || !y ||
+      (((uintptr_t)pre | (uintptr_t)act | (uintptr_t)y) & 15))
+    return refuse("bb_expert_mlp_fwd: null or misaligned pointer, a size that is not positive or no multiple of 8, rows that overlap, or more than 256 experts");
   BackToBack overlap(m->max_ctas == 0);
   bb_grouped_desc d = part_of(m, BB_GROUPED_ROWS, m->inner, m->in, BB_EPI_BIAS_GELU);
   d.x = x; d.ld_x = ld_x; d.weight = m->w1; d.bias = m->b1; d.out = act; d.ld_out = m->inner; d.out2 = pre;
@@ -829,7 +838,16 @@ extern "C" int bb_expert_mlp_fwd(const bb_expert_mlp_desc* m, const void* x, lon
 
 extern "C" int bb_expert_mlp_bwd(const bb_expert_mlp_desc* m, const void* x, long long ld_x, const void* pre, const void* act, const void* dy, long long ld_dy, void* dpre,
                                  void* dx, void* stream) {
-  if (bad_mlp(m)) return refuse("bb_expert_mlp_bwd: null pointer or a size that is not positive");
+  if (bad_mlp(m) || bad_matrix(x, ld_x, m->in) || bad_matrix(dy, ld_dy, m->out) || !pre || !act || (((uintptr_t)pre | (uintptr_t)act | (uintptr_t)dpre | (uintptr_t)dx) & 15) ||
+      (((uintptr_t)m->dw1 | (uintptr_t)m->dw2 | (uintptr_t)m->g_w1 | (uintptr_t)m->g_w2) & 15) ||
+      (((uintptr_t)m->db1 | (uintptr_t)m->db2) & 1) || (((uintptr_t)m->g_b1 | (uintptr_t)m->g_b2) & 3))
+    return refuse("bb_expert_mlp_bwd: null or misaligned pointer, a size that is not positive or no multiple of 8, rows that overlap, or more than 256 experts");
+  if (bad_scratch(m, (m->dw1 || m->g_w1) && (m->db1 || m->g_b1), m->inner, m->in) || bad_scratch(m, (m->dw2 || m->g_w2) && (m->db2 || m->g_b2), m->out, m->inner))
+    return refuse("bb_expert_mlp_bwd: a bias gradient that comes with a weight gradient takes bb_grouped_bias_bytes() of scratch");
+  if (m->rows > (1 << 27) && (m->dw1 || m->g_w1 || m->dw2 || m->g_w2)) {
+    bb_set_last_error_msg("bb_expert_mlp_bwd: a weight gradient over more than 2^27 rows");
+    return BB_ERR_TOO_LARGE;
+  }
   BackToBack overlap(m->max_ctas == 0);
   if (dpre) {
     bb_grouped_desc d = part_of(m, BB_GROUPED_INPUT, m->out, m->inner, BB_EPI_MUL_DGELU);

@@ -135,6 +135,16 @@ def test_native_calls_refuse_what_python_would_not_send():
     for args in ((None, 64, at, 4, at, None, 8, 64), (at, 64, at, 4, None, None, 8, 64), (at, 64, at, 4, at, at, 8, 64), (at, 64, at, 0, at, None, 8, 64),
                  (at, 64, at, 257, at, None, 8, 64), (at, 64, at, 4, at, None, 0, 64), (at, 64, at, 4, at, None, 8, 60), (at, 32, at, 4, at, None, 8, 64)):
         assert handle.bb_grouped_colsum(*args, None) == -1 and b"bb_grouped_colsum" in handle.bb_last_error(), args
+    mlp = dict(rows=8, inputs=64, inner=64, outputs=64, experts=4, offsets=at, w1=at, b1=at, w2=at, b2=at)
+    assert handle.bb_expert_mlp_fwd(None, at, 64, at, at, at, None) == -1 and handle.bb_expert_mlp_bwd(None, at, 64, at, at, at, 64, at, at, None) == -1
+    for change in (dict(rows=0), dict(inputs=60), dict(inner=0), dict(outputs=12), dict(experts=300), dict(offsets=None), dict(w1=None), dict(b1=None)):
+        d = lib.ExpertMLPDesc(**{**mlp, **change})
+        assert handle.bb_expert_mlp_fwd(ctypes.byref(d), at, 64, at, at, at, None) == -1, change
+    d = lib.ExpertMLPDesc(**mlp)
+    assert handle.bb_expert_mlp_fwd(ctypes.byref(d), None, 64, at, at, at, None) == -1
+    assert handle.bb_expert_mlp_bwd(ctypes.byref(d), at, 64, at, at, at, 64, None, at, None) == -1 and b"dpre" in handle.bb_last_error()
+    d = lib.ExpertMLPDesc(**mlp, dw2=at, db2=at)                                                    # a bias gradient without scratch
+    assert handle.bb_expert_mlp_bwd(ctypes.byref(d), at, 64, at, at, at, 64, None, None, None) == -1 and b"bb_grouped_bias_bytes" in handle.bb_last_error()
     route = dict(tokens=16, experts=8, k=2, normalize=1, dtype=0, cols=8, ld=8)
     for change in (dict(tokens=0), dict(experts=0), dict(experts=257), dict(k=0), dict(k=9), dict(experts=64, cols=64, ld=64, k=33), dict(ld=7), dict(cols=7), dict(dtype=2), dict(tokens=1 << 30, k=4)):
         d = lib.RouteDesc(**{**route, **change})
@@ -284,3 +294,17 @@ def test_constants_given_as_tensors(recorded):
         value.fill_(want)
         run(optim, lists(), lr=value, weight_decay=value, beta1=value, grad_scale=value)
         assert [seen[-1][2][n] for n in ("lr", "weight_decay", "beta1", "grad_scale")] == [want] * 4
+
+
+def test_native_list_step_refuses():
+    import struct
+    from bamboo_b200 import lib
+    handle, at = lib.load(), 1 << 20
+
+    def call(param=at, master=0, grad=at, m=at, v=at, scales=0, numel=300, dtype=1, count=1, step=1, beta1=0.9, max_norm=0.0, norm=None, ws=None, ws_bytes=0):
+        table = struct.pack("QQQQQQqiI", param, master, grad, m, v, scales, numel, dtype, 0)
+        return handle.bb_adamw_list(table, count, 1e-3, beta1, 0.999, 1e-8, step, 0.0, 1.0, 0, max_norm, None, norm, ws, ws_bytes, None)
+    for bad in (dict(param=0), dict(grad=0), dict(m=0), dict(v=0), dict(numel=0), dict(numel=-1), dict(numel=1 << 39), dict(dtype=2), dict(param=at + 2), dict(param=at + 1, master=at),
+                dict(master=at + 2), dict(grad=at + 2), dict(grad=at + 1, dtype=0), dict(m=at + 2), dict(scales=at + 2), dict(count=0), dict(count=-1), dict(step=0), dict(beta1=1.0),
+                dict(max_norm=-1.0), dict(max_norm=1.0), dict(max_norm=1.0, norm=at, ws=at, ws_bytes=16), dict(max_norm=1.0, norm=at, ws=at + 4, ws_bytes=1 << 20)):
+        assert call(**bad) == -1 and b"bb_adamw_list" in handle.bb_last_error(), bad

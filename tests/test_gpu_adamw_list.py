@@ -309,3 +309,17 @@ def test_two_captured_clipped_steps_at_once(optim):
             want = e.step(optim, step=5, max_norm=0.5)
         assert norm.item() == want.item()
         assert all(torch.equal(a, b) for a, b in zip(l.masters, e.masters))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_large_and_small_gradients(optim, bits):
+    """Second moments as far as 32 bits hold (1 - beta2) g^2: gradients up to 1e20 with beta2 = 0.999, and down to where the square is lost."""
+    g = torch.tensor([1e20, -1e20, 1.0, 1e-15, 1e-18], device="cuda")
+    for value in g:
+        p, m, v = torch.zeros(300, device="cuda"), torch.zeros(300, device="cuda"), torch.zeros(300, device="cuda")
+        scales = None
+        if bits == 8:
+            m, v, scales = m.to(E4M3), v.to(E4M3), [torch.zeros(2, 2, device="cuda")]
+        optim.adamw_step_([p], [value.expand(300).contiguous()], [m], [v], scales=scales, step=1, lr=1.0, beta2=0.999, eps=0.0)
+        # (the first step is the sign of the gradient: m / bias and sqrt(v / bias) are both the gradient's size)
+        near(p, -torch.sign(value).double().expand(300), 2 ** -12 if abs(value) < 1e-17 else 2 ** -19)
