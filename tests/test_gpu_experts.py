@@ -738,3 +738,75 @@ def test_offsets_beyond_32_bits(ex):
     matmul(Bound(x[-2:].double()), Bound(w[-1].detach().double().t())).rounded().check(y[-2:].detach())
     (dw,) = torch.autograd.grad(y, w, dy)
     matmul(Bound(dy[-2:].double().t()), Bound(x[-2:].double())).rounded().check(dw[-1])
+
+
+def test_padding_columns_may_hold_anything(ex):
+    for n, cols in ((5, 8), (8, 16), (31, 32), (62, 64), (125, 128), (200, 256), (6, 7)):
+        for dtype in (FP32, BF16):
+            x = randn(300, cols, seed=n, scale=2.0).to(dtype)
+            clean = x.clone()
+            clean[:, n:] = 0
+            x[:, n:] = math.nan
+            x[::2, n:] = math.inf
+            results = []
+            for t in (clean, x):
+                leaf = t.clone().requires_grad_(True)
+                r = ex.route(leaf, 3, n)
+                (g,) = torch.autograd.grad((r.weights, r.balance), leaf, (torch.ones_like(r.weights), torch.tensor(1.0, device="cuda")))
+                results.append([r.weights.detach(), r.experts, r.rows, r.slots, r.offsets, r.balance.detach(), g])
+            assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_one_token_without_a_dimension_for_tokens(ex):
+    inputs = mixture_inputs(1)
+    r = ex.route(torch.randn(5, device="cuda"), 2)
+    assert r.weights.shape == r.rows.shape == (2,)
+    x = inputs[0][0]
+    rows = ex.dispatch(x, r)
+    y = ex.combine(ex.expert_mlp(rows, r.offsets, *inputs[2:]), r, residual=x)
+    many = ex.Routing(r.weights[None], r.experts[None], r.rows[None], r.slots, r.offsets)
+    assert torch.equal(rows, ex.dispatch(x[None], many)) and y.shape == (64,)
+    assert torch.equal(y[None], ex.combine(ex.expert_mlp(rows, r.offsets, *inputs[2:]), many, residual=x[None]))
+
+
+def test_gradients_of_what_is_shared(ex):
+    """One weight for all experts and one bias for all columns, by expand: their gradients are the sums."""
+    lengths, n, k = [40, 0, 100, 7], 64, 72
+    x, w, _, dy = product_inputs(lengths, 0, 0, n, k)
+    offsets, _ = offsets_of(lengths)
+    one, value = w[0].clone().requires_grad_(True), torch.tensor(0.5, device="cuda", dtype=BF16, requires_grad=True)
+    y = ex.grouped_linear(x, one.expand(4, n, k), offsets, value.expand(4, n))
+    dw, dv = torch.autograd.grad(y, (one, value), dy)
+    p = matmul(Bound(x.double()), Bound(one.detach().double().t()))
+    Bound(p.value + 0.5, p.err + 2 ** -23 * (p.value.abs() + 1)).rounded().check(y.detach())
+    d = dy.double()
+    # each expert's gradient is rounded to bf16, then autograd adds four, rounding again at most three times
+    parts = [matmul(Bound(a.t()), Bound(b)) for a, b in zip(d.split(lengths), x.double().split(lengths)) if len(a)]
+    size = sum(q.value.abs() + q.err for q in parts)
+    Bound(sum(q.value for q in parts), sum(q.err for q in parts) + 4 * 2 ** -8 * size).check(dw)
+    sums = torch.stack([a.sum(0) for a in d.split(lengths)])
+    # (256 rounded values, added with at most as many roundings of the partial sum in bf16 or better)
+    assert abs(dv.item() - sums.sum().item()) <= 2 ** -8 * (sums.abs().sum().item() + 256 * sums.cumsum(0).abs().max().item())
+
+
+@pytest.mark.parametrize("wanted", [(0,), (1,), (2,), (3,), (4,), (1, 2), (3, 4), (2, 4), (0, 2), (1, 3)])
+def test_some_gradients_of_the_mlp(ex, wanted):
+    """Those that are asked for alone, twice over one graph: the same as among all (a bias's sums without its weight go in another order)."""
+    lengths = [40, 0, 130, 7, 64]
+    offsets, _ = offsets_of(lengths)
+    inputs = [randn(241, 136, seed=1, dtype=BF16), *mixture_inputs(1, 136, 264, 5, seed=170)[2:]]
+    dy = randn(241, 136, seed=2, dtype=BF16)
+    every = [t.clone().requires_grad_(True) for t in inputs]
+    full = torch.autograd.grad(ex.expert_mlp(every[0], offsets, *every[1:]), every, dy)
+    some = [t.clone().requires_grad_(i in wanted) for i, t in enumerate(inputs)]
+    y = ex.expert_mlp(some[0], offsets, *some[1:])
+    leaves = [some[i] for i in wanted]
+    first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    again = torch.autograd.grad(y, leaves, dy)
+    for i, a, b in zip(wanted, first, again):
+        assert torch.equal(a, b)
+        if i in (2, 4) and i - 1 not in wanted:
+            # fp32 sums of up to 130 values in two orders, each rounded to bf16
+            near(a, full[i].double(), 2 ** -7, 130 * 2 ** -23 * 130)
+        else:
+            assert torch.equal(a, full[i]), i
