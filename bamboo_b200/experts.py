@@ -22,7 +22,8 @@ from .post_training import _aligned_rows, _on_current, _once_differentiable, _ro
 
 
 class Routing(NamedTuple):
-    """Where every token's rows are.  Slot s = t * k + j is the j-th choice of token t (the tokens of all leading dimensions counted through)."""
+    """Where every token's rows are.  Slot s = t * k + j is the j-th choice of token t (the tokens of all leading dimensions counted through).
+    ``rows`` and ``slots`` are each other's inverse; -1 put into ``rows`` alone drops a choice: its row then counts for nothing, in gradients too."""
     weights: torch.Tensor                       # [..., k] fp32
     experts: torch.Tensor                       # [..., k] int32, -1 where a token has fewer than k
     rows: torch.Tensor                          # [..., k] int32: place of every slot in the order by expert, -1: none

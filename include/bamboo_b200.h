@@ -494,7 +494,8 @@ int bb_dispatch_rows(const void* x, long long ld, int dtype, const int* slots, i
  * with -1 count for nothing.  residual may be NULL.  x has `rows` rows. */
 int bb_combine_rows(const void* x, long long ld, int dtype, const int* rows_of, const float* weights, const void* residual, long long ld_residual,
                     int k, void* out, long long tokens, long long rows, int h, void* stream);
-/* Backward of the weighted sum: dx[r] = weights[s] * dy[t] at the place of every slot s = t k + j, zeros in rows without a slot; d_weights[s] = dy[t] .
+/* Backward of the weighted sum: dx[r] = weights[s] * dy[t] at the place of every slot s = t k + j, zeros in rows without a slot (those that -1 in rows_of
+ * gave up included, whatever slots says); a place whose entry in slots is another slot sets the status word and is left out; d_weights[s] = dy[t] .
  * x[r] in fp32, 0 for slots without a place.  dx and x have `rows` rows, at most tokens k.  dx and d_weights may be NULL (x then too, where d_weights is). */
 int bb_combine_rows_bwd(const void* dy, long long ld_dy, int dtype, const void* x, long long ld, const int* rows_of, const int* slots,
                         const float* weights, int k, void* dx, float* d_weights, long long tokens, long long rows, int h, void* stream);

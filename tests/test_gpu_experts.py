@@ -295,6 +295,41 @@ def test_indexes_that_point_nowhere_are_left_out(ex):
     assert lib.read_status() == 0
 
 
+@pytest.mark.parametrize("hidden", [64, 77, 4104])
+def test_choices_dropped_by_their_place(ex, hidden):
+    """-1 in ``rows`` alone: the row that stays behind has a gradient of zeros, whatever lay in its memory."""
+    r = routing_of(ex, 40, 4, 2, 44)
+    rows = r.rows.clone()
+    rows[5:25, 1] = -1
+    r = r._replace(rows=rows)
+    places = rows[rows >= 0].long()
+    xs, dy = randn(80, hidden, seed=45).requires_grad_(True), randn(40, hidden, seed=46)
+    y = ex.combine(xs, r)
+    junk = [torch.full((80, hidden), math.nan, device="cuda") for _ in range(4)]
+    del junk
+    (dxs,) = torch.autograd.grad(y, xs, dy)
+    want = torch.zeros(80, hidden, dtype=torch.float64, device="cuda")
+    want[places] = (r.weights.double()[:, :, None] * dy.double()[:, None])[rows >= 0]
+    near(dxs, want, 2 ** -23)
+
+
+def test_places_that_name_another_slot_are_left_out(ex):
+    from bamboo_b200 import lib
+    r = routing_of(ex, 20, 4, 2, 47, masked=0.0)
+    rows = r.rows.clone()
+    there = rows >= 0
+    a, b = rows[there].long()[:2].tolist()                              # two slots at one place
+    rows[rows == b] = a
+    xs, dy = randn(40, 64, seed=48).requires_grad_(True), randn(20, 64, seed=49)
+    (dxs,) = torch.autograd.grad(ex.combine(xs, r._replace(rows=rows)), xs, dy)
+    torch.cuda.synchronize()
+    assert lib.read_status() == -1
+    (want,) = torch.autograd.grad(ex.combine(xs, r), xs, dy)
+    assert torch.all(dxs[b] == 0)
+    want[b] = 0
+    assert torch.equal(dxs, want)
+
+
 # ----------------------------------------------------------------------------------- products
 class Bound:
     """A value in 64 bits with a bound on how far the kernels' may be from it."""
