@@ -69,22 +69,27 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, scales=None, masters=No
     grads, exp_avgs, exp_avg_sqs, scales, masters = lists
     count = len(params)
     if not count:
-        return torch.zeros(()) if max_norm > 0 else None
+        if not max_norm > 0:
+            return None
+        return torch.zeros(()) if sumsq is None else (sumsq.detach().sqrt() * grad_scale).to(torch.float32).reshape(())
     _on_current(params[0], "params")
     device = params[0].get_device()
     moments = _FP32 if scales is None else _CODES
     addresses = list(_column(params, "params", count, _FP32 if masters is None else _BF16, None, device))
-    if len(set(addresses)) != count:
-        raise ValueError("params: a tensor stands in the list twice")
     if scales is not None and list(map(_sizes, scales)) != [2 * -(-n // BLOCK) for n in sizes]:
         raise ValueError("scales: [2, blocks of 256 values] for every parameter")
     if sumsq is not None and (sumsq.get_device() != device or sumsq.dtype != torch.float64):
         raise L.BambooNativeError("sumsq is fp64, on the parameters' device")
     nothing = itertools.repeat(0)
+    first = list(_column(exp_avgs, "exp_avgs", count, moments, sizes, device))
+    second = list(_column(exp_avg_sqs, "exp_avg_sqs", count, moments, sizes, device))
+    full = () if masters is None else list(_column(masters, "masters", count, _FP32, sizes, device))
+    scaled = () if scales is None else list(_column(scales, "scales", count, _FP32, None, device))
+    if len({*addresses, *first, *second, *full, *scaled}) != 3 * count + len(full) + len(scaled):
+        raise ValueError("a tensor stands twice among params, moments, scales and masters")
     fields = itertools.chain.from_iterable(zip(
-        addresses, nothing if masters is None else _column(masters, "masters", count, _FP32, sizes, device), _column(grads, "grads", count, _EITHER, sizes, device),
-        _column(exp_avgs, "exp_avgs", count, moments, sizes, device), _column(exp_avg_sqs, "exp_avg_sqs", count, moments, sizes, device),
-        nothing if scales is None else _column(scales, "scales", count, _FP32, None, device), sizes, map(L.dtype_codes().get, map(_dtype_of, grads)), nothing))
+        addresses, full or nothing, _column(grads, "grads", count, _EITHER, sizes, device), first, second, scaled or nothing, sizes,
+        map(L.dtype_codes().get, map(_dtype_of, grads)), nothing))
     norm = scratch = None
     if max_norm > 0:            # (no buffer that calls share: a captured one keeps its own)
         norm = torch.empty((), dtype=torch.float32, device=params[0].device)

@@ -233,6 +233,31 @@ def test_adamw_leaves_out_what_has_no_gradient(recorded):
     assert run(optim, args) is None and run(optim, args, max_norm=1.0) == 0.0 and not seen
 
 
+def test_adamw_refuses_a_state_that_two_parameters_share(recorded):
+    _, optim, seen = recorded
+    for kind in (dict(), dict(bits=8), dict(dtype=BF16)):
+        for name in ("exp_avgs", "exp_avg_sqs", "scales", "masters"):
+            args = lists(**kind)
+            if args.get(name) is None:
+                continue
+            args[name][2] = args[name][0]
+            with pytest.raises(ValueError, match="twice"):
+                run(optim, args)
+        args = lists(**kind)
+        args["exp_avg_sqs"] = args["exp_avgs"]
+        with pytest.raises(ValueError, match="twice"):
+            run(optim, args)
+    assert not seen
+
+
+def test_adamw_without_gradients_still_tells_the_norm_of_all(recorded):
+    _, optim, seen = recorded
+    args = lists()
+    args["grads"] = [None] * len(args["params"])
+    norm = run(optim, args, max_norm=1.0, sumsq=torch.full((1,), 9.0, dtype=torch.float64), grad_scale=0.5)
+    assert norm.shape == () and norm.dtype == torch.float32 and norm.item() == 1.5 and not seen
+
+
 def test_optimizer_object_refuses(recorded):
     _, optim, _ = recorded
     from bamboo_b200 import lib
