@@ -17,6 +17,7 @@
 #include "bamboo_b200.h"
 #include "gemm_panels.cuh"
 #include "tma_host.cuh"
+#include <atomic>
 #include <limits.h>
 #include <math.h>
 
@@ -49,6 +50,7 @@ struct GroupParams {
   int experts;
   int epi;
   int stage_bytes;            // that the copies of one CTA bring
+  int split, quarters;        // grouped_split_kernel: CTAs that share a tile's reduction, runs of 32 rows that an expert can have in a tile
   int rotate;                 // column tile i begins its reduction with k-block i: of few rows all CTAs would ask for the same few lines at once
   const int* offsets;
   void* D; void* D2; const void* bias; const void* aux;
@@ -193,6 +195,57 @@ struct ColumnSums {
   }
 };
 
+// A panel of 32 rows and 64 columns, its rows' sums in the lanes' `v` (and `aux`, where there is one, in the slab): through the epilogue and out
+__device__ __forceinline__ void finish_panel(const GroupParams& p, uint8_t* slab, const __nv_bfloat16* bias, bool dual, bool has_aux, long long base, int r0, int nb,
+                                             int end, int cols, int lane, float* v) {
+  if (bias) {
+    if (nb + 64 <= cols) {
+#pragma unroll
+      for (int i = 0; i < 64; i += 8) {
+        float f[8]; unpack8(__ldg(reinterpret_cast<const uint4*>(bias + nb + i)), f);
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) set2(v + i + k, bb::add2(get2(v + i + k), make_float2(f[k], f[k + 1])));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 64; ++i) if (nb + i < cols) v[i] += __bfloat162float(bias[nb + i]);
+    }
+  }
+  if (dual) {
+    panel_store_row_bf16(slab, lane, v);     // pre-activation first
+    __syncwarp();
+    slab_flush_bf16(slab, reinterpret_cast<__nv_bfloat16*>(p.D2), p.ldd, r0, nb, end, cols, lane);
+    // (of the sum itself: its rounding above is for the backward pass alone)
+#pragma unroll
+    for (int i = 0; i < 64; i += 2) set2(v + i, bb::gelu_tanh2(get2(v + i)));
+    __syncwarp();
+  } else if (has_aux) {
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float x[32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) unpack8(*reinterpret_cast<const uint4*>(slab + slab_off(lane, 4 * h + c)), x + 8 * c);
+      apply_aux<32>(p.epi, v + 32 * h, x);
+    }
+    __syncwarp();
+  }
+  panel_store_row_bf16(slab, lane, v);
+  __syncwarp();
+  slab_flush_bf16(slab, reinterpret_cast<__nv_bfloat16*>(p.D) + base, p.ldd, r0, nb, end, cols, lane);
+  __syncwarp();
+}
+
+// rows that belong to no expert
+__device__ __forceinline__ void zero_the_rest(const GroupParams& p, const int* start, int threads) {
+  const int before = start[0], after = p.rows - start[p.experts], chunks = p.n >> 3;
+  for (long long i = (long long)blockIdx.x * threads + threadIdx.x; i < (long long)(before + after) * chunks; i += (long long)gridDim.x * threads) {
+    const int r = (int)(i / chunks), c = (int)(i - (long long)r * chunks);
+    reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.D) + (long long)(r < before ? r : start[p.experts] + r - before) * p.ldd)[c] =
+        make_uint4(0, 0, 0, 0);
+  }
+}
+
 template <int MODE, int BN, bool PAIR>
 __global__ void __launch_bounds__(THREADS<MODE == WGRAD>, 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GroupParams p) {
@@ -252,13 +305,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
     __syncthreads();
   } else {
-    // rows that belong to no expert
-    const int before = start[0], after = p.rows - start[p.experts], chunks = p.n >> 3;
-    for (long long i = (long long)blockIdx.x * THREADS<false> + threadIdx.x; i < (long long)(before + after) * chunks; i += (long long)gridDim.x * THREADS<false>) {
-      const int r = (int)(i / chunks), c = (int)(i - (long long)r * chunks);
-      reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.D) + (long long)(r < before ? r : start[p.experts] + r - before) * p.ldd)[c] =
-          make_uint4(0, 0, 0, 0);
-    }
+    zero_the_rest(p, start, THREADS<false>);
   }
   Walk<MODE == WGRAD, BN, C::TILE_M> walk(p, start, order, worker, workers);
   Unit u;
@@ -440,9 +487,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   } else {
     // ------------------------------------------------ epilogue: eight warps, two per TMEM lane quarter, panels of 128 bytes in turn
     const int eg = (warp - EPI_WARP) >> 2, quarter = warp & 3;
-    const int epi = p.epi;
-    const bool f32 = MODE == WGRAD && epi == BB_EPI_ACCUM_F32, dual = MODE == ROWS && epi == BB_EPI_BIAS_GELU;
-    const bool has_aux = MODE == ROWS_T && epi == BB_EPI_MUL_DGELU, has_bias = MODE == ROWS && (epi == BB_EPI_BIAS || dual);
+    const bool f32 = MODE == WGRAD && p.epi == BB_EPI_ACCUM_F32, dual = MODE == ROWS && p.epi == BB_EPI_BIAS_GELU;
+    const bool has_aux = MODE == ROWS_T && p.epi == BB_EPI_MUL_DGELU, has_bias = MODE == ROWS && (p.epi == BB_EPI_BIAS || dual);
     const int cols = MODE == WGRAD ? p.k : p.n;
     uint8_t* slab = panels + (warp - EPI_WARP) * SLAB_BYTES;
     int acc = 0; uint32_t acc_phase = 0;
@@ -503,42 +549,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           __syncwarp();
           continue;
         }
-        if (has_bias) {
-          if (nb + 64 <= cols) {
-#pragma unroll
-            for (int i = 0; i < 64; i += 8) {
-              float f[8]; unpack8(__ldg(reinterpret_cast<const uint4*>(bias + nb + i)), f);
-#pragma unroll
-              for (int k = 0; k < 8; k += 2) set2(v + i + k, bb::add2(get2(v + i + k), make_float2(f[k], f[k + 1])));
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) if (nb + i < cols) v[i] += __bfloat162float(bias[nb + i]);
-          }
-        }
-        if (dual) {
-          panel_store_row_bf16(slab, lane, v);     // pre-activation first
-          __syncwarp();
-          slab_flush_bf16(slab, reinterpret_cast<__nv_bfloat16*>(p.D2), p.ldd, r0, nb, u.end, cols, lane);
-          // (of the sum itself: its rounding above is for the backward pass alone)
-#pragma unroll
-          for (int i = 0; i < 64; i += 2) set2(v + i, bb::gelu_tanh2(get2(v + i)));
-          __syncwarp();
-        } else if (has_aux) {
-          __syncwarp();
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float x[32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) unpack8(*reinterpret_cast<const uint4*>(slab + slab_off(lane, 4 * h + c)), x + 8 * c);
-            apply_aux<32>(epi, v + 32 * h, x);
-          }
-          __syncwarp();
-        }
-        panel_store_row_bf16(slab, lane, v);
-        __syncwarp();
-        slab_flush_bf16(slab, reinterpret_cast<__nv_bfloat16*>(p.D) + base, p.ldd, r0, nb, u.end, cols, lane);
-        __syncwarp();
+        finish_panel(p, slab, bias, dual, has_aux, base, r0, nb, u.end, cols, lane, v);
       }
       if (!none && ++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
@@ -554,6 +565,174 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     __syncthreads();
     if (warp == MMA_WARP) bb::tmem_dealloc(tmem_base, C::TMEM_COLS);
   }
+}
+
+// Few tiles and a long reduction: a cluster of 2, 4 or 8 CTAs shares a tile's reduction, each over a run of its k-blocks (a k-block takes about 0.28 us
+// however idle the GPU is: its latency, not its bytes).  Panels of 64 columns are dealt out to the CTAs; each sends its sums of the others' panels into their
+// operand stages, by then unused, and adds what it received to its own in the order of the CTAs: the same bits every time.  A cluster has one tile.
+// Received panels: [other CTA][run of 32 rows][16 bytes of a row][row], so that a warp's access is one run of memory.
+template <int MODE, int BN>
+__global__ void __launch_bounds__(THREADS<false>, 1)
+grouped_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GroupParams p) {
+  using C = Cfg<BN, false>;
+  constexpr int NP = BN / 64, PART_BYTES = 32 * 64 * 4;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + C::STAGES * A_STAGE_BYTES;
+  uint8_t* panels = smem + C::STAGES * C::STAGE_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(panels + EPI_WARPS * SLAB_BYTES);      // [STAGES]
+  uint64_t* empty_bar = full_bar + C::STAGES;       // [STAGES]
+  uint64_t* tmem_full = empty_bar + C::STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* start = reinterpret_cast<int*>(tmem_slot + 2);                                     // [experts + 1]
+
+  const int warp = bb::warp_index(), lane = threadIdx.x & 31;
+  const int S = p.split, ks = (int)bb::cluster_ctarank();
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < C::STAGES; ++s) { bb::mbar_init(&full_bar[s], 1); bb::mbar_init(&empty_bar[s], 1); }
+    bb::mbar_init(tmem_full, 1);
+    bb::fence_barrier_init();
+    bb::tma_prefetch_desc(&tmA);
+    bb::tma_prefetch_desc(&tmB);
+  }
+  if (warp == MMA_WARP) { bb::tmem_alloc(tmem_slot, BN); bb::tmem_relinquish(); }
+  bb::pdl_sync();
+  if (warp == EPI_WARP) read_offsets(p, start, lane);
+  bb::tc_fence_before_sync();
+  __syncthreads();
+  bb::tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  zero_the_rest(p, start, THREADS<false>);
+  Walk<false, BN, BM> walk(p, start, nullptr, (int)bb::cluster_id(), (int)gridDim.x / S);
+  Unit u = {};
+  const bool some = walk.next(u);
+  const int kb0 = ks * u.num_kb / S, num_kb = (ks + 1) * u.num_kb / S - kb0;                       // (at least one: the host sees to it)
+
+  const int eg = (warp - EPI_WARP) >> 2, quarter = warp & 3, r0 = u.m0 + quarter * 32, cols = p.n;
+  const bool dual = MODE == ROWS && p.epi == BB_EPI_BIAS_GELU;
+  const bool has_aux = MODE == ROWS_T && p.epi == BB_EPI_MUL_DGELU, has_bias = MODE == ROWS && (p.epi == BB_EPI_BIAS || dual);
+  uint8_t* slab = panels + (warp - EPI_WARP) * SLAB_BYTES;
+  const int own = ks + eg * S, nb_own = u.n0 + own * 64;    // this warp's panel
+  bool summed = false;
+  if (!some) {
+  } else if (warp == TMA_WARP_0 || warp == TMA_WARP_1) {
+    const int turn = warp == TMA_WARP_1 ? 1 : 0;
+    int s = 0; uint32_t phase = 0;
+    bool alive = true;
+    int at = p.rotate ? u.ni % num_kb : 0;
+    for (int kb = 0; kb < num_kb; ++kb) {
+      if ((s & 1) == turn) {
+        if (!bb::mbar_wait_warp(&empty_bar[s], phase ^ 1, abort_flag, p.status)) { alive = false; break; }
+        uint8_t* a = sA + s * A_STAGE_BYTES;
+        uint8_t* b = sB + s * C::B_STAGE_BYTES;
+        const int k0 = (kb0 + at) * BK;
+        if (bb::elect_one()) {
+          bb::mbar_arrive_expect_tx(&full_bar[s], p.stage_bytes);
+          bb::tma_load_2d(a, &tmA, &full_bar[s], k0, u.m0);
+          if constexpr (MODE == ROWS) {
+            bb::tma_load_3d(b, &tmB, &full_bar[s], k0, u.n0, u.e);
+          } else {
+#pragma unroll
+            for (int j = 0; j < C::B_ROWS / 64; ++j) bb::tma_load_3d(b + j * 8192, &tmB, &full_bar[s], u.n0 + 64 * j, k0, u.e);
+          }
+        }
+        __syncwarp();
+      }
+      if (++at == num_kb) at = 0;
+      if (++s == C::STAGES) { s = 0; phase ^= 1; }
+    }
+    if (!alive) {
+      // copies still in flight get time to land (bounded)
+      const uint64_t t0 = bb::globaltimer_ns();
+      while (bb::globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    }
+  } else if (warp == MMA_WARP) {
+    constexpr uint32_t B_MN = MODE != ROWS;
+    constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | (B_MN << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+    constexpr uint32_t B_LBO = B_MN ? 8192u : 16u, B_STEP = B_MN ? 2048u : 32u;
+    int s = 0; uint32_t phase = 0;
+    for (int kb = 0; kb < num_kb; ++kb) {
+      if (!bb::mbar_wait_warp(&full_bar[s], phase, abort_flag, p.status)) break;
+      bb::tc_fence_after_sync();
+      if (bb::elect_one()) {
+        const uint64_t ad0 = bb::make_smem_desc_sw128(bb::smem_u32(sA + s * A_STAGE_BYTES), 16u, 1024u);
+        const uint64_t bd0 = bb::make_smem_desc_sw128(bb::smem_u32(sB + s * C::B_STAGE_BYTES), B_LBO, 1024u);
+#pragma unroll
+        for (int k = 0; k < BK / UMMA_K; ++k)
+          bb::umma_f16(tmem_base, ad0 + (uint64_t)(k * (32u >> 4)), bd0 + (uint64_t)(k * (B_STEP >> 4)), IDESC, (kb > 0 || k > 0) ? 1u : 0u);
+        bb::umma_commit(&empty_bar[s]);
+        if (kb == num_kb - 1) bb::umma_commit(tmem_full);
+      }
+      __syncwarp();
+      if (++s == C::STAGES) { s = 0; phase ^= 1; }
+    }
+  } else {
+    // the pre-activation of the own panel comes under the main loop
+    if (has_aux && own < NP && nb_own < cols && r0 < u.end) {
+      uint4 ax[8];
+      slab_fetch_bf16(reinterpret_cast<const __nv_bfloat16*>(p.aux), p.ld_aux, r0, nb_own, u.end, cols, lane, ax);
+      slab_put(slab, lane, ax);
+    }
+    summed = bb::mbar_wait_warp(tmem_full, 0, abort_flag, p.status) && r0 < u.end;
+    bb::tc_fence_after_sync();
+  }
+  __syncwarp();
+  // every CTA's MMAs have retired, so its stages can receive (all of its copies have landed)
+  bb::cluster_sync();
+  const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16);
+  if (summed) {
+    int turn = 0;
+    for (int i = 1; i < S; ++i) {                           // the CTAs start with different owners
+      const int owner = ks + i < S ? ks + i : ks + i - S, slot = ks < owner ? ks : ks - 1;
+      for (int pn = owner, from = slot; pn < NP; pn += S, from += S - 1) {
+        if ((turn++ & 1) != eg || u.n0 + pn * 64 >= cols) continue;
+        const uint32_t dst = bb::mapa_shared(bb::smem_u32(smem) + (from * p.quarters + quarter) * PART_BYTES + lane * 16, owner);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r[32];
+          bb::tmem_ld_32x32b_x32(t_row + pn * 64 + h * 32, r);
+          bb::tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) bb::st_shared_cluster_v4(dst + (h * 8 + j) * 512, r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  bb::cluster_sync();
+  if (summed && own < NP && nb_own < cols) {
+    float v[64];
+#pragma unroll
+    for (int i = 0; i < 64; ++i) v[i] = 0.f;
+    const uint8_t* part = smem + (eg * (S - 1) * p.quarters + quarter) * PART_BYTES + lane * 16;
+    for (int t = 0; t < S; ++t) {
+      if (t == ks) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r[32];
+          bb::tmem_ld_32x32b_x32(t_row + own * 64 + h * 32, r);
+          bb::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[h * 32 + i] += __uint_as_float(r[i]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float4 q = *reinterpret_cast<const float4*>(part + j * 512);
+          v[4 * j] += q.x; v[4 * j + 1] += q.y; v[4 * j + 2] += q.z; v[4 * j + 3] += q.w;
+        }
+        part += p.quarters * PART_BYTES;
+      }
+    }
+    const __nv_bfloat16* bias = has_bias ? reinterpret_cast<const __nv_bfloat16*>(p.bias) + (long long)u.e * p.n : nullptr;
+    finish_panel(p, slab, bias, dual, has_aux, 0, r0, nb_own, u.end, cols, lane, v);
+  }
+  bb::tc_fence_before_sync();
+  __syncthreads();
+  if (warp == MMA_WARP) bb::tmem_dealloc(tmem_base, BN);
 }
 
 // The column tiles' sums (see ColumnSums), in their order
@@ -645,8 +824,43 @@ grouped_colsum_kernel(const __nv_bfloat16* dy, long long ld, const int* offsets,
 // ---------------------------------------------------------------- host side
 int refuse(const char* msg) { bb_set_last_error_msg(msg); return BB_ERR_INVALID_ARG; }
 
+// Whether S CTAs can share a tile's reduction: each has a k-block at least, and what it receives fits its operand stages
+int quarters_of(const bb_grouped_desc* d) { return d->rows < BM ? (d->rows + 31) / 32 : BM / 32; }
+template <int BN> bool can_split(const bb_grouped_desc* d, int S, int num_kb) {
+  const int owned = (BN / 64 + S - 1) / S;
+  return num_kb >= S && num_kb < INT_MAX / 8 && owned * (S - 1) * quarters_of(d) * 8192 <= Cfg<BN, false>::STAGES * Cfg<BN, false>::STAGE_BYTES;
+}
+template <int BN> cudaLaunchConfig_t split_config(int S, long long tiles, cudaLaunchAttribute (&attr)[2]) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles < 1 ? 1 : tiles) * S); cfg.blockDim = dim3(THREADS<false>); cfg.dynamicSmemBytes = Cfg<BN, false>::SMEM_BYTES;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = S; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = 1;
+  return cfg;
+}
+// Clusters of S CTAs that the device holds at the same time (of 2: 74, of 4: 33, of 8: 15); 0 when it cannot be asked
+template <int MODE, int BN> int clusters_at_once(int S) {
+  static std::atomic<int> cache[64][9];
+  const int dev = bb_current_device();
+  if (dev < 0) return 0;
+  int n = cache[dev][S].load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaLaunchAttribute attr[2];
+    const cudaLaunchConfig_t cfg = split_config<BN>(S, 1, attr);
+    if (cudaFuncSetAttribute(grouped_split_kernel<MODE, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<BN, false>::SMEM_BYTES) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, grouped_split_kernel<MODE, BN>, &cfg) != cudaSuccess) {
+      (void)cudaGetLastError();
+      n = 0;
+    }
+    if (n <= 0) n = -1;
+    cache[dev][S].store(n, std::memory_order_relaxed);
+  }
+  return n > 0 ? n : 0;
+}
+
 template <int MODE, int BN, bool PAIR>
-int launch(const bb_grouped_desc* d, cudaStream_t stream) {
+int launch(const bb_grouped_desc* d, cudaStream_t stream, int split = 1) {
   using C = Cfg<BN, PAIR>;
   CUtensorMap tmA, tmB;
   GroupParams p = {};
@@ -679,7 +893,20 @@ int launch(const bb_grouped_desc* d, cudaStream_t stream) {
     tiles = row_tiles * ((p.n + BN - 1) / BN);
   }
   if (rc) return rc;
-  if (tiles > INT_MAX / 2) return refuse("bb_grouped_gemm: more tiles than one launch covers");
+  if (tiles > INT_MAX / 2 / split) return refuse("bb_grouped_gemm: more tiles than one launch covers");
+  if constexpr (MODE != WGRAD && !PAIR) {
+    if (split > 1) {
+      p.split = split;
+      p.quarters = quarters_of(d);
+      BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(grouped_split_kernel<MODE, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES)));
+      cudaLaunchAttribute attr[2];
+      cudaLaunchConfig_t cfg = split_config<BN>(split, tiles, attr);
+      cfg.stream = stream;
+      if (bb_back_to_back > 0) cfg.numAttrs = 2;
+      BB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, grouped_split_kernel<MODE, BN>, tmA, tmB, p));
+      return BB_OK;
+    }
+  }
   BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(grouped_gemm_kernel<MODE, BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES)));
   int workers = PAIR ? bb_num_sms() / 2 : bb_num_sms();
   if (d->max_ctas > 0 && d->max_ctas / (PAIR ? 2 : 1) < workers) workers = d->max_ctas / (PAIR ? 2 : 1);
@@ -712,16 +939,20 @@ int launch(const bb_grouped_desc* d, cudaStream_t stream) {
 // an epilogue: 16384 rows of 8 experts, 4096 x 1024, 103 | 116 | 144 (1.33 PFLOP/s); 16384 of 64, 1024 x 1024, 44 | 49 | 54; 4096 of 64,
 // 2048 x 512, 33 | 31 | 31; 2000 of 16, 1416 x 776, 19 | 15 | 16; 1024 of 8, 1024 x 256, 9.2 | 8.3 | 6.8; 14 of 8, 4096 x 1024, 19 | 15 | 20.  Tiles of 64
 // columns were never quicker (248 | 7.4 | 26 us).
+// A shared reduction where one wave of clusters holds all tiles that there may be, every CTA has four k-blocks or more, and it is expected to be quicker by a
+// twentieth; the exchange grows with the CTAs and with the rows.  us, whole | shared by 2 | 4 | 8, the quickest kinds: 14 rows of 8 experts, 1024 x 4096, 23 | 17 |
+// 17 | 24; 2 rows of it 22 | 15 | 11 | 11; 1024 rows of 8, 512 x 2048, 14 | 12 | 13; 2000 of 8, 512 x 4096, 23 | 20 | 27; 1 row, 4096 x 4096, 22 | 15 | 12 | 20;
+// 14 of 8, 4096 x 1024, 14.5 | 21 | 32.
 template <int MODE> int choose(const bb_grouped_desc* d, cudaStream_t stream) {
-  static const struct { int bn; bool pair; double kblock, wave, once; } kinds[3] = {
-      {256, true, 0.32, 1.9, 5.0}, {256, false, 0.375, 1.8, 3.7}, {128, false, 0.283, 1.0, 3.7}};
+  static const struct { int bn; bool pair; double kblock, wave, once, shared; } kinds[3] = {
+      {256, true, 0.32, 1.9, 5.0, 0}, {256, false, 0.375, 1.8, 3.7, 6.0}, {128, false, 0.283, 1.0, 3.7, 5.0}};
   const double used = d->rows < d->experts ? d->rows : d->experts, each = d->rows / used;
-  int best = 0;
+  int best = 0, best_split = 1;
   double best_us = -1;
   for (int i = 0; i < 3; ++i) {
     const auto& k = kinds[i];
     if ((d->tile_n && d->tile_n != k.bn) || (d->cta_pair && (d->cta_pair > 0) != k.pair)) continue;
-    const int tm = k.pair ? 2 * BM : BM, n = MODE == ROWS ? d->n : d->k;
+    const int tm = k.pair ? 2 * BM : BM, n = MODE == ROWS ? d->n : d->k, num_kb = ((MODE == ROWS ? d->k : d->n) + BK - 1) / BK;
     double row_tiles, kb;
     if (MODE == WGRAD) {
       row_tiles = (double)d->experts * ((d->n + tm - 1) / tm);
@@ -729,15 +960,26 @@ template <int MODE> int choose(const bb_grouped_desc* d, cudaStream_t stream) {
     } else {
       const double per = each / tm + 0.5;
       row_tiles = used * (per > 1 ? per : 1);
-      kb = ((MODE == ROWS ? d->k : d->n) + BK - 1) / BK;
+      kb = num_kb;
     }
     int workers = bb_num_sms();
     if (d->max_ctas > 0 && d->max_ctas < workers) workers = d->max_ctas;
     if (k.pair) workers = workers > 1 ? workers / 2 : 1;
-    const double us = ceil(row_tiles * ((n + k.bn - 1) / k.bn) / workers) * (kb * k.kblock + k.wave) + k.once;
-    if (best_us < 0 || us < best_us) { best_us = us; best = i; }
+    const double whole = ceil(row_tiles * ((n + k.bn - 1) / k.bn) / workers) * (kb * k.kblock + k.wave) + k.once;
+    if (d->split < 2 && (best_us < 0 || whole < best_us)) { best_us = whole; best = i; best_split = 1; }
+    if constexpr (MODE != WGRAD) {
+      const long long most = ((long long)d->rows / BM + (long long)used) * ((n + k.bn - 1) / k.bn);
+      for (int S = 2; S <= 8 && !k.pair && d->max_ctas == 0 && d->split != 1; S *= 2) {
+        if (d->split > 1 && S != d->split) continue;
+        if (!(k.bn == 128 ? can_split<128>(d, S, num_kb) : can_split<256>(d, S, num_kb))) continue;
+        if (d->split < 2 && (num_kb < 4 * S || most > (k.bn == 128 ? clusters_at_once<MODE, 128>(S) : clusters_at_once<MODE, 256>(S)))) continue;
+        const double us = 1.05 * ((num_kb + S - 1) / S * k.kblock + k.shared + 0.2 * quarters_of(d) * S);
+        if (best_us < 0 || us < best_us) { best_us = us; best = i; best_split = S; }
+      }
+    }
   }
-  return best == 0 ? launch<MODE, 256, true>(d, stream) : best == 1 ? launch<MODE, 256, false>(d, stream) : launch<MODE, 128, false>(d, stream);
+  if (best_us < 0) return refuse("bb_grouped_gemm: a reduction that cannot be split like this");
+  return best == 0 ? launch<MODE, 256, true>(d, stream) : best == 1 ? launch<MODE, 256, false>(d, stream, best_split) : launch<MODE, 128, false>(d, stream, best_split);
 }
 
 bool bad_sizes(const bb_grouped_desc* d) {
@@ -764,6 +1006,9 @@ extern "C" int bb_grouped_gemm(const bb_grouped_desc* d, void* stream) {
     return refuse("bb_grouped_gemm: operands are 16-byte aligned, with rows of a multiple of 8 values that do not overlap");
   if ((d->tile_n != 0 && d->tile_n != 128 && d->tile_n != 256) || (d->cta_pair > 0 && d->tile_n == 128))
     return refuse("bb_grouped_gemm: tile_n is 128 or 256, of a CTA pair 256");
+  if (d->split != 0 && d->split != 1 && d->split != 2 && d->split != 4 && d->split != 8) return refuse("bb_grouped_gemm: a reduction is split in 1, 2, 4 or 8");
+  if (d->split > 1 && (wgrad || d->cta_pair > 0 || d->max_ctas > 0))
+    return refuse("bb_grouped_gemm: a reduction is split among single CTAs, without max_ctas, and not that of a weight gradient");
   if ((d->bias_grad || d->bias_accum) && (!wgrad || (d->bias_grad && d->bias_accum) || ((uintptr_t)d->bias_grad & 1) || ((uintptr_t)d->bias_accum & 3)))
     return refuse("bb_grouped_gemm: a bias gradient goes with a weight gradient, to one place");
   if ((d->bias_grad || d->bias_accum) && (!d->bias_parts || ((uintptr_t)d->bias_parts & 15) || d->bias_parts_bytes < bb_grouped_bias_bytes(d->n, d->k, d->experts)))

@@ -99,7 +99,7 @@ class GroupedDesc(ctypes.Structure):
         ("out", ctypes.c_void_p), ("ld_out", ctypes.c_longlong),
         ("bias", ctypes.c_void_p), ("out2", ctypes.c_void_p),
         ("aux", ctypes.c_void_p), ("ld_aux", ctypes.c_longlong),
-        ("max_ctas", ctypes.c_int), ("tile_n", ctypes.c_int), ("cta_pair", ctypes.c_int),
+        ("max_ctas", ctypes.c_int), ("tile_n", ctypes.c_int), ("cta_pair", ctypes.c_int), ("split", ctypes.c_int),
         ("bias_grad", ctypes.c_void_p), ("bias_accum", ctypes.c_void_p), ("bias_parts", ctypes.c_void_p), ("bias_parts_bytes", ctypes.c_longlong),
     ]
 
@@ -840,7 +840,7 @@ def grouped_bias_scratch(experts, n, k):
     return load().bb_grouped_bias_bytes(n, k, experts)
 
 
-def grouped_gemm(mode, x, weight, offsets, out, *, epilogue=EPI_STORE, bias=None, out2=None, aux=None, max_ctas=0, tile_n=0, cta_pair=0, bias_grad=None,
+def grouped_gemm(mode, x, weight, offsets, out, *, epilogue=EPI_STORE, bias=None, out2=None, aux=None, max_ctas=0, tile_n=0, cta_pair=0, split=0, bias_grad=None,
                  bias_accum=None, bias_parts=None):
     """GROUPED_ROWS: x [rows, k], weight [experts, n, k], out [rows, n]; GROUPED_INPUT: x [rows, n], out [rows, k]; GROUPED_WEIGHT: x [rows, n],
     weight [rows, k], out [experts, n, k].  2-D tensors have unit inner stride, rows on 16 bytes; see bb_grouped_gemm."""
@@ -852,7 +852,7 @@ def grouped_gemm(mode, x, weight, offsets, out, *, epilogue=EPI_STORE, bias=None
     d = GroupedDesc(mode=mode, rows=x.shape[0], n=n, k=k, experts=experts, epilogue=epilogue, offsets=offsets.data_ptr(), x=x.data_ptr(),
                     ld_x=_ld(x), weight=weight.data_ptr(), ld_weight=_ld(weight) if wgrad else 0, out=out.data_ptr(),
                     ld_out=0 if wgrad else _ld(out), bias=_addr(bias), out2=_addr(out2), aux=_addr(aux), ld_aux=0 if aux is None else _ld(aux),
-                    max_ctas=max_ctas or GEMM_MAX_CTAS, tile_n=tile_n, cta_pair=cta_pair, bias_grad=_addr(bias_grad), bias_accum=_addr(bias_accum),
+                    max_ctas=max_ctas or GEMM_MAX_CTAS, tile_n=tile_n, cta_pair=cta_pair, split=split, bias_grad=_addr(bias_grad), bias_accum=_addr(bias_accum),
                     bias_parts=_addr(bias_parts), bias_parts_bytes=0 if bias_parts is None else bias_parts.numel())
     check((_lib or load()).bb_grouped_gemm(ctypes.byref(d), _raw_stream()), "bb_grouped_gemm")
     return out

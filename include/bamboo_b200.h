@@ -439,6 +439,7 @@ typedef struct bb_grouped_desc {
   int max_ctas;                                 /* see bb_gemm_desc.max_ctas */
   int tile_n;                                   /* 0 = choose, else 128 or 256 columns */
   int cta_pair;                                 /* 0 = choose, 1 = CTA pairs (256 x 256 tiles), -1 = single CTAs */
+  int split;                                    /* CTAs that share a tile's reduction: 0 = choose, else 1, 2, 4 or 8 (single CTAs; not a weight gradient, and not with max_ctas) */
   void* bias_grad; float* bias_accum;           /* BB_GROUPED_WEIGHT: also the sum of every expert's rows of x, to one of them: bf16 [experts, n], or
                                                    fp32 [experts, n] (+=); NULL: not wanted */
   float* bias_parts; long long bias_parts_bytes;/* scratch for it, bb_grouped_bias_bytes() */

@@ -117,6 +117,15 @@ def test_products_refuse(recorded):
     assert seen[0][0] == "grouped_gemm" and seen[0][1][3].dtype == torch.int32
 
 
+def test_native_calls_refuse_reductions_that_cannot_be_split():
+    from bamboo_b200 import lib
+    handle, at = lib.load(), 1 << 20
+    good = dict(mode=0, rows=64, n=64, k=64, experts=4, epilogue=0, offsets=at, x=at, ld_x=64, weight=at, out=at, ld_out=64)
+    for change in (dict(split=3), dict(split=-2), dict(split=16), dict(split=2, max_ctas=8), dict(split=4, tile_n=256, cta_pair=1), dict(split=2, mode=2, ld_weight=64)):
+        d = lib.GroupedDesc(**{**good, **change})
+        assert handle.bb_grouped_gemm(ctypes.byref(d), None) == -1 and b"split" in handle.bb_last_error(), change
+
+
 def test_native_calls_refuse_what_python_would_not_send():
     from bamboo_b200 import lib
     handle, at = lib.load(), 1 << 20

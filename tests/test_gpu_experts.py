@@ -547,6 +547,64 @@ def test_many_tiles_a_cta_on_every_kind(ex, tile):
     test_grouped_linear(ex, [5] * 200, 0, 0, 264, 520, True)
 
 
+SPLITS = [(2, 128), (4, 128), (8, 128), (2, 256), (4, 256), (8, 256)]
+
+
+@pytest.fixture
+def split(request, ex, monkeypatch):
+    """Reductions shared by so many CTAs wherever they are long enough."""
+    from bamboo_b200 import lib
+    ctas, tile_n = request.param
+    product, calls = lib.grouped_gemm, []
+
+    def shared(mode, x, w, offsets, out, **kw):
+        length = -(-x.shape[1] // 64)
+        if mode == lib.GROUPED_WEIGHT or length < ctas or (ctas == 8 and x.shape[0] > 96):
+            return product(mode, x, w, offsets, out, **kw)
+        calls.append(mode)
+        return product(mode, x, w, offsets, out, tile_n=tile_n, cta_pair=-1, split=ctas, **kw)
+
+    monkeypatch.setattr(lib, "grouped_gemm", shared)
+    return calls
+
+
+@pytest.mark.parametrize("split", SPLITS, indirect=True)
+@pytest.mark.parametrize("n,k", [(136, 520), (1000, 264), (2056, 1032)])
+@pytest.mark.parametrize("lengths,before,after", [([1], 0, 0), ([5, 0, 3], 2, 5), ([33, 0, 31, 32], 0, 0), ([0, 0], 0, 9), ([1] * 40, 0, 3), ([64, 65, 127, 129], 3, 1)])
+def test_grouped_linear_with_shared_reductions(ex, split, lengths, before, after, n, k):
+    test_grouped_linear(ex, lengths, before, after, n, k, True)
+    assert split or before + sum(lengths) + after > 96
+
+
+@pytest.mark.parametrize("split", SPLITS, indirect=True)
+def test_epilogues_of_shared_reductions(ex, split):
+    from bamboo_b200 import lib
+    lengths, before, after, n, k = [40, 0, 7, 33], 2, 3, 1000, 776
+    x, w, b, dy = product_inputs(lengths, before, after, n, k, seed=61)
+    offsets, _ = offsets_of(lengths, before)
+    pre, act, dx = (torch.full((x.shape[0], c), math.nan, device="cuda", dtype=BF16) for c in (n, n, k))
+    aux = randn(x.shape[0], k, seed=65, dtype=BF16)
+    lib.grouped_gemm(lib.GROUPED_ROWS, x, w, offsets, act, epilogue=lib.EPI_BIAS_GELU, bias=b, out2=pre)
+    lib.grouped_gemm(lib.GROUPED_INPUT, dy, w, offsets, dx, epilogue=lib.EPI_MUL_DGELU, aux=aux)
+    assert len(split) == 2
+    own = torch.zeros(x.shape[0], dtype=torch.bool, device="cuda")
+    for e, at, count, _ in per_expert(lambda e: None, lengths, before):
+        if not count:
+            continue
+        rows = slice(at, at + count)
+        own[rows] = True
+        p = matmul(Bound(x[rows].double()), Bound(w[e].double().t()))
+        p = Bound(p.value + b[e].double(), p.err + 2 ** -23 * (p.value.abs() + b[e].double().abs()))
+        p.rounded().check(pre[rows])
+        gelu_bound(p).rounded().check(act[rows])
+        z = aux[rows].double().requires_grad_(True)
+        (slope,) = torch.autograd.grad(gelu(z).sum(), z)
+        g = matmul(Bound(dy[rows].double()), Bound(w[e].double()))
+        # (the slope's tanh is off by 2^-10.9 in two places, as in the expert MLP's test)
+        Bound(g.value * slope, g.err * (slope.abs() + 2 ** -9) + g.value.abs() * 2 ** -9).rounded().check(dx[rows])
+    assert torch.all(act[~own] == 0) and torch.all(dx[~own] == 0)
+
+
 @pytest.mark.parametrize("lengths,before,after", [([3], 0, 0), ([40, 0, 130, 7], 0, 5), ([300, 200], 1, 0), ([16] * 12, 0, 0)])
 @pytest.mark.parametrize("inner,k", [(64, 64), (264, 136), (1024, 256)])
 def test_expert_mlp(ex, lengths, before, after, inner, k):
