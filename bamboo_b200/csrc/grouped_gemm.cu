@@ -13,6 +13,7 @@
 //
 // The main loop is that of the dense product (gemm_tcgen05.cu): two producer warps, one MMA warp, eight epilogue warps, six
 // stages of 32 KiB, two accumulators; pairs of CTAs (cta_group::2) on 256 x 256 tiles where the experts are large enough.
+// Where tiles are few and reductions long, CTAs share them: rows in clusters (grouped_split_kernel), weight gradients in parts (grouped_join_kernel).
 #include "common.cuh"
 #include "bamboo_b200.h"
 #include "gemm_panels.cuh"
@@ -50,12 +51,14 @@ struct GroupParams {
   int experts;
   int epi;
   int stage_bytes;            // that the copies of one CTA bring
-  int split, quarters;        // grouped_split_kernel: CTAs that share a tile's reduction, runs of 32 rows that an expert can have in a tile
+  int split, quarters;        // grouped_split_kernel: CTAs that share a tile's reduction, runs of 32 rows that an expert can have in a tile; weight
+                              // gradient: parts of each reduction, every one a unit of its own
   int rotate;                 // column tile i begins its reduction with k-block i: of few rows all CTAs would ask for the same few lines at once
   const int* offsets;
   void* D; void* D2; const void* bias; const void* aux;
   __nv_bfloat16* bias_grad; float* bias_accum;            // weight gradient: where db_e goes (one of them, or none) ...
-  float* bias_parts;          // ... by way of [column tiles][experts][n], where there is more than one column of tiles
+  float* bias_parts;          // ... by way of [parts][column tiles][experts][n], where these are more than one
+  float* parts;               // weight gradient in parts: [parts][experts][n][k]
   long long ldd, ld_aux, expert_stride;       // expert_stride: values of one dW_e
   int* status;
 };
@@ -64,12 +67,14 @@ struct Unit {
   int e, ni, m0, n0;          // first row (a row of x, or of dW_e) and column of the tile
   int end;                    // where its rows end
   int k0, num_kb, tail;       // weight gradient: first row of the reduction, rows of the last k-block
+  int part;                   // ... and which part of it this is
 };
 
 // The units of a CTA (pair) one after the other: one of each `workers` in a row.  Those of a weight gradient, longest reductions first, are dealt out there and
 // back - worker w gets the w-th of a round, then the w-th from the end of the next - so that shares come out alike (16384 rows of 8 unequal experts, 4096 x
 // 1024: 16 % over the mean share when dealt in one direction, 7 % now).
-template <bool WGRAD, int BN, int TILE_M> struct Walk {
+// PARTS: a weight gradient in parts (p.split of them); the arithmetic for it would cost short units of the others half a microsecond each.
+template <bool WGRAD, int BN, int TILE_M, bool PARTS = false> struct Walk {
   const GroupParams& p;
   const int* start;
   const unsigned char* order;
@@ -91,15 +96,19 @@ template <bool WGRAD, int BN, int TILE_M> struct Walk {
       if (++e == p.experts) return false;
       first += tiles;
       if constexpr (!WGRAD) m_tiles = (start[e + 1] - start[e] + TILE_M - 1) / TILE_M;
-      tiles = m_tiles * cols;
+      tiles = m_tiles * cols * (PARTS ? p.split : 1);
     }
-    const int local = unit - first, ni = local / m_tiles, mi = local - ni * m_tiles;
+    const int local = unit - first, col = local / m_tiles, mi = local - col * m_tiles, part = PARTS ? col / cols : 0, ni = col - part * cols;
     u.ni = ni; u.n0 = ni * BN;
     if constexpr (WGRAD) {
       u.e = order[e];
       const int n = start[u.e + 1] - start[u.e];
       u.m0 = mi * TILE_M; u.end = p.n;
-      u.k0 = start[u.e]; u.num_kb = (n + BK - 1) / BK; u.tail = n - (u.num_kb - 1) * BK;
+      const int all = (n + BK - 1) / BK;
+      int from = 0, to = all;
+      if constexpr (PARTS) { from = part * all / p.split; to = (part + 1) * all / p.split; }        // (at most 2^21 k-blocks, 32 parts)
+      u.part = part;
+      u.k0 = start[u.e] + from * BK; u.num_kb = to - from; u.tail = to == all ? n - (all - 1) * BK : BK;
     } else {
       u.e = e;
       u.m0 = start[e] + mi * TILE_M; u.end = start[e + 1];
@@ -141,7 +150,7 @@ enum { ROWS = 0, ROWS_T = 1, WGRAD = 2 };     // B as stored, B turned, weight g
 // db_e along with dW_e: one warp adds up rows of dy that stand in shared memory anyway, behind the MMAs that read them (`read_bar`) and in front of the
 // copies that replace them (`summed_bar`).  (Beside the MMAs, told by the warp that issues them when a stage has landed: pairs took 85 us for 52 even
 // without a bias.)  It takes longer for a k-block than its MMAs (512 cycles), so the column tiles that share the rows take
-// their k-blocks in turn - tile i the k-blocks i, i + tiles, ... - and a second kernel adds the tiles' sums in their order (16384 rows of 8 experts,
+// their k-blocks in turn - tile i the k-blocks i, i + tiles, ... - and `grouped_join_kernel` adds the tiles' sums in their order (16384 rows of 8 experts,
 // 4096 x 1024, us: 116, of which 108 are the weight gradient's; by the tiles of the first columns alone 169, with a pass of its own 108 + 33).  A lane keeps eight columns of each
 // box and every fourth row.
 struct ColumnSums {
@@ -173,7 +182,7 @@ struct ColumnSums {
       }
     }
   }
-  __device__ __forceinline__ void write(const GroupParams& p, int e, int ni, int m0, int lane) {
+  __device__ __forceinline__ void write(const GroupParams& p, int e, int tile, int m0, int lane) {
 #pragma unroll
     for (int b = 0; b < BM / 64; ++b)
 #pragma unroll
@@ -187,7 +196,7 @@ struct ColumnSums {
         const int c = m0 + b * 64 + (lane & 7) * 8 + i * 2;
         if (lane < 8 && c < p.n) {             // (n is even)
           const long long at = (long long)e * p.n + c;
-          if (p.bias_parts) *reinterpret_cast<float2*>(p.bias_parts + (long long)ni * p.experts * p.n + at) = s;
+          if (p.bias_parts) *reinterpret_cast<float2*>(p.bias_parts + (long long)tile * p.experts * p.n + at) = s;
           else if (p.bias_accum) { p.bias_accum[at] += s.x; p.bias_accum[at + 1] += s.y; }
           else { p.bias_grad[at] = __float2bfloat16(s.x); p.bias_grad[at + 1] = __float2bfloat16(s.y); }
         }
@@ -196,9 +205,10 @@ struct ColumnSums {
 };
 
 // A panel of 32 rows and 64 columns, its rows' sums in the lanes' `v` (and `aux`, where there is one, in the slab): through the epilogue and out
-__device__ __forceinline__ void finish_panel(const GroupParams& p, uint8_t* slab, const __nv_bfloat16* bias, bool dual, bool has_aux, long long base, int r0, int nb,
-                                             int end, int cols, int lane, float* v) {
-  if (bias) {
+template <int MODE>
+__device__ __forceinline__ void finish_panel(const GroupParams& p, uint8_t* slab, const __nv_bfloat16* bias, bool has_bias, bool dual, bool has_aux, long long base, int r0,
+                                             int nb, int end, int cols, int lane, float (&v)[64]) {
+  if (MODE == ROWS && has_bias) {
     if (nb + 64 <= cols) {
 #pragma unroll
       for (int i = 0; i < 64; i += 8) {
@@ -211,7 +221,7 @@ __device__ __forceinline__ void finish_panel(const GroupParams& p, uint8_t* slab
       for (int i = 0; i < 64; ++i) if (nb + i < cols) v[i] += __bfloat162float(bias[nb + i]);
     }
   }
-  if (dual) {
+  if (MODE == ROWS && dual) {
     panel_store_row_bf16(slab, lane, v);     // pre-activation first
     __syncwarp();
     slab_flush_bf16(slab, reinterpret_cast<__nv_bfloat16*>(p.D2), p.ldd, r0, nb, end, cols, lane);
@@ -219,7 +229,7 @@ __device__ __forceinline__ void finish_panel(const GroupParams& p, uint8_t* slab
 #pragma unroll
     for (int i = 0; i < 64; i += 2) set2(v + i, bb::gelu_tanh2(get2(v + i)));
     __syncwarp();
-  } else if (has_aux) {
+  } else if (MODE == ROWS_T && has_aux) {
     __syncwarp();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -246,7 +256,7 @@ __device__ __forceinline__ void zero_the_rest(const GroupParams& p, const int* s
   }
 }
 
-template <int MODE, int BN, bool PAIR>
+template <int MODE, int BN, bool PAIR, bool PARTS = false>
 __global__ void __launch_bounds__(THREADS<MODE == WGRAD>, 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GroupParams p) {
   using C = Cfg<BN, PAIR>;
@@ -307,7 +317,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   } else {
     zero_the_rest(p, start, THREADS<false>);
   }
-  Walk<MODE == WGRAD, BN, C::TILE_M> walk(p, start, order, worker, workers);
+  Walk<MODE == WGRAD, BN, C::TILE_M, PARTS> walk(p, start, order, worker, workers);
   Unit u;
   const bool with_bias = MODE == WGRAD && (p.bias_grad || p.bias_accum);
 
@@ -482,12 +492,13 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         if (lane == 0) bb::mbar_arrive(&summed_bar[st]);
       }
       s = (s + u.num_kb) % C::STAGES;
-      if (alive) sums.write(p, u.e, u.ni, u.m0 + (int)rank * BM, lane);
+      if (alive) sums.write(p, u.e, PARTS ? u.part * walk.cols + u.ni : u.ni, u.m0 + (int)rank * BM, lane);
     }
   } else {
     // ------------------------------------------------ epilogue: eight warps, two per TMEM lane quarter, panels of 128 bytes in turn
     const int eg = (warp - EPI_WARP) >> 2, quarter = warp & 3;
-    const bool f32 = MODE == WGRAD && p.epi == BB_EPI_ACCUM_F32, dual = MODE == ROWS && p.epi == BB_EPI_BIAS_GELU;
+    const bool f32 = MODE == WGRAD && (PARTS || p.epi == BB_EPI_ACCUM_F32);
+    const bool dual = MODE == ROWS && p.epi == BB_EPI_BIAS_GELU;
     const bool has_aux = MODE == ROWS_T && p.epi == BB_EPI_MUL_DGELU, has_bias = MODE == ROWS && (p.epi == BB_EPI_BIAS || dual);
     const int cols = MODE == WGRAD ? p.k : p.n;
     uint8_t* slab = panels + (warp - EPI_WARP) * SLAB_BYTES;
@@ -496,7 +507,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     while (alive && walk.next(u)) {
       const int r0 = u.m0 + (int)rank * BM + quarter * 32, n0 = u.n0;
       const bool none = MODE == WGRAD && u.num_kb == 0;
-      if (none && f32) continue;               // nothing to add
+      if (none && f32 && !PARTS) continue;  // nothing to add
       uint32_t t_row = 0;
       if (!none) {
         if (!bb::mbar_wait_warp(&tmem_full[acc], acc_phase, abort_flag, p.status)) { alive = false; break; }
@@ -545,11 +556,12 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         if (f32) {
           panel_store_row_f32(slab, lane, v);
           __syncwarp();
-          slab_flush_f32<true>(slab, reinterpret_cast<float*>(p.D) + base, p.ldd, r0, nb, u.end, cols, lane);
+          if (PARTS) slab_flush_f32<false>(slab, p.parts + (long long)u.part * p.experts * p.expert_stride + base, p.ldd, r0, nb, u.end, cols, lane);
+          else slab_flush_f32<true>(slab, reinterpret_cast<float*>(p.D) + base, p.ldd, r0, nb, u.end, cols, lane);
           __syncwarp();
           continue;
         }
-        finish_panel(p, slab, bias, dual, has_aux, base, r0, nb, u.end, cols, lane, v);
+        finish_panel<MODE>(p, slab, bias, has_bias, dual, has_aux, base, r0, nb, u.end, cols, lane, v);
       }
       if (!none && ++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
@@ -728,24 +740,44 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       }
     }
     const __nv_bfloat16* bias = has_bias ? reinterpret_cast<const __nv_bfloat16*>(p.bias) + (long long)u.e * p.n : nullptr;
-    finish_panel(p, slab, bias, dual, has_aux, 0, r0, nb_own, u.end, cols, lane, v);
+    finish_panel<MODE>(p, slab, bias, has_bias, dual, has_aux, 0, r0, nb_own, u.end, cols, lane, v);
   }
   bb::tc_fence_before_sync();
   __syncthreads();
   if (warp == MMA_WARP) bb::tmem_dealloc(tmem_base, BN);
 }
 
-// The column tiles' sums (see ColumnSums), in their order
+// The sums of the parts, and of the column tiles for the bias (see ColumnSums), in their order; four weights a thread, one bias (with four, 16 tiles of 15000
+// took 6 us longer)
+struct Join { const float* parts; int count; long long values; __nv_bfloat16* out; float* accum; };
 __global__ void __launch_bounds__(256)
-grouped_bias_join_kernel(const float* parts, int tiles, long long values, __nv_bfloat16* out, float* accum) {
+grouped_join_kernel(const Join bias, const Join weight, int bias_blocks) {
   bb::pdl_sync();
-  const long long i = blockIdx.x * 256LL + threadIdx.x;
-  if (i >= values) return;
-  float s = 0.f;
+  if ((int)blockIdx.x < bias_blocks) {
+    const long long i = blockIdx.x * 256LL + threadIdx.x;
+    if (i >= bias.values) return;
+    float s = 0.f;
 #pragma unroll 4
-  for (int t = 0; t < tiles; ++t) s += parts[t * values + i];
-  if (accum) accum[i] += s;
-  else out[i] = __float2bfloat16(s);
+    for (int t = 0; t < bias.count; ++t) s += bias.parts[t * bias.values + i];
+    if (bias.accum) bias.accum[i] += s;
+    else bias.out[i] = __float2bfloat16(s);
+    return;
+  }
+  const long long i = (((int)blockIdx.x - bias_blocks) * 256LL + threadIdx.x) * 4;
+  if (i >= weight.values) return;            // (a multiple of 64)
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int t = 0; t < weight.count; ++t) {
+    const float4 q = *reinterpret_cast<const float4*>(weight.parts + t * weight.values + i);
+    s.x += q.x; s.y += q.y; s.z += q.z; s.w += q.w;
+  }
+  if (weight.accum) {
+    float4* to = reinterpret_cast<float4*>(weight.accum + i);
+    const float4 q = *to;
+    *to = make_float4(q.x + s.x, q.y + s.y, q.z + s.z, q.w + s.w);
+  } else {
+    *reinterpret_cast<uint2*>(weight.out + i) = make_uint2(bb::pack_bf16x2(s.x, s.y), bb::pack_bf16x2(s.z, s.w));
+  }
 }
 
 // ---------------------------------------------------------------- bias gradients
@@ -826,6 +858,7 @@ int refuse(const char* msg) { bb_set_last_error_msg(msg); return BB_ERR_INVALID_
 
 // Whether S CTAs can share a tile's reduction: each has a k-block at least, and what it receives fits its operand stages
 int quarters_of(const bb_grouped_desc* d) { return d->rows < BM ? (d->rows + 31) / 32 : BM / 32; }
+constexpr int MOST_PARTS = 32;
 template <int BN> bool can_split(const bb_grouped_desc* d, int S, int num_kb) {
   const int owned = (BN / 64 + S - 1) / S;
   return num_kb >= S && num_kb < INT_MAX / 8 && owned * (S - 1) * quarters_of(d) * 8192 <= Cfg<BN, false>::STAGES * Cfg<BN, false>::STAGE_BYTES;
@@ -859,7 +892,7 @@ template <int MODE, int BN> int clusters_at_once(int S) {
   return n > 0 ? n : 0;
 }
 
-template <int MODE, int BN, bool PAIR>
+template <int MODE, int BN, bool PAIR, bool PARTS = false>
 int launch(const bb_grouped_desc* d, cudaStream_t stream, int split = 1) {
   using C = Cfg<BN, PAIR>;
   CUtensorMap tmA, tmB;
@@ -867,8 +900,11 @@ int launch(const bb_grouped_desc* d, cudaStream_t stream, int split = 1) {
   p.rows = d->rows; p.experts = d->experts; p.epi = d->epilogue; p.offsets = d->offsets;
   p.D = d->out; p.D2 = d->out2; p.bias = d->bias; p.aux = d->aux;
   p.ldd = d->ld_out; p.ld_aux = d->ld_aux ? d->ld_aux : d->ld_out;
-  const int bias_tiles = d->bias_grad || d->bias_accum ? (d->k + BN - 1) / BN : 0;
+  const int bias_tiles = d->bias_grad || d->bias_accum ? (d->k + BN - 1) / BN * split : 0;
   p.bias_grad = (__nv_bfloat16*)d->bias_grad; p.bias_accum = d->bias_accum; p.bias_parts = bias_tiles > 1 ? d->bias_parts : nullptr;
+  p.split = split;
+  const long long bias_values = (long long)d->experts * d->n, weight_values = bias_values * d->k;
+  if (PARTS) p.parts = d->bias_parts + bias_tiles * bias_values;
   p.status = bb_device_status_word();
   int rc;
   long long tiles;
@@ -878,7 +914,7 @@ int launch(const bb_grouped_desc* d, cudaStream_t stream, int split = 1) {
     p.n = d->n; p.k = d->k; p.expert_stride = (long long)d->n * d->k; p.ldd = d->k;
     rc = bbhost::encode_2d(&tmA, d->x, d->rows, d->n, d->ld_x, 64, BK);
     if (!rc) rc = bbhost::encode_2d(&tmB, d->weight, d->rows, d->k, d->ld_weight, 64, BK);
-    tiles = (long long)d->experts * ((d->n + C::TILE_M - 1) / C::TILE_M) * ((d->k + BN - 1) / BN);
+    tiles = (long long)d->experts * ((d->n + C::TILE_M - 1) / C::TILE_M) * ((d->k + BN - 1) / BN) * split;
   } else {
     p.n = MODE == ROWS ? d->n : d->k; p.k = MODE == ROWS ? d->k : d->n;
     // no expert has more rows than there are: of few rows a tile loads those alone (what stands in shared memory below them makes rows that are
@@ -896,7 +932,6 @@ int launch(const bb_grouped_desc* d, cudaStream_t stream, int split = 1) {
   if (tiles > INT_MAX / 2 / split) return refuse("bb_grouped_gemm: more tiles than one launch covers");
   if constexpr (MODE != WGRAD && !PAIR) {
     if (split > 1) {
-      p.split = split;
       p.quarters = quarters_of(d);
       BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(grouped_split_kernel<MODE, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES)));
       cudaLaunchAttribute attr[2];
@@ -907,7 +942,7 @@ int launch(const bb_grouped_desc* d, cudaStream_t stream, int split = 1) {
       return BB_OK;
     }
   }
-  BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(grouped_gemm_kernel<MODE, BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES)));
+  BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(grouped_gemm_kernel<MODE, BN, PAIR, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES)));
   int workers = PAIR ? bb_num_sms() / 2 : bb_num_sms();
   if (d->max_ctas > 0 && d->max_ctas / (PAIR ? 2 : 1) < workers) workers = d->max_ctas / (PAIR ? 2 : 1);
   if (workers < 1) workers = 1;
@@ -924,14 +959,22 @@ int launch(const bb_grouped_desc* d, cudaStream_t stream, int split = 1) {
     if (!cfg.numAttrs) attr[0] = attr[1];
     ++cfg.numAttrs;
   }
-  BackToBack overlap(bias_tiles > 1 && d->max_ctas == 0);
-  BB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, grouped_gemm_kernel<MODE, BN, PAIR>, tmA, tmB, p));
-  if (bias_tiles > 1) {
-    const long long values = (long long)d->experts * d->n;
-    BB_CUDA_CHECK(bb_launch(grouped_bias_join_kernel, (unsigned)((values + 255) / 256), 256, 0, stream, (const float*)p.bias_parts, bias_tiles, values, p.bias_grad,
-                            p.bias_accum));
+  BackToBack overlap((bias_tiles > 1 || p.parts) && d->max_ctas == 0);
+  BB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, grouped_gemm_kernel<MODE, BN, PAIR, PARTS>, tmA, tmB, p));
+  if (bias_tiles > 1 || p.parts) {
+    const Join bias = {p.bias_parts, bias_tiles, bias_values, p.bias_grad, p.bias_accum};
+    const bool f32 = d->epilogue == BB_EPI_ACCUM_F32;
+    const Join weight = {p.parts, split, weight_values, f32 ? nullptr : (__nv_bfloat16*)d->out, f32 ? (float*)d->out : nullptr};
+    const long long bias_blocks = bias_tiles > 1 ? (bias_values + 255) / 256 : 0, weight_blocks = p.parts ? (weight_values + 1023) / 1024 : 0;
+    BB_CUDA_CHECK(bb_launch(grouped_join_kernel, (unsigned)(bias_blocks + weight_blocks), 256, 0, stream, bias, weight, (int)bias_blocks));
   }
   return BB_OK;
+}
+
+// Floats of scratch of a weight gradient in `split` parts, with tiles of `bn` columns
+long long part_values(int n, int k, int experts, int bn, int split, bool bias) {
+  const long long values = (long long)experts * n;
+  return (bias ? (long long)((k + bn - 1) / bn) * split * values : 0) + (split > 1 ? split * values * k : 0);
 }
 
 // The tile by the time that it is expected to take, as for stored products (gemm_tcgen05.cu), with the number of row tiles that evenly spread rows
@@ -943,43 +986,79 @@ int launch(const bb_grouped_desc* d, cudaStream_t stream, int split = 1) {
 // twentieth; the exchange grows with the CTAs and with the rows.  us, whole | shared by 2 | 4 | 8, the quickest kinds: 14 rows of 8 experts, 1024 x 4096, 23 | 17 |
 // 17 | 24; 2 rows of it 22 | 15 | 11 | 11; 1024 rows of 8, 512 x 2048, 14 | 12 | 13; 2000 of 8, 512 x 4096, 23 | 20 | 27; 1 row, 4096 x 4096, 22 | 15 | 12 | 20;
 // 14 of 8, 4096 x 1024, 14.5 | 21 | 32.
-template <int MODE> int choose(const bb_grouped_desc* d, cudaStream_t stream) {
-  static const struct { int bn; bool pair; double kblock, wave, once, shared; } kinds[3] = {
-      {256, true, 0.32, 1.9, 5.0, 0}, {256, false, 0.375, 1.8, 3.7, 6.0}, {128, false, 0.283, 1.0, 3.7, 5.0}};
+struct Plan { int kind, split; };
+struct Kind { int bn; bool pair; double kblock, wave, once, shared; };
+constexpr Kind KINDS[3] = {{256, true, 0.32, 1.9, 5.0, 0}, {256, false, 0.375, 1.8, 3.7, 6.0}, {128, false, 0.283, 1.0, 3.7, 5.0}};
+int workers_of(const bb_grouped_desc* d, const Kind& k) {
+  int workers = bb_num_sms();
+  if (d->max_ctas > 0 && d->max_ctas < workers) workers = d->max_ctas;
+  return !k.pair ? workers : workers > 1 ? workers / 2 : 1;
+}
+bool allowed(const bb_grouped_desc* d, const Kind& k) { return !(d->tile_n && d->tile_n != k.bn) && !(d->cta_pair && (d->cta_pair > 0) != k.pair); }
+
+template <int MODE> Plan plan(const bb_grouped_desc* d) {
   const double used = d->rows < d->experts ? d->rows : d->experts, each = d->rows / used;
   int best = 0, best_split = 1;
   double best_us = -1;
   for (int i = 0; i < 3; ++i) {
-    const auto& k = kinds[i];
-    if ((d->tile_n && d->tile_n != k.bn) || (d->cta_pair && (d->cta_pair > 0) != k.pair)) continue;
+    const Kind& k = KINDS[i];
+    if (!allowed(d, k)) continue;
     const int tm = k.pair ? 2 * BM : BM, n = MODE == ROWS ? d->n : d->k, num_kb = ((MODE == ROWS ? d->k : d->n) + BK - 1) / BK;
-    double row_tiles, kb;
-    if (MODE == WGRAD) {
-      row_tiles = (double)d->experts * ((d->n + tm - 1) / tm);
-      kb = each / BK + 0.5;
-    } else {
-      const double per = each / tm + 0.5;
-      row_tiles = used * (per > 1 ? per : 1);
-      kb = num_kb;
-    }
-    int workers = bb_num_sms();
-    if (d->max_ctas > 0 && d->max_ctas < workers) workers = d->max_ctas;
-    if (k.pair) workers = workers > 1 ? workers / 2 : 1;
-    const double whole = ceil(row_tiles * ((n + k.bn - 1) / k.bn) / workers) * (kb * k.kblock + k.wave) + k.once;
+    const double per = each / tm + 0.5, tiles = used * (per > 1 ? per : 1) * ((n + k.bn - 1) / k.bn);
+    const double whole = ceil(tiles / workers_of(d, k)) * (num_kb * k.kblock + k.wave) + k.once;
     if (d->split < 2 && (best_us < 0 || whole < best_us)) { best_us = whole; best = i; best_split = 1; }
-    if constexpr (MODE != WGRAD) {
-      const long long most = ((long long)d->rows / BM + (long long)used) * ((n + k.bn - 1) / k.bn);
-      for (int S = 2; S <= 8 && !k.pair && d->max_ctas == 0 && d->split != 1; S *= 2) {
-        if (d->split > 1 && S != d->split) continue;
-        if (!(k.bn == 128 ? can_split<128>(d, S, num_kb) : can_split<256>(d, S, num_kb))) continue;
-        if (d->split < 2 && (num_kb < 4 * S || most > (k.bn == 128 ? clusters_at_once<MODE, 128>(S) : clusters_at_once<MODE, 256>(S)))) continue;
-        const double us = 1.05 * ((num_kb + S - 1) / S * k.kblock + k.shared + 0.2 * quarters_of(d) * S);
-        if (best_us < 0 || us < best_us) { best_us = us; best = i; best_split = S; }
-      }
+    const long long most = ((long long)d->rows / BM + (long long)used) * ((n + k.bn - 1) / k.bn);
+    for (int S = 2; S <= 8 && !k.pair && d->max_ctas == 0 && d->split != 1; S *= 2) {
+      if (d->split > 1 && S != d->split) continue;
+      if (!(k.bn == 128 ? can_split<128>(d, S, num_kb) : can_split<256>(d, S, num_kb))) continue;
+      if (d->split < 2 && (num_kb < 4 * S || most > (k.bn == 128 ? clusters_at_once<MODE, 128>(S) : clusters_at_once<MODE, 256>(S)))) continue;
+      const double us = 1.05 * ((num_kb + S - 1) / S * k.kblock + k.shared + 0.2 * quarters_of(d) * S);
+      if (best_us < 0 || us < best_us) { best_us = us; best = i; best_split = S; }
     }
   }
-  if (best_us < 0) return refuse("bb_grouped_gemm: a reduction that cannot be split like this");
-  return best == 0 ? launch<MODE, 256, true>(d, stream) : best == 1 ? launch<MODE, 256, false>(d, stream, best_split) : launch<MODE, 128, false>(d, stream, best_split);
+  return {best_us < 0 ? -1 : best, best_split};
+}
+
+// A weight gradient of few tiles takes its reductions in parts, each a unit of its own, whose sums a second kernel adds up.  The time of one wave is that of the
+// longest expert, k-blocks take up to half as long again when all SMs ask for them, and the warp that sums the bias 0.7 us for one; the join costs a launch, and
+// the parts' way to memory and back.  Fitted to 90 sizes from 400 to 20000 rows, 1 to 64 experts, with and without a bias: whole reductions take 1.21 times
+// the quickest tile and number of parts in the mean, these 1.02.  us, whole | in parts, with the bias: 12874 rows of 1 expert, 352 x 208, 74 | 17; 8520 of 1,
+// 1056 x 672, 45 | 23; 17253 of 13, 88 x 536, 25 | 17; 9249 of 15, 120 x 72, 19 | 12.
+template <> Plan plan<WGRAD>(const bb_grouped_desc* d) {
+  static const int counts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24};
+  const double used = d->rows < d->experts ? d->rows : d->experts, each = d->rows / used / BK, values = (double)d->experts * d->n * d->k;
+  const bool bias = d->bias_grad || d->bias_accum;
+  Plan best = {-1, 1};
+  double best_us = -1;
+  for (int i = 0; i < 3; ++i) {
+    const Kind& k = KINDS[i];
+    if (!allowed(d, k)) continue;
+    const int tm = k.pair ? 2 * BM : BM, workers = workers_of(d, k), cols = (d->k + k.bn - 1) / k.bn;
+    const double tiles = (double)d->experts * ((d->n + tm - 1) / tm) * cols;
+    for (int at = 0; at < (int)(sizeof(counts) / sizeof(counts[0])); ++at) {
+      const int S = d->split ? d->split : counts[at];
+      if (!d->split && S > 1 && (tiles * S > 2 * workers || each < 2 * S)) break;
+      if (S > 1 && d->bias_parts_bytes < 4 * part_values(d->n, d->k, d->experts, k.bn, S, bias)) break;
+      double kblock = k.kblock * (1 + 0.5 * (tiles * S < workers ? tiles * S / workers : 1));
+      if (bias && kblock < 0.7 / cols) kblock = 0.7 / cols;
+      const double longest = tiles * S <= workers ? each * (1 + 0.8 * (1 - 1 / used)) : each;
+      double us = ceil(tiles * S / workers) * ((longest / S + 0.5) * kblock + k.wave) + k.once;
+      if (S > 1) us = 1.05 * (us + 1 + 0.1 * S + 0.8e-6 * S * values);
+      if (best_us < 0 || us < best_us) { best_us = us; best = {i, S}; }
+      if (d->split) break;
+    }
+  }
+  return best;
+}
+
+template <int MODE> int choose(const bb_grouped_desc* d, cudaStream_t stream) {
+  const Plan b = plan<MODE>(d);
+  if (b.kind < 0) return refuse("bb_grouped_gemm: a reduction that cannot be split like this, or not with this scratch");
+  if constexpr (MODE == WGRAD) {
+    if (b.split > 1)
+      return b.kind == 0 ? launch<MODE, 256, true, true>(d, stream, b.split) : b.kind == 1 ? launch<MODE, 256, false, true>(d, stream, b.split) : launch<MODE, 128, false, true>(d, stream, b.split);
+  }
+  return b.kind == 0 ? launch<MODE, 256, true>(d, stream, b.split) : b.kind == 1 ? launch<MODE, 256, false>(d, stream, b.split) : launch<MODE, 128, false>(d, stream, b.split);
 }
 
 bool bad_sizes(const bb_grouped_desc* d) {
@@ -994,6 +1073,19 @@ extern "C" long long bb_grouped_bias_bytes(int n, int k, int experts) {
   return n <= 0 || k <= 0 || experts <= 0 ? 0 : 4LL * ((k + 127) / 128) * experts * n;
 }
 
+extern "C" long long bb_grouped_weight_bytes(int rows, int n, int k, int experts, int with_bias) {
+  if (n <= 0 || k <= 0 || experts <= 0) return 0;
+  const long long least = with_bias ? bb_grouped_bias_bytes(n, k, experts) : 0;
+  bb_grouped_desc d = {};
+  d.mode = BB_GROUPED_WEIGHT; d.rows = rows; d.n = n; d.k = k; d.experts = experts; d.bias_parts_bytes = LLONG_MAX;
+  float none;
+  if (with_bias) d.bias_accum = &none;               // (not written to)
+  if (bad_sizes(&d)) return least;
+  const Plan b = plan<WGRAD>(&d);
+  const long long bytes = b.split > 1 ? 4 * part_values(n, k, experts, b.kind == 2 ? 128 : 256, b.split, with_bias) : 0;
+  return bytes > least ? bytes : least;
+}
+
 extern "C" int bb_grouped_gemm(const bb_grouped_desc* d, void* stream) {
   if (!d || !d->offsets || ((uintptr_t)d->offsets & 3) || bad_sizes(d))
     return refuse("bb_grouped_gemm: null pointer, a size that is not positive, n or k not a multiple of 8, or more than 256 experts");
@@ -1006,12 +1098,13 @@ extern "C" int bb_grouped_gemm(const bb_grouped_desc* d, void* stream) {
     return refuse("bb_grouped_gemm: operands are 16-byte aligned, with rows of a multiple of 8 values that do not overlap");
   if ((d->tile_n != 0 && d->tile_n != 128 && d->tile_n != 256) || (d->cta_pair > 0 && d->tile_n == 128))
     return refuse("bb_grouped_gemm: tile_n is 128 or 256, of a CTA pair 256");
-  if (d->split != 0 && d->split != 1 && d->split != 2 && d->split != 4 && d->split != 8) return refuse("bb_grouped_gemm: a reduction is split in 1, 2, 4 or 8");
-  if (d->split > 1 && (wgrad || d->cta_pair > 0 || d->max_ctas > 0))
-    return refuse("bb_grouped_gemm: a reduction is split among single CTAs, without max_ctas, and not that of a weight gradient");
+  if (d->split < 0 || (wgrad ? d->split > MOST_PARTS : d->split != 0 && d->split != 1 && d->split != 2 && d->split != 4 && d->split != 8) ||
+      (d->split > 1 && (wgrad ? !d->bias_parts : d->cta_pair > 0 || d->max_ctas > 0)))
+    return refuse("bb_grouped_gemm: split is 1, 2, 4 or 8, for single CTAs without max_ctas, or up to 32 parts of a weight gradient, which take scratch");
   if ((d->bias_grad || d->bias_accum) && (!wgrad || (d->bias_grad && d->bias_accum) || ((uintptr_t)d->bias_grad & 1) || ((uintptr_t)d->bias_accum & 3)))
     return refuse("bb_grouped_gemm: a bias gradient goes with a weight gradient, to one place");
-  if ((d->bias_grad || d->bias_accum) && (!d->bias_parts || ((uintptr_t)d->bias_parts & 15) || d->bias_parts_bytes < bb_grouped_bias_bytes(d->n, d->k, d->experts)))
+  if (wgrad && (((uintptr_t)d->bias_parts & 15) || (!d->bias_parts && d->bias_parts_bytes != 0))) return refuse("bb_grouped_gemm: scratch that is null or not 16-byte aligned");
+  if ((d->bias_grad || d->bias_accum) && (!d->bias_parts || d->bias_parts_bytes < bb_grouped_bias_bytes(d->n, d->k, d->experts)))
     return refuse("bb_grouped_gemm: a bias gradient takes bb_grouped_bias_bytes() of scratch");
   const int e = d->epilogue;
   if (wgrad ? (e != BB_EPI_STORE && e != BB_EPI_ACCUM_F32)

@@ -300,7 +300,8 @@ def _weight_gradients(dy, x, offsets, weight, bias, need_w, need_b):
         places[name] = main
     if need_w and not empty:
         main = places["weight"]
-        scratch = torch.empty(L.grouped_bias_scratch(*weight.shape), dtype=torch.uint8, device=dy.device) if need_b else None
+        size = L.grouped_weight_scratch(dy.shape[0], *weight.shape, need_b)
+        scratch = torch.empty(size, dtype=torch.uint8, device=dy.device) if size else None
         L.grouped_gemm(L.GROUPED_WEIGHT, dy, x, offsets, grads["weight"] if main is None else main, epilogue=L.EPI_STORE if main is None else L.EPI_ACCUM_F32,
                        bias_grad=grads["bias"], bias_accum=places["bias"], bias_parts=scratch)
     elif need_b and not empty:
@@ -398,8 +399,8 @@ class _ExpertMLPFn(torch.autograd.Function):
         if rows:
             inner = w1.shape[1]
             first = need[0] or need[1] or need[2]
-            behind = (2 * rows * inner + 255) & ~255 if first else 0         # the gradient of the pre-activation, then scratch of the bias gradients
-            size = L.expert_mlp_scratch(x.shape[1], inner, w2.shape[1], w1.shape[0])
+            behind = (2 * rows * inner + 255) & ~255 if first else 0         # the gradient of the pre-activation, then scratch of the weight gradients
+            size = L.expert_mlp_scratch(rows, x.shape[1], inner, w2.shape[1], w1.shape[0])
             work = torch.empty(behind + size, dtype=torch.uint8, device=dev)
             L.expert_mlp_bwd(_mlp_desc(x, w1, b1, w2, b2, offsets, *to, *added, work.data_ptr() + behind, size), x, kept, dy, work.data_ptr() if first else None, dx)
         return dx, *grads, None

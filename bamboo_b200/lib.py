@@ -188,6 +188,7 @@ def load():
         lib.bb_adam_step_clipped.argtypes = [vp] * 5 + [ll, d, d, d, d, i, i, i, d, d, i, vp, d, vp, vp, ll, vp]
         lib.bb_grouped_gemm.argtypes = [vp, vp]
         lib.bb_grouped_bias_bytes.argtypes, lib.bb_grouped_bias_bytes.restype = [i, i, i], ll
+        lib.bb_grouped_weight_bytes.argtypes, lib.bb_grouped_weight_bytes.restype = [i, i, i, i, i], ll
         lib.bb_grouped_colsum.argtypes = [vp, ll, vp, i, vp, vp, i, i, vp]
         lib.bb_expert_mlp_fwd.argtypes = [vp, vp, ll, vp, vp, vp, vp]
         lib.bb_expert_mlp_bwd.argtypes = [vp, vp, ll, vp, vp, vp, ll, vp, vp, vp]
@@ -840,6 +841,12 @@ def grouped_bias_scratch(experts, n, k):
     return load().bb_grouped_bias_bytes(n, k, experts)
 
 
+@functools.lru_cache(maxsize=1024)
+def grouped_weight_scratch(rows, experts, n, k, bias):
+    """Bytes of scratch for a weight gradient [experts, n, k] over ``rows``, with or without a bias gradient; 0: none."""
+    return load().bb_grouped_weight_bytes(rows, n, k, experts, int(bias))
+
+
 def grouped_gemm(mode, x, weight, offsets, out, *, epilogue=EPI_STORE, bias=None, out2=None, aux=None, max_ctas=0, tile_n=0, cta_pair=0, split=0, bias_grad=None,
                  bias_accum=None, bias_parts=None):
     """GROUPED_ROWS: x [rows, k], weight [experts, n, k], out [rows, n]; GROUPED_INPUT: x [rows, n], out [rows, k]; GROUPED_WEIGHT: x [rows, n],
@@ -877,10 +884,10 @@ def expert_mlp_fwd(desc, x, kept, y):
     return y
 
 
-@functools.lru_cache(maxsize=256)
-def expert_mlp_scratch(inputs, inner, outputs, experts):
-    """Bytes of scratch for the bias gradients that come with weight gradients."""
-    return max(grouped_bias_scratch(experts, inner, inputs), grouped_bias_scratch(experts, outputs, inner))
+@functools.lru_cache(maxsize=1024)
+def expert_mlp_scratch(rows, inputs, inner, outputs, experts):
+    """Bytes of scratch for weight gradients and the bias gradients that come with them."""
+    return max(grouped_weight_scratch(rows, experts, inner, inputs, True), grouped_weight_scratch(rows, experts, outputs, inner, True))
 
 
 def expert_mlp_bwd(desc, x, kept, dy, dpre, dx):

@@ -439,12 +439,15 @@ typedef struct bb_grouped_desc {
   int max_ctas;                                 /* see bb_gemm_desc.max_ctas */
   int tile_n;                                   /* 0 = choose, else 128 or 256 columns */
   int cta_pair;                                 /* 0 = choose, 1 = CTA pairs (256 x 256 tiles), -1 = single CTAs */
-  int split;                                    /* CTAs that share a tile's reduction: 0 = choose, else 1, 2, 4 or 8 (single CTAs; not a weight gradient, and not with max_ctas) */
+  int split;                                    /* 0 = choose, else 1, 2, 4 or 8 CTAs that share a tile's reduction (single CTAs, without max_ctas); BB_GROUPED_WEIGHT: 1 to 32 parts
+                                                   of a reduction, which take scratch */
   void* bias_grad; float* bias_accum;           /* BB_GROUPED_WEIGHT: also the sum of every expert's rows of x, to one of them: bf16 [experts, n], or
                                                    fp32 [experts, n] (+=); NULL: not wanted */
-  float* bias_parts; long long bias_parts_bytes;/* scratch for it, bb_grouped_bias_bytes() */
+  float* bias_parts; long long bias_parts_bytes;/* BB_GROUPED_WEIGHT: scratch, 16-byte aligned; bb_grouped_bias_bytes() for a bias gradient, bb_grouped_weight_bytes()
+                                                   for the quickest way: reductions over many rows for few tiles go in parts where it suffices for them */
 } bb_grouped_desc;
 long long bb_grouped_bias_bytes(int n, int k, int experts);
+long long bb_grouped_weight_bytes(int rows, int n, int k, int experts, int with_bias);        /* 0: needs none */
 int bb_grouped_max_experts(void);
 int bb_grouped_gemm(const bb_grouped_desc* d, void* stream);
 /* Bias gradients of such a layer without its weight gradients: out_bf16[e, n] = sum of its rows of dy, or accum[e, n] (fp32) += it; a fixed order of additions. */
@@ -460,7 +463,8 @@ typedef struct bb_expert_mlp_desc {
   const void *w1, *b1, *w2, *b2;
   void *dw1, *db1, *dw2, *db2;
   float *g_w1, *g_b1, *g_w2, *g_b2;
-  float* scratch; long long scratch_bytes;      /* where bias gradients come with weight gradients: the larger bb_grouped_bias_bytes() of the two layers */
+  float* scratch; long long scratch_bytes;      /* the larger bb_grouped_weight_bytes() of the two layers; where bias gradients come with weight gradients, the larger
+                                                   bb_grouped_bias_bytes() at least */
 } bb_expert_mlp_desc;
 int bb_expert_mlp_fwd(const bb_expert_mlp_desc* m, const void* x, long long ld_x, void* pre, void* act, void* y, void* stream);
 int bb_expert_mlp_bwd(const bb_expert_mlp_desc* m, const void* x, long long ld_x, const void* pre, const void* act, const void* dy, long long ld_dy, void* dpre,

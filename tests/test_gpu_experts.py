@@ -547,6 +547,49 @@ def test_many_tiles_a_cta_on_every_kind(ex, tile):
     test_grouped_linear(ex, [5] * 200, 0, 0, 264, 520, True)
 
 
+@pytest.mark.parametrize("parts", [2, 3, 7, 32])
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("lengths,before,after", [([1], 0, 0), ([0, 0], 0, 9), ([64, 65, 0, 127, 1], 3, 1), ([1300, 30], 0, 20)])
+@pytest.mark.parametrize("n,k", [(8, 8), (136, 264), (520, 1000)])
+def test_weight_gradients_in_parts(ex, lengths, before, after, n, k, tile, parts):
+    from bamboo_b200 import lib
+    x, _, _, dy = product_inputs(lengths, before, after, n, k, seed=91)
+    offsets, _ = offsets_of(lengths, before)
+    e, tiles = len(lengths), -(-k // tile[0])
+    scratch = torch.full((4 * parts * e * n * (k + tiles),), 255, dtype=torch.uint8, device="cuda")           # (all NaN)
+    dw, db = torch.full((e, n, k), math.nan, device="cuda", dtype=BF16), torch.full((e, n), math.nan, device="cuda", dtype=BF16)
+    kw = dict(tile_n=tile[0], cta_pair=tile[1], split=parts, bias_parts=scratch)
+    lib.grouped_gemm(lib.GROUPED_WEIGHT, dy, x, offsets, dw, bias_grad=db, **kw)
+    added, added_b = randn(e, n, k, seed=93), randn(e, n, seed=94)
+    before_w, before_b = added.clone(), added_b.clone()
+    lib.grouped_gemm(lib.GROUPED_WEIGHT, dy, x, offsets, added, epilogue=lib.EPI_ACCUM_F32, bias_accum=added_b, **kw)
+    alone = torch.empty_like(dw)
+    lib.grouped_gemm(lib.GROUPED_WEIGHT, dy, x, offsets, alone, **kw)
+    assert torch.equal(alone, dw)
+    with pytest.raises(lib.BambooNativeError, match="scratch"):
+        lib.grouped_gemm(lib.GROUPED_WEIGHT, dy, x, offsets, dw, bias_grad=db, **{**kw, "bias_parts": scratch[:-4 * parts * e * n]})
+    for i, at, count, _ in per_expert(lambda e: None, lengths, before):
+        rows = slice(at, at + count)
+        de = dy[rows].double()
+        w = matmul(Bound(de.t()), Bound(x[rows].double())) if count else Bound(torch.zeros(n, k, dtype=torch.float64, device="cuda"))
+        w = Bound(w.value, w.err + parts * 2 ** -24 * (de.abs().t() @ x[rows].double().abs()))
+        w.rounded().check(dw[i])
+        Bound(w.value + before_w[i].double(), w.err + 2 ** -23 * (w.value.abs() + before_w[i].double().abs())).check(added[i])
+        b = Bound(de.sum(0), (count + 8 + parts) * 2 ** -24 * de.abs().sum(0))
+        b.rounded().check(db[i])
+        Bound(b.value + before_b[i].double(), b.err + 2 ** -23 * (b.value.abs() + before_b[i].double().abs())).check(added_b[i])
+
+
+def test_long_reductions_for_few_tiles_go_in_parts(ex):
+    from bamboo_b200 import lib
+    lengths = [9000, 13, 4100]
+    assert lib.grouped_weight_scratch(sum(lengths), 3, 136, 264, True) > lib.grouped_bias_scratch(3, 136, 264)
+    assert lib.grouped_weight_scratch(100, 3, 136, 264, True) == lib.grouped_bias_scratch(3, 136, 264) and lib.grouped_weight_scratch(100, 3, 136, 264, False) == 0
+    test_grouped_linear(ex, lengths, 1, 5, 136, 264, True)
+    test_grouped_linear(ex, lengths, 0, 0, 136, 264, False)
+    test_expert_mlp(ex, [5000, 0, 700], 0, 3, 264, 136)
+
+
 SPLITS = [(2, 128), (4, 128), (8, 128), (2, 256), (4, 256), (8, 256)]
 
 
