@@ -122,6 +122,41 @@ template <int G> __device__ __forceinline__ uint32_t team_max(uint32_t v) {
   return v;
 }
 
+// Where every expert's places begin, from how many it has; by one warp
+__device__ __forceinline__ void places_of(const int* total, int* base, int n, int lane) {
+  int carry = 0;
+  for (int at = 0; at < n; at += 32) {
+    const int e = at + lane, c = e < n ? total[e] : 0;
+    int v = c;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += o;
+    }
+    if (e < n) base[e] = carry + v - c;
+    carry += __shfl_sync(0xffffffffu, v, 31);
+  }
+  if (lane == 0) base[n] = carry;
+}
+// Offsets, shares and the balance term, by a block; `sum` is the e-th thread's sum of softmax
+__device__ __forceinline__ void put_shares(const RouteParams& p, const int* total, const int* base, double* part, double sum) {
+  const int n = p.experts, e = threadIdx.x, lane = threadIdx.x & 31, tokens = max(total[n], 1), places = max(base[n], 1);
+  if (e < n) {
+    p.offsets[e] = base[e];
+    p.load[e] = (float)total[e] / (float)places;
+    part[e] = (double)total[e] * sum;
+  }
+  if (e == 0) { p.offsets[n] = base[n]; p.load[n] = (float)tokens; }
+  __syncthreads();
+  if (e < 32) {
+    double all = 0.0;
+    for (int i = lane; i < n; i += 32) all += part[i];
+#pragma unroll
+    for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+    if (lane == 0) p.balance[0] = (float)(n * all / ((double)places * (double)tokens));
+  }
+}
+
 // A team of G lanes per token (8, 16 or the warp, 32 / G tokens at a time), PER consecutive logits a lane, sorted; k rounds of a team-wide maximum, which goes
 // to the first lane that has it in front, the j-th choice to lane j.  Then the block's slots are ranked within their experts, in order: every warp counts a run of
 // them, and ranks it behind the runs before.  Instructions bound it: both kernels, us, 65536 tokens, 2 of 8 experts 17 (a warp per token 36), 6 of 64 34 (64);
@@ -134,7 +169,9 @@ route_choose_kernel(const T* logits, const RouteParams p) {
   extern __shared__ int shared[];
   int* hist = shared;                                                        // [ROUTE_WARPS][experts]
   float* sums = reinterpret_cast<float*>(shared + ROUTE_WARPS * p.experts);  // [ROUTE_WARPS][experts]
-  __shared__ int some_tokens;
+  __shared__ int some_tokens, total_of[MAX_EXPERTS + 1], base[MAX_EXPERTS + 1];
+  __shared__ double part[MAX_EXPERTS];
+  const bool alone = p.blocks == 1;          // a block that has all tokens places them too
   bb::pdl_sync();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = p.experts, seat = lane & (G - 1), first = seat * PER;
   const unsigned team = G == 32 ? 0xffffffffu : ((1u << (G & 31)) - 1) << (lane & ~(G - 1));
@@ -222,16 +259,28 @@ route_choose_kernel(const T* logits, const RouteParams p) {
     __syncwarp();
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < n; e += ROUTE_THREADS) {
+  float mass = 0.f;
+  if (threadIdx.x < n) {
+    const int e = threadIdx.x;
     int total = 0;
-    float s = 0.f;
 #pragma unroll 8
-    for (int w = 0; w < ROUTE_WARPS; ++w) { const int c = hist[w * n + e]; hist[w * n + e] = total; total += c; s += sums[w * n + e]; }
-    p.counts[(long long)blockIdx.x * (n + 1) + e] = total;
-    p.probs[(long long)blockIdx.x * n + e] = s;
+    for (int w = 0; w < ROUTE_WARPS; ++w) { const int c = hist[w * n + e]; hist[w * n + e] = total; total += c; mass += sums[w * n + e]; }
+    if (alone) {
+      total_of[e] = total;
+    } else {
+      p.counts[(long long)blockIdx.x * (n + 1) + e] = total;
+      p.probs[(long long)blockIdx.x * n + e] = mass;
+    }
   }
-  if (threadIdx.x == 0) p.counts[(long long)blockIdx.x * (n + 1) + n] = some_tokens;
+  if (threadIdx.x == 0) {
+    total_of[n] = some_tokens;
+    if (!alone) p.counts[(long long)blockIdx.x * (n + 1) + n] = some_tokens;
+  }
   __syncthreads();
+  if (alone) {
+    if (warp == 0) places_of(total_of, base, n, lane);
+    __syncthreads();
+  }
   for (int i = a + lane; i - lane < b; i += 32) {
     const int e = i < b ? p.chosen[slot0 + i] : -1;
     const unsigned same = __match_any_sync(0xffffffffu, e);
@@ -240,8 +289,16 @@ route_choose_kernel(const T* logits, const RouteParams p) {
     if (e >= 0) at = mine[e];
     __syncwarp();
     if (e >= 0 && before == 0) mine[e] = at + __popc(same);
-    if (i < b) p.rows[slot0 + i] = e >= 0 ? at + __popc(before) : -1;
+    if (i < b) {
+      const int place = e < 0 ? -1 : at + __popc(before) + (alone ? base[e] : 0);
+      p.rows[slot0 + i] = place;
+      if (alone && place >= 0) p.slots[place] = i;
+    }
     __syncwarp();
+  }
+  if (alone) {
+    for (int r = base[n] + threadIdx.x; r < count; r += ROUTE_THREADS) p.slots[r] = -1;
+    put_shares(p, total_of, base, part, (double)mass);
   }
 }
 
@@ -269,21 +326,7 @@ route_place_kernel(const RouteParams p) {
     atomicAdd(&before[e0], ahead);
   }
   __syncthreads();
-  if (warp == 0) {
-    int carry = 0;
-    for (int at = 0; at < n; at += 32) {
-      const int e = at + lane, c = e < n ? total[e] : 0;
-      int v = c;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, v, d);
-        if (lane >= d) v += o;
-      }
-      if (e < n) base[e] = carry + v - c;
-      carry += __shfl_sync(0xffffffffu, v, 31);
-    }
-    if (lane == 0) base[n] = carry;
-  }
+  if (warp == 0) places_of(total, base, n, lane);
   __syncthreads();
   const int routed = base[n];
   if (!extra) {
@@ -308,23 +351,9 @@ route_place_kernel(const RouteParams p) {
   }
   mass[threadIdx.x] = m;
   __syncthreads();
-  const int tokens = max(total[n], 1), places = max(routed, 1);
-  if (threadIdx.x < n) {
-    double sum = 0.0;
-    for (int i = 0; i < teams; ++i) sum += (double)mass[i * n + threadIdx.x];
-    p.offsets[threadIdx.x] = base[threadIdx.x];
-    p.load[threadIdx.x] = (float)total[threadIdx.x] / (float)places;
-    part[threadIdx.x] = (double)total[threadIdx.x] * sum;
-  }
-  if (threadIdx.x == 0) { p.offsets[n] = routed; p.load[n] = (float)tokens; }
-  __syncthreads();
-  if (warp == 0) {
-    double sum = 0.0;
-    for (int i = lane; i < n; i += 32) sum += part[i];
-#pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) p.balance[0] = (float)(n * sum / ((double)places * (double)tokens));
-  }
+  double sum = 0.0;
+  if (threadIdx.x < n) for (int i = 0; i < teams; ++i) sum += (double)mass[i * n + threadIdx.x];
+  put_shares(p, total, base, part, sum);
 }
 
 // A lane's run in shared memory (on its size, 16 bytes at most)
@@ -670,6 +699,9 @@ RouteParams route_params(const bb_route_desc* d) {
   const int most = bb_num_sms();
   p.chunk = (d->tokens + most - 1) / most;
   if (p.chunk < ROUTE_WARPS) p.chunk = ROUTE_WARPS;
+  // One block does it all, in one launch, where its teams have a token each: us, 128 tokens, 2 of 8 experts 7.9 -> 4.7; 64, 6 of 64, 7.9 -> 6.9; 32, 8 of 200, 12.4 ->
+  // 9.7 (with two tokens each 12.4 -> 14.2)
+  if (d->tokens <= ROUTE_THREADS / team_of(d->experts, d->k).lanes) p.chunk = d->tokens;
   p.blocks = (d->tokens + p.chunk - 1) / p.chunk;
   return p;
 }
@@ -681,7 +713,7 @@ template <typename T> struct RouteCall {
 template <typename T, int PER, int G> int route_fwd_as(const RouteCall<T>& c) {
   BB_ONCE_PER_DEVICE(BB_CUDA_CHECK(cudaFuncSetAttribute(route_choose_kernel<T, PER, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * ROUTE_WARPS * G * PER * 4)));
   BB_CUDA_CHECK(bb_launch(route_choose_kernel<T, PER, G>, c.p.blocks, ROUTE_THREADS, 2 * ROUTE_WARPS * c.p.experts * 4, c.s, c.logits, c.p));
-  BB_CUDA_CHECK(bb_launch(route_place_kernel, c.p.blocks + 1, ROUTE_THREADS, 0, c.s, c.p));
+  if (c.p.blocks > 1) BB_CUDA_CHECK(bb_launch(route_place_kernel, c.p.blocks + 1, ROUTE_THREADS, 0, c.s, c.p));
   return BB_OK;
 }
 template <typename T, int PER, int G> int route_bwd_as(const RouteCall<T>& c) {

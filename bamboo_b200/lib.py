@@ -908,7 +908,7 @@ def route_scratch(desc):
 def route_fwd(desc, logits, weights, experts, rows, slots, offsets, balance, kept):
     """``kept``: 2 tokens + experts + 1 fp32 values that route_bwd needs, the softmax statistics and behind them the experts' shares, then scratch."""
     global LAUNCHES
-    LAUNCHES += 2
+    LAUNCHES += 1 + (route_scratch(desc) > 4 * (2 * desc.experts + 1))          # (a single block places what it chose)
     lib = _lib or load()
     at = kept.data_ptr()
     scratch = at + 4 * (2 * desc.tokens + desc.experts + 1)

@@ -126,6 +126,14 @@ def test_route_and_gradient(ex, tokens, experts, cols, k, dtype, normalize):
         assert torch.all(got[:, experts:] == 0)
 
 
+@pytest.mark.parametrize("tokens,experts,cols,k", [(t + more, e, c, k) for t, e, c, k in ((128, 8, 8, 2), (128, 17, 24, 8), (64, 64, 64, 16), (32, 129, 129, 8))
+                                                   for more in (-1, 0, 1)])
+def test_route_by_one_block_and_by_several(ex, tokens, experts, cols, k):
+    test_route_and_gradient(ex, tokens, experts, cols, k, FP32, True)
+    none = ex.route(torch.full((tokens, experts), -math.inf, device="cuda"), k)
+    assert torch.all(none.rows == -1) and torch.all(none.slots == -1) and torch.all(none.offsets == 0) and torch.all(none.weights == 0)
+
+
 def test_route_ties_go_to_the_lower_index(ex):
     x = torch.zeros(70, 40, device="cuda")
     x[1::2, 7], x[1::2, 30], x[::3, 2] = 1.0, 1.0, -0.0
