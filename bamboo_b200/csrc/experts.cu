@@ -738,8 +738,9 @@ template <typename T> bool whole(const void* a, long long lda, const void* b, lo
   const long long item = sizeof(T);
   return !odd(a, 15) && !odd(b, 15) && !odd(c, 15) && !odd(d, 15) && lda * item % 16 == 0 && ldb * item % 16 == 0 && ldc * item % 16 == 0 && h * item % 16 == 0;
 }
-// Rows from 16 KB on, or few rows from 4 KB on, by a block each
-bool long_rows(long long rows, long long bytes) { return bytes >= 16384 || (bytes >= 4096 && rows < 1024); }
+// Rows from 16 KB on, few rows from 4 KB on, fewer from 2 KB on, by a block each (bf16, 8 rows a token, us, a warp | a block a row, combine and its gradient: 160 tokens
+// of 1024 6.7, 7.4 | 4.0, 6.9; 500 6.8, 7.4 | 5.2, 10.7; 160 of 1600 11.7, 12.3 | 4.2, 7.2; 900 11.6, 12.4 | 7.5, 16.9)
+bool long_rows(long long rows, long long bytes, int few = 256) { return bytes >= 16384 || (bytes >= 4096 && rows < 1024) || (bytes >= 2048 && rows < few); }
 
 #define MOVE(kernel, T, vec, big, rows, ...)                                                                                        \
   do {                                                                                                                              \
@@ -756,7 +757,7 @@ template <typename T> int dispatch(const T* x, long long ld, const int* slots, i
 }
 template <typename T>
 int combine(const T* x, long long ld, const int* rows_of, const float* w, const T* res, long long ld_res, int k, T* out, int tokens, int rows, int h, cudaStream_t s) {
-  const bool vec = whole<T>(x, ld, out, 0, res, res ? ld_res : 0, nullptr, h), big = long_rows(tokens, (long long)h * sizeof(T));
+  const bool vec = whole<T>(x, ld, out, 0, res, res ? ld_res : 0, nullptr, h), big = long_rows(tokens, (long long)h * sizeof(T), 768);
   MOVE(combine_kernel, T, vec, big, tokens, x, ld, rows_of, w, res, ld_res, k, out, tokens, rows, h, bb_device_status_word());
 }
 template <typename T>
