@@ -3,6 +3,10 @@
 // Memory bounds it: 18 bytes a parameter with moments in 8 bits, an fp32 master, a bf16 gradient and a bf16 working copy (28 in 32 bits).
 // A warp works on one block of 256 values, eight per lane, which is also the unit of the 8-bit scales: a block's largest magnitude is a
 // warp-wide maximum of bit patterns, under which NaN and infinity are the largest.  The list travels as a kernel argument.
+//
+// Codes are 6 to 12 % apart and one step changes a root by (1 - beta2) / 2 of itself, so codes rounded to nearest stand still from step to step (bamboo_b200.h).
+// Codes rounded up or down at random keep the average: the conversion takes 16 random bits, two neighbouring values share them from either end, and they are
+// hashed from seed, step, place and the parameter's new bits, so the same call gives the same codes.
 #include "common.cuh"
 #include "bamboo_b200.h"
 #include <cuda_fp8.h>
@@ -29,7 +33,8 @@ struct AdamTable {
   int count;
 };
 // (lr is folded into the rest: p -= rate m / (root sqrt(v) + eps) + shrink p, rate = lr / (1 - beta1^step), root = 1 / sqrt(1 - beta2^step))
-struct AdamArgs { float b1, omb1, b2, omb2, eps, rate, root, shrink, grad_scale; int zero_grad; const float* coef; };
+struct AdamArgs { float b1, omb1, b2, omb2, eps, rate, root, shrink, grad_scale; int zero_grad; const float* coef; uint32_t key; };
+enum { BITS_32 = 0, NEAREST = 1, STOCHASTIC = 2 };           // moments in 32 bits, in 8 bits with the nearest codes, with codes rounded up or down at random
 
 // One instruction each, within 2^-22 of the value; subnormal arguments count.  The update that they make is of the order of lr.
 __device__ __forceinline__ float root_of(float v) {
@@ -49,8 +54,27 @@ __device__ __forceinline__ float2 code_pair(uint32_t two) {
 }
 __device__ __forceinline__ uint32_t pair_code(float a, float b) { return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3); }
 
-// Codes of a lane's eight values under the block's scale, which every lane receives; ROOT: see CODE_MIN
-template <bool ROOT> __device__ __forceinline__ uint2 encode(const float* v, float& scale) {
+// Multiplicative hashing, twice (odd multipliers: the golden ratio's and the square root of two's first 32 bits)
+__host__ __device__ __forceinline__ uint32_t hashed(uint32_t x) {
+  x ^= x >> 16; x *= 0x9e3779b9u;
+  x ^= x >> 15; x *= 0xb504f333u;
+  return x ^ (x >> 16);
+}
+// One more product each, with other odd numbers, makes several words of a hash
+__device__ __forceinline__ uint32_t word(uint32_t hash, uint32_t odd) {
+  const uint32_t w = hash * odd;
+  return w ^ (w >> 16);
+}
+// Codes of a, b, c, d (in the bytes from the lowest), each the neighbour above or below with the probability that makes its mean the value, in steps of 2^-16
+__device__ __forceinline__ uint32_t stochastic_codes(float a, float b, float c, float d, uint32_t random) {
+  uint32_t q;
+  asm("cvt.rs.satfinite.e4m3x4.f32 %0, {%1, %2, %3, %4}, %5;" : "=r"(q) : "f"(d), "f"(c), "f"(b), "f"(a), "r"(random));
+  return q;
+}
+
+// Codes of a lane's eight values under the block's scale, which every lane receives; ROOT: see CODE_MIN.  Rounded at random, the largest value is put at 256 and
+// a little more, where it cannot become the code below.
+template <bool ROOT, int KIND> __device__ __forceinline__ uint2 encode(const float* v, float& scale, uint32_t random0, uint32_t random1) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
@@ -58,13 +82,14 @@ template <bool ROOT> __device__ __forceinline__ uint2 encode(const float* v, flo
   scale = __uint_as_float(top);
   if (top >= 0x7f800000u) { scale = __uint_as_float(0x7fc00000u); return make_uint2(0, 0); }
   if (scale <= TINY) return make_uint2(0, 0);
-  const float f = TOP * over(scale);
+  const float f = (KIND == STOCHASTIC ? TOP * (1.f + 0x1p-21f) : TOP) * over(scale);
   float c[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     c[i] = v[i] * f;
     if (ROOT && v[i] > 0.f) c[i] = fmaxf(c[i], CODE_MIN);
   }
+  if (KIND == STOCHASTIC) return make_uint2(stochastic_codes(c[0], c[1], c[2], c[3], random0), stochastic_codes(c[4], c[5], c[6], c[7], random1));
   return make_uint2(pair_code(c[0], c[1]) | pair_code(c[2], c[3]) << 16, pair_code(c[4], c[5]) | pair_code(c[6], c[7]) << 16);
 }
 __device__ __forceinline__ void decode(uint2 q, float scale, float* v) {
@@ -139,8 +164,9 @@ template <bool VEC> __device__ __forceinline__ void store_codes(uint8_t* p, int 
   }
 }
 
-template <bool EIGHT, bool VEC>
+template <int KIND, bool VEC>
 __device__ __forceinline__ void block_step(const bb_adamw_tensor& t, long long at, long long block, int n, int lane, const AdamArgs& a, float gs) {
+  constexpr bool EIGHT = KIND != BITS_32;
   float p[8], g[8], m[8], v[8], sm = 0.f, sv = 0.f;
   const long long blocks = (t.numel + BLOCK - 1) / BLOCK;
   float* master = t.master ? t.master : reinterpret_cast<float*>(t.param);
@@ -181,7 +207,9 @@ __device__ __forceinline__ void block_step(const bb_adamw_tensor& t, long long a
 #pragma unroll
       for (int i = 0; i < 8; ++i) if (place(lane, i) >= n) { m[i] = 0.f; v[i] = 0.f; }
     }
-    const uint2 cm = encode<false>(m, sm), cv = encode<true>(v, sv);
+    uint32_t h = 0;
+    if (KIND == STOCHASTIC) h = hashed(((uint32_t)block * 32 + lane) ^ (t.seed * 0x9e3779b9u + a.key) ^ __float_as_uint(p[0]));
+    const uint2 cm = encode<false, KIND>(m, sm, h, word(h, 0xbb67ae85u)), cv = encode<true, KIND>(v, sv, word(h, 0xc6ef3721u), word(h, 0xa54ff53bu));
     store_codes<VEC>(reinterpret_cast<uint8_t*>(t.exp_avg) + at, lane, n, cm);
     store_codes<VEC>(reinterpret_cast<uint8_t*>(t.exp_avg_sq) + at, lane, n, cv);
     if (lane == 0) { t.scales[block] = sm; t.scales[blocks + block] = sv; }
@@ -191,7 +219,7 @@ __device__ __forceinline__ void block_step(const bb_adamw_tensor& t, long long a
   }
 }
 
-template <bool EIGHT>
+template <int KIND>
 __global__ void __launch_bounds__(THREADS, CTAS)
 adamw_list_kernel(const __grid_constant__ AdamTable table, const AdamArgs a) {
   bb::pdl_sync();
@@ -204,8 +232,8 @@ adamw_list_kernel(const __grid_constant__ AdamTable table, const AdamArgs a) {
   const bb_adamw_tensor& t = table.t[lo];
   const long long block = unit - table.first[lo], at = block * BLOCK, left = t.numel - at;
   const float gs = a.coef ? a.coef[0] * a.grad_scale : a.grad_scale;
-  if (table.vec[lo] && left >= BLOCK) block_step<EIGHT, true>(t, at, block, BLOCK, lane, a, gs);
-  else block_step<EIGHT, false>(t, at, block, left < BLOCK ? (int)left : BLOCK, lane, a, gs);
+  if (table.vec[lo] && left >= BLOCK) block_step<KIND, true>(t, at, block, BLOCK, lane, a, gs);
+  else block_step<KIND, false>(t, at, block, left < BLOCK ? (int)left : BLOCK, lane, a, gs);
 }
 
 bool bad_tensor(const bb_adamw_tensor& t, bool eight) {
@@ -226,15 +254,16 @@ extern "C" int bb_adamw_list(const bb_adamw_tensor* tensors, int count, double l
   if (!tensors || count <= 0 || step < 1 || !(max_norm >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0) ||
       (max_norm > 0.0 && (!norm || !workspace || ((uintptr_t)workspace & 7) || workspace_bytes < bb_grad_norm_workspace_bytes())))
     return refuse("bb_adamw_list: an empty list, step < 1, a beta outside [0, 1), a negative norm, or clipping without a place for the norm or with a workspace that is too small");
-  const bool eight = tensors[0].scales != nullptr;
+  const bool eight = tensors[0].scales != nullptr, at_random = eight && tensors[0].seed != 0;
   for (int i = 0; i < count; ++i)
-    if (bad_tensor(tensors[i], eight))
-      return refuse("bb_adamw_list: a null or misaligned pointer, an empty tensor, a gradient that is neither bf16 nor fp32, or scales for a part of the list only");
+    if (bad_tensor(tensors[i], eight) || at_random != (eight && tensors[i].seed != 0))
+      return refuse("bb_adamw_list: a null or misaligned pointer, an empty tensor, a gradient that is neither bf16 nor fp32, or scales or seeds for a part of the list only");
   cudaStream_t s = (cudaStream_t)stream;
   AdamArgs a;
   a.b1 = (float)beta1; a.omb1 = (float)(1.0 - beta1); a.b2 = (float)beta2; a.omb2 = (float)(1.0 - beta2); a.eps = (float)eps;
   a.rate = (float)(lr / (1.0 - pow(beta1, (double)step))); a.root = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
   a.shrink = (float)(lr * weight_decay); a.grad_scale = (float)grad_scale; a.zero_grad = zero_grad; a.coef = nullptr;
+  a.key = hashed((uint32_t)step ^ hashed((uint32_t)(step >> 32) + 1));
   BackToBack overlap;
   if (max_norm > 0.0) {
     if (int rc = bb_list_clip_coef(tensors, count, sumsq, grad_scale, max_norm, norm, workspace, s)) return rc;
@@ -255,7 +284,7 @@ extern "C" int bb_adamw_list(const bb_adamw_tensor* tensors, int count, double l
     t.count = n;
     t.first[n] = (int)blocks;
     for (int i = n + 1; i <= LIST; ++i) t.first[i] = INT_MAX;
-    BB_CUDA_CHECK(bb_launch(eight ? adamw_list_kernel<true> : adamw_list_kernel<false>, dim3((unsigned)((blocks + WARPS - 1) / WARPS)), THREADS, 0, s, t, a));
+    BB_CUDA_CHECK(bb_launch(!eight ? adamw_list_kernel<BITS_32> : at_random ? adamw_list_kernel<STOCHASTIC> : adamw_list_kernel<NEAREST>, dim3((unsigned)((blocks + WARPS - 1) / WARPS)), THREADS, 0, s, t, a));
     from += n;
   }
   return BB_OK;

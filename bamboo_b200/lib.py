@@ -961,7 +961,7 @@ def _adamw_table(n):
 
 
 def adamw_tensors(fields, count):
-    """bb_adamw_tensor[count] from (param, master, gradient, exp_avg, exp_avg_sq, scales, elements, type of the gradient, 0) of every tensor."""
+    """bb_adamw_tensor[count] from (param, master, gradient, exp_avg, exp_avg_sq, scales, elements, type of the gradient, seed) of every tensor."""
     return _adamw_table(count).pack(*fields)
 
 

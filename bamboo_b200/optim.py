@@ -42,11 +42,14 @@ _BF16, _FP32, _EITHER, _CODES = {torch.bfloat16}, {torch.float32}, {torch.bfloat
 
 
 def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, scales=None, masters=None, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8,
-                weight_decay=0.0, grad_scale=1.0, max_norm=0.0, sumsq=None, zero_grad=False):
+                weight_decay=0.0, grad_scale=1.0, max_norm=0.0, sumsq=None, zero_grad=False, rounding="nearest"):
     """One AdamW step, number ``step`` (from 1), in place over lists of contiguous tensors; a parameter whose gradient is None is left out.
 
     ``params``: fp32, or bf16 with fp32 ``masters``.  ``grads``: bf16 or fp32.  Moments: fp32; or float8_e4m3fn with ``scales``, a fp32 tensor
     [2, blocks of 256 values] for each parameter, where ``exp_avg_sqs`` holds the SQUARE ROOT of the second moment.
+    ``rounding`` of those codes: "nearest", or "stochastic", up or down by a hash of the step number and the value's place (the same call gives the same
+    codes).  Training wants the latter: a step changes a root by (1 - beta2) / 2 of itself, and the nearest of codes that are 6 to 12 % apart stays the same,
+    so that from beta2 = 0.99 on roots stop following their gradients (bb_adamw_list has figures).
     ``grad_scale`` multiplies the gradients first.  ``max_norm`` > 0: on gradients clipped to that norm over the whole list, or over ``sumsq``
     (sum of squares of unscaled gradients, fp64 [1], device) where it covers more; returns the norm before clipping (fp32 scalar, device).
     A captured call repeats its step number at every replay."""
@@ -55,6 +58,8 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, scales=None, masters=No
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if step < 1:
         raise ValueError(f"step counts from 1, got {step}")
+    if rounding not in ("nearest", "stochastic"):
+        raise ValueError(f"rounding {rounding!r}: 'nearest' or 'stochastic'")
     if not (0 <= beta1 < 1 and 0 <= beta2 < 1):
         raise ValueError(f"beta1 {beta1}, beta2 {beta2}: from 0 to below 1")
     lists = [grads, *(None if column is None else list(column) for column in (exp_avgs, exp_avg_sqs, scales, masters))]
@@ -62,9 +67,10 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, scales=None, masters=No
         if column is not None and len(column) != len(params):
             raise ValueError(f"{name}: {len(column)} tensors for {len(params)} parameters")
     sizes = list(map(_sizes, params))
+    seeds = range(1, len(params) + 1)
     if not all(sizes) or type(None) in set(map(type, grads)):
         keep = [i for i, g in enumerate(grads) if g is not None and sizes[i]]
-        params, sizes = [params[i] for i in keep], [sizes[i] for i in keep]
+        params, sizes, seeds = [params[i] for i in keep], [sizes[i] for i in keep], [i + 1 for i in keep]
         lists = [None if column is None else [column[i] for i in keep] for column in lists]
     grads, exp_avgs, exp_avg_sqs, scales, masters = lists
     count = len(params)
@@ -89,7 +95,7 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, scales=None, masters=No
         raise ValueError("a tensor stands twice among params, moments, scales and masters")
     fields = itertools.chain.from_iterable(zip(
         addresses, full or nothing, _column(grads, "grads", count, _EITHER, sizes, device), first, second, scaled or nothing, sizes,
-        map(L.dtype_codes().get, map(_dtype_of, grads)), nothing))
+        map(L.dtype_codes().get, map(_dtype_of, grads)), seeds if rounding == "stochastic" else nothing))
     norm = scratch = None
     if max_norm > 0:            # (no buffer that calls share: a captured one keeps its own)
         norm = torch.empty((), dtype=torch.float32, device=params[0].device)
@@ -104,7 +110,7 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, scales=None, masters=No
 class AdamW:
     """``adamw_step_`` over ``params`` (leaf tensors, fp32 or all bf16), with the state that it needs.
 
-    ``state_bits``: 32, or 8 for moments of one byte each.  bf16 parameters get fp32 masters, which the steps are taken on.  ``max_norm`` > 0 clips
+    ``state_bits``: 32, or 8 for moments of one byte each, their codes rounded "stochastic".  bf16 parameters get fp32 masters, which the steps are taken on.  ``max_norm`` > 0 clips
     the gradients' global norm.  ``step()`` reads ``main_grad`` of a parameter where it has one, else ``grad``."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, *, state_bits=32, max_norm=0.0):
@@ -132,7 +138,7 @@ class AdamW:
         with torch.no_grad():
             data = [p.detach() for p in self.params]
             norm = adamw_step_(data, [_gradient_of(p) if p.requires_grad else None for p in self.params], self.exp_avgs, self.exp_avg_sqs,
-                               scales=self.scales, masters=self.masters, step=self.step_count + 1, lr=self.lr, beta1=self.betas[0],
+                               scales=self.scales, masters=self.masters, step=self.step_count + 1, rounding="stochastic", lr=self.lr, beta1=self.betas[0],
                                beta2=self.betas[1], eps=self.eps, weight_decay=self.weight_decay, grad_scale=grad_scale, max_norm=self.max_norm, sumsq=sumsq)
         self.step_count += 1
         return norm

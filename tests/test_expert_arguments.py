@@ -342,3 +342,33 @@ def test_native_list_step_refuses():
                 dict(master=at + 2), dict(grad=at + 2), dict(grad=at + 1, dtype=0), dict(m=at + 2), dict(scales=at + 2), dict(count=0), dict(count=-1), dict(step=0), dict(beta1=1.0),
                 dict(max_norm=-1.0), dict(max_norm=1.0), dict(max_norm=1.0, norm=at, ws=at, ws_bytes=16), dict(max_norm=1.0, norm=at, ws=at + 4, ws_bytes=1 << 20)):
         assert call(**bad) == -1 and b"bb_adamw_list" in handle.bb_last_error(), bad
+
+
+def test_rounding_of_codes(recorded):
+    _, optim, seen = recorded
+    import struct
+    for bad in ("up", None, 1):
+        with pytest.raises(ValueError, match="rounding"):
+            run(optim, lists(bits=8), rounding=bad)
+    assert not seen
+    for rounding, want in (("nearest", [0, 0]), ("stochastic", [1, 3])):
+        args = lists(bits=8)
+        args["grads"][1] = None
+        run(optim, args, rounding=rounding)
+        table, count = seen[-1][1]
+        assert list(struct.unpack("QQQQQQqiI" * count, table)[8::9]) == want
+    p = torch.zeros(300, requires_grad=True)
+    p.grad = torch.ones(300)
+    opt = optim.AdamW([p], state_bits=8)
+    with pytest.MonkeyPatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+        opt.step()
+    assert struct.unpack("QQQQQQqiI", seen[-1][1][0])[8] == 1
+
+
+def test_native_list_step_refuses_seeds_for_a_part_of_a_list():
+    import struct
+    from bamboo_b200 import lib
+    handle, at = lib.load(), 1 << 20
+    table = struct.pack("QQQQQQqiI" * 2, *(at, 0, at, at, at, at, 300, 1, 1), *(at, 0, at, at, at, at, 300, 1, 0))
+    assert handle.bb_adamw_list(table, 2, 1e-3, 0.9, 0.999, 1e-8, 1, 0.0, 1.0, 0, 0.0, None, None, None, 0, None) == -1 and b"seeds" in handle.bb_last_error()
