@@ -1064,6 +1064,7 @@ template <int MODE> int choose(const bb_grouped_desc* d, cudaStream_t stream) {
 bool bad_sizes(const bb_grouped_desc* d) {
   return d->rows <= 0 || d->rows > INT_MAX - 1024 || d->n <= 0 || d->k <= 0 || (d->n & 7) || (d->k & 7) || d->experts <= 0 || d->experts > MAX_EXPERTS;
 }
+bool too_wide(int n) { return n > 65535 * COLSUM_COLS; }
 bool bad_matrix(const void* p, long long ld, int cols) { return !p || ((uintptr_t)p & 15) || ld < cols || (ld & 7); }
 }  // namespace
 
@@ -1124,7 +1125,7 @@ extern "C" int bb_grouped_colsum(const void* dy, long long ld, const int* offset
   if (rows <= 0 || n <= 0 || (n & 7) || experts <= 0 || experts > MAX_EXPERTS || !offsets || ((uintptr_t)offsets & 3) || bad_matrix(dy, ld, n) || (!out_bf16 == !accum) ||
       ((uintptr_t)out_bf16 & 1) || ((uintptr_t)accum & 3))
     return refuse("bb_grouped_colsum: null or misaligned pointer, a size that is not positive, n no multiple of 8, more than 256 experts, or not one output");
-  if ((n + COLSUM_COLS - 1) / COLSUM_COLS > 65535) return refuse("bb_grouped_colsum: more columns than one launch covers");
+  if (too_wide(n)) return refuse("bb_grouped_colsum: more columns than one launch covers");
   int parts = 1;
   while (parts < COLSUM_MOST && rows / experts >= 64 * parts) parts *= 2;
   cudaLaunchConfig_t cfg = {};
@@ -1150,8 +1151,9 @@ bool bad_mlp(const bb_expert_mlp_desc* m) {
   return !m || m->rows <= 0 || m->rows > INT_MAX - 1024 || m->in <= 0 || m->inner <= 0 || m->out <= 0 || ((m->in | m->inner | m->out) & 7) || m->experts <= 0 ||
          m->experts > MAX_EXPERTS || !m->offsets || ((uintptr_t)m->offsets & 3) || !m->w1 || !m->w2 || (((uintptr_t)m->w1 | (uintptr_t)m->w2) & 15);
 }
-bool bad_scratch(const bb_expert_mlp_desc* m, bool wanted, int n, int k) {
-  return wanted && (!m->scratch || ((uintptr_t)m->scratch & 15) || m->scratch_bytes < bb_grouped_bias_bytes(n, k, m->experts));
+bool bad_scratch(const bb_expert_mlp_desc* m, bool weight, bool bias, int n, int k) {
+  return weight && (((uintptr_t)m->scratch & 15) || (!m->scratch && m->scratch_bytes != 0) ||
+                    (bias && (!m->scratch || m->scratch_bytes < bb_grouped_bias_bytes(n, k, m->experts))));
 }
 // the weight's and the bias's gradient of one layer, each where it is asked for
 int weight_and_bias(const bb_expert_mlp_desc* m, const void* dy, long long ld_dy, int n, const void* x, long long ld_x, int k, void* dw, float* g_w, void* db, float* g_b,
@@ -1186,8 +1188,10 @@ extern "C" int bb_expert_mlp_bwd(const bb_expert_mlp_desc* m, const void* x, lon
       (((uintptr_t)m->dw1 | (uintptr_t)m->dw2 | (uintptr_t)m->g_w1 | (uintptr_t)m->g_w2) & 15) ||
       (((uintptr_t)m->db1 | (uintptr_t)m->db2) & 1) || (((uintptr_t)m->g_b1 | (uintptr_t)m->g_b2) & 3))
     return refuse("bb_expert_mlp_bwd: null or misaligned pointer, a size that is not positive or no multiple of 8, rows that overlap, or more than 256 experts");
-  if (bad_scratch(m, (m->dw1 || m->g_w1) && (m->db1 || m->g_b1), m->inner, m->in) || bad_scratch(m, (m->dw2 || m->g_w2) && (m->db2 || m->g_b2), m->out, m->inner))
-    return refuse("bb_expert_mlp_bwd: a bias gradient that comes with a weight gradient takes bb_grouped_bias_bytes() of scratch");
+  const bool dw1 = m->dw1 || m->g_w1, db1 = m->db1 || m->g_b1, dw2 = m->dw2 || m->g_w2, db2 = m->db2 || m->g_b2;
+  if (bad_scratch(m, dw1, db1, m->inner, m->in) || bad_scratch(m, dw2, db2, m->out, m->inner))
+    return refuse("bb_expert_mlp_bwd: scratch that is null or not 16-byte aligned; a bias gradient that comes with a weight gradient takes bb_grouped_bias_bytes() of it");
+  if ((db1 && !dw1 && too_wide(m->inner)) || (db2 && !dw2 && too_wide(m->out))) return refuse("bb_expert_mlp_bwd: more columns than a bias gradient alone covers");
   if (m->rows > (1 << 27) && (m->dw1 || m->g_w1 || m->dw2 || m->g_w2)) {
     bb_set_last_error_msg("bb_expert_mlp_bwd: a weight gradient over more than 2^27 rows");
     return BB_ERR_TOO_LARGE;

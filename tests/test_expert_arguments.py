@@ -372,3 +372,20 @@ def test_native_list_step_refuses_seeds_for_a_part_of_a_list():
     handle, at = lib.load(), 1 << 20
     table = struct.pack("QQQQQQqiI" * 2, *(at, 0, at, at, at, at, 300, 1, 1), *(at, 0, at, at, at, at, 300, 1, 0))
     assert handle.bb_adamw_list(table, 2, 1e-3, 0.9, 0.999, 1e-8, 1, 0.0, 1.0, 0, 0.0, None, None, None, 0, None) == -1 and b"seeds" in handle.bb_last_error()
+
+
+def test_native_expert_mlp_refuses_scratch_before_anything_is_launched():
+    """Gradients added to an arena would be added twice by a caller that tries again after a refusal half way."""
+    from bamboo_b200 import lib
+    handle, at = lib.load(), 1 << 20
+    mlp = dict(rows=8, inputs=64, inner=64, outputs=64, experts=4, offsets=at, w1=at, b1=at, w2=at, b2=at)
+    for layer in (dict(g_w1=at), dict(dw1=at), dict(g_w2=at), dict(dw2=at), dict(g_w1=at, g_w2=at)):
+        for scratch in (dict(scratch=at + 8, scratch_bytes=1 << 20), dict(scratch_bytes=64), dict(scratch=at + 4)):
+            d = lib.ExpertMLPDesc(**mlp, **layer, **scratch)
+            assert handle.bb_expert_mlp_bwd(ctypes.byref(d), at, 64, at, at, at, 64, at, at, None) == -1, (layer, scratch)
+            assert b"bb_expert_mlp_bwd" in handle.bb_last_error() and b"scratch" in handle.bb_last_error(), handle.bb_last_error()
+    for layer in (dict(db1=at), dict(g_b2=at)):                              # bias gradients alone cover 65535 x 128 columns
+        sizes = dict(inner=1 << 23) if "db1" in layer else dict(outputs=1 << 23)
+        d = lib.ExpertMLPDesc(**{**mlp, **sizes}, **layer)
+        assert handle.bb_expert_mlp_bwd(ctypes.byref(d), at, 64, at, at, at, 1 << 23, at, at, None) == -1
+        assert b"bb_expert_mlp_bwd" in handle.bb_last_error() and b"columns" in handle.bb_last_error()
