@@ -696,7 +696,7 @@ template <typename T> bool in_runs(const T* p, long long ld, int experts, int co
 RouteParams route_params(const bb_route_desc* d) {
   RouteParams p = {};
   p.tokens = d->tokens; p.experts = d->experts; p.k = d->k; p.normalize = d->normalize; p.ld = d->ld;
-  const int most = bb_num_sms();
+  const int sms = bb_num_sms(), most = d->max_ctas > 0 && d->max_ctas < sms ? d->max_ctas : sms;
   p.chunk = (d->tokens + most - 1) / most;
   if (p.chunk < ROUTE_WARPS) p.chunk = ROUTE_WARPS;
   // One block does it all, in one launch, where its teams have a token each: us, 128 tokens, 2 of 8 experts 7.9 -> 4.7; 64, 6 of 64, 7.9 -> 6.9; 32, 8 of 200, 12.4 ->
@@ -788,7 +788,7 @@ extern "C" int bb_route_fwd(const bb_route_desc* d, const void* logits, float* w
   RouteParams p = route_params(d);
   p.weights = weights; p.chosen = experts_out; p.rows = rows_out; p.slots = slots_out; p.offsets = offsets; p.balance = balance; p.stats = (float2*)stats; p.load = load;
   p.counts = (int*)workspace; p.probs = (float*)((int*)workspace + (long long)p.blocks * (p.experts + 1));
-  BackToBack overlap;
+  BackToBack overlap(d->max_ctas == 0);
   return d->dtype == BB_DTYPE_BF16 ? route(RouteCall<__nv_bfloat16>{(const __nv_bfloat16*)logits, p, (cudaStream_t)stream}, d->cols, false)
                                    : route(RouteCall<float>{(const float*)logits, p, (cudaStream_t)stream}, d->cols, false);
 }

@@ -80,8 +80,8 @@ def _plan(routing, tokens=None):
 
 # ----------------------------------------------------------------------------------- routing
 @functools.lru_cache(maxsize=256)
-def _route_desc(tokens, experts, k, normalize, dtype, cols, ld):
-    return L.RouteDesc(tokens=tokens, experts=experts, k=k, normalize=normalize, dtype=dtype, cols=cols, ld=ld)
+def _route_desc(tokens, experts, k, normalize, dtype, cols, ld, max_ctas):
+    return L.RouteDesc(tokens=tokens, experts=experts, k=k, normalize=normalize, dtype=dtype, cols=cols, ld=ld, max_ctas=max_ctas)
 
 
 def _route(logits, k, experts, normalize):
@@ -102,7 +102,7 @@ def _route(logits, k, experts, normalize):
     offsets, balance = make(n + 1, dtype=torch.int32, device=dev), make((), dtype=torch.float32, device=dev)
     if tokens * k > _MOST:
         raise ValueError(f"{tokens} tokens with {k} experts each: at most {_MOST} rows")
-    desc = _route_desc(tokens, n, k, int(bool(normalize)), L.dtype_codes()[lg.dtype], lg.shape[-1], L._ld(lg) if tokens else lg.shape[-1])
+    desc = _route_desc(tokens, n, k, int(bool(normalize)), L.dtype_codes()[lg.dtype], lg.shape[-1], L._ld(lg) if tokens else lg.shape[-1], L.GEMM_MAX_CTAS)
     # what the backward pass needs of each softmax, then the shares, then scratch of this call (no buffer that calls share: a captured one keeps its own)
     kept = torch.empty(2 * tokens + n + 1 + L.route_scratch(desc) // 4, dtype=torch.float32, device=dev)
     if tokens:

@@ -120,7 +120,7 @@ class RouteDesc(ctypes.Structure):
     """bb_route_desc: tokens, experts and how many are chosen (see include/bamboo_b200.h)."""
     _fields_ = [
         ("tokens", ctypes.c_int), ("experts", ctypes.c_int), ("k", ctypes.c_int), ("normalize", ctypes.c_int), ("dtype", ctypes.c_int),
-        ("cols", ctypes.c_int), ("ld", ctypes.c_longlong),
+        ("cols", ctypes.c_int), ("ld", ctypes.c_longlong), ("max_ctas", ctypes.c_int),
     ]
 
 

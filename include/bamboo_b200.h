@@ -483,6 +483,7 @@ typedef struct bb_route_desc {
   int tokens, experts, k, normalize, dtype;
   int cols;                                     /* of a row of logits, >= experts: those behind may be read, and count for nothing */
   long long ld;
+  int max_ctas;                                 /* as for products: other than 0, launched plainly; > 0, the choice takes that many CTAs */
 } bb_route_desc;
 long long bb_route_workspace_bytes(const bb_route_desc* d);
 int bb_route_fwd(const bb_route_desc* d, const void* logits, float* weights, int* experts_out, int* rows_out, int* slots_out, int* offsets,

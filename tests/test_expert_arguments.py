@@ -389,3 +389,12 @@ def test_native_expert_mlp_refuses_scratch_before_anything_is_launched():
         d = lib.ExpertMLPDesc(**{**mlp, **sizes}, **layer)
         assert handle.bb_expert_mlp_bwd(ctypes.byref(d), at, 64, at, at, at, 1 << 23, at, at, None) == -1
         assert b"bb_expert_mlp_bwd" in handle.bb_last_error() and b"columns" in handle.bb_last_error()
+
+
+def test_routing_beside_the_main_stream_is_told_its_budget(recorded, monkeypatch):
+    ex, _, seen = recorded
+    from bamboo_b200 import lib
+    for budget in (0, 20, -1, 0):
+        monkeypatch.setattr(lib, "GEMM_MAX_CTAS", budget)
+        ex.route(torch.zeros(4, 8), 2)
+        assert seen[-1][1][0].max_ctas == budget
