@@ -53,7 +53,8 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, scales=None, masters=No
     ``grad_scale`` multiplies the gradients first.  ``max_norm`` > 0: on gradients clipped to that norm over the whole list, or over ``sumsq``
     (sum of squares of unscaled gradients, fp64 [1], device) where it covers more; returns the norm before clipping (fp32 scalar, device).
     A captured call repeats its step number at every replay."""
-    params, grads = list(params), list(grads)
+    given = params = list(params)
+    grads = list(grads)
     if not max_norm >= 0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if step < 1:
@@ -77,7 +78,9 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, scales=None, masters=No
     if not count:
         if not max_norm > 0:
             return None
-        return torch.zeros(()) if sumsq is None else (sumsq.detach().sqrt() * grad_scale).to(torch.float32).reshape(())
+        if sumsq is None:           # (on the device, as of any other list)
+            return torch.zeros((), device=given[0].device if given else "cuda" if torch.cuda.is_available() else "cpu")
+        return (sumsq.detach().sqrt() * grad_scale).to(torch.float32).reshape(())
     _on_current(params[0], "params")
     device = params[0].get_device()
     moments = _FP32 if scales is None else _CODES

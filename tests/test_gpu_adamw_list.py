@@ -323,3 +323,12 @@ def test_large_and_small_gradients(optim, bits):
         optim.adamw_step_([p], [value.expand(300).contiguous()], [m], [v], scales=scales, step=1, lr=1.0, beta2=0.999, eps=0.0)
         # (the first step is the sign of the gradient: m / bias and sqrt(v / bias) are both the gradient's size)
         near(p, -torch.sign(value).double().expand(300), 2 ** -12 if abs(value) < 1e-17 else 2 ** -19)
+
+
+def test_the_norm_of_a_list_without_gradients_is_on_the_device(optim):
+    p = torch.zeros(300, device="cuda", requires_grad=True)
+    for opt in (optim.AdamW([p], max_norm=1.0), optim.AdamW([p], max_norm=1.0, state_bits=8)):
+        norm = opt.step()
+        assert norm.is_cuda and norm.dtype == FP32 and norm.shape == () and norm.item() == 0.0
+    assert optim.adamw_step_([], [], [], [], step=1, max_norm=1.0).is_cuda
+    assert optim.adamw_step_([p[:0].detach()], [p[:0].detach()], [p[:0].detach()], [p[:0].detach()], step=1, max_norm=1.0).is_cuda
