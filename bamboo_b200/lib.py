@@ -198,6 +198,7 @@ def load():
         lib.bb_dispatch_rows.argtypes = [vp, ll, i, vp, i, vp, ll, ll, i, vp]
         lib.bb_combine_rows.argtypes = [vp, ll, i, vp, vp, vp, ll, i, vp, ll, ll, i, vp]
         lib.bb_combine_rows_bwd.argtypes = [vp, ll, i, vp, ll, vp, vp, vp, i, vp, vp, ll, ll, i, vp]
+        lib.bb_adamw_list_overlaps.argtypes = [vp, i, i]
         lib.bb_adamw_list.argtypes = [vp, i, d, d, d, d, ll, d, d, i, d, vp, vp, vp, ll, vp]
         _lib = lib
     return _lib
@@ -963,6 +964,11 @@ def _adamw_table(n):
 def adamw_tensors(fields, count):
     """bb_adamw_tensor[count] from (param, master, gradient, exp_avg, exp_avg_sq, scales, elements, type of the gradient, seed) of every tensor."""
     return _adamw_table(count).pack(*fields)
+
+
+def adamw_overlaps(table, count, zero_grad):
+    """Whether a tensor that the step writes shares memory with another of the list."""
+    return bool((_lib or load()).bb_adamw_list_overlaps(table, count, int(bool(zero_grad))))
 
 
 def adamw_list(table, count, *, lr, beta1, beta2, eps, step, weight_decay, grad_scale, zero_grad, max_norm, sumsq, norm, scratch):

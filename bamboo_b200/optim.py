@@ -84,26 +84,27 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, scales=None, masters=No
     _on_current(params[0], "params")
     device = params[0].get_device()
     moments = _FP32 if scales is None else _CODES
-    addresses = list(_column(params, "params", count, _FP32 if masters is None else _BF16, None, device))
+    addresses = _column(params, "params", count, _FP32 if masters is None else _BF16, None, device)
     if scales is not None and list(map(_sizes, scales)) != [2 * -(-n // BLOCK) for n in sizes]:
         raise ValueError("scales: [2, blocks of 256 values] for every parameter")
     if sumsq is not None and (sumsq.get_device() != device or sumsq.dtype != torch.float64):
         raise L.BambooNativeError("sumsq is fp64, on the parameters' device")
     nothing = itertools.repeat(0)
-    first = list(_column(exp_avgs, "exp_avgs", count, moments, sizes, device))
-    second = list(_column(exp_avg_sqs, "exp_avg_sqs", count, moments, sizes, device))
-    full = () if masters is None else list(_column(masters, "masters", count, _FP32, sizes, device))
-    scaled = () if scales is None else list(_column(scales, "scales", count, _FP32, None, device))
-    if len({*addresses, *first, *second, *full, *scaled}) != 3 * count + len(full) + len(scaled):
-        raise ValueError("a tensor stands twice among params, moments, scales and masters")
+    first = _column(exp_avgs, "exp_avgs", count, moments, sizes, device)
+    second = _column(exp_avg_sqs, "exp_avg_sqs", count, moments, sizes, device)
+    full = nothing if masters is None else _column(masters, "masters", count, _FP32, sizes, device)
+    scaled = nothing if scales is None else _column(scales, "scales", count, _FP32, None, device)
     fields = itertools.chain.from_iterable(zip(
-        addresses, full or nothing, _column(grads, "grads", count, _EITHER, sizes, device), first, second, scaled or nothing, sizes,
+        addresses, full, _column(grads, "grads", count, _EITHER, sizes, device), first, second, scaled, sizes,
         map(L.dtype_codes().get, map(_dtype_of, grads)), seeds if rounding == "stochastic" else nothing))
+    table = L.adamw_tensors(fields, count)
+    if L.adamw_overlaps(table, count, zero_grad):
+        raise ValueError("a tensor stands twice among params, moments, scales and masters (and gradients that are zeroed), or shares memory with another")
     norm = scratch = None
     if max_norm > 0:            # (no buffer that calls share: a captured one keeps its own)
         norm = torch.empty((), dtype=torch.float32, device=params[0].device)
         scratch = torch.empty(L.grad_norm_bytes(), dtype=torch.uint8, device=params[0].device)
-    L.adamw_list(L.adamw_tensors(fields, count), count, lr=float(lr), beta1=float(beta1), beta2=float(beta2), eps=float(eps), step=int(step),
+    L.adamw_list(table, count, lr=float(lr), beta1=float(beta1), beta2=float(beta2), eps=float(eps), step=int(step),
                  weight_decay=float(weight_decay), grad_scale=float(grad_scale), zero_grad=zero_grad, max_norm=float(max_norm), sumsq=sumsq, norm=norm,
                  scratch=scratch)
     torch.autograd.graph.increment_version(params + grads if zero_grad else params)

@@ -532,6 +532,9 @@ typedef struct bb_adamw_tensor {
   int grad_dtype;
   unsigned seed;                     /* 0: nearest codes */
 } bb_adamw_tensor;
+/* Whether a tensor that such a step writes (parameters, masters, moments, scales; gradients where it zeroes them) shares memory with another of the list: its
+ * result would depend on which CTA comes first.  1: one does, 0: none does.  On the host. */
+int bb_adamw_list_overlaps(const bb_adamw_tensor* tensors, int count, int zero_grad);
 int bb_adamw_list(const bb_adamw_tensor* tensors, int count, double lr, double beta1, double beta2, double eps, long long step,
                   double weight_decay, double grad_scale, int zero_grad, double max_norm, const double* sumsq, float* norm, void* workspace,
                   long long workspace_bytes, void* stream);

@@ -398,3 +398,58 @@ def test_routing_beside_the_main_stream_is_told_its_budget(recorded, monkeypatch
         monkeypatch.setattr(lib, "GEMM_MAX_CTAS", budget)
         ex.route(torch.zeros(4, 8), 2)
         assert seen[-1][1][0].max_ctas == budget
+
+
+@pytest.mark.parametrize("kind", [dict(), dict(bits=8), dict(dtype=BF16)])
+def test_adamw_refuses_tensors_that_share_memory(recorded, kind):
+    """Not only those that begin at one address: a value that two CTAs step on has the last one's result."""
+    _, optim, seen = recorded
+    for name in ("params", "exp_avgs", "exp_avg_sqs", "scales", "masters"):
+        args = lists(**kind)
+        if args.get(name) is None:
+            continue
+        buffer = torch.zeros(900, dtype=args[name][0].dtype)
+        shape, n = args[name][0].shape, args[name][0].numel()
+        args[name][:2] = [buffer[at:at + n].view(shape) for at in (0, n - 1)]
+        with pytest.raises(ValueError, match="shares memory"):
+            run(optim, args)
+        args[name][:2] = [buffer[at:at + n].view(shape) for at in (n, 0)]                # neighbours
+        run(optim, args)
+        assert seen.pop()
+    args = lists(**kind)
+    both = torch.zeros(599, dtype=args["grads"][0].dtype)
+    args["grads"][:2] = both[:300], both[299:]
+    run(optim, args)                                      # gradients that overlap are only read ...
+    assert seen.pop()
+    with pytest.raises(ValueError, match="zeroed"):       # ... unless they are zeroed while another reads them
+        run(optim, args, zero_grad=True)
+    args["grads"][1] = args["grads"][0]
+    with pytest.raises(ValueError, match="zeroed"):
+        run(optim, args, zero_grad=True)
+    args = lists(**kind)
+    if "bits" not in kind:
+        place = "masters" if kind else "params"
+        args["grads"][0] = args[place][2]                 # a gradient that the step overwrites
+        with pytest.raises(ValueError, match="shares memory"):
+            run(optim, args)
+    assert not seen
+
+
+def test_native_list_tells_of_shared_memory():
+    import random
+    import struct
+    from bamboo_b200 import lib
+    handle, rng = lib.load(), random.Random(3)
+    assert handle.bb_adamw_list_overlaps(None, 1, 0) == 0
+    for _ in range(300):
+        count, bits, zero = rng.randint(1, 9), rng.choice([8, 32]), rng.randint(0, 1)
+        rows, ranges = [], []
+        for _ in range(count):
+            n, master, dtype = rng.randint(1, 700), rng.randint(0, 1), rng.randint(0, 1)
+            place = lambda size: rng.randrange(16, 1 << rng.choice([15, 22]), 8) if size else 0  # noqa: E731
+            sizes = (2 * n if master else 4 * n, 4 * n * master, (2, 4)[dtype] * n, n * bits // 8, n * bits // 8, 8 * -(-n // 256) * (bits == 8))
+            at = [place(size) for size in sizes]
+            rows += [*at, n, dtype, 0]
+            ranges += [(a, a + size, i != 2 or zero) for i, (a, size) in enumerate(zip(at, sizes)) if size]
+        want = any(a[0] < b[1] and b[0] < a[1] and (a[2] or b[2]) for i, a in enumerate(ranges) for b in ranges[:i])
+        assert handle.bb_adamw_list_overlaps(struct.pack("QQQQQQqiI" * count, *rows), count, zero) == want
