@@ -26,6 +26,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 constexpr int MAX_EXPERTS = 256, MAX_CHOSEN = 32;
 constexpr int ROUTE_WARPS = 32, ROUTE_THREADS = 32 * ROUTE_WARPS;
 constexpr int BWD_WARPS = 8;
+constexpr int WIDEST = INT_MAX - 4096;                // values of a row are counted in 32 bits, up to some thousand beyond the last
 
 struct RouteParams {
   int tokens, experts, k, normalize;
@@ -675,7 +676,7 @@ combine_bwd_kernel(const T* dy, long long ld_dy, const T* x, long long ld, const
 
 // ------------------------------------------------------------------ host side
 bool bad_route(const bb_route_desc* d) {
-  return !d || d->tokens <= 0 || d->experts <= 0 || d->experts > MAX_EXPERTS || d->k <= 0 || d->k > d->experts || d->k > MAX_CHOSEN || d->cols < d->experts || d->ld < d->cols ||
+  return !d || d->tokens <= 0 || d->experts <= 0 || d->experts > MAX_EXPERTS || d->k <= 0 || d->k > d->experts || d->k > MAX_CHOSEN || d->cols < d->experts || d->cols > WIDEST || d->ld < d->cols ||
          (d->dtype != BB_DTYPE_BF16 && d->dtype != BB_DTYPE_F32) || (long long)d->tokens * d->k > INT_MAX - 1024;
 }
 
@@ -768,7 +769,7 @@ int combine_bwd(const T* dy, long long ld_dy, const T* x, long long ld, const in
 }
 
 bool bad_move(const void* x, long long ld, int dtype, const void* index, int k, long long rows, long long tokens, int h) {
-  return k > MAX_CHOSEN || !x || tokens <= 0 || k > INT_MAX / tokens || !index || odd(index, 3) || k <= 0 || rows <= 0 || rows > INT_MAX || h <= 0 || ld < h || (dtype != BB_DTYPE_BF16 && dtype != BB_DTYPE_F32) ||
+  return k > MAX_CHOSEN || !x || tokens <= 0 || k > INT_MAX / tokens || !index || odd(index, 3) || k <= 0 || rows <= 0 || rows > INT_MAX || h <= 0 || h > WIDEST || ld < h || (dtype != BB_DTYPE_BF16 && dtype != BB_DTYPE_F32) ||
          odd(x, dtype == BB_DTYPE_F32 ? 3 : 1);
 }
 }  // namespace
@@ -796,7 +797,7 @@ extern "C" int bb_route_fwd(const bb_route_desc* d, const void* logits, float* w
 extern "C" int bb_route_bwd(const bb_route_desc* d, const void* logits, const int* experts_out, const float* stats, const float* load,
                             const float* d_weights, const float* d_balance, void* dlogits, long long ldd, int cols, void* stream) {
   if (bad_route(d) || !logits || odd(logits, d->dtype == BB_DTYPE_F32 ? 3 : 1) || !experts_out || !stats || odd(stats, 7) || !load || !dlogits ||
-      odd(dlogits, d->dtype == BB_DTYPE_F32 ? 3 : 1) || cols < d->experts || ldd < cols)
+      odd(dlogits, d->dtype == BB_DTYPE_F32 ? 3 : 1) || cols < d->experts || cols > WIDEST || ldd < cols)
     return refuse("bb_route_bwd: null or misaligned pointer, a descriptor that bb_route_fwd refuses, cols < experts or ldd < cols");
   RouteParams p = route_params(d);
   p.chosen = const_cast<int*>(experts_out); p.stats = (float2*)stats; p.load = const_cast<float*>(load);

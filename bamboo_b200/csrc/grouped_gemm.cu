@@ -31,6 +31,7 @@ template <bool WEIGHT> constexpr int THREADS = 32 * (SUM_WARP + (WEIGHT ? 1 : 0)
 constexpr int A_STAGE_BYTES = BM * BK * 2;
 constexpr int SLAB_BYTES = 32 * 128;
 constexpr int MAX_EXPERTS = 256;
+constexpr int WIDEST = INT_MAX - 4096;                // columns are counted in 32 bits, up to a tile beyond the last
 
 template <int BN, bool PAIR> struct Cfg {
   static constexpr int B_ROWS = PAIR ? BN / 2 : BN;
@@ -1062,7 +1063,7 @@ template <int MODE> int choose(const bb_grouped_desc* d, cudaStream_t stream) {
 }
 
 bool bad_sizes(const bb_grouped_desc* d) {
-  return d->rows <= 0 || d->rows > INT_MAX - 1024 || d->n <= 0 || d->k <= 0 || (d->n & 7) || (d->k & 7) || d->experts <= 0 || d->experts > MAX_EXPERTS;
+  return d->rows <= 0 || d->rows > INT_MAX - 1024 || d->n <= 0 || d->n > WIDEST || d->k <= 0 || d->k > WIDEST || (d->n & 7) || (d->k & 7) || d->experts <= 0 || d->experts > MAX_EXPERTS;
 }
 bool too_wide(int n) { return n > 65535 * COLSUM_COLS; }
 bool bad_matrix(const void* p, long long ld, int cols) { return !p || ((uintptr_t)p & 15) || ld < cols || (ld & 7); }
@@ -1071,7 +1072,7 @@ bool bad_matrix(const void* p, long long ld, int cols) { return !p || ((uintptr_
 extern "C" int bb_grouped_max_experts(void) { return MAX_EXPERTS; }
 
 extern "C" long long bb_grouped_bias_bytes(int n, int k, int experts) {
-  return n <= 0 || k <= 0 || experts <= 0 ? 0 : 4LL * ((k + 127) / 128) * experts * n;
+  return n <= 0 || k <= 0 || experts <= 0 ? 0 : 4LL * ((k + 127LL) / 128) * experts * n;
 }
 
 extern "C" long long bb_grouped_weight_bytes(int rows, int n, int k, int experts, int with_bias) {
@@ -1089,7 +1090,7 @@ extern "C" long long bb_grouped_weight_bytes(int rows, int n, int k, int experts
 
 extern "C" int bb_grouped_gemm(const bb_grouped_desc* d, void* stream) {
   if (!d || !d->offsets || ((uintptr_t)d->offsets & 3) || bad_sizes(d))
-    return refuse("bb_grouped_gemm: null pointer, a size that is not positive, n or k not a multiple of 8, or more than 256 experts");
+    return refuse("bb_grouped_gemm: null pointer, a size that is not positive or close to 2^31, n or k not a multiple of 8, or more than 256 experts");
   const bool turned = d->mode == BB_GROUPED_INPUT, wgrad = d->mode == BB_GROUPED_WEIGHT;
   if (d->mode != BB_GROUPED_ROWS && !turned && !wgrad) return refuse("bb_grouped_gemm: an unknown mode");
   // (a tile of a weight gradient sums all of an expert's rows: about 0.3 us for 64 of them, and a wait inside the kernel has 2 s)
@@ -1148,7 +1149,7 @@ bb_grouped_desc part_of(const bb_expert_mlp_desc* m, int mode, int n, int k, int
 }
 // (all that the later products of a call could refuse, before the first is launched)
 bool bad_mlp(const bb_expert_mlp_desc* m) {
-  return !m || m->rows <= 0 || m->rows > INT_MAX - 1024 || m->in <= 0 || m->inner <= 0 || m->out <= 0 || ((m->in | m->inner | m->out) & 7) || m->experts <= 0 ||
+  return !m || m->rows <= 0 || m->rows > INT_MAX - 1024 || m->in <= 0 || m->in > WIDEST || m->inner <= 0 || m->inner > WIDEST || m->out <= 0 || m->out > WIDEST || ((m->in | m->inner | m->out) & 7) || m->experts <= 0 ||
          m->experts > MAX_EXPERTS || !m->offsets || ((uintptr_t)m->offsets & 3) || !m->w1 || !m->w2 || (((uintptr_t)m->w1 | (uintptr_t)m->w2) & 15);
 }
 bool bad_scratch(const bb_expert_mlp_desc* m, bool weight, bool bias, int n, int k) {

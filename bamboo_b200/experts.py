@@ -34,6 +34,7 @@ class Routing(NamedTuple):
 
 # ----------------------------------------------------------------------------------- arguments
 _MOST = 2 ** 31 - 1025          # rows and places are counted in 32 bits
+_WIDEST = 2 ** 31 - 4097        # ... and so are a row's values, of which loops look some thousand ahead
 _device = torch._C._cuda_getDevice
 
 
@@ -53,13 +54,15 @@ def _int32(t, name, numel=None):
 def _row_matrix(t, name):
     """(tensor, rows, row width, stride between rows) of [..., h]: as it is where rows have unit stride and one distance, else a copy."""
     h = t.shape[-1]
-    if h and t.is_contiguous() and t.is_cuda and t.get_device() == _device() and t.dtype in L.dtype_codes():
+    if 0 < h <= _WIDEST and t.is_contiguous() and t.is_cuda and t.get_device() == _device() and t.dtype in L.dtype_codes():
         return t, t.numel() // h, h, h
     _on_current(t, name)
     if t.dtype not in L.dtype_codes():
         raise L.BambooNativeError(f"{name}: bf16 or fp32 expected, got {t.dtype}")
     if h == 0:
         raise ValueError(f"{name}: rows without values")
+    if h > _WIDEST:
+        raise ValueError(f"{name}: rows of {h} values, at most {_WIDEST}")
     if t.is_contiguous():
         return t, t.numel() // h, h, h
     t = t.detach().reshape(-1, h)
@@ -72,6 +75,8 @@ def _plan(routing, tokens=None):
     """(rows, slots, k, tokens) of a routing, checked against each other."""
     rows = _int32(routing.rows, "rows")
     k, count = rows.shape[-1], rows.numel()
+    if count > _MOST:
+        raise ValueError(f"a routing of {count} rows, at most {_MOST}")
     slots = _int32(routing.slots, "slots", count)
     if tokens is not None and count != tokens * k:
         raise ValueError(f"a routing of {count // k} tokens for {tokens}")
@@ -89,6 +94,8 @@ def _route(logits, k, experts, normalize):
     if logits.dtype not in L.dtype_codes():
         _on_current(logits, "logits")
         raise L.BambooNativeError(f"logits: bf16 or fp32 expected, got {logits.dtype}")
+    if logits.shape[-1] > _WIDEST:
+        raise ValueError(f"logits of {logits.shape[-1]} columns, at most {_WIDEST}")
     lg, tokens, n = _rows(logits, experts)
     if n > 256:
         raise ValueError(f"{n} experts: at most 256")
@@ -247,6 +254,8 @@ def _weight(w, name, x, transposed=False):
         raise ValueError(f"{name}: {w.shape[0]} experts, 1 to 256 are possible")
     if w.shape[1] == 0 or w.shape[1] % 8 or w.shape[2] == 0 or w.shape[2] % 8:
         raise ValueError(f"{name} {tuple(w.shape)}: sizes that are multiples of 8 are needed (16-byte rows)")
+    if w.shape[1] > _WIDEST or w.shape[2] > _WIDEST:
+        raise ValueError(f"{name} {tuple(w.shape)}: sizes of at most {_WIDEST}")
     if w.shape[2] != x:
         raise ValueError(f"{name} {tuple(w.shape)} for rows of {x}")
     return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.detach().clone(memory_format=torch.contiguous_format)

@@ -453,3 +453,41 @@ def test_native_list_tells_of_shared_memory():
             ranges += [(a, a + size, i != 2 or zero) for i, (a, size) in enumerate(zip(at, sizes)) if size]
         want = any(a[0] < b[1] and b[0] < a[1] and (a[2] or b[2]) for i, a in enumerate(ranges) for b in ranges[:i])
         assert handle.bb_adamw_list_overlaps(struct.pack("QQQQQQqiI" * count, *rows), count, zero) == want
+
+
+def test_rows_that_32_bits_do_not_count(recorded):
+    """A size of 2^32 + 8 would reach the native call as 8."""
+    ex, _, seen = recorded
+    from bamboo_b200 import lib
+    wide = torch.zeros(1, 1).expand(4, 2 ** 32 + 8)
+    ints = torch.zeros(4, 1, dtype=torch.int32)
+    r = ex.Routing(torch.zeros(4, 1), ints, ints, ints.view(-1), None)
+    for call in (lambda: ex.dispatch(wide, r), lambda: ex.combine(wide, r), lambda: ex.dispatch(wide[:, :2 ** 31 - 8], r)):
+        with pytest.raises(ValueError, match="values, at most"):
+            call()
+    with pytest.raises(ValueError, match="columns, at most"):
+        ex.route(wide, 1, 8)
+    many = torch.zeros(1, 1, dtype=torch.int32).expand(2 ** 31, 1)
+    with pytest.raises(ValueError, match="rows, at most"):
+        ex.dispatch(torch.zeros(1, 1).expand(2 ** 31, 8), r._replace(rows=many, slots=many.view(-1)))
+    x, offsets = torch.zeros(6, 8, dtype=BF16), torch.zeros(2, dtype=torch.int32)
+    for shape in ((1, 2 ** 32 + 8, 8), (1, 8, 2 ** 32 + 8)):
+        with pytest.raises(ValueError, match="sizes of at most"):
+            ex.grouped_linear(x, torch.zeros(1, 1, 1, dtype=BF16).expand(shape), offsets)
+    assert not seen
+    handle, at, n = lib.load(), 1 << 20, 2 ** 31 - 8
+    good = dict(mode=0, rows=64, n=64, k=64, experts=4, epilogue=0, offsets=at, x=at, ld_x=64, weight=at, out=at, ld_out=64)
+    for change in (dict(n=n, ld_out=n), dict(k=n, ld_x=n), dict(mode=1, k=n, ld_out=n), dict(mode=2, k=n, ld_weight=n)):
+        assert handle.bb_grouped_gemm(ctypes.byref(lib.GroupedDesc(**{**good, **change})), None) == -1, change
+    mlp = dict(rows=8, inputs=64, inner=64, outputs=64, experts=4, offsets=at, w1=at, b1=at, w2=at, b2=at)
+    for name in ("inputs", "inner", "outputs"):
+        d = lib.ExpertMLPDesc(**{**mlp, name: n})
+        assert handle.bb_expert_mlp_fwd(ctypes.byref(d), at, n, at, at, at, None) == -1
+        assert handle.bb_expert_mlp_bwd(ctypes.byref(d), at, n, at, at, at, n, at, at, None) == -1
+    d = lib.RouteDesc(tokens=16, experts=8, k=2, normalize=1, dtype=0, cols=n, ld=n)
+    assert handle.bb_route_fwd(ctypes.byref(d), *[at] * 10, 1 << 40, None) == -1 and handle.bb_route_bwd(ctypes.byref(d), *[at] * 7, n, 8, None) == -1
+    d = lib.RouteDesc(tokens=16, experts=8, k=2, normalize=1, dtype=0, cols=8, ld=8)
+    assert handle.bb_route_bwd(ctypes.byref(d), *[at] * 7, n, n, None) == -1
+    assert handle.bb_dispatch_rows(at, n, 0, at, 2, at, 8, 4, n, None) == -1
+    assert handle.bb_combine_rows(at, n, 0, at, at, None, 0, 2, at, 4, 8, n, None) == -1
+    assert handle.bb_combine_rows_bwd(at, n, 0, at, n, at, at, at, 2, at, at, 4, 8, n, None) == -1
