@@ -97,8 +97,8 @@ def _route(logits, k, experts, normalize):
     if logits.shape[-1] > _WIDEST:
         raise ValueError(f"logits of {logits.shape[-1]} columns, at most {_WIDEST}")
     lg, tokens, n = _rows(logits, experts)
-    if n > 256:
-        raise ValueError(f"{n} experts: at most 256")
+    if n > L.max_experts():
+        raise ValueError(f"{n} experts: at most {L.max_experts()}")
     if not 0 < k <= min(n, 32):
         raise ValueError(f"k {k}: from 1 to the number of experts ({n}), at most 32")
     dev, shape = lg.device, (*logits.shape[:-1], k)
@@ -250,8 +250,8 @@ def _weight(w, name, x, transposed=False):
         raise L.BambooNativeError(f"{name}: bf16 expected, got {w.dtype}")
     if w.dim() != 3:
         raise ValueError(f"{name} {tuple(w.shape)}: [experts, out, in] is expected")
-    if w.shape[0] == 0 or w.shape[0] > 256:
-        raise ValueError(f"{name}: {w.shape[0]} experts, 1 to 256 are possible")
+    if not 0 < w.shape[0] <= L.max_experts():
+        raise ValueError(f"{name}: {w.shape[0]} experts, 1 to {L.max_experts()} are possible")
     if w.shape[1] == 0 or w.shape[1] % 8 or w.shape[2] == 0 or w.shape[2] % 8:
         raise ValueError(f"{name} {tuple(w.shape)}: sizes that are multiples of 8 are needed (16-byte rows)")
     if w.shape[1] > _WIDEST or w.shape[2] > _WIDEST:

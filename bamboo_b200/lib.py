@@ -836,6 +836,11 @@ def adam_step_clipped(master, grad, exp_avg, exp_avg_sq, param_lp, *, lr, beta1=
 
 
 # ---------------------------------------------------------------------------- mixture of experts
+@functools.lru_cache(maxsize=None)
+def max_experts():
+    return load().bb_grouped_max_experts()
+
+
 @functools.lru_cache(maxsize=256)
 def grouped_bias_scratch(experts, n, k):
     """Bytes of scratch for a bias gradient that comes with a weight gradient [experts, n, k]."""
