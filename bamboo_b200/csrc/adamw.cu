@@ -1,6 +1,6 @@
 // One AdamW step over a list of tensors, moments in 32 or 8 bits (formulas and formats: bamboo_b200.h, bb_adamw_list).
 //
-// Memory bounds it: 18 bytes a parameter with moments in 8 bits, an fp32 master, a bf16 gradient and a bf16 working copy (28 in 32 bits).
+// Memory bounds it: 16 bytes a parameter with moments in 8 bits, an fp32 master, a bf16 gradient and a bf16 working copy (28 in 32 bits).
 // A warp works on one block of 256 values, eight per lane, which is also the unit of the 8-bit scales: a block's largest magnitude is a
 // warp-wide maximum of bit patterns, under which NaN and infinity are the largest.  The list travels as a kernel argument.
 //
@@ -21,8 +21,9 @@ int refuse(const char* msg) { bb_set_last_error_msg(msg); return BB_ERR_INVALID_
 
 constexpr int LIST = 64;                       // tensors of one launch
 // Ten CTAs of four warps per SM: with moments in 8 bits a warp spends longer between its loads and its stores than in 32, and 48 registers let 40 of
-// them cover that.  150 M parameters, bf16 gradients and working copies, us: 8 bits 354 (6.8 TB/s); eight CTAs 385, twelve (which spill) 400; 32 bits 613
-// whatever the number.  Before, lanes with eight neighbouring values each, exact quotients and a tensor found by comparisons in all lanes (constant
+// them cover that.  150 M parameters, bf16 gradients and working copies, us: 8 bits 367 (6.5 TB/s) with the nearest codes, 355 (6.8) with codes rounded at
+// random, which four conversions make instead of eight; 32 bits 612 (6.9).  With eight CTAs 8 bits took 30 more, with twelve (which spill) 45.  Instructions are never
+// far from memory's time here: at the clocks that a power cap leaves (1.3 GHz) 8 bits come to 5.5 TB/s.  Before, lanes with eight neighbouring values each, exact quotients and a tensor found by comparisons in all lanes (constant
 // memory gives one address at a time): 498.
 constexpr int BLOCK = 256, THREADS = 128, WARPS = THREADS / 32, CTAS = 10;
 constexpr float TOP = 256.f, TINY = 0x1p-100f; // code of a block's largest value; scales up to TINY hold nothing

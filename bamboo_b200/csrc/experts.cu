@@ -524,8 +524,8 @@ dispatch_kernel(const T* x, long long ld, const int* slots, int k, T* out, int r
   for (int i = i0; i < n; i += TEAM) to[i] = from[i];
 }
 
-// A team goes through its token's row in runs of TEAM x U pieces: their loads are in flight together, of every row that the token has.  Row numbers and
-// weights wait in the lanes of each warp.
+// A team goes through its token's row in runs of TEAM x U pieces: their loads are in flight together, those of two rows where neither is dropped; the residual's
+// follow the rows' (8192 tokens of 1024, two rows and a residual each: 15.2 us, 4.4 TB/s).  Row numbers and weights wait in the lanes of each warp.
 template <typename T, int BYTES, int TEAM>
 __global__ void __launch_bounds__(MOVE_THREADS)
 combine_kernel(const T* x, long long ld, const int* rows_of, const float* weights, const T* residual, long long ld_res, int k, T* out, int tokens, int rows, int h,
@@ -740,7 +740,8 @@ template <typename T> bool whole(const void* a, long long lda, const void* b, lo
   return !odd(a, 15) && !odd(b, 15) && !odd(c, 15) && !odd(d, 15) && lda * item % 16 == 0 && ldb * item % 16 == 0 && ldc * item % 16 == 0 && h * item % 16 == 0;
 }
 // Rows from 16 KB on, few rows from 4 KB on, fewer from 2 KB on, by a block each (bf16, 8 rows a token, us, a warp | a block a row, combine and its gradient: 160 tokens
-// of 1024 6.7, 7.4 | 4.0, 6.9; 500 6.8, 7.4 | 5.2, 10.7; 160 of 1600 11.7, 12.3 | 4.2, 7.2; 900 11.6, 12.4 | 7.5, 16.9)
+// of 1024 6.7, 7.4 | 4.0, 6.9; 500 6.8, 7.4 | 5.2, 10.7; 160 of 1600 11.7, 12.3 | 4.2, 7.2; 900 11.6, 12.4 | 7.5, 16.9; dispatch, 200 rows of 1024 2.3 | 1.7, of
+// 1600 2.9 | 1.7, 512 of 2048 6.3 | 2.6, 4096 of 8192 25.6 | 16.8)
 bool long_rows(long long rows, long long bytes, int few = 256) { return bytes >= 16384 || (bytes >= 4096 && rows < 1024) || (bytes >= 2048 && rows < few); }
 
 #define MOVE(kernel, T, vec, big, rows, ...)                                                                                        \

@@ -580,8 +580,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
 }
 
-// Few tiles and a long reduction: a cluster of 2, 4 or 8 CTAs shares a tile's reduction, each over a run of its k-blocks (a k-block takes about 0.28 us
-// however idle the GPU is: its latency, not its bytes).  Panels of 64 columns are dealt out to the CTAs; each sends its sums of the others' panels into their
+// Few tiles and a long reduction: a cluster of 2, 4 or 8 CTAs shares a tile's reduction, each over a run of its k-blocks (a k-block takes 0.28 us with
+// 128 columns, 0.37 with 256, however idle the GPU is; its MMAs alone, of 128 rows whether they exist or not, 0.14 and 0.27).  Panels of 64 columns are dealt out to the CTAs; each sends its sums of the others' panels into their
 // operand stages, by then unused, and adds what it received to its own in the order of the CTAs: the same bits every time.  A cluster has one tile.
 // Received panels: [other CTA][run of 32 rows][16 bytes of a row][row], so that a warp's access is one run of memory.
 template <int MODE, int BN>
@@ -920,7 +920,7 @@ int launch(const bb_grouped_desc* d, cudaStream_t stream, int split = 1) {
     p.n = MODE == ROWS ? d->n : d->k; p.k = MODE == ROWS ? d->k : d->n;
     // no expert has more rows than there are: of few rows a tile loads those alone (what stands in shared memory below them makes rows that are
     // not stored).  14 rows of 8 experts, 4096 x 1024, from memory: 17.5 -> 15.4 us, with `rotate` 14.8.
-    // (Tiles of 64 columns and 16 stages of 16 rows took 22: a k-block takes 0.28 us whatever it holds.)
+    // (Tiles of 64 columns and 16 stages of 16 rows took 22.)
     const int box = d->rows < BM ? (d->rows + 7) & ~7 : BM;
     p.stage_bytes = box * BK * 2 + C::B_STAGE_BYTES;
     p.rotate = d->rows < BM;

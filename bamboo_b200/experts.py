@@ -417,7 +417,8 @@ class _ExpertMLPFn(torch.autograd.Function):
 
 def expert_mlp(x, offsets, w1, b1, w2, b2):
     """Two layers per expert with a tanh GeLU between: grouped_linear(gelu(grouped_linear(x, w1, offsets, b1)), w2, offsets, b2), where the GeLU
-    is taken of the unrounded sums and rounded to bf16 (its slope in the backward pass of the rounded ones).
+    is taken of the unrounded sums and rounded to bf16 (its slope in the backward pass of the rounded ones): operands of the second product, as the gradient of the
+    sums is of the first one's, are bf16.  Together with the result's own rounding 0.24 % in the 2-norm (0.17 % with a GeLU kept in 32 bits).
 
     w1 [experts, inner, k], b1 [experts, inner], w2 [experts, n, inner], b2 [experts, n]; otherwise as ``grouped_linear``."""
     _on_current(x, "x")

@@ -576,7 +576,8 @@ class _RouterFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         (x2,) = ctx.saved_tensors
-        d2 = dy.reshape(-1, dy.shape[-1]).to(torch.bfloat16).contiguous()       # (operands of the two products are bf16)
+        # (operands of both products are bf16: half a step, 2^-8, of each logit's gradient, as the other products' incoming gradients have)
+        d2 = dy.reshape(-1, dy.shape[-1]).to(torch.bfloat16).contiguous()
         return _linear_backward(d2, x2, ctx.mod.gate, None).view(ctx.shape), None, None
 
 

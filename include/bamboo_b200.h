@@ -515,8 +515,8 @@ int bb_combine_rows_bwd(const void* dy, long long ld_dy, int dtype, const void* 
  * `seed` other than 0 (in all tensors or none) takes the code above or below instead, each with the probability that makes the mean the value, by a hash of
  * seed, step, place and parameter: the same call gives the same codes.  A sequence of steps wants that.  The nearest code stands still: a step changes a root
  * by (1 - beta2) / 2 of itself, codes are 6 to 12 % apart.  Measured, roots in 8 bits over those in 32 after 5000 steps, half of each block's gradients ten
- * times smaller from the 1000th on, mean and root mean square distance from 1 of that half: nearest, beta2 = 0.999 4.9, 4.6; 0.99 4.6, 4.3; 0.95 1.01, 0.08;
- * with a seed 1.03, 0.29; 1.02, 0.16; 1.00, 0.11.
+ * times smaller from the 1000th on, mean and root mean square distance from 1 of that half: nearest, beta2 = 0.999 5.4, 4.9; 0.99 4.4, 4.0; 0.95 1.00, 0.08;
+ * with a seed 1.04, 0.32; 1.01, 0.16; 1.01, 0.11.
  *   g = grad * grad_scale (* min(1, max_norm / (norm + 1e-6)));  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   p -= lr * (m / (1 - beta1^step) / (sqrt(v / (1 - beta2^step)) + eps) + weight_decay * p)
  * max_norm > 0 clips to the norm over the list (times grad_scale), or over `sumsq` (sum of squares of unscaled gradients, device) where that covers
