@@ -12,7 +12,7 @@ which is taken as 2 (1 - b): the largest among several that are nearly so, with 
 while sqrt(b r^2 + c) is convex in r, so that the mean of the root in 8 bits is at least the exact one, r.  The mean of (root / r - 1)^2 is then at most E u / r^2 - 1, that of
 root / r at most sqrt(E u / r^2) (Jensen).  Means are over 4096 values and more, whose sample means are off by 3 % at the most here (six times 0.3 / 64).
 
-With b = 0.999 nearest codes end 3 to 7 times too high where gradients have shrunk, or have grown four-fold beside others, and 1.1 times too high with 0.99 throughout."""
+With b = 0.999 nearest codes end 3 to 7 times too high where gradients have shrunk, or have grown four-fold beside others; with 0.99 throughout, 1.06 times."""
 import math
 
 import pytest
